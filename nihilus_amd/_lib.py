@@ -1,4 +1,4 @@
-"""ctypes binding of libnihilus_q8_hip.so, the C ABI declared in include/nihilus_amd/q8_0_abi.h.
+"""ctypes binding of libnihilus_q8_hip.so, the C ABI declared in include/nihilus_amd/q8_0_abi.h and attention_abi.h.
 
 There is no fallback: if the library is missing, loading raises, and every wrapper turns a non-zero
 status into ``Q8Error``.
@@ -77,6 +77,29 @@ SIGNATURES = {
     "nh_q8_0_fill_activations": (_int, [_vp, _u64, _i64, _vp]),
 }
 
+# the same of attention_abi.h
+ATTENTION_SIGNATURES = {
+    "nh_attn_append_rope": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp]),
+    "nh_attn_prompt": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, C.c_float, _vp]),
+    "nh_attn_decode_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "nh_attn_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, C.c_float, _vp, _i64, _vp]),
+    "nh_attn_pages_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "nh_attn_cache_step": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "nh_attn_cache_compact": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+}
+
+
+class AttnCache(C.Structure):
+    """nh_attn_cache"""
+
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("layers", _i64), ("pages", _i64), ("kv_heads", _i64), ("page_size", _i64), ("head_dim", _i64), ("type", C.c_int32)]
+
+
+class AttnBatch(C.Structure):
+    """nh_attn_batch"""
+
+    _fields_ = [("page_table", _vp), ("lengths", _vp), ("starts", _vp), ("sequences", _i64), ("table_width", _i64)]
+
 
 class MulMatOp(C.Structure):
     """nh_q8_0_mul_mat_op"""
@@ -105,7 +128,7 @@ def lib() -> C.CDLL:
                 "there is no CPU fallback for this path"
             )
         handle = C.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **ATTENTION_SIGNATURES}.items():
             fn = getattr(handle, name)  # AttributeError if the library does not export a declared symbol
             fn.restype, fn.argtypes = res, args
         _lib = handle

@@ -1,0 +1,220 @@
+// extern "C" surface of the attention and cache calls: argument checks, then the launch functions.  What lies in device memory (tables,
+// lengths, starts) cannot be looked at here; the kernels check it where they use it.
+#include "../../include/nihilus_amd/attention_abi.h"
+#include "abi_checks.h"
+#include "attention_device.h"
+
+#include <cmath>
+
+namespace {
+
+using nh::aligned16;
+using nh::as_stream;
+using nh::from_hip;
+using nh::require_device;
+
+// row, token and tile numbers are 32-bit inside the kernels, with room for sums of two
+constexpr int64_t MAX_KEYS		= int64_t{ 1 } << 30; // of a sequence's table, of a prefix
+constexpr int64_t MAX_ROW_HEADS = int64_t{ 1 } << 30; // rows * q_heads
+constexpr int64_t MAX_SEQUENCES = int64_t{ 1 } << 20;
+constexpr int64_t MAX_ALL_KEYS	= int64_t{ 1 } << 35; // sequences * keys of a table: their number in steps of 32 is a 32-bit sum
+
+inline int page_shift(int64_t page_size) {
+	for (int shift = 4; shift <= 8; ++shift) {
+		if (page_size == int64_t{ 1 } << shift) {
+			return shift;
+		}
+	}
+	return -1;
+}
+inline int check_cache(const nh_attn_cache* c) {
+	NH_REQUIRE(c, NH_ERR_NULL_POINTER);
+	NH_REQUIRE(c->type == NH_F16 || c->type == NH_BF16, NH_ERR_ARGUMENT);
+	NH_REQUIRE(c->layers > 0 && c->pages > 0 && c->kv_heads > 0 && page_shift(c->page_size) > 0 && (c->head_dim == 64 || c->head_dim == 128), NH_ERR_SHAPE);
+	NH_REQUIRE(c->layers <= 65536 && c->kv_heads <= 65536 && c->pages <= (int64_t{ 1 } << 28), NH_ERR_TOO_LARGE);
+	NH_REQUIRE(c->k_pages && c->v_pages, NH_ERR_NULL_POINTER);
+	NH_REQUIRE(aligned16(c->k_pages) && aligned16(c->v_pages), NH_ERR_ALIGNMENT);
+	return NH_OK;
+}
+// for batches that have sequences
+inline int check_batch(const nh_attn_batch* b, int64_t page_size) {
+	NH_REQUIRE(b, NH_ERR_NULL_POINTER);
+	NH_REQUIRE(b->sequences >= 0 && b->table_width >= 0, NH_ERR_SHAPE);
+	NH_REQUIRE(b->sequences <= MAX_SEQUENCES && b->table_width <= MAX_KEYS / page_size && b->sequences * b->table_width * page_size <= MAX_ALL_KEYS, NH_ERR_TOO_LARGE);
+	NH_REQUIRE(b->sequences == 0 || (b->lengths && (b->page_table || b->table_width == 0)), NH_ERR_NULL_POINTER);
+	return NH_OK;
+}
+inline int64_t value_bytes(int type) {
+	return type == NH_F32 ? 4 : 2;
+}
+// q (k, v, out): type, heads, strides
+inline int check_rows(const nh_attn_cache* c, int type, int64_t rows, int64_t heads, int64_t stride) {
+	NH_REQUIRE(type == NH_F32 || type == c->type, NH_ERR_ARGUMENT);
+	NH_REQUIRE(rows >= 0 && heads > 0 && heads % c->kv_heads == 0, NH_ERR_SHAPE);
+	NH_REQUIRE(heads <= 65536 && rows <= MAX_ROW_HEADS / heads, NH_ERR_TOO_LARGE);
+	NH_REQUIRE(stride >= heads * c->head_dim && stride <= (int64_t{ 1 } << 40), NH_ERR_SHAPE);
+	NH_REQUIRE(stride * value_bytes(type) % 16 == 0, NH_ERR_ALIGNMENT);
+	return NH_OK;
+}
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+	const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+	return a && b && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
+inline nh::cache_view view(const nh_attn_cache* c) {
+	return nh::cache_view{ static_cast<uint16_t*>(c->k_pages), static_cast<uint16_t*>(c->v_pages), c->kv_heads * c->page_size * c->head_dim, static_cast<int>(c->pages),
+		static_cast<int>(c->kv_heads), page_shift(c->page_size) };
+}
+inline nh::batch_view view(const nh_attn_batch* b) {
+	return nh::batch_view{ b->page_table, b->lengths, b->starts, static_cast<int>(b->sequences), static_cast<int>(b->table_width) };
+}
+
+} // namespace
+
+extern "C" {
+
+int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, const void* k, const void* v, void* q_out, int type, int64_t rows, int64_t q_heads,
+	int64_t q_stride, int64_t k_stride, int64_t v_stride, const double* turns, int64_t pairs, int interleaved, void* stream) {
+	NH_TRY(check_cache(host_cache));
+	NH_REQUIRE(host_cache->layers == 1, NH_ERR_SHAPE);
+	NH_TRY(check_batch(host_batch, host_cache->page_size));
+	NH_TRY(check_rows(host_cache, type, rows, q_heads, q_stride));
+	NH_TRY(check_rows(host_cache, type, rows, host_cache->kv_heads, k_stride));
+	NH_TRY(check_rows(host_cache, type, rows, host_cache->kv_heads, v_stride));
+	NH_REQUIRE(pairs >= 0 && pairs % 8 == 0 && 2 * pairs <= host_cache->head_dim, NH_ERR_SHAPE);
+	NH_REQUIRE(host_batch->starts || rows == host_batch->sequences, NH_ERR_ARGUMENT);
+	if (rows == 0 || host_batch->sequences == 0) {
+		return NH_OK;
+	}
+	NH_REQUIRE(q && k && v && q_out && (turns || pairs == 0), NH_ERR_NULL_POINTER);
+	NH_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out), NH_ERR_ALIGNMENT);
+	NH_REQUIRE(q_out != q || q_stride == q_heads * host_cache->head_dim, NH_ERR_ARGUMENT);
+	NH_TRY(require_device());
+	nh::append_args a{};
+	a.cache = view(host_cache), a.batch = view(host_batch);
+	a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.turns = turns;
+	a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
+	a.rows = static_cast<int>(rows), a.q_heads = static_cast<int>(q_heads), a.head_dim = static_cast<int>(host_cache->head_dim), a.pairs = static_cast<int>(pairs);
+	a.interleaved = interleaved != 0;
+	return from_hip(nh::launch_append_rope(a, host_cache->type, type, as_stream(stream)));
+}
+
+static int check_attention(const nh_attn_cache* c, const nh_attn_batch* b, int type, int64_t rows, int64_t q_heads, int64_t q_stride, float scale) {
+	NH_TRY(check_cache(c));
+	NH_REQUIRE(c->layers == 1, NH_ERR_SHAPE);
+	NH_TRY(check_batch(b, c->page_size));
+	NH_TRY(check_rows(c, type, rows, q_heads, q_stride));
+	NH_REQUIRE(scale > 0.0f && std::isfinite(scale), NH_ERR_ARGUMENT);
+	return NH_OK;
+}
+static nh::attention_args attention(const nh_attn_cache* c, const nh_attn_batch* b, const void* q, void* out, int64_t rows, int64_t q_heads, int64_t q_stride, float scale) {
+	nh::attention_args a{};
+	a.cache = view(c), a.batch = view(b);
+	a.q = q, a.out = out, a.q_stride = q_stride;
+	a.rows = static_cast<int>(rows), a.q_heads = static_cast<int>(q_heads), a.head_dim = static_cast<int>(c->head_dim);
+	a.scale = scale;
+	return a;
+}
+
+int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, void* out, int type, int64_t rows, int64_t q_heads, int64_t q_stride, float scale,
+	void* stream) {
+	NH_TRY(check_attention(host_cache, host_batch, type, rows, q_heads, q_stride, scale));
+	if (rows == 0 || host_batch->sequences == 0) {
+		return NH_OK;
+	}
+	NH_REQUIRE(host_batch->starts && q && out, NH_ERR_NULL_POINTER);
+	NH_REQUIRE(aligned16(q) && aligned16(out), NH_ERR_ALIGNMENT);
+	// one workgroup for 128 rows of a kv head, and one more for each sequence and kv head
+	NH_REQUIRE(rows * q_heads / 128 + host_batch->sequences * host_cache->kv_heads <= MAX_ROW_HEADS, NH_ERR_TOO_LARGE);
+	NH_TRY(require_device());
+	return from_hip(nh::launch_attention_prompt(attention(host_cache, host_batch, q, out, rows, q_heads, q_stride, scale), host_cache->type, type, as_stream(stream)));
+}
+
+int64_t nh_attn_decode_workspace_bytes(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_count, int64_t page_size) {
+	if (sequences < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128) || prefix_count < 0 || page_shift(page_size) < 0) {
+		return NH_ERR_SHAPE;
+	}
+	if (sequences > MAX_SEQUENCES || q_heads > 65536 || sequences > MAX_ROW_HEADS / q_heads || prefix_count > MAX_KEYS / page_size) {
+		return NH_ERR_TOO_LARGE;
+	}
+	return nh::attention_decode_workspace(sequences, q_heads, kv_heads, head_dim, prefix_count * page_size);
+}
+
+int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* prefix_pages, int64_t prefix_count, const void* q, void* out, int type, int64_t q_heads,
+	int64_t q_stride, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+	NH_REQUIRE(host_batch, NH_ERR_NULL_POINTER);
+	NH_TRY(check_attention(host_cache, host_batch, type, host_batch->sequences, q_heads, q_stride, scale));
+	NH_REQUIRE(!host_batch->starts, NH_ERR_ARGUMENT);
+	const int64_t need = nh_attn_decode_workspace_bytes(host_batch->sequences, q_heads, host_cache->kv_heads, host_cache->head_dim, prefix_count, host_cache->page_size);
+	NH_REQUIRE(need >= 0, static_cast<int>(need));
+	if (host_batch->sequences == 0) {
+		return NH_OK;
+	}
+	NH_REQUIRE(q && out && workspace && (prefix_pages || prefix_count == 0), NH_ERR_NULL_POINTER);
+	NH_REQUIRE(aligned16(q) && aligned16(out) && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, NH_ERR_ALIGNMENT);
+	NH_REQUIRE(workspace_bytes >= need, NH_ERR_ARGUMENT);
+	NH_TRY(require_device());
+	nh::attention_args a = attention(host_cache, host_batch, q, out, host_batch->sequences, q_heads, q_stride, scale);
+	a.prefix_pages		 = prefix_pages;
+	a.prefix_count		 = static_cast<int>(prefix_count);
+	a.workspace			 = workspace;
+	return from_hip(nh::launch_attention_decode(a, host_cache->type, type, as_stream(stream)));
+}
+
+int64_t nh_attn_pages_workspace_bytes(int64_t pages, int64_t sequences, int64_t table_width) {
+	if (pages <= 0 || sequences < 0 || table_width < 0) {
+		return NH_ERR_SHAPE;
+	}
+	if (pages > (int64_t{ 1 } << 28) || sequences > MAX_SEQUENCES) {
+		return NH_ERR_TOO_LARGE;
+	}
+	return nh::cache_pages_workspace(pages, sequences, table_width);
+}
+
+static int check_pages(const nh_attn_cache* c, const nh_attn_batch* b, int64_t children, const int32_t* new_table, const int32_t* info, const void* workspace, int64_t workspace_bytes) {
+	NH_TRY(check_cache(c));
+	NH_TRY(check_batch(b, c->page_size));
+	NH_REQUIRE(children >= 0, NH_ERR_SHAPE);
+	NH_REQUIRE(children <= MAX_SEQUENCES && children * b->table_width * c->page_size <= MAX_ALL_KEYS, NH_ERR_TOO_LARGE);
+	const int64_t need = nh_attn_pages_workspace_bytes(c->pages, children, b->table_width);
+	NH_REQUIRE(need >= 0, static_cast<int>(need));
+	NH_REQUIRE(info && workspace && (new_table || children * b->table_width == 0), NH_ERR_NULL_POINTER);
+	NH_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, NH_ERR_ALIGNMENT);
+	NH_REQUIRE(workspace_bytes >= need, NH_ERR_ARGUMENT);
+	// the new table is written while the old one is read
+	NH_REQUIRE(!overlap(new_table, children * b->table_width * 4, b->page_table, b->sequences * b->table_width * 4), NH_ERR_ARGUMENT);
+	return NH_OK;
+}
+static nh::pages_args pages(const nh_attn_cache* c, const nh_attn_batch* b, int32_t* new_table, int32_t* info, void* workspace) {
+	nh::pages_args a{};
+	a.k = static_cast<uint16_t*>(c->k_pages), a.v = static_cast<uint16_t*>(c->v_pages);
+	a.page_bytes = c->kv_heads * c->page_size * c->head_dim * 2;
+	a.layers	 = c->layers;
+	a.pages		 = static_cast<int>(c->pages);
+	a.page_shift = page_shift(c->page_size);
+	a.batch		 = view(b);
+	a.new_table = new_table, a.info = info, a.workspace = workspace;
+	return a;
+}
+
+int nh_attn_cache_step(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* parents, const int32_t* grow, int64_t children, int32_t* new_table, int32_t* new_lengths,
+	int32_t* info, void* workspace, int64_t workspace_bytes, void* stream) {
+	NH_TRY(check_pages(host_cache, host_batch, children, new_table, info, workspace, workspace_bytes));
+	NH_REQUIRE(children == 0 || (parents && grow && new_lengths), NH_ERR_NULL_POINTER);
+	NH_REQUIRE(!overlap(new_lengths, children * 4, host_batch->lengths, host_batch->sequences * 4) && !overlap(new_lengths, children * 4, parents, children * 4) &&
+			!overlap(new_lengths, children * 4, grow, children * 4),
+		NH_ERR_ARGUMENT);
+	NH_TRY(require_device());
+	nh::pages_args a = pages(host_cache, host_batch, new_table, info, workspace);
+	a.parents = parents, a.grow = grow, a.new_lengths = new_lengths;
+	a.children = static_cast<int>(children);
+	return from_hip(nh::launch_cache_step(a, as_stream(stream)));
+}
+
+int nh_attn_cache_compact(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, int32_t* new_table, int32_t* info, void* workspace, int64_t workspace_bytes, void* stream) {
+	NH_REQUIRE(host_batch, NH_ERR_NULL_POINTER);
+	NH_TRY(check_pages(host_cache, host_batch, host_batch->sequences, new_table, info, workspace, workspace_bytes));
+	NH_TRY(require_device());
+	return from_hip(nh::launch_cache_compact(pages(host_cache, host_batch, new_table, info, workspace), as_stream(stream)));
+}
+
+} // extern "C"

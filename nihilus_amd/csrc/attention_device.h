@@ -1,0 +1,209 @@
+// Device-side helpers shared by the gfx950 attention kernels: operand types of the 16-bit matrix instructions, the paged cache's
+// addressing, the splitting of fp32 values into 16-bit terms, and the launch functions each translation unit exports.
+#pragma once
+
+#include "../../include/nihilus_amd/attention_abi.h"
+#include "q8_0_device.h"
+
+namespace nh {
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+
+// The matrix instructions of one 16-bit type.  A: 16 (32) rows, B: 16 (32) columns; lane l holds 8 values of row / column l % 16 (32) along the
+// axis that is added up, from 8 * (l / 16 (32)) on.  Result: column l % 16 (32); rows 4 (l / 16) + i, or 8 (i / 4) + 4 (l / 32) + i % 4.
+template<int TYPE> struct half_type;
+template<> struct half_type<NH_F16> {
+	using value = _Float16;
+	using vec	= v8h;
+	static constexpr int terms_of_f32 = 2; // 11 + 11 bits
+	static __device__ __forceinline__ v4f mfma16(vec a, vec b, v4f c) {
+		return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+	}
+	static __device__ __forceinline__ v16f mfma32(vec a, vec b, v16f c) {
+		return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+	}
+};
+template<> struct half_type<NH_BF16> {
+	using value = __bf16;
+	using vec	= v8b;
+	static constexpr int terms_of_f32 = 3; // 8 + 8 + 8 bits
+	static __device__ __forceinline__ v4f mfma16(vec a, vec b, v4f c) {
+		return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+	}
+	static __device__ __forceinline__ v16f mfma32(vec a, vec b, v16f c) {
+		return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+	}
+};
+// fp32 q: as many terms as make up an fp32 value; q of the cache's type: itself
+template<int CACHE, int Q> constexpr int terms = Q == NH_F32 ? half_type<CACHE>::terms_of_f32 : 1;
+
+// x as a sum of N values of 16 bits, each the rounded rest of those before it (round to nearest even).  Eight at once, as one operand of
+// a matrix instruction for each term.
+template<int CACHE, int N> __device__ __forceinline__ void split8(const float (&x)[8], typename half_type<CACHE>::vec (&t)[N]) {
+	using value = typename half_type<CACHE>::value;
+#pragma unroll
+	for (int j = 0; j < 8; ++j) {
+		float rest = x[j];
+#pragma unroll
+		for (int n = 0; n < N; ++n) {
+			const value v = static_cast<value>(rest);
+			t[n][j]		  = v;
+			rest		  = __fsub_rn(rest, static_cast<float>(v));
+		}
+	}
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+	return __builtin_amdgcn_exp2f(x); // v_exp_f32: 1 ulp; arguments here are <= 0, results below 2^-126 are flushed, far under a sum that holds a 1
+}
+// the larger / the sum of this lane's value and that of lane ^ 32 (^ 16)
+__device__ __forceinline__ float swap32(float x) {
+	const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+	return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float swap16(float x) {
+	const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
+	return __builtin_bit_cast(float, (threadIdx.x & 16) ? r[0] : r[1]);
+}
+
+// One layer's pages as the kernels see them.
+struct cache_view {
+	uint16_t* k;
+	uint16_t* v;
+	int64_t page_values; // values of one page: kv_heads * page_size * head_dim
+	int pages;
+	int kv_heads;
+	int page_shift; // log2(page_size)
+};
+struct batch_view {
+	const int32_t* table;
+	const int32_t* lengths;
+	const int32_t* starts;
+	int sequences;
+	int width;
+};
+
+// The sequence that packed row `row` belongs to, the number of its first row that is not below `row`'s... : b with starts[b] <= row <
+// starts[b + 1], or -1.  starts ascends; an empty sequence shares its start with the next one and is passed over.
+__device__ __forceinline__ int sequence_of_row(const int32_t* starts, int sequences, int row) {
+	int lo = 0, hi = sequences + 1; // the first index whose start is above row lies in [lo, hi]
+	while (lo < hi) {
+		const int mid = (lo + hi) >> 1;
+		if (starts[mid] > row) {
+			hi = mid;
+		} else {
+			lo = mid + 1;
+		}
+	}
+	return lo > 0 && lo <= sequences ? lo - 1 : -1;
+}
+
+// Softmax weights are formed as 2^(t - m + bias), t = scale log2(e) q.k, m the row's running maximum of t: sums and products carry the
+// same factor, which the last division takes out.  fp16 weights then lie in (0, 2^8] and keep all their bits down to 2^-22 of the largest.
+template<int CACHE> constexpr float weight_bias = CACHE == NH_F16 ? 8.0f : 0.0f;
+constexpr float LOG2_E = 1.44269504088896340736f;
+
+// Eight consecutive values of a q row as fp32 (all zero where there is no row).
+template<int TYPE> __device__ __forceinline__ void load_q8(const void* q, int64_t at, bool there, float (&x)[8]) {
+	if (!there) {
+#pragma unroll
+		for (int j = 0; j < 8; ++j) {
+			x[j] = 0.0f;
+		}
+		return;
+	}
+	if constexpr (TYPE == NH_F32) {
+		const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(q) + at);
+		const float4 a = p[0], b = p[1];
+		x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+	} else {
+		const auto v = *reinterpret_cast<const typename half_type<TYPE>::vec*>(static_cast<const uint16_t*>(q) + at);
+#pragma unroll
+		for (int j = 0; j < 8; ++j) {
+			x[j] = static_cast<float>(v[j]);
+		}
+	}
+}
+// The power of two that brings a row of fp32 q values, the largest of them `largest`, into the middle of fp16's range: q * 2^(14 - e) with
+// 2^(e-1) <= largest < 2^e, so that two fp16 terms hold 22 bits of each value that matters beside the largest.  bf16 has fp32's range: e = 14.
+template<int CACHE, int TYPE> __device__ __forceinline__ int q_exponent(float largest) {
+	if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
+		int e = 14;
+		if (largest > 0.0f && largest < __builtin_inff()) {
+			(void)frexpf(largest, &e);
+			e = max(e, -60); // (a row this small gives scores of 2^-60: what is lost of it does not show)
+		}
+		return e;
+	}
+	return 14;
+}
+
+// Four values of an output row, rounded once.
+template<int TYPE> __device__ __forceinline__ void store_out4(void* out, int64_t at, float a, float b, float c, float d) {
+	if constexpr (TYPE == NH_F32) {
+		*reinterpret_cast<float4*>(static_cast<float*>(out) + at) = make_float4(a, b, c, d);
+	} else {
+		typedef typename half_type<TYPE>::value v4t __attribute__((ext_vector_type(4)));
+		using value = typename half_type<TYPE>::value;
+		const v4t v{ static_cast<value>(a), static_cast<value>(b), static_cast<value>(c), static_cast<value>(d) };
+		*reinterpret_cast<v4t*>(static_cast<uint16_t*>(out) + at) = v;
+	}
+}
+
+// ---- launch functions (after argument checks) ----
+
+struct append_args {
+	cache_view cache;
+	batch_view batch;
+	const void *q, *k, *v;
+	void* q_out;
+	const double* turns;
+	int64_t q_stride, k_stride, v_stride;
+	int rows, q_heads, head_dim, pairs;
+	bool interleaved;
+};
+hipError_t launch_append_rope(const append_args& a, int cache_type, int type, hipStream_t s);
+
+struct attention_args {
+	cache_view cache;
+	batch_view batch;
+	const void* q;
+	void* out;
+	int64_t q_stride;
+	int rows, q_heads, head_dim;
+	float scale;
+	const int32_t* prefix_pages; // decode only
+	int prefix_count;
+	void* workspace;
+};
+hipError_t launch_attention_prompt(const attention_args& a, int cache_type, int type, hipStream_t s);
+// The part of a decode step over a prefix that all sequences share: the batch's rows as tiles, the keys in pieces.
+struct prefix_cut {
+	int64_t pieces, keys, row_tiles; // keys of a piece
+};
+prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64_t prefix_keys);
+// partial results [piece][sequence][q_head]: o unnormalised, ml the running maximum (log2) and the sum of the weights
+hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s);
+int64_t attention_decode_workspace(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
+hipError_t launch_attention_decode(const attention_args& a, int cache_type, int type, hipStream_t s);
+
+struct pages_args {
+	uint16_t *k, *v;
+	int64_t page_bytes; // of the keys, or of the values, of one page in one layer
+	int64_t layers;
+	int pages;
+	int page_shift;
+	batch_view batch;
+	const int32_t *parents, *grow; // step only
+	int children;
+	int32_t *new_table, *new_lengths, *info;
+	void* workspace;
+};
+int64_t cache_pages_workspace(int64_t pages, int64_t sequences, int64_t width);
+hipError_t launch_cache_step(const pages_args& a, hipStream_t s);
+hipError_t launch_cache_compact(const pages_args& a, hipStream_t s);
+
+} // namespace nh

@@ -1,0 +1,399 @@
+// Attention of many rows over the same paged keys and values, gfx950: the causal attention of packed sequences' new rows, and the part of a
+// decode step's attention that goes over a prefix which the whole batch shares.
+//
+//   out[r] = sum_j softmax_j(scale q[r] . k_j) v_j,  j <= position of row r
+//
+// (k.q, softmax, .v and the head merge of the reference's mega_attention core, infra/core_traits.hpp:743-766, whose GPU body is empty.)
+//
+// A workgroup owns 128 rows of one kv head of one sequence (of the batch, for a prefix), four waves of 32: the rows of all query heads that share the kv head, token after
+// token (row = token * group + head in the group), so that keys and values are fetched once for the group and the diagonal stays short.  It walks the
+// keys in tiles of 64, which it brings into LDS, the next tile's loads in flight under this one's arithmetic.
+//
+// Both products are transposed, S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16): a lane then holds scores of ONE row, the running
+// maximum and sum are the lane's own (one exchange with lane ^ 32 per tile), rescaling O is a product with a number of the lane's own, and, with the rows of
+// the K operand put in the right order, the lane holds exactly the scores that it has to supply as the P^T operand: no shuffle, no LDS.
+// Result rows 8 (i / 4) + 4 (l / 32) + i % 4 of a lane have to be keys 16 (i / 8) + 8 (l / 32) + i % 8, so operand row m takes key m with bits
+// 2 and 3 swapped.
+#include "attention_device.h"
+
+#include <algorithm>
+
+namespace nh {
+
+namespace {
+
+constexpr int WAVES = 4;
+constexpr int ROWS	= 32 * WAVES;
+constexpr int KEYS	= 64; // of a tile
+
+// the key (of 32) that row m of the K operand holds
+__device__ __forceinline__ int key_of_row(int m) {
+	return (m & 0x13) | ((m & 4) << 1) | ((m & 8) >> 1);
+}
+// Pieces of 16 bytes of a K tile row (head_dim values) and of a V tile row (64 keys) are permuted in LDS so that eight lanes that read the
+// same piece of eight rows hit different banks: the rows differ in bits 0, 1, 3 (K: see key_of_row) or 0, 1, 2 (V).
+__device__ __forceinline__ int k_swizzle(int row) {
+	return (row & 3) | ((row >> 1) & 4);
+}
+__device__ __forceinline__ int v_swizzle(int row) {
+	return row & 7;
+}
+
+struct tile_place {
+	int seq, first_token, tokens, first_row, pos0; // the tile's rows start at first_row of tokens * group; pos0: position of the sequence's first token
+	bool there;
+};
+// Which sequence tile `t` belongs to: every wave adds up the sequences' tiles by itself, 64 at a time.
+__device__ __forceinline__ tile_place place_of_tile(const batch_view& b, int rows, int group, int t) {
+	const int lane = threadIdx.x & 63;
+	tile_place p{ 0, 0, 0, 0, 0, false };
+	int before = 0;
+	for (int base = 0; base < b.sequences; base += 64) {
+		const int seq = base + lane;
+		int first = 0, n = 0, end = 0;
+		if (seq < b.sequences) {
+			end	  = b.starts[seq + 1];
+			first = max(b.starts[seq], 0);
+			n	  = max(min(end, rows) - first, 0);
+		}
+		const int tiles = static_cast<int>((static_cast<int64_t>(n) * group + ROWS - 1) / ROWS);
+		int sum			= tiles;
+#pragma unroll
+		for (int d = 1; d < 64; d <<= 1) {
+			const int other = __shfl_up(sum, d);
+			sum += lane >= d ? other : 0;
+		}
+		const uint64_t over = __builtin_amdgcn_ballot_w64(before + sum > t);
+		if (over) {
+			const int src = __builtin_ctzll(over);
+			p.seq		  = base + src;
+			p.first_token = __builtin_amdgcn_readlane(first, src);
+			p.tokens	  = __builtin_amdgcn_readlane(n, src);
+			const int k	  = t - before - (__builtin_amdgcn_readlane(sum, src) - __builtin_amdgcn_readlane(tiles, src));
+			p.first_row	  = (__builtin_amdgcn_readlane(tiles, src) - 1 - k) * ROWS; // the last tiles have the most keys: first
+			p.pos0		  = b.lengths[p.seq] - (__builtin_amdgcn_readlane(end, src) - p.first_token);
+			p.there		  = true;
+			return p;
+		}
+		before += __builtin_amdgcn_readlane(sum, 63);
+	}
+	return p;
+}
+
+} // namespace
+
+// Where a prefix's partial results go: piece i of the keys, row (b, query head): o [i][b][q_heads][D] unnormalised, ml the maximum and the sum.
+struct prefix_out {
+	float* o;
+	float2* ml;
+	int keys; // of a piece, a multiple of KEYS
+	int row_tiles;
+};
+
+template<int CACHE, int TYPE, int D, bool PREFIX>
+__global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void attention_tile_kernel(attention_args a, prefix_out out) {
+	using H				= half_type<CACHE>;
+	using vec			= typename H::vec;
+	constexpr int N		= terms<CACHE, TYPE>;
+	constexpr int STEPS = D / 16; // of q.k
+	constexpr int DT	= D / 32; // tiles of O^T
+	constexpr int PIECES = D / 8; // 16-byte pieces of a key
+	constexpr int LOADS	 = KEYS * PIECES / (64 * WAVES); // pieces of K, and of V, per thread
+	__shared__ v4u k_tile[KEYS * PIECES];
+	__shared__ v4u v_tile[D * (KEYS / 8)];
+
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int col = lane & 31, half = lane >> 5;
+	const int group = a.q_heads / a.cache.kv_heads;
+	const int head	= blockIdx.x % a.cache.kv_heads;
+	tile_place p{};
+	int first_key = 0, piece = 0;
+	if constexpr (PREFIX) {
+		const int t	= blockIdx.x / a.cache.kv_heads;
+		piece		= t / out.row_tiles;
+		first_key	= piece * out.keys;
+		p			= tile_place{ 0, 0, a.batch.sequences, t % out.row_tiles * ROWS, 0, true };
+	} else {
+		p = place_of_tile(a.batch, a.rows, group, blockIdx.x / a.cache.kv_heads);
+		if (!p.there) {
+			return;
+		}
+	}
+	const int32_t* table = PREFIX ? a.prefix_pages : a.batch.table + static_cast<int64_t>(p.seq) * a.batch.width;
+	const int width		 = PREFIX ? a.prefix_count : a.batch.width;
+	const int held		 = width << a.cache.page_shift; // keys that the table has room for (below 2^31: checked on the host)
+	const int all_rows	 = p.tokens * group; // (likewise)
+	const int row		 = p.first_row + 32 * wave + col;
+	const bool there	 = row < all_rows;
+	const int token		 = row / group;
+	const int q_head	 = head * group + row - token * group;
+	int pos				 = -1; // of this lane's row: it sees keys 0 .. pos
+	int limit, wave_min, wave_limit; // no row of the tile sees a key from limit on, none of the wave one from wave_limit on, and all of the wave's see those up to wave_min
+	if constexpr (PREFIX) {
+		limit = min(first_key + out.keys, held);
+		pos	  = there ? min(a.batch.lengths[token], limit) - 1 : -1;
+		wave_min = there ? pos : limit, wave_limit = pos + 1;
+#pragma unroll
+		for (int d = 1; d < 32; d <<= 1) {
+			wave_min   = min(wave_min, __shfl_xor(wave_min, d));
+			wave_limit = max(wave_limit, __shfl_xor(wave_limit, d));
+		}
+		wave_min   = __builtin_amdgcn_readfirstlane(wave_min);
+		wave_limit = __builtin_amdgcn_readfirstlane(wave_limit);
+	} else {
+		const int last_row	 = min(p.first_row + ROWS, all_rows) - 1;
+		const int wave_first = p.first_row + 32 * wave;
+		pos					 = there ? p.pos0 + token : -1;
+		limit				 = max(0, min(held, p.pos0 + last_row / group + 1));
+		wave_min			 = p.pos0 + wave_first / group;
+		wave_limit			 = wave_first < all_rows ? p.pos0 + min(wave_first + 31, all_rows - 1) / group + 1 : 0;
+	}
+
+	// q as the B operand: column = row, values 16 s + 8 half .. + 7
+	vec q[N][STEPS];
+	float c; // scores times c are log2 of the weights
+	{
+		const int64_t at = static_cast<int64_t>(p.first_token + token) * a.q_stride + static_cast<int64_t>(q_head) * D + 8 * half;
+		int e			 = 14;
+		if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
+			float largest = 0.0f;
+#pragma unroll
+			for (int s = 0; s < STEPS; ++s) {
+				float x[8];
+				load_q8<TYPE>(a.q, at + 16 * s, there, x);
+#pragma unroll
+				for (int j = 0; j < 8; ++j) {
+					largest = fmaxf(largest, fabsf(x[j]));
+				}
+			}
+			e = q_exponent<CACHE, TYPE>(fmaxf(largest, swap32(largest)));
+		}
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			float x[8];
+			load_q8<TYPE>(a.q, at + 16 * s, there, x);
+			if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
+#pragma unroll
+				for (int j = 0; j < 8; ++j) {
+					x[j] = ldexpf(x[j], 14 - e);
+				}
+			}
+			vec t[N];
+			split8<CACHE, N>(x, t);
+#pragma unroll
+			for (int n = 0; n < N; ++n) {
+				q[n][s] = t[n];
+			}
+		}
+		c = ldexpf(a.scale * LOG2_E, e - 14);
+	}
+
+	// the pages of a tile: lane i holds that of keys 16 (i % 4) .. + 15, -1 where there is none
+	auto page_ids = [&](int kt) {
+		const int slot = (kt * KEYS + 16 * (lane & 3)) >> a.cache.page_shift;
+		const int id   = slot < width ? table[slot] : -1;
+		return id >= 0 && id < a.cache.pages ? id : -1;
+	};
+	const int page_size = 1 << a.cache.page_shift;
+	v4u k_reg[LOADS], v_reg[LOADS];
+	auto load_tile = [&](int kt, int ids) {
+#pragma unroll
+		for (int i = 0; i < LOADS; ++i) {
+			const int piece = tid + 64 * WAVES * i;
+			const int r = piece / PIECES, x = piece % PIECES;
+			const int key  = kt * KEYS + r;
+			const int page = max(__shfl(ids, r >> 4), 0);
+			k_reg[i] = *reinterpret_cast<const v4u*>(a.cache.k + page * a.cache.page_values + (static_cast<int64_t>(head) * page_size + (key & (page_size - 1))) * D + 8 * x);
+		}
+#pragma unroll
+		for (int i = 0; i < LOADS; ++i) {
+			const int piece = tid + 64 * WAVES * i;
+			const int d = piece >> 3, x = piece & 7;
+			const int key  = kt * KEYS + 8 * x;
+			const int page = max(__shfl(ids, x >> 1), 0);
+			v_reg[i] = *reinterpret_cast<const v4u*>(a.cache.v + page * a.cache.page_values + (static_cast<int64_t>(head) * D + d) * page_size + (key & (page_size - 1)));
+		}
+	};
+	auto store_tile_to_lds = [&](int kt, uint32_t bad) {
+		const bool edge = kt * KEYS + KEYS > limit || bad;
+#pragma unroll
+		for (int i = 0; i < LOADS; ++i) {
+			const int piece = tid + 64 * WAVES * i;
+			const int r = piece / PIECES, x = piece % PIECES;
+			k_tile[r * PIECES + (x ^ k_swizzle(r))] = k_reg[i];
+		}
+#pragma unroll
+		for (int i = 0; i < LOADS; ++i) {
+			const int piece = tid + 64 * WAVES * i;
+			const int d = piece >> 3, x = piece & 7;
+			v4u v = v_reg[i];
+			if (edge) { // values of keys that no row has: nothing, whatever lies there (a weight of zero times infinity is not zero)
+				const int n = ((bad >> (x >> 1)) & 1) ? 0 : limit - (kt * KEYS + 8 * x); // the first n keys of the piece are real
+#pragma unroll
+				for (int w = 0; w < 4; ++w) {
+					v[w] = n >= 2 * w + 2 ? v[w] : n == 2 * w + 1 ? v[w] & 0xFFFFu : 0u;
+				}
+			}
+			v_tile[d * 8 + (x ^ v_swizzle(d))] = v;
+		}
+	};
+
+	v16f o[DT];
+#pragma unroll
+	for (int t = 0; t < DT; ++t) {
+		o[t] = v16f{};
+	}
+	float m = -__builtin_inff(), l = 0.0f; // running maximum of c * scores, this lane's part of the sum of the weights
+	const int first_tile = first_key / KEYS, tiles = (limit + KEYS - 1) / KEYS;
+	int ids				 = -1;
+	if (first_tile < tiles) {
+		ids = page_ids(first_tile);
+		load_tile(first_tile, ids);
+	}
+	for (int kt = first_tile; kt < tiles; ++kt) {
+		const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ids < 0)) & 15u;
+		__syncthreads(); // the last tile has been read
+		store_tile_to_lds(kt, bad);
+		__syncthreads();
+		if (kt + 1 < tiles) {
+			ids = page_ids(kt + 1);
+			load_tile(kt + 1, ids);
+		}
+		if (kt * KEYS >= wave_limit) {
+			continue; // (wave-uniform; the barriers are at the top)
+		}
+		v16f s[2];
+#pragma unroll
+		for (int kb = 0; kb < 2; ++kb) {
+			s[kb]		  = v16f{};
+			const int r	  = 32 * kb + key_of_row(col);
+			const int swz = k_swizzle(r);
+#pragma unroll
+			for (int st = 0; st < STEPS; ++st) {
+				const vec k = __builtin_bit_cast(vec, k_tile[r * PIECES + ((2 * st + half) ^ swz)]);
+#pragma unroll
+				for (int n = N - 1; n >= 0; --n) { // the small terms first
+					s[kb] = H::mfma32(k, q[n][st], s[kb]);
+				}
+			}
+		}
+		if (kt * KEYS + KEYS - 1 > wave_min || bad) {
+#pragma unroll
+			for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+				for (int i = 0; i < 16; ++i) {
+					const int key = kt * KEYS + 32 * kb + 16 * (i >> 3) + 8 * half + (i & 7);
+					if (key > pos || key >= limit || ((bad >> (2 * kb + (i >> 3))) & 1)) {
+						s[kb][i] = -__builtin_inff();
+					}
+				}
+			}
+		}
+		float top = s[0][0];
+#pragma unroll
+		for (int i = 1; i < 32; ++i) {
+			top = fmaxf(top, s[i >> 4][i & 15]);
+		}
+		top				  = fmaxf(top, swap32(top)) * c;
+		const float m_new = fmaxf(m, top);
+		const float base  = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
+		if (__builtin_amdgcn_ballot_w64(m_new != m)) {
+			const float f = exp2_fast(m - base);
+			l *= f;
+#pragma unroll
+			for (int t = 0; t < DT; ++t) {
+				o[t] *= f;
+			}
+			m = m_new;
+		}
+		const float shift = weight_bias<CACHE> - base;
+#pragma unroll
+		for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+			for (int h = 0; h < 2; ++h) {
+				float w[8];
+#pragma unroll
+				for (int j = 0; j < 8; ++j) {
+					w[j] = exp2_fast(fmaf(s[kb][8 * h + j], c, shift));
+					l += w[j];
+				}
+				vec t[N];
+				split8<CACHE, N>(w, t);
+#pragma unroll
+				for (int dt = 0; dt < DT; ++dt) {
+					const int d = 32 * dt + col;
+					const vec v = __builtin_bit_cast(vec, v_tile[d * 8 + ((4 * kb + 2 * h + half) ^ v_swizzle(d))]);
+#pragma unroll
+					for (int n = N - 1; n >= 0; --n) {
+						o[dt] = H::mfma32(v, t[n], o[dt]);
+					}
+				}
+			}
+		}
+	}
+	if (!there) {
+		return;
+	}
+	l += swap32(l);
+	if constexpr (PREFIX) {
+		const int64_t to = (static_cast<int64_t>(piece) * a.batch.sequences + token) * a.q_heads + q_head;
+		if (half == 0) {
+			out.ml[to] = make_float2(m, l);
+		}
+#pragma unroll
+		for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+			for (int i = 0; i < 16; i += 4) {
+				store_out4<NH_F32>(out.o, to * D + 4 * half + 32 * dt + 2 * i, o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]);
+			}
+		}
+		return;
+	}
+	const float inv	 = l > 0.0f || l != l ? 1.0f / l : 0.0f; // no key at all: zeros
+	const int64_t at = (static_cast<int64_t>(p.first_token + token) * a.q_heads + q_head) * D + 4 * half;
+#pragma unroll
+	for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+		for (int i = 0; i < 16; i += 4) {
+			store_out4<TYPE>(a.out, at + 32 * dt + 2 * i, o[dt][i] * inv, o[dt][i + 1] * inv, o[dt][i + 2] * inv, o[dt][i + 3] * inv);
+		}
+	}
+}
+
+template<int CACHE, int TYPE, bool PREFIX> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, int64_t tiles, hipStream_t s) {
+	const dim3 grid(static_cast<unsigned>(tiles * a.cache.kv_heads));
+	if (a.head_dim == 64) {
+		attention_tile_kernel<CACHE, TYPE, 64, PREFIX><<<grid, dim3(64 * WAVES), 0, s>>>(a, out);
+	} else {
+		attention_tile_kernel<CACHE, TYPE, 128, PREFIX><<<grid, dim3(64 * WAVES), 0, s>>>(a, out);
+	}
+	return hipGetLastError();
+}
+template<bool PREFIX> static hipError_t launch_tiles(const attention_args& a, int cache_type, int type, const prefix_out& out, int64_t tiles, hipStream_t s) {
+	if (cache_type == NH_F16) {
+		return type == NH_F32 ? launch_tiles<NH_F16, NH_F32, PREFIX>(a, out, tiles, s) : launch_tiles<NH_F16, NH_F16, PREFIX>(a, out, tiles, s);
+	}
+	return type == NH_F32 ? launch_tiles<NH_BF16, NH_F32, PREFIX>(a, out, tiles, s) : launch_tiles<NH_BF16, NH_BF16, PREFIX>(a, out, tiles, s);
+}
+
+hipError_t launch_attention_prompt(const attention_args& a, int cache_type, int type, hipStream_t s) {
+	const int64_t group = a.q_heads / a.cache.kv_heads;
+	return launch_tiles<false>(a, cache_type, type, prefix_out{}, a.rows * group / ROWS + a.batch.sequences, s); // (each sequence adds less than a tile)
+}
+
+prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64_t prefix_keys) {
+	prefix_cut c{};
+	if (prefix_keys == 0) {
+		return c;
+	}
+	c.row_tiles			 = (sequences * group + ROWS - 1) / ROWS;
+	const int64_t wanted = std::max<int64_t>(1, 512 / (c.row_tiles * kv_heads)); // two workgroups per CU
+	c.keys				 = ((prefix_keys + wanted - 1) / wanted + KEYS - 1) / KEYS * KEYS;
+	c.pieces			 = (prefix_keys + c.keys - 1) / c.keys;
+	return c;
+}
+hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s) {
+	return launch_tiles<true>(a, cache_type, type, prefix_out{ o, ml, static_cast<int>(cut.keys), static_cast<int>(cut.row_tiles) }, cut.pieces * cut.row_tiles, s);
+}
+
+} // namespace nh

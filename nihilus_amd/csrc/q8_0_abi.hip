@@ -2,6 +2,7 @@
 // Nothing here computes; every rejected argument returns a negative nh_status before any launch, so a
 // malformed call can never reach a kernel with shapes the kernel does not expect.
 #include "../../include/nihilus_amd/q8_0_abi.h"
+#include "abi_checks.h"
 #include "q8_0_plan.h"
 
 #include <cstdlib>
@@ -9,23 +10,15 @@
 
 namespace {
 
+using nh::aligned16;
+using nh::as_stream;
+using nh::from_hip;
+using nh::require_device;
+
 constexpr int64_t MAX_ROWS = int64_t{ 1 } << 30; // row and strip indices are 32-bit inside the kernels
 constexpr int64_t MAX_BLOCKS = int64_t{ 1 } << 35; // blocks per matrix the element-wise kernels can index
 constexpr int64_t MAX_K	   = int64_t{ 1 } << 24; // block and group indices along K are 32-bit
 constexpr int64_t MAX_K_BLOCKS_GEMV = 49152; // the blocks-layout mat-vec keeps the whole activation row (K + K/8 bytes) in 64 KiB of LDS
-
-inline bool aligned16(const void* p) {
-	return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
-}
-inline hipStream_t as_stream(void* s) {
-	return static_cast<hipStream_t>(s);
-}
-inline int from_hip(hipError_t e) {
-	if (e == hipErrorNotReady) {
-		return NH_ERR_BUSY; // the only source: the per-device scratch is still in use by a launch on another stream
-	}
-	return e == hipSuccess ? NH_OK : static_cast<int>(e);
-}
 
 // Common shape checks: sizes non-negative, K a whole number of blocks (of groups for a tiled operand).
 inline int check_shape(int64_t rows_a, int64_t rows_b, int64_t K, bool tiled) {
@@ -44,44 +37,7 @@ inline int check_shape(int64_t rows_a, int64_t rows_b, int64_t K, bool tiled) {
 	return NH_OK;
 }
 
-// First call on a thread: make sure a gfx950 device is current.  Returns NH_OK or NH_ERR_NO_DEVICE.
-int require_device() {
-	static thread_local int cached = 1; // 1 = not checked yet
-	if (cached != 1) {
-		return cached;
-	}
-	int count = 0;
-	if (hipGetDeviceCount(&count) != hipSuccess || count <= 0) {
-		(void)hipGetLastError();
-		return cached = NH_ERR_NO_DEVICE;
-	}
-	int dev = 0;
-	hipDeviceProp_t prop;
-	if (hipGetDevice(&dev) != hipSuccess || hipGetDeviceProperties(&prop, dev) != hipSuccess) {
-		(void)hipGetLastError();
-		return cached = NH_ERR_NO_DEVICE;
-	}
-	if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0) {
-		return cached = NH_ERR_NO_DEVICE; // the code object holds gfx950 ISA only
-	}
-	return cached = NH_OK;
-}
-
 } // namespace
-
-#define NH_REQUIRE(cond, code) \
-	do {                       \
-		if (!(cond)) {         \
-			return (code);     \
-		}                      \
-	} while (0)
-#define NH_TRY(expr)        \
-	do {                    \
-		const int rc_ = (expr); \
-		if (rc_ != NH_OK) { \
-			return rc_;     \
-		}                   \
-	} while (0)
 
 extern "C" {
 
