@@ -19,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from .q8_0 import _stream
+from .q8_0 import _calls, _native, _stream
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 PAGE_SIZES = (16, 32, 64, 128, 256)
@@ -109,6 +109,10 @@ def append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torc
     q [rows, q_heads, head_dim], k and v [rows, kv_heads, head_dim], rows apart by any multiple of 16 bytes; turns as rope_turns gives them, for the first
     2 * len(turns) values of a head: pairs are neighbours if interleaved, else half of those values apart.  Rows that no sequence has are left alone
     (in `out` too)."""
+    if out is None and _calls is not None:
+        r = _native(_calls.append_rope(q, k, v, k_pages, v_pages, page_table, lengths, turns, starts, int(interleaved)), "nh_attn_append_rope")
+        if r is not None:
+            return r
     cache, batch = _pages(k_pages, v_pages, 4), _batch(page_table, lengths, starts, k_pages)
     strides = _rows(q, k_pages, None, "q"), _rows(k, k_pages, k_pages.shape[1], "k"), _rows(v, k_pages, k_pages.shape[1], "v")
     if not (q.dtype == k.dtype == v.dtype) or not (q.shape[0] == k.shape[0] == v.shape[0]):
@@ -126,11 +130,16 @@ def attention_prompt(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     """Causal attention of packed rows [rows, q_heads, head_dim] over what their sequences' pages hold, keys and values of these rows among it.
 
     scale is 1 / sqrt(head_dim) unless given.  Rows that no sequence has are not written (in `out` they keep what they held)."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if out is None and _calls is not None:
+        r = _native(_calls.attention_prompt(q, k_pages, v_pages, page_table, lengths, starts, scale), "nh_attn_prompt")
+        if r is not None:
+            return r
     cache, batch = _pages(k_pages, v_pages, 4), _batch(page_table, lengths, starts, k_pages)
     stride = _rows(q, k_pages, None, "q")
     out = _out(out, q)
     _call("nh_attn_prompt", q.device, C.byref(cache), C.byref(batch), q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[0], q.shape[1], stride,
-          q.shape[2] ** -0.5 if scale is None else scale)
+          scale)
     return out
 
 
@@ -147,6 +156,11 @@ def attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
 
     prefix_pages, int32: pages whose keys every sequence begins with; they are read once for the whole batch, and that many entries at the front of
     each page_table row are not looked at.  A sequence of no tokens gives zeros.  workspace: see decode_workspace; without one the call has its own."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if out is None and workspace is None and _calls is not None:
+        r = _native(_calls.attention_decode(q, k_pages, v_pages, page_table, lengths, prefix_pages, scale), "nh_attn_decode")
+        if r is not None:
+            return r
     cache, batch = _pages(k_pages, v_pages, 4), _batch(page_table, lengths, None, k_pages)
     stride = _rows(q, k_pages, None, "q")
     if q.shape[0] != page_table.shape[0]:
@@ -162,7 +176,7 @@ def attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     elif workspace.device != q.device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise TypeError("workspace must be a contiguous uint8 tensor on the cache's GPU")
     _call("nh_attn_decode", q.device, C.byref(cache), C.byref(batch), prefix_pages.data_ptr() if count else None, count, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[1], stride,
-          q.shape[2] ** -0.5 if scale is None else scale, workspace.data_ptr(), workspace.numel())
+          scale, workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -179,6 +193,10 @@ def cache_step(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.T
     Returns (page_table, lengths, info): the new tables, whose lengths count the tokens to come (what append_rope takes next), and int32 [3]: pages held now,
     pages copied, pages missing.  Full pages are shared, a page that several would go on writing into is copied (keys and values, all layers), sequences
     that nobody goes on with are ended and their pages free.  The old tables stay as they are."""
+    if _calls is not None:
+        r = _native(_calls.cache_step(k_pages, v_pages, page_table, lengths, parents, grow), "nh_attn_cache_step")
+        if r is not None:
+            return r
     cache, batch = _pages(k_pages, v_pages, 5), _batch(page_table, lengths, None, k_pages)
     if parents.dim() != 1:
         raise ValueError("parents must be a vector")
@@ -195,6 +213,10 @@ def cache_compact(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torc
     """Moves the pages that hold the sequences' tokens to the front of the cache, in all layers.
 
     Returns (page_table, info): where they are then, and int32 [3]: pages in use (from that index on nothing is held), pages moved, entries that named no page."""
+    if _calls is not None:
+        r = _native(_calls.cache_compact(k_pages, v_pages, page_table, lengths), "nh_attn_cache_compact")
+        if r is not None:
+            return r
     cache, batch = _pages(k_pages, v_pages, 5), _batch(page_table, lengths, None, k_pages)
     n, width = page_table.shape
     table, info = (torch.empty(s, dtype=torch.int32, device=k_pages.device) for s in ((n, width), (3,)))

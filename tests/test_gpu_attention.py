@@ -508,3 +508,86 @@ def test_prompt_and_decode_agree(A):
     used = [int(p) for p in table[0, : -(-n // page)]]
     for id in used[:-1]:
         assert torch.equal(caches[0][0][id], caches[1][0][id]) and torch.equal(caches[0][1][id], caches[1][1][id])
+
+
+def test_native_calls_and_the_python_way_agree(A, monkeypatch):
+    # the same bits either way, and the native calls are the ones that run
+    b = Batch(67, [50, 0, 90], 16, 2, 64, F16)
+    q, kk, vv = (b.rows(40, h, F32).cuda() for h in (8, 2, 2))
+    starts, turns = torch.tensor([0, 30, 30, 40], dtype=torch.int32).cuda(), A.rope_turns(64)
+    parents, grow = torch.tensor([0, 0, 2], dtype=torch.int32).cuda(), torch.tensor([1, 1, -2], dtype=torch.int32).cuda()
+    k0, v0, table, dl = b.device()
+
+    def calls():
+        k, v = k0.clone(), v0.clone()
+        r = A.append_rope(q, kk, vv, k, v, table, dl, turns, starts=starts, interleaved=False)
+        res = [r, A.attention_prompt(r, k, v, table, dl, starts, scale=0.2), A.attention_decode(r[:3], k, v, table, dl), A.attention_decode(r[:3], k, v, table, dl, prefix_pages=table[0, :1].contiguous()),
+               *A.cache_step(k[None], v[None], table, dl, parents, grow), *A.cache_compact(k[None], v[None], table, dl)]
+        return [*res, k.view(torch.int16), v.view(torch.int16)]
+
+    names = ["append_rope", "attention_prompt", "attention_decode", "cache_step", "cache_compact"]
+    ran = []
+    real = A._calls
+    assert real is not None
+
+    class Seen:
+        def __getattr__(self, name):
+            def call(*args):
+                r = getattr(real, name)(*args)
+                ran.append((name, r is not None))
+                return r
+
+            return call
+
+    monkeypatch.setattr(A, "_calls", Seen())
+    native = calls()
+    assert {n for n, ok in ran if ok} == set(names) and all(ok for _, ok in ran)
+    monkeypatch.setattr(A, "_calls", None)
+    assert all(torch.equal(x, y) for x, y in zip(native, calls()))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_tensors_that_are_refused(A, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(A, "_calls", None)
+    b = Batch(71, [20, 5], 16, 2, 64, F16)
+    k, v, table, dl = b.device()
+    q, turns, starts = b.rows(2, 4, F32).cuda(), A.rope_turns(64), torch.tensor([0, 1, 2], dtype=torch.int32).cuda()
+    kv = b.rows(2, 2, F32).cuda()
+    A.attention_decode(q, k, v, table, dl)
+    errors = (TypeError, ValueError, RuntimeError)
+    for args in [(q, k, v.float(), table, dl), (q, k, v.transpose(-1, -2), table, dl), (q, k, v[:-1], table, dl), (q, k, k, table, dl), (q, k, v, table.long(), dl), (q, k, v, table[0], dl),
+                 (q, k, v, table, dl[:1]), (q, k, v, table.cpu(), dl), (q, k, v, table, dl.cpu()), (q.cpu(), k, v, table, dl), (q.to(BF16), k, v, table, dl), (q[:1], k, v, table, dl),
+                 (q[:, :3], k, v, table, dl), (q[:, :, :32], k, v, table, dl), (q.reshape(2, -1), k, v, table, dl), (q, k[None], v[None], table, dl), (q, k.to(BF16), v, table, dl),
+                 (q, k, v, table.t().contiguous().t(), dl)]:
+        with pytest.raises(errors):
+            A.attention_decode(*args)
+        if args[0].shape[0] == 2:  # (rows that are not there are nobody's for a prompt)
+            with pytest.raises(errors):
+                A.attention_prompt(*args, starts)
+    for s in (starts[:2], starts.long(), starts.cpu(), None):
+        with pytest.raises(errors + (AttributeError,)):
+            A.attention_prompt(q, k, v, table, dl, s)
+    for scale in (0.0, -0.1, float("inf"), float("nan")):
+        with pytest.raises(errors):
+            A.attention_decode(q, k, v, table, dl, scale=scale)
+    with pytest.raises(errors):
+        A.attention_decode(q, k, v, table, dl, prefix_pages=table[0].long())
+    with pytest.raises(errors):
+        A.attention_decode(q, k, v, table, dl, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    for out in (q[:1], q.half(), q.cpu(), torch.empty(2, 64, 4, device="cuda").transpose(1, 2)):
+        with pytest.raises(errors):
+            A.attention_decode(q, k, v, table, dl, out=out)
+    for bad in [(q, kv[:1], kv), (q, kv, kv.half()), (q, kv[:, :1], kv), (q, kv, kv.cpu()), (q.half(), kv, kv)]:
+        with pytest.raises(errors):
+            A.append_rope(*bad, k, v, table, dl, turns)
+    for t in (turns.float(), turns.cpu(), turns[:12], turns[None], A.rope_turns(128)):
+        with pytest.raises(errors):
+            A.append_rope(q, kv, kv, k, v, table, dl, t)
+    parents = torch.zeros(2, dtype=torch.int32).cuda()
+    for args in [(k, v, table, dl, parents, parents), (k[None], v[None], table, dl, parents, parents[:1]), (k[None], v[None], table, dl, parents.long(), parents),
+                 (k[None], v[None], table, dl, parents[None], parents)]:
+        with pytest.raises(errors):
+            A.cache_step(*args)
+    with pytest.raises(errors):
+        A.cache_compact(k, v, table, dl)
