@@ -4,8 +4,10 @@
  *
  * The conventions of q8_0_abi.h hold here too: plain C, device pointers unless a name starts with host_, `stream` a hipStream_t,
  * 0 / negative nh_status / positive hipError_t as the result, no exception.  Calls are asynchronous on their stream, allocate nothing
- * and keep nothing: what a call needs between its launches is in the workspace that it is given.  Calls on different streams with
- * workspaces of their own are independent, also while captured into graphs; two calls, or two graphs, that share a workspace must not overlap.
+ * and keep nothing: what a call needs for itself is in the memory that it is given.  That is a workspace, whose contents mean nothing
+ * before and after a call, and for attention counters, which must be zero when they are first used and are left zero by every call.  Calls on
+ * different streams with workspaces and counters of their own are independent, also while captured into graphs; two calls, or two graphs,
+ * that share either must not overlap.
  *
  * In the reference these are nodes of the mega cores whose GPU bodies are empty: rope and the cache write of
  * mega_qkv_prep_and_cache_publish (infra/core_traits.hpp:596-616), k.q, softmax, .v and the head merge of mega_attention_apply
@@ -75,16 +77,24 @@ int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* ho
  * reads kv head h / (q_heads / kv_heads).  q_heads is a multiple of kv_heads.  starts must not be NULL.
  * type NH_F32: q and the softmax weights go through the 16-bit matrix instructions as sums of two (fp16 cache) or three (bf16) terms,
  * 22 or 24 bits; type = the cache's: q as it is, the weights rounded once.  Everything else (products' sums, maxima, sums) is fp32. */
+/* Memory: nh_attn_prompt_needs says how many bytes (0: many rows need none, and the pointers may be NULL), 256-byte aligned. */
+int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes);
 int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, void* out, int type, int64_t rows, int64_t q_heads, int64_t q_stride, float scale,
-	void* stream);
+	void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream);
+
+/* Which kernel nh_attn_prompt runs for these sizes: 1 the one for few rows (16 at a time, the keys of long sequences over several workgroups), 2 the
+ * one for many (128 at a time, keys and values through LDS).  Needs no GPU.  force: 0 lets the sizes decide from now on, 1 or 2 takes
+ * that kernel always, -1 changes nothing; a test hook, process-wide, which anything but -1 is refused for (NH_ERR_ARGUMENT) unless
+ * the process has NH_Q8_0_DEBUG_HOOKS=1 in its environment. */
+int nh_attn_debug_prompt_kernel(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int force);
 
 /* The same for one row per sequence over all of its keys (starts must be NULL, rows = sequences).  The keys j < prefix_count *
  * page_size of EVERY sequence (as far as its length goes) are those of the pages prefix_pages[0 .. prefix_count): they are read once for the
- * whole batch, and the first prefix_count entries of a page_table row are not looked at.  prefix_count = 0: none shared.
- * workspace: nh_attn_decode_workspace_bytes(...) bytes, 256-byte aligned. */
-int64_t nh_attn_decode_workspace_bytes(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_count, int64_t page_size);
+ * whole batch, and the first prefix_count entries of a page_table row are not looked at.  prefix_count = 0: none shared. */
+int nh_attn_decode_needs(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_count, int64_t page_size, int64_t* host_workspace_bytes,
+	int64_t* host_counter_bytes);
 int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* prefix_pages, int64_t prefix_count, const void* q, void* out, int type, int64_t q_heads,
-	int64_t q_stride, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+	int64_t q_stride, float scale, void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream);
 
 /* From one step's sequences to the next one's.  New sequence i (i < children) goes on where sequence parents[i] stands (a number
  * outside [0, sequences): it is empty), longer by grow[i] tokens or, if that is negative, shorter; its length stays within

@@ -80,9 +80,11 @@ SIGNATURES = {
 # the same of attention_abi.h
 ATTENTION_SIGNATURES = {
     "nh_attn_append_rope": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp]),
-    "nh_attn_prompt": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, C.c_float, _vp]),
-    "nh_attn_decode_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
-    "nh_attn_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, C.c_float, _vp, _i64, _vp]),
+    "nh_attn_prompt_needs": (_int, [_i64, _i64, _i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64)]),
+    "nh_attn_prompt": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, C.c_float, _vp, _i64, _vp, _i64, _vp]),
+    "nh_attn_debug_prompt_kernel": (_int, [_i64, _i64, _i64, _i64, _int]),
+    "nh_attn_decode_needs": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, C.POINTER(_i64), C.POINTER(_i64)]),
+    "nh_attn_decode": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _int, _i64, _i64, C.c_float, _vp, _i64, _vp, _i64, _vp]),
     "nh_attn_pages_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "nh_attn_cache_step": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
     "nh_attn_cache_compact": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp]),

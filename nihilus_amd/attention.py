@@ -125,33 +125,55 @@ def append_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torc
     return out
 
 
+class Workspace:
+    """Memory for the attentions' own use, for callers that keep it: of one stream, or one captured graph, at a time."""
+
+    def __init__(self, nbytes: int, counter_bytes: int, device):
+        self.memory = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        self.counters = torch.zeros(counter_bytes // 4, dtype=torch.int32, device=device)  # every call leaves them zero
+
+    def args(self, like: torch.Tensor):
+        if self.memory.device != like.device:
+            raise TypeError("the workspace must be on the cache's GPU")
+        return self.memory.data_ptr(), self.memory.numel(), self.counters.data_ptr(), 4 * self.counters.numel()
+
+
+def _needs(fn: str, *sizes) -> tuple[int, int]:
+    n, c = C.c_int64(), C.c_int64()
+    _lib.check(fn, getattr(_lib.lib(), fn)(*sizes, C.byref(n), C.byref(c)))
+    return n.value, c.value
+
+
+def prompt_workspace(rows: int, sequences: int, q_heads: int, kv_heads: int, head_dim: int, device="cuda") -> Workspace:
+    return Workspace(*_needs("nh_attn_prompt_needs", rows, sequences, q_heads, kv_heads, head_dim), device)
+
+
+def decode_workspace(sequences: int, q_heads: int, kv_heads: int, head_dim: int, prefix_pages: int = 0, page_size: int = 64, device="cuda") -> Workspace:
+    return Workspace(*_needs("nh_attn_decode_needs", sequences, q_heads, kv_heads, head_dim, prefix_pages, page_size), device)
+
+
 def attention_prompt(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, starts: torch.Tensor, scale: float | None = None,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, workspace: Workspace | None = None) -> torch.Tensor:
     """Causal attention of packed rows [rows, q_heads, head_dim] over what their sequences' pages hold, keys and values of these rows among it.
 
-    scale is 1 / sqrt(head_dim) unless given.  Rows that no sequence has are not written (in `out` they keep what they held)."""
+    scale is 1 / sqrt(head_dim) unless given.  Rows that no sequence has are not written (in `out` they keep what they held).  workspace: see
+    prompt_workspace; without one the call has its own."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    if out is None and _calls is not None:
+    if out is None and workspace is None and _calls is not None:
         r = _native(_calls.attention_prompt(q, k_pages, v_pages, page_table, lengths, starts, scale), "nh_attn_prompt")
         if r is not None:
             return r
     cache, batch = _pages(k_pages, v_pages, 4), _batch(page_table, lengths, starts, k_pages)
     stride = _rows(q, k_pages, None, "q")
     out = _out(out, q)
-    _call("nh_attn_prompt", q.device, C.byref(cache), C.byref(batch), q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[0], q.shape[1], stride,
-          scale)
+    if workspace is None:
+        workspace = prompt_workspace(q.shape[0], page_table.shape[0], q.shape[1], k_pages.shape[1], k_pages.shape[3], q.device)
+    _call("nh_attn_prompt", q.device, C.byref(cache), C.byref(batch), q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[0], q.shape[1], stride, scale, *workspace.args(k_pages))
     return out
 
 
-def decode_workspace(sequences: int, q_heads: int, kv_heads: int, head_dim: int, prefix_pages: int = 0, page_size: int = 64, device="cuda") -> torch.Tensor:
-    """Memory for attention_decode's own use, for callers that keep it: of one stream, or one captured graph, at a time."""
-    n = _lib.lib().nh_attn_decode_workspace_bytes(sequences, q_heads, kv_heads, head_dim, prefix_pages, page_size)
-    _lib.check("nh_attn_decode_workspace_bytes", n if n < 0 else 0)
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
 def attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, prefix_pages: torch.Tensor | None = None,
-                     scale: float | None = None, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+                     scale: float | None = None, out: torch.Tensor | None = None, workspace: Workspace | None = None) -> torch.Tensor:
     """Attention of one row per sequence, q [sequences, q_heads, head_dim], over all of its keys.
 
     prefix_pages, int32: pages whose keys every sequence begins with; they are read once for the whole batch, and that many entries at the front of
@@ -170,13 +192,11 @@ def attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
         count = prefix_pages.numel()
         _ints(prefix_pages, k_pages, (count,), "prefix_pages")
     out = _out(out, q)
-    _, kv_heads, page_size, head_dim = k_pages.shape
     if workspace is None:
+        _, kv_heads, page_size, head_dim = k_pages.shape
         workspace = decode_workspace(q.shape[0], q.shape[1], kv_heads, head_dim, count, page_size, q.device)
-    elif workspace.device != q.device or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise TypeError("workspace must be a contiguous uint8 tensor on the cache's GPU")
-    _call("nh_attn_decode", q.device, C.byref(cache), C.byref(batch), prefix_pages.data_ptr() if count else None, count, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[1], stride,
-          scale, workspace.data_ptr(), workspace.numel())
+    _call("nh_attn_decode", q.device, C.byref(cache), C.byref(batch), prefix_pages.data_ptr() if count else None, count, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[1], stride, scale,
+          *workspace.args(k_pages))
     return out
 
 

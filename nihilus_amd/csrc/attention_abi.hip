@@ -4,7 +4,9 @@
 #include "abi_checks.h"
 #include "attention_device.h"
 
+#include <atomic>
 #include <cmath>
+#include <cstdlib>
 
 namespace {
 
@@ -68,7 +70,17 @@ inline nh::batch_view view(const nh_attn_batch* b) {
 	return nh::batch_view{ b->page_table, b->lengths, b->starts, static_cast<int>(b->sequences), static_cast<int>(b->table_width) };
 }
 
+std::atomic<int> forced_prompt_kernel{ 0 };
+
 } // namespace
+
+bool nh::prompt_by_rows(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads) {
+	if (const int forced = forced_prompt_kernel.load(std::memory_order_relaxed)) {
+		return forced == 1;
+	}
+	(void)sequences, (void)kv_heads;
+	return rows * q_heads < 128 * 128;
+}
 
 extern "C" {
 
@@ -115,49 +127,87 @@ static nh::attention_args attention(const nh_attn_cache* c, const nh_attn_batch*
 	return a;
 }
 
+static int check_memory(int64_t workspace_need, int64_t counter_need, const void* workspace, int64_t workspace_bytes, const void* counters, int64_t counter_bytes) {
+	NH_REQUIRE((workspace || workspace_need == 0) && (counters || counter_need == 0), NH_ERR_NULL_POINTER);
+	NH_REQUIRE(((reinterpret_cast<uintptr_t>(workspace) | reinterpret_cast<uintptr_t>(counters)) & 255u) == 0, NH_ERR_ALIGNMENT);
+	NH_REQUIRE(workspace_bytes >= workspace_need && counter_bytes >= counter_need, NH_ERR_ARGUMENT);
+	return NH_OK;
+}
+static int check_heads(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, const int64_t* a, const int64_t* b) {
+	NH_REQUIRE(a && b, NH_ERR_NULL_POINTER);
+	NH_REQUIRE(rows >= 0 && sequences >= 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128), NH_ERR_SHAPE);
+	// one workgroup for 16 rows of a kv head, and one more for each sequence and kv head
+	NH_REQUIRE(sequences <= MAX_SEQUENCES && q_heads <= 65536 && rows <= MAX_ROW_HEADS / q_heads && sequences * kv_heads <= MAX_ROW_HEADS / 4, NH_ERR_TOO_LARGE);
+	return NH_OK;
+}
+
+int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes) {
+	NH_TRY(check_heads(rows, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
+	const nh::rows_needs n = nh::prompt_by_rows(rows, sequences, q_heads, kv_heads) ? nh::attention_rows_needs(rows, sequences, false, q_heads, kv_heads, head_dim, 0) : nh::rows_needs{ 0, 0 };
+	*host_workspace_bytes  = n.workspace;
+	*host_counter_bytes	   = n.counters;
+	return NH_OK;
+}
+
 int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, void* out, int type, int64_t rows, int64_t q_heads, int64_t q_stride, float scale,
-	void* stream) {
+	void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream) {
 	NH_TRY(check_attention(host_cache, host_batch, type, rows, q_heads, q_stride, scale));
+	int64_t need = 0, counter_need = 0;
+	NH_TRY(nh_attn_prompt_needs(rows, host_batch->sequences, q_heads, host_cache->kv_heads, host_cache->head_dim, &need, &counter_need));
 	if (rows == 0 || host_batch->sequences == 0) {
 		return NH_OK;
 	}
 	NH_REQUIRE(host_batch->starts && q && out, NH_ERR_NULL_POINTER);
 	NH_REQUIRE(aligned16(q) && aligned16(out), NH_ERR_ALIGNMENT);
-	// one workgroup for 128 rows of a kv head, and one more for each sequence and kv head
-	NH_REQUIRE(rows * q_heads / 128 + host_batch->sequences * host_cache->kv_heads <= MAX_ROW_HEADS, NH_ERR_TOO_LARGE);
+	NH_TRY(check_memory(need, counter_need, workspace, workspace_bytes, counters, counter_bytes));
 	NH_TRY(require_device());
-	return from_hip(nh::launch_attention_prompt(attention(host_cache, host_batch, q, out, rows, q_heads, q_stride, scale), host_cache->type, type, as_stream(stream)));
+	nh::attention_args a = attention(host_cache, host_batch, q, out, rows, q_heads, q_stride, scale);
+	a.workspace			 = workspace;
+	a.counters			 = static_cast<int32_t*>(counters);
+	const bool by_rows	 = nh::prompt_by_rows(rows, host_batch->sequences, q_heads, host_cache->kv_heads);
+	return from_hip(by_rows ? nh::launch_attention_rows(a, host_cache->type, type, as_stream(stream)) : nh::launch_attention_tiles(a, host_cache->type, type, as_stream(stream)));
 }
 
-int64_t nh_attn_decode_workspace_bytes(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_count, int64_t page_size) {
-	if (sequences < 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || (head_dim != 64 && head_dim != 128) || prefix_count < 0 || page_shift(page_size) < 0) {
-		return NH_ERR_SHAPE;
+int nh_attn_debug_prompt_kernel(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int force) {
+	if (force != -1) {
+		const char* hooks = std::getenv("NH_Q8_0_DEBUG_HOOKS");
+		NH_REQUIRE(hooks && hooks[0] == '1' && hooks[1] == '\0' && force >= 0 && force <= 2, NH_ERR_ARGUMENT);
+		forced_prompt_kernel.store(force, std::memory_order_relaxed);
 	}
-	if (sequences > MAX_SEQUENCES || q_heads > 65536 || sequences > MAX_ROW_HEADS / q_heads || prefix_count > MAX_KEYS / page_size) {
-		return NH_ERR_TOO_LARGE;
-	}
-	return nh::attention_decode_workspace(sequences, q_heads, kv_heads, head_dim, prefix_count * page_size);
+	return nh::prompt_by_rows(rows, sequences, q_heads, kv_heads) ? 1 : 2;
+}
+
+int nh_attn_decode_needs(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_count, int64_t page_size, int64_t* host_workspace_bytes,
+	int64_t* host_counter_bytes) {
+	NH_TRY(check_heads(sequences, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
+	NH_REQUIRE(prefix_count >= 0 && page_shift(page_size) > 0, NH_ERR_SHAPE);
+	NH_REQUIRE(prefix_count <= MAX_KEYS / page_size, NH_ERR_TOO_LARGE);
+	const nh::rows_needs n = nh::attention_rows_needs(sequences, sequences, true, q_heads, kv_heads, head_dim, prefix_count * page_size);
+	*host_workspace_bytes  = n.workspace;
+	*host_counter_bytes	   = n.counters;
+	return NH_OK;
 }
 
 int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* prefix_pages, int64_t prefix_count, const void* q, void* out, int type, int64_t q_heads,
-	int64_t q_stride, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+	int64_t q_stride, float scale, void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream) {
 	NH_REQUIRE(host_batch, NH_ERR_NULL_POINTER);
 	NH_TRY(check_attention(host_cache, host_batch, type, host_batch->sequences, q_heads, q_stride, scale));
 	NH_REQUIRE(!host_batch->starts, NH_ERR_ARGUMENT);
-	const int64_t need = nh_attn_decode_workspace_bytes(host_batch->sequences, q_heads, host_cache->kv_heads, host_cache->head_dim, prefix_count, host_cache->page_size);
-	NH_REQUIRE(need >= 0, static_cast<int>(need));
+	int64_t need = 0, counter_need = 0;
+	NH_TRY(nh_attn_decode_needs(host_batch->sequences, q_heads, host_cache->kv_heads, host_cache->head_dim, prefix_count, host_cache->page_size, &need, &counter_need));
 	if (host_batch->sequences == 0) {
 		return NH_OK;
 	}
-	NH_REQUIRE(q && out && workspace && (prefix_pages || prefix_count == 0), NH_ERR_NULL_POINTER);
-	NH_REQUIRE(aligned16(q) && aligned16(out) && (reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, NH_ERR_ALIGNMENT);
-	NH_REQUIRE(workspace_bytes >= need, NH_ERR_ARGUMENT);
+	NH_REQUIRE(q && out && (prefix_pages || prefix_count == 0), NH_ERR_NULL_POINTER);
+	NH_REQUIRE(aligned16(q) && aligned16(out), NH_ERR_ALIGNMENT);
+	NH_TRY(check_memory(need, counter_need, workspace, workspace_bytes, counters, counter_bytes));
 	NH_TRY(require_device());
 	nh::attention_args a = attention(host_cache, host_batch, q, out, host_batch->sequences, q_heads, q_stride, scale);
 	a.prefix_pages		 = prefix_pages;
 	a.prefix_count		 = static_cast<int>(prefix_count);
 	a.workspace			 = workspace;
-	return from_hip(nh::launch_attention_decode(a, host_cache->type, type, as_stream(stream)));
+	a.counters			 = static_cast<int32_t*>(counters);
+	return from_hip(nh::launch_attention_rows(a, host_cache->type, type, as_stream(stream)));
 }
 
 int64_t nh_attn_pages_workspace_bytes(int64_t pages, int64_t sequences, int64_t table_width) {

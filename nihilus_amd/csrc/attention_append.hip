@@ -55,11 +55,11 @@ __device__ __forceinline__ bool place_of_row(const batch_view& b, int row, int& 
 		if (seq < 0) {
 			return false;
 		}
-		pos = b.lengths[seq] - (b.starts[seq + 1] - row);
+		pos = max(b.lengths[seq], 0) - (b.starts[seq + 1] - row);
 		return true;
 	}
 	seq = row;
-	pos = b.lengths[row] - 1;
+	pos = max(b.lengths[row], 0) - 1;
 	return true;
 }
 // the page of a position, or -1

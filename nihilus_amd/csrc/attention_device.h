@@ -177,9 +177,11 @@ struct attention_args {
 	float scale;
 	const int32_t* prefix_pages; // decode only
 	int prefix_count;
-	void* workspace;
+	void* workspace; // rows kernel only
+	int32_t* counters;
 };
-hipError_t launch_attention_prompt(const attention_args& a, int cache_type, int type, hipStream_t s);
+// The tile kernel (attention_prompt.hip): 128 rows of a sequence at a time, keys and values through LDS.
+hipError_t launch_attention_tiles(const attention_args& a, int cache_type, int type, hipStream_t s);
 // The part of a decode step over a prefix that all sequences share: the batch's rows as tiles, the keys in pieces.
 struct prefix_cut {
 	int64_t pieces, keys, row_tiles; // keys of a piece
@@ -187,8 +189,14 @@ struct prefix_cut {
 prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64_t prefix_keys);
 // partial results [piece][sequence][q_head]: o unnormalised, ml the running maximum (log2) and the sum of the weights
 hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s);
-int64_t attention_decode_workspace(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
-hipError_t launch_attention_decode(const attention_args& a, int cache_type, int type, hipStream_t s);
+// The rows kernel (attention_rows.hip): 16 rows of a sequence at a time, keys and values straight from memory and cut into pieces.
+struct rows_needs {
+	int64_t workspace, counters; // bytes
+};
+rows_needs attention_rows_needs(int64_t rows, int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
+hipError_t launch_attention_rows(const attention_args& a, int cache_type, int type, hipStream_t s);
+// Which of the two a prompt's rows take (attention_abi.hip).
+bool prompt_by_rows(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads);
 
 struct pages_args {
 	uint16_t *k, *v;

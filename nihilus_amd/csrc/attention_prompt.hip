@@ -71,7 +71,7 @@ __device__ __forceinline__ tile_place place_of_tile(const batch_view& b, int row
 			p.tokens	  = __builtin_amdgcn_readlane(n, src);
 			const int k	  = t - before - (__builtin_amdgcn_readlane(sum, src) - __builtin_amdgcn_readlane(tiles, src));
 			p.first_row	  = (__builtin_amdgcn_readlane(tiles, src) - 1 - k) * ROWS; // the last tiles have the most keys: first
-			p.pos0		  = b.lengths[p.seq] - (__builtin_amdgcn_readlane(end, src) - p.first_token);
+			p.pos0		  = max(b.lengths[p.seq], 0) - (__builtin_amdgcn_readlane(end, src) - p.first_token);
 			p.there		  = true;
 			return p;
 		}
@@ -376,7 +376,7 @@ template<bool PREFIX> static hipError_t launch_tiles(const attention_args& a, in
 	return type == NH_F32 ? launch_tiles<NH_BF16, NH_F32, PREFIX>(a, out, tiles, s) : launch_tiles<NH_BF16, NH_BF16, PREFIX>(a, out, tiles, s);
 }
 
-hipError_t launch_attention_prompt(const attention_args& a, int cache_type, int type, hipStream_t s) {
+hipError_t launch_attention_tiles(const attention_args& a, int cache_type, int type, hipStream_t s) {
 	const int64_t group = a.q_heads / a.cache.kv_heads;
 	return launch_tiles<false>(a, cache_type, type, prefix_out{}, a.rows * group / ROWS + a.batch.sequences, s); // (each sequence adds less than a tile)
 }

@@ -1,0 +1,532 @@
+// Attention of few rows per sequence over its paged keys and values, gfx950: a decode step's one row, a short prompt's or a chunk's few.
+//
+//   out[r] = sum_j softmax_j(scale q[r] . k_j) v_j,  j <= position of row r
+//
+// (mega_attention's eval_time core in the reference, infra/core_traits.hpp:743-766, whose GPU body is empty.)
+//
+// Memory-bound: 4 * head_dim bytes of keys and values against 4 * head_dim * group operations per row.  Every key and value of a row group is read once,
+// straight from its page into the registers that the matrix instruction takes it from (no LDS), by the one wave that owns the key; the rows of
+// all query heads of the kv head, token after token, are the columns of the instruction (v_mfma_f32_16x16x32), 16 of them a row group.  As in
+// the tile kernel the products are transposed, S^T = K Q^T and O^T = V^T P^T: a lane's scores belong to one row, and the operand rows
+// of K are put so that the lane holds the scores that it has to supply as P^T: result rows 4 (l / 16) + i of the two key tiles of a step are keys
+// 8 (l / 16) + 4 tile + i, so operand row m of tile t takes key 8 (m / 4) + 4 t + m % 4.
+//
+// Work: the sequences' keys are cut into pieces of the same length, worked out on the GPU from the lengths (by every wave for itself), so that
+// WORKGROUPS workgroups have about the same work, however the lengths differ.  A piece's four waves take its steps of 32 keys in turn
+// and join their results in LDS.  Where a row group has more pieces than one, each puts its result into the workspace and counts itself; the last
+// to do so joins them, in the pieces' order, so the result does not hang on who that is.
+// A prefix that all sequences share is left to the tile kernel, whose rows are then the heads of all sequences; its pieces are
+// joined with the sequences' own.
+#include "attention_device.h"
+
+#include <algorithm>
+
+namespace nh {
+
+namespace {
+
+constexpr int WAVES		 = 4;
+constexpr int THREADS	 = 64 * WAVES;
+constexpr int STEP		 = 32; // keys of a wave's step
+constexpr int COLUMNS	 = 16; // rows of a row group
+// What the pieces are cut for: twice what the chip holds at once (two per CU), so that the last ones to start are short.  decode of 64 sequences of up to 8192 keys
+// (32 / 8 heads): 512 61.5 us, 1024 55.4, 2048 60.0, 4096 68.5.
+constexpr int WORKGROUPS = 1024;
+
+struct rows_workspace {
+	float* o; // [slot][columns][D]  a piece's sums of weighted values; slot = piece * kv_heads + kv head
+	float2* ml; // [slot][columns]  their maximum (log2) and the sum of the weights
+	float* prefix_o; // [prefix piece][sequences][q_heads][D]
+	float2* prefix_ml;
+	int columns;
+	int prefix_pieces;
+	int32_t* counters; // [slot]  of a row group's first piece: how many of its pieces are done; zero before and after every call
+};
+struct rows_cut {
+	int64_t units; // pieces that the keys are cut into at most, beside one per row group
+	int64_t pieces; // most pieces there can be
+	int64_t columns; // rows of a row group that are kept in the workspace
+};
+rows_cut plan_rows(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t kv_heads) {
+	rows_cut c{};
+	c.units	  = std::max<int64_t>(1, WORKGROUPS / kv_heads);
+	c.pieces  = c.units + (one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : rows * group / COLUMNS + sequences);
+	c.columns = one_each ? std::min<int64_t>(group, COLUMNS) : COLUMNS;
+	return c;
+}
+
+int64_t rounded(int64_t bytes) {
+	return (bytes + 255) / 256 * 256;
+}
+// lays the parts out behind `base`; returns the bytes they take
+int64_t lay_out(char* base, const rows_cut& c, const prefix_cut& prefix, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, rows_workspace* w) {
+	int64_t at = 0;
+	auto part  = [&](int64_t bytes) {
+		char* p = base + at;
+		at += rounded(bytes);
+		return p;
+	};
+	const int64_t own = c.pieces * kv_heads * c.columns, shared = prefix.pieces * sequences * q_heads;
+	w->ml			 = reinterpret_cast<float2*>(part(own * 8));
+	w->o			 = reinterpret_cast<float*>(part(own * head_dim * 4));
+	w->prefix_ml	 = reinterpret_cast<float2*>(part(shared * 8));
+	w->prefix_o		 = reinterpret_cast<float*>(part(shared * head_dim * 4));
+	w->columns		 = static_cast<int>(c.columns);
+	w->prefix_pieces = static_cast<int>(prefix.pieces);
+	return at;
+}
+
+// Sum of a value over lanes 0 .. this one, by data-parallel primitives: within rows of 16 lanes, then from row to row.
+__device__ __forceinline__ int scan64(int x) {
+	x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false); // row_shr:1 (lanes that have no source add 0)
+	x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+	x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); // row_bcast:15 into rows 1 and 3
+	x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); // row_bcast:31 into rows 2 and 3
+	return x;
+}
+
+// What a lane knows of sequence `seq`: its rows, its keys behind the prefix.
+struct sequence_size {
+	int first_row, rows, end; // packed rows first_row .. first_row + rows - 1; starts[seq + 1]
+	int keys;
+};
+__device__ __forceinline__ sequence_size size_of(const batch_view& b, int all_rows, int prefix_keys, int held, int seq) {
+	sequence_size z{ 0, 0, 0, 0 };
+	if (seq < b.sequences) {
+		z.end		= b.starts ? b.starts[seq + 1] : seq + 1;
+		z.first_row = b.starts ? max(b.starts[seq], 0) : seq;
+		z.rows		= max(min(z.end, all_rows) - z.first_row, 0);
+		z.keys		= max(0, min(b.lengths[seq], held) - prefix_keys);
+	}
+	return z;
+}
+
+struct piece_place {
+	int seq, first_row, rows, pos0; // pos0: position of the sequence's first row
+	int row_group, index; // this piece is piece `index` of that row group
+	int stride; // pieces of the sequence's row groups lie so far apart
+	int length; // keys of a piece
+	bool there;
+};
+// Piece `t` of the batch.  Every wave adds the work up by itself, 64 sequences at a time; `units` pieces' worth of it makes the length of a piece.
+__device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int all_rows, int group, int prefix_keys, int held, int units, int t) {
+	const int lane = threadIdx.x & 63;
+	int64_t total  = 0; // steps
+	sequence_size z;
+	for (int base = 0; base < b.sequences; base += 64) {
+		z				 = size_of(b, all_rows, prefix_keys, held, base + lane);
+		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS;
+		// (a sequence's steps are below 2^25; 64 of them times their row groups in halves of 16 bits, each added up in 32)
+		const int64_t work = static_cast<int64_t>(groups) * ((z.keys + STEP - 1) / STEP);
+		total += __builtin_amdgcn_readlane(scan64(static_cast<int>(work & 0xFFFF)), 63);
+		total += static_cast<int64_t>(__builtin_amdgcn_readlane(scan64(static_cast<int>((work >> 16) & 0xFFFFFF)), 63)) << 16;
+		total += static_cast<int64_t>(__builtin_amdgcn_readlane(scan64(static_cast<int>(work >> 40)), 63)) << 40;
+	}
+	const int64_t steps = (total + units - 1) / units;
+	const int length	= static_cast<int>(min(max(steps, int64_t{ 1 }) + WAVES - 1, int64_t{ 1 } << 25)) / WAVES * WAVES * STEP; // (2^30 keys are all that a table holds)
+	piece_place p{};
+	int before = 0;
+	for (int base = 0; base < b.sequences; base += 64) {
+		if (b.sequences > 64) {
+			z = size_of(b, all_rows, prefix_keys, held, base + lane);
+		}
+		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS;
+		const int each	 = max(1, (z.keys + length - 1) / length);
+		const int count = groups * each, upto = scan64(count);
+		const uint64_t over = __builtin_amdgcn_ballot_w64(before + upto > t);
+		if (over) {
+			const int src = __builtin_ctzll(over);
+			p.seq		  = base + src;
+			p.first_row	  = __builtin_amdgcn_readlane(z.first_row, src);
+			p.rows		  = __builtin_amdgcn_readlane(z.rows, src);
+			p.pos0		  = max(b.lengths[p.seq], 0) - (__builtin_amdgcn_readlane(z.end, src) - p.first_row);
+			p.stride	  = __builtin_amdgcn_readlane(groups, src);
+			const int k	  = t - before - (__builtin_amdgcn_readlane(upto, src) - __builtin_amdgcn_readlane(count, src));
+			p.row_group	  = k % p.stride; // row groups side by side: they read the same keys
+			p.index		  = k / p.stride;
+			p.length	  = length;
+			p.there		  = true;
+			return p;
+		}
+		before += __builtin_amdgcn_readlane(upto, 63);
+	}
+	return p;
+}
+
+// Results between workgroups: device-scope stores and loads, past the caches that another XCD does not see.
+__device__ __forceinline__ void put4(float* p, v4f v) {
+	__hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, float2{ v[0], v[1] }), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+	__hip_atomic_store(reinterpret_cast<uint64_t*>(p) + 1, __builtin_bit_cast(uint64_t, float2{ v[2], v[3] }), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float2* p) {
+	return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// a running result and another one, both sums of weights and of weighted values below their own maximum
+struct running {
+	float m, l;
+	v4f o;
+	__device__ __forceinline__ void add(float m2, float l2, v4f o2) {
+		const float both = fmaxf(m, m2), at = both == -__builtin_inff() ? 0.0f : both;
+		const float f1 = exp2_fast(m - at), f2 = exp2_fast(m2 - at);
+		l = l * f1 + l2 * f2;
+		o = o * f1 + o2 * f2;
+		m = both;
+	}
+};
+
+} // namespace
+
+template<int CACHE, int TYPE, int D>
+__global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_args a, rows_workspace w, int units) {
+	using H				= half_type<CACHE>;
+	using vec			= typename H::vec;
+	constexpr int N		= terms<CACHE, TYPE>;
+	constexpr int STEPS = D / 32; // of q.k
+	constexpr int DT	= D / 16; // tiles of O^T
+	__shared__ v4f join_o[WAVES][DT][64];
+	__shared__ float2 join_ml[WAVES][COLUMNS];
+	__shared__ int is_last;
+
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int col = lane & 15, quarter = lane >> 4;
+	const int group		  = a.q_heads / a.cache.kv_heads;
+	const int head		  = blockIdx.x % a.cache.kv_heads;
+	const int prefix_keys = a.prefix_count << a.cache.page_shift, held = a.batch.width << a.cache.page_shift;
+	const int piece		  = blockIdx.x / a.cache.kv_heads;
+	const piece_place p	  = place_of_piece(a.batch, a.rows, group, prefix_keys, held, units, piece);
+	if (!p.there) {
+		return;
+	}
+	// the row group's rows: first .. first + count - 1 of the sequence's rows * group
+	const int first = p.row_group * COLUMNS, count = min(COLUMNS, p.rows * group - first);
+	const bool there = col < count;
+	const int token	 = (first + min(col, count - 1)) / group;
+	const int q_head = head * group + first + min(col, count - 1) - token * group;
+	// keys: the sequence's own ones that the lane's row sees end at `seen`, those that some row of the group sees at end, that all see at all_seen
+	const int seen	   = min(held, p.pos0 + token + 1);
+	const int all_seen = min(held, p.pos0 + first / group + 1), most_seen = min(held, p.pos0 + (first + count - 1) / group + 1);
+	const int pieces   = max(1, (max(0, most_seen - prefix_keys) + p.length - 1) / p.length); // of this row group
+	if (p.index >= pieces) {
+		return; // (rows in front of the sequence's last see less)
+	}
+	const int first_key = prefix_keys + p.index * p.length;
+	const int end_key	= min(first_key + p.length, most_seen);
+
+	// q as the B operand: column = row, values 32 s + 8 quarter .. + 7
+	vec q[N][STEPS];
+	float c;
+	{
+		const int64_t at = (static_cast<int64_t>(p.first_row) + token) * a.q_stride + static_cast<int64_t>(q_head) * D + 8 * quarter;
+		float x[STEPS][8];
+		float largest = 0.0f;
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			load_q8<TYPE>(a.q, at + 32 * s, there, x[s]);
+		}
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+			for (int j = 0; j < 8; ++j) {
+				largest = fmaxf(largest, fabsf(x[s][j]));
+			}
+		}
+		largest		= fmaxf(largest, swap16(largest));
+		largest		= fmaxf(largest, swap32(largest));
+		const int e = q_exponent<CACHE, TYPE>(largest);
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
+#pragma unroll
+				for (int j = 0; j < 8; ++j) {
+					x[s][j] = ldexpf(x[s][j], 14 - e);
+				}
+			}
+			vec t[N];
+			split8<CACHE, N>(x[s], t);
+#pragma unroll
+			for (int n = 0; n < N; ++n) {
+				q[n][s] = t[n];
+			}
+		}
+		c = ldexpf(a.scale * LOG2_E, e - 14);
+	}
+
+	const int32_t* table = a.batch.table + static_cast<int64_t>(p.seq) * a.batch.width;
+	const int page_size	 = 1 << a.cache.page_shift;
+	// A step's keys base .. base + 31 lie in the pages of its two halves of 16.
+	struct step_data {
+		vec k[2][STEPS], v[DT];
+		int base, page_lo, page_hi;
+	};
+	auto load_pages = [&](int base, step_data& d) {
+		d.base			 = base;
+		const int slot_0 = base >> a.cache.page_shift, slot_1 = (base + 16) >> a.cache.page_shift;
+		d.page_lo		 = base < end_key ? table[slot_0] : -1;
+		d.page_hi		 = base + 16 < end_key ? table[slot_1] : -1;
+	};
+	auto page_there = [&](int id) {
+		return id >= 0 && id < a.cache.pages;
+	};
+	auto load_step = [&](step_data& d) {
+		const int lo = page_there(d.page_lo) ? d.page_lo : 0, hi = page_there(d.page_hi) ? d.page_hi : 0;
+		const int64_t k_page = (col & 8 ? hi : lo) * a.cache.page_values, v_page = (quarter & 2 ? hi : lo) * a.cache.page_values;
+#pragma unroll
+		for (int t = 0; t < 2; ++t) {
+			const int key	   = (d.base + 8 * (col >> 2) + 4 * t + (col & 3)) & (page_size - 1);
+			const uint16_t* at = a.cache.k + k_page + (static_cast<int64_t>(head) * page_size + key) * D + 8 * quarter;
+#pragma unroll
+			for (int s = 0; s < STEPS; ++s) {
+				d.k[t][s] = *reinterpret_cast<const vec*>(at + 32 * s);
+			}
+		}
+		const uint16_t* at = a.cache.v + v_page + (static_cast<int64_t>(head) * D + col) * page_size + ((d.base + 8 * quarter) & (page_size - 1));
+#pragma unroll
+		for (int dt = 0; dt < DT; ++dt) {
+			d.v[dt] = *reinterpret_cast<const vec*>(at + static_cast<int64_t>(dt) * 16 * page_size);
+		}
+	};
+
+	v4f o[DT];
+#pragma unroll
+	for (int t = 0; t < DT; ++t) {
+		o[t] = v4f{};
+	}
+	float m = -__builtin_inff(), l = 0.0f;
+	auto compute = [&](step_data& d) {
+		v4f s[2];
+#pragma unroll
+		for (int t = 0; t < 2; ++t) {
+			s[t] = v4f{};
+#pragma unroll
+			for (int st = 0; st < STEPS; ++st) {
+#pragma unroll
+				for (int n = N - 1; n >= 0; --n) { // the small terms first
+					s[t] = H::mfma16(d.k[t][st], q[n][st], s[t]);
+				}
+			}
+		}
+		const bool lo = page_there(d.page_lo), hi = page_there(d.page_hi);
+		if (d.base + STEP > min(all_seen, end_key) || !lo || !hi) {
+			const int from	= d.base + 8 * quarter; // the lane's keys are from .. from + 7, of its scores and of its values
+			const bool page = quarter & 2 ? hi : lo;
+			const int n = page ? min(seen, end_key) - from : 0, n_all = page ? end_key - from : 0; // so many of them are its row's, some row's
+#pragma unroll
+			for (int t = 0; t < 2; ++t) {
+#pragma unroll
+				for (int i = 0; i < 4; ++i) {
+					s[t][i] = 4 * t + i < n ? s[t][i] : -__builtin_inff();
+				}
+			}
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) { // no values of the others either, whatever lies there (a weight of zero times infinity is not zero)
+				v4u v = __builtin_bit_cast(v4u, d.v[dt]);
+#pragma unroll
+				for (int x = 0; x < 4; ++x) {
+					v[x] = n_all >= 2 * x + 2 ? v[x] : n_all == 2 * x + 1 ? v[x] & 0xFFFFu : 0u;
+				}
+				d.v[dt] = __builtin_bit_cast(vec, v);
+			}
+		}
+		float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+		top		  = fmaxf(top, swap16(top));
+		top		  = fmaxf(top, swap32(top)) * c;
+		const float m_new = fmaxf(m, top);
+		const float base  = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
+		if (__builtin_amdgcn_ballot_w64(m_new != m)) {
+			const float f = exp2_fast(m - base);
+			l *= f;
+#pragma unroll
+			for (int t = 0; t < DT; ++t) {
+				o[t] *= f;
+			}
+			m = m_new;
+		}
+		const float shift = weight_bias<CACHE> - base;
+		float x[8];
+#pragma unroll
+		for (int j = 0; j < 8; ++j) {
+			x[j] = exp2_fast(fmaf(s[j >> 2][j & 3], c, shift));
+			l += x[j];
+		}
+		vec t[N];
+		split8<CACHE, N>(x, t);
+#pragma unroll
+		for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+			for (int n = N - 1; n >= 0; --n) {
+				o[dt] = H::mfma16(d.v[dt], t[n], o[dt]);
+			}
+		}
+	};
+
+	// two steps in turn: one's loads in flight under the other's arithmetic, the page numbers a step ahead of the loads
+	step_data d0, d1;
+	constexpr int stride = STEP * WAVES;
+	int base			 = first_key + wave * STEP;
+	load_pages(base, d0);
+	load_pages(base + stride, d1);
+	if (base < end_key) {
+		load_step(d0);
+	}
+	while (base < end_key) {
+		if (base + stride < end_key) {
+			load_step(d1);
+		}
+		compute(d0);
+		load_pages(base + 2 * stride, d0);
+		base += stride;
+		if (base >= end_key) {
+			break;
+		}
+		if (base + stride < end_key) {
+			load_step(d0);
+		}
+		compute(d1);
+		load_pages(base + 2 * stride, d1);
+		base += stride;
+	}
+
+	// the four waves' results into one: a thread takes four values of a row at a time
+	l += swap16(l);
+	l += swap32(l);
+#pragma unroll
+	for (int dt = 0; dt < DT; ++dt) {
+		join_o[wave][dt][lane] = o[dt];
+	}
+	if (quarter == 0) {
+		join_ml[wave][col] = make_float2(m, l);
+	}
+	__syncthreads();
+	const bool alone	= pieces == 1 && w.prefix_pieces == 0;
+	const int64_t slot	= static_cast<int64_t>(piece) * a.cache.kv_heads + head;
+	if (there) {
+		float2 ml[WAVES];
+#pragma unroll
+		for (int x = 0; x < WAVES; ++x) {
+			ml[x] = join_ml[x][col];
+		}
+		const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), at = top == -__builtin_inff() ? 0.0f : top;
+		float f[WAVES], sum = 0.0f;
+#pragma unroll
+		for (int x = 0; x < WAVES; ++x) {
+			f[x] = exp2_fast(ml[x].x - at);
+			sum += ml[x].y * f[x];
+		}
+		const float inv		  = alone ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f; // no key at all: zeros
+		const int64_t out_row = ((static_cast<int64_t>(p.first_row) + token) * a.q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D;
+#pragma unroll
+		for (int dt = wave; dt < DT; dt += WAVES) {
+			v4f v{};
+#pragma unroll
+			for (int x = 0; x < WAVES; ++x) {
+				v += join_o[x][dt][lane] * f[x];
+			}
+			if (alone) {
+				store_out4<TYPE>(a.out, out_row + 16 * dt + 4 * quarter, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+			} else {
+				put4(w.o + slot_row + 16 * dt + 4 * quarter, v);
+			}
+		}
+		if (!alone && wave == 0 && quarter == 0) {
+			__hip_atomic_store(reinterpret_cast<uint64_t*>(w.ml + slot * w.columns + col), __builtin_bit_cast(uint64_t, make_float2(top, sum)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+		}
+	}
+	if (alone) {
+		return;
+	}
+	const int64_t first_slot = slot - static_cast<int64_t>(p.index) * p.stride * a.cache.kv_heads;
+	if (pieces > 1) {
+		wait_stores_acknowledged();
+		__syncthreads();
+		if (tid == 0) {
+			const int done = __hip_atomic_fetch_add(w.counters + first_slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+			is_last		   = done == pieces - 1;
+			if (is_last) {
+				__hip_atomic_store(w.counters + first_slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+			}
+		}
+		__syncthreads();
+		if (!is_last) {
+			return;
+		}
+	} else {
+		wait_stores_acknowledged();
+		__syncthreads();
+	}
+	// Joins the row group's pieces, those over the shared prefix first: D / 4 threads to a row, the pieces of few rows over what threads are left.
+	constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
+	running* parts		= reinterpret_cast<running*>(&join_o[0][0][0]); // [GROUPS][LANES], 24 (32 aligned) bytes each
+	static_assert(sizeof(running) * THREADS <= sizeof(join_o), "the parts of the join fit where the waves' results were");
+	const int x = tid % LANES, g = tid / LANES;
+	const int rows_at_once = count <= 1 ? 1 : count <= 2 ? 2 : count <= 4 ? 4 : 8; // a divisor of GROUPS
+	const int ways = GROUPS / rows_at_once, way = g / rows_at_once;
+	const int all = w.prefix_pieces + pieces;
+	for (int r0 = 0; r0 < count; r0 += rows_at_once) {
+		const int r		  = r0 + g % rows_at_once;
+		const bool mine	  = r < count;
+		const int tok	  = (first + min(r, count - 1)) / group;
+		const int q_h	  = head * group + first + min(r, count - 1) - tok * group;
+		running sum{ -__builtin_inff(), 0.0f, v4f{} };
+		if (mine) {
+#pragma unroll 4
+			for (int i = way; i < all; i += ways) {
+				const bool shared = i < w.prefix_pieces;
+				const int64_t at  = shared ? (static_cast<int64_t>(i) * a.batch.sequences + p.seq) * a.q_heads + q_h
+										   : (first_slot + static_cast<int64_t>(i - w.prefix_pieces) * p.stride * a.cache.kv_heads) * w.columns + r;
+				const float2 ml	  = get2((shared ? w.prefix_ml : w.ml) + at);
+				const float2* v	  = reinterpret_cast<const float2*>((shared ? w.prefix_o : w.o) + at * D + 4 * x);
+				const float2 lo = get2(v), hi = get2(v + 1);
+				sum.add(ml.x, ml.y, v4f{ lo.x, lo.y, hi.x, hi.y });
+			}
+		}
+		__syncthreads(); // (the last rows' parts have been read)
+		parts[tid] = sum;
+		__syncthreads();
+		if (mine && way == 0) {
+			for (int i = 1; i < min(ways, all); ++i) {
+				const running& other = parts[tid + i * rows_at_once * LANES];
+				sum.add(other.m, other.l, other.o);
+			}
+			const float inv = sum.l > 0.0f || sum.l != sum.l ? 1.0f / sum.l : 0.0f;
+			store_out4<TYPE>(a.out, ((static_cast<int64_t>(p.first_row) + tok) * a.q_heads + q_h) * D + 4 * x, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
+		}
+	}
+}
+
+rows_needs attention_rows_needs(int64_t rows, int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
+	rows_workspace w;
+	const rows_cut cut = plan_rows(rows, sequences, one_each, q_heads / kv_heads, kv_heads);
+	return rows_needs{ lay_out(nullptr, cut, plan_prefix(sequences, q_heads / kv_heads, kv_heads, prefix_keys), sequences, q_heads, kv_heads, head_dim, &w), cut.pieces * kv_heads * 4 };
+}
+
+template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
+	const int64_t group = a.q_heads / a.cache.kv_heads, sequences = a.batch.sequences;
+	const rows_cut cut		= plan_rows(a.rows, sequences, a.batch.starts == nullptr, group, a.cache.kv_heads);
+	const prefix_cut prefix = plan_prefix(sequences, group, a.cache.kv_heads, static_cast<int64_t>(a.prefix_count) << a.cache.page_shift);
+	rows_workspace w;
+	(void)lay_out(static_cast<char*>(a.workspace), cut, prefix, sequences, a.q_heads, a.cache.kv_heads, D, &w);
+	w.counters = a.counters;
+	if (prefix.pieces > 0) {
+		const hipError_t e = launch_attention_prefix(a, CACHE, TYPE, prefix, w.prefix_o, w.prefix_ml, s);
+		if (e != hipSuccess) {
+			return e;
+		}
+	}
+	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(cut.pieces * a.cache.kv_heads)), dim3(THREADS), 0, s>>>(a, w, static_cast<int>(cut.units));
+	return hipGetLastError();
+}
+template<int CACHE, int TYPE> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
+	return a.head_dim == 64 ? launch_rows<CACHE, TYPE, 64>(a, s) : launch_rows<CACHE, TYPE, 128>(a, s);
+}
+
+hipError_t launch_attention_rows(const attention_args& a, int cache_type, int type, hipStream_t s) {
+	if (cache_type == NH_F16) {
+		return type == NH_F32 ? launch_rows<NH_F16, NH_F32>(a, s) : launch_rows<NH_F16, NH_F16>(a, s);
+	}
+	return type == NH_F32 ? launch_rows<NH_BF16, NH_F32>(a, s) : launch_rows<NH_BF16, NH_BF16>(a, s);
+}
+
+} // namespace nh

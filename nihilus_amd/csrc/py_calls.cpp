@@ -11,11 +11,15 @@
 // also makes the error messages.  Nothing is enqueued before None is returned.
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "nihilus_amd/attention_abi.h"
+
+#include <map>
+#include <utility>
 
 namespace {
 
@@ -266,6 +270,23 @@ at::Tensor ints_like(const at::Tensor& t, at::IntArrayRef sizes) {
 	return at::empty(sizes, t.options());
 }
 
+// Counters of zeros for a call on stream s of t's device.  Every call leaves them zero, so the calls of a stream, which run one after the other,
+// share theirs; a stream that is being captured gets new ones, whose clearing is captured with the call.
+at::Tensor counters_for(const at::Tensor& t, void* s, int64_t bytes) {
+	static auto* kept = new std::map<std::pair<int, void*>, at::Tensor>; // (never destroyed: the interpreter's end is too late to free device memory)
+	hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+	const bool plain = hipStreamIsCapturing(static_cast<hipStream_t>(s), &capturing) == hipSuccess && capturing == hipStreamCaptureStatusNone;
+	const auto zeros = [&](int64_t n) { return at::zeros({ n }, t.options().dtype(at::kInt)); };
+	if (!plain) {
+		return zeros(bytes / 4);
+	}
+	at::Tensor& mine = (*kept)[{ t.device().index(), s }];
+	if (!mine.defined() || mine.numel() * 4 < bytes) {
+		mine = zeros(std::max<int64_t>(bytes / 4, 16384));
+	}
+	return mine;
+}
+
 // append_rope(q, k, v, k_pages, v_pages, page_table, lengths, turns, starts or None, interleaved)
 PyObject* append_rope(args& in) {
 	const at::Tensor *q = rows_tensor(in), *k = rows_tensor(in), *v = rows_tensor(in), *kp = rows_tensor(in), *vp = rows_tensor(in);
@@ -302,12 +323,22 @@ PyObject* attention_prompt(args& in) {
 	if (!p.good || !p.starts(starts) || !p.rows(q, 0, &qs)) {
 		return nullptr;
 	}
-	const at::Tensor out = like(*q);
-	const void* qp		 = q->const_data_ptr();
-	void *op = out.mutable_data_ptr(), *s = stream();
-	const int type	   = type_of(*q);
 	const int64_t rows = q->size(0), heads = q->size(1);
-	return finish(out, [&] { return nh_attn_prompt(&p.cache, &p.batch, qp, op, type, rows, heads, qs, scale, s); });
+	int64_t need, counter_need;
+	if (nh_attn_prompt_needs(rows, p.batch.sequences, heads, p.cache.kv_heads, p.cache.head_dim, &need, &counter_need) != 0) {
+		return nullptr;
+	}
+	const at::Tensor out = like(*q);
+	at::Tensor workspace, counters;
+	void *s = stream(), *ws = nullptr, *cs = nullptr;
+	if (need > 0) {
+		workspace = bytes_like(*q, need), counters = counters_for(*q, s, counter_need);
+		ws = workspace.mutable_data_ptr(), cs = counters.mutable_data_ptr();
+	}
+	const void* qp = q->const_data_ptr();
+	void* op	   = out.mutable_data_ptr();
+	const int type = type_of(*q);
+	return finish(out, [&] { return nh_attn_prompt(&p.cache, &p.batch, qp, op, type, rows, heads, qs, scale, ws, need, cs, counter_need, s); });
 }
 
 // attention_decode(q, k_pages, v_pages, page_table, lengths, prefix_pages or None, scale)
@@ -324,16 +355,17 @@ PyObject* attention_decode(args& in) {
 		return nullptr;
 	}
 	const int64_t heads = q->size(1), count = prefix ? prefix->size(0) : 0;
-	const int64_t need = nh_attn_decode_workspace_bytes(p.batch.sequences, heads, p.cache.kv_heads, p.cache.head_dim, count, p.cache.page_size);
-	if (need < 0) {
+	int64_t need, counter_need;
+	if (nh_attn_decode_needs(p.batch.sequences, heads, p.cache.kv_heads, p.cache.head_dim, count, p.cache.page_size, &need, &counter_need) != 0) {
 		return nullptr;
 	}
-	const at::Tensor out = like(*q), workspace = bytes_like(*q, need);
+	void* s				 = stream();
+	const at::Tensor out = like(*q), workspace = bytes_like(*q, need), counters = counters_for(*q, s, counter_need);
 	const void* qp	  = q->const_data_ptr();
 	const int32_t* pp = count > 0 ? static_cast<const int32_t*>(prefix->const_data_ptr()) : nullptr;
-	void *op = out.mutable_data_ptr(), *ws = workspace.mutable_data_ptr(), *s = stream();
+	void *op = out.mutable_data_ptr(), *ws = workspace.mutable_data_ptr(), *cs = counters.mutable_data_ptr();
 	const int type = type_of(*q);
-	return finish(out, [&] { return nh_attn_decode(&p.cache, &p.batch, pp, count, qp, op, type, heads, qs, scale, ws, need, s); });
+	return finish(out, [&] { return nh_attn_decode(&p.cache, &p.batch, pp, count, qp, op, type, heads, qs, scale, ws, need, cs, counter_need, s); });
 }
 
 // cache_step(k_pages, v_pages, page_table, lengths, parents, grow): (page_table, lengths, info)

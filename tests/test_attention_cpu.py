@@ -48,16 +48,19 @@ def _append(cache=None, batch=None, q=BOGUS, k=BOGUS, v=BOGUS, out=BOGUS, type=0
     return _lib.lib().nh_attn_append_rope(C.byref(cache or _cache()), C.byref(batch or _batch()), q, k, v, out, type, rows, heads, *strides, turns, pairs, 1, None)
 
 
-def _prompt(cache=None, batch=None, q=BOGUS, out=BOGUS, type=0, rows=3, heads=4, stride=256, scale=0.125):
+MEMORY = dict(ws=BOGUS, bytes=1 << 30, counters=BOGUS, counter_bytes=1 << 30)
+
+
+def _prompt(cache=None, batch=None, q=BOGUS, out=BOGUS, type=0, rows=3, heads=4, stride=256, scale=0.125, **memory):
     from nihilus_amd import _lib
 
-    return _lib.lib().nh_attn_prompt(C.byref(cache or _cache()), C.byref(batch or _batch(starts=BOGUS)), q, out, type, rows, heads, stride, scale, None)
+    return _lib.lib().nh_attn_prompt(C.byref(cache or _cache()), C.byref(batch or _batch(starts=BOGUS)), q, out, type, rows, heads, stride, scale, *{**MEMORY, **memory}.values(), None)
 
 
-def _decode(cache=None, batch=None, prefix=None, count=0, q=BOGUS, out=BOGUS, type=0, heads=4, stride=256, scale=0.125, ws=BOGUS, bytes=1 << 30):
+def _decode(cache=None, batch=None, prefix=None, count=0, q=BOGUS, out=BOGUS, type=0, heads=4, stride=256, scale=0.125, **memory):
     from nihilus_amd import _lib
 
-    return _lib.lib().nh_attn_decode(C.byref(cache or _cache()), C.byref(batch or _batch()), prefix, count, q, out, type, heads, stride, scale, ws, bytes, None)
+    return _lib.lib().nh_attn_decode(C.byref(cache or _cache()), C.byref(batch or _batch()), prefix, count, q, out, type, heads, stride, scale, *{**MEMORY, **memory}.values(), None)
 
 
 def _step(cache=None, batch=None, parents=BOGUS, grow=BOGUS, children=3, table=BOGUS * 2, lengths=BOGUS * 3, info=BOGUS * 4, ws=BOGUS, bytes=1 << 30):
@@ -113,9 +116,11 @@ def test_attention_refusals():
     assert _prompt(rows=-1) == -3 and _prompt(rows=1 << 29) == -5
     assert _prompt(rows=0, q=None, out=None) == 0 and _prompt(batch=_batch(starts=BOGUS, sequences=0), q=None, out=None) == 0
     assert _decode(batch=_batch(starts=BOGUS)) == -6
-    assert _decode(ws=None) == -1 and _decode(ws=BOGUS + 16) == -2 and _decode(bytes=100) == -6
+    for call in (_prompt, _decode):
+        assert call(ws=None) == -1 and call(ws=BOGUS + 16) == -2 and call(bytes=100) == -6
+        assert call(counters=None) == -1 and call(counters=BOGUS + 64) == -2 and call(counter_bytes=8) == -6
     assert _decode(count=1) == -1 and _decode(count=-1) == -3 and _decode(count=1 << 40) == -5
-    assert _decode(batch=_batch(sequences=0), q=None, out=None, ws=None) == 0
+    assert _decode(batch=_batch(sequences=0), q=None, out=None, ws=None, counters=None) == 0
 
 
 def test_pages_refusals():
@@ -132,13 +137,36 @@ def test_workspace_sizes():
     from nihilus_amd import _lib
 
     lib = _lib.lib()
-    f = lib.nh_attn_decode_workspace_bytes
-    assert f(0, 32, 8, 128, 0, 64) > 0 and f(64, 32, 8, 128, 0, 64) >= 64 * 32 * 128 * 4
-    assert f(64, 32, 8, 128, 128, 64) > f(64, 32, 8, 128, 0, 64)
-    assert f(4, 33, 8, 128, 0, 64) == -3 and f(4, 32, 0, 128, 0, 64) == -3 and f(4, 32, 8, 80, 0, 64) == -3 and f(4, 32, 8, 128, 0, 24) == -3 and f(-1, 32, 8, 128, 0, 64) == -3
-    assert f(1 << 21, 32, 8, 128, 0, 64) == -5
+    n, c = C.c_int64(), C.c_int64()
+
+    def decode(*sizes):
+        status = lib.nh_attn_decode_needs(*sizes, C.byref(n), C.byref(c))
+        return status or n.value
+
+    def prompt(*sizes):
+        status = lib.nh_attn_prompt_needs(*sizes, C.byref(n), C.byref(c))
+        return status or n.value
+
+    assert decode(64, 32, 8, 128, 0, 64) >= 64 * 32 * 128 * 4 and c.value >= 64 * 8 * 4
+    assert decode(64, 32, 8, 128, 128, 64) > decode(64, 32, 8, 128, 0, 64)
+    assert decode(4, 33, 8, 128, 0, 64) == -3 and decode(4, 32, 0, 128, 0, 64) == -3 and decode(4, 32, 8, 80, 0, 64) == -3 and decode(4, 32, 8, 128, 0, 24) == -3 and decode(-1, 32, 8, 128, 0, 64) == -3
+    assert decode(1 << 21, 32, 8, 128, 0, 64) == -5 and decode(4, 32, 8, 128, -1, 64) == -3
+    assert prompt(20, 2, 32, 8, 128) > 0 and c.value > 0 and prompt(8192, 1, 64, 8, 128) == 0 and c.value == 0  # many rows: the tile kernel, which needs nothing
+    assert prompt(-1, 2, 32, 8, 128) == -3 and prompt(20, 2, 32, 8, 96) == -3 and prompt(1 << 29, 2, 32, 8, 128) == -5
+    assert lib.nh_attn_prompt_needs(20, 2, 32, 8, 128, None, C.byref(c)) == -1 and lib.nh_attn_decode_needs(4, 32, 8, 128, 0, 64, C.byref(n), None) == -1
     g = lib.nh_attn_pages_workspace_bytes
     assert g(1, 0, 0) > 0 and g(1000, 64, 10) >= 1000 * 8 and g(0, 1, 1) == -3 and g(1, -1, 1) == -3 and g(1 << 40, 1, 1) == -5
+
+
+def test_which_kernel_a_prompt_takes(monkeypatch):
+    from nihilus_amd import _lib
+
+    f = _lib.lib().nh_attn_debug_prompt_kernel
+    assert f(117, 1, 32, 8, -1) == 1 and f(8192, 1, 64, 8, -1) == 2
+    monkeypatch.delenv("NH_Q8_0_DEBUG_HOOKS", raising=False)
+    assert f(117, 1, 32, 8, 2) == -6
+    monkeypatch.setenv("NH_Q8_0_DEBUG_HOOKS", "1")
+    assert f(117, 1, 32, 8, 2) == 2 and f(117, 1, 32, 8, -1) == 2 and f(117, 1, 32, 8, 3) == -6 and f(117, 1, 32, 8, 0) == 1
 
 
 def test_without_a_gpu_calls_fail_loudly():

@@ -24,6 +24,16 @@ def A():
     return attention
 
 
+@pytest.fixture(params=[1, 2], ids=["rows", "tiles"])
+def kernel(A, request, monkeypatch):
+    """Each of the two kernels that a prompt may take, whatever its size."""
+    monkeypatch.setenv("NH_Q8_0_DEBUG_HOOKS", "1")
+    force = A._lib.lib().nh_attn_debug_prompt_kernel
+    assert force(1, 1, 1, 1, request.param) == request.param
+    yield request.param
+    assert force(1, 1, 1, 1, 0) in (1, 2)
+
+
 class Batch:
     """A cache with sequences in scattered pages; what lies outside the sequences is NaN."""
 
@@ -89,7 +99,7 @@ def _starts(new):
 @pytest.mark.parametrize("dtype,cache", KINDS)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("page", [16, 64])
-def test_prompt_ragged(A, dtype, cache, dim, page):
+def test_prompt_ragged(A, kernel, dtype, cache, dim, page):
     new, cached = [1, 0, 33, 64, 5, 130, 0, 1], [0, 70, 0, 1, 200, 31, 0, 64]
     b = Batch(1, [a + c for a, c in zip(new, cached)], page, 2, dim, cache)
     starts = _starts(new)
@@ -102,7 +112,7 @@ def test_prompt_ragged(A, dtype, cache, dim, page):
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 3), (6, 2), (7, 1), (40, 2), (5, 5), (129, 1)])
-def test_prompt_groupings_and_pages(A, heads, kv_heads, page):
+def test_prompt_groupings_and_pages(A, kernel, heads, kv_heads, page):
     new, cached = [67, 3], [0, 300]
     b = Batch(heads + page, [a + c for a, c in zip(new, cached)], page, kv_heads, 64, F16)
     q = b.rows(sum(new), heads, F32)
@@ -112,7 +122,7 @@ def test_prompt_groupings_and_pages(A, heads, kv_heads, page):
 
 
 @pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 257])
-def test_prompt_lengths(A, n):
+def test_prompt_lengths(A, kernel, n):
     b = Batch(n, [n], 32, 1, 128, F16)
     q = b.rows(n, 4, F16)
     k, v, table, lengths = b.device()
@@ -120,7 +130,7 @@ def test_prompt_lengths(A, n):
     _check_prompt(b, out, q, [0, n], [n], F16, 128**-0.5)
 
 
-def test_prompt_of_many_sequences(A):
+def test_prompt_of_many_sequences(A, kernel):
     rng = random.Random(5)  # more than the 64 that a wave adds up at a time, empty ones among them
     new = [rng.choice([0, 0, 1, 2, 40]) for _ in range(150)]
     b = Batch(5, [n + rng.choice([0, 17]) for n in new], 16, 1, 64, F16)
@@ -130,7 +140,7 @@ def test_prompt_of_many_sequences(A):
     _check_prompt(b, out, q, _starts(new), new, F32, 0.125)
 
 
-def test_rows_of_nobody_stay_as_they_are(A):
+def test_rows_of_nobody_stay_as_they_are(A, kernel):
     new = [3, 0, 4]
     b = Batch(7, [20, 5, 4], 16, 2, 64, F16)
     k, v, table, lengths = b.device()
@@ -157,7 +167,7 @@ def test_rows_of_nobody_stay_as_they_are(A):
 
 
 @pytest.mark.parametrize("call", ["prompt", "decode"])
-def test_pages_that_the_cache_does_not_have(A, call):
+def test_pages_that_the_cache_does_not_have(A, kernel, call):
     lengths = [100, 40, 16, 90]
     b = Batch(9, lengths, 16, 2, 64, F16, extra_width=0)
     total = len(b.k)
@@ -181,7 +191,7 @@ def test_pages_that_the_cache_does_not_have(A, call):
 
 
 @pytest.mark.parametrize("length", [0, -5])
-def test_sequences_without_keys_give_zeros(A, length):
+def test_sequences_without_keys_give_zeros(A, kernel, length):
     b = Batch(11, [10, 0, 40], 16, 1, 64, F16)
     b.lengths[1] = length
     k, v, table, lengths = b.device()
@@ -283,7 +293,7 @@ def test_prefix_of_many_rows_in_pieces(A):
 
 
 @pytest.mark.parametrize("std", [1e-30, 1e-6, 300.0, 1e6])
-def test_sizes_of_q(A, std):
+def test_sizes_of_q(A, kernel, std):
     # fp32 q goes through fp16 terms: neither what fp16 cannot hold nor its small numbers may show
     b = Batch(31, [150], 16, 1, 64, F16)
     q = b.rows(150, 4, F32, std=std)
@@ -296,7 +306,7 @@ def test_sizes_of_q(A, std):
 
 
 @pytest.mark.parametrize("cache", [F16, BF16])
-def test_peaked_and_flat_scores(A, cache):
+def test_peaked_and_flat_scores(A, kernel, cache):
     b = Batch(37, [400], 32, 1, 64, cache)
     k, v, table, dl = b.device()
     for std, dtype in ((60.0, F32), (0.0, F32), (60.0, cache)):
@@ -307,7 +317,7 @@ def test_peaked_and_flat_scores(A, cache):
         _check(out[0], *R.attend(q[0], *b.keys(0, 400), 0.125), dtype, std)
 
 
-def test_strided_rows_and_in_place(A):
+def test_strided_rows_and_in_place(A, kernel):
     # q, k and v as parts of one fused projection
     b = Batch(41, [50, 20], 16, 2, 64, F16)
     k, v, table, dl = b.device()
@@ -390,7 +400,7 @@ def test_append_one_row_per_sequence(A):
     assert sorted(torch.nonzero(changed).flatten().tolist()) == sorted(b.table[s][(n - 1) // 16] for s, n in enumerate(lengths) if n)
 
 
-def test_offsets_past_32_bits(A):
+def test_offsets_past_32_bits(A, kernel):
     # pages behind 2^32 bytes and 2^31 values of the cache
     pages, page, heads, dim = 20000, 256, 8, 128  # 2^18 values of K each: 10.5 GB
     k, v = A.empty_cache(1, pages, heads, page, dim)
@@ -414,7 +424,7 @@ def test_offsets_past_32_bits(A):
     assert torch.equal(v[16500, :, :, 697 - 512 : 700 - 512], x.to(F16).permute(1, 2, 0))
 
 
-def test_streams_and_captured_graphs(A):
+def test_streams_and_captured_graphs(A, kernel):
     # replays with new inputs, eager calls between them, a second graph with a workspace of its own on another stream
     lengths = [700, 33, 1, 260]
     b = Batch(53, lengths, 32, 2, 128, F16, shared=0)
@@ -477,6 +487,50 @@ def test_two_streams_at_once(A):
         assert all(torch.equal(x, want[i]) for x in got[i])
 
 
+def test_the_two_prompt_kernels_agree(A, monkeypatch):
+    # a chunk of few rows behind long cached parts: pieces on one side, tiles on the other
+    new, cached = [5, 1, 40, 0], [3000, 0, 700, 50]
+    b = Batch(73, [n + c for n, c in zip(new, cached)], 32, 2, 128, F16)
+    q = b.rows(sum(new), 8, F32).cuda()
+    k, v, table, dl = b.device()
+    starts = torch.tensor(_starts(new), dtype=torch.int32).cuda()
+    monkeypatch.setenv("NH_Q8_0_DEBUG_HOOKS", "1")
+    force = A._lib.lib().nh_attn_debug_prompt_kernel
+    got = []
+    try:
+        for which in (1, 2):
+            force(1, 1, 1, 1, which)
+            got.append(A.attention_prompt(q, k, v, table, dl, starts))
+    finally:
+        force(1, 1, 1, 1, 0)
+    _check_prompt(b, got[0], q.cpu(), _starts(new), new, F32, 128**-0.5)
+    _check_prompt(b, got[1], q.cpu(), _starts(new), new, F32, 128**-0.5)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_counters_are_left_zero(A, graph):
+    b = Batch(79, [3000, 900, 1, 0, 257], 32, 2, 64, F16)
+    k, v, table, dl = b.device()
+    q = b.rows(5, 8, F32).cuda()
+    ws = A.decode_workspace(5, 8, 2, 64)
+    want = A.attention_decode(q, k, v, table, dl)
+    if graph:
+        A.attention_decode(q, k, v, table, dl, workspace=ws)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = A.attention_decode(q, k, v, table, dl, workspace=ws)
+            own = A.attention_decode(q, k, v, table, dl)
+        for _ in range(4):
+            out.zero_(), own.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(own, want) and not bool(ws.counters.any())
+    for _ in range(3):
+        assert torch.equal(A.attention_decode(q, k, v, table, dl, workspace=ws), want)
+    assert not bool(ws.counters.any())
+
+
 def test_same_bits_every_time(A):
     b = Batch(61, [2500, 700, 31], 16, 2, 128, F16)
     k, v, table, dl = b.device()
@@ -488,7 +542,7 @@ def test_same_bits_every_time(A):
     assert torch.equal(first, A.attention_decode(q, k, v, table, dl))
 
 
-def test_prompt_and_decode_agree(A):
+def test_prompt_and_decode_agree(A, kernel):
     # a sequence written token by token and decoded gives what the same sequence in one prompt gives
     n, heads, kv_heads, dim, page = 70, 4, 2, 64, 16
     gen = torch.Generator(device="cuda").manual_seed(3)
@@ -574,7 +628,7 @@ def test_tensors_that_are_refused(A, monkeypatch, native):
     with pytest.raises(errors):
         A.attention_decode(q, k, v, table, dl, prefix_pages=table[0].long())
     with pytest.raises(errors):
-        A.attention_decode(q, k, v, table, dl, workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+        A.attention_decode(q, k, v, table, dl, workspace=A.decode_workspace(1, 2, 2, 64))  # too small
     for out in (q[:1], q.half(), q.cpu(), torch.empty(2, 64, 4, device="cuda").transpose(1, 2)):
         with pytest.raises(errors):
             A.attention_decode(q, k, v, table, dl, out=out)
