@@ -32,6 +32,9 @@ constexpr int COLUMNS	 = 16; // rows of a row group
 // What the pieces are cut for: twice what the chip holds at once (two per CU), so that the last ones to start are short.  decode of 64 sequences of up to 8192 keys
 // (32 / 8 heads): 512 61.5 us, 1024 55.4, 2048 60.0, 4096 68.5.
 constexpr int WORKGROUPS = 1024;
+constexpr int AT_ONCE		= 512; // workgroups that the chip holds at once
+constexpr int SHORT_LENGTHS = 4; // short pieces are of 1, 2, 4 or 8 steps for each wave
+constexpr int64_t MOST_SHORT = (int64_t{ WAVES } << (SHORT_LENGTHS - 1)) * WORKGROUPS; // more steps than that make long pieces
 
 struct rows_workspace {
 	float* o; // [slot][columns][D]  a piece's sums of weighted values; slot = piece * kv_heads + kv head
@@ -89,16 +92,17 @@ __device__ __forceinline__ int scan64(int x) {
 
 // What a lane knows of sequence `seq`: its rows, its keys behind the prefix.
 struct sequence_size {
-	int first_row, rows, end; // packed rows first_row .. first_row + rows - 1; starts[seq + 1]
+	int first_row, rows, pos0; // packed rows first_row .. first_row + rows - 1; position of the first
 	int keys;
 };
 __device__ __forceinline__ sequence_size size_of(const batch_view& b, int all_rows, int prefix_keys, int held, int seq) {
 	sequence_size z{ 0, 0, 0, 0 };
 	if (seq < b.sequences) {
-		z.end		= b.starts ? b.starts[seq + 1] : seq + 1;
-		z.first_row = b.starts ? max(b.starts[seq], 0) : seq;
-		z.rows		= max(min(z.end, all_rows) - z.first_row, 0);
-		z.keys		= max(0, min(b.lengths[seq], held) - prefix_keys);
+		const int end = b.starts ? b.starts[seq + 1] : seq + 1, length = max(b.lengths[seq], 0);
+		z.first_row	  = b.starts ? max(b.starts[seq], 0) : seq;
+		z.rows		  = max(min(end, all_rows) - z.first_row, 0);
+		z.pos0		  = length - (end - z.first_row);
+		z.keys		  = max(0, min(length, held) - prefix_keys);
 	}
 	return z;
 }
@@ -110,23 +114,64 @@ struct piece_place {
 	int length; // keys of a piece
 	bool there;
 };
-// Piece `t` of the batch.  Every wave adds the work up by itself, 64 sequences at a time; `units` pieces' worth of it makes the length of a piece.
-__device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int all_rows, int group, int prefix_keys, int held, int units, int t) {
+__device__ __forceinline__ int sum64(int x) {
+	return __builtin_amdgcn_readlane(scan64(x), 63);
+}
+// How long a piece is, in steps: see place_of_piece.
+__device__ __forceinline__ int piece_steps(int64_t total, const int (&pieces)[SHORT_LENGTHS], int units, int fit) {
+	int64_t steps = (total + units - 1) / units;
+	if (steps <= WAVES << (SHORT_LENGTHS - 1)) {
+#pragma unroll
+		for (int i = 0; i < SHORT_LENGTHS; ++i) {
+			if (steps <= WAVES << i && (i == SHORT_LENGTHS - 1 || pieces[i] <= fit)) {
+				return WAVES << i;
+			}
+		}
+	}
+	return static_cast<int>(min(steps + WAVES - 1, int64_t{ 1 } << 25)) / WAVES * WAVES; // (2^30 keys are all that a table holds)
+}
+// Piece `t` of the batch.  Every wave adds the work up by itself, 64 sequences at a time.  A piece is `units`th of the work long, but not so short
+// that the pieces do not fit on the chip at once (`fit`) when a piece of twice the length is still short: a workgroup takes some 5 us
+// before and behind its steps, a step 0.6.
+__device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int all_rows, int group, int prefix_keys, int held, int units, int fit, int t) {
 	const int lane = threadIdx.x & 63;
+	piece_place p{};
+	if (b.sequences == 1) { // nothing to add up, and nothing to wait for but the one length
+		const sequence_size z = size_of(b, all_rows, prefix_keys, held, 0);
+		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS, steps = (z.keys + STEP - 1) / STEP;
+		int pieces[SHORT_LENGTHS];
+#pragma unroll
+		for (int i = 0; i < SHORT_LENGTHS; ++i) {
+			pieces[i] = groups * max(1, (steps + (WAVES << i) - 1) / (WAVES << i));
+		}
+		p.first_row = z.first_row, p.rows = z.rows, p.pos0 = z.pos0;
+		p.stride	= max(groups, 1);
+		p.row_group = t % p.stride, p.index = t / p.stride;
+		p.length	= piece_steps(static_cast<int64_t>(groups) * steps, pieces, units, fit) * STEP;
+		p.there		= groups > 0;
+		return p;
+	}
 	int64_t total  = 0; // steps
+	int pieces[SHORT_LENGTHS] = {}; // that there are with 1, 2, 4, ... steps for each wave
 	sequence_size z;
 	for (int base = 0; base < b.sequences; base += 64) {
 		z				 = size_of(b, all_rows, prefix_keys, held, base + lane);
-		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS;
-		// (a sequence's steps are below 2^25; 64 of them times their row groups in halves of 16 bits, each added up in 32)
-		const int64_t work = static_cast<int64_t>(groups) * ((z.keys + STEP - 1) / STEP);
-		total += __builtin_amdgcn_readlane(scan64(static_cast<int>(work & 0xFFFF)), 63);
-		total += static_cast<int64_t>(__builtin_amdgcn_readlane(scan64(static_cast<int>((work >> 16) & 0xFFFFFF)), 63)) << 16;
-		total += static_cast<int64_t>(__builtin_amdgcn_readlane(scan64(static_cast<int>(work >> 40)), 63)) << 40;
+		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS, steps = (z.keys + STEP - 1) / STEP;
+		// (a sequence's steps are below 2^25: the sum in halves, each within 32 bits)
+		const int64_t work = static_cast<int64_t>(groups) * steps;
+		total += sum64(static_cast<int>(work & 0xFFFF));
+		if (__builtin_amdgcn_ballot_w64(work > 0xFFFF)) {
+			total += static_cast<int64_t>(sum64(static_cast<int>((work >> 16) & 0xFFFFFF))) << 16;
+			total += static_cast<int64_t>(sum64(static_cast<int>(work >> 40))) << 40;
+		}
+		if (total <= MOST_SHORT) {
+#pragma unroll
+			for (int i = 0; i < SHORT_LENGTHS; ++i) {
+				pieces[i] += sum64(groups * max(1, (steps + (WAVES << i) - 1) / (WAVES << i)));
+			}
+		}
 	}
-	const int64_t steps = (total + units - 1) / units;
-	const int length	= static_cast<int>(min(max(steps, int64_t{ 1 }) + WAVES - 1, int64_t{ 1 } << 25)) / WAVES * WAVES * STEP; // (2^30 keys are all that a table holds)
-	piece_place p{};
+	const int length = piece_steps(total, pieces, units, fit) * STEP;
 	int before = 0;
 	for (int base = 0; base < b.sequences; base += 64) {
 		if (b.sequences > 64) {
@@ -141,7 +186,7 @@ __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int a
 			p.seq		  = base + src;
 			p.first_row	  = __builtin_amdgcn_readlane(z.first_row, src);
 			p.rows		  = __builtin_amdgcn_readlane(z.rows, src);
-			p.pos0		  = max(b.lengths[p.seq], 0) - (__builtin_amdgcn_readlane(z.end, src) - p.first_row);
+			p.pos0		  = __builtin_amdgcn_readlane(z.pos0, src);
 			p.stride	  = __builtin_amdgcn_readlane(groups, src);
 			const int k	  = t - before - (__builtin_amdgcn_readlane(upto, src) - __builtin_amdgcn_readlane(count, src));
 			p.row_group	  = k % p.stride; // row groups side by side: they read the same keys
@@ -155,13 +200,29 @@ __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int a
 	return p;
 }
 
-// Results between workgroups: device-scope stores and loads, past the caches that another XCD does not see.
+// Results between workgroups: device-scope stores and loads (sc1), past the caches that another XCD does not see.
 __device__ __forceinline__ void put4(float* p, v4f v) {
-	__hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, float2{ v[0], v[1] }), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-	__hip_atomic_store(reinterpret_cast<uint64_t*>(p) + 1, __builtin_bit_cast(uint64_t, float2{ v[2], v[3] }), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+	asm volatile("global_store_dwordx4 %0, %1, off sc1" ::"v"(p), "v"(v) : "memory");
 }
-__device__ __forceinline__ float2 get2(const float2* p) {
-	return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+__device__ __forceinline__ void put2(float2* p, float2 v) {
+	asm volatile("global_store_dwordx2 %0, %1, off sc1" ::"v"(p), "v"(__builtin_bit_cast(v2u, v)) : "memory");
+}
+// Four results at once, {maximum, sum} and four values of each: eight loads under one wait.
+__device__ __forceinline__ void get_parts(const float2* const (&ml)[4], const float* const (&o)[4], float2 (&got_ml)[4], v4f (&got_o)[4]) {
+	v2u m0, m1, m2, m3;
+	asm volatile("global_load_dwordx2 %0, %8, off sc1\n\t"
+				 "global_load_dwordx2 %1, %9, off sc1\n\t"
+				 "global_load_dwordx2 %2, %10, off sc1\n\t"
+				 "global_load_dwordx2 %3, %11, off sc1\n\t"
+				 "global_load_dwordx4 %4, %12, off sc1\n\t"
+				 "global_load_dwordx4 %5, %13, off sc1\n\t"
+				 "global_load_dwordx4 %6, %14, off sc1\n\t"
+				 "global_load_dwordx4 %7, %15, off sc1\n\t"
+				 "s_waitcnt vmcnt(0)"
+				 : "=&v"(m0), "=&v"(m1), "=&v"(m2), "=&v"(m3), "=&v"(got_o[0]), "=&v"(got_o[1]), "=&v"(got_o[2]), "=&v"(got_o[3])
+				 : "v"(ml[0]), "v"(ml[1]), "v"(ml[2]), "v"(ml[3]), "v"(o[0]), "v"(o[1]), "v"(o[2]), "v"(o[3])
+				 : "memory");
+	got_ml[0] = __builtin_bit_cast(float2, m0), got_ml[1] = __builtin_bit_cast(float2, m1), got_ml[2] = __builtin_bit_cast(float2, m2), got_ml[3] = __builtin_bit_cast(float2, m3);
 }
 
 // a running result and another one, both sums of weights and of weighted values below their own maximum
@@ -180,7 +241,10 @@ struct running {
 } // namespace
 
 template<int CACHE, int TYPE, int D>
-__global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_args a, rows_workspace w, int units) {
+__global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* starts, const int32_t* page_table, int sequences, int width, int all_rows,
+	int q_heads, int kv_heads, int page_shift, int prefix_count, int units, int fit, attention_args a, rows_workspace w) {
+	// (what the first loads take comes first: the leading arguments arrive in registers, the rest is read from memory)
+	const batch_view batch{ page_table, lengths, starts, sequences, width };
 	using H				= half_type<CACHE>;
 	using vec			= typename H::vec;
 	constexpr int N		= terms<CACHE, TYPE>;
@@ -192,11 +256,27 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int col = lane & 15, quarter = lane >> 4;
-	const int group		  = a.q_heads / a.cache.kv_heads;
-	const int head		  = blockIdx.x % a.cache.kv_heads;
-	const int prefix_keys = a.prefix_count << a.cache.page_shift, held = a.batch.width << a.cache.page_shift;
-	const int piece		  = blockIdx.x / a.cache.kv_heads;
-	const piece_place p	  = place_of_piece(a.batch, a.rows, group, prefix_keys, held, units, piece);
+	const int group		  = q_heads / kv_heads;
+	const int head		  = blockIdx.x % kv_heads;
+	const int prefix_keys = prefix_count << page_shift, held = width << page_shift;
+	const int piece		  = blockIdx.x / kv_heads;
+	// One sequence of one row: whose q and pages these are is known ahead of its length, so they are asked for together.
+	const bool single = sequences == 1 && starts == nullptr;
+	float x[STEPS][8];
+	int first_pages = -1; // lane i: the i-th page of the one sequence
+	auto load_q		= [&](int row, int q_head, bool there) {
+		const int64_t at = static_cast<int64_t>(row) * a.q_stride + static_cast<int64_t>(q_head) * D + 8 * quarter;
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			load_q8<TYPE>(a.q, at + 32 * s, there, x[s]);
+		}
+	};
+	if (single) {
+		const int in_group = piece % ((group + COLUMNS - 1) / COLUMNS) * COLUMNS + col;
+		load_q(0, head * group + min(in_group, group - 1), in_group < group);
+		first_pages = lane < width ? page_table[lane] : -1;
+	}
+	const piece_place p = place_of_piece(batch, all_rows, group, prefix_keys, held, units, fit, piece);
 	if (!p.there) {
 		return;
 	}
@@ -215,16 +295,62 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 	const int first_key = prefix_keys + p.index * p.length;
 	const int end_key	= min(first_key + p.length, most_seen);
 
+	const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
+	const int page_size	 = 1 << page_shift;
+	// A step's keys base .. base + 31 lie in the pages of its two halves of 16.
+	struct step_data {
+		vec k[2][STEPS], v[DT];
+		int base, page_lo, page_hi;
+	};
+	auto load_pages = [&](int base, step_data& d) {
+		d.base			 = base;
+		const int slot_0 = base >> page_shift, slot_1 = (base + 16) >> page_shift;
+		if (single && slot_1 < 64) {
+			d.page_lo = base < end_key ? __builtin_amdgcn_readlane(first_pages, slot_0) : -1;
+			d.page_hi = base + 16 < end_key ? __builtin_amdgcn_readlane(first_pages, slot_1) : -1;
+			return;
+		}
+		d.page_lo = base < end_key ? table[slot_0] : -1;
+		d.page_hi = base + 16 < end_key ? table[slot_1] : -1;
+	};
+	auto page_there = [&](int id) {
+		return id >= 0 && id < a.cache.pages;
+	};
+	auto load_step = [&](step_data& d) {
+		const int lo = page_there(d.page_lo) ? d.page_lo : 0, hi = page_there(d.page_hi) ? d.page_hi : 0;
+		const int64_t k_page = (col & 8 ? hi : lo) * a.cache.page_values, v_page = (quarter & 2 ? hi : lo) * a.cache.page_values;
+#pragma unroll
+		for (int t = 0; t < 2; ++t) {
+			const int key	   = (d.base + 8 * (col >> 2) + 4 * t + (col & 3)) & (page_size - 1);
+			const uint16_t* at = a.cache.k + k_page + (static_cast<int64_t>(head) * page_size + key) * D + 8 * quarter;
+#pragma unroll
+			for (int s = 0; s < STEPS; ++s) {
+				d.k[t][s] = *reinterpret_cast<const vec*>(at + 32 * s);
+			}
+		}
+		const uint16_t* at = a.cache.v + v_page + (static_cast<int64_t>(head) * D + col) * page_size + ((d.base + 8 * quarter) & (page_size - 1));
+#pragma unroll
+		for (int dt = 0; dt < DT; ++dt) {
+			d.v[dt] = *reinterpret_cast<const vec*>(at + static_cast<int64_t>(dt) * 16 * page_size);
+		}
+	};
+
+	// two steps in turn: one's loads in flight under the other's arithmetic, the page numbers a step ahead of the loads
+	step_data d0, d1;
+	constexpr int stride = STEP * WAVES;
+	int base			 = first_key + wave * STEP;
+	load_pages(base, d0);
+	load_pages(base + stride, d1);
 	// q as the B operand: column = row, values 32 s + 8 quarter .. + 7
 	vec q[N][STEPS];
 	float c;
 	{
-		const int64_t at = (static_cast<int64_t>(p.first_row) + token) * a.q_stride + static_cast<int64_t>(q_head) * D + 8 * quarter;
-		float x[STEPS][8];
+		if (!single) {
+			load_q(p.first_row + token, q_head, there);
+		}
 		float largest = 0.0f;
-#pragma unroll
-		for (int s = 0; s < STEPS; ++s) {
-			load_q8<TYPE>(a.q, at + 32 * s, there, x[s]);
+		if (base < end_key) {
+			load_step(d0); // (behind q's own loads, ahead of what is done with them)
 		}
 #pragma unroll
 		for (int s = 0; s < STEPS; ++s) {
@@ -253,41 +379,6 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 		}
 		c = ldexpf(a.scale * LOG2_E, e - 14);
 	}
-
-	const int32_t* table = a.batch.table + static_cast<int64_t>(p.seq) * a.batch.width;
-	const int page_size	 = 1 << a.cache.page_shift;
-	// A step's keys base .. base + 31 lie in the pages of its two halves of 16.
-	struct step_data {
-		vec k[2][STEPS], v[DT];
-		int base, page_lo, page_hi;
-	};
-	auto load_pages = [&](int base, step_data& d) {
-		d.base			 = base;
-		const int slot_0 = base >> a.cache.page_shift, slot_1 = (base + 16) >> a.cache.page_shift;
-		d.page_lo		 = base < end_key ? table[slot_0] : -1;
-		d.page_hi		 = base + 16 < end_key ? table[slot_1] : -1;
-	};
-	auto page_there = [&](int id) {
-		return id >= 0 && id < a.cache.pages;
-	};
-	auto load_step = [&](step_data& d) {
-		const int lo = page_there(d.page_lo) ? d.page_lo : 0, hi = page_there(d.page_hi) ? d.page_hi : 0;
-		const int64_t k_page = (col & 8 ? hi : lo) * a.cache.page_values, v_page = (quarter & 2 ? hi : lo) * a.cache.page_values;
-#pragma unroll
-		for (int t = 0; t < 2; ++t) {
-			const int key	   = (d.base + 8 * (col >> 2) + 4 * t + (col & 3)) & (page_size - 1);
-			const uint16_t* at = a.cache.k + k_page + (static_cast<int64_t>(head) * page_size + key) * D + 8 * quarter;
-#pragma unroll
-			for (int s = 0; s < STEPS; ++s) {
-				d.k[t][s] = *reinterpret_cast<const vec*>(at + 32 * s);
-			}
-		}
-		const uint16_t* at = a.cache.v + v_page + (static_cast<int64_t>(head) * D + col) * page_size + ((d.base + 8 * quarter) & (page_size - 1));
-#pragma unroll
-		for (int dt = 0; dt < DT; ++dt) {
-			d.v[dt] = *reinterpret_cast<const vec*>(at + static_cast<int64_t>(dt) * 16 * page_size);
-		}
-	};
 
 	v4f o[DT];
 #pragma unroll
@@ -362,15 +453,6 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 		}
 	};
 
-	// two steps in turn: one's loads in flight under the other's arithmetic, the page numbers a step ahead of the loads
-	step_data d0, d1;
-	constexpr int stride = STEP * WAVES;
-	int base			 = first_key + wave * STEP;
-	load_pages(base, d0);
-	load_pages(base + stride, d1);
-	if (base < end_key) {
-		load_step(d0);
-	}
 	while (base < end_key) {
 		if (base + stride < end_key) {
 			load_step(d1);
@@ -401,7 +483,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 	}
 	__syncthreads();
 	const bool alone	= pieces == 1 && w.prefix_pieces == 0;
-	const int64_t slot	= static_cast<int64_t>(piece) * a.cache.kv_heads + head;
+	const int64_t slot	= static_cast<int64_t>(piece) * kv_heads + head;
 	if (there) {
 		float2 ml[WAVES];
 #pragma unroll
@@ -416,7 +498,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 			sum += ml[x].y * f[x];
 		}
 		const float inv		  = alone ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f; // no key at all: zeros
-		const int64_t out_row = ((static_cast<int64_t>(p.first_row) + token) * a.q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D;
+		const int64_t out_row = ((static_cast<int64_t>(p.first_row) + token) * q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D;
 #pragma unroll
 		for (int dt = wave; dt < DT; dt += WAVES) {
 			v4f v{};
@@ -431,13 +513,13 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 			}
 		}
 		if (!alone && wave == 0 && quarter == 0) {
-			__hip_atomic_store(reinterpret_cast<uint64_t*>(w.ml + slot * w.columns + col), __builtin_bit_cast(uint64_t, make_float2(top, sum)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+			put2(w.ml + slot * w.columns + col, make_float2(top, sum));
 		}
 	}
 	if (alone) {
 		return;
 	}
-	const int64_t first_slot = slot - static_cast<int64_t>(p.index) * p.stride * a.cache.kv_heads;
+	const int64_t first_slot = slot - static_cast<int64_t>(p.index) * p.stride * kv_heads;
 	if (pieces > 1) {
 		wait_stores_acknowledged();
 		__syncthreads();
@@ -460,7 +542,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 	constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
 	running* parts		= reinterpret_cast<running*>(&join_o[0][0][0]); // [GROUPS][LANES], 24 (32 aligned) bytes each
 	static_assert(sizeof(running) * THREADS <= sizeof(join_o), "the parts of the join fit where the waves' results were");
-	const int x = tid % LANES, g = tid / LANES;
+	const int part = tid % LANES, g = tid / LANES;
 	const int rows_at_once = count <= 1 ? 1 : count <= 2 ? 2 : count <= 4 ? 4 : 8; // a divisor of GROUPS
 	const int ways = GROUPS / rows_at_once, way = g / rows_at_once;
 	const int all = w.prefix_pieces + pieces;
@@ -471,15 +553,27 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 		const int q_h	  = head * group + first + min(r, count - 1) - tok * group;
 		running sum{ -__builtin_inff(), 0.0f, v4f{} };
 		if (mine) {
-#pragma unroll 4
-			for (int i = way; i < all; i += ways) {
-				const bool shared = i < w.prefix_pieces;
-				const int64_t at  = shared ? (static_cast<int64_t>(i) * a.batch.sequences + p.seq) * a.q_heads + q_h
-										   : (first_slot + static_cast<int64_t>(i - w.prefix_pieces) * p.stride * a.cache.kv_heads) * w.columns + r;
-				const float2 ml	  = get2((shared ? w.prefix_ml : w.ml) + at);
-				const float2* v	  = reinterpret_cast<const float2*>((shared ? w.prefix_o : w.o) + at * D + 4 * x);
-				const float2 lo = get2(v), hi = get2(v + 1);
-				sum.add(ml.x, ml.y, v4f{ lo.x, lo.y, hi.x, hi.y });
+			for (int i0 = way; i0 < all; i0 += 4 * ways) {
+				const float2* ml[4];
+				const float* o4[4];
+				float2 got_ml[4];
+				v4f got_o[4];
+#pragma unroll
+				for (int k = 0; k < 4; ++k) {
+					const int i		  = min(i0 + k * ways, all - 1); // (past the last one: the last one again, not added)
+					const bool shared = i < w.prefix_pieces;
+					const int64_t at  = shared ? (static_cast<int64_t>(i) * sequences + p.seq) * q_heads + q_h
+											   : (first_slot + static_cast<int64_t>(i - w.prefix_pieces) * p.stride * kv_heads) * w.columns + r;
+					ml[k]			  = (shared ? w.prefix_ml : w.ml) + at;
+					o4[k]			  = (shared ? w.prefix_o : w.o) + at * D + 4 * part;
+				}
+				get_parts(ml, o4, got_ml, got_o);
+#pragma unroll
+				for (int k = 0; k < 4; ++k) {
+					if (i0 + k * ways < all) {
+						sum.add(got_ml[k].x, got_ml[k].y, got_o[k]);
+					}
+				}
 			}
 		}
 		__syncthreads(); // (the last rows' parts have been read)
@@ -491,7 +585,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(attention_ar
 				sum.add(other.m, other.l, other.o);
 			}
 			const float inv = sum.l > 0.0f || sum.l != sum.l ? 1.0f / sum.l : 0.0f;
-			store_out4<TYPE>(a.out, ((static_cast<int64_t>(p.first_row) + tok) * a.q_heads + q_h) * D + 4 * x, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
+			store_out4<TYPE>(a.out, ((static_cast<int64_t>(p.first_row) + tok) * q_heads + q_h) * D + 4 * part, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
 		}
 	}
 }
@@ -515,7 +609,12 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 			return e;
 		}
 	}
-	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(cut.pieces * a.cache.kv_heads)), dim3(THREADS), 0, s>>>(a, w, static_cast<int>(cut.units));
+	// no row group has more pieces than its table has keys for
+	const int64_t row_groups = cut.pieces - cut.units, keys = static_cast<int64_t>(a.batch.width) << a.cache.page_shift;
+	const int64_t pieces	 = std::min(cut.pieces, row_groups * std::max<int64_t>(1, (keys + STEP * WAVES - 1) / (STEP * WAVES)));
+	attention_rows_kernel<CACHE, TYPE, D>
+		<<<dim3(static_cast<unsigned>(pieces * a.cache.kv_heads)), dim3(THREADS), 0, s>>>(a.batch.lengths, a.batch.starts, a.batch.table, a.batch.sequences, a.batch.width, a.rows, a.q_heads,
+			a.cache.kv_heads, a.cache.page_shift, a.prefix_count, static_cast<int>(cut.units), std::max(1, AT_ONCE / a.cache.kv_heads), a, w);
 	return hipGetLastError();
 }
 template<int CACHE, int TYPE> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
