@@ -33,7 +33,7 @@ inline int check_cache(const nh_attn_cache* c) {
 	NH_REQUIRE(c, NH_ERR_NULL_POINTER);
 	NH_REQUIRE(c->type == NH_F16 || c->type == NH_BF16, NH_ERR_ARGUMENT);
 	NH_REQUIRE(c->layers > 0 && c->pages > 0 && c->kv_heads > 0 && page_shift(c->page_size) > 0 && (c->head_dim == 64 || c->head_dim == 128), NH_ERR_SHAPE);
-	NH_REQUIRE(c->layers <= 65536 && c->kv_heads <= 65536 && c->pages <= (int64_t{ 1 } << 28), NH_ERR_TOO_LARGE);
+	NH_REQUIRE(c->layers <= 65536 && c->kv_heads < 65536 && c->pages <= (int64_t{ 1 } << 28), NH_ERR_TOO_LARGE);
 	NH_REQUIRE(c->k_pages && c->v_pages, NH_ERR_NULL_POINTER);
 	NH_REQUIRE(aligned16(c->k_pages) && aligned16(c->v_pages), NH_ERR_ALIGNMENT);
 	return NH_OK;
@@ -53,7 +53,7 @@ inline int64_t value_bytes(int type) {
 inline int check_rows(const nh_attn_cache* c, int type, int64_t rows, int64_t heads, int64_t stride) {
 	NH_REQUIRE(type == NH_F32 || type == c->type, NH_ERR_ARGUMENT);
 	NH_REQUIRE(rows >= 0 && heads > 0 && heads % c->kv_heads == 0, NH_ERR_SHAPE);
-	NH_REQUIRE(heads <= 65536 && rows <= MAX_ROW_HEADS / heads, NH_ERR_TOO_LARGE);
+	NH_REQUIRE(heads < 65536 && rows <= MAX_ROW_HEADS / heads, NH_ERR_TOO_LARGE);
 	NH_REQUIRE(stride >= heads * c->head_dim && stride <= (int64_t{ 1 } << 40), NH_ERR_SHAPE);
 	NH_REQUIRE(stride * value_bytes(type) % 16 == 0, NH_ERR_ALIGNMENT);
 	return NH_OK;
@@ -137,7 +137,7 @@ static int check_heads(int64_t rows, int64_t sequences, int64_t q_heads, int64_t
 	NH_REQUIRE(a && b, NH_ERR_NULL_POINTER);
 	NH_REQUIRE(rows >= 0 && sequences >= 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128), NH_ERR_SHAPE);
 	// one workgroup for 16 rows of a kv head, and one more for each sequence and kv head
-	NH_REQUIRE(sequences <= MAX_SEQUENCES && q_heads <= 65536 && rows <= MAX_ROW_HEADS / q_heads && sequences * kv_heads <= MAX_ROW_HEADS / 4, NH_ERR_TOO_LARGE);
+	NH_REQUIRE(sequences <= MAX_SEQUENCES && q_heads < 65536 && rows <= MAX_ROW_HEADS / q_heads && sequences * kv_heads <= MAX_ROW_HEADS / 4, NH_ERR_TOO_LARGE);
 	return NH_OK;
 }
 

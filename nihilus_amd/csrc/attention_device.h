@@ -131,12 +131,7 @@ template<int TYPE> __device__ __forceinline__ void load_q8(const void* q, int64_
 // 2^(e-1) <= largest < 2^e, so that two fp16 terms hold 22 bits of each value that matters beside the largest.  bf16 has fp32's range: e = 14.
 template<int CACHE, int TYPE> __device__ __forceinline__ int q_exponent(float largest) {
 	if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
-		int e = 14;
-		if (largest > 0.0f && largest < __builtin_inff()) {
-			(void)frexpf(largest, &e);
-			e = max(e, -60); // (a row this small gives scores of 2^-60: what is lost of it does not show)
-		}
-		return e;
+		return max(__builtin_amdgcn_frexp_expf(largest), -60); // (0 for zero, infinity and NaN; a row smaller than 2^-60 gives scores of 2^-60: what is lost of it does not show)
 	}
 	return 14;
 }

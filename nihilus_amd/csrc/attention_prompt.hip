@@ -168,6 +168,7 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 			}
 			e = q_exponent<CACHE, TYPE>(fmaxf(largest, swap32(largest)));
 		}
+		const float up = ldexpf(1.0f, 14 - e);
 #pragma unroll
 		for (int s = 0; s < STEPS; ++s) {
 			float x[8];
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 			if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
 #pragma unroll
 				for (int j = 0; j < 8; ++j) {
-					x[j] = ldexpf(x[j], 14 - e);
+					x[j] *= up;
 				}
 			}
 			vec t[N];

@@ -32,7 +32,7 @@ constexpr int COLUMNS	 = 16; // rows of a row group
 // What the pieces are cut for: twice what the chip holds at once (two per CU), so that the last ones to start are short.  decode of 64 sequences of up to 8192 keys
 // (32 / 8 heads): 512 61.5 us, 1024 55.4, 2048 60.0, 4096 68.5.
 constexpr int WORKGROUPS = 1024;
-constexpr int AT_ONCE		= 512; // workgroups that the chip holds at once
+constexpr int AT_ONCE		= 256; // workgroups that the chip holds at once
 constexpr int SHORT_LENGTHS = 4; // short pieces are of 1, 2, 4 or 8 steps for each wave
 constexpr int64_t MOST_SHORT = (int64_t{ WAVES } << (SHORT_LENGTHS - 1)) * WORKGROUPS; // more steps than that make long pieces
 
@@ -46,13 +46,17 @@ struct rows_workspace {
 	int32_t* counters; // [slot]  of a row group's first piece: how many of its pieces are done; zero before and after every call
 };
 struct rows_cut {
-	int64_t units; // pieces that the keys are cut into at most, beside one per row group
+	int64_t units; // pieces that the keys are cut into at most, beside one per row group: a power of two
+	int units_log2;
 	int64_t pieces; // most pieces there can be
 	int64_t columns; // rows of a row group that are kept in the workspace
 };
 rows_cut plan_rows(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t kv_heads) {
 	rows_cut c{};
-	c.units	  = std::max<int64_t>(1, WORKGROUPS / kv_heads);
+	while ((int64_t{ 2 } << c.units_log2) * kv_heads <= WORKGROUPS) {
+		++c.units_log2;
+	}
+	c.units	  = int64_t{ 1 } << c.units_log2;
 	c.pieces  = c.units + (one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : rows * group / COLUMNS + sequences);
 	c.columns = one_each ? std::min<int64_t>(group, COLUMNS) : COLUMNS;
 	return c;
@@ -118,8 +122,8 @@ __device__ __forceinline__ int sum64(int x) {
 	return __builtin_amdgcn_readlane(scan64(x), 63);
 }
 // How long a piece is, in steps: see place_of_piece.
-__device__ __forceinline__ int piece_steps(int64_t total, const int (&pieces)[SHORT_LENGTHS], int units, int fit) {
-	int64_t steps = (total + units - 1) / units;
+__device__ __forceinline__ int piece_steps(int64_t total, const int (&pieces)[SHORT_LENGTHS], int units_log2, int fit) {
+	const int64_t steps = (total + (int64_t{ 1 } << units_log2) - 1) >> units_log2;
 	if (steps <= WAVES << (SHORT_LENGTHS - 1)) {
 #pragma unroll
 		for (int i = 0; i < SHORT_LENGTHS; ++i) {
@@ -128,12 +132,12 @@ __device__ __forceinline__ int piece_steps(int64_t total, const int (&pieces)[SH
 			}
 		}
 	}
-	return static_cast<int>(min(steps + WAVES - 1, int64_t{ 1 } << 25)) / WAVES * WAVES; // (2^30 keys are all that a table holds)
+	return (static_cast<int>(min(steps, (int64_t{ 1 } << 25) - WAVES)) + WAVES - 1) & -WAVES; // (2^30 keys are all that a table holds)
 }
 // Piece `t` of the batch.  Every wave adds the work up by itself, 64 sequences at a time.  A piece is `units`th of the work long, but not so short
 // that the pieces do not fit on the chip at once (`fit`) when a piece of twice the length is still short: a workgroup takes some 5 us
 // before and behind its steps, a step 0.6.
-__device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int all_rows, int group, int prefix_keys, int held, int units, int fit, int t) {
+__device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int all_rows, int group, int prefix_keys, int held, int units_log2, int fit, int t) {
 	const int lane = threadIdx.x & 63;
 	piece_place p{};
 	if (b.sequences == 1) { // nothing to add up, and nothing to wait for but the one length
@@ -146,8 +150,9 @@ __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int a
 		}
 		p.first_row = z.first_row, p.rows = z.rows, p.pos0 = z.pos0;
 		p.stride	= max(groups, 1);
-		p.row_group = t % p.stride, p.index = t / p.stride;
-		p.length	= piece_steps(static_cast<int64_t>(groups) * steps, pieces, units, fit) * STEP;
+		p.index		= p.stride == 1 ? t : t / p.stride;
+		p.row_group = t - p.index * p.stride;
+		p.length	= piece_steps(static_cast<int64_t>(groups) * steps, pieces, units_log2, fit) * STEP;
 		p.there		= groups > 0;
 		return p;
 	}
@@ -171,7 +176,7 @@ __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int a
 			}
 		}
 	}
-	const int length = piece_steps(total, pieces, units, fit) * STEP;
+	const int length = piece_steps(total, pieces, units_log2, fit) * STEP;
 	int before = 0;
 	for (int base = 0; base < b.sequences; base += 64) {
 		if (b.sequences > 64) {
@@ -189,8 +194,8 @@ __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int a
 			p.pos0		  = __builtin_amdgcn_readlane(z.pos0, src);
 			p.stride	  = __builtin_amdgcn_readlane(groups, src);
 			const int k	  = t - before - (__builtin_amdgcn_readlane(upto, src) - __builtin_amdgcn_readlane(count, src));
-			p.row_group	  = k % p.stride; // row groups side by side: they read the same keys
-			p.index		  = k / p.stride;
+			p.index		  = p.stride == 1 ? k : k / p.stride;
+			p.row_group	  = k - p.index * p.stride; // row groups side by side: they read the same keys
 			p.length	  = length;
 			p.there		  = true;
 			return p;
@@ -241,140 +246,166 @@ struct running {
 } // namespace
 
 template<int CACHE, int TYPE, int D>
-__global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* starts, const int32_t* page_table, int sequences, int width, int all_rows,
-	int q_heads, int kv_heads, int page_shift, int prefix_count, int units, int fit, attention_args a, rows_workspace w) {
-	// (what the first loads take comes first: the leading arguments arrive in registers, the rest is read from memory)
-	const batch_view batch{ page_table, lengths, starts, sequences, width };
-	using H				= half_type<CACHE>;
-	using vec			= typename H::vec;
-	constexpr int N		= terms<CACHE, TYPE>;
-	constexpr int STEPS = D / 32; // of q.k
-	constexpr int DT	= D / 16; // tiles of O^T
-	__shared__ v4f join_o[WAVES][DT][64];
+__global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const uint16_t* v_pages,
+	uint32_t shape, int width, int prefix_count, uint32_t heads, attention_args a, rows_workspace w) {
+	// What the first loads take comes first, in fourteen dwords: those arrive in registers, the rest is read from memory, as far away as the data.
+	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | one row per sequence << 31
+	const int kv_heads = heads & 0xFFFF, group = heads >> 16, sequences = shape & 0x1FFFFF, page_shift = (shape >> 21) & 15, units_log2 = (shape >> 25) & 15;
+	const bool one_each = (shape >> 31) != 0;
+	const int all_rows	= one_each ? sequences : a.rows;
+	const batch_view batch{ page_table, lengths, one_each ? nullptr : a.batch.starts, sequences, width };
+	const int fit = max(1, AT_ONCE >> (kv_heads > 1 ? 32 - __builtin_clz(kv_heads - 1) : 0)); // pieces per kv head (or fewer) that the chip holds at once
+	using H				 = half_type<CACHE>;
+	using vec			 = typename H::vec;
+	constexpr int N		 = terms<CACHE, TYPE>;
+	constexpr int STEPS	 = D / 32; // of q.k
+	constexpr int DT	 = D / 16; // tiles of O^T
+	constexpr int PIECES = D / 8; // 16-byte pieces of a key
+	constexpr int LOADS	 = STEP * PIECES / 64; // instructions for a step's keys, and for its values
+	constexpr int SLOT	 = 2 * STEP * PIECES; // pieces of a step
+	__shared__ v4u slots[WAVES][2][SLOT];
 	__shared__ float2 join_ml[WAVES][COLUMNS];
 	__shared__ int is_last;
 
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int col = lane & 15, quarter = lane >> 4;
-	const int group		  = q_heads / kv_heads;
-	const int head		  = blockIdx.x % kv_heads;
+	const int q_heads	  = group * kv_heads;
+	const int head		  = blockIdx.x;
 	const int prefix_keys = prefix_count << page_shift, held = width << page_shift;
-	const int piece		  = blockIdx.x / kv_heads;
-	// One sequence of one row: whose q and pages these are is known ahead of its length, so they are asked for together.
-	const bool single = sequences == 1 && starts == nullptr;
-	float x[STEPS][8];
-	int first_pages = -1; // lane i: the i-th page of the one sequence
-	auto load_q		= [&](int row, int q_head, bool there) {
-		const int64_t at = static_cast<int64_t>(row) * a.q_stride + static_cast<int64_t>(q_head) * D + 8 * quarter;
+	const int piece		  = blockIdx.z * gridDim.y + blockIdx.y;
+
+	// The row group's q goes into the second slot, which is not needed before the second step: as many 16-byte pieces of a row as it has, piece x of row r
+	// at x ^ (r % 8).  Columns past the last row hold that one again; their results go nowhere.
+	constexpr int Q_PIECES = TYPE == NH_F32 ? D / 4 : D / 8;
+	auto load_q			   = [&](int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
 #pragma unroll
-		for (int s = 0; s < STEPS; ++s) {
-			load_q8<TYPE>(a.q, at + 32 * s, there, x[s]);
+		for (int j = 0; j < COLUMNS * Q_PIECES / 64; ++j) {
+			const int at = 64 * j + lane, r = at / Q_PIECES, x = (at % Q_PIECES) ^ (r & 7);
+			const int i = rest + min(r, rows - 1), tok = static_cast<int>((static_cast<float>(i) + 0.5f) * inverse);
+			const int64_t from = (row0 + tok == 0 ? 0 : (row0 + tok) * a.q_stride) + static_cast<int64_t>(head0 + i - tok * group) * D;
+			load_global_to_lds_b128(static_cast<const char*>(q_rows) + from * (TYPE == NH_F32 ? 4 : 2) + 16 * x, &slots[wave][1][64 * j]);
 		}
 	};
+	const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
+	// One sequence of one row: whose q and pages these are is known ahead of its length, so all three are asked for together.
+	const bool single = sequences == 1 && one_each;
+	int ids			  = page_table[min(lane, max(width, 1) - 1)]; // lane i: page first_id + i of the sequence (the host gives a table that can be read)
+	int first_id	  = 0;
 	if (single) {
-		const int in_group = piece % ((group + COLUMNS - 1) / COLUMNS) * COLUMNS + col;
-		load_q(0, head * group + min(in_group, group - 1), in_group < group);
-		first_pages = lane < width ? page_table[lane] : -1;
+		const int groups = (group + COLUMNS - 1) / COLUMNS;
+		const int row	 = (groups == 1 ? 0 : piece % groups) * COLUMNS;
+		load_q(0, head * group, row, 0.0f, min(COLUMNS, group - row)); // (all of them rows of token 0)
 	}
-	const piece_place p = place_of_piece(batch, all_rows, group, prefix_keys, held, units, fit, piece);
+	const piece_place p = place_of_piece(batch, all_rows, group, prefix_keys, held, units_log2, fit, piece);
 	if (!p.there) {
+		wait_stores_acknowledged(); // (nothing may still be on its way into LDS when the workgroup ends)
 		return;
 	}
 	// the row group's rows: first .. first + count - 1 of the sequence's rows * group
 	const int first = p.row_group * COLUMNS, count = min(COLUMNS, p.rows * group - first);
+	const int first_token = first / group, first_rest = first - first_token * group;
+	// the token of the group's row i: (first + i) / group, as first_token + (first_rest + i) / group, whose numerator is below 2^17: exact in fp32, half a
+	// numerator's step away from the next whole number
+	auto token_of = [&](int i) {
+		return first_token + static_cast<int>((static_cast<float>(first_rest + i) + 0.5f) * inv_group);
+	};
 	const bool there = col < count;
-	const int token	 = (first + min(col, count - 1)) / group;
+	const int token	 = token_of(min(col, count - 1));
 	const int q_head = head * group + first + min(col, count - 1) - token * group;
-	// keys: the sequence's own ones that the lane's row sees end at `seen`, those that some row of the group sees at end, that all see at all_seen
+	// keys: the sequence's own ones that the lane's row sees end at `seen`, those that some row of the group sees at most_seen, that all see at all_seen
 	const int seen	   = min(held, p.pos0 + token + 1);
-	const int all_seen = min(held, p.pos0 + first / group + 1), most_seen = min(held, p.pos0 + (first + count - 1) / group + 1);
+	const int all_seen = min(held, p.pos0 + first_token + 1), most_seen = min(held, p.pos0 + token_of(count - 1) + 1);
 	const int pieces   = max(1, (max(0, most_seen - prefix_keys) + p.length - 1) / p.length); // of this row group
-	if (p.index >= pieces) {
-		return; // (rows in front of the sequence's last see less)
+	if (p.index >= pieces) { // (rows in front of the sequence's last see less)
+		wait_stores_acknowledged();
+		return;
 	}
 	const int first_key = prefix_keys + p.index * p.length;
 	const int end_key	= min(first_key + p.length, most_seen);
 
 	const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
 	const int page_size	 = 1 << page_shift;
-	// A step's keys base .. base + 31 lie in the pages of its two halves of 16.
-	struct step_data {
-		vec k[2][STEPS], v[DT];
-		int base, page_lo, page_hi;
-	};
-	auto load_pages = [&](int base, step_data& d) {
-		d.base			 = base;
-		const int slot_0 = base >> page_shift, slot_1 = (base + 16) >> page_shift;
-		if (single && slot_1 < 64) {
-			d.page_lo = base < end_key ? __builtin_amdgcn_readlane(first_pages, slot_0) : -1;
-			d.page_hi = base + 16 < end_key ? __builtin_amdgcn_readlane(first_pages, slot_1) : -1;
-			return;
+	if (!single) {
+		first_id = first_key >> page_shift;
+		ids		 = table[min(first_id + lane, max(width, 1) - 1)];
+		load_q(p.first_row + first_token, head * group, first_rest, inv_group, count);
+	}
+	// The page of the 16 keys from `key` on, -1 if there is none: of the first 64 pages from a register, of the others from memory.
+	auto page_of = [&](int key) {
+		if (key >= end_key) {
+			return -1;
 		}
-		d.page_lo = base < end_key ? table[slot_0] : -1;
-		d.page_hi = base + 16 < end_key ? table[slot_1] : -1;
+		const int slot = key >> page_shift, id = slot - first_id < 64 ? __builtin_amdgcn_readlane(ids, slot - first_id) : table[slot];
+		return id >= 0 && id < a.cache.pages ? id : -1;
 	};
-	auto page_there = [&](int id) {
-		return id >= 0 && id < a.cache.pages;
+	// A step's 32 keys into a slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
+	// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).  Eight
+	// lanes that read the same piece of eight operand rows hit different banks: K rows differ in bits 0, 1, 3, V rows in bits 0 .. 2.
+	const int64_t page_values = static_cast<int64_t>(kv_heads) * D << page_shift, head_values = static_cast<int64_t>(head) * D << page_shift;
+	auto load_step			  = [&](int base, int lo, int hi, int slot) {
+		 const int64_t lo_at = max(lo, 0) * page_values + head_values, hi_at = max(hi, 0) * page_values + head_values;
+#pragma unroll
+		 for (int j = 0; j < LOADS; ++j) {
+			 const int at = 64 * j + lane, r = at / PIECES, x = (at % PIECES) ^ ((r & 3) | ((r >> 1) & 4));
+			 const int key = (base + r) & (page_size - 1);
+			 load_global_to_lds_b128(k_pages + (2 * j < LOADS ? lo_at : hi_at) + key * D + 8 * x, &slots[wave][slot][64 * j]);
+		 }
+#pragma unroll
+		 for (int j = 0; j < LOADS; ++j) {
+			 const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 1) & 3);
+			 const int key = (base + 8 * x) & (page_size - 1);
+			 load_global_to_lds_b128(v_pages + (x & 2 ? hi_at : lo_at) + d * page_size + key, &slots[wave][slot][STEP * PIECES + 64 * j]);
+		 }
 	};
-	auto load_step = [&](step_data& d) {
-		const int lo = page_there(d.page_lo) ? d.page_lo : 0, hi = page_there(d.page_hi) ? d.page_hi : 0;
-		const int64_t k_page = (col & 8 ? hi : lo) * a.cache.page_values, v_page = (quarter & 2 ? hi : lo) * a.cache.page_values;
-#pragma unroll
-		for (int t = 0; t < 2; ++t) {
-			const int key	   = (d.base + 8 * (col >> 2) + 4 * t + (col & 3)) & (page_size - 1);
-			const uint16_t* at = a.cache.k + k_page + (static_cast<int64_t>(head) * page_size + key) * D + 8 * quarter;
-#pragma unroll
-			for (int s = 0; s < STEPS; ++s) {
-				d.k[t][s] = *reinterpret_cast<const vec*>(at + 32 * s);
-			}
-		}
-		const uint16_t* at = a.cache.v + v_page + (static_cast<int64_t>(head) * D + col) * page_size + ((d.base + 8 * quarter) & (page_size - 1));
-#pragma unroll
-		for (int dt = 0; dt < DT; ++dt) {
-			d.v[dt] = *reinterpret_cast<const vec*>(at + static_cast<int64_t>(dt) * 16 * page_size);
-		}
-	};
-
-	// two steps in turn: one's loads in flight under the other's arithmetic, the page numbers a step ahead of the loads
-	step_data d0, d1;
 	constexpr int stride = STEP * WAVES;
 	int base			 = first_key + wave * STEP;
-	load_pages(base, d0);
-	load_pages(base + stride, d1);
+	int lo = page_of(base), hi = page_of(base + 16);
+	load_step(base, lo, hi, 0);
+
 	// q as the B operand: column = row, values 32 s + 8 quarter .. + 7
 	vec q[N][STEPS];
 	float c;
 	{
-		if (!single) {
-			load_q(p.first_row + token, q_head, there);
-		}
+		asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory"); // q is there, the step behind it on its way
+		float x[STEPS][8];
 		float largest = 0.0f;
-		if (base < end_key) {
-			load_step(d0); // (behind q's own loads, ahead of what is done with them)
-		}
+		const char* mine = reinterpret_cast<const char*>(&slots[wave][1][col * Q_PIECES]);
 #pragma unroll
 		for (int s = 0; s < STEPS; ++s) {
+			if constexpr (TYPE == NH_F32) {
 #pragma unroll
-			for (int j = 0; j < 8; ++j) {
-				largest = fmaxf(largest, fabsf(x[s][j]));
-			}
-		}
-		largest		= fmaxf(largest, swap16(largest));
-		largest		= fmaxf(largest, swap32(largest));
-		const int e = q_exponent<CACHE, TYPE>(largest);
+				for (int h = 0; h < 2; ++h) {
+					const v4f v = *reinterpret_cast<const v4f*>(mine + 16 * ((8 * s + 2 * quarter + h) ^ (col & 7)));
 #pragma unroll
-		for (int s = 0; s < STEPS; ++s) {
-			if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
-#pragma unroll
-				for (int j = 0; j < 8; ++j) {
-					x[s][j] = ldexpf(x[s][j], 14 - e);
+					for (int j = 0; j < 4; ++j) {
+						x[s][4 * h + j] = v[j];
+						largest			= fmaxf(largest, fabsf(v[j]));
+					}
 				}
+			} else {
+				q[0][s] = *reinterpret_cast<const vec*>(mine + 16 * ((4 * s + quarter) ^ (col & 7)));
 			}
-			vec t[N];
-			split8<CACHE, N>(x[s], t);
+		}
+		int e = 14;
+		if constexpr (TYPE == NH_F32) {
+			largest		   = fmaxf(largest, swap16(largest));
+			largest		   = fmaxf(largest, swap32(largest));
+			e			   = q_exponent<CACHE, TYPE>(largest);
+			const float up = ldexpf(1.0f, 14 - e);
 #pragma unroll
-			for (int n = 0; n < N; ++n) {
-				q[n][s] = t[n];
+			for (int s = 0; s < STEPS; ++s) {
+				if constexpr (CACHE == NH_F16) {
+#pragma unroll
+					for (int j = 0; j < 8; ++j) {
+						x[s][j] *= up;
+					}
+				}
+				vec t[N];
+				split8<CACHE, N>(x[s], t);
+#pragma unroll
+				for (int n = 0; n < N; ++n) {
+					q[n][s] = t[n];
+				}
 			}
 		}
 		c = ldexpf(a.scale * LOG2_E, e - 14);
@@ -386,23 +417,32 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		o[t] = v4f{};
 	}
 	float m = -__builtin_inff(), l = 0.0f;
-	auto compute = [&](step_data& d) {
+	auto compute = [&](int base, int lo, int hi, int slot) {
+		const v4u* keys	  = &slots[wave][slot][0];
+		const v4u* values = &slots[wave][slot][STEP * PIECES];
 		v4f s[2];
 #pragma unroll
 		for (int t = 0; t < 2; ++t) {
+			const int r = 8 * (col >> 2) + 4 * t + (col & 3), swizzle = (r & 3) | ((r >> 1) & 4);
 			s[t] = v4f{};
 #pragma unroll
 			for (int st = 0; st < STEPS; ++st) {
+				const vec k = __builtin_bit_cast(vec, keys[r * PIECES + ((4 * st + quarter) ^ swizzle)]);
 #pragma unroll
 				for (int n = N - 1; n >= 0; --n) { // the small terms first
-					s[t] = H::mfma16(d.k[t][st], q[n][st], s[t]);
+					s[t] = H::mfma16(k, q[n][st], s[t]);
 				}
 			}
 		}
-		const bool lo = page_there(d.page_lo), hi = page_there(d.page_hi);
-		if (d.base + STEP > min(all_seen, end_key) || !lo || !hi) {
-			const int from	= d.base + 8 * quarter; // the lane's keys are from .. from + 7, of its scores and of its values
-			const bool page = quarter & 2 ? hi : lo;
+		vec v[DT];
+#pragma unroll
+		for (int dt = 0; dt < DT; ++dt) {
+			const int d = 16 * dt + col;
+			v[dt]		= __builtin_bit_cast(vec, values[4 * d + (quarter ^ ((d >> 1) & 3))]);
+		}
+		if (base + STEP > min(all_seen, end_key) || lo < 0 || hi < 0) {
+			const int from	= base + 8 * quarter; // the lane's keys are from .. from + 7, of its scores and of its values
+			const bool page = (quarter & 2 ? hi : lo) >= 0;
 			const int n = page ? min(seen, end_key) - from : 0, n_all = page ? end_key - from : 0; // so many of them are its row's, some row's
 #pragma unroll
 			for (int t = 0; t < 2; ++t) {
@@ -411,23 +451,23 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 					s[t][i] = 4 * t + i < n ? s[t][i] : -__builtin_inff();
 				}
 			}
+			v4u keep; // no values of the others either, whatever lies there (a weight of zero times infinity is not zero)
 #pragma unroll
-			for (int dt = 0; dt < DT; ++dt) { // no values of the others either, whatever lies there (a weight of zero times infinity is not zero)
-				v4u v = __builtin_bit_cast(v4u, d.v[dt]);
+			for (int x = 0; x < 4; ++x) {
+				keep[x] = n_all >= 2 * x + 2 ? 0xFFFFFFFFu : n_all == 2 * x + 1 ? 0xFFFFu : 0u;
+			}
 #pragma unroll
-				for (int x = 0; x < 4; ++x) {
-					v[x] = n_all >= 2 * x + 2 ? v[x] : n_all == 2 * x + 1 ? v[x] & 0xFFFFu : 0u;
-				}
-				d.v[dt] = __builtin_bit_cast(vec, v);
+			for (int dt = 0; dt < DT; ++dt) {
+				v[dt] = __builtin_bit_cast(vec, __builtin_bit_cast(v4u, v[dt]) & keep);
 			}
 		}
 		float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
 		top		  = fmaxf(top, swap16(top));
 		top		  = fmaxf(top, swap32(top)) * c;
 		const float m_new = fmaxf(m, top);
-		const float base  = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
+		const float below = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
 		if (__builtin_amdgcn_ballot_w64(m_new != m)) {
-			const float f = exp2_fast(m - base);
+			const float f = exp2_fast(m - below);
 			l *= f;
 #pragma unroll
 			for (int t = 0; t < DT; ++t) {
@@ -435,7 +475,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			}
 			m = m_new;
 		}
-		const float shift = weight_bias<CACHE> - base;
+		const float shift = weight_bias<CACHE> - below;
 		float x[8];
 #pragma unroll
 		for (int j = 0; j < 8; ++j) {
@@ -448,32 +488,32 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
 			for (int n = N - 1; n >= 0; --n) {
-				o[dt] = H::mfma16(d.v[dt], t[n], o[dt]);
+				o[dt] = H::mfma16(v[dt], t[n], o[dt]);
 			}
 		}
 	};
 
-	while (base < end_key) {
-		if (base + stride < end_key) {
-			load_step(d1);
+	// a step's transfers in flight under the arithmetic of the one before
+	for (int slot = 0; base < end_key; slot ^= 1) {
+		const int next = base + stride, next_lo = page_of(next), next_hi = page_of(next + 16);
+		if (next < end_key) {
+			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // what was in the other slot has been read
+			load_step(next, next_lo, next_hi, slot ^ 1);
+			asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory"); // loads complete in order: those of this step have
+		} else {
+			asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 		}
-		compute(d0);
-		load_pages(base + 2 * stride, d0);
-		base += stride;
-		if (base >= end_key) {
-			break;
-		}
-		if (base + stride < end_key) {
-			load_step(d0);
-		}
-		compute(d1);
-		load_pages(base + 2 * stride, d1);
-		base += stride;
+		compute(base, lo, hi, slot);
+		base = next, lo = next_lo, hi = next_hi;
 	}
+	wait_stores_acknowledged(); // (a wave without a step has one on its way all the same)
 
 	// the four waves' results into one: a thread takes four values of a row at a time
+	v4f(*join_o)[DT][64] = reinterpret_cast<v4f(*)[DT][64]>(&slots[0][0][0]);
+	static_assert(sizeof(v4f) * WAVES * DT * 64 <= sizeof(slots), "the waves' results fit where the keys were");
 	l += swap16(l);
 	l += swap32(l);
+	__syncthreads(); // (every wave is through with its slots)
 #pragma unroll
 	for (int dt = 0; dt < DT; ++dt) {
 		join_o[wave][dt][lane] = o[dt];
@@ -540,8 +580,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	}
 	// Joins the row group's pieces, those over the shared prefix first: D / 4 threads to a row, the pieces of few rows over what threads are left.
 	constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
-	running* parts		= reinterpret_cast<running*>(&join_o[0][0][0]); // [GROUPS][LANES], 24 (32 aligned) bytes each
-	static_assert(sizeof(running) * THREADS <= sizeof(join_o), "the parts of the join fit where the waves' results were");
+	running* parts		= reinterpret_cast<running*>(&slots[0][0][0]); // [GROUPS][LANES]
+	static_assert(sizeof(running) * THREADS <= sizeof(slots), "the parts of the join fit where the waves' results were");
 	const int part = tid % LANES, g = tid / LANES;
 	const int rows_at_once = count <= 1 ? 1 : count <= 2 ? 2 : count <= 4 ? 4 : 8; // a divisor of GROUPS
 	const int ways = GROUPS / rows_at_once, way = g / rows_at_once;
@@ -549,7 +589,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	for (int r0 = 0; r0 < count; r0 += rows_at_once) {
 		const int r		  = r0 + g % rows_at_once;
 		const bool mine	  = r < count;
-		const int tok	  = (first + min(r, count - 1)) / group;
+		const int tok	  = token_of(min(r, count - 1));
 		const int q_h	  = head * group + first + min(r, count - 1) - tok * group;
 		running sum{ -__builtin_inff(), 0.0f, v4f{} };
 		if (mine) {
@@ -612,9 +652,12 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 	// no row group has more pieces than its table has keys for
 	const int64_t row_groups = cut.pieces - cut.units, keys = static_cast<int64_t>(a.batch.width) << a.cache.page_shift;
 	const int64_t pieces	 = std::min(cut.pieces, row_groups * std::max<int64_t>(1, (keys + STEP * WAVES - 1) / (STEP * WAVES)));
-	attention_rows_kernel<CACHE, TYPE, D>
-		<<<dim3(static_cast<unsigned>(pieces * a.cache.kv_heads)), dim3(THREADS), 0, s>>>(a.batch.lengths, a.batch.starts, a.batch.table, a.batch.sequences, a.batch.width, a.rows, a.q_heads,
-			a.cache.kv_heads, a.cache.page_shift, a.prefix_count, static_cast<int>(cut.units), std::max(1, AT_ONCE / a.cache.kv_heads), a, w);
+	const int64_t y			 = std::min<int64_t>(pieces, 32768), z = (pieces + y - 1) / y;
+	const bool one_each = a.batch.starts == nullptr;
+	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), static_cast<unsigned>(y), static_cast<unsigned>(z)), dim3(THREADS), 0, s>>>(a.batch.lengths,
+		a.batch.width > 0 ? a.batch.table : a.batch.lengths, a.q, a.cache.k, a.cache.v,
+		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | static_cast<uint32_t>(cut.units_log2) << 25 | (one_each ? 1u << 31 : 0u), a.batch.width,
+		a.prefix_count, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, a, w);
 	return hipGetLastError();
 }
 template<int CACHE, int TYPE> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
