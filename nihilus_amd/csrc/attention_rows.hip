@@ -32,7 +32,7 @@ constexpr int COLUMNS	 = 16; // rows of a row group
 // What the pieces are cut for: twice what the chip holds at once (two per CU), so that the last ones to start are short.  decode of 64 sequences of up to 8192 keys
 // (32 / 8 heads): 512 61.5 us, 1024 55.4, 2048 60.0, 4096 68.5.
 constexpr int WORKGROUPS = 1024;
-constexpr int AT_ONCE		= 256; // workgroups that the chip holds at once
+constexpr int AT_ONCE		= 512; // workgroups that the chip holds at once
 constexpr int SHORT_LENGTHS = 4; // short pieces are of 1, 2, 4 or 8 steps for each wave
 constexpr int64_t MOST_SHORT = (int64_t{ WAVES } << (SHORT_LENGTHS - 1)) * WORKGROUPS; // more steps than that make long pieces
 
@@ -246,7 +246,7 @@ struct running {
 } // namespace
 
 template<int CACHE, int TYPE, int D>
-__global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const uint16_t* v_pages,
+__global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const uint16_t* v_pages,
 	uint32_t shape, int width, int prefix_count, uint32_t heads, attention_args a, rows_workspace w) {
 	// What the first loads take comes first, in fourteen dwords: those arrive in registers, the rest is read from memory, as far away as the data.
 	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | one row per sequence << 31
@@ -263,7 +263,9 @@ __global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_
 	constexpr int PIECES = D / 8; // 16-byte pieces of a key
 	constexpr int LOADS	 = STEP * PIECES / 64; // instructions for a step's keys, and for its values
 	constexpr int SLOT	 = 2 * STEP * PIECES; // pieces of a step
-	__shared__ v4u slots[WAVES][2][SLOT];
+	constexpr int Q_PIECES = TYPE == NH_F32 ? D / 4 : D / 8; // of a row of q
+	__shared__ v4u slots[WAVES][SLOT];
+	__shared__ v4u q_share[COLUMNS * Q_PIECES];
 	__shared__ float2 join_ml[WAVES][COLUMNS];
 	__shared__ int is_last;
 
@@ -274,16 +276,17 @@ __global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_
 	const int prefix_keys = prefix_count << page_shift, held = width << page_shift;
 	const int piece		  = blockIdx.z * gridDim.y + blockIdx.y;
 
-	// The row group's q goes into the second slot, which is not needed before the second step: as many 16-byte pieces of a row as it has, piece x of row r
-	// at x ^ (r % 8).  Columns past the last row hold that one again; their results go nowhere.
-	constexpr int Q_PIECES = TYPE == NH_F32 ? D / 4 : D / 8;
-	auto load_q			   = [&](int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
+	// The row group's q, a part by each wave: piece x of row r at x ^ (r % 8).  Columns past the last row hold that one again; their results go nowhere.
+	auto load_q = [&](int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
 #pragma unroll
-		for (int j = 0; j < COLUMNS * Q_PIECES / 64; ++j) {
-			const int at = 64 * j + lane, r = at / Q_PIECES, x = (at % Q_PIECES) ^ (r & 7);
-			const int i = rest + min(r, rows - 1), tok = static_cast<int>((static_cast<float>(i) + 0.5f) * inverse);
-			const int64_t from = (row0 + tok == 0 ? 0 : (row0 + tok) * a.q_stride) + static_cast<int64_t>(head0 + i - tok * group) * D;
-			load_global_to_lds_b128(static_cast<const char*>(q_rows) + from * (TYPE == NH_F32 ? 4 : 2) + 16 * x, &slots[wave][1][64 * j]);
+		for (int j = 0; j < (COLUMNS * Q_PIECES / 64 + WAVES - 1) / WAVES; ++j) {
+			const int part = j * WAVES + wave;
+			if (part < COLUMNS * Q_PIECES / 64) {
+				const int at = 64 * part + lane, r = at / Q_PIECES, x = (at % Q_PIECES) ^ (r & 7);
+				const int i = rest + min(r, rows - 1), tok = static_cast<int>((static_cast<float>(i) + 0.5f) * inverse);
+				const int64_t from = (row0 + tok == 0 ? 0 : (row0 + tok) * a.q_stride) + static_cast<int64_t>(head0 + i - tok * group) * D;
+				load_global_to_lds_b128(static_cast<const char*>(q_rows) + from * (TYPE == NH_F32 ? 4 : 2) + 16 * x, &q_share[64 * part]);
+			}
 		}
 	};
 	const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
@@ -342,34 +345,35 @@ __global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_
 	// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).  Eight
 	// lanes that read the same piece of eight operand rows hit different banks: K rows differ in bits 0, 1, 3, V rows in bits 0 .. 2.
 	const int64_t page_values = static_cast<int64_t>(kv_heads) * D << page_shift, head_values = static_cast<int64_t>(head) * D << page_shift;
-	auto load_step			  = [&](int base, int lo, int hi, int slot) {
+	auto load_step			  = [&](int base, int lo, int hi) {
 		 const int64_t lo_at = max(lo, 0) * page_values + head_values, hi_at = max(hi, 0) * page_values + head_values;
 #pragma unroll
 		 for (int j = 0; j < LOADS; ++j) {
 			 const int at = 64 * j + lane, r = at / PIECES, x = (at % PIECES) ^ ((r & 3) | ((r >> 1) & 4));
 			 const int key = (base + r) & (page_size - 1);
-			 load_global_to_lds_b128(k_pages + (2 * j < LOADS ? lo_at : hi_at) + key * D + 8 * x, &slots[wave][slot][64 * j]);
+			 load_global_to_lds_b128(k_pages + (2 * j < LOADS ? lo_at : hi_at) + key * D + 8 * x, &slots[wave][64 * j]);
 		 }
 #pragma unroll
 		 for (int j = 0; j < LOADS; ++j) {
 			 const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 1) & 3);
 			 const int key = (base + 8 * x) & (page_size - 1);
-			 load_global_to_lds_b128(v_pages + (x & 2 ? hi_at : lo_at) + d * page_size + key, &slots[wave][slot][STEP * PIECES + 64 * j]);
+			 load_global_to_lds_b128(v_pages + (x & 2 ? hi_at : lo_at) + d * page_size + key, &slots[wave][STEP * PIECES + 64 * j]);
 		 }
 	};
 	constexpr int stride = STEP * WAVES;
 	int base			 = first_key + wave * STEP;
 	int lo = page_of(base), hi = page_of(base + 16);
-	load_step(base, lo, hi, 0);
+	load_step(base, lo, hi);
 
 	// q as the B operand: column = row, values 32 s + 8 quarter .. + 7
 	vec q[N][STEPS];
 	float c;
 	{
-		asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory"); // q is there, the step behind it on its way
+		asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory"); // this wave's part of q is there, the step behind it on its way
+		__syncthreads();
 		float x[STEPS][8];
 		float largest = 0.0f;
-		const char* mine = reinterpret_cast<const char*>(&slots[wave][1][col * Q_PIECES]);
+		const char* mine = reinterpret_cast<const char*>(&q_share[col * Q_PIECES]);
 #pragma unroll
 		for (int s = 0; s < STEPS; ++s) {
 			if constexpr (TYPE == NH_F32) {
@@ -417,28 +421,37 @@ __global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_
 		o[t] = v4f{};
 	}
 	float m = -__builtin_inff(), l = 0.0f;
-	auto compute = [&](int base, int lo, int hi, int slot) {
-		const v4u* keys	  = &slots[wave][slot][0];
-		const v4u* values = &slots[wave][slot][STEP * PIECES];
-		v4f s[2];
+	// A step's operands: out of the slot into registers, so that the next step can be on its way into the slot under this one's arithmetic.
+	vec k[2][STEPS], v[DT];
+	auto read_step = [&] {
+		const v4u* keys	  = &slots[wave][0];
+		const v4u* values = &slots[wave][STEP * PIECES];
 #pragma unroll
 		for (int t = 0; t < 2; ++t) {
 			const int r = 8 * (col >> 2) + 4 * t + (col & 3), swizzle = (r & 3) | ((r >> 1) & 4);
-			s[t] = v4f{};
 #pragma unroll
 			for (int st = 0; st < STEPS; ++st) {
-				const vec k = __builtin_bit_cast(vec, keys[r * PIECES + ((4 * st + quarter) ^ swizzle)]);
-#pragma unroll
-				for (int n = N - 1; n >= 0; --n) { // the small terms first
-					s[t] = H::mfma16(k, q[n][st], s[t]);
-				}
+				k[t][st] = __builtin_bit_cast(vec, keys[r * PIECES + ((4 * st + quarter) ^ swizzle)]);
 			}
 		}
-		vec v[DT];
 #pragma unroll
 		for (int dt = 0; dt < DT; ++dt) {
 			const int d = 16 * dt + col;
 			v[dt]		= __builtin_bit_cast(vec, values[4 * d + (quarter ^ ((d >> 1) & 3))]);
+		}
+	};
+	auto compute = [&](int base, int lo, int hi) {
+		v4f s[2];
+#pragma unroll
+		for (int t = 0; t < 2; ++t) {
+			s[t] = v4f{};
+#pragma unroll
+			for (int st = 0; st < STEPS; ++st) {
+#pragma unroll
+				for (int n = N - 1; n >= 0; --n) { // the small terms first
+					s[t] = H::mfma16(k[t][st], q[n][st], s[t]);
+				}
+			}
 		}
 		if (base + STEP > min(all_seen, end_key) || lo < 0 || hi < 0) {
 			const int from	= base + 8 * quarter; // the lane's keys are from .. from + 7, of its scores and of its values
@@ -493,23 +506,22 @@ __global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_
 		}
 	};
 
-	// a step's transfers in flight under the arithmetic of the one before
-	for (int slot = 0; base < end_key; slot ^= 1) {
+	while (base < end_key) {
 		const int next = base + stride, next_lo = page_of(next), next_hi = page_of(next + 16);
+		asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the step is in the slot
+		read_step();
+		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // ... and out of it
+		__builtin_amdgcn_sched_barrier(0);
 		if (next < end_key) {
-			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // what was in the other slot has been read
-			load_step(next, next_lo, next_hi, slot ^ 1);
-			asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory"); // loads complete in order: those of this step have
-		} else {
-			asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+			load_step(next, next_lo, next_hi);
 		}
-		compute(base, lo, hi, slot);
+		compute(base, lo, hi);
 		base = next, lo = next_lo, hi = next_hi;
 	}
 	wait_stores_acknowledged(); // (a wave without a step has one on its way all the same)
 
 	// the four waves' results into one: a thread takes four values of a row at a time
-	v4f(*join_o)[DT][64] = reinterpret_cast<v4f(*)[DT][64]>(&slots[0][0][0]);
+	v4f(*join_o)[DT][64] = reinterpret_cast<v4f(*)[DT][64]>(&slots[0][0]);
 	static_assert(sizeof(v4f) * WAVES * DT * 64 <= sizeof(slots), "the waves' results fit where the keys were");
 	l += swap16(l);
 	l += swap32(l);
@@ -580,7 +592,7 @@ __global__ __launch_bounds__(THREADS, 1) void attention_rows_kernel(const int32_
 	}
 	// Joins the row group's pieces, those over the shared prefix first: D / 4 threads to a row, the pieces of few rows over what threads are left.
 	constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
-	running* parts		= reinterpret_cast<running*>(&slots[0][0][0]); // [GROUPS][LANES]
+	running* parts		= reinterpret_cast<running*>(&slots[0][0]); // [GROUPS][LANES]
 	static_assert(sizeof(running) * THREADS <= sizeof(slots), "the parts of the join fit where the waves' results were");
 	const int part = tid % LANES, g = tid / LANES;
 	const int rows_at_once = count <= 1 ? 1 : count <= 2 ? 2 : count <= 4 ? 4 : 8; // a divisor of GROUPS
