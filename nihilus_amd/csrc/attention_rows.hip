@@ -34,6 +34,7 @@ constexpr int COLUMNS	 = 16; // rows of a row group
 constexpr int WORKGROUPS = 1024;
 constexpr int AT_ONCE		= 512; // workgroups that the chip holds at once
 constexpr int SHORT_LENGTHS = 4; // short pieces are of 1, 2, 4 or 8 steps for each wave
+constexpr int SHORT_WORK	= 4 * WAVES; // steps for each workgroup that the chip holds, up to which pieces are short
 constexpr int64_t MOST_SHORT = (int64_t{ WAVES } << (SHORT_LENGTHS - 1)) * WORKGROUPS; // more steps than that make long pieces
 
 struct rows_workspace {
@@ -114,7 +115,8 @@ __device__ __forceinline__ sequence_size size_of(const batch_view& b, int all_ro
 struct piece_place {
 	int seq, first_row, rows, pos0; // pos0: position of the sequence's first row
 	int row_group, index; // this piece is piece `index` of that row group
-	int stride; // pieces of the sequence's row groups lie so far apart
+	int row_groups, whole; // the sequence's row groups, and whole pieces of each
+	int first_whole, first_rest; // numbers of the sequence's first whole piece, and of its first rest of a piece
 	int length; // keys of a piece
 	bool there;
 };
@@ -124,7 +126,7 @@ __device__ __forceinline__ int sum64(int x) {
 // How long a piece is, in steps: see place_of_piece.
 __device__ __forceinline__ int piece_steps(int64_t total, const int (&pieces)[SHORT_LENGTHS], int units_log2, int fit) {
 	const int64_t steps = (total + (int64_t{ 1 } << units_log2) - 1) >> units_log2;
-	if (steps <= WAVES << (SHORT_LENGTHS - 1)) {
+	if (total <= static_cast<int64_t>(fit) * SHORT_WORK && steps <= WAVES << (SHORT_LENGTHS - 1)) {
 #pragma unroll
 		for (int i = 0; i < SHORT_LENGTHS; ++i) {
 			if (steps <= WAVES << i && (i == SHORT_LENGTHS - 1 || pieces[i] <= fit)) {
@@ -134,9 +136,11 @@ __device__ __forceinline__ int piece_steps(int64_t total, const int (&pieces)[SH
 	}
 	return (static_cast<int>(min(steps, (int64_t{ 1 } << 25) - WAVES)) + WAVES - 1) & -WAVES; // (2^30 keys are all that a table holds)
 }
-// Piece `t` of the batch.  Every wave adds the work up by itself, 64 sequences at a time.  A piece is `units`th of the work long, but not so short
+// Piece `t` of the batch.  Every wave adds the work up by itself, 64 sequences at a time.  A piece is one `units`th of the work long, but not so short
 // that the pieces do not fit on the chip at once (`fit`) when a piece of twice the length is still short: a workgroup takes some 5 us
-// before and behind its steps, a step 0.6.
+// before and behind its steps, a step 0.6.  The whole pieces of all sequences come first and what is left of each sequence behind them (the whole
+// sequence, if it is shorter than a piece; a piece without keys, if it has none), so that the workgroups that start last have the least to do.
+// Pieces of a sequence's row groups lie side by side: they read the same keys.
 __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int all_rows, int group, int prefix_keys, int held, int units_log2, int fit, int t) {
 	const int lane = threadIdx.x & 63;
 	piece_place p{};
@@ -149,11 +153,12 @@ __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int a
 			pieces[i] = groups * max(1, (steps + (WAVES << i) - 1) / (WAVES << i));
 		}
 		p.first_row = z.first_row, p.rows = z.rows, p.pos0 = z.pos0;
-		p.stride	= max(groups, 1);
-		p.index		= p.stride == 1 ? t : t / p.stride;
-		p.row_group = t - p.index * p.stride;
-		p.length	= piece_steps(static_cast<int64_t>(groups) * steps, pieces, units_log2, fit) * STEP;
-		p.there		= groups > 0;
+		p.row_groups = max(groups, 1);
+		p.index		 = groups <= 1 ? t : t / groups;
+		p.row_group	 = t - p.index * p.row_groups;
+		p.length	 = piece_steps(static_cast<int64_t>(groups) * steps, pieces, units_log2, fit) * STEP;
+		p.whole		 = 1 << 30; // (one after the other, whole or not)
+		p.there		 = groups > 0;
 		return p;
 	}
 	int64_t total  = 0; // steps
@@ -177,30 +182,42 @@ __device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int a
 		}
 	}
 	const int length = piece_steps(total, pieces, units_log2, fit) * STEP;
-	int before = 0;
+	int whole_pieces = 0; // of all sequences
 	for (int base = 0; base < b.sequences; base += 64) {
 		if (b.sequences > 64) {
 			z = size_of(b, all_rows, prefix_keys, held, base + lane);
 		}
-		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS;
-		const int each	 = max(1, (z.keys + length - 1) / length);
-		const int count = groups * each, upto = scan64(count);
-		const uint64_t over = __builtin_amdgcn_ballot_w64(before + upto > t);
+		whole_pieces += sum64((z.rows * group + COLUMNS - 1) / COLUMNS * (z.keys / length));
+	}
+	int whole_before = 0, rest_before = whole_pieces;
+	for (int base = 0; base < b.sequences; base += 64) {
+		if (b.sequences > 64) {
+			z = size_of(b, all_rows, prefix_keys, held, base + lane);
+		}
+		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS, whole = z.keys / length;
+		const int wholes = groups * whole, rests = z.keys > whole * length || whole == 0 ? groups : 0;
+		const int whole_upto = scan64(wholes), rest_upto = scan64(rests);
+		const bool in_whole = t < whole_pieces;
+		const uint64_t over = __builtin_amdgcn_ballot_w64(in_whole ? whole_before + whole_upto > t : rest_before + rest_upto > t);
 		if (over) {
 			const int src = __builtin_ctzll(over);
 			p.seq		  = base + src;
 			p.first_row	  = __builtin_amdgcn_readlane(z.first_row, src);
 			p.rows		  = __builtin_amdgcn_readlane(z.rows, src);
 			p.pos0		  = __builtin_amdgcn_readlane(z.pos0, src);
-			p.stride	  = __builtin_amdgcn_readlane(groups, src);
-			const int k	  = t - before - (__builtin_amdgcn_readlane(upto, src) - __builtin_amdgcn_readlane(count, src));
-			p.index		  = p.stride == 1 ? k : k / p.stride;
-			p.row_group	  = k - p.index * p.stride; // row groups side by side: they read the same keys
+			p.row_groups  = __builtin_amdgcn_readlane(groups, src);
+			p.whole		  = __builtin_amdgcn_readlane(whole, src);
+			p.first_whole = whole_before + __builtin_amdgcn_readlane(whole_upto, src) - __builtin_amdgcn_readlane(wholes, src);
+			p.first_rest  = rest_before + __builtin_amdgcn_readlane(rest_upto, src) - __builtin_amdgcn_readlane(rests, src);
+			const int k	  = t - (in_whole ? p.first_whole : p.first_rest);
+			p.index		  = !in_whole ? p.whole : p.row_groups == 1 ? k : k / p.row_groups;
+			p.row_group	  = in_whole ? k - p.index * p.row_groups : k;
 			p.length	  = length;
 			p.there		  = true;
 			return p;
 		}
-		before += __builtin_amdgcn_readlane(upto, 63);
+		whole_before += __builtin_amdgcn_readlane(whole_upto, 63);
+		rest_before += __builtin_amdgcn_readlane(rest_upto, 63);
 	}
 	return p;
 }
@@ -571,7 +588,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	if (alone) {
 		return;
 	}
-	const int64_t first_slot = slot - static_cast<int64_t>(p.index) * p.stride * kv_heads;
+	// the slot of piece i of this row group
+	auto slot_of = [&](int i) {
+		return static_cast<int64_t>(i < p.whole ? p.first_whole + i * p.row_groups + p.row_group : p.first_rest + p.row_group) * kv_heads + head;
+	};
+	const int64_t first_slot = slot_of(0);
 	if (pieces > 1) {
 		wait_stores_acknowledged();
 		__syncthreads();
@@ -615,7 +636,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 					const int i		  = min(i0 + k * ways, all - 1); // (past the last one: the last one again, not added)
 					const bool shared = i < w.prefix_pieces;
 					const int64_t at  = shared ? (static_cast<int64_t>(i) * sequences + p.seq) * q_heads + q_h
-											   : (first_slot + static_cast<int64_t>(i - w.prefix_pieces) * p.stride * kv_heads) * w.columns + r;
+											   : slot_of(i - w.prefix_pieces) * w.columns + r;
 					ml[k]			  = (shared ? w.prefix_ml : w.ml) + at;
 					o4[k]			  = (shared ? w.prefix_o : w.o) + at * D + 4 * part;
 				}
