@@ -143,7 +143,7 @@ static int check_heads(int64_t rows, int64_t sequences, int64_t q_heads, int64_t
 
 int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes) {
 	NH_TRY(check_heads(rows, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
-	const nh::rows_needs n = nh::prompt_by_rows(rows, sequences, q_heads, kv_heads) ? nh::attention_rows_needs(rows, sequences, false, q_heads, kv_heads, head_dim, 0) : nh::rows_needs{ 0, 0 };
+	const nh::rows_needs n = nh::prompt_by_rows(rows, sequences, q_heads, kv_heads) ? nh::attention_rows_needs(sequences, false, q_heads, kv_heads, head_dim, 0) : nh::rows_needs{ 0, 0 };
 	*host_workspace_bytes  = n.workspace;
 	*host_counter_bytes	   = n.counters;
 	return NH_OK;
@@ -164,7 +164,9 @@ int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 	nh::attention_args a = attention(host_cache, host_batch, q, out, rows, q_heads, q_stride, scale);
 	a.workspace			 = workspace;
 	a.counters			 = static_cast<int32_t*>(counters);
-	const bool by_rows	 = nh::prompt_by_rows(rows, host_batch->sequences, q_heads, host_cache->kv_heads);
+	// (few rows against tables of a billion keys: more work than the rows kernel can number)
+	const bool by_rows = nh::prompt_by_rows(rows, host_batch->sequences, q_heads, host_cache->kv_heads) &&
+		nh::attention_rows_fit(rows, host_batch->sequences, false, q_heads / host_cache->kv_heads, host_batch->table_width * host_cache->page_size);
 	return from_hip(by_rows ? nh::launch_attention_rows(a, host_cache->type, type, as_stream(stream)) : nh::launch_attention_tiles(a, host_cache->type, type, as_stream(stream)));
 }
 
@@ -182,7 +184,7 @@ int nh_attn_decode_needs(int64_t sequences, int64_t q_heads, int64_t kv_heads, i
 	NH_TRY(check_heads(sequences, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
 	NH_REQUIRE(prefix_count >= 0 && page_shift(page_size) > 0, NH_ERR_SHAPE);
 	NH_REQUIRE(prefix_count <= MAX_KEYS / page_size, NH_ERR_TOO_LARGE);
-	const nh::rows_needs n = nh::attention_rows_needs(sequences, sequences, true, q_heads, kv_heads, head_dim, prefix_count * page_size);
+	const nh::rows_needs n = nh::attention_rows_needs(sequences, true, q_heads, kv_heads, head_dim, prefix_count * page_size);
 	*host_workspace_bytes  = n.workspace;
 	*host_counter_bytes	   = n.counters;
 	return NH_OK;
@@ -193,6 +195,7 @@ int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 	NH_REQUIRE(host_batch, NH_ERR_NULL_POINTER);
 	NH_TRY(check_attention(host_cache, host_batch, type, host_batch->sequences, q_heads, q_stride, scale));
 	NH_REQUIRE(!host_batch->starts, NH_ERR_ARGUMENT);
+	NH_REQUIRE(nh::attention_rows_fit(host_batch->sequences, host_batch->sequences, true, q_heads / host_cache->kv_heads, host_batch->table_width * host_cache->page_size), NH_ERR_TOO_LARGE);
 	int64_t need = 0, counter_need = 0;
 	NH_TRY(nh_attn_decode_needs(host_batch->sequences, q_heads, host_cache->kv_heads, host_cache->head_dim, prefix_count, host_cache->page_size, &need, &counter_need));
 	if (host_batch->sequences == 0) {

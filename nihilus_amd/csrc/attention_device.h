@@ -188,7 +188,9 @@ hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int 
 struct rows_needs {
 	int64_t workspace, counters; // bytes
 };
-rows_needs attention_rows_needs(int64_t rows, int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
+rows_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
+// whether all work, in steps of 32 keys, surely has a 32-bit number (table_keys: what a sequence's table has room for)
+bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t table_keys);
 hipError_t launch_attention_rows(const attention_args& a, int cache_type, int type, hipStream_t s);
 // Which of the two a prompt's rows take (attention_abi.hip).
 bool prompt_by_rows(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads);

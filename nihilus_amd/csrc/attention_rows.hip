@@ -11,10 +11,12 @@
 // of K are put so that the lane holds the scores that it has to supply as P^T: result rows 4 (l / 16) + i of the two key tiles of a step are keys
 // 8 (l / 16) + 4 tile + i, so operand row m of tile t takes key 8 (m / 4) + 4 t + m % 4.
 //
-// Work: the sequences' keys are cut into pieces of the same length, worked out on the GPU from the lengths (by every wave for itself), so that
-// WORKGROUPS workgroups have about the same work, however the lengths differ.  A piece's four waves take its steps of 32 keys in turn
-// and join their results in LDS.  Where a row group has more pieces than one, each puts its result into the workspace and counts itself; the last
-// to do so joins them, in the pieces' order, so the result does not hang on who that is.
+// Work: the row groups of all sequences, each as many steps of 32 keys as its sequence has, stand in a row, and every workgroup takes an equal
+// stretch of it, worked out on the GPU from the lengths (by every wave for itself): all workgroups are on the chip at once and end together,
+// however the lengths differ.  (Pieces of one length, a workgroup each, were 15 to 30 % slower: a workgroup takes some 5 us before its first step and behind
+// its last, two or three times over, and the last ones run alone.)  A workgroup's four waves take the steps of a row group in turn and
+// join their results in LDS.  Where a row group has been cut, each workgroup puts its result into the workspace and counts itself; the last to do so
+// joins them, in the pieces' order, so the result does not hang on who that is.
 // A prefix that all sequences share is left to the tile kernel, whose rows are then the heads of all sequences; its pieces are
 // joined with the sequences' own.
 #include "attention_device.h"
@@ -29,36 +31,31 @@ constexpr int WAVES		 = 4;
 constexpr int THREADS	 = 64 * WAVES;
 constexpr int STEP		 = 32; // keys of a wave's step
 constexpr int COLUMNS	 = 16; // rows of a row group
-// What the pieces are cut for: twice what the chip holds at once (two per CU), so that the last ones to start are short.  decode of 64 sequences of up to 8192 keys
-// (32 / 8 heads): 512 61.5 us, 1024 55.4, 2048 60.0, 4096 68.5.
-constexpr int WORKGROUPS = 1024;
-constexpr int AT_ONCE		= 512; // workgroups that the chip holds at once
-constexpr int SHORT_LENGTHS = 4; // short pieces are of 1, 2, 4 or 8 steps for each wave
-constexpr int SHORT_WORK	= 4 * WAVES; // steps for each workgroup that the chip holds, up to which pieces are short
-constexpr int64_t MOST_SHORT = (int64_t{ WAVES } << (SHORT_LENGTHS - 1)) * WORKGROUPS; // more steps than that make long pieces
+constexpr int WORKGROUPS = 512; // that the chip holds at once: two per CU
+// What a row group takes beside its steps (its q, its first step's way, the joins), in steps.
+constexpr int FIXED = 12;
 
 struct rows_workspace {
-	float* o; // [slot][columns][D]  a piece's sums of weighted values; slot = piece * kv_heads + kv head
-	float2* ml; // [slot][columns]  their maximum (log2) and the sum of the weights
+	// [slot][columns][D]  a piece's sums of weighted values, and [slot][columns] their maximum (log2) and the sum of the weights; slot = (2 * unit + (1 if the
+	// piece is the first of its row group and does not begin with the unit)) * kv_heads + kv head
+	float* o;
+	float2* ml;
 	float* prefix_o; // [prefix piece][sequences][q_heads][D]
 	float2* prefix_ml;
 	int columns;
 	int prefix_pieces;
-	int32_t* counters; // [slot]  of a row group's first piece: how many of its pieces are done; zero before and after every call
+	int32_t* counters; // [unit][kv_heads]  of the unit that a cut row group begins in: how many of its pieces are done; zero before and after every call
 };
 struct rows_cut {
-	int64_t units; // pieces that the keys are cut into at most, beside one per row group: a power of two
-	int units_log2;
-	int64_t pieces; // most pieces there can be
+	int64_t units; // workgroups per kv head: a power of two
 	int64_t columns; // rows of a row group that are kept in the workspace
 };
-rows_cut plan_rows(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t kv_heads) {
+rows_cut plan_rows(bool one_each, int64_t group, int64_t kv_heads) {
 	rows_cut c{};
-	while ((int64_t{ 2 } << c.units_log2) * kv_heads <= WORKGROUPS) {
-		++c.units_log2;
+	c.units = 1;
+	while (2 * c.units * kv_heads <= WORKGROUPS) {
+		c.units *= 2;
 	}
-	c.units	  = int64_t{ 1 } << c.units_log2;
-	c.pieces  = c.units + (one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : rows * group / COLUMNS + sequences);
 	c.columns = one_each ? std::min<int64_t>(group, COLUMNS) : COLUMNS;
 	return c;
 }
@@ -74,7 +71,7 @@ int64_t lay_out(char* base, const rows_cut& c, const prefix_cut& prefix, int64_t
 		at += rounded(bytes);
 		return p;
 	};
-	const int64_t own = c.pieces * kv_heads * c.columns, shared = prefix.pieces * sequences * q_heads;
+	const int64_t own = 2 * c.units * kv_heads * c.columns, shared = prefix.pieces * sequences * q_heads;
 	w->ml			 = reinterpret_cast<float2*>(part(own * 8));
 	w->o			 = reinterpret_cast<float*>(part(own * head_dim * 4));
 	w->prefix_ml	 = reinterpret_cast<float2*>(part(shared * 8));
@@ -112,115 +109,23 @@ __device__ __forceinline__ sequence_size size_of(const batch_view& b, int all_ro
 	return z;
 }
 
-struct piece_place {
-	int seq, first_row, rows, pos0; // pos0: position of the sequence's first row
-	int row_group, index; // this piece is piece `index` of that row group
-	int row_groups, whole; // the sequence's row groups, and whole pieces of each
-	int first_whole, first_rest; // numbers of the sequence's first whole piece, and of its first rest of a piece
-	int length; // keys of a piece
-	bool there;
-};
 __device__ __forceinline__ int sum64(int x) {
 	return __builtin_amdgcn_readlane(scan64(x), 63);
 }
-// How long a piece is, in steps: see place_of_piece.
-__device__ __forceinline__ int piece_steps(int64_t total, const int (&pieces)[SHORT_LENGTHS], int units_log2, int fit) {
-	const int64_t steps = (total + (int64_t{ 1 } << units_log2) - 1) >> units_log2;
-	if (total <= static_cast<int64_t>(fit) * SHORT_WORK && steps <= WAVES << (SHORT_LENGTHS - 1)) {
-#pragma unroll
-		for (int i = 0; i < SHORT_LENGTHS; ++i) {
-			if (steps <= WAVES << i && (i == SHORT_LENGTHS - 1 || pieces[i] <= fit)) {
-				return WAVES << i;
-			}
-		}
-	}
-	return (static_cast<int>(min(steps, (int64_t{ 1 } << 25) - WAVES)) + WAVES - 1) & -WAVES; // (2^30 keys are all that a table holds)
+// Steps of a row group of a sequence: one, without a key, if it has none.
+__device__ __forceinline__ int steps_of(const sequence_size& z) {
+	return max(1, (z.keys + STEP - 1) / STEP);
 }
-// Piece `t` of the batch.  Every wave adds the work up by itself, 64 sequences at a time.  A piece is one `units`th of the work long, but not so short
-// that the pieces do not fit on the chip at once (`fit`) when a piece of twice the length is still short: a workgroup takes some 5 us
-// before and behind its steps, a step 0.6.  The whole pieces of all sequences come first and what is left of each sequence behind them (the whole
-// sequence, if it is shorter than a piece; a piece without keys, if it has none), so that the workgroups that start last have the least to do.
-// Pieces of a sequence's row groups lie side by side: they read the same keys.
-__device__ __forceinline__ piece_place place_of_piece(const batch_view& b, int all_rows, int group, int prefix_keys, int held, int units_log2, int fit, int t) {
-	const int lane = threadIdx.x & 63;
-	piece_place p{};
-	if (b.sequences == 1) { // nothing to add up, and nothing to wait for but the one length
-		const sequence_size z = size_of(b, all_rows, prefix_keys, held, 0);
-		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS, steps = (z.keys + STEP - 1) / STEP;
-		int pieces[SHORT_LENGTHS];
-#pragma unroll
-		for (int i = 0; i < SHORT_LENGTHS; ++i) {
-			pieces[i] = groups * max(1, (steps + (WAVES << i) - 1) / (WAVES << i));
-		}
-		p.first_row = z.first_row, p.rows = z.rows, p.pos0 = z.pos0;
-		p.row_groups = max(groups, 1);
-		p.index		 = groups <= 1 ? t : t / groups;
-		p.row_group	 = t - p.index * p.row_groups;
-		p.length	 = piece_steps(static_cast<int64_t>(groups) * steps, pieces, units_log2, fit) * STEP;
-		p.whole		 = 1 << 30; // (one after the other, whole or not)
-		p.there		 = groups > 0;
-		return p;
-	}
-	int64_t total  = 0; // steps
-	int pieces[SHORT_LENGTHS] = {}; // that there are with 1, 2, 4, ... steps for each wave
-	sequence_size z;
-	for (int base = 0; base < b.sequences; base += 64) {
-		z				 = size_of(b, all_rows, prefix_keys, held, base + lane);
-		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS, steps = (z.keys + STEP - 1) / STEP;
-		// (a sequence's steps are below 2^25: the sum in halves, each within 32 bits)
-		const int64_t work = static_cast<int64_t>(groups) * steps;
-		total += sum64(static_cast<int>(work & 0xFFFF));
-		if (__builtin_amdgcn_ballot_w64(work > 0xFFFF)) {
-			total += static_cast<int64_t>(sum64(static_cast<int>((work >> 16) & 0xFFFFFF))) << 16;
-			total += static_cast<int64_t>(sum64(static_cast<int>(work >> 40))) << 40;
-		}
-		if (total <= MOST_SHORT) {
-#pragma unroll
-			for (int i = 0; i < SHORT_LENGTHS; ++i) {
-				pieces[i] += sum64(groups * max(1, (steps + (WAVES << i) - 1) / (WAVES << i)));
-			}
-		}
-	}
-	const int length = piece_steps(total, pieces, units_log2, fit) * STEP;
-	int whole_pieces = 0; // of all sequences
-	for (int base = 0; base < b.sequences; base += 64) {
-		if (b.sequences > 64) {
-			z = size_of(b, all_rows, prefix_keys, held, base + lane);
-		}
-		whole_pieces += sum64((z.rows * group + COLUMNS - 1) / COLUMNS * (z.keys / length));
-	}
-	int whole_before = 0, rest_before = whole_pieces;
-	for (int base = 0; base < b.sequences; base += 64) {
-		if (b.sequences > 64) {
-			z = size_of(b, all_rows, prefix_keys, held, base + lane);
-		}
-		const int groups = (z.rows * group + COLUMNS - 1) / COLUMNS, whole = z.keys / length;
-		const int wholes = groups * whole, rests = z.keys > whole * length || whole == 0 ? groups : 0;
-		const int whole_upto = scan64(wholes), rest_upto = scan64(rests);
-		const bool in_whole = t < whole_pieces;
-		const uint64_t over = __builtin_amdgcn_ballot_w64(in_whole ? whole_before + whole_upto > t : rest_before + rest_upto > t);
-		if (over) {
-			const int src = __builtin_ctzll(over);
-			p.seq		  = base + src;
-			p.first_row	  = __builtin_amdgcn_readlane(z.first_row, src);
-			p.rows		  = __builtin_amdgcn_readlane(z.rows, src);
-			p.pos0		  = __builtin_amdgcn_readlane(z.pos0, src);
-			p.row_groups  = __builtin_amdgcn_readlane(groups, src);
-			p.whole		  = __builtin_amdgcn_readlane(whole, src);
-			p.first_whole = whole_before + __builtin_amdgcn_readlane(whole_upto, src) - __builtin_amdgcn_readlane(wholes, src);
-			p.first_rest  = rest_before + __builtin_amdgcn_readlane(rest_upto, src) - __builtin_amdgcn_readlane(rests, src);
-			const int k	  = t - (in_whole ? p.first_whole : p.first_rest);
-			p.index		  = !in_whole ? p.whole : p.row_groups == 1 ? k : k / p.row_groups;
-			p.row_group	  = in_whole ? k - p.index * p.row_groups : k;
-			p.length	  = length;
-			p.there		  = true;
-			return p;
-		}
-		whole_before += __builtin_amdgcn_readlane(whole_upto, 63);
-		rest_before += __builtin_amdgcn_readlane(rest_upto, 63);
-	}
-	return p;
+__device__ __forceinline__ int row_groups_of(const sequence_size& z, int group) {
+	return (z.rows * group + COLUMNS - 1) / COLUMNS;
 }
+
+// A stretch of one row group's steps.
+struct segment {
+	int seq, first_row, rows, pos0; // pos0: position of the sequence's first row
+	int row_group, steps; // of all of the row group
+	int begin; // of the row group's steps in the row of all work
+};
 
 // Results between workgroups: device-scope stores and loads (sc1), past the caches that another XCD does not see.
 __device__ __forceinline__ void put4(float* p, v4f v) {
@@ -266,12 +171,11 @@ template<int CACHE, int TYPE, int D>
 __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const uint16_t* v_pages,
 	uint32_t shape, int width, int prefix_count, uint32_t heads, attention_args a, rows_workspace w) {
 	// What the first loads take comes first, in fourteen dwords: those arrive in registers, the rest is read from memory, as far away as the data.
-	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | one row per sequence << 31
-	const int kv_heads = heads & 0xFFFF, group = heads >> 16, sequences = shape & 0x1FFFFF, page_shift = (shape >> 21) & 15, units_log2 = (shape >> 25) & 15;
+	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | one row per sequence << 31
+	const int kv_heads = heads & 0xFFFF, group = heads >> 16, sequences = shape & 0x1FFFFF, page_shift = (shape >> 21) & 15;
 	const bool one_each = (shape >> 31) != 0;
 	const int all_rows	= one_each ? sequences : a.rows;
 	const batch_view batch{ page_table, lengths, one_each ? nullptr : a.batch.starts, sequences, width };
-	const int fit = max(1, AT_ONCE >> (kv_heads > 1 ? 32 - __builtin_clz(kv_heads - 1) : 0)); // pieces per kv head (or fewer) that the chip holds at once
 	using H				 = half_type<CACHE>;
 	using vec			 = typename H::vec;
 	constexpr int N		 = terms<CACHE, TYPE>;
@@ -291,7 +195,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	const int q_heads	  = group * kv_heads;
 	const int head		  = blockIdx.x;
 	const int prefix_keys = prefix_count << page_shift, held = width << page_shift;
-	const int piece		  = blockIdx.z * gridDim.y + blockIdx.y;
+	const int unit		  = blockIdx.y, units = gridDim.y;
 
 	// The row group's q, a part by each wave: piece x of row r at x ^ (r % 8).  Columns past the last row hold that one again; their results go nowhere.
 	auto load_q = [&](int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
@@ -307,19 +211,62 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		}
 	};
 	const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
-	// One sequence of one row: whose q and pages these are is known ahead of its length, so all three are asked for together.
-	const bool single = sequences == 1 && one_each;
+	// One sequence of one row group: whose q and pages these are is known ahead of its length, so all three are asked for together.
+	const bool single = sequences == 1 && one_each && group <= COLUMNS;
 	int ids			  = page_table[min(lane, max(width, 1) - 1)]; // lane i: page first_id + i of the sequence (the host gives a table that can be read)
 	int first_id	  = 0;
 	if (single) {
-		const int groups = (group + COLUMNS - 1) / COLUMNS;
-		const int row	 = (groups == 1 ? 0 : piece % groups) * COLUMNS;
-		load_q(0, head * group, row, 0.0f, min(COLUMNS, group - row)); // (all of them rows of token 0)
+		load_q(0, head * group, 0, 0.0f, group); // (all of them rows of token 0)
 	}
-	const piece_place p = place_of_piece(batch, all_rows, group, prefix_keys, held, units_log2, fit, piece);
-	if (!p.there) {
+	// All work, in steps: 64 sequences at a time, one for each lane.  (Their number is below 2^31: checked on the host.)
+	sequence_size z;
+	int total = 0;
+	for (int base = 0; base < sequences; base += 64) {
+		z = size_of(batch, all_rows, prefix_keys, held, base + lane);
+		total += sum64(row_groups_of(z, group) * (FIXED + steps_of(z)));
+	}
+	const int share = ((total + units - 1) / units + WAVES - 1) & -WAVES; // of a workgroup
+	int at			= unit * share;
+	const int end	= min(at + share, total);
+	if (at >= end) {
 		wait_stores_acknowledged(); // (nothing may still be on its way into LDS when the workgroup ends)
 		return;
+	}
+	// where the stretch begins
+	int chunk = 0, before = 0; // the lanes' sequences are chunk .. chunk + 63; work in front of them
+	segment p{};
+	auto find = [&] {
+		for (;;) {
+			if (sequences > 64) {
+				z = size_of(batch, all_rows, prefix_keys, held, chunk + lane);
+			}
+			const int groups = row_groups_of(z, group), steps = steps_of(z), work = groups * (FIXED + steps), upto = scan64(work);
+			const uint64_t over = __builtin_amdgcn_ballot_w64(before + upto > at);
+			if (over) {
+				const int src  = __builtin_ctzll(over);
+				p.seq		   = chunk + src;
+				p.first_row	   = __builtin_amdgcn_readlane(z.first_row, src);
+				p.rows		   = __builtin_amdgcn_readlane(z.rows, src);
+				p.pos0		   = __builtin_amdgcn_readlane(z.pos0, src);
+				p.steps		   = __builtin_amdgcn_readlane(steps, src);
+				const int start = before + __builtin_amdgcn_readlane(upto, src) - __builtin_amdgcn_readlane(work, src); // of the sequence
+				p.row_group	   = at - start < FIXED + p.steps ? 0 : (at - start) / (FIXED + p.steps);
+				p.begin		   = start + p.row_group * (FIXED + p.steps) + FIXED;
+				return;
+			}
+			before += __builtin_amdgcn_readlane(upto, 63); // (at is below the total: there is a next chunk)
+			chunk += 64;
+		}
+	};
+	for (bool again = false;; again = true) {
+	find();
+	const int segment_end = min(p.begin + p.steps, end), segment_begin = max(at, p.begin);
+	if (segment_begin >= segment_end) { // what the row group takes beside its steps, and the steps themselves are the next unit's
+		wait_stores_acknowledged();
+		return;
+	}
+	if (again) {
+		__syncthreads(); // (what the last row group left in LDS has been read)
 	}
 	// the row group's rows: first .. first + count - 1 of the sequence's rows * group
 	const int first = p.row_group * COLUMNS, count = min(COLUMNS, p.rows * group - first);
@@ -335,17 +282,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	// keys: the sequence's own ones that the lane's row sees end at `seen`, those that some row of the group sees at most_seen, that all see at all_seen
 	const int seen	   = min(held, p.pos0 + token + 1);
 	const int all_seen = min(held, p.pos0 + first_token + 1), most_seen = min(held, p.pos0 + token_of(count - 1) + 1);
-	const int pieces   = max(1, (max(0, most_seen - prefix_keys) + p.length - 1) / p.length); // of this row group
-	if (p.index >= pieces) { // (rows in front of the sequence's last see less)
-		wait_stores_acknowledged();
-		return;
-	}
-	const int first_key = prefix_keys + p.index * p.length;
-	const int end_key	= min(first_key + p.length, most_seen);
+	const int first_key = prefix_keys + (segment_begin - p.begin) * STEP, end_key = min(prefix_keys + (segment_end - p.begin) * STEP, most_seen);
+	// the units that the row group is cut over
+	const int first_unit = p.begin >= unit * share ? unit : p.begin / share, last_unit = p.begin + p.steps <= end ? unit : (p.begin + p.steps - 1) / share;
+	const int pieces	 = last_unit - first_unit + 1;
 
 	const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
 	const int page_size	 = 1 << page_shift;
-	if (!single) {
+	if (!single || again) {
 		first_id = first_key >> page_shift;
 		ids		 = table[min(first_id + lane, max(width, 1) - 1)];
 		load_q(p.first_row + first_token, head * group, first_rest, inv_group, count);
@@ -552,7 +496,11 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	}
 	__syncthreads();
 	const bool alone	= pieces == 1 && w.prefix_pieces == 0;
-	const int64_t slot	= static_cast<int64_t>(piece) * kv_heads + head;
+	// the slot of the piece in unit i
+	auto slot_of = [&](int i) {
+		return static_cast<int64_t>(2 * i + (i == first_unit && p.begin > first_unit * share ? 1 : 0)) * kv_heads + head;
+	};
+	const int64_t slot = slot_of(unit);
 	if (there) {
 		float2 ml[WAVES];
 #pragma unroll
@@ -585,32 +533,24 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			put2(w.ml + slot * w.columns + col, make_float2(top, sum));
 		}
 	}
-	if (alone) {
-		return;
-	}
-	// the slot of piece i of this row group
-	auto slot_of = [&](int i) {
-		return static_cast<int64_t>(i < p.whole ? p.first_whole + i * p.row_groups + p.row_group : p.first_rest + p.row_group) * kv_heads + head;
-	};
-	const int64_t first_slot = slot_of(0);
-	if (pieces > 1) {
+	bool join = !alone;
+	if (join) {
 		wait_stores_acknowledged();
 		__syncthreads();
-		if (tid == 0) {
-			const int done = __hip_atomic_fetch_add(w.counters + first_slot, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-			is_last		   = done == pieces - 1;
-			if (is_last) {
-				__hip_atomic_store(w.counters + first_slot, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+		if (pieces > 1) {
+			if (tid == 0) {
+				int32_t* counter = w.counters + first_unit * kv_heads + head;
+				const int done	 = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+				is_last			 = done == pieces - 1;
+				if (is_last) {
+					__hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+				}
 			}
+			__syncthreads();
+			join = is_last != 0;
 		}
-		__syncthreads();
-		if (!is_last) {
-			return;
-		}
-	} else {
-		wait_stores_acknowledged();
-		__syncthreads();
 	}
+	if (join) {
 	// Joins the row group's pieces, those over the shared prefix first: D / 4 threads to a row, the pieces of few rows over what threads are left.
 	constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
 	running* parts		= reinterpret_cast<running*>(&slots[0][0]); // [GROUPS][LANES]
@@ -636,7 +576,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 					const int i		  = min(i0 + k * ways, all - 1); // (past the last one: the last one again, not added)
 					const bool shared = i < w.prefix_pieces;
 					const int64_t at  = shared ? (static_cast<int64_t>(i) * sequences + p.seq) * q_heads + q_h
-											   : slot_of(i - w.prefix_pieces) * w.columns + r;
+											   : slot_of(first_unit + i - w.prefix_pieces) * w.columns + r;
 					ml[k]			  = (shared ? w.prefix_ml : w.ml) + at;
 					o4[k]			  = (shared ? w.prefix_o : w.o) + at * D + 4 * part;
 				}
@@ -661,17 +601,28 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			store_out4<TYPE>(a.out, ((static_cast<int64_t>(p.first_row) + tok) * q_heads + q_h) * D + 4 * part, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
 		}
 	}
+	}
+	at = segment_end;
+	if (at >= end) {
+		return;
+	}
+	}
 }
 
-rows_needs attention_rows_needs(int64_t rows, int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
+rows_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
 	rows_workspace w;
-	const rows_cut cut = plan_rows(rows, sequences, one_each, q_heads / kv_heads, kv_heads);
-	return rows_needs{ lay_out(nullptr, cut, plan_prefix(sequences, q_heads / kv_heads, kv_heads, prefix_keys), sequences, q_heads, kv_heads, head_dim, &w), cut.pieces * kv_heads * 4 };
+	const rows_cut cut = plan_rows(one_each, q_heads / kv_heads, kv_heads);
+	return rows_needs{ lay_out(nullptr, cut, plan_prefix(sequences, q_heads / kv_heads, kv_heads, prefix_keys), sequences, q_heads, kv_heads, head_dim, &w), cut.units * kv_heads * 4 };
+}
+bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t table_keys) {
+	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : rows * group / COLUMNS + sequences;
+	return row_groups * (table_keys / STEP + 1 + FIXED) < (int64_t{ 1 } << 30);
 }
 
 template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
 	const int64_t group = a.q_heads / a.cache.kv_heads, sequences = a.batch.sequences;
-	const rows_cut cut		= plan_rows(a.rows, sequences, a.batch.starts == nullptr, group, a.cache.kv_heads);
+	const bool one_each		= a.batch.starts == nullptr;
+	const rows_cut cut		= plan_rows(one_each, group, a.cache.kv_heads);
 	const prefix_cut prefix = plan_prefix(sequences, group, a.cache.kv_heads, static_cast<int64_t>(a.prefix_count) << a.cache.page_shift);
 	rows_workspace w;
 	(void)lay_out(static_cast<char*>(a.workspace), cut, prefix, sequences, a.q_heads, a.cache.kv_heads, D, &w);
@@ -682,15 +633,14 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 			return e;
 		}
 	}
-	// no row group has more pieces than its table has keys for
-	const int64_t row_groups = cut.pieces - cut.units, keys = static_cast<int64_t>(a.batch.width) << a.cache.page_shift;
-	const int64_t pieces	 = std::min(cut.pieces, row_groups * std::max<int64_t>(1, (keys + STEP * WAVES - 1) / (STEP * WAVES)));
-	const int64_t y			 = std::min<int64_t>(pieces, 32768), z = (pieces + y - 1) / y;
-	const bool one_each = a.batch.starts == nullptr;
-	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), static_cast<unsigned>(y), static_cast<unsigned>(z)), dim3(THREADS), 0, s>>>(a.batch.lengths,
+	// (no more workgroups than the tables have keys for, four steps each at least)
+	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : a.rows * group / COLUMNS + sequences;
+	const int64_t steps		 = (static_cast<int64_t>(a.batch.width) << a.cache.page_shift) / STEP + 1 + FIXED;
+	const int64_t units		 = std::max<int64_t>(1, std::min(cut.units, (row_groups * steps + WAVES - 1) / WAVES));
+	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), static_cast<unsigned>(units)), dim3(THREADS), 0, s>>>(a.batch.lengths,
 		a.batch.width > 0 ? a.batch.table : a.batch.lengths, a.q, a.cache.k, a.cache.v,
-		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | static_cast<uint32_t>(cut.units_log2) << 25 | (one_each ? 1u << 31 : 0u), a.batch.width,
-		a.prefix_count, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, a, w);
+		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | (one_each ? 1u << 31 : 0u), a.batch.width, a.prefix_count,
+		static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, a, w);
 	return hipGetLastError();
 }
 template<int CACHE, int TYPE> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
