@@ -106,7 +106,8 @@ int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
  * new_table int32 [children][table_width] (entries past a child's last page are -1), new_lengths int32 [children], none of them an input.
  * info int32 [3]: pages held afterwards, pages copied, pages that could not be given (too few free) or that the old table did not
  * have; their entries are -1, which the calls above leave out.  Nothing of the inputs changes, so a caller that finds pages missing can end
- * sequences and call again.  starts is not used.  workspace: nh_attn_pages_workspace_bytes(pages, children, table_width). */
+ * sequences and call again.  starts is not used.  workspace: nh_attn_pages_workspace_bytes(pages, children, table_width) bytes, 0 (and it may
+ * be NULL) unless the cache is large. */
 int64_t nh_attn_pages_workspace_bytes(int64_t pages, int64_t sequences, int64_t table_width);
 int nh_attn_cache_step(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* parents, const int32_t* grow, int64_t children, int32_t* new_table, int32_t* new_lengths,
 	int32_t* info, void* workspace, int64_t workspace_bytes, void* stream);

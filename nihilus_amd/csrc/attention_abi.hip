@@ -230,7 +230,7 @@ static int check_pages(const nh_attn_cache* c, const nh_attn_batch* b, int64_t c
 	NH_REQUIRE(children <= MAX_SEQUENCES && children * b->table_width * c->page_size <= MAX_ALL_KEYS, NH_ERR_TOO_LARGE);
 	const int64_t need = nh_attn_pages_workspace_bytes(c->pages, children, b->table_width);
 	NH_REQUIRE(need >= 0, static_cast<int>(need));
-	NH_REQUIRE(info && workspace && (new_table || children * b->table_width == 0), NH_ERR_NULL_POINTER);
+	NH_REQUIRE(info && (workspace || need == 0) && (new_table || children * b->table_width == 0), NH_ERR_NULL_POINTER);
 	NH_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, NH_ERR_ALIGNMENT);
 	NH_REQUIRE(workspace_bytes >= need, NH_ERR_ARGUMENT);
 	// the new table is written while the old one is read

@@ -383,10 +383,11 @@ PyObject* cache_step(args& in) {
 	if (need < 0) {
 		return nullptr;
 	}
-	const at::Tensor new_table = ints_like(*table, { n, p.batch.table_width }), now = ints_like(*table, { n }), info = ints_like(*table, { 3 }), workspace = bytes_like(*table, need);
+	const at::Tensor new_table = ints_like(*table, { n, p.batch.table_width }), now = ints_like(*table, { n }), info = ints_like(*table, { 3 });
+	const at::Tensor workspace = need > 0 ? bytes_like(*table, need) : at::Tensor();
 	const auto *pp = static_cast<const int32_t*>(parents->const_data_ptr()), *gp = static_cast<const int32_t*>(grow->const_data_ptr());
 	auto *tp = static_cast<int32_t*>(new_table.mutable_data_ptr()), *np = static_cast<int32_t*>(now.mutable_data_ptr()), *ip = static_cast<int32_t*>(info.mutable_data_ptr());
-	void *ws = workspace.mutable_data_ptr(), *s = stream();
+	void *ws = need > 0 ? workspace.mutable_data_ptr() : nullptr, *s = stream();
 	PyObject* first = finish(new_table, [&] { return nh_attn_cache_step(&p.cache, &p.batch, pp, gp, n, tp, np, ip, ws, need, s); });
 	return first && THPVariable_Check(first) ? Py_BuildValue("NNN", first, THPVariable_Wrap(now), THPVariable_Wrap(info)) : first;
 }
@@ -406,9 +407,10 @@ PyObject* cache_compact(args& in) {
 	if (need < 0) {
 		return nullptr;
 	}
-	const at::Tensor new_table = like(*table), info = ints_like(*table, { 3 }), workspace = bytes_like(*table, need);
+	const at::Tensor new_table = like(*table), info = ints_like(*table, { 3 });
+	const at::Tensor workspace = need > 0 ? bytes_like(*table, need) : at::Tensor();
 	auto *tp = static_cast<int32_t*>(new_table.mutable_data_ptr()), *ip = static_cast<int32_t*>(info.mutable_data_ptr());
-	void *ws = workspace.mutable_data_ptr(), *s = stream();
+	void *ws = need > 0 ? workspace.mutable_data_ptr() : nullptr, *s = stream();
 	PyObject* first = finish(new_table, [&] { return nh_attn_cache_compact(&p.cache, &p.batch, tp, ip, ws, need, s); });
 	return first && THPVariable_Check(first) ? Py_BuildValue("NN", first, THPVariable_Wrap(info)) : first;
 }

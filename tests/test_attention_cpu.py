@@ -125,8 +125,9 @@ def test_attention_refusals():
 
 def test_pages_refusals():
     for call in (_step, _compact):
-        assert call(info=None) == -1 and call(table=None) == -1 and call(ws=None) == -1
-        assert call(ws=BOGUS + 128) == -2 and call(bytes=64) == -6
+        assert call(info=None) == -1 and call(table=None) == -1
+        large = dict(cache=_cache(pages=100000))  # (a small one needs no workspace)
+        assert call(ws=None, **large) == -1 and call(ws=BOGUS + 128) == -2 and call(bytes=64, **large) == -6
         assert call(table=BOGUS + 16) == -6  # the old table, in part
     assert _step(parents=None) == -1 and _step(grow=None) == -1 and _step(lengths=None) == -1
     assert _step(children=-1) == -3 and _step(children=1 << 21) == -5
@@ -155,7 +156,7 @@ def test_workspace_sizes():
     assert prompt(-1, 2, 32, 8, 128) == -3 and prompt(20, 2, 32, 8, 96) == -3 and prompt(1 << 29, 2, 32, 8, 128) == -5
     assert lib.nh_attn_prompt_needs(20, 2, 32, 8, 128, None, C.byref(c)) == -1 and lib.nh_attn_decode_needs(4, 32, 8, 128, 0, 64, C.byref(n), None) == -1
     g = lib.nh_attn_pages_workspace_bytes
-    assert g(1, 0, 0) > 0 and g(1000, 64, 10) >= 1000 * 8 and g(0, 1, 1) == -3 and g(1, -1, 1) == -3 and g(1 << 40, 1, 1) == -5
+    assert g(1, 0, 0) == 0 and g(1000, 64, 10) == 0 and g(100000, 64, 10) >= 100000 * 8 and g(5000, 20000, 1) >= 20000 * 8 and g(0, 1, 1) == -3 and g(1, -1, 1) == -3 and g(1 << 40, 1, 1) == -5
 
 
 def test_which_kernel_a_prompt_takes(monkeypatch):
