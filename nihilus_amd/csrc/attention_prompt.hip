@@ -30,13 +30,14 @@ constexpr int KEYS	= 64; // of a tile
 __device__ __forceinline__ int key_of_row(int m) {
 	return (m & 0x13) | ((m & 4) << 1) | ((m & 8) >> 1);
 }
-// Pieces of 16 bytes of a K tile row (head_dim values) and of a V tile row (64 keys) are permuted in LDS so that eight lanes that read the
-// same piece of eight rows hit different banks: the rows differ in bits 0, 1, 3 (K: see key_of_row) or 0, 1, 2 (V).
-__device__ __forceinline__ int k_swizzle(int row) {
-	return (row & 3) | ((row >> 1) & 4);
+// Pieces of 16 bytes of a K tile row (head_dim values) and of a V tile row (64 keys) are permuted in LDS so that the sixteen lanes that read
+// the same piece of sixteen rows at a time hit different banks, of which there are 256 bytes: rows of 256 bytes differ in bits 0 .. 3 of their number (K,
+// see key_of_row, and V alike); of rows of 128 bytes two lie side by side, so bit 0 tells the halves apart and bits 1 .. 3 the rest.
+template<int D> __device__ __forceinline__ int k_swizzle(int row) {
+	return D == 128 ? row & 15 : (row >> 1) & 7;
 }
 __device__ __forceinline__ int v_swizzle(int row) {
-	return row & 7;
+	return (row >> 1) & 7;
 }
 
 struct tile_place {
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 		for (int i = 0; i < LOADS; ++i) {
 			const int piece = tid + 64 * WAVES * i;
 			const int r = piece / PIECES, x = piece % PIECES;
-			k_tile[r * PIECES + (x ^ k_swizzle(r))] = k_reg[i];
+			k_tile[r * PIECES + (x ^ k_swizzle<D>(r))] = k_reg[i];
 		}
 #pragma unroll
 		for (int i = 0; i < LOADS; ++i) {
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 		for (int kb = 0; kb < 2; ++kb) {
 			s[kb]		  = v16f{};
 			const int r	  = 32 * kb + key_of_row(col);
-			const int swz = k_swizzle(r);
+			const int swz = k_swizzle<D>(r);
 #pragma unroll
 			for (int st = 0; st < STEPS; ++st) {
 				const vec k = __builtin_bit_cast(vec, k_tile[r * PIECES + ((2 * st + half) ^ swz)]);

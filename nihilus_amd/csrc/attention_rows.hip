@@ -152,6 +152,12 @@ __device__ __forceinline__ void get_parts(const float2* const (&ml)[4], const fl
 	got_ml[0] = __builtin_bit_cast(float2, m0), got_ml[1] = __builtin_bit_cast(float2, m1), got_ml[2] = __builtin_bit_cast(float2, m2), got_ml[3] = __builtin_bit_cast(float2, m3);
 }
 
+// Where piece x of row r of a step's keys lies in LDS: at x ^ k_swizzle(r), so that the sixteen lanes that read the same piece of sixteen rows hit
+// different banks, of which there are 256 bytes.  The rows of an operand differ in bits 0, 1, 3 and 4.  (Values: rows of 64 bytes, four side by side.)
+template<int D> __device__ __forceinline__ int k_swizzle(int r) {
+	return D == 128 ? (r & 3) | ((r >> 1) & 12) : ((r >> 1) & 1) | ((r >> 2) & 6);
+}
+
 // a running result and another one, both sums of weights and of weighted values below their own maximum
 struct running {
 	float m, l;
@@ -303,20 +309,19 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		return id >= 0 && id < a.cache.pages ? id : -1;
 	};
 	// A step's 32 keys into a slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
-	// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).  Eight
-	// lanes that read the same piece of eight operand rows hit different banks: K rows differ in bits 0, 1, 3, V rows in bits 0 .. 2.
+	// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).
 	const int64_t page_values = static_cast<int64_t>(kv_heads) * D << page_shift, head_values = static_cast<int64_t>(head) * D << page_shift;
 	auto load_step			  = [&](int base, int lo, int hi) {
 		 const int64_t lo_at = max(lo, 0) * page_values + head_values, hi_at = max(hi, 0) * page_values + head_values;
 #pragma unroll
 		 for (int j = 0; j < LOADS; ++j) {
-			 const int at = 64 * j + lane, r = at / PIECES, x = (at % PIECES) ^ ((r & 3) | ((r >> 1) & 4));
+			 const int at = 64 * j + lane, r = at / PIECES, x = (at % PIECES) ^ k_swizzle<D>(r);
 			 const int key = (base + r) & (page_size - 1);
 			 load_global_to_lds_b128(k_pages + (2 * j < LOADS ? lo_at : hi_at) + key * D + 8 * x, &slots[wave][64 * j]);
 		 }
 #pragma unroll
 		 for (int j = 0; j < LOADS; ++j) {
-			 const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 1) & 3);
+			 const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 2) & 3);
 			 const int key = (base + 8 * x) & (page_size - 1);
 			 load_global_to_lds_b128(v_pages + (x & 2 ? hi_at : lo_at) + d * page_size + key, &slots[wave][STEP * PIECES + 64 * j]);
 		 }
@@ -389,7 +394,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		const v4u* values = &slots[wave][STEP * PIECES];
 #pragma unroll
 		for (int t = 0; t < 2; ++t) {
-			const int r = 8 * (col >> 2) + 4 * t + (col & 3), swizzle = (r & 3) | ((r >> 1) & 4);
+			const int r = 8 * (col >> 2) + 4 * t + (col & 3), swizzle = k_swizzle<D>(r);
 #pragma unroll
 			for (int st = 0; st < STEPS; ++st) {
 				k[t][st] = __builtin_bit_cast(vec, keys[r * PIECES + ((4 * st + quarter) ^ swizzle)]);
@@ -398,7 +403,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 #pragma unroll
 		for (int dt = 0; dt < DT; ++dt) {
 			const int d = 16 * dt + col;
-			v[dt]		= __builtin_bit_cast(vec, values[4 * d + (quarter ^ ((d >> 1) & 3))]);
+			v[dt]		= __builtin_bit_cast(vec, values[4 * d + (quarter ^ ((d >> 2) & 3))]);
 		}
 	};
 	auto compute = [&](int base, int lo, int hi) {
