@@ -40,6 +40,10 @@ __device__ __forceinline__ int v_swizzle(int row) {
 	return (row >> 1) & 7;
 }
 
+// The weights of a row are formed below a maximum that is followed only when the scores rise above it by more than this (as a power of two): fp16
+// weights stay below 2^(8 + 7), and after a row's first tiles its results are hardly ever brought below a new one.
+constexpr float RISE = 7.0f;
+
 struct tile_place {
 	int seq, first_token, tokens, first_row, pos0; // the tile's rows start at first_row of tokens * group; pos0: position of the sequence's first token
 	bool there;
@@ -100,8 +104,8 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 	constexpr int DT	= D / 32; // tiles of O^T
 	constexpr int PIECES = D / 8; // 16-byte pieces of a key
 	constexpr int LOADS	 = KEYS * PIECES / (64 * WAVES); // pieces of K, and of V, per thread
-	__shared__ v4u k_tile[KEYS * PIECES];
-	__shared__ v4u v_tile[D * (KEYS / 8)];
+	__shared__ v4u k_tile[2][KEYS * PIECES]; // of tile kt in [kt % 2]
+	__shared__ v4u v_tile[2][D * (KEYS / 8)];
 
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int col = lane & 31, half = lane >> 5;
@@ -190,53 +194,48 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 		c = ldexpf(a.scale * LOG2_E, e - 14);
 	}
 
-	// the pages of a tile: lane i holds that of keys 16 (i % 4) .. + 15, -1 where there is none
-	auto page_ids = [&](int kt) {
-		const int slot = (kt * KEYS + 16 * (lane & 3)) >> a.cache.page_shift;
-		const int id   = slot < width ? table[slot] : -1;
-		return id >= 0 && id < a.cache.pages ? id : -1;
+	// Pages: lane i holds that of the 16 keys from 16 i on of the stretch of 1024 keys that a tile is in, -1 where there is none; and the next stretch's.
+	auto load_ids = [&](int stretch) {
+		const int slot = (1024 * stretch + 16 * lane) >> a.cache.page_shift;
+		const int id   = table[min(slot, width - 1)]; // (there are keys, so there is an entry)
+		return slot < width && id >= 0 && id < a.cache.pages ? id : -1;
 	};
-	const int page_size = 1 << a.cache.page_shift;
-	v4u k_reg[LOADS], v_reg[LOADS];
-	auto load_tile = [&](int kt, int ids) {
+	const int page_size		= 1 << a.cache.page_shift;
+	const int64_t head_part = static_cast<int64_t>(head) * D << a.cache.page_shift;
+	// What a tile's 16-byte pieces are to a thread: K rows 16 w .. 16 w + 15 are wave w's (of one page), V rows (D / 4) w on likewise.
+	constexpr int K_ROWS = 64 / PIECES; // of an instruction
+	uint32_t k_offset[LOADS], v_offset[LOADS]; // bytes behind the tile's first key of the wave; v: behind the wave's first row, without the part that the page size is a factor of
 #pragma unroll
-		for (int i = 0; i < LOADS; ++i) {
-			const int piece = tid + 64 * WAVES * i;
-			const int r = piece / PIECES, x = piece % PIECES;
-			const int key  = kt * KEYS + r;
-			const int page = max(__shfl(ids, r >> 4), 0);
-			k_reg[i] = *reinterpret_cast<const v4u*>(a.cache.k + page * a.cache.page_values + (static_cast<int64_t>(head) * page_size + (key & (page_size - 1))) * D + 8 * x);
-		}
+	for (int j = 0; j < LOADS; ++j) {
+		const int r = K_ROWS * j + lane / PIECES, d = 8 * j + lane / 8; // in the wave's part
+		k_offset[j] = 2 * (r * D + 8 * ((lane % PIECES) ^ k_swizzle<D>(r)));
+		v_offset[j] = 2 * (d * page_size + 8 * ((lane & 7) ^ v_swizzle(d)));
+	}
+	auto load_k = [&](int kt, int ids) {
+		const int key	  = kt * KEYS + 16 * wave;
+		const int page	  = max(__builtin_amdgcn_readlane(ids, (kt & 15) * 4 + wave), 0);
+		const uint16_t* at = a.cache.k + page * a.cache.page_values + head_part + static_cast<int64_t>(key & (page_size - 1)) * D;
 #pragma unroll
-		for (int i = 0; i < LOADS; ++i) {
-			const int piece = tid + 64 * WAVES * i;
-			const int d = piece >> 3, x = piece & 7;
-			const int key  = kt * KEYS + 8 * x;
-			const int page = max(__shfl(ids, x >> 1), 0);
-			v_reg[i] = *reinterpret_cast<const v4u*>(a.cache.v + page * a.cache.page_values + (static_cast<int64_t>(head) * D + d) * page_size + (key & (page_size - 1)));
+		for (int j = 0; j < LOADS; ++j) {
+			load_global_to_lds_b128(at, k_offset[j], &k_tile[kt & 1][(LOADS * wave + j) * 64]);
 		}
 	};
-	auto store_tile_to_lds = [&](int kt, uint32_t bad) {
-		const bool edge = kt * KEYS + KEYS > limit || bad;
+	auto load_v = [&](int kt, int ids) {
+		const uint16_t* base = a.cache.v + head_part + static_cast<int64_t>(D / WAVES) * wave * page_size;
+		if (page_size >= KEYS) { // the tile is in one page
+			const int page	   = max(__builtin_amdgcn_readlane(ids, (kt & 15) * 4), 0);
+			const uint16_t* at = base + page * a.cache.page_values + ((kt * KEYS) & (page_size - 1));
 #pragma unroll
-		for (int i = 0; i < LOADS; ++i) {
-			const int piece = tid + 64 * WAVES * i;
-			const int r = piece / PIECES, x = piece % PIECES;
-			k_tile[r * PIECES + (x ^ k_swizzle<D>(r))] = k_reg[i];
-		}
-#pragma unroll
-		for (int i = 0; i < LOADS; ++i) {
-			const int piece = tid + 64 * WAVES * i;
-			const int d = piece >> 3, x = piece & 7;
-			v4u v = v_reg[i];
-			if (edge) { // values of keys that no row has: nothing, whatever lies there (a weight of zero times infinity is not zero)
-				const int n = ((bad >> (x >> 1)) & 1) ? 0 : limit - (kt * KEYS + 8 * x); // the first n keys of the piece are real
-#pragma unroll
-				for (int w = 0; w < 4; ++w) {
-					v[w] = n >= 2 * w + 2 ? v[w] : n == 2 * w + 1 ? v[w] & 0xFFFFu : 0u;
-				}
+			for (int j = 0; j < LOADS; ++j) {
+				load_global_to_lds_b128(at, v_offset[j], &v_tile[kt & 1][(LOADS * wave + j) * 64]);
 			}
-			v_tile[d * 8 + (x ^ v_swizzle(d))] = v;
+			return;
+		}
+#pragma unroll
+		for (int j = 0; j < LOADS; ++j) {
+			const int d = 8 * j + lane / 8, x = (lane & 7) ^ v_swizzle(d); // keys 8 x .. + 7 of the tile
+			const int page = max(__shfl(ids, (kt & 15) * 4 + (x >> 1)), 0);
+			load_global_to_lds_b128(base + page * a.cache.page_values + d * page_size + ((8 * x) & (page_size - 1)), &v_tile[kt & 1][(LOADS * wave + j) * 64]);
 		}
 	};
 
@@ -245,94 +244,140 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 	for (int t = 0; t < DT; ++t) {
 		o[t] = v16f{};
 	}
-	float m = -__builtin_inff(), l = 0.0f; // running maximum of c * scores, this lane's part of the sum of the weights
+	float m = -__builtin_inff(), l = 0.0f; // what the weights are below (see RISE), this lane's part of the sum of the weights
 	const int first_tile = first_key / KEYS, tiles = (limit + KEYS - 1) / KEYS;
-	int ids				 = -1;
-	if (first_tile < tiles) {
-		ids = page_ids(first_tile);
-		load_tile(first_tile, ids);
-	}
-	for (int kt = first_tile; kt < tiles; ++kt) {
-		const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ids < 0)) & 15u;
-		__syncthreads(); // the last tile has been read
-		store_tile_to_lds(kt, bad);
-		__syncthreads();
-		if (kt + 1 < tiles) {
-			ids = page_ids(kt + 1);
-			load_tile(kt + 1, ids);
-		}
-		if (kt * KEYS >= wave_limit) {
-			continue; // (wave-uniform; the barriers are at the top)
-		}
-		v16f s[2];
+	// scores of tile kt, whose keys are in LDS
+	auto scores = [&](int kt, v16f (&s)[2]) {
+		const v4u* keys = k_tile[kt & 1];
+		s[0] = v16f{}, s[1] = v16f{};
 #pragma unroll
-		for (int kb = 0; kb < 2; ++kb) {
-			s[kb]		  = v16f{};
-			const int r	  = 32 * kb + key_of_row(col);
-			const int swz = k_swizzle<D>(r);
+		for (int st = 0; st < STEPS; ++st) {
 #pragma unroll
-			for (int st = 0; st < STEPS; ++st) {
-				const vec k = __builtin_bit_cast(vec, k_tile[r * PIECES + ((2 * st + half) ^ swz)]);
+			for (int kb = 0; kb < 2; ++kb) {
+				const int r = 32 * kb + key_of_row(col);
+				const vec k = __builtin_bit_cast(vec, keys[r * PIECES + ((2 * st + half) ^ k_swizzle<D>(r))]);
 #pragma unroll
 				for (int n = N - 1; n >= 0; --n) { // the small terms first
 					s[kb] = H::mfma32(k, q[n][st], s[kb]);
 				}
 			}
 		}
-		if (kt * KEYS + KEYS - 1 > wave_min || bad) {
+	};
+	if (first_tile < tiles) {
+		int ids = load_ids(first_tile >> 4), next_ids = ids;
+		int stretch = first_tile >> 4; // that ids are of
+		// ids for tile kt, of the stretch that kt is in or the one after
+		auto ids_of = [&](int kt) {
+			return (kt >> 4) == stretch ? ids : next_ids;
+		};
+		next_ids = load_ids(stretch + 1);
+		load_k(first_tile, ids_of(first_tile));
+		load_v(first_tile, ids_of(first_tile));
+		if (first_tile + 1 < tiles) {
+			load_k(first_tile + 1, ids_of(first_tile + 1));
+		}
+		v16f s[2];
+		for (int kt = first_tile; kt < tiles; ++kt) {
+			// Tile kt's values and the next one's keys, asked for an iteration ago, have come, and all waves are through with what they take the place of.
+			asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+			__syncthreads();
+			if (kt == first_tile) {
+				scores(kt, s);
+				__syncthreads();
+			}
+			const bool new_stretch = (kt >> 4) != stretch;
+			if (new_stretch) {
+				stretch = kt >> 4;
+				ids		= next_ids;
+			}
+			const int tile_ids = ids;
+			if (kt + 2 < tiles) {
+				load_k(kt + 2, ids_of(kt + 2));
+			}
+			if (kt + 1 < tiles) {
+				load_v(kt + 1, ids_of(kt + 1));
+			}
+			if (new_stretch) { // (not needed before the next iteration, whose first wait it is under)
+				next_ids = load_ids(stretch + 1);
+			}
+			const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(tile_ids < 0) >> ((kt & 15) * 4)) & 15u; // groups of 16 keys without a page
+			if (kt * KEYS + KEYS > limit || bad) { // (the same for all waves) values of keys that no row has: nothing, whatever lies there (a weight of zero times infinity is not zero)
 #pragma unroll
-			for (int kb = 0; kb < 2; ++kb) {
+				for (int i = 0; i < LOADS; ++i) {
+					const int at = tid + 64 * WAVES * i, d = at >> 3, x = (at & 7) ^ v_swizzle(d);
+					const int n = ((bad >> (x >> 1)) & 1) ? 0 : limit - (kt * KEYS + 8 * x); // so many of the eight keys are real
+					v4u v = v_tile[kt & 1][at];
 #pragma unroll
-				for (int i = 0; i < 16; ++i) {
-					const int key = kt * KEYS + 32 * kb + 16 * (i >> 3) + 8 * half + (i & 7);
-					if (key > pos || key >= limit || ((bad >> (2 * kb + (i >> 3))) & 1)) {
-						s[kb][i] = -__builtin_inff();
+					for (int w = 0; w < 4; ++w) {
+						v[w] = n >= 2 * w + 2 ? v[w] : n == 2 * w + 1 ? v[w] & 0xFFFFu : 0u;
+					}
+					v_tile[kt & 1][at] = v;
+				}
+				__syncthreads();
+			}
+			if (kt * KEYS >= wave_limit) {
+				continue; // (wave-uniform; the barriers are at the top)
+			}
+			if (kt * KEYS + KEYS - 1 > wave_min || bad) {
+#pragma unroll
+				for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+					for (int i = 0; i < 16; ++i) {
+						const int key = kt * KEYS + 32 * kb + 16 * (i >> 3) + 8 * half + (i & 7);
+						if (key > pos || key >= limit || ((bad >> (2 * kb + (i >> 3))) & 1)) {
+							s[kb][i] = -__builtin_inff();
+						}
 					}
 				}
 			}
-		}
-		float top = s[0][0];
+			float top = s[0][0];
 #pragma unroll
-		for (int i = 1; i < 32; ++i) {
-			top = fmaxf(top, s[i >> 4][i & 15]);
-		}
-		top				  = fmaxf(top, swap32(top)) * c;
-		const float m_new = fmaxf(m, top);
-		const float base  = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
-		if (__builtin_amdgcn_ballot_w64(m_new != m)) {
-			const float f = exp2_fast(m - base);
-			l *= f;
-#pragma unroll
-			for (int t = 0; t < DT; ++t) {
-				o[t] *= f;
+			for (int i = 1; i < 32; ++i) {
+				top = fmaxf(top, s[i >> 4][i & 15]);
 			}
-			m = m_new;
-		}
-		const float shift = weight_bias<CACHE> - base;
+			top = fmaxf(top, swap32(top)) * c;
+			if (__builtin_amdgcn_ballot_w64(top > m + RISE)) { // a larger maximum: what there is so far is brought below it
+				const float m_new = fmaxf(m, top);
+				const float f	  = exp2_fast(m - (m_new == -__builtin_inff() ? 0.0f : m_new));
+				l *= f;
 #pragma unroll
-		for (int kb = 0; kb < 2; ++kb) {
+				for (int t = 0; t < DT; ++t) {
+					o[t] *= f;
+				}
+				m = m_new;
+			}
+			const float shift = weight_bias<CACHE> - (m == -__builtin_inff() ? 0.0f : m); // (no key yet: every weight is 2^-inf)
+			// the next tile's scores beside this one's weights: the matrix unit and the vector unit at once
+			v16f next[2];
+			scores(kt + 1, next); // (behind the last tile: of whatever is there, for nothing)
+			vec t[4][N];
 #pragma unroll
-			for (int h = 0; h < 2; ++h) {
+			for (int g = 0; g < 4; ++g) {
 				float w[8];
 #pragma unroll
 				for (int j = 0; j < 8; ++j) {
-					w[j] = exp2_fast(fmaf(s[kb][8 * h + j], c, shift));
+					w[j] = exp2_fast(fmaf(s[g >> 1][8 * (g & 1) + j], c, shift));
 					l += w[j];
 				}
-				vec t[N];
-				split8<CACHE, N>(w, t);
+				split8<CACHE, N>(w, t[g]);
+			}
+			const v4u* values = v_tile[kt & 1];
+#pragma unroll
+			for (int g = 0; g < 4; ++g) {
 #pragma unroll
 				for (int dt = 0; dt < DT; ++dt) {
 					const int d = 32 * dt + col;
-					const vec v = __builtin_bit_cast(vec, v_tile[d * 8 + ((4 * kb + 2 * h + half) ^ v_swizzle(d))]);
+					const vec v = __builtin_bit_cast(vec, values[d * 8 + ((2 * g + half) ^ v_swizzle(d))]);
 #pragma unroll
 					for (int n = N - 1; n >= 0; --n) {
-						o[dt] = H::mfma32(v, t[n], o[dt]);
+						o[dt] = H::mfma32(v, t[g][n], o[dt]);
 					}
 				}
 			}
+			s[0] = next[0], s[1] = next[1];
 		}
 	}
+	asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (nothing may still be on its way into LDS when the workgroup ends)
 	if (!there) {
 		return;
 	}

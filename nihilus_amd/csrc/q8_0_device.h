@@ -247,6 +247,13 @@ __device__ __forceinline__ void load_global_to_lds_b128(const void* src, void* l
 	asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0" : "=&s"(saved_m0) : "v"(src), "s"(lds_addr) : "memory");
 }
 
+// The same from `offset` bytes behind an address that the whole wave has.
+__device__ __forceinline__ void load_global_to_lds_b128(const void* src, uint32_t offset, void* lds_dst) {
+	const uint32_t lds_addr = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(static_cast<char*>(lds_dst))));
+	uint32_t saved_m0;
+	asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(saved_m0) : "v"(offset), "s"(src), "s"(lds_addr) : "memory");
+}
+
 // Blocks the wave until every memory operation it has issued, stores included, has been acknowledged.  Placed
 // between device-scope (write-through) stores of data and the device-scope store or atomic that tells another
 // workgroup the data is there: a workgroup-scope release fence does not wait for the stores on this target, and an
