@@ -102,6 +102,8 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 	constexpr int N		= terms<CACHE, TYPE>;
 	constexpr int STEPS = D / 16; // of q.k
 	constexpr int DT	= D / 32; // tiles of O^T
+	// The next tile's scores beside this one's weights; not where q alone, in two or three terms, leaves no registers for them.
+	constexpr bool AHEAD = N == 1;
 	constexpr int PIECES = D / 8; // 16-byte pieces of a key
 	constexpr int LOADS	 = KEYS * PIECES / (64 * WAVES); // pieces of K, and of V, per thread
 	__shared__ v4u k_tile[2][KEYS * PIECES]; // of tile kt in [kt % 2]
@@ -273,7 +275,7 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 		next_ids = load_ids(stretch + 1);
 		load_k(first_tile, ids_of(first_tile));
 		load_v(first_tile, ids_of(first_tile));
-		if (first_tile + 1 < tiles) {
+		if (AHEAD && first_tile + 1 < tiles) {
 			load_k(first_tile + 1, ids_of(first_tile + 1));
 		}
 		v16f s[2];
@@ -281,7 +283,7 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 			// Tile kt's values and the next one's keys, asked for an iteration ago, have come, and all waves are through with what they take the place of.
 			asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 			__syncthreads();
-			if (kt == first_tile) {
+			if (AHEAD && kt == first_tile) {
 				scores(kt, s);
 				__syncthreads();
 			}
@@ -291,8 +293,8 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 				ids		= next_ids;
 			}
 			const int tile_ids = ids;
-			if (kt + 2 < tiles) {
-				load_k(kt + 2, ids_of(kt + 2));
+			if (kt + 1 + AHEAD < tiles) {
+				load_k(kt + 1 + AHEAD, ids_of(kt + 1 + AHEAD));
 			}
 			if (kt + 1 < tiles) {
 				load_v(kt + 1, ids_of(kt + 1));
@@ -317,6 +319,9 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 			}
 			if (kt * KEYS >= wave_limit) {
 				continue; // (wave-uniform; the barriers are at the top)
+			}
+			if constexpr (!AHEAD) {
+				scores(kt, s);
 			}
 			if (kt * KEYS + KEYS - 1 > wave_min || bad) {
 #pragma unroll
@@ -349,7 +354,9 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 			const float shift = weight_bias<CACHE> - (m == -__builtin_inff() ? 0.0f : m); // (no key yet: every weight is 2^-inf)
 			// the next tile's scores beside this one's weights: the matrix unit and the vector unit at once
 			v16f next[2];
-			scores(kt + 1, next); // (behind the last tile: of whatever is there, for nothing)
+			if constexpr (AHEAD) {
+				scores(kt + 1, next); // (behind the last tile: of whatever is there, for nothing)
+			}
 			vec t[4][N];
 #pragma unroll
 			for (int g = 0; g < 4; ++g) {
@@ -374,7 +381,9 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 					}
 				}
 			}
-			s[0] = next[0], s[1] = next[1];
+			if constexpr (AHEAD) {
+				s[0] = next[0], s[1] = next[1];
+			}
 		}
 	}
 	asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (nothing may still be on its way into LDS when the workgroup ends)
