@@ -86,8 +86,8 @@ struct batch_view {
 	int width;
 };
 
-// The sequence that packed row `row` belongs to, the number of its first row that is not below `row`'s... : b with starts[b] <= row <
-// starts[b + 1], or -1.  starts ascends; an empty sequence shares its start with the next one and is passed over.
+// The sequence that packed row `row` belongs to: the b with starts[b] <= row < starts[b + 1], -1 if there is none.  starts ascends; an empty
+// sequence shares its start with the next one and is passed over.
 __device__ __forceinline__ int sequence_of_row(const int32_t* starts, int sequences, int row) {
 	int lo = 0, hi = sequences + 1; // the first index whose start is above row lies in [lo, hi]
 	while (lo < hi) {
@@ -147,6 +147,35 @@ template<int TYPE> __device__ __forceinline__ void store_out4(void* out, int64_t
 		*reinterpret_cast<v4t*>(static_cast<uint16_t*>(out) + at) = v;
 	}
 }
+
+// Values that are infinite or NaN: in a product they reach rows that do not see their keys too, and make NaN of what ought to be infinite (a weight of zero,
+// or the negative rest of a weight in several terms, times infinity).  A result that is not finite is therefore formed once more: this time such values
+// are taken out of the tiles and noted here, for each column of V the first such key, and a row that sees that key adds the value at the end.
+template<int D> struct not_finite {
+	int first_key[3][D]; // of NaN, +inf, -inf
+	__device__ __forceinline__ void clear(int thread, int threads) {
+		for (int i = thread; i < 3 * D; i += threads) {
+			(&first_key[0][0])[i] = INT_MAX;
+		}
+	}
+	// takes them out of the first n of eight values of column d, keys key .. key + 7
+	template<int CACHE> __device__ __forceinline__ void take(uint16_t* eight, int d, int key, int n) {
+		constexpr unsigned E = CACHE == NH_F16 ? 0x7C00u : 0x7F80u;
+#pragma unroll 1
+		for (int x = 0; x < min(n, 8); ++x) {
+			const unsigned h = eight[x];
+			if ((h & E) == E) {
+				atomicMin(&first_key[(h & (E ^ 0x7FFFu)) ? 0 : 1 + (h >> 15)][d], key + x);
+				eight[x] = 0;
+			}
+		}
+	}
+	// what a row that sees the keys below `seen` adds to column d
+	__device__ __forceinline__ float of(int d, int seen) const {
+		const bool nan = first_key[0][d] < seen, plus = first_key[1][d] < seen, minus = first_key[2][d] < seen;
+		return nan || (plus && minus) ? __builtin_nanf("") : plus ? __builtin_inff() : minus ? -__builtin_inff() : 0.0f;
+	}
+};
 
 // ---- launch functions (after argument checks) ----
 

@@ -95,8 +95,9 @@ struct prefix_out {
 	int row_tiles;
 };
 
-template<int CACHE, int TYPE, int D, bool PREFIX>
-__global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void attention_tile_kernel(attention_args a, prefix_out out) {
+// PARTS: groups of four waves that have the same rows and a part of the keys each, joined in LDS at the end.
+template<int CACHE, int TYPE, int D, bool PREFIX, int PARTS>
+__global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PARTS == 1 ? 1 : 2) void attention_tile_kernel(attention_args a, prefix_out out) {
 	using H				= half_type<CACHE>;
 	using vec			= typename H::vec;
 	constexpr int N		= terms<CACHE, TYPE>;
@@ -106,10 +107,16 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 	constexpr bool AHEAD = N == 1;
 	constexpr int PIECES = D / 8; // 16-byte pieces of a key
 	constexpr int LOADS	 = KEYS * PIECES / (64 * WAVES); // pieces of K, and of V, per thread
-	__shared__ v4u k_tile[2][KEYS * PIECES]; // of tile kt in [kt % 2]
-	__shared__ v4u v_tile[2][D * (KEYS / 8)];
+	struct tiles_of_part {
+		v4u k[2][KEYS * PIECES]; // of tile kt in [kt % 2]
+		v4u v[2][D * (KEYS / 8)];
+	};
+	__shared__ tiles_of_part lds[PARTS];
+	__shared__ not_finite<D> odd;
 
-	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % WAVES, part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / WAVES;
+	auto& k_tile = lds[part].k;
+	auto& v_tile = lds[part].v;
 	const int col = lane & 31, half = lane >> 5;
 	const int group = a.q_heads / a.cache.kv_heads;
 	const int head	= blockIdx.x % a.cache.kv_heads;
@@ -138,7 +145,7 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 	int limit, wave_min, wave_limit; // no row of the tile sees a key from limit on, none of the wave one from wave_limit on, and all of the wave's see those up to wave_min
 	if constexpr (PREFIX) {
 		limit = min(first_key + out.keys, held);
-		pos	  = there ? min(a.batch.lengths[token], limit) - 1 : -1;
+		pos	  = there ? min(max(a.batch.lengths[token], 0), limit) - 1 : -1;
 		wave_min = there ? pos : limit, wave_limit = pos + 1;
 #pragma unroll
 		for (int d = 1; d < 32; d <<= 1) {
@@ -154,46 +161,6 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 		limit				 = max(0, min(held, p.pos0 + last_row / group + 1));
 		wave_min			 = p.pos0 + wave_first / group;
 		wave_limit			 = wave_first < all_rows ? p.pos0 + min(wave_first + 31, all_rows - 1) / group + 1 : 0;
-	}
-
-	// q as the B operand: column = row, values 16 s + 8 half .. + 7
-	vec q[N][STEPS];
-	float c; // scores times c are log2 of the weights
-	{
-		const int64_t at = static_cast<int64_t>(p.first_token + token) * a.q_stride + static_cast<int64_t>(q_head) * D + 8 * half;
-		int e			 = 14;
-		if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
-			float largest = 0.0f;
-#pragma unroll
-			for (int s = 0; s < STEPS; ++s) {
-				float x[8];
-				load_q8<TYPE>(a.q, at + 16 * s, there, x);
-#pragma unroll
-				for (int j = 0; j < 8; ++j) {
-					largest = fmaxf(largest, fabsf(x[j]));
-				}
-			}
-			e = q_exponent<CACHE, TYPE>(fmaxf(largest, swap32(largest)));
-		}
-		const float up = ldexpf(1.0f, 14 - e);
-#pragma unroll
-		for (int s = 0; s < STEPS; ++s) {
-			float x[8];
-			load_q8<TYPE>(a.q, at + 16 * s, there, x);
-			if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
-#pragma unroll
-				for (int j = 0; j < 8; ++j) {
-					x[j] *= up;
-				}
-			}
-			vec t[N];
-			split8<CACHE, N>(x, t);
-#pragma unroll
-			for (int n = 0; n < N; ++n) {
-				q[n][s] = t[n];
-			}
-		}
-		c = ldexpf(a.scale * LOG2_E, e - 14);
 	}
 
 	// Pages: lane i holds that of the 16 keys from 16 i on of the stretch of 1024 keys that a tile is in, -1 where there is none; and the next stretch's.
@@ -241,13 +208,71 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 		}
 	};
 
-	v16f o[DT];
+	// This part's tiles: first_tile .. end_tile - 1; all parts go round as often (the barriers are for all).
+	const int all_tiles	 = max(0, (limit + KEYS - 1) / KEYS - first_key / KEYS), rounds = (all_tiles + PARTS - 1) / PARTS;
+	const int first_tile = first_key / KEYS + part * rounds, end_tile = min(first_tile + rounds, first_key / KEYS + all_tiles);
+	int ids = -1, next_ids = -1, stretch = 0; // that ids are of
+	auto ids_of = [&](int kt) { // kt in the stretch or in the one after
+		return (kt >> 4) == stretch ? ids : next_ids;
+	};
+	auto load_first = [&] {
+		stretch = first_tile >> 4;
+		if (first_tile < end_tile) {
+			ids		 = load_ids(stretch);
+			next_ids = load_ids(stretch + 1);
+			load_k(first_tile, ids_of(first_tile));
+			load_v(first_tile, ids_of(first_tile));
+			if (AHEAD && first_tile + 1 < end_tile) {
+				load_k(first_tile + 1, ids_of(first_tile + 1));
+			}
+		}
+	};
+	load_first();
+
+	// q as the B operand: column = row, values 16 s + 8 half .. + 7
+	vec q[N][STEPS];
+	float c; // scores times c are log2 of the weights
+	{
+		const int64_t at = static_cast<int64_t>(p.first_token + token) * a.q_stride + static_cast<int64_t>(q_head) * D + 8 * half;
+		float x[STEPS][8];
+		float largest = 0.0f;
 #pragma unroll
-	for (int t = 0; t < DT; ++t) {
-		o[t] = v16f{};
+		for (int s = 0; s < STEPS; ++s) {
+			load_q8<TYPE>(a.q, at + 16 * s, there, x[s]);
+		}
+		int e = 14;
+		if constexpr (CACHE == NH_F16 && TYPE == NH_F32) {
+#pragma unroll
+			for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+				for (int j = 0; j < 8; ++j) {
+					largest = fmaxf(largest, fabsf(x[s][j]));
+				}
+			}
+			e			   = q_exponent<CACHE, TYPE>(fmaxf(largest, swap32(largest)));
+			const float up = ldexpf(1.0f, 14 - e);
+#pragma unroll
+			for (int s = 0; s < STEPS; ++s) {
+#pragma unroll
+				for (int j = 0; j < 8; ++j) {
+					x[s][j] *= up;
+				}
+			}
+		}
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			vec t[N];
+			split8<CACHE, N>(x[s], t);
+#pragma unroll
+			for (int n = 0; n < N; ++n) {
+				q[n][s] = t[n];
+			}
+		}
+		c = ldexpf(a.scale * LOG2_E, e - 14);
 	}
-	float m = -__builtin_inff(), l = 0.0f; // what the weights are below (see RISE), this lane's part of the sum of the weights
-	const int first_tile = first_key / KEYS, tiles = (limit + KEYS - 1) / KEYS;
+
+	v16f o[DT];
+	float m, l; // what the weights are below (see RISE), this lane's part of the sum of the weights
 	// scores of tile kt, whose keys are in LDS
 	auto scores = [&](int kt, v16f (&s)[2]) {
 		const v4u* keys = k_tile[kt & 1];
@@ -265,57 +290,62 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 			}
 		}
 	};
-	if (first_tile < tiles) {
-		int ids = load_ids(first_tile >> 4), next_ids = ids;
-		int stretch = first_tile >> 4; // that ids are of
-		// ids for tile kt, of the stretch that kt is in or the one after
-		auto ids_of = [&](int kt) {
-			return (kt >> 4) == stretch ? ids : next_ids;
-		};
-		next_ids = load_ids(stretch + 1);
-		load_k(first_tile, ids_of(first_tile));
-		load_v(first_tile, ids_of(first_tile));
-		if (AHEAD && first_tile + 1 < tiles) {
-			load_k(first_tile + 1, ids_of(first_tile + 1));
+	bool again = false; // see not_finite
+	for (;;) {
+#pragma unroll
+		for (int t = 0; t < DT; ++t) {
+			o[t] = v16f{};
 		}
+		m = -__builtin_inff(), l = 0.0f;
+		const int whole = again ? 0 : limit; // tiles up to here are taken as they are
 		v16f s[2];
-		for (int kt = first_tile; kt < tiles; ++kt) {
-			// Tile kt's values and the next one's keys, asked for an iteration ago, have come, and all waves are through with what they take the place of.
-			asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-			__syncthreads();
-			if (AHEAD && kt == first_tile) {
-				scores(kt, s);
-				__syncthreads();
-			}
+		if constexpr (AHEAD) {
+			asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+		}
+		__syncthreads();
+		if constexpr (AHEAD) {
+			scores(first_tile, s); // (without a tile: of whatever is there, for nothing)
+		}
+		for (int i = 0; i < rounds; ++i) {
+			const int kt		   = first_tile + i;
 			const bool new_stretch = (kt >> 4) != stretch;
 			if (new_stretch) {
 				stretch = kt >> 4;
 				ids		= next_ids;
 			}
-			const int tile_ids = ids;
-			if (kt + 1 + AHEAD < tiles) {
-				load_k(kt + 1 + AHEAD, ids_of(kt + 1 + AHEAD));
-			}
-			if (kt + 1 < tiles) {
-				load_v(kt + 1, ids_of(kt + 1));
-			}
-			if (new_stretch) { // (not needed before the next iteration, whose first wait it is under)
-				next_ids = load_ids(stretch + 1);
-			}
-			const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(tile_ids < 0) >> ((kt & 15) * 4)) & 15u; // groups of 16 keys without a page
-			if (kt * KEYS + KEYS > limit || bad) { // (the same for all waves) values of keys that no row has: nothing, whatever lies there (a weight of zero times infinity is not zero)
-#pragma unroll
-				for (int i = 0; i < LOADS; ++i) {
-					const int at = tid + 64 * WAVES * i, d = at >> 3, x = (at & 7) ^ v_swizzle(d);
-					const int n = ((bad >> (x >> 1)) & 1) ? 0 : limit - (kt * KEYS + 8 * x); // so many of the eight keys are real
-					v4u v = v_tile[kt & 1][at];
+			const uint32_t bad = static_cast<uint32_t>(__builtin_amdgcn_ballot_w64(ids < 0) >> ((kt & 15) * 4)) & 15u; // groups of 16 keys without a page
+			// Tile kt's values and the keys asked for with them an iteration ago have come, and all waves are through with what the next ones take the place of.
+			asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+			const bool mine = PARTS == 1 || kt < end_tile; // (the last round of the second part may have none)
+			if (mine && (kt * KEYS + KEYS > whole || bad)) { // values of keys that no row has: nothing, whatever lies there
+#pragma unroll 1
+				for (int j = 0; j < LOADS; ++j) { // (each wave in what it has loaded itself)
+					const int at = (LOADS * wave + j) * 64 + lane, d = at >> 3, x = (at & 7) ^ v_swizzle(d);
+					const int n	 = ((bad >> (x >> 1)) & 1) ? 0 : limit - (kt * KEYS + 8 * x); // so many of the eight keys are real
+					v4u v		 = v_tile[kt & 1][at];
 #pragma unroll
 					for (int w = 0; w < 4; ++w) {
 						v[w] = n >= 2 * w + 2 ? v[w] : n == 2 * w + 1 ? v[w] & 0xFFFFu : 0u;
 					}
 					v_tile[kt & 1][at] = v;
+					if (again) {
+						odd.template take<CACHE>(reinterpret_cast<uint16_t*>(&v_tile[kt & 1][at]), d, kt * KEYS + 8 * x, 8);
+					}
 				}
-				__syncthreads();
+			}
+			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+			__syncthreads();
+			if (!mine) {
+				continue;
+			}
+			if (kt + 1 + AHEAD < end_tile) {
+				load_k(kt + 1 + AHEAD, ids_of(kt + 1 + AHEAD));
+			}
+			if (kt + 1 < end_tile) {
+				load_v(kt + 1, ids_of(kt + 1));
+			}
+			if (new_stretch) { // (not needed before the next iteration, whose first wait it is under)
+				next_ids = load_ids(stretch + 1);
 			}
 			if (kt * KEYS >= wave_limit) {
 				continue; // (wave-uniform; the barriers are at the top)
@@ -385,12 +415,66 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 				s[0] = next[0], s[1] = next[1];
 			}
 		}
+		float nothing = 0.0f; // NaN if one of them is not finite
+#pragma unroll
+		for (int t = 0; t < DT; ++t) {
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				nothing = fmaf(o[t][i], 0.0f, nothing);
+			}
+		}
+		if (again || !__syncthreads_or(nothing != 0.0f)) {
+			break;
+		}
+		again = true;
+		odd.clear(threadIdx.x, 64 * WAVES * PARTS);
+		load_first();
 	}
-	asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (nothing may still be on its way into LDS when the workgroup ends)
+	l += swap32(l);
+	if constexpr (PARTS == 2) { // the second part's result into the first one's
+		float* const theirs = reinterpret_cast<float*>(lds) + wave * (16 * DT + 2) * 64 + lane;
+		static_assert(sizeof(float) * WAVES * (16 * DT + 2) * 64 <= sizeof(lds), "the second part's results fit where the keys were");
+		__syncthreads();
+		if (part == 1) {
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+				for (int i = 0; i < 16; ++i) {
+					theirs[(16 * dt + i) * 64] = o[dt][i];
+				}
+			}
+			theirs[16 * DT * 64]	   = m;
+			theirs[(16 * DT + 1) * 64] = l;
+		}
+		__syncthreads();
+		if (part == 1) {
+			return;
+		}
+		const float m2 = theirs[16 * DT * 64], l2 = theirs[(16 * DT + 1) * 64];
+		const float both = fmaxf(m, m2), below = both == -__builtin_inff() ? 0.0f : both;
+		const float f1 = exp2_fast(m - below), f2 = exp2_fast(m2 - below);
+		l = l * f1 + l2 * f2;
+		m = both;
+#pragma unroll
+		for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				o[dt][i] = o[dt][i] * f1 + theirs[(16 * dt + i) * 64] * f2;
+			}
+		}
+	}
+	if (again) { // (the last round's barrier is behind the last note)
+#pragma unroll
+		for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+			for (int i = 0; i < 16; ++i) {
+				o[dt][i] += odd.of(32 * dt + 8 * (i >> 2) + 4 * half + (i & 3), pos + 1);
+			}
+		}
+	}
 	if (!there) {
 		return;
 	}
-	l += swap32(l);
 	if constexpr (PREFIX) {
 		const int64_t to = (static_cast<int64_t>(piece) * a.batch.sequences + token) * a.q_heads + q_head;
 		if (half == 0) {
@@ -416,25 +500,35 @@ __global__ __launch_bounds__(64 * WAVES, (terms<CACHE, TYPE>) == 3 ? 1 : 2) void
 	}
 }
 
-template<int CACHE, int TYPE, bool PREFIX> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, int64_t tiles, hipStream_t s) {
+template<int CACHE, int TYPE, int D, bool PREFIX> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, int64_t tiles, bool parts, hipStream_t s) {
 	const dim3 grid(static_cast<unsigned>(tiles * a.cache.kv_heads));
-	if (a.head_dim == 64) {
-		attention_tile_kernel<CACHE, TYPE, 64, PREFIX><<<grid, dim3(64 * WAVES), 0, s>>>(a, out);
-	} else {
-		attention_tile_kernel<CACHE, TYPE, 128, PREFIX><<<grid, dim3(64 * WAVES), 0, s>>>(a, out);
+	constexpr bool FITS = D == 64 || terms<CACHE, TYPE> < 3; // (three terms of 128 values: no registers for a second wave per SIMD)
+	if constexpr (FITS) {
+		if (PREFIX || parts) {
+			attention_tile_kernel<CACHE, TYPE, D, PREFIX, 2><<<grid, dim3(64 * WAVES * 2), 0, s>>>(a, out);
+			return hipGetLastError();
+		}
+	}
+	if constexpr (!FITS || !PREFIX) {
+		attention_tile_kernel<CACHE, TYPE, D, PREFIX, 1><<<grid, dim3(64 * WAVES), 0, s>>>(a, out);
 	}
 	return hipGetLastError();
 }
-template<bool PREFIX> static hipError_t launch_tiles(const attention_args& a, int cache_type, int type, const prefix_out& out, int64_t tiles, hipStream_t s) {
+template<int CACHE, int TYPE, bool PREFIX> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, int64_t tiles, bool parts, hipStream_t s) {
+	return a.head_dim == 64 ? launch_tiles<CACHE, TYPE, 64, PREFIX>(a, out, tiles, parts, s) : launch_tiles<CACHE, TYPE, 128, PREFIX>(a, out, tiles, parts, s);
+}
+template<bool PREFIX> static hipError_t launch_tiles(const attention_args& a, int cache_type, int type, const prefix_out& out, int64_t tiles, bool parts, hipStream_t s) {
 	if (cache_type == NH_F16) {
-		return type == NH_F32 ? launch_tiles<NH_F16, NH_F32, PREFIX>(a, out, tiles, s) : launch_tiles<NH_F16, NH_F16, PREFIX>(a, out, tiles, s);
+		return type == NH_F32 ? launch_tiles<NH_F16, NH_F32, PREFIX>(a, out, tiles, parts, s) : launch_tiles<NH_F16, NH_F16, PREFIX>(a, out, tiles, parts, s);
 	}
-	return type == NH_F32 ? launch_tiles<NH_BF16, NH_F32, PREFIX>(a, out, tiles, s) : launch_tiles<NH_BF16, NH_BF16, PREFIX>(a, out, tiles, s);
+	return type == NH_F32 ? launch_tiles<NH_BF16, NH_F32, PREFIX>(a, out, tiles, parts, s) : launch_tiles<NH_BF16, NH_BF16, PREFIX>(a, out, tiles, parts, s);
 }
 
 hipError_t launch_attention_tiles(const attention_args& a, int cache_type, int type, hipStream_t s) {
 	const int64_t group = a.q_heads / a.cache.kv_heads;
-	return launch_tiles<false>(a, cache_type, type, prefix_out{}, a.rows * group / ROWS + a.batch.sequences, s); // (each sequence adds less than a tile)
+	const int64_t tiles = a.rows * group / ROWS + a.batch.sequences; // (each sequence adds less than a tile)
+	// two parts where there is no more than a workgroup per CU
+	return launch_tiles<false>(a, cache_type, type, prefix_out{}, tiles, tiles * a.cache.kv_heads <= 256, s);
 }
 
 prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64_t prefix_keys) {
@@ -443,13 +537,13 @@ prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64
 		return c;
 	}
 	c.row_tiles			 = (sequences * group + ROWS - 1) / ROWS;
-	const int64_t wanted = std::max<int64_t>(1, 512 / (c.row_tiles * kv_heads)); // two workgroups per CU
-	c.keys				 = ((prefix_keys + wanted - 1) / wanted + KEYS - 1) / KEYS * KEYS;
+	const int64_t wanted = std::max<int64_t>(1, 256 / (c.row_tiles * kv_heads)); // a workgroup of two parts per CU
+	c.keys				 = ((prefix_keys + wanted - 1) / wanted + 2 * KEYS - 1) / (2 * KEYS) * (2 * KEYS);
 	c.pieces			 = (prefix_keys + c.keys - 1) / c.keys;
 	return c;
 }
 hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s) {
-	return launch_tiles<true>(a, cache_type, type, prefix_out{ o, ml, static_cast<int>(cut.keys), static_cast<int>(cut.row_tiles) }, cut.pieces * cut.row_tiles, s);
+	return launch_tiles<true>(a, cache_type, type, prefix_out{ o, ml, static_cast<int>(cut.keys), static_cast<int>(cut.row_tiles) }, cut.pieces * cut.row_tiles, true, s);
 }
 
 } // namespace nh

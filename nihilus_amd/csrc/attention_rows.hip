@@ -158,6 +158,26 @@ template<int D> __device__ __forceinline__ int k_swizzle(int r) {
 	return D == 128 ? (r & 3) | ((r >> 1) & 12) : ((r >> 1) & 1) | ((r >> 2) & 6);
 }
 
+// 64 lanes' 16 bytes each, two or four times over, 1024 bytes further on in memory and in LDS every time (the instruction's offset counts for both), from `offset`
+// bytes behind an address that the wave has.  As load_global_to_lds_b128.
+__device__ __forceinline__ void load_2_to_lds(const void* src, uint32_t o0, uint32_t o1, const void* lds_dst) {
+	const uint32_t lds_addr = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(static_cast<const char*>(lds_dst))));
+	uint32_t saved_m0;
+	asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024\n\ts_mov_b32 m0, %0"
+				 : "=&s"(saved_m0)
+				 : "v"(o0), "v"(o1), "s"(src), "s"(lds_addr)
+				 : "memory");
+}
+__device__ __forceinline__ void load_4_to_lds(const void* src, uint32_t o01, uint32_t o23, const void* lds_dst) {
+	const uint32_t lds_addr = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(static_cast<const char*>(lds_dst))));
+	uint32_t saved_m0;
+	asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %1, %3 offset:1024\n\t"
+				 "global_load_lds_dwordx4 %2, %3 offset:2048\n\tglobal_load_lds_dwordx4 %2, %3 offset:3072\n\ts_mov_b32 m0, %0"
+				 : "=&s"(saved_m0)
+				 : "v"(o01), "v"(o23), "s"(src), "s"(lds_addr)
+				 : "memory");
+}
+
 // a running result and another one, both sums of weights and of weighted values below their own maximum
 struct running {
 	float m, l;
@@ -174,14 +194,15 @@ struct running {
 } // namespace
 
 template<int CACHE, int TYPE, int D>
-__global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const uint16_t* v_pages,
+__global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const int32_t* starts,
 	uint32_t shape, int width, int prefix_count, uint32_t heads, attention_args a, rows_workspace w) {
 	// What the first loads take comes first, in fourteen dwords: those arrive in registers, the rest is read from memory, as far away as the data.
-	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | one row per sequence << 31
+	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | one row per sequence << 31
 	const int kv_heads = heads & 0xFFFF, group = heads >> 16, sequences = shape & 0x1FFFFF, page_shift = (shape >> 21) & 15;
 	const bool one_each = (shape >> 31) != 0;
 	const int all_rows	= one_each ? sequences : a.rows;
-	const batch_view batch{ page_table, lengths, one_each ? nullptr : a.batch.starts, sequences, width };
+	const batch_view batch{ page_table, lengths, one_each ? nullptr : starts, sequences, width };
+	const uint16_t* const v_pages = a.cache.v;
 	using H				 = half_type<CACHE>;
 	using vec			 = typename H::vec;
 	constexpr int N		 = terms<CACHE, TYPE>;
@@ -195,13 +216,14 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	__shared__ v4u q_share[COLUMNS * Q_PIECES];
 	__shared__ float2 join_ml[WAVES][COLUMNS];
 	__shared__ int is_last;
+	__shared__ not_finite<D> odd_of_wave[WAVES];
 
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int col = lane & 15, quarter = lane >> 4;
 	const int q_heads	  = group * kv_heads;
 	const int head		  = blockIdx.x;
 	const int prefix_keys = prefix_count << page_shift, held = width << page_shift;
-	const int unit		  = blockIdx.y, units = gridDim.y;
+	const int unit		  = blockIdx.y, log2_units = (shape >> 25) & 15;
 
 	// The row group's q, a part by each wave: piece x of row r at x ^ (r % 8).  Columns past the last row hold that one again; their results go nowhere.
 	auto load_q = [&](int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
@@ -219,19 +241,30 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
 	// One sequence of one row group: whose q and pages these are is known ahead of its length, so all three are asked for together.
 	const bool single = sequences == 1 && one_each && group <= COLUMNS;
-	int ids			  = page_table[min(lane, max(width, 1) - 1)]; // lane i: page first_id + i of the sequence (the host gives a table that can be read)
-	int first_id	  = 0;
+	const int front	  = page_table[min(lane, max(width, 1) - 1)]; // of the first sequence (the host gives a table that can be read)
+	int ids = front, first_id = 0; // lane i: page first_id + i of the sequence
 	if (single) {
 		load_q(0, head * group, 0, 0.0f, group); // (all of them rows of token 0)
 	}
+	sequence_size z = size_of(batch, all_rows, prefix_keys, held, lane);
+	// Offsets of a step's pieces (see load_step), under the way of what has been asked for so far.
+	uint32_t k_offset[4], v_offset;
+#pragma unroll
+	for (int i = 0; i < 4; ++i) {
+		k_offset[i] = D == 128 ? (lane >> 4) * 256 + 16 * ((lane & 15) ^ (lane >> 4) ^ (4 * i)) : (lane >> 3) * 128 + 16 * ((lane & 7) ^ ((lane >> 4) & 1) ^ (2 * i));
+		asm volatile("" : "+v"(k_offset[i]));
+	}
+	v_offset = 2 * ((lane >> 2) << page_shift) + 16 * ((lane & 3) ^ (lane >> 4));
+	asm volatile("" : "+v"(v_offset));
 	// All work, in steps: 64 sequences at a time, one for each lane.  (Their number is below 2^31: checked on the host.)
-	sequence_size z;
 	int total = 0;
 	for (int base = 0; base < sequences; base += 64) {
-		z = size_of(batch, all_rows, prefix_keys, held, base + lane);
+		if (base > 0) {
+			z = size_of(batch, all_rows, prefix_keys, held, base + lane);
+		}
 		total += sum64(row_groups_of(z, group) * (FIXED + steps_of(z)));
 	}
-	const int share = ((total + units - 1) / units + WAVES - 1) & -WAVES; // of a workgroup
+	const int share = (((total + (1 << log2_units) - 1) >> log2_units) + WAVES - 1) & -WAVES; // of a workgroup
 	int at			= unit * share;
 	const int end	= min(at + share, total);
 	if (at >= end) {
@@ -295,9 +328,13 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 
 	const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
 	const int page_size	 = 1 << page_shift;
-	if (!single || again) {
+	if (p.seq == 0 && end_key <= 64 << page_shift) {
+		ids = front, first_id = 0;
+	} else {
 		first_id = first_key >> page_shift;
 		ids		 = table[min(first_id + lane, max(width, 1) - 1)];
+	}
+	if (!single) { // (a single sequence has one row group: it has been asked for)
 		load_q(p.first_row + first_token, head * group, first_rest, inv_group, count);
 	}
 	// The page of the 16 keys from `key` on, -1 if there is none: of the first 64 pages from a register, of the others from memory.
@@ -308,27 +345,41 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		const int slot = key >> page_shift, id = slot - first_id < 64 ? __builtin_amdgcn_readlane(ids, slot - first_id) : table[slot];
 		return id >= 0 && id < a.cache.pages ? id : -1;
 	};
-	// A step's 32 keys into a slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
+	// A step's 32 keys into the wave's slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
 	// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).
+	// Instruction j holds rows (64 / PIECES) j + lane / PIECES of the keys, whose swizzle is a part of the lane's and one of j's, and columns
+	// 16 j + lane / 4 of the values, whose swizzle is the lane's.
 	const int64_t page_values = static_cast<int64_t>(kv_heads) * D << page_shift, head_values = static_cast<int64_t>(head) * D << page_shift;
 	auto load_step			  = [&](int base, int lo, int hi) {
 		 const int64_t lo_at = max(lo, 0) * page_values + head_values, hi_at = max(hi, 0) * page_values + head_values;
-#pragma unroll
-		 for (int j = 0; j < LOADS; ++j) {
-			 const int at = 64 * j + lane, r = at / PIECES, x = (at % PIECES) ^ k_swizzle<D>(r);
-			 const int key = (base + r) & (page_size - 1);
-			 load_global_to_lds_b128(k_pages + (2 * j < LOADS ? lo_at : hi_at) + key * D + 8 * x, &slots[wave][64 * j]);
+		 const uint16_t* const k_lo = k_pages + lo_at + (base & (page_size - 1)) * D;
+		 const uint16_t* const k_hi = k_pages + hi_at + ((base + 16) & (page_size - 1)) * D;
+		 v4u* const slot			= &slots[wave][0];
+		 if constexpr (D == 128) {
+			 load_4_to_lds(k_lo, k_offset[0], k_offset[1], slot);
+			 load_4_to_lds(k_hi, k_offset[2], k_offset[3], slot + 4 * 64);
+		 } else {
+			 load_2_to_lds(k_lo, k_offset[0], k_offset[1], slot);
+			 load_2_to_lds(k_hi, k_offset[2], k_offset[3], slot + 2 * 64);
 		 }
+		 if (page_shift > 4) { // one page
+			 const uint16_t* const v_lo = v_pages + lo_at + (base & (page_size - 1));
+#pragma unroll
+			 for (int j = 0; j < LOADS; ++j) {
+				 load_global_to_lds_b128(v_lo + ((16 * j) << page_shift), v_offset, slot + STEP * PIECES + 64 * j);
+			 }
+			 return;
+		 }
+		 const int x			 = (lane & 3) ^ (lane >> 4);
+		 const uint16_t* const v = v_pages + (x & 2 ? hi_at : lo_at) + 16 * (lane >> 2) + 8 * (x & 1);
 #pragma unroll
 		 for (int j = 0; j < LOADS; ++j) {
-			 const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 2) & 3);
-			 const int key = (base + 8 * x) & (page_size - 1);
-			 load_global_to_lds_b128(v_pages + (x & 2 ? hi_at : lo_at) + d * page_size + key, &slots[wave][STEP * PIECES + 64 * j]);
+			 load_global_to_lds_b128(v + 256 * j, slot + STEP * PIECES + 64 * j);
 		 }
 	};
 	constexpr int stride = STEP * WAVES;
 	int base			 = first_key + wave * STEP;
-	int lo = page_of(base), hi = page_of(base + 16);
+	int lo = page_of(base), hi = page_shift > 4 ? lo : page_of(base + 16);
 	load_step(base, lo, hi);
 
 	// q as the B operand: column = row, values 32 s + 8 quarter .. + 7
@@ -472,17 +523,57 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		}
 	};
 
+	bool strict = false; // see not_finite
 	while (base < end_key) {
-		const int next = base + stride, next_lo = page_of(next), next_hi = page_of(next + 16);
+		const int next = base + stride, next_lo = page_of(next), next_hi = page_shift > 4 ? next_lo : page_of(next + 16);
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the step is in the slot
+		if (strict) {
+#pragma unroll 1
+			for (int j = 0; j < LOADS; ++j) {
+				const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 2) & 3);
+				odd_of_wave[wave].template take<CACHE>(reinterpret_cast<uint16_t*>(&slots[wave][STEP * PIECES + at]), d, base + 8 * x, (x & 2 ? hi : lo) < 0 ? 0 : end_key - base - 8 * x);
+			}
+		}
 		read_step();
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // ... and out of it
 		__builtin_amdgcn_sched_barrier(0);
 		if (next < end_key) {
 			load_step(next, next_lo, next_hi);
 		}
-		compute(base, lo, hi);
+		if (base >= first_key) {
+			compute(base, lo, hi);
+		}
 		base = next, lo = next_lo, hi = next_hi;
+		if (base >= end_key) {
+			float nothing = 0.0f; // NaN if one of them is not finite
+#pragma unroll
+			for (int t = 0; t < DT; ++t) {
+#pragma unroll
+				for (int i = 0; i < 4; ++i) {
+					nothing = fmaf(o[t][i], 0.0f, nothing);
+				}
+			}
+			if (__builtin_expect(__builtin_amdgcn_ballot_w64(nothing != 0.0f) != 0 || strict, 0)) {
+				if (!strict) { // once more, from a step in front of the first, without a key
+					strict = true;
+					odd_of_wave[wave].clear(lane, 64);
+#pragma unroll
+					for (int t = 0; t < DT; ++t) {
+						o[t] = v4f{};
+					}
+					m = -__builtin_inff(), l = 0.0f;
+					base = first_key + wave * STEP - stride, lo = -1, hi = -1;
+				} else {
+#pragma unroll
+					for (int t = 0; t < DT; ++t) {
+#pragma unroll
+						for (int i = 0; i < 4; ++i) {
+							o[t][i] += odd_of_wave[wave].of(16 * t + 4 * quarter + i, seen);
+						}
+					}
+				}
+			}
+		}
 	}
 	wait_stores_acknowledged(); // (a wave without a step has one on its way all the same)
 
@@ -641,11 +732,14 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 	// (no more workgroups than the tables have keys for, four steps each at least)
 	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : a.rows * group / COLUMNS + sequences;
 	const int64_t steps		 = (static_cast<int64_t>(a.batch.width) << a.cache.page_shift) / STEP + 1 + FIXED;
-	const int64_t units		 = std::max<int64_t>(1, std::min(cut.units, (row_groups * steps + WAVES - 1) / WAVES));
-	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), static_cast<unsigned>(units)), dim3(THREADS), 0, s>>>(a.batch.lengths,
-		a.batch.width > 0 ? a.batch.table : a.batch.lengths, a.q, a.cache.k, a.cache.v,
-		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | (one_each ? 1u << 31 : 0u), a.batch.width, a.prefix_count,
-		static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, a, w);
+	int log2_units			 = 0;
+	while ((2 << log2_units) <= cut.units && (WAVES << log2_units) < row_groups * steps) {
+		++log2_units;
+	}
+	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), 1u << log2_units), dim3(THREADS), 0, s>>>(a.batch.lengths,
+		a.batch.width > 0 ? a.batch.table : a.batch.lengths, a.q, a.cache.k, a.batch.starts,
+		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | static_cast<uint32_t>(log2_units) << 25 | (one_each ? 1u << 31 : 0u), a.batch.width,
+		a.prefix_count, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, a, w);
 	return hipGetLastError();
 }
 template<int CACHE, int TYPE> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {

@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 KINDS = [(F32, F16), (F16, F16), (F32, BF16), (BF16, BF16)]
-NAN = float("nan")
+NAN, INF = float("nan"), float("inf")
 
 
 @pytest.fixture(scope="module")
@@ -645,3 +645,85 @@ def test_tensors_that_are_refused(A, monkeypatch, native):
             A.cache_step(*args)
     with pytest.raises(errors):
         A.cache_compact(k, v, table, dl)
+
+
+def _check_with_odd_values(got, q, k, v, there, scale, dtype, what):
+    """Values that are infinite or NaN reach the rows that see their keys, in their column, and no others."""
+    clean = torch.where(torch.isfinite(v), v, 0.0)
+    ref, mean, d, n = R.attend(q, k, clean, there, scale)
+    group = q.shape[0] // k.shape[0]
+    odd = torch.where(torch.isfinite(v), 0.0, v)[:, there].sum(1).repeat_interleave(group, 0)  # [heads, dim]: 0, an infinity or NaN
+    got = got.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(odd)) and torch.equal(torch.isinf(got), torch.isinf(odd)), what
+    assert torch.equal(got[torch.isinf(odd)], odd[torch.isinf(odd)]), what
+    _check(torch.where(odd == 0, got, ref), ref, mean, d, n, dtype, what)
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_odd_values_of_later_rows(A, kernel, dtype, cache, dim, page):
+    new, cached = [70, 3, 200], [20, 0, 65]
+    b = Batch(17, [a + c for a, c in zip(new, cached)], page, 2, dim, cache)
+    for seq, places in enumerate([[(25, 0, INF), (26, 0, -INF), (40, 1, NAN), (63, 5, INF), (64, 6, -INF), (89, 7, NAN)], [(2, 3, INF)], [(66, 9, -INF), (200, 9, INF), (201, 40, NAN), (264, 63, INF)]]):
+        for j, d, x in places:
+            b.v[b.table[seq][j // page], seq % 2, d, j % page] = x
+    starts = _starts(new)
+    q = b.rows(sum(new), 4, dtype)
+    k, v, table, lengths = b.device()
+    out = A.attention_prompt(q.cuda(), k, v, table, lengths, torch.tensor(starts, dtype=torch.int32).cuda()).cpu()
+    for seq, n in enumerate(new):
+        keys, values, there = b.keys(seq, b.lengths[seq])
+        for i in range(n):
+            seen = cached[seq] + i + 1
+            _check_with_odd_values(out[starts[seq] + i], q[starts[seq] + i], keys[:, :seen], values[:, :seen], there[:seen], dim**-0.5, dtype, (seq, i))
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_odd_values_in_a_prefix_that_some_rows_see_in_part(A, dtype, cache, dim):
+    page, pages = 16, 9
+    lengths = [300, 144, 150, 17, 40, 100, 0, -(2**31), 129, 128]
+    b = Batch(23, lengths, page, 2, dim, cache, shared=pages)
+    for j, d, x in [(16, 0, INF), (30, 0, -INF), (39, 2, NAN), (40, 3, INF), (99, 4, -INF), (128, 5, NAN), (143, 6, INF)]:
+        b.v[b.common[j // page], j % 2, d, j % page] = x
+    q = b.rows(len(lengths), 8, dtype)
+    k, v, table, n = b.device()
+    out = A.attention_decode(q.cuda(), k, v, table, n, prefix_pages=torch.tensor(b.common, dtype=torch.int32).cuda()).cpu()
+    for seq, length in enumerate(lengths):
+        keys, values, there = b.keys(seq, max(length, 0), b.common)
+        _check_with_odd_values(out[seq], q[seq], keys, values, there, dim**-0.5, dtype, seq)
+
+
+def test_a_stretch_of_many_small_pages(A):
+    lengths = [20011, 3]  # pages of 16 keys: a workgroup's stretch has more of them than a wave holds in a register
+    b = Batch(29, lengths, 16, 64, 64, F16)
+    q = b.rows(2, 64, F16)
+    k, v, table, n = b.device()
+    out = A.attention_decode(q.cuda(), k, v, table, n).cpu()
+    for seq, length in enumerate(lengths):
+        ref = R.attend(q[seq], *b.keys(seq, length), 0.125)
+        _check(out[seq], *ref, F16, seq)
+
+
+def test_decode_behind_a_prefix_replayed(A):
+    lengths = [700, 64, 65, 130, 256]
+    b = Batch(31, lengths, 64, 2, 128, F16, shared=1)
+    q = b.rows(5, 8, F32)
+    k, v, table, n = b.device()
+    x, prefix = q.cuda(), torch.tensor(b.common, dtype=torch.int32).cuda()
+    out = torch.empty_like(x)
+    space = A.decode_workspace(5, 8, 2, 128, prefix_pages=1, page_size=64)
+    A.attention_decode(x, k, v, table, n, prefix_pages=prefix, out=out, workspace=space)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        A.attention_decode(x, k, v, table, n, prefix_pages=prefix, out=out, workspace=space)
+    for turn in range(3):
+        q = b.rows(5, 8, F32)
+        x.copy_(q)
+        out.fill_(NAN)
+        graph.replay()
+        got = out.cpu()
+        eager = A.attention_decode(x, k, v, table, n, prefix_pages=prefix).cpu()
+        assert torch.equal(got, eager)
+        for seq, length in enumerate(lengths):
+            _check(got[seq], *R.attend(q[seq], *b.keys(seq, length, b.common), 128**-0.5), F32, (turn, seq))
