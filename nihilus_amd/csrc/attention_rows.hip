@@ -34,10 +34,12 @@ constexpr int COLUMNS	 = 16; // rows of a row group
 constexpr int WORKGROUPS = 512; // that the chip holds at once: two per CU
 // What a row group takes beside its steps (its q, its first step's way, the joins), in steps.
 constexpr int FIXED = 12;
+// A row group is not cut where a piece would have fewer steps than this (or than a whole stretch).
+constexpr int LEAST = 8;
 
 struct rows_workspace {
 	// [slot][columns][D]  a piece's sums of weighted values, and [slot][columns] their maximum (log2) and the sum of the weights; slot = (2 * unit + (1 if the
-	// piece is the first of its row group and does not begin with the unit)) * kv_heads + kv head
+	// piece is the first of its row group)) * kv_heads + kv head
 	float* o;
 	float2* ml;
 	float* prefix_o; // [prefix piece][sequences][q_heads][D]
@@ -50,10 +52,10 @@ struct rows_cut {
 	int64_t units; // workgroups per kv head: a power of two
 	int64_t columns; // rows of a row group that are kept in the workspace
 };
-rows_cut plan_rows(bool one_each, int64_t group, int64_t kv_heads) {
+rows_cut plan_rows(bool one_each, int64_t group, int64_t kv_heads, int64_t row_groups) {
 	rows_cut c{};
 	c.units = 1;
-	while (2 * c.units * kv_heads <= WORKGROUPS) {
+	while (2 * c.units * kv_heads <= (row_groups * kv_heads > WORKGROUPS / 2 ? WORKGROUPS : WORKGROUPS / 2)) {
 		c.units *= 2;
 	}
 	c.columns = one_each ? std::min<int64_t>(group, COLUMNS) : COLUMNS;
@@ -178,6 +180,16 @@ __device__ __forceinline__ void load_4_to_lds(const void* src, uint32_t o01, uin
 				 : "memory");
 }
 
+// the same number, of the lane or of the wave, which the compiler takes for another one
+__device__ __forceinline__ int own(int x) {
+	asm volatile("" : "+v"(x));
+	return x;
+}
+__device__ __forceinline__ int same(int x) {
+	asm volatile("" : "+s"(x));
+	return __builtin_amdgcn_readfirstlane(x);
+}
+
 // a running result and another one, both sums of weights and of weighted values below their own maximum
 struct running {
 	float m, l;
@@ -195,13 +207,13 @@ struct running {
 
 template<int CACHE, int TYPE, int D>
 __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const int32_t* starts,
-	uint32_t shape, int width, int prefix_count, uint32_t heads, attention_args a, rows_workspace w) {
+	uint32_t shape, int first_width, int prefix_count, uint32_t heads, attention_args a, rows_workspace w) {
 	// What the first loads take comes first, in fourteen dwords: those arrive in registers, the rest is read from memory, as far away as the data.
 	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | one row per sequence << 31
-	const int kv_heads = heads & 0xFFFF, group = heads >> 16, sequences = shape & 0x1FFFFF, page_shift = (shape >> 21) & 15;
+	const int first_kv_heads = heads & 0xFFFF, first_group = heads >> 16, sequences = shape & 0x1FFFFF, first_page_shift = (shape >> 21) & 15;
 	const bool one_each = (shape >> 31) != 0;
 	const int all_rows	= one_each ? sequences : a.rows;
-	const batch_view batch{ page_table, lengths, one_each ? nullptr : starts, sequences, width };
+	const batch_view batch{ page_table, lengths, one_each ? nullptr : starts, sequences, first_width };
 	const uint16_t* const v_pages = a.cache.v;
 	using H				 = half_type<CACHE>;
 	using vec			 = typename H::vec;
@@ -218,55 +230,54 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	__shared__ int is_last;
 	__shared__ not_finite<D> odd_of_wave[WAVES];
 
-	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-	const int col = lane & 15, quarter = lane >> 4;
-	const int q_heads	  = group * kv_heads;
+	const int first_lane = threadIdx.x & 63, first_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int head		  = blockIdx.x;
-	const int prefix_keys = prefix_count << page_shift, held = width << page_shift;
+	const int prefix_keys = prefix_count << first_page_shift, held = first_width << first_page_shift;
 	const int unit		  = blockIdx.y, log2_units = (shape >> 25) & 15;
 
 	// The row group's q, a part by each wave: piece x of row r at x ^ (r % 8).  Columns past the last row hold that one again; their results go nowhere.
 	auto load_q = [&](int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
 #pragma unroll
 		for (int j = 0; j < (COLUMNS * Q_PIECES / 64 + WAVES - 1) / WAVES; ++j) {
-			const int part = j * WAVES + wave;
+			const int part = j * WAVES + first_wave;
 			if (part < COLUMNS * Q_PIECES / 64) {
-				const int at = 64 * part + lane, r = at / Q_PIECES, x = (at % Q_PIECES) ^ (r & 7);
+				const int at = 64 * part + first_lane, r = at / Q_PIECES, x = (at % Q_PIECES) ^ (r & 7);
 				const int i = rest + min(r, rows - 1), tok = static_cast<int>((static_cast<float>(i) + 0.5f) * inverse);
-				const int64_t from = (row0 + tok == 0 ? 0 : (row0 + tok) * a.q_stride) + static_cast<int64_t>(head0 + i - tok * group) * D;
+				const int64_t from = (row0 + tok == 0 ? 0 : (row0 + tok) * a.q_stride) + static_cast<int64_t>(head0 + i - tok * first_group) * D;
 				load_global_to_lds_b128(static_cast<const char*>(q_rows) + from * (TYPE == NH_F32 ? 4 : 2) + 16 * x, &q_share[64 * part]);
 			}
 		}
 	};
-	const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
+	const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(first_group));
 	// One sequence of one row group: whose q and pages these are is known ahead of its length, so all three are asked for together.
-	const bool single = sequences == 1 && one_each && group <= COLUMNS;
-	const int front	  = page_table[min(lane, max(width, 1) - 1)]; // of the first sequence (the host gives a table that can be read)
+	const bool single = sequences == 1 && one_each && first_group <= COLUMNS;
+	const int front	  = page_table[min(first_lane, max(first_width, 1) - 1)]; // of the first sequence (the host gives a table that can be read)
 	int ids = front, first_id = 0; // lane i: page first_id + i of the sequence
 	if (single) {
-		load_q(0, head * group, 0, 0.0f, group); // (all of them rows of token 0)
+		load_q(0, head * first_group, 0, 0.0f, first_group); // (all of them rows of token 0)
 	}
-	sequence_size z = size_of(batch, all_rows, prefix_keys, held, lane);
+	sequence_size z = size_of(batch, all_rows, prefix_keys, held, first_lane);
 	// Offsets of a step's pieces (see load_step), under the way of what has been asked for so far.
 	uint32_t k_offset[4], v_offset;
 #pragma unroll
 	for (int i = 0; i < 4; ++i) {
-		k_offset[i] = D == 128 ? (lane >> 4) * 256 + 16 * ((lane & 15) ^ (lane >> 4) ^ (4 * i)) : (lane >> 3) * 128 + 16 * ((lane & 7) ^ ((lane >> 4) & 1) ^ (2 * i));
+		k_offset[i] = D == 128 ? (first_lane >> 4) * 256 + 16 * ((first_lane & 15) ^ (first_lane >> 4) ^ (4 * i)) : (first_lane >> 3) * 128 + 16 * ((first_lane & 7) ^ ((first_lane >> 4) & 1) ^ (2 * i));
 		asm volatile("" : "+v"(k_offset[i]));
 	}
-	v_offset = 2 * ((lane >> 2) << page_shift) + 16 * ((lane & 3) ^ (lane >> 4));
+	v_offset = 2 * ((first_lane >> 2) << first_page_shift) + 16 * ((first_lane & 3) ^ (first_lane >> 4));
 	asm volatile("" : "+v"(v_offset));
 	// All work, in steps: 64 sequences at a time, one for each lane.  (Their number is below 2^31: checked on the host.)
 	int total = 0;
 	for (int base = 0; base < sequences; base += 64) {
 		if (base > 0) {
-			z = size_of(batch, all_rows, prefix_keys, held, base + lane);
+			z = size_of(batch, all_rows, prefix_keys, held, base + first_lane);
 		}
-		total += sum64(row_groups_of(z, group) * (FIXED + steps_of(z)));
+		total += sum64(row_groups_of(z, first_group) * (FIXED + steps_of(z)));
 	}
-	const int share = (((total + (1 << log2_units) - 1) >> log2_units) + WAVES - 1) & -WAVES; // of a workgroup
-	int at			= unit * share;
-	const int end	= min(at + share, total);
+	const int first_share = max((total + (1 << log2_units) - 1) >> log2_units, WAVES); // of a workgroup
+	int at			= unit * first_share;
+	const int end	= min(at + first_share, total);
+	const int least = min(first_share, LEAST);
 	if (at >= end) {
 		wait_stores_acknowledged(); // (nothing may still be on its way into LDS when the workgroup ends)
 		return;
@@ -277,9 +288,9 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	auto find = [&] {
 		for (;;) {
 			if (sequences > 64) {
-				z = size_of(batch, all_rows, prefix_keys, held, chunk + lane);
+				z = size_of(batch, all_rows, prefix_keys, held, chunk + first_lane);
 			}
-			const int groups = row_groups_of(z, group), steps = steps_of(z), work = groups * (FIXED + steps), upto = scan64(work);
+			const int groups = row_groups_of(z, first_group), steps = steps_of(z), work = groups * (FIXED + steps), upto = scan64(work);
 			const uint64_t over = __builtin_amdgcn_ballot_w64(before + upto > at);
 			if (over) {
 				const int src  = __builtin_ctzll(over);
@@ -297,16 +308,44 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			chunk += 64;
 		}
 	};
-	for (bool again = false;; again = true) {
+	// Where a stretch's end at x cuts the row group: at whole turns of the waves.
+	auto cut_at = [&](int x) {
+		return p.begin + ((x - p.begin + WAVES / 2) & -WAVES);
+	};
+	for (bool again = false;;) {
+	// Nothing of what follows is to be worked out ahead of this loop, as the compiler would: it would be kept in far more registers than there are.
+	const int lane = own(first_lane), wave = same(first_wave), group = same(first_group), kv_heads = same(first_kv_heads), page_shift = same(first_page_shift), width = same(first_width);
+	const int head = same(blockIdx.x), unit = same(blockIdx.y), share = same(first_share), held = width << page_shift;
+	const int tid = 64 * wave + lane, col = lane & 15, quarter = lane >> 4, q_heads = group * kv_heads;
 	find();
-	const int segment_end = min(p.begin + p.steps, end), segment_begin = max(at, p.begin);
-	if (segment_begin >= segment_end) { // what the row group takes beside its steps, and the steps themselves are the next unit's
-		wait_stores_acknowledged();
-		return;
+	const int row_group_end = p.begin + p.steps;
+	int segment_begin = p.begin, segment_end = row_group_end;
+	if (at > p.begin) { // (only where the stretch begins)
+		if (at - p.begin >= least) {
+			if (row_group_end - at < least) { // the one in front takes it all
+				at = row_group_end;
+				if (at >= end) {
+					wait_stores_acknowledged();
+					return;
+				}
+				continue;
+			}
+			segment_begin = cut_at(at);
+		}
+	}
+	if (end < row_group_end) {
+		if (end - p.begin < least) { // the next one takes it all
+			wait_stores_acknowledged();
+			return;
+		}
+		if (row_group_end - end >= least) {
+			segment_end = cut_at(end);
+		}
 	}
 	if (again) {
 		__syncthreads(); // (what the last row group left in LDS has been read)
 	}
+	again = true;
 	// the row group's rows: first .. first + count - 1 of the sequence's rows * group
 	const int first = p.row_group * COLUMNS, count = min(COLUMNS, p.rows * group - first);
 	const int first_token = first / group, first_rest = first - first_token * group;
@@ -322,9 +361,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	const int seen	   = min(held, p.pos0 + token + 1);
 	const int all_seen = min(held, p.pos0 + first_token + 1), most_seen = min(held, p.pos0 + token_of(count - 1) + 1);
 	const int first_key = prefix_keys + (segment_begin - p.begin) * STEP, end_key = min(prefix_keys + (segment_end - p.begin) * STEP, most_seen);
-	// the units that the row group is cut over
-	const int first_unit = p.begin >= unit * share ? unit : p.begin / share, last_unit = p.begin + p.steps <= end ? unit : (p.begin + p.steps - 1) / share;
-	const int pieces	 = last_unit - first_unit + 1;
+	// the units that the row group is cut over: the first piece is that of the unit in front of the first cut
+	int first_unit = unit, pieces = 1;
+	if (segment_begin > p.begin || segment_end < row_group_end) {
+		first_unit = (p.begin + least - 1) / share;
+		pieces	   = (row_group_end - least) / share - first_unit + 1;
+	}
 
 	const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
 	const int page_size	 = 1 << page_shift;
@@ -594,7 +636,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	const bool alone	= pieces == 1 && w.prefix_pieces == 0;
 	// the slot of the piece in unit i
 	auto slot_of = [&](int i) {
-		return static_cast<int64_t>(2 * i + (i == first_unit && p.begin > first_unit * share ? 1 : 0)) * kv_heads + head;
+		return static_cast<int64_t>(2 * i + (i == first_unit ? 1 : 0)) * kv_heads + head;
 	};
 	const int64_t slot = slot_of(unit);
 	if (there) {
@@ -613,7 +655,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		const float inv		  = alone ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f; // no key at all: zeros
 		const int64_t out_row = ((static_cast<int64_t>(p.first_row) + token) * q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D;
 #pragma unroll
-		for (int dt = wave; dt < DT; dt += WAVES) {
+		for (int j = 0; j < DT / WAVES; ++j) {
+			const int dt = wave + WAVES * j;
 			v4f v{};
 #pragma unroll
 			for (int x = 0; x < WAVES; ++x) {
@@ -698,8 +741,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		}
 	}
 	}
-	at = segment_end;
-	if (at >= end) {
+	at = row_group_end;
+	if (at >= end) { // (also where its rest is the next unit's)
 		return;
 	}
 	}
@@ -707,7 +750,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 
 rows_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
 	rows_workspace w;
-	const rows_cut cut = plan_rows(one_each, q_heads / kv_heads, kv_heads);
+	const rows_cut cut = plan_rows(one_each, q_heads / kv_heads, kv_heads, WORKGROUPS); // (the most that a call may have)
 	return rows_needs{ lay_out(nullptr, cut, plan_prefix(sequences, q_heads / kv_heads, kv_heads, prefix_keys), sequences, q_heads, kv_heads, head_dim, &w), cut.units * kv_heads * 4 };
 }
 bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t table_keys) {
@@ -718,7 +761,8 @@ bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t 
 template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
 	const int64_t group = a.q_heads / a.cache.kv_heads, sequences = a.batch.sequences;
 	const bool one_each		= a.batch.starts == nullptr;
-	const rows_cut cut		= plan_rows(one_each, group, a.cache.kv_heads);
+	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : a.rows * group / COLUMNS + sequences;
+	const rows_cut cut		= plan_rows(one_each, group, a.cache.kv_heads, row_groups);
 	const prefix_cut prefix = plan_prefix(sequences, group, a.cache.kv_heads, static_cast<int64_t>(a.prefix_count) << a.cache.page_shift);
 	rows_workspace w;
 	(void)lay_out(static_cast<char*>(a.workspace), cut, prefix, sequences, a.q_heads, a.cache.kv_heads, D, &w);
@@ -730,7 +774,6 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 		}
 	}
 	// (no more workgroups than the tables have keys for, four steps each at least)
-	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : a.rows * group / COLUMNS + sequences;
 	const int64_t steps		 = (static_cast<int64_t>(a.batch.width) << a.cache.page_shift) / STEP + 1 + FIXED;
 	int log2_units			 = 0;
 	while ((2 << log2_units) <= cut.units && (WAVES << log2_units) < row_groups * steps) {
