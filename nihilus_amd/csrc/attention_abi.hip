@@ -153,9 +153,11 @@ static int check_heads(int64_t rows, int64_t sequences, int64_t q_heads, int64_t
 
 int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes) {
 	NH_TRY(check_heads(rows, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
-	const nh::rows_needs n = nh::prompt_by_rows(rows, sequences, q_heads, kv_heads) ? nh::attention_rows_needs(sequences, false, q_heads, kv_heads, head_dim, 0) : nh::rows_needs{ 0, 0 };
-	*host_workspace_bytes  = n.workspace;
-	*host_counter_bytes	   = n.counters;
+	const nh::attention_needs n = rows == 0 || sequences == 0 ? nh::attention_needs{ 0, 0 }
+		: nh::prompt_by_rows(rows, sequences, q_heads, kv_heads)  ? nh::attention_rows_needs(sequences, false, q_heads, kv_heads, head_dim, 0)
+																  : nh::attention_tiles_needs(rows, sequences, q_heads, kv_heads, head_dim);
+	*host_workspace_bytes		= n.workspace;
+	*host_counter_bytes			= n.counters;
 	return NH_OK;
 }
 
@@ -174,9 +176,11 @@ int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 	nh::attention_args a = attention(host_cache, host_batch, q, out, rows, q_heads, q_stride, scale);
 	a.workspace			 = workspace;
 	a.counters			 = static_cast<int32_t*>(counters);
-	// (few rows against tables of a billion keys: more work than the rows kernel can number)
-	const bool by_rows = nh::prompt_by_rows(rows, host_batch->sequences, q_heads, host_cache->kv_heads) &&
-		nh::attention_rows_fit(rows, host_batch->sequences, false, q_heads / host_cache->kv_heads, host_batch->table_width * host_cache->page_size);
+	bool by_rows		 = nh::prompt_by_rows(rows, host_batch->sequences, q_heads, host_cache->kv_heads);
+	if (by_rows && !nh::attention_rows_fit(rows, host_batch->sequences, false, q_heads / host_cache->kv_heads, host_batch->table_width * host_cache->page_size)) {
+		by_rows		= false; // few rows against tables of a billion keys: more work than the rows kernel can number; the tile kernel without memory of its own
+		a.workspace = nullptr;
+	}
 	return from_hip(by_rows ? nh::launch_attention_rows(a, host_cache->type, type, as_stream(stream)) : nh::launch_attention_tiles(a, host_cache->type, type, as_stream(stream)));
 }
 
@@ -194,9 +198,9 @@ int nh_attn_decode_needs(int64_t sequences, int64_t q_heads, int64_t kv_heads, i
 	NH_TRY(check_heads(sequences, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
 	NH_REQUIRE(prefix_count >= 0 && page_shift(page_size) > 0, NH_ERR_SHAPE);
 	NH_REQUIRE(prefix_count <= MAX_KEYS / page_size, NH_ERR_TOO_LARGE);
-	const nh::rows_needs n = nh::attention_rows_needs(sequences, true, q_heads, kv_heads, head_dim, prefix_count * page_size);
-	*host_workspace_bytes  = n.workspace;
-	*host_counter_bytes	   = n.counters;
+	const nh::attention_needs n = nh::attention_rows_needs(sequences, true, q_heads, kv_heads, head_dim, prefix_count * page_size);
+	*host_workspace_bytes		= n.workspace;
+	*host_counter_bytes			= n.counters;
 	return NH_OK;
 }
 

@@ -201,10 +201,15 @@ struct attention_args {
 	float scale;
 	const int32_t* prefix_pages; // decode only
 	int prefix_count;
-	void* workspace; // rows kernel only
+	void* workspace;
 	int32_t* counters;
 };
-// The tile kernel (attention_prompt.hip): 128 rows of a sequence at a time, keys and values through LDS.
+// What a kernel takes of the caller's memory, in bytes: its workspace, and counters that are zero before and after every call.
+struct attention_needs {
+	int64_t workspace, counters;
+};
+// The tile kernel (attention_prompt.hip): 128 rows of a sequence at a time.
+attention_needs attention_tiles_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
 hipError_t launch_attention_tiles(const attention_args& a, int cache_type, int type, hipStream_t s);
 // The part of a decode step over a prefix that all sequences share: the batch's rows as tiles, the keys in pieces.
 struct prefix_cut {
@@ -214,10 +219,7 @@ prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64
 // partial results [piece][sequence][q_head]: o unnormalised, ml the running maximum (log2) and the sum of the weights
 hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s);
 // The rows kernel (attention_rows.hip): 16 rows of a sequence at a time, keys and values straight from memory and cut into pieces.
-struct rows_needs {
-	int64_t workspace, counters; // bytes
-};
-rows_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
+attention_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
 // whether all work, in steps of 32 keys, surely has a 32-bit number (table_keys: what a sequence's table has room for)
 bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t table_keys);
 hipError_t launch_attention_rows(const attention_args& a, int cache_type, int type, hipStream_t s);

@@ -44,6 +44,14 @@ __device__ __forceinline__ int v_swizzle(int row) {
 // weights stay below 2^(8 + 7), and after a row's first tiles its results are hardly ever brought below a new one.
 constexpr float RISE = 7.0f;
 
+// Results between workgroups: device scope, past the caches that another XCD does not see.
+__device__ __forceinline__ void put(float* p, float x) {
+	__hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get(const float* p) {
+	return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 struct tile_place {
 	int seq, first_token, tokens, first_row, pos0; // the tile's rows start at first_row of tokens * group; pos0: position of the sequence's first token
 	bool there;
@@ -87,6 +95,17 @@ __device__ __forceinline__ tile_place place_of_tile(const batch_view& b, int row
 
 } // namespace
 
+// Key tiles that a piece of a tile's keys has at least: 512 keys, some 8 us, against the 4 us that writing and joining the pieces take.
+constexpr int PIECE_TILES = 8;
+
+// Where the results of a tile's pieces go, as their lanes hold them: [workgroup][wave][16 DT values, maximum, sum][lane].  counters [tile]: how many of the
+// pieces are done, zero before and after every call.
+struct tile_pieces {
+	float* parts;
+	int32_t* counters;
+	int pieces; // that a tile's workgroups may take
+};
+
 // Where a prefix's partial results go: piece i of the keys, row (b, query head): o [i][b][q_heads][D] unnormalised, ml the maximum and the sum.
 struct prefix_out {
 	float* o;
@@ -95,9 +114,11 @@ struct prefix_out {
 	int row_tiles;
 };
 
+enum tile_kind { WHOLE, IN_PIECES, OVER_PREFIX }; // a workgroup has all of its rows' keys, a piece of them, a piece of the shared prefix
 // PARTS: groups of four waves that have the same rows and a part of the keys each, joined in LDS at the end.
-template<int CACHE, int TYPE, int D, bool PREFIX, int PARTS>
-__global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PARTS == 1 ? 1 : 2) void attention_tile_kernel(attention_args a, prefix_out out) {
+template<int CACHE, int TYPE, int D, int KIND, int PARTS>
+__global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PARTS == 1 ? 1 : 2) void attention_tile_kernel(attention_args a, prefix_out out, tile_pieces cut) {
+	constexpr bool PREFIX = KIND == OVER_PREFIX;
 	using H				= half_type<CACHE>;
 	using vec			= typename H::vec;
 	constexpr int N		= terms<CACHE, TYPE>;
@@ -120,6 +141,7 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 	const int col = lane & 31, half = lane >> 5;
 	const int group = a.q_heads / a.cache.kv_heads;
 	const int head	= blockIdx.x % a.cache.kv_heads;
+	const int pieces = KIND == IN_PIECES ? cut.pieces : 1;
 	tile_place p{};
 	int first_key = 0, piece = 0;
 	if constexpr (PREFIX) {
@@ -128,7 +150,7 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 		first_key	= piece * out.keys;
 		p			= tile_place{ 0, 0, a.batch.sequences, t % out.row_tiles * ROWS, 0, true };
 	} else {
-		p = place_of_tile(a.batch, a.rows, group, blockIdx.x / a.cache.kv_heads);
+		p = place_of_tile(a.batch, a.rows, group, blockIdx.x / a.cache.kv_heads / pieces);
 		if (!p.there) {
 			return;
 		}
@@ -163,6 +185,17 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 		wave_limit			 = wave_first < all_rows ? p.pos0 + min(wave_first + 31, all_rows - 1) / group + 1 : 0;
 	}
 
+	int in_pieces = 1; // so many workgroups have some of the keys
+	if constexpr (KIND == IN_PIECES) {
+		const int all = (limit + KEYS - 1) / KEYS, of_piece = max(PIECE_TILES, (all + pieces - 1) / pieces);
+		piece		  = blockIdx.x / a.cache.kv_heads % pieces;
+		in_pieces	  = max(1, (all + of_piece - 1) / of_piece);
+		if (piece >= in_pieces) {
+			return;
+		}
+		first_key = piece * of_piece * KEYS;
+		limit	  = min(limit, first_key + of_piece * KEYS);
+	}
 	// Pages: lane i holds that of the 16 keys from 16 i on of the stretch of 1024 keys that a tile is in, -1 where there is none; and the next stretch's.
 	auto load_ids = [&](int stretch) {
 		const int slot = (1024 * stretch + 16 * lane) >> a.cache.page_shift;
@@ -463,14 +496,79 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 			}
 		}
 	}
-	if (again) { // (the last round's barrier is behind the last note)
+	auto odd_values_into = [&](v16f (&o)[DT]) {
+		if (again) { // (the last round's barrier is behind the last note)
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+				for (int i = 0; i < 16; ++i) {
+					o[dt][i] += odd.of(32 * dt + 8 * (i >> 2) + 4 * half + (i & 3), pos + 1);
+				}
+			}
+		}
+	};
+	__shared__ int is_last;
+	if (KIND == IN_PIECES && in_pieces > 1) { // (only the first part's waves are still here)
+		const int tile	   = blockIdx.x / a.cache.kv_heads / pieces * a.cache.kv_heads + head;
+		auto of_piece	   = [&](int i) {
+			  return cut.parts + ((static_cast<int64_t>(tile) * pieces + i) * WAVES + wave) * (16 * DT + 2) * 64 + lane;
+		};
+		odd_values_into(o);
+		float* mine = of_piece(piece);
 #pragma unroll
 		for (int dt = 0; dt < DT; ++dt) {
 #pragma unroll
 			for (int i = 0; i < 16; ++i) {
-				o[dt][i] += odd.of(32 * dt + 8 * (i >> 2) + 4 * half + (i & 3), pos + 1);
+				put(mine + (16 * dt + i) * 64, o[dt][i]);
 			}
 		}
+		put(mine + 16 * DT * 64, m);
+		put(mine + (16 * DT + 1) * 64, l);
+		wait_stores_acknowledged();
+		__syncthreads();
+		if (threadIdx.x == 0) {
+			const int done = __hip_atomic_fetch_add(cut.counters + tile, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+			is_last		   = done == in_pieces - 1;
+			if (is_last) {
+				__hip_atomic_store(cut.counters + tile, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+			}
+		}
+		__syncthreads();
+		if (!is_last) {
+			return;
+		}
+		// the pieces in their order, whoever joins them
+		m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+		for (int t = 0; t < DT; ++t) {
+			o[t] = v16f{};
+		}
+#pragma unroll 1
+		for (int j = 0; j < in_pieces; ++j) {
+			const float* other = of_piece(j);
+			const float m2 = get(other + 16 * DT * 64), l2 = get(other + (16 * DT + 1) * 64);
+			v16f o2[DT];
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+				for (int i = 0; i < 16; ++i) {
+					o2[dt][i] = get(other + (16 * dt + i) * 64);
+				}
+			}
+			const float both = fmaxf(m, m2), below = both == -__builtin_inff() ? 0.0f : both;
+			const float f1 = exp2_fast(m - below), f2 = exp2_fast(m2 - below);
+			l = l * f1 + l2 * f2;
+			m = both;
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+				for (int i = 0; i < 16; ++i) {
+					o[dt][i] = o[dt][i] * f1 + o2[dt][i] * f2;
+				}
+			}
+		}
+	} else {
+		odd_values_into(o);
 	}
 	if (!there) {
 		return;
@@ -500,35 +598,57 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 	}
 }
 
-template<int CACHE, int TYPE, int D, bool PREFIX> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, int64_t tiles, bool parts, hipStream_t s) {
-	const dim3 grid(static_cast<unsigned>(tiles * a.cache.kv_heads));
+// How a prompt's tiles are launched: `tiles` is more than there are; two parts where there is no more than a workgroup per CU, and where there are
+// far fewer, pieces.
+struct tiles_cut {
+	int64_t tiles;
+	int pieces;
+	bool parts;
+};
+static tiles_cut plan_tiles(int64_t rows, int64_t sequences, int64_t group, int64_t kv_heads) {
+	tiles_cut c{};
+	c.tiles	 = rows * group / ROWS + sequences; // (each sequence adds less than a tile)
+	c.parts	 = c.tiles * kv_heads <= 320; // (256 with what is counted too many)
+	c.pieces = static_cast<int>(std::min<int64_t>(8, std::max<int64_t>(1, 320 / (c.tiles * kv_heads))));
+	return c;
+}
+attention_needs attention_tiles_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+	const tiles_cut c = plan_tiles(rows, sequences, q_heads / kv_heads, kv_heads);
+	return c.pieces > 1 ? attention_needs{ c.tiles * kv_heads * c.pieces * WAVES * (head_dim / 2 + 2) * 64 * 4, c.tiles * kv_heads * 4 } : attention_needs{ 0, 0 };
+}
+
+template<int CACHE, int TYPE, int D, int KIND> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, const tile_pieces& cut, int64_t tiles, bool parts, hipStream_t s) {
+	const dim3 grid(static_cast<unsigned>(tiles * a.cache.kv_heads * cut.pieces));
 	constexpr bool FITS = D == 64 || terms<CACHE, TYPE> < 3; // (three terms of 128 values: no registers for a second wave per SIMD)
 	if constexpr (FITS) {
-		if (PREFIX || parts) {
-			attention_tile_kernel<CACHE, TYPE, D, PREFIX, 2><<<grid, dim3(64 * WAVES * 2), 0, s>>>(a, out);
+		if (KIND != WHOLE || parts) {
+			attention_tile_kernel<CACHE, TYPE, D, KIND, 2><<<grid, dim3(64 * WAVES * 2), 0, s>>>(a, out, cut);
 			return hipGetLastError();
 		}
 	}
-	if constexpr (!FITS || !PREFIX) {
-		attention_tile_kernel<CACHE, TYPE, D, PREFIX, 1><<<grid, dim3(64 * WAVES), 0, s>>>(a, out);
+	if constexpr (!FITS || KIND == WHOLE) {
+		attention_tile_kernel<CACHE, TYPE, D, KIND, 1><<<grid, dim3(64 * WAVES), 0, s>>>(a, out, cut);
 	}
 	return hipGetLastError();
 }
-template<int CACHE, int TYPE, bool PREFIX> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, int64_t tiles, bool parts, hipStream_t s) {
-	return a.head_dim == 64 ? launch_tiles<CACHE, TYPE, 64, PREFIX>(a, out, tiles, parts, s) : launch_tiles<CACHE, TYPE, 128, PREFIX>(a, out, tiles, parts, s);
+template<int CACHE, int TYPE, int KIND> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, const tile_pieces& cut, int64_t tiles, bool parts, hipStream_t s) {
+	return a.head_dim == 64 ? launch_tiles<CACHE, TYPE, 64, KIND>(a, out, cut, tiles, parts, s) : launch_tiles<CACHE, TYPE, 128, KIND>(a, out, cut, tiles, parts, s);
 }
-template<bool PREFIX> static hipError_t launch_tiles(const attention_args& a, int cache_type, int type, const prefix_out& out, int64_t tiles, bool parts, hipStream_t s) {
+template<int KIND> static hipError_t launch_tiles(const attention_args& a, int cache_type, int type, const prefix_out& out, const tile_pieces& cut, int64_t tiles, bool parts, hipStream_t s) {
 	if (cache_type == NH_F16) {
-		return type == NH_F32 ? launch_tiles<NH_F16, NH_F32, PREFIX>(a, out, tiles, parts, s) : launch_tiles<NH_F16, NH_F16, PREFIX>(a, out, tiles, parts, s);
+		return type == NH_F32 ? launch_tiles<NH_F16, NH_F32, KIND>(a, out, cut, tiles, parts, s) : launch_tiles<NH_F16, NH_F16, KIND>(a, out, cut, tiles, parts, s);
 	}
-	return type == NH_F32 ? launch_tiles<NH_BF16, NH_F32, PREFIX>(a, out, tiles, parts, s) : launch_tiles<NH_BF16, NH_BF16, PREFIX>(a, out, tiles, parts, s);
+	return type == NH_F32 ? launch_tiles<NH_BF16, NH_F32, KIND>(a, out, cut, tiles, parts, s) : launch_tiles<NH_BF16, NH_BF16, KIND>(a, out, cut, tiles, parts, s);
 }
 
 hipError_t launch_attention_tiles(const attention_args& a, int cache_type, int type, hipStream_t s) {
-	const int64_t group = a.q_heads / a.cache.kv_heads;
-	const int64_t tiles = a.rows * group / ROWS + a.batch.sequences; // (each sequence adds less than a tile)
-	// two parts where there is no more than a workgroup per CU
-	return launch_tiles<false>(a, cache_type, type, prefix_out{}, tiles, tiles * a.cache.kv_heads <= 256, s);
+	const tiles_cut c		 = plan_tiles(a.rows, a.batch.sequences, a.q_heads / a.cache.kv_heads, a.cache.kv_heads);
+	const int64_t key_tiles	 = (static_cast<int64_t>(a.batch.width) << a.cache.page_shift) / KEYS + 1;
+	const tile_pieces pieces = { static_cast<float*>(a.workspace), a.counters, static_cast<int>(std::min<int64_t>(c.pieces, std::max<int64_t>(1, key_tiles / PIECE_TILES))) };
+	if (pieces.pieces > 1 && a.workspace != nullptr) {
+		return launch_tiles<IN_PIECES>(a, cache_type, type, prefix_out{}, pieces, c.tiles, true, s);
+	}
+	return launch_tiles<WHOLE>(a, cache_type, type, prefix_out{}, tile_pieces{ nullptr, nullptr, 1 }, c.tiles, c.parts, s);
 }
 
 prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64_t prefix_keys) {
@@ -543,7 +663,8 @@ prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64
 	return c;
 }
 hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s) {
-	return launch_tiles<true>(a, cache_type, type, prefix_out{ o, ml, static_cast<int>(cut.keys), static_cast<int>(cut.row_tiles) }, cut.pieces * cut.row_tiles, true, s);
+	return launch_tiles<OVER_PREFIX>(a, cache_type, type, prefix_out{ o, ml, static_cast<int>(cut.keys), static_cast<int>(cut.row_tiles) }, tile_pieces{ nullptr, nullptr, 1 }, cut.pieces * cut.row_tiles,
+		true, s);
 }
 
 } // namespace nh

@@ -748,10 +748,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	}
 }
 
-rows_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
+attention_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
 	rows_workspace w;
 	const rows_cut cut = plan_rows(one_each, q_heads / kv_heads, kv_heads, WORKGROUPS); // (the most that a call may have)
-	return rows_needs{ lay_out(nullptr, cut, plan_prefix(sequences, q_heads / kv_heads, kv_heads, prefix_keys), sequences, q_heads, kv_heads, head_dim, &w), cut.units * kv_heads * 4 };
+	return attention_needs{ lay_out(nullptr, cut, plan_prefix(sequences, q_heads / kv_heads, kv_heads, prefix_keys), sequences, q_heads, kv_heads, head_dim, &w), cut.units * kv_heads * 4 };
 }
 bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t table_keys) {
 	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : rows * group / COLUMNS + sequences;

@@ -727,3 +727,29 @@ def test_decode_behind_a_prefix_replayed(A):
         assert torch.equal(got, eager)
         for seq, length in enumerate(lengths):
             _check(got[seq], *R.attend(q[seq], *b.keys(seq, length, b.common), 128**-0.5), F32, (turn, seq))
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_few_rows_behind_long_caches(A, kernel, dtype, cache, dim, page):
+    # tiles whose keys are cut into pieces, and others, in one call; twice, for the counters; the same bits each time
+    new, cached = [5, 40, 1, 130, 0], [4000, 0, 700, 1100, 2000]
+    b = Batch(37, [a + c for a, c in zip(new, cached)], page, 1, dim, cache)
+    b.v[b.table[0][3990 // page], 0, 7, 3990 % page] = -INF
+    b.v[b.table[3][1200 // page], 0, 9, 1200 % page] = NAN
+    starts = _starts(new)
+    q = b.rows(sum(new), 4, dtype)
+    k, v, table, lengths = b.device()
+    x, at = q.cuda(), torch.tensor(starts, dtype=torch.int32).cuda()
+    space = A.prompt_workspace(sum(new), len(new), 4, 1, dim)
+    first = A.attention_prompt(x, k, v, table, lengths, at, workspace=space)
+    for _ in range(3):
+        again = A.attention_prompt(x, k, v, table, lengths, at, workspace=space)
+        assert torch.equal(again.view(torch.int16), first.view(torch.int16))
+        assert int(space.counters.abs().sum()) == 0
+    first = first.cpu()
+    for seq, n in enumerate(new):
+        keys, values, there = b.keys(seq, b.lengths[seq])
+        for i in sorted({0, n // 2, n - 1} & set(range(n))):
+            seen = cached[seq] + i + 1
+            _check_with_odd_values(first[starts[seq] + i], q[starts[seq] + i], keys[:, :seen], values[:, :seen], there[:seen], dim**-0.5, dtype, (seq, i))
