@@ -81,15 +81,17 @@ bool nh::prompt_by_rows(int64_t rows, int64_t sequences, int64_t q_heads, int64_
 	if (sequences <= 0 || kv_heads <= 0) {
 		return true;
 	}
-	// The rows kernel reads a sequence's keys again for every 16 rows, but spreads any shape over the chip; the tile kernel reads them for every 128, one
-	// workgroup after the other, and a workgroup's way to its first result is longer.  So: the first while its row groups are all on the chip at once,
-	// or half again as many, or where no tile has more than one.  us, rows | tiles (fp16, 32 / 8 heads of 128 where nothing else is said):
-	//   512 row groups:  a prompt of 256 rows 8.8 | 14.4, behind 1024 keys 22 | 28, behind 8192 keys 114 | 123; 8 of 32 rows 7.0 | 11.6
-	//   1024:            a prompt of 512 rows 19.6 | 18.5, behind 1024 keys 42 | 32, behind 8192 keys 212 | 127; 16 / 2 heads of 64, 64 of 16 rows 9.3 | 8.5
+	// The rows kernel reads a sequence's keys again for every 16 rows, but spreads any shape over the chip; the tile kernel reads them for every 128, and a
+	// workgroup's way to its first result is longer.  So: the first while its row groups are all on the chip at once, or where no tile has more than one.
+	// us, rows | tiles (fp16, 32 / 8 heads of 128 where nothing else is said):
+	//   256 row groups:  a prompt of 128 rows 7.2 | 12.6, behind 1024 keys 19 | 23, behind 8192 keys 63 | 40
+	//   512:             a prompt of 256 rows 8.8 | 14.6, behind 1024 keys 22 | 24, behind 8192 keys 109 | 54; 8 of 32 rows 7.0 | 11.6
+	//   1024:            a prompt of 512 rows 19.6 | 18.5, behind 1024 keys 41 | 28, behind 8192 keys 205 | 89; 16 / 2 heads of 64, 64 of 16 rows 9.3 | 8.5
 	//   2048:            8 prompts of 128 rows 22 | 12.5, 64 of 16 rows 19 | 12; but 32 / 32 heads, 64 of 16 rows, each tile with one row group: 21 | 33
+	// (How many keys there are is not known on the host: a table has room for more.)
 	const int64_t each = (rows + sequences - 1) / sequences * (q_heads / kv_heads); // the lengths are not known here: as if all were alike
 	const int64_t row_groups = sequences * kv_heads * ((each + 15) / 16), tiles = sequences * kv_heads * ((each + 127) / 128);
-	return row_groups <= 768 || row_groups <= tiles;
+	return row_groups <= 512 || row_groups <= tiles;
 }
 
 extern "C" {

@@ -619,6 +619,28 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	}
 	wait_stores_acknowledged(); // (a wave without a step has one on its way all the same)
 
+	// The pieces of the shared prefix, whose results the first piece of the row group takes in, a part by each wave.
+	if (w.prefix_pieces > 0 && segment_begin == p.begin) {
+		const int64_t row = static_cast<int64_t>(p.seq) * q_heads + q_head, rows = static_cast<int64_t>(sequences) * q_heads;
+#pragma unroll 2
+		for (int i = wave; i < w.prefix_pieces; i += WAVES) {
+			const float2 ml = w.prefix_ml[i * rows + row];
+			const float* from = w.prefix_o + (i * rows + row) * D + 4 * quarter;
+			v4f x[DT];
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) {
+				x[dt] = *reinterpret_cast<const v4f*>(from + 16 * dt);
+			}
+			const float both = fmaxf(m, ml.x), below = both == -__builtin_inff() ? 0.0f : both;
+			const float f1 = exp2_fast(m - below), f2 = exp2_fast(ml.x - below);
+			m = both;
+			l = l * f1 + (quarter == 0 ? ml.y * f2 : 0.0f); // (l is added up over the quarters below)
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) {
+				o[dt] = o[dt] * f1 + x[dt] * f2;
+			}
+		}
+	}
 	// the four waves' results into one: a thread takes four values of a row at a time
 	v4f(*join_o)[DT][64] = reinterpret_cast<v4f(*)[DT][64]>(&slots[0][0]);
 	static_assert(sizeof(v4f) * WAVES * DT * 64 <= sizeof(slots), "the waves' results fit where the keys were");
@@ -633,7 +655,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		join_ml[wave][col] = make_float2(m, l);
 	}
 	__syncthreads();
-	const bool alone	= pieces == 1 && w.prefix_pieces == 0;
+	const bool alone = pieces == 1;
 	// the slot of the piece in unit i
 	auto slot_of = [&](int i) {
 		return static_cast<int64_t>(2 * i + (i == first_unit ? 1 : 0)) * kv_heads + head;
@@ -672,32 +694,29 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			put2(w.ml + slot * w.columns + col, make_float2(top, sum));
 		}
 	}
-	bool join = !alone;
-	if (join) {
+	bool join = false;
+	if (!alone) {
 		wait_stores_acknowledged();
 		__syncthreads();
-		if (pieces > 1) {
-			if (tid == 0) {
-				int32_t* counter = w.counters + first_unit * kv_heads + head;
-				const int done	 = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-				is_last			 = done == pieces - 1;
-				if (is_last) {
-					__hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
-				}
+		if (tid == 0) {
+			int32_t* counter = w.counters + first_unit * kv_heads + head;
+			const int done	 = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+			is_last			 = done == pieces - 1;
+			if (is_last) {
+				__hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
 			}
-			__syncthreads();
-			join = is_last != 0;
 		}
+		__syncthreads();
+		join = is_last != 0;
 	}
 	if (join) {
-	// Joins the row group's pieces, those over the shared prefix first: D / 4 threads to a row, the pieces of few rows over what threads are left.
+	// Joins the row group's pieces: D / 4 threads to a row, the pieces of few rows over what threads are left.
 	constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
 	running* parts		= reinterpret_cast<running*>(&slots[0][0]); // [GROUPS][LANES]
 	static_assert(sizeof(running) * THREADS <= sizeof(slots), "the parts of the join fit where the waves' results were");
 	const int part = tid % LANES, g = tid / LANES;
 	const int rows_at_once = count <= 1 ? 1 : count <= 2 ? 2 : count <= 4 ? 4 : 8; // a divisor of GROUPS
 	const int ways = GROUPS / rows_at_once, way = g / rows_at_once;
-	const int all = w.prefix_pieces + pieces;
 	for (int r0 = 0; r0 < count; r0 += rows_at_once) {
 		const int r		  = r0 + g % rows_at_once;
 		const bool mine	  = r < count;
@@ -705,24 +724,21 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		const int q_h	  = head * group + first + min(r, count - 1) - tok * group;
 		running sum{ -__builtin_inff(), 0.0f, v4f{} };
 		if (mine) {
-			for (int i0 = way; i0 < all; i0 += 4 * ways) {
+			for (int i0 = way; i0 < pieces; i0 += 4 * ways) {
 				const float2* ml[4];
 				const float* o4[4];
 				float2 got_ml[4];
 				v4f got_o[4];
 #pragma unroll
 				for (int k = 0; k < 4; ++k) {
-					const int i		  = min(i0 + k * ways, all - 1); // (past the last one: the last one again, not added)
-					const bool shared = i < w.prefix_pieces;
-					const int64_t at  = shared ? (static_cast<int64_t>(i) * sequences + p.seq) * q_heads + q_h
-											   : slot_of(first_unit + i - w.prefix_pieces) * w.columns + r;
-					ml[k]			  = (shared ? w.prefix_ml : w.ml) + at;
-					o4[k]			  = (shared ? w.prefix_o : w.o) + at * D + 4 * part;
+					const int64_t at = slot_of(first_unit + min(i0 + k * ways, pieces - 1)) * w.columns + r; // (past the last one: the last one again, not added)
+					ml[k]			 = w.ml + at;
+					o4[k]			 = w.o + at * D + 4 * part;
 				}
 				get_parts(ml, o4, got_ml, got_o);
 #pragma unroll
 				for (int k = 0; k < 4; ++k) {
-					if (i0 + k * ways < all) {
+					if (i0 + k * ways < pieces) {
 						sum.add(got_ml[k].x, got_ml[k].y, got_o[k]);
 					}
 				}
@@ -732,7 +748,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		parts[tid] = sum;
 		__syncthreads();
 		if (mine && way == 0) {
-			for (int i = 1; i < min(ways, all); ++i) {
+			for (int i = 1; i < min(ways, pieces); ++i) {
 				const running& other = parts[tid + i * rows_at_once * LANES];
 				sum.add(other.m, other.l, other.o);
 			}
