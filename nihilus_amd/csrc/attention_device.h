@@ -59,14 +59,14 @@ template<int CACHE, int N> __device__ __forceinline__ void split8(const float (&
 __device__ __forceinline__ float exp2_fast(float x) {
 	return __builtin_amdgcn_exp2f(x); // v_exp_f32: 1 ulp; arguments here are <= 0, results below 2^-126 are flushed, far under a sum that holds a 1
 }
-// the larger / the sum of this lane's value and that of lane ^ 32 (^ 16)
-__device__ __forceinline__ float swap32(float x) {
+// the value of lane ^ 32 (^ 16)
+__device__ __forceinline__ float swap32(float x, int lane) {
 	const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
-	return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+	return __builtin_bit_cast(float, (lane & 32) ? r[0] : r[1]);
 }
-__device__ __forceinline__ float swap16(float x) {
+__device__ __forceinline__ float swap16(float x, int lane) {
 	const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
-	return __builtin_bit_cast(float, (threadIdx.x & 16) ? r[0] : r[1]);
+	return __builtin_bit_cast(float, (lane & 16) ? r[0] : r[1]);
 }
 
 // One layer's pages as the kernels see them.

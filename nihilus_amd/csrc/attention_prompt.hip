@@ -290,7 +290,7 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 					largest = fmaxf(largest, fabsf(x[s][j]));
 				}
 			}
-			e			   = q_exponent<CACHE, TYPE>(fmaxf(largest, swap32(largest)));
+			e			   = q_exponent<CACHE, TYPE>(fmaxf(largest, swap32(largest, lane)));
 			const float up = ldexpf(1.0f, 14 - e);
 #pragma unroll
 			for (int s = 0; s < STEPS; ++s) {
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 			for (int i = 1; i < 32; ++i) {
 				top = fmaxf(top, s[i >> 4][i & 15]);
 			}
-			top = fmaxf(top, swap32(top)) * c;
+			top = fmaxf(top, swap32(top, lane)) * c;
 			if (__builtin_amdgcn_ballot_w64(top > m + RISE)) { // a larger maximum: what there is so far is brought below it
 				const float m_new = fmaxf(m, top);
 				const float f	  = exp2_fast(m - (m_new == -__builtin_inff() ? 0.0f : m_new));
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 		odd.clear(threadIdx.x, 64 * WAVES * PARTS);
 		load_first();
 	}
-	l += swap32(l);
+	l += swap32(l, lane);
 	if constexpr (PARTS == 2) { // the second part's result into the first one's
 		float* const theirs = reinterpret_cast<float*>(lds) + wave * (16 * DT + 2) * 64 + lane;
 		static_assert(sizeof(float) * WAVES * (16 * DT + 2) * 64 <= sizeof(lds), "the second part's results fit where the keys were");

@@ -118,9 +118,6 @@ __device__ __forceinline__ sequence_size size_of(const batch_view& b, int all_ro
 	return z;
 }
 
-__device__ __forceinline__ int sum64(int x) {
-	return __builtin_amdgcn_readlane(scan64(x), 63);
-}
 // Steps of a row group of a sequence: one, without a key, if it has none.
 __device__ __forceinline__ int steps_of(const sequence_size& z) {
 	return max(1, (z.keys + STEP - 1) / STEP);
@@ -212,16 +209,22 @@ struct running {
 
 } // namespace
 
+// The kernel's arguments behind the ones that arrive in registers.
+struct rows_args {
+	attention_args a;
+	rows_workspace w;
+};
+constexpr int ROWS_ARGS_AT = 5 * 8 + 4 * 4; // where they are among all of them
+
 template<int CACHE, int TYPE, int D>
 __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const int32_t* starts,
-	uint32_t shape, int first_width, int prefix_count, uint32_t heads, attention_args a, rows_workspace w) {
+	uint32_t shape, int first_width, int prefix_or_rows, uint32_t heads, rows_args) {
 	// What the first loads take comes first, in fourteen dwords: those arrive in registers, the rest is read from memory, as far away as the data.
 	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | one row per sequence << 31
 	const int first_kv_heads = heads & 0xFFFF, first_group = heads >> 16, sequences = shape & 0x1FFFFF, first_page_shift = (shape >> 21) & 15;
 	const bool one_each = (shape >> 31) != 0;
-	const int all_rows	= one_each ? sequences : a.rows;
+	const int all_rows	= one_each ? sequences : prefix_or_rows, prefix_count = one_each ? prefix_or_rows : 0; // (only a decode step has a prefix)
 	const batch_view batch{ page_table, lengths, one_each ? nullptr : starts, sequences, first_width };
-	const uint16_t* const v_pages = a.cache.v;
 	using H				 = half_type<CACHE>;
 	using vec			 = typename H::vec;
 	constexpr int N		 = terms<CACHE, TYPE>;
@@ -238,30 +241,28 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	__shared__ not_finite<D> odd_of_wave[WAVES];
 
 	const int first_lane = threadIdx.x & 63, first_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const int head		  = blockIdx.x;
 	const int prefix_keys = prefix_count << first_page_shift, held = first_width << first_page_shift;
-	const int unit		  = blockIdx.y, log2_units = (shape >> 25) & 15;
+	const int log2_units  = (shape >> 25) & 15;
 
 	// The row group's q, a part by each wave: piece x of row r at x ^ (r % 8).  Columns past the last row hold that one again; their results go nowhere.
-	auto load_q = [&](int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
+	auto load_q = [&](int lane, int wave, int group, int64_t stride, int row0, int head0, int rest, float inverse, int rows) { // row i: token row0 + (rest + i) / group, head head0 + (rest + i) % group
 #pragma unroll
 		for (int j = 0; j < (COLUMNS * Q_PIECES / 64 + WAVES - 1) / WAVES; ++j) {
-			const int part = j * WAVES + first_wave;
+			const int part = j * WAVES + wave;
 			if (part < COLUMNS * Q_PIECES / 64) {
-				const int at = 64 * part + first_lane, r = at / Q_PIECES, x = (at % Q_PIECES) ^ (r & 7);
+				const int at = 64 * part + lane, r = at / Q_PIECES, x = (at % Q_PIECES) ^ (r & 7);
 				const int i = rest + min(r, rows - 1), tok = static_cast<int>((static_cast<float>(i) + 0.5f) * inverse);
-				const int64_t from = (row0 + tok == 0 ? 0 : (row0 + tok) * a.q_stride) + static_cast<int64_t>(head0 + i - tok * first_group) * D;
+				const int64_t from = (row0 + tok) * stride + static_cast<int64_t>(head0 + i - tok * group) * D;
 				load_global_to_lds_b128(static_cast<const char*>(q_rows) + from * (TYPE == NH_F32 ? 4 : 2) + 16 * x, &q_share[64 * part]);
 			}
 		}
 	};
-	const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(first_group));
 	// One sequence of one row group: whose q and pages these are is known ahead of its length, so all three are asked for together.
 	const bool single = sequences == 1 && one_each && first_group <= COLUMNS;
 	const int front	  = page_table[min(first_lane, max(first_width, 1) - 1)]; // of the first sequence (the host gives a table that can be read)
 	int ids = front, first_id = 0; // lane i: page first_id + i of the sequence
 	if (single) {
-		load_q(0, head * first_group, 0, 0.0f, first_group); // (all of them rows of token 0)
+		load_q(first_lane, first_wave, first_group, 0, 0, blockIdx.x * first_group, 0, 0.0f, first_group); // (all of them rows of token 0)
 	}
 	sequence_size z = size_of(batch, all_rows, prefix_keys, held, first_lane);
 	// Offsets of a step's pieces (see load_step), under the way of what has been asked for so far.
@@ -274,15 +275,20 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	v_offset = 2 * ((first_lane >> 2) << first_page_shift) + 16 * ((first_lane & 3) ^ (first_lane >> 4));
 	asm volatile("" : "+v"(v_offset));
 	// All work, in steps: 64 sequences at a time, one for each lane.  (Their number is below 2^31: checked on the host.)
-	int total = 0;
-	for (int base = 0; base < sequences; base += 64) {
-		if (base > 0) {
-			z = size_of(batch, all_rows, prefix_keys, held, base + first_lane);
-		}
-		total += sum64(row_groups_of(z, first_group) * (FIXED + steps_of(z)));
+	int steps, work, upto; // of the lane's sequence: steps of a row group, work of all, work up to its end from the lane 0's start on
+	auto add_up = [&](int group) {
+		steps = steps_of(z);
+		work  = row_groups_of(z, group) * (FIXED + steps);
+		upto  = scan64(work);
+		return __builtin_amdgcn_readlane(upto, 63);
+	};
+	int total = add_up(first_group);
+	for (int base = 64; base < sequences; base += 64) {
+		z = size_of(batch, all_rows, prefix_keys, held, base + first_lane);
+		total += add_up(first_group);
 	}
 	const int first_share = max((total + (1 << log2_units) - 1) >> log2_units, WAVES); // of a workgroup
-	int at			= unit * first_share;
+	int at			= blockIdx.y * first_share;
 	const int end	= min(at + first_share, total);
 	const int least = min(first_share, LEAST);
 	if (at >= end) {
@@ -292,12 +298,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	// where the stretch begins
 	int chunk = 0, before = 0; // the lanes' sequences are chunk .. chunk + 63; work in front of them
 	segment p{};
-	auto find = [&] {
+	auto find = [&](int lane, int group) {
 		for (;;) {
 			if (sequences > 64) {
-				z = size_of(batch, all_rows, prefix_keys, held, chunk + first_lane);
+				z = size_of(batch, all_rows, prefix_keys, held, chunk + lane);
+				add_up(group);
 			}
-			const int groups = row_groups_of(z, first_group), steps = steps_of(z), work = groups * (FIXED + steps), upto = scan64(work);
 			const uint64_t over = __builtin_amdgcn_ballot_w64(before + upto > at);
 			if (over) {
 				const int src  = __builtin_ctzll(over);
@@ -324,7 +330,19 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		const int lane = own(first_lane), wave = same(first_wave), group = same(first_group), kv_heads = same(first_kv_heads), page_shift = same(first_page_shift), width = same(first_width);
 		const int head = same(blockIdx.x), unit = same(blockIdx.y), share = same(first_share), held = width << page_shift;
 		const int tid = 64 * wave + lane, col = lane & 15, quarter = lane >> 4, q_heads = group * kv_heads;
-		find();
+		// (the other arguments are read here and no earlier, where the compiler would wait for them in front of the lengths)
+		const auto at_args = reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr()) + ROWS_ARGS_AT;
+		const auto& late   = *reinterpret_cast<const __attribute__((address_space(4))) rows_args*>(static_cast<uintptr_t>(static_cast<uint32_t>(same(static_cast<int>(at_args)))) |
+			static_cast<uintptr_t>(static_cast<uint32_t>(same(static_cast<int>(at_args >> 32)))) << 32);
+		const auto& a = late.a;
+		const auto& w = late.w;
+		const uint16_t* const v_pages = a.cache.v;
+		const int64_t q_stride		  = a.q_stride;
+		const int cache_pages_here	  = a.cache.pages;
+		const float scale			  = a.scale;
+		const int prefix_pieces_here  = w.prefix_pieces;
+		find(lane, group);
+		const int cache_pages = same(cache_pages_here), prefix_pieces = same(prefix_pieces_here);
 		const int row_group_end = p.begin + p.steps;
 		int segment_begin = p.begin, segment_end = row_group_end;
 		if (at > p.begin) { // (only where the stretch begins)
@@ -353,9 +371,20 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			__syncthreads(); // (what the last row group left in LDS has been read)
 		}
 		again = true;
+		// The pages of its first keys (in registers already if they are the first sequence's first), asked for ahead of everything else: the keys wait for them.
+		const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
+		const int first_key	 = prefix_keys + (segment_begin - p.begin) * STEP;
+		if (p.seq == 0 && prefix_keys + (segment_end - p.begin) * STEP <= 64 << page_shift) {
+			ids = front, first_id = 0;
+		} else {
+			first_id = first_key >> page_shift;
+			ids		 = table[min(first_id + lane, max(width, 1) - 1)];
+		}
+		__builtin_amdgcn_sched_barrier(0);
 		// the row group's rows: first .. first + count - 1 of the sequence's rows * group
+		const float inv_group = __builtin_amdgcn_rcpf(static_cast<float>(group));
 		const int first = p.row_group * COLUMNS, count = min(COLUMNS, p.rows * group - first);
-		const int first_token = first / group, first_rest = first - first_token * group;
+		const int first_token = p.row_group == 0 ? 0 : first / group, first_rest = first - first_token * group;
 		// the token of the group's row i: (first + i) / group, as first_token + (first_rest + i) / group, whose numerator is below 2^17: exact in fp32, half a
 		// numerator's step away from the next whole number
 		auto token_of = [&](int i) {
@@ -367,7 +396,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		// keys: the sequence's own ones that the lane's row sees end at `seen`, those that some row of the group sees at most_seen, that all see at all_seen
 		const int seen	   = min(held, p.pos0 + token + 1);
 		const int all_seen = min(held, p.pos0 + first_token + 1), most_seen = min(held, p.pos0 + token_of(count - 1) + 1);
-		const int first_key = prefix_keys + (segment_begin - p.begin) * STEP, end_key = min(prefix_keys + (segment_end - p.begin) * STEP, most_seen);
+		const int end_key = min(prefix_keys + (segment_end - p.begin) * STEP, most_seen);
 		// the units that the row group is cut over: the first piece is that of the unit in front of the first cut
 		int first_unit = unit, pieces = 1;
 		if (segment_begin > p.begin || segment_end < row_group_end) {
@@ -375,16 +404,9 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			pieces	   = (row_group_end - least) / share - first_unit + 1;
 		}
 
-		const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
-		const int page_size	 = 1 << page_shift;
-		if (p.seq == 0 && end_key <= 64 << page_shift) {
-			ids = front, first_id = 0;
-		} else {
-			first_id = first_key >> page_shift;
-			ids		 = table[min(first_id + lane, max(width, 1) - 1)];
-		}
+		const int page_size = 1 << page_shift;
 		if (!single) { // (a single sequence has one row group: it has been asked for)
-			load_q(p.first_row + first_token, head * group, first_rest, inv_group, count);
+			load_q(lane, wave, group, q_stride, p.first_row + first_token, head * group, first_rest, inv_group, count);
 		}
 		// The page of the 16 keys from `key` on, -1 if there is none: of the first 64 pages from a register, of the others from memory.
 		auto page_of = [&](int key) {
@@ -392,7 +414,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 				return -1;
 			}
 			const int slot = key >> page_shift, id = slot - first_id < 64 ? __builtin_amdgcn_readlane(ids, slot - first_id) : table[slot];
-			return id >= 0 && id < a.cache.pages ? id : -1;
+			return id >= 0 && id < cache_pages ? id : -1;
 		};
 		// A step's 32 keys into the wave's slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
 		// of a quad make one request of it (straight into the operand's registers consecutive lanes are different rows: that took 2.6 us for a step).
@@ -458,8 +480,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			}
 			int e = 14;
 			if constexpr (TYPE == NH_F32) {
-				largest		   = fmaxf(largest, swap16(largest));
-				largest		   = fmaxf(largest, swap32(largest));
+				largest		   = fmaxf(largest, swap16(largest, lane));
+				largest		   = fmaxf(largest, swap32(largest, lane));
 				e			   = q_exponent<CACHE, TYPE>(largest);
 				const float up = ldexpf(1.0f, 14 - e);
 #pragma unroll
@@ -478,7 +500,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 					}
 				}
 			}
-			c = ldexpf(a.scale * LOG2_E, e - 14);
+			c = ldexpf(scale * LOG2_E, e - 14);
 		}
 
 		v4f o[DT];
@@ -541,8 +563,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 				}
 			}
 			float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-			top		  = fmaxf(top, swap16(top));
-			top		  = fmaxf(top, swap32(top)) * c;
+			top		  = fmaxf(top, swap16(top, lane));
+			top		  = fmaxf(top, swap32(top, lane)) * c;
 			const float m_new = fmaxf(m, top);
 			const float below = m_new == -__builtin_inff() ? 0.0f : m_new; // (no key yet: every weight is 2^-inf)
 			if (__builtin_amdgcn_ballot_w64(m_new != m)) {
@@ -627,10 +649,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		wait_stores_acknowledged(); // (a wave without a step has one on its way all the same)
 
 		// The pieces of the shared prefix, whose results the first piece of the row group takes in, a part by each wave.
-		if (w.prefix_pieces > 0 && segment_begin == p.begin) {
+		if (prefix_pieces > 0 && segment_begin == p.begin) {
 			const int64_t row = static_cast<int64_t>(p.seq) * q_heads + q_head, rows = static_cast<int64_t>(sequences) * q_heads;
 #pragma unroll 2
-			for (int i = wave; i < w.prefix_pieces; i += WAVES) {
+			for (int i = wave; i < prefix_pieces; i += WAVES) {
 				const float2 ml = w.prefix_ml[i * rows + row];
 				const float* from = w.prefix_o + (i * rows + row) * D + 4 * quarter;
 				v4f x[DT];
@@ -651,8 +673,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		// the four waves' results into one: a thread takes four values of a row at a time
 		v4f(*join_o)[DT][64] = reinterpret_cast<v4f(*)[DT][64]>(&slots[0][0]);
 		static_assert(sizeof(v4f) * WAVES * DT * 64 <= sizeof(slots), "the waves' results fit where the keys were");
-		l += swap16(l);
-		l += swap32(l);
+		l += swap16(l, lane);
+		l += swap32(l, lane);
 		__syncthreads(); // (every wave is through with its slots)
 #pragma unroll
 		for (int dt = 0; dt < DT; ++dt) {
@@ -681,8 +703,8 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 				f[x] = exp2_fast(ml[x].x - at);
 				sum += ml[x].y * f[x];
 			}
-			const float inv		  = alone ? (sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f) : 1.0f; // no key at all: zeros
-			const int64_t out_row = ((static_cast<int64_t>(p.first_row) + token) * q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D;
+			const float inv		  = sum > 0.0f || sum != sum ? __builtin_amdgcn_rcpf(sum) : 0.0f; // (within 2^-23; no key at all: zeros)
+			const int64_t out_row = static_cast<int64_t>((p.first_row + token) * q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D; // (rows * q_heads <= 2^30)
 #pragma unroll
 			for (int j = 0; j < DT / WAVES; ++j) {
 				const int dt = wave + WAVES * j;
@@ -805,7 +827,7 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), 1u << log2_units), dim3(THREADS), 0, s>>>(a.batch.lengths,
 		a.batch.width > 0 ? a.batch.table : a.batch.lengths, a.q, a.cache.k, a.batch.starts,
 		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | static_cast<uint32_t>(log2_units) << 25 | (one_each ? 1u << 31 : 0u), a.batch.width,
-		a.prefix_count, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, a, w);
+		one_each ? a.prefix_count : a.rows, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, rows_args{ a, w });
 	return hipGetLastError();
 }
 template<int CACHE, int TYPE> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
