@@ -37,9 +37,10 @@ constexpr int COLUMNS	 = 16; // rows of a row group
 constexpr int WORKGROUPS = 512; // that the chip holds at once: two per CU
 // What a row group takes beside its steps (its q, its first step's way, the joins), in steps.  (64 sequences of up to 8192 tokens, and those of up to 600 behind a
 // shared prefix of 8192: 8 steps 54.6 and 53.2 us, 12: 55.4 and 50.4, 20: 57.2 and 53.7.)
-constexpr int FIXED = 12;
-// A row group is not cut where a piece would have fewer steps than this (or than a whole stretch).  (64 sequences of up to 8192 tokens: 8 steps 57.1 us, 24: 58.6;
-// 16 of 256, behind 4096 shared keys: alike.)
+constexpr int FIXED = 8;
+// A row group of fewer steps than WHOLE is not cut (one sequence of 256 tokens: 4.7 us, in two pieces 6.1; of 512 in four 6.3, whole 6.5), others not where a piece
+// would have fewer than LEAST, or than a whole stretch (64 sequences of up to 8192 tokens: 8 steps 57.1 us, 24: 58.6).
+constexpr int WHOLE = 14;
 constexpr int LEAST = 8;
 
 struct rows_workspace {
@@ -275,11 +276,13 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	v_offset = 2 * ((first_lane >> 2) << first_page_shift) + 16 * ((first_lane & 3) ^ (first_lane >> 4));
 	asm volatile("" : "+v"(v_offset));
 	// All work, in steps: 64 sequences at a time, one for each lane.  (Their number is below 2^31: checked on the host.)
+	int longest = 0; // most steps that a row group of the lane's sequences has
 	int steps, work, upto; // of the lane's sequence: steps of a row group, work of all, work up to its end from the lane 0's start on
 	auto add_up = [&](int group) {
-		steps = steps_of(z);
-		work  = row_groups_of(z, group) * (FIXED + steps);
-		upto  = scan64(work);
+		steps	= steps_of(z);
+		longest = max(longest, steps);
+		work	= row_groups_of(z, group) * (FIXED + steps);
+		upto	= scan64(work);
 		return __builtin_amdgcn_readlane(upto, 63);
 	};
 	int total = add_up(first_group);
@@ -287,10 +290,15 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		z = size_of(batch, all_rows, prefix_keys, held, base + first_lane);
 		total += add_up(first_group);
 	}
-	const int first_share = max((total + (1 << log2_units) - 1) >> log2_units, WAVES); // of a workgroup
+	// A workgroup's stretch: all work over all workgroups, or, where that is little, about the root of the longest row group's steps, as a piece more costs its
+	// join about what a turn of the waves does (one sequence, one kv head, 16384 keys: pieces of 4 steps 31 us, of 24 16; 1000 keys: of 4 8.4, of 8 9.6).
+	const auto longer_than = [&](int than) {
+		return __builtin_amdgcn_ballot_w64(longest > than) != 0;
+	};
+	const int little	  = longer_than(1024) ? 32 : longer_than(384) ? 20 : longer_than(64) ? 8 : WAVES;
+	const int first_share = max((total + (1 << log2_units) - 1) >> log2_units, little);
 	int at			= blockIdx.y * first_share;
 	const int end	= min(at + first_share, total);
-	const int least = min(first_share, LEAST);
 	if (at >= end) {
 		wait_stores_acknowledged(); // (nothing may still be on its way into LDS when the workgroup ends)
 		return;
@@ -343,7 +351,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		const int prefix_pieces_here  = w.prefix_pieces;
 		find(lane, group);
 		const int cache_pages = same(cache_pages_here), prefix_pieces = same(prefix_pieces_here);
-		const int row_group_end = p.begin + p.steps;
+		const int row_group_end = p.begin + p.steps, least = p.steps < WHOLE ? p.steps : min(share, LEAST); // (as many as it has: it is not cut)
 		int segment_begin = p.begin, segment_end = row_group_end;
 		if (at > p.begin) { // (only where the stretch begins)
 			if (at - p.begin >= least) {
@@ -689,7 +697,6 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		auto slot_of = [&](int i) {
 			return static_cast<int64_t>(2 * i + (i == first_unit ? 1 : 0)) * kv_heads + head;
 		};
-		const int64_t slot = slot_of(unit);
 		if (there) {
 			float2 ml[WAVES];
 #pragma unroll
@@ -703,24 +710,33 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 				f[x] = exp2_fast(ml[x].x - at);
 				sum += ml[x].y * f[x];
 			}
-			const float inv		  = sum > 0.0f || sum != sum ? __builtin_amdgcn_rcpf(sum) : 0.0f; // (within 2^-23; no key at all: zeros)
-			const int64_t out_row = static_cast<int64_t>((p.first_row + token) * q_heads + q_head) * D, slot_row = (slot * w.columns + col) * D; // (rows * q_heads <= 2^30)
+			v4f v[DT / WAVES];
 #pragma unroll
 			for (int j = 0; j < DT / WAVES; ++j) {
-				const int dt = wave + WAVES * j;
-				v4f v{};
+				v4f of_wave[WAVES];
 #pragma unroll
 				for (int x = 0; x < WAVES; ++x) {
-					v += join_o[x][dt][lane] * f[x];
+					of_wave[x] = join_o[x][wave + WAVES * j][lane];
 				}
-				if (alone) {
-					store_out4<TYPE>(a.out, out_row + 16 * dt + 4 * quarter, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-				} else {
-					put4(w.o + slot_row + 16 * dt + 4 * quarter, v);
-				}
+				v[j] = of_wave[0] * f[0] + of_wave[1] * f[1] + (of_wave[2] * f[2] + of_wave[3] * f[3]);
 			}
-			if (!alone && wave == 0 && quarter == 0) {
-				put2(w.ml + slot * w.columns + col, make_float2(top, sum));
+			static_assert(WAVES == 4);
+			if (alone) {
+				const float inv = sum > 0.0f || sum != sum ? __builtin_amdgcn_rcpf(sum) : 0.0f; // (within 2^-23; no key at all: zeros)
+				const int64_t out_at = static_cast<int64_t>((p.first_row + token) * q_heads + q_head) * D + 16 * wave + 4 * quarter; // (rows * q_heads <= 2^30)
+#pragma unroll
+				for (int j = 0; j < DT / WAVES; ++j) {
+					store_out4<TYPE>(a.out, out_at + 16 * WAVES * j, v[j][0] * inv, v[j][1] * inv, v[j][2] * inv, v[j][3] * inv);
+				}
+			} else {
+				const int64_t slot_row = slot_of(unit) * w.columns + col;
+#pragma unroll
+				for (int j = 0; j < DT / WAVES; ++j) {
+					put4(w.o + slot_row * D + 16 * (wave + WAVES * j) + 4 * quarter, v[j]);
+				}
+				if (wave == 0 && quarter == 0) {
+					put2(w.ml + slot_row, make_float2(top, sum));
+				}
 			}
 		}
 		bool join = false;
