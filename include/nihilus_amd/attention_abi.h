@@ -69,13 +69,14 @@ typedef struct nh_attn_batch {
  * (a, b) being values (2i, 2i + 1) of a head if interleaved != 0, else (i, i + pairs); values from 2 pairs on are passed through.
  * turns is fp64: the angle of a far position is reduced to a part of a turn in 64 bits, its sine and cosine and the rotation are
  * fp32, and the result is rounded once.  q_stride, k_stride, v_stride: elements from one row to the next (heads of a row are side by side),
- * multiples of 16 bytes, so that parts of one fused projection can be given; q_out is [rows][q_heads][head_dim] without gaps, and may
- * be q itself if q has none.  `type` is that of q, k, v and q_out: NH_F32 or the cache's. */
+ * multiples of 16 bytes, so that parts of one fused projection can be given; q_out is [rows][q_heads][head_dim] without gaps, may be
+ * q itself if q has none, and otherwise has no byte in common with q, k or v (NH_ERR_ARGUMENT).  `type` is that of q, k, v and q_out: NH_F32 or the cache's. */
 int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, const void* k, const void* v, void* q_out, int type, int64_t rows, int64_t q_heads,
 	int64_t q_stride, int64_t k_stride, int64_t v_stride, const double* turns, int64_t pairs, int interleaved, void* stream);
 
 /* out[r] = sum_j softmax_j(scale q[r] . k_j) v_j over the keys j <= position of row r, for every row of every sequence; query head h
- * reads kv head h / (q_heads / kv_heads).  q_heads is a multiple of kv_heads.  starts must not be NULL.
+ * reads kv head h / (q_heads / kv_heads).  q_heads is a multiple of kv_heads.  starts must not be NULL.  out has no gaps and no byte in
+ * common with q (NH_ERR_ARGUMENT).
  * type NH_F32: q and the softmax weights go through the 16-bit matrix instructions as sums of two (fp16 cache) or three (bf16) terms,
  * 22 or 24 bits; type = the cache's: q as it is, the weights rounded once.  Everything else (products' sums, maxima, sums) is fp32.
  * Memory: nh_attn_prompt_needs says how many bytes (0: many rows need none, and the pointers may be NULL), 256-byte aligned. */

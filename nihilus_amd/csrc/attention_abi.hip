@@ -62,6 +62,10 @@ inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_byt
 	const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
 	return a && b && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
 }
+// bytes that rows of a stride reach over
+inline int64_t span(int64_t rows, int64_t heads, int64_t head_dim, int64_t stride, int type) {
+	return ((rows - 1) * stride + heads * head_dim) * value_bytes(type);
+}
 inline nh::cache_view view(const nh_attn_cache* c) {
 	return nh::cache_view{ static_cast<uint16_t*>(c->k_pages), static_cast<uint16_t*>(c->v_pages), c->kv_heads * c->page_size * c->head_dim, static_cast<int>(c->pages),
 		static_cast<int>(c->kv_heads), page_shift(c->page_size) };
@@ -111,7 +115,9 @@ int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* ho
 	}
 	NH_REQUIRE(q && k && v && q_out && (turns || pairs == 0), NH_ERR_NULL_POINTER);
 	NH_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out), NH_ERR_ALIGNMENT);
-	NH_REQUIRE(q_out != q || q_stride == q_heads * host_cache->head_dim, NH_ERR_ARGUMENT);
+	const int64_t dim = host_cache->head_dim, kv_heads = host_cache->kv_heads, out_bytes = span(rows, q_heads, dim, q_heads * dim, type);
+	NH_REQUIRE(q_out == q ? q_stride == q_heads * dim : !overlap(q_out, out_bytes, q, span(rows, q_heads, dim, q_stride, type)), NH_ERR_ARGUMENT);
+	NH_REQUIRE(!overlap(q_out, out_bytes, k, span(rows, kv_heads, dim, k_stride, type)) && !overlap(q_out, out_bytes, v, span(rows, kv_heads, dim, v_stride, type)), NH_ERR_ARGUMENT);
 	NH_TRY(require_device());
 	nh::append_args a{};
 	a.cache = view(host_cache), a.batch = view(host_batch);
@@ -137,6 +143,10 @@ static nh::attention_args attention(const nh_attn_cache* c, const nh_attn_batch*
 	a.rows = static_cast<int>(rows), a.q_heads = static_cast<int>(q_heads), a.head_dim = static_cast<int>(c->head_dim);
 	a.scale = scale;
 	return a;
+}
+
+static bool out_over_q(const nh_attn_cache* c, const void* q, const void* out, int type, int64_t rows, int64_t q_heads, int64_t q_stride) {
+	return overlap(out, span(rows, q_heads, c->head_dim, q_heads * c->head_dim, type), q, span(rows, q_heads, c->head_dim, q_stride, type));
 }
 
 static int check_memory(int64_t workspace_need, int64_t counter_need, const void* workspace, int64_t workspace_bytes, const void* counters, int64_t counter_bytes) {
@@ -173,6 +183,7 @@ int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 	}
 	NH_REQUIRE(host_batch->starts && q && out, NH_ERR_NULL_POINTER);
 	NH_REQUIRE(aligned16(q) && aligned16(out), NH_ERR_ALIGNMENT);
+	NH_REQUIRE(!out_over_q(host_cache, q, out, type, rows, q_heads, q_stride), NH_ERR_ARGUMENT);
 	NH_TRY(check_memory(need, counter_need, workspace, workspace_bytes, counters, counter_bytes));
 	NH_TRY(require_device());
 	nh::attention_args a = attention(host_cache, host_batch, q, out, rows, q_heads, q_stride, scale);
@@ -219,6 +230,7 @@ int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 	}
 	NH_REQUIRE(q && out && (prefix_pages || prefix_count == 0), NH_ERR_NULL_POINTER);
 	NH_REQUIRE(aligned16(q) && aligned16(out), NH_ERR_ALIGNMENT);
+	NH_REQUIRE(!out_over_q(host_cache, q, out, type, host_batch->sequences, q_heads, q_stride), NH_ERR_ARGUMENT);
 	NH_TRY(check_memory(need, counter_need, workspace, workspace_bytes, counters, counter_bytes));
 	NH_TRY(require_device());
 	nh::attention_args a = attention(host_cache, host_batch, q, out, host_batch->sequences, q_heads, q_stride, scale);

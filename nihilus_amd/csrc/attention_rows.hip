@@ -35,8 +35,8 @@ constexpr int THREADS	 = 64 * WAVES;
 constexpr int STEP		 = 32; // keys of a wave's step
 constexpr int COLUMNS	 = 16; // rows of a row group
 constexpr int WORKGROUPS = 512; // that the chip holds at once: two per CU
-// What a row group takes beside its steps (its q, its first step's way, the joins), in steps.  (64 sequences of up to 8192 tokens, and those of up to 600 behind a
-// shared prefix of 8192: 8 steps 54.6 and 53.2 us, 12: 55.4 and 50.4, 20: 57.2 and 53.7.)
+// What a row group takes beside its steps (its q, its first step's way, the joins), in steps.  (Times with the launch of a graph: 64 sequences of up
+// to 8192 tokens, those of up to 600 behind a shared prefix of 8192, and 64 of 1024: 6 steps 55.7, 48.3 and 42.9 us, 8: 54.0, 52.1 and 42.7, 12: 54.8, 50.2 and 44.2.)
 constexpr int FIXED = 8;
 // A row group of fewer steps than WHOLE is not cut (one sequence of 256 tokens: 4.7 us, in two pieces 6.1; of 512 in four 6.3, whole 6.5), others not where a piece
 // would have fewer than LEAST, or than a whole stretch (64 sequences of up to 8192 tokens: 8 steps 57.1 us, 24: 58.6).
@@ -165,23 +165,14 @@ template<int D> __device__ __forceinline__ int k_swizzle(int r) {
 	return D == 128 ? (r & 3) | ((r >> 1) & 12) : ((r >> 1) & 1) | ((r >> 2) & 6);
 }
 
-// 64 lanes' 16 bytes each, two or four times over, 1024 bytes further on in memory and in LDS every time (the instruction's offset counts for both), from `offset`
-// bytes behind an address that the wave has.  As load_global_to_lds_b128.
+// 64 lanes' 16 bytes each, twice, the second time 1024 bytes further on in memory and in LDS (the instruction's offset counts for both), from offsets behind
+// an address that the wave has.  As load_global_to_lds_b128.
 __device__ __forceinline__ void load_2_to_lds(const void* src, uint32_t o0, uint32_t o1, const void* lds_dst) {
 	const uint32_t lds_addr = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(static_cast<const char*>(lds_dst))));
 	uint32_t saved_m0;
 	asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %2, %3 offset:1024\n\ts_mov_b32 m0, %0"
 				 : "=&s"(saved_m0)
 				 : "v"(o0), "v"(o1), "s"(src), "s"(lds_addr)
-				 : "memory");
-}
-__device__ __forceinline__ void load_4_to_lds(const void* src, uint32_t o01, uint32_t o23, const void* lds_dst) {
-	const uint32_t lds_addr = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char*)(static_cast<const char*>(lds_dst))));
-	uint32_t saved_m0;
-	asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\tglobal_load_lds_dwordx4 %1, %3 offset:1024\n\t"
-				 "global_load_lds_dwordx4 %2, %3 offset:2048\n\tglobal_load_lds_dwordx4 %2, %3 offset:3072\n\ts_mov_b32 m0, %0"
-				 : "=&s"(saved_m0)
-				 : "v"(o01), "v"(o23), "s"(src), "s"(lds_addr)
 				 : "memory");
 }
 
@@ -435,8 +426,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			 const uint16_t* const k_hi = k_pages + hi_at + ((base + 16) & (page_size - 1)) * D;
 			 v4u* const slot			= &slots[wave][0];
 			 if constexpr (D == 128) {
-				 load_4_to_lds(k_lo, k_offset[0], k_offset[1], slot);
-				 load_4_to_lds(k_hi, k_offset[2], k_offset[3], slot + 4 * 64);
+				 load_2_to_lds(k_lo, k_offset[0], k_offset[0], slot);
+				 load_2_to_lds(k_lo + 8 * D, k_offset[1], k_offset[1], slot + 2 * 64);
+				 load_2_to_lds(k_hi, k_offset[2], k_offset[2], slot + 4 * 64);
+				 load_2_to_lds(k_hi + 8 * D, k_offset[3], k_offset[3], slot + 6 * 64);
 			 } else {
 				 load_2_to_lds(k_lo, k_offset[0], k_offset[1], slot);
 				 load_2_to_lds(k_hi, k_offset[2], k_offset[3], slot + 2 * 64);

@@ -42,7 +42,7 @@ def test_the_header_is_plain_c():
     assert res.returncode == 0, res.stderr
 
 
-def _append(cache=None, batch=None, q=BOGUS, k=BOGUS, v=BOGUS, out=BOGUS, type=0, rows=3, heads=4, strides=(256, 128, 128), turns=BOGUS, pairs=32):
+def _append(cache=None, batch=None, q=BOGUS, k=BOGUS, v=BOGUS, out=BOGUS * 2, type=0, rows=3, heads=4, strides=(256, 128, 128), turns=BOGUS, pairs=32):
     from nihilus_amd import _lib
 
     return _lib.lib().nh_attn_append_rope(C.byref(cache or _cache()), C.byref(batch or _batch()), q, k, v, out, type, rows, heads, *strides, turns, pairs, 1, None)
@@ -51,13 +51,13 @@ def _append(cache=None, batch=None, q=BOGUS, k=BOGUS, v=BOGUS, out=BOGUS, type=0
 MEMORY = dict(ws=BOGUS, bytes=1 << 30, counters=BOGUS, counter_bytes=1 << 30)
 
 
-def _prompt(cache=None, batch=None, q=BOGUS, out=BOGUS, type=0, rows=3, heads=4, stride=256, scale=0.125, **memory):
+def _prompt(cache=None, batch=None, q=BOGUS, out=BOGUS * 2, type=0, rows=3, heads=4, stride=256, scale=0.125, **memory):
     from nihilus_amd import _lib
 
     return _lib.lib().nh_attn_prompt(C.byref(cache or _cache()), C.byref(batch or _batch(starts=BOGUS)), q, out, type, rows, heads, stride, scale, *{**MEMORY, **memory}.values(), None)
 
 
-def _decode(cache=None, batch=None, prefix=None, count=0, q=BOGUS, out=BOGUS, type=0, heads=4, stride=256, scale=0.125, **memory):
+def _decode(cache=None, batch=None, prefix=None, count=0, q=BOGUS, out=BOGUS * 2, type=0, heads=4, stride=256, scale=0.125, **memory):
     from nihilus_amd import _lib
 
     return _lib.lib().nh_attn_decode(C.byref(cache or _cache()), C.byref(batch or _batch()), prefix, count, q, out, type, heads, stride, scale, *{**MEMORY, **memory}.values(), None)
@@ -157,6 +157,20 @@ def test_workspace_sizes():
     assert lib.nh_attn_prompt_needs(20, 2, 32, 8, 128, None, C.byref(c)) == -1 and lib.nh_attn_decode_needs(4, 32, 8, 128, 0, 64, C.byref(n), None) == -1
     g = lib.nh_attn_pages_workspace_bytes
     assert g(1, 0, 0) == 0 and g(1000, 64, 10) == 0 and g(100000, 64, 10) >= 100000 * 8 and g(5000, 20000, 1) >= 20000 * 8 and g(0, 1, 1) == -3 and g(1, -1, 1) == -3 and g(1 << 40, 1, 1) == -5
+
+
+def test_results_over_inputs_are_refused():
+    size = 3 * 6 * 64 * 4  # rows, heads, values of fp32
+    for call in (_prompt, _decode):
+        for out in (BOGUS, BOGUS + size - 16, BOGUS - size + 16):
+            assert call(out=out, heads=6, stride=384) == -6, (call, out)
+        for out in (BOGUS + size, BOGUS - size):
+            assert call(out=out, heads=6, stride=384) != -6, (call, out)
+    far = {"k": BOGUS * 4, "v": BOGUS * 6, "heads": 6}
+    assert _append(out=BOGUS, strides=(384, 128, 128), **far) != -6  # in place
+    assert _append(out=BOGUS, strides=(512, 128, 128), **far) == -6 and _append(out=BOGUS + 16, strides=(384, 128, 128), **far) == -6
+    assert _append(out=BOGUS * 4, strides=(384, 128, 128), **far) == -6 and _append(out=BOGUS * 6 - size + 16, strides=(384, 128, 128), **far) == -6
+    assert _append(out=BOGUS * 6 - size, strides=(384, 128, 128), **far) != -6
 
 
 def test_which_kernel_a_prompt_takes(monkeypatch):
