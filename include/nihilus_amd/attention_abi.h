@@ -86,13 +86,13 @@ int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 
 /* Which kernel nh_attn_prompt runs for these sizes: 1 the one for few rows (16 at a time, the keys of long sequences over several workgroups), 2 the
  * one for many (128 at a time).  Needs no GPU.  force: 0 lets the sizes decide from now on, 1 or 2 takes
- * that kernel always, -1 changes nothing; a test hook, process-wide, which anything but -1 is refused for (NH_ERR_ARGUMENT) unless
+ * that kernel always (and goes over a decode step's shared prefix with each sequence's own keys, or apart), -1 changes nothing; a test hook, process-wide, which anything but -1 is refused for (NH_ERR_ARGUMENT) unless
  * the process has NH_Q8_0_DEBUG_HOOKS=1 in its environment. */
 int nh_attn_debug_prompt_kernel(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int force);
 
 /* The same for one row per sequence over all of its keys (starts must be NULL, rows = sequences).  The keys j < prefix_count *
  * page_size of EVERY sequence (as far as its length goes) are those of the pages prefix_pages[0 .. prefix_count): they are read once for the
- * whole batch, and the first prefix_count entries of a page_table row are not looked at.  prefix_count = 0: none shared. */
+ * whole batch (where that is faster), and the first prefix_count entries of a page_table row are not looked at.  prefix_count = 0: none shared. */
 int nh_attn_decode_needs(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_count, int64_t page_size, int64_t* host_workspace_bytes,
 	int64_t* host_counter_bytes);
 int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* prefix_pages, int64_t prefix_count, const void* q, void* out, int type, int64_t q_heads,

@@ -78,6 +78,17 @@ std::atomic<int> forced_prompt_kernel{ 0 };
 
 } // namespace
 
+// Whether a decode step's shared prefix is gone over once for all sequences, by the tile kernel, or by each with its own keys.  The first takes a launch more
+// and the join of its results, some 7 us and more with more sequences; the second reads the prefix from the caches once for each sequence.
+// us, apart | with their own (fp16, own keys 200; 32 / 8 heads of 128): prefix 1024: 8 sequences 16.0 | 11.8, 64 28.1 | 23.9;  4096: 8 19.6 | 15.8, 16 24.2 | 25.1,
+// 64 34.6 | 58.8;  8192: 4 23.0 | 16.6, 8 24.5 | 23.7, 16 27.1 | 39.2;  16 / 2 heads, 8192: 32 34.0 | 25.8, 64 30.5 | 39.2
+static bool prefix_apart(int64_t sequences, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
+	if (const int forced = forced_prompt_kernel.load(std::memory_order_relaxed)) {
+		return forced == 2;
+	}
+	return static_cast<double>(sequences) * static_cast<double>(kv_heads * head_dim) * static_cast<double>(prefix_keys) > 67108864.0;
+}
+
 bool nh::prompt_by_rows(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads) {
 	if (const int forced = forced_prompt_kernel.load(std::memory_order_relaxed)) {
 		return forced == 1;
@@ -236,6 +247,7 @@ int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 	nh::attention_args a = attention(host_cache, host_batch, q, out, host_batch->sequences, q_heads, q_stride, scale);
 	a.prefix_pages		 = prefix_pages;
 	a.prefix_count		 = static_cast<int>(prefix_count);
+	a.prefix_apart		 = prefix_count > host_batch->table_width || prefix_apart(host_batch->sequences, host_cache->kv_heads, host_cache->head_dim, prefix_count * host_cache->page_size);
 	a.workspace			 = workspace;
 	a.counters			 = static_cast<int32_t*>(counters);
 	return from_hip(nh::launch_attention_rows(a, host_cache->type, type, as_stream(stream)));

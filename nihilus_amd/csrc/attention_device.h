@@ -201,6 +201,7 @@ struct attention_args {
 	float scale;
 	const int32_t* prefix_pages; // decode only
 	int prefix_count;
+	bool prefix_apart; // for all sequences at once, by the tile kernel; else each reads it with its own keys
 	void* workspace;
 	int32_t* counters;
 };

@@ -339,9 +339,10 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		const int64_t q_stride		  = a.q_stride;
 		const int cache_pages_here	  = a.cache.pages;
 		const float scale			  = a.scale;
-		const int prefix_pieces_here  = w.prefix_pieces;
+		const int prefix_pieces_here  = w.prefix_pieces, in_front_here = a.prefix_count; // pages that all sequences begin with, read like their own
+		const int32_t* const pages_in_front = a.prefix_pages;
 		find(lane, group);
-		const int cache_pages = same(cache_pages_here), prefix_pieces = same(prefix_pieces_here);
+		const int cache_pages = same(cache_pages_here), prefix_pieces = same(prefix_pieces_here), in_front = same(in_front_here);
 		const int row_group_end = p.begin + p.steps, least = p.steps < WHOLE ? p.steps : min(share, LEAST); // (as many as it has: it is not cut)
 		int segment_begin = p.begin, segment_end = row_group_end;
 		if (at > p.begin) { // (only where the stretch begins)
@@ -373,11 +374,12 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 		// The pages of its first keys (in registers already if they are the first sequence's first), asked for ahead of everything else: the keys wait for them.
 		const int32_t* table = page_table + static_cast<int64_t>(p.seq) * width;
 		const int first_key	 = prefix_keys + (segment_begin - p.begin) * STEP;
-		if (p.seq == 0 && prefix_keys + (segment_end - p.begin) * STEP <= 64 << page_shift) {
+		if (p.seq == 0 && in_front == 0 && prefix_keys + (segment_end - p.begin) * STEP <= 64 << page_shift) {
 			ids = front, first_id = 0;
 		} else {
 			first_id = first_key >> page_shift;
-			ids		 = table[min(first_id + lane, max(width, 1) - 1)];
+			const int slot = min(first_id + lane, max(width, 1) - 1);
+			ids			   = (slot < in_front ? pages_in_front : table)[slot];
 		}
 		__builtin_amdgcn_sched_barrier(0);
 		// the row group's rows: first .. first + count - 1 of the sequence's rows * group
@@ -412,7 +414,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			if (key >= end_key) {
 				return -1;
 			}
-			const int slot = key >> page_shift, id = slot - first_id < 64 ? __builtin_amdgcn_readlane(ids, slot - first_id) : table[slot];
+			const int slot = key >> page_shift, id = slot - first_id < 64 ? __builtin_amdgcn_readlane(ids, slot - first_id) : (slot < in_front ? pages_in_front : table)[slot];
 			return id >= 0 && id < cache_pages ? id : -1;
 		};
 		// A step's 32 keys into the wave's slot of LDS: keys, then values, 64 pieces an instruction, the pieces of a row side by side in memory so that the lanes
@@ -817,7 +819,7 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 	const bool one_each		= a.batch.starts == nullptr;
 	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : a.rows * group / COLUMNS + sequences;
 	const rows_cut cut		= plan_rows(one_each, group, a.cache.kv_heads, row_groups);
-	const prefix_cut prefix = plan_prefix(sequences, group, a.cache.kv_heads, static_cast<int64_t>(a.prefix_count) << a.cache.page_shift);
+	const prefix_cut prefix = a.prefix_apart ? plan_prefix(sequences, group, a.cache.kv_heads, static_cast<int64_t>(a.prefix_count) << a.cache.page_shift) : prefix_cut{};
 	rows_workspace w;
 	(void)lay_out(static_cast<char*>(a.workspace), cut, prefix, sequences, a.q_heads, a.cache.kv_heads, D, &w);
 	w.counters = a.counters;
@@ -829,6 +831,8 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 	}
 	// (no more workgroups than the tables have keys for, four steps each at least)
 	const int64_t steps		 = (static_cast<int64_t>(a.batch.width) << a.cache.page_shift) / STEP + 1 + FIXED;
+	attention_args late = a;
+	late.prefix_count	= one_each && !a.prefix_apart ? a.prefix_count : 0;
 	int log2_units			 = 0;
 	while ((2 << log2_units) <= cut.units && (WAVES << log2_units) < row_groups * steps) {
 		++log2_units;
@@ -836,7 +840,7 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), 1u << log2_units), dim3(THREADS), 0, s>>>(a.batch.lengths,
 		a.batch.width > 0 ? a.batch.table : a.batch.lengths, a.q, a.cache.k, a.batch.starts,
 		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | static_cast<uint32_t>(log2_units) << 25 | (one_each ? 1u << 31 : 0u), a.batch.width,
-		one_each ? a.prefix_count : a.rows, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, rows_args{ a, w });
+		one_each ? (a.prefix_apart ? a.prefix_count : 0) : a.rows, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, rows_args{ late, w });
 	return hipGetLastError();
 }
 template<int CACHE, int TYPE> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {

@@ -26,7 +26,7 @@ def A():
 
 @pytest.fixture(params=[1, 2], ids=["rows", "tiles"])
 def kernel(A, request, monkeypatch):
-    """Each of the two kernels that a prompt may take, whatever its size."""
+    """Each of the two kernels that a prompt may take, and each of the two ways over a decode step's shared prefix, whatever the sizes."""
     monkeypatch.setenv("NH_Q8_0_DEBUG_HOOKS", "1")
     force = A._lib.lib().nh_attn_debug_prompt_kernel
     assert force(1, 1, 1, 1, request.param) == request.param
@@ -256,7 +256,7 @@ def test_decode_of_a_long_sequence(A):
 
 @pytest.mark.parametrize("dtype,cache", KINDS)
 @pytest.mark.parametrize("dim,page,pages", [(64, 16, 1), (64, 16, 9), (128, 64, 3), (128, 256, 1)])
-def test_decode_behind_a_shared_prefix(A, dtype, cache, dim, page, pages):
+def test_decode_behind_a_shared_prefix(A, kernel, dtype, cache, dim, page, pages):
     prefix = page * pages
     own = [1, 0, 40, 100, 5, 33, 300, -3, -prefix, 64]  # negative: a sequence that ends inside the prefix, or has nothing
     b = Batch(23, [prefix + n for n in own], page, 2, dim, cache, shared=pages)
@@ -271,7 +271,7 @@ def test_decode_behind_a_shared_prefix(A, dtype, cache, dim, page, pages):
         _check(plain[s], *ref, dtype, ("not shared", s))
 
 
-def test_prefix_of_many_rows_in_pieces(A):
+def test_prefix_of_many_rows_in_pieces(A, kernel):
     page, pages, n = 32, 40, 70  # 560 rows: five tiles; 1280 keys: several pieces
     own = [i % 37 for i in range(n)]
     b = Batch(29, [page * pages + x for x in own], page, 1, 64, F16, shared=pages)
@@ -680,7 +680,7 @@ def test_odd_values_of_later_rows(A, kernel, dtype, cache, dim, page):
 
 @pytest.mark.parametrize("dtype,cache", KINDS)
 @pytest.mark.parametrize("dim", [64, 128])
-def test_odd_values_in_a_prefix_that_some_rows_see_in_part(A, dtype, cache, dim):
+def test_odd_values_in_a_prefix_that_some_rows_see_in_part(A, kernel, dtype, cache, dim):
     page, pages = 16, 9
     lengths = [300, 144, 150, 17, 40, 100, 0, -(2**31), 129, 128]
     b = Batch(23, lengths, page, 2, dim, cache, shared=pages)
@@ -705,7 +705,7 @@ def test_a_stretch_of_many_small_pages(A):
         _check(out[seq], *ref, F16, seq)
 
 
-def test_decode_behind_a_prefix_replayed(A):
+def test_decode_behind_a_prefix_replayed(A, kernel):
     lengths = [700, 64, 65, 130, 256]
     b = Batch(31, lengths, 64, 2, 128, F16, shared=1)
     q = b.rows(5, 8, F32)
