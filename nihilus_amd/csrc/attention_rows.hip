@@ -19,9 +19,9 @@
 // turn and join their results in LDS.  Where a row group has been cut, each workgroup puts its result into the workspace and counts itself; the last to
 // do so joins them, in the pieces' order, so the result does not hang on who that is.
 //
-// Measured (fp16, 32 query heads over 8 kv heads of 128): 64 sequences of up to 8192 tokens, 238 MB, 53 us; 64 of 4096, 1074 MB, 181 us: 5.9 TB/s, against 6.35 TB/s
-// that a kernel which only reads reaches.  Small calls are bound by a chain of trips to memory and by instructions that are fetched for the first time (a
-// step's arithmetic takes 0.8 us then, one of many 0.3): one sequence of 1000 tokens 8.9 us, of 64 tokens 4.3, a prompt of 117 rows 7.1.
+// Measured (fp16, 32 query heads over 8 kv heads of 128): 64 sequences of up to 8192 tokens, 238 MB, 52 us; 64 of 4096, 1074 MB, 181 us: 5.9 TB/s, against 6.35 TB/s
+// that a kernel which only reads reaches.  Small calls are bound by a chain of trips to memory (arguments, lengths, pages, keys) with some hundred instructions of a
+// lone wave between them: one sequence of 1000 tokens (fp32 q) 8.3 us, of 64 tokens 3.7, a prompt of 117 rows 5.9.
 #include "attention_device.h"
 
 #include <algorithm>
@@ -58,7 +58,7 @@ struct rows_cut {
 	int64_t units; // workgroups per kv head: a power of two
 	int64_t columns; // rows of a row group that are kept in the workspace
 };
-// One workgroup per CU where that is one for each row group (a prompt of 117 rows: 7.1 us, with two per CU, of which every second one has nothing to do, 8.1),
+// One workgroup per CU where that is one for each row group (a prompt of 117 rows: 1.2 us less than with two per CU, of which every second one has nothing to do),
 // else two (128 sequences of 256 tokens: 25 us, with one 30).
 rows_cut plan_rows(bool one_each, int64_t group, int64_t kv_heads, int64_t row_groups) {
 	rows_cut c{};
