@@ -47,6 +47,8 @@ def rope_turns(head_dim: int, base: float = 500000.0, factors=None, rotary: int 
 def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dims: int):
     if not (k_pages.is_cuda and k_pages.is_contiguous() and v_pages.is_contiguous()) or k_pages.dtype not in (torch.float16, torch.bfloat16) or v_pages.dtype != k_pages.dtype:
         raise TypeError("k_pages and v_pages must be contiguous float16 or bfloat16 tensors on the GPU")
+    if v_pages.device != k_pages.device:
+        raise TypeError("k_pages and v_pages must be on the same GPU")
     if k_pages.dim() != dims or v_pages.shape != (*k_pages.shape[:-2], k_pages.shape[-1], k_pages.shape[-2]):
         raise ValueError(f"k_pages must be [{'layers, ' if dims == 5 else ''}pages, kv_heads, page_size, head_dim], v_pages the same with its last two the other way round")
     layers, (pages, kv_heads, page_size, head_dim) = (k_pages.shape[0] if dims == 5 else 1), k_pages.shape[-4:]

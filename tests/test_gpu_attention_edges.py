@@ -1,0 +1,23 @@
+"""GPU: attention and the paged cache where a call stands on the edge of what it takes, beside test_gpu_attention.py and test_gpu_cache_pages.py: tensors of
+another device, batches of nobody, peaked scores across the pieces of a row's keys, streams of other owners, the forms that only large calls take."""
+import pytest
+import torch
+
+from test_gpu_attention import A, BF16, F16, F32, INF, KINDS, NAN, Batch, _check, _check_prompt, _check_with_odd_values, _starts, kernel  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_value_pages_on_the_host_are_refused(A, monkeypatch, native):  # noqa: F811
+    if not native:
+        monkeypatch.setattr(A, "_calls", None)
+    b = Batch(3, [20, 5], 16, 2, 64, F16)
+    k, v, table, dl = b.device()
+    q, kv = b.rows(2, 4, F32).cuda(), b.rows(2, 2, F32).cuda()
+    ints, starts = torch.zeros(2, dtype=torch.int32).cuda(), torch.tensor([0, 1, 2], dtype=torch.int32).cuda()
+    host = v.cpu()
+    for call in (lambda: A.append_rope(q, kv, kv, k, host, table, dl, A.rope_turns(64)), lambda: A.attention_prompt(q, k, host, table, dl, starts), lambda: A.attention_decode(q, k, host, table, dl),
+                 lambda: A.cache_step(k[None], host[None], table, dl, ints, ints), lambda: A.cache_compact(k[None], host[None], table, dl)):
+        with pytest.raises(TypeError):
+            call()
