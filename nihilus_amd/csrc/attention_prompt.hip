@@ -661,7 +661,7 @@ hipError_t launch_attention_tiles(const attention_args& a, int cache_type, int t
 
 prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64_t prefix_keys) {
 	prefix_cut c{};
-	if (prefix_keys == 0) {
+	if (prefix_keys == 0 || sequences == 0) { // (nobody to share it)
 		return c;
 	}
 	c.row_tiles			 = (sequences * group + ROWS - 1) / ROWS;

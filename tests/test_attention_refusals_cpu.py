@@ -30,3 +30,15 @@ def test_value_pages_of_another_device_are_refused(where, dims):
     assert (cache.pages, cache.kv_heads, cache.page_size, cache.head_dim) == (4, 2, 16, 64)
     with pytest.raises(TypeError):
         A._pages(_On(k, "cuda:0"), _On(v, where), dims)
+
+
+@pytest.mark.parametrize("page_size,count", [(16, 1), (64, 4), (256, 1 << 22)])
+def test_a_prefix_that_no_sequence_shares(page_size, count):
+    from nihilus_amd import _lib
+
+    n, c = C.c_int64(), C.c_int64()
+    assert _lib.lib().nh_attn_decode_needs(0, 4, 2, 64, 0, page_size, C.byref(n), C.byref(c)) == 0
+    without = n.value, c.value
+    assert _lib.lib().nh_attn_decode_needs(0, 4, 2, 64, count, page_size, C.byref(n), C.byref(c)) == 0
+    assert (n.value, c.value) == without
+    assert _decode(cache=_cache(page_size=page_size), batch=_batch(sequences=0), prefix=BOGUS, count=count, q=None, out=None, ws=None, counters=None) == 0

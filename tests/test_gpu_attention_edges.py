@@ -21,3 +21,22 @@ def test_value_pages_on_the_host_are_refused(A, monkeypatch, native):  # noqa: F
                  lambda: A.cache_step(k[None], host[None], table, dl, ints, ints), lambda: A.cache_compact(k[None], host[None], table, dl)):
         with pytest.raises(TypeError):
             call()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_calls_for_nobody(A, monkeypatch, native):  # noqa: F811
+    if not native:
+        monkeypatch.setattr(A, "_calls", None)
+    b = Batch(5, [70], 16, 2, 64, F16, shared=4)
+    k, v, table, dl = b.device()
+    prefix = torch.tensor(b.common, dtype=torch.int32).cuda()
+    q, kv, none = torch.empty(0, 8, 64, device="cuda"), torch.empty(0, 2, 64, device="cuda"), dl[:0]
+    assert A.attention_decode(q, k, v, table[:0], none, prefix_pages=prefix).shape == (0, 8, 64)
+    assert A.attention_decode(q, k, v, table[:0], none, prefix_pages=prefix, workspace=A.decode_workspace(0, 8, 2, 64, prefix_pages=4, page_size=16)).shape == (0, 8, 64)
+    assert A.attention_decode(q, k, v, table[:0], none).shape == (0, 8, 64)
+    assert A.attention_prompt(q, k, v, table[:0], none, torch.zeros(1, dtype=torch.int32).cuda()).shape == (0, 8, 64)
+    assert A.append_rope(q, kv, kv, k, v, table[:0], none, A.rope_turns(64)).shape == (0, 8, 64)
+    new, lengths, info = A.cache_step(k[None], v[None], table, dl, none, none)  # everybody has ended
+    assert new.shape == (0, table.shape[1]) and lengths.shape == (0,) and info.tolist() == [0, 0, 0]
+    new, info = A.cache_compact(k[None], v[None], table[:0], none)
+    assert new.shape == (0, table.shape[1]) and info.tolist() == [0, 0, 0]
