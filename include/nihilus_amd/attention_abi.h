@@ -105,7 +105,8 @@ int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
  *     the lowest of them keeps it (unless some child holds it as a full page) and the others get copies.
  *   - Pages that a child needs beyond its parent's are given to it; tokens in them are not written.
  *   Free pages are given in ascending order, to the children in theirs, to each its copy first; copies move keys and values of all layers.
- * new_table int32 [children][table_width] (entries past a child's last page are -1), new_lengths int32 [children], none of them an input.
+ * new_table int32 [children][table_width] (entries past a child's last page are -1), new_lengths int32 [children]; these, info and the workspace have no byte in
+ * common with each other, the inputs or the cache (NH_ERR_ARGUMENT).
  * info int32 [3]: pages held afterwards, pages copied, pages that could not be given (too few free) or that the old table did not
  * have; their entries are -1, which the calls above leave out.  Nothing of the inputs changes, so a caller that finds pages missing can end
  * sequences and call again.  starts is not used.  workspace: nh_attn_pages_workspace_bytes(pages, children, table_width) bytes, 0 (and it may
@@ -117,7 +118,7 @@ int nh_attn_cache_step(const nh_attn_cache* host_cache, const nh_attn_batch* hos
 /* Moves the pages that hold the sequences' tokens to the front: with n pages in use, the k-th lowest used page >= n goes to the k-th lowest free
  * page < n, in all layers.  new_table int32 [sequences][table_width] names the pages where they are then (entries past a sequence's
  * last page, and those outside the cache, are -1); info int32 [3]: n, pages moved, entries that were outside the cache.  Pages that
- * were free keep what they held unless something moved there.  Workspace as above. */
+ * were free keep what they held unless something moved there.  Workspace, and what may not lie over what, as above. */
 int nh_attn_cache_compact(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, int32_t* new_table, int32_t* info, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -4,9 +4,11 @@
 #include "abi_checks.h"
 #include "attention_device.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdlib>
+#include <iterator>
 
 namespace {
 
@@ -273,8 +275,33 @@ static int check_pages(const nh_attn_cache* c, const nh_attn_batch* b, int64_t c
 	NH_REQUIRE(info && (workspace || need == 0) && (new_table || children * b->table_width == 0), NH_ERR_NULL_POINTER);
 	NH_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, NH_ERR_ALIGNMENT);
 	NH_REQUIRE(workspace_bytes >= need, NH_ERR_ARGUMENT);
-	// the new table is written while the old one is read
-	NH_REQUIRE(!overlap(new_table, children * b->table_width * 4, b->page_table, b->sequences * b->table_width * 4), NH_ERR_ARGUMENT);
+	return NH_OK;
+}
+// Nothing that a call on the pages writes may lie over what it reads (every workgroup plans from the inputs while the first one writes the results), nor over
+// another result, nor the workspace over either.
+static int check_page_results(const nh_attn_cache* c, const nh_attn_batch* b, int64_t children, const int32_t* parents, const int32_t* grow, const int32_t* new_table, const int32_t* new_lengths,
+	const int32_t* info, const void* workspace) {
+	struct part {
+		const void* at;
+		int64_t bytes;
+	};
+	const int64_t cache_bytes = static_cast<int64_t>(
+		std::min<__int128>(static_cast<__int128>(c->layers * c->pages) * (c->kv_heads * c->page_size * c->head_dim * 2), int64_t{ 1 } << 62));
+	const int64_t need = nh_attn_pages_workspace_bytes(c->pages, children, b->table_width);
+	const part inputs[] = { { c->k_pages, cache_bytes }, { c->v_pages, cache_bytes }, { b->page_table, b->sequences * b->table_width * 4 }, { b->lengths, b->sequences * 4 }, { parents, children * 4 },
+		{ grow, children * 4 } };
+	const part results[] = { { new_table, children * b->table_width * 4 }, { new_lengths, children * 4 }, { info, 12 }, { workspace, need } };
+	auto apart = [](const part& x, const part& y) {
+		return x.bytes == 0 || y.bytes == 0 || !overlap(x.at, x.bytes, y.at, y.bytes);
+	};
+	for (const part* r = std::begin(results); r != std::end(results); ++r) {
+		for (const part& in : inputs) {
+			NH_REQUIRE(apart(*r, in), NH_ERR_ARGUMENT);
+		}
+		for (const part* other = std::begin(results); other != r; ++other) {
+			NH_REQUIRE(apart(*r, *other), NH_ERR_ARGUMENT);
+		}
+	}
 	return NH_OK;
 }
 static nh::pages_args pages(const nh_attn_cache* c, const nh_attn_batch* b, int32_t* new_table, int32_t* info, void* workspace) {
@@ -293,9 +320,7 @@ int nh_attn_cache_step(const nh_attn_cache* host_cache, const nh_attn_batch* hos
 	int32_t* info, void* workspace, int64_t workspace_bytes, void* stream) {
 	NH_TRY(check_pages(host_cache, host_batch, children, new_table, info, workspace, workspace_bytes));
 	NH_REQUIRE(children == 0 || (parents && grow && new_lengths), NH_ERR_NULL_POINTER);
-	NH_REQUIRE(!overlap(new_lengths, children * 4, host_batch->lengths, host_batch->sequences * 4) && !overlap(new_lengths, children * 4, parents, children * 4) &&
-			!overlap(new_lengths, children * 4, grow, children * 4),
-		NH_ERR_ARGUMENT);
+	NH_TRY(check_page_results(host_cache, host_batch, children, parents, grow, new_table, new_lengths, info, workspace));
 	NH_TRY(require_device());
 	nh::pages_args a = pages(host_cache, host_batch, new_table, info, workspace);
 	a.parents = parents, a.grow = grow, a.new_lengths = new_lengths;
@@ -306,6 +331,7 @@ int nh_attn_cache_step(const nh_attn_cache* host_cache, const nh_attn_batch* hos
 int nh_attn_cache_compact(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, int32_t* new_table, int32_t* info, void* workspace, int64_t workspace_bytes, void* stream) {
 	NH_REQUIRE(host_batch, NH_ERR_NULL_POINTER);
 	NH_TRY(check_pages(host_cache, host_batch, host_batch->sequences, new_table, info, workspace, workspace_bytes));
+	NH_TRY(check_page_results(host_cache, host_batch, host_batch->sequences, nullptr, nullptr, new_table, nullptr, info, workspace));
 	NH_TRY(require_device());
 	return from_hip(nh::launch_cache_compact(pages(host_cache, host_batch, new_table, info, workspace), as_stream(stream)));
 }
