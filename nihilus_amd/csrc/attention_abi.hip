@@ -123,6 +123,7 @@ int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* ho
 	NH_TRY(check_rows(host_cache, type, rows, host_cache->kv_heads, v_stride));
 	NH_REQUIRE(pairs >= 0 && pairs % 8 == 0 && 2 * pairs <= host_cache->head_dim, NH_ERR_SHAPE);
 	NH_REQUIRE(host_batch->starts || rows == host_batch->sequences, NH_ERR_ARGUMENT);
+	NH_REQUIRE(nh::append_rope_fits(rows, host_cache->kv_heads), NH_ERR_TOO_LARGE);
 	if (rows == 0 || host_batch->sequences == 0) {
 		return NH_OK;
 	}
@@ -171,15 +172,16 @@ static int check_memory(int64_t workspace_need, int64_t counter_need, const void
 static int check_heads(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, const int64_t* a, const int64_t* b) {
 	NH_REQUIRE(a && b, NH_ERR_NULL_POINTER);
 	NH_REQUIRE(rows >= 0 && sequences >= 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 && (head_dim == 64 || head_dim == 128), NH_ERR_SHAPE);
-	// one workgroup for 16 rows of a kv head, and one more for each sequence and kv head
 	NH_REQUIRE(sequences <= MAX_SEQUENCES && q_heads < 65536 && rows <= MAX_ROW_HEADS / q_heads && sequences * kv_heads <= MAX_ROW_HEADS / 4, NH_ERR_TOO_LARGE);
 	return NH_OK;
 }
 
 int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes) {
 	NH_TRY(check_heads(rows, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
+	const bool by_rows = nh::prompt_by_rows(rows, sequences, q_heads, kv_heads);
+	NH_REQUIRE(by_rows || nh::attention_tiles_fit(rows, sequences, q_heads, kv_heads), NH_ERR_TOO_LARGE);
 	const nh::attention_needs n = rows == 0 || sequences == 0 ? nh::attention_needs{ 0, 0 }
-		: nh::prompt_by_rows(rows, sequences, q_heads, kv_heads)  ? nh::attention_rows_needs(sequences, false, q_heads, kv_heads, head_dim, 0)
+		: by_rows												  ? nh::attention_rows_needs(sequences, false, q_heads, kv_heads, head_dim, 0)
 																  : nh::attention_tiles_needs(rows, sequences, q_heads, kv_heads, head_dim);
 	*host_workspace_bytes		= n.workspace;
 	*host_counter_bytes			= n.counters;
@@ -204,6 +206,7 @@ int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
 	a.counters			 = static_cast<int32_t*>(counters);
 	bool by_rows		 = nh::prompt_by_rows(rows, host_batch->sequences, q_heads, host_cache->kv_heads);
 	if (by_rows && !nh::attention_rows_fit(rows, host_batch->sequences, false, q_heads / host_cache->kv_heads, host_batch->table_width * host_cache->page_size)) {
+		NH_REQUIRE(nh::attention_tiles_fit(rows, host_batch->sequences, q_heads, host_cache->kv_heads), NH_ERR_TOO_LARGE);
 		by_rows		= false; // few rows against tables of a billion keys: more work than the rows kernel can number; the tile kernel without memory of its own
 		a.workspace = nullptr;
 	}
@@ -224,6 +227,7 @@ int nh_attn_decode_needs(int64_t sequences, int64_t q_heads, int64_t kv_heads, i
 	NH_TRY(check_heads(sequences, sequences, q_heads, kv_heads, head_dim, host_workspace_bytes, host_counter_bytes));
 	NH_REQUIRE(prefix_count >= 0 && page_shift(page_size) > 0, NH_ERR_SHAPE);
 	NH_REQUIRE(prefix_count <= MAX_KEYS / page_size, NH_ERR_TOO_LARGE);
+	NH_REQUIRE(nh::prefix_fits(nh::plan_prefix(sequences, q_heads / kv_heads, kv_heads, prefix_count * page_size), kv_heads), NH_ERR_TOO_LARGE);
 	const nh::attention_needs n = nh::attention_rows_needs(sequences, true, q_heads, kv_heads, head_dim, prefix_count * page_size);
 	*host_workspace_bytes		= n.workspace;
 	*host_counter_bytes			= n.counters;
@@ -269,7 +273,8 @@ static int check_pages(const nh_attn_cache* c, const nh_attn_batch* b, int64_t c
 	NH_TRY(check_cache(c));
 	NH_TRY(check_batch(b, c->page_size));
 	NH_REQUIRE(children >= 0, NH_ERR_SHAPE);
-	NH_REQUIRE(children <= MAX_SEQUENCES && children * b->table_width * c->page_size <= MAX_ALL_KEYS, NH_ERR_TOO_LARGE);
+	// (the page calls count a table's entries in 32 bits)
+	NH_REQUIRE(children <= MAX_SEQUENCES && children * b->table_width * c->page_size <= MAX_ALL_KEYS && children * b->table_width <= INT32_MAX, NH_ERR_TOO_LARGE);
 	const int64_t need = nh_attn_pages_workspace_bytes(c->pages, children, b->table_width);
 	NH_REQUIRE(need >= 0, static_cast<int>(need));
 	NH_REQUIRE(info && (workspace || need == 0) && (new_table || children * b->table_width == 0), NH_ERR_NULL_POINTER);

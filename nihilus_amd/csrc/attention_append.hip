@@ -160,6 +160,11 @@ __global__ __launch_bounds__(THREADS) void append_rope_kernel(append_args a, int
 	}
 }
 
+// (with the heads of a row over several workgroups there are 2048 of those at most)
+bool append_rope_fits(int64_t rows, int64_t kv_heads) {
+	return (rows + (rows + V_ROWS - 1) / V_ROWS * kv_heads) * THREADS < GRID_THREADS;
+}
+
 template<int CACHE, int TYPE, int D> static hipError_t launch_append(const append_args& a, hipStream_t s) {
 	constexpr int HEADS = THREADS / (D / 4);
 	const int64_t full	= (a.q_heads + a.cache.kv_heads + HEADS - 1) / HEADS;

@@ -179,6 +179,9 @@ template<int D> struct not_finite {
 
 // ---- launch functions (after argument checks) ----
 
+// a launch has fewer threads along its grid than this
+constexpr int64_t GRID_THREADS = int64_t{ 1 } << 32;
+
 struct append_args {
 	cache_view cache;
 	batch_view batch;
@@ -189,6 +192,7 @@ struct append_args {
 	int rows, q_heads, head_dim, pairs;
 	bool interleaved;
 };
+bool append_rope_fits(int64_t rows, int64_t kv_heads); // one launch
 hipError_t launch_append_rope(const append_args& a, int cache_type, int type, hipStream_t s);
 
 struct attention_args {
@@ -211,12 +215,14 @@ struct attention_needs {
 };
 // The tile kernel (attention_prompt.hip): 128 rows of a sequence at a time.
 attention_needs attention_tiles_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+bool attention_tiles_fit(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads); // one launch
 hipError_t launch_attention_tiles(const attention_args& a, int cache_type, int type, hipStream_t s);
 // The part of a decode step over a prefix that all sequences share: the batch's rows as tiles, the keys in pieces.
 struct prefix_cut {
 	int64_t pieces, keys, row_tiles; // keys of a piece
 };
 prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64_t prefix_keys);
+bool prefix_fits(const prefix_cut& cut, int64_t kv_heads); // one launch
 // partial results [piece][sequence][q_head]: o unnormalised, ml the running maximum (log2) and the sum of the weights
 hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s);
 // The rows kernel (attention_rows.hip): 16 rows of a sequence at a time, keys and values straight from memory and cut into pieces.

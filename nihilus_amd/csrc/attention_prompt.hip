@@ -625,6 +625,11 @@ attention_needs attention_tiles_needs(int64_t rows, int64_t sequences, int64_t q
 	return c.pieces > 1 ? attention_needs{ c.tiles * kv_heads * c.pieces * WAVES * (head_dim / 2 + 2) * 64 * 4, c.tiles * kv_heads * 4 } : attention_needs{ 0, 0 };
 }
 
+// (a second group of waves, or pieces, only where the workgroups are few)
+bool attention_tiles_fit(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads) {
+	return plan_tiles(rows, sequences, q_heads / kv_heads, kv_heads).tiles * kv_heads * 64 * WAVES < GRID_THREADS;
+}
+
 template<int CACHE, int TYPE, int D, int KIND> static hipError_t launch_tiles(const attention_args& a, const prefix_out& out, const tile_pieces& cut, int64_t tiles, bool parts, hipStream_t s) {
 	const dim3 grid(static_cast<unsigned>(tiles * a.cache.kv_heads * cut.pieces));
 	constexpr bool FITS = D == 64 || terms<CACHE, TYPE> < 3; // (three terms of 128 values: no registers for a second wave per SIMD)
@@ -669,6 +674,9 @@ prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64
 	c.keys				 = ((prefix_keys + wanted - 1) / wanted + 2 * KEYS - 1) / (2 * KEYS) * (2 * KEYS);
 	c.pieces			 = (prefix_keys + c.keys - 1) / c.keys;
 	return c;
+}
+bool prefix_fits(const prefix_cut& cut, int64_t kv_heads) {
+	return cut.pieces * cut.row_tiles * kv_heads * 64 * WAVES * 2 < GRID_THREADS;
 }
 hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s) {
 	return launch_tiles<OVER_PREFIX>(a, cache_type, type, prefix_out{ o, ml, static_cast<int>(cut.keys), static_cast<int>(cut.row_tiles) }, tile_pieces{ nullptr, nullptr, 1 }, cut.pieces * cut.row_tiles,

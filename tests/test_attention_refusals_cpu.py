@@ -91,3 +91,57 @@ def test_a_workspace_of_the_page_calls_over_anything_else_is_refused(name):
         assert _step(cache, batch, here["parents"], here["grow"], 3, here["new_table"], here["new_lengths"], here["info"], ws, need) == -6, at
         if name not in ("parents", "grow", "new_lengths"):
             assert _compact(cache, batch, here["new_table"], here["info"], ws, need) == -6, at
+
+
+# A launch has fewer than 2^32 threads along its grid: what the kernels would need more for is refused ahead of it.
+
+
+def _fits(status):
+    """What is not refused ends at the missing GPU; with one it would run."""
+    return status == -4
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,fits", [((1 << 24) - 270000, 1, 1, True), ((1 << 24) - 250000, 1, 1, False), (1 << 24, 2, 1, False), (1 << 28, 4, 2, False), (1 << 30, 1, 1, False),
+                                                       (1 << 14, 65535, 65535, False), (8191, 65535, 65535, True)])
+def test_rows_of_append_that_no_launch_has_workgroups_for(rows, heads, kv_heads, fits):
+    # a workgroup of 256 threads for each row, and one for 64 rows of a head's values
+    assert (rows + -(-rows // 64) * kv_heads < 1 << 24) == fits
+    if fits and torch.cuda.is_available():
+        return
+    far = dict(q=1 << 44, out=1 << 45, k=1 << 46, v=(1 << 46) + (1 << 45), batch=_batch(starts=BOGUS), cache=_cache(kv_heads=kv_heads))
+    status = _append(rows=rows, heads=heads, strides=(heads * 64, kv_heads * 64, kv_heads * 64), **far)
+    assert _fits(status) if fits else status == -5
+
+
+@pytest.mark.parametrize("rows,sequences,heads,kv_heads,fits", [(5 << 20, 1 << 20, 32, 8, True), (5 << 20, 1 << 20, 64, 16, False), (1 << 20, 200000, 256, 64, True), (1 << 21, 1 << 18, 256, 64, False)])
+def test_tiles_of_a_prompt_that_no_launch_has_workgroups_for(rows, sequences, heads, kv_heads, fits):
+    from nihilus_amd import _lib
+
+    tiles = (rows * (heads // kv_heads) // 128 + sequences) * kv_heads
+    assert (tiles < 1 << 24) == fits and _lib.lib().nh_attn_debug_prompt_kernel(rows, sequences, heads, kv_heads, -1) == 2
+    n, c = C.c_int64(), C.c_int64()
+    assert _lib.lib().nh_attn_prompt_needs(rows, sequences, heads, kv_heads, 64, C.byref(n), C.byref(c)) == (0 if fits else -5)
+    if fits and torch.cuda.is_available():
+        return
+    status = _prompt(cache=_cache(kv_heads=kv_heads), batch=_batch(starts=BOGUS, sequences=sequences), q=1 << 44, out=1 << 45, rows=rows, heads=heads, stride=heads * 64, bytes=1 << 60, counter_bytes=1 << 60)
+    assert _fits(status) if fits else status == -5
+
+
+def test_tiles_of_a_prefix_that_no_launch_has_workgroups_for():
+    from nihilus_amd import _lib
+
+    n, c = C.c_int64(), C.c_int64()
+    for sequences, status in [((1 << 20) - 8, 0), (1 << 20, -5)]:  # 1024 query heads of one kv head: eight tiles of 512 threads each
+        assert _lib.lib().nh_attn_decode_needs(sequences, 1024, 1, 64, 1, 16, C.byref(n), C.byref(c)) == status
+        assert _lib.lib().nh_attn_decode_needs(sequences, 1024, 1, 64, 0, 16, C.byref(n), C.byref(c)) == 0
+    assert _decode(cache=_cache(kv_heads=1), batch=_batch(sequences=1 << 20, table_width=1), prefix=BOGUS, count=1, q=1 << 44, out=1 << 45, heads=1024, stride=65536, bytes=1 << 60, counter_bytes=1 << 60) == -5
+
+
+def test_more_table_entries_than_a_step_can_count():
+    # 2^31 pages could be wanted at once, one more than the counts of `info` hold
+    sequences, width = 1 << 20, 1 << 11
+    batch = _batch(page_table=1 << 40, sequences=sequences, table_width=width)
+    assert _step(batch=batch, children=sequences, parents=1 << 41, grow=1 << 42, table=1 << 43, lengths=1 << 44) == -5
+    assert _compact(batch=batch, table=1 << 43) == -5
+    if not torch.cuda.is_available():
+        assert _fits(_step(batch=_batch(page_table=1 << 40, lengths=1 << 39, sequences=sequences, table_width=width), children=sequences - 1, parents=1 << 41, grow=1 << 42, table=1 << 43, lengths=1 << 44, ws=1 << 45))
