@@ -59,6 +59,12 @@ template<int CACHE, int N> __device__ __forceinline__ void split8(const float (&
 __device__ __forceinline__ float exp2_fast(float x) {
 	return __builtin_amdgcn_exp2f(x); // v_exp_f32: 1 ulp; arguments here are <= 0, results below 2^-126 are flushed, far under a sum that holds a 1
 }
+// What the sums of a part of the keys are multiplied with when parts are joined: 2^x, x how far (in powers of two) the part's maximum lies below the joint one.
+// Never zero: an infinite value has been added to its part by then and has to stay one (infinity times zero is NaN), and 2^-126 of a part shows nowhere
+// beside one whose weights add up to 1 and more.
+__device__ __forceinline__ float part_factor(float x) {
+	return fmaxf(exp2_fast(x), 0x1p-126f);
+}
 // the value of lane ^ 32 (^ 16)
 __device__ __forceinline__ float swap32(float x, int lane) {
 	const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);

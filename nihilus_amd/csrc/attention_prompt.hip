@@ -493,7 +493,7 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 		}
 		const float m2 = theirs[16 * DT * 64], l2 = theirs[(16 * DT + 1) * 64];
 		const float both = fmaxf(m, m2), below = both == -__builtin_inff() ? 0.0f : both;
-		const float f1 = exp2_fast(m - below), f2 = exp2_fast(m2 - below);
+		const float f1 = part_factor(m - below), f2 = part_factor(m2 - below);
 		l = l * f1 + l2 * f2;
 		m = both;
 #pragma unroll
@@ -564,7 +564,7 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 				}
 			}
 			const float both = fmaxf(m, m2), below = both == -__builtin_inff() ? 0.0f : both;
-			const float f1 = exp2_fast(m - below), f2 = exp2_fast(m2 - below);
+			const float f1 = part_factor(m - below), f2 = part_factor(m2 - below);
 			l = l * f1 + l2 * f2;
 			m = both;
 #pragma unroll

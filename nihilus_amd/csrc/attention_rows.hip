@@ -192,7 +192,7 @@ struct running {
 	v4f o;
 	__device__ __forceinline__ void add(float m2, float l2, v4f o2) {
 		const float both = fmaxf(m, m2), at = both == -__builtin_inff() ? 0.0f : both;
-		const float f1 = exp2_fast(m - at), f2 = exp2_fast(m2 - at);
+		const float f1 = part_factor(m - at), f2 = part_factor(m2 - at);
 		l = l * f1 + l2 * f2;
 		o = o * f1 + o2 * f2;
 		m = both;
@@ -664,7 +664,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 					x[dt] = *reinterpret_cast<const v4f*>(from + 16 * dt);
 				}
 				const float both = fmaxf(m, ml.x), below = both == -__builtin_inff() ? 0.0f : both;
-				const float f1 = exp2_fast(m - below), f2 = exp2_fast(ml.x - below);
+				const float f1 = part_factor(m - below), f2 = part_factor(ml.x - below);
 				m = both;
 				l = l * f1 + (quarter == 0 ? ml.y * f2 : 0.0f); // (l is added up over the quarters below)
 #pragma unroll
@@ -702,7 +702,7 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 			float f[WAVES], sum = 0.0f;
 #pragma unroll
 			for (int x = 0; x < WAVES; ++x) {
-				f[x] = exp2_fast(ml[x].x - at);
+				f[x] = part_factor(ml[x].x - at);
 				sum += ml[x].y * f[x];
 			}
 			v4f v[DT / WAVES];

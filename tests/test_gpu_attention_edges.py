@@ -40,3 +40,29 @@ def test_calls_for_nobody(A, monkeypatch, native):  # noqa: F811
     assert new.shape == (0, table.shape[1]) and lengths.shape == (0,) and info.tolist() == [0, 0, 0]
     new, info = A.cache_compact(k[None], v[None], table[:0], none)
     assert new.shape == (0, table.shape[1]) and info.tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("length", [150, 3000])
+def test_odd_values_far_below_the_largest_score(A, kernel, dtype, cache, dim, page, length):  # noqa: F811
+    # One key's score is thousands above all others, so that what any other part of the keys adds up to is joined with a factor that is too small for fp32. An
+    # infinite value there stays infinite all the same, wherever the keys are cut: over waves, groups of waves, workgroups, a prefix and its pieces.
+    pages = 1280 // page if length == 3000 else 64 // page
+    for top in (5, length // 2, length - 10):
+        b = Batch(41, [length], page, 2, dim, cache, shared=pages)
+        ahead = torch.sign(torch.randn(2, dim, generator=b.g))  # the direction that the largest score has, for each kv head
+        b.k[b.table[0][top // page], :, top % page] = (8 * ahead).to(cache)
+        for i, j in enumerate(range(3, length - 6, max(1, length // 40))):
+            if j != top:
+                b.v[b.table[0][j // page], i % 2, i, j % page] = (INF, -INF, INF, NAN)[i % 4]
+        q = (60 * ahead.repeat_interleave(4, 0) + b.rows(5, 8, F32)).to(dtype)
+        k, v, table, lengths = b.device()
+        keys, values, there = b.keys(0, length)
+        out = A.attention_prompt(q.cuda(), k, v, table, lengths, torch.tensor([0, 5], dtype=torch.int32).cuda()).cpu()
+        for i in range(5):
+            seen = length - 4 + i
+            _check_with_odd_values(out[i], q[i], keys[:, :seen], values[:, :seen], there[:seen], dim**-0.5, dtype, ("prompt", top, i))
+        for prefix in (None, torch.tensor(b.common, dtype=torch.int32).cuda()):
+            out = A.attention_decode(q[:1].cuda(), k, v, table, lengths, prefix_pages=prefix).cpu()
+            _check_with_odd_values(out[0], q[0], keys, values, there, dim**-0.5, dtype, ("decode", top, prefix is not None))
