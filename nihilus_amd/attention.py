@@ -140,6 +140,15 @@ class Workspace:
         return self.memory.data_ptr(), self.memory.numel(), self.counters.data_ptr(), 4 * self.counters.numel()
 
 
+_PER_THREAD = 2  # hipStreamPerThread: the handle that names the calling thread's own default stream
+
+
+def _own_memory(nbytes: int, device: torch.device) -> None:
+    """Refuses memory of the call's own where torch's allocator would give it to another thread's call while this one runs: it tells streams apart by their handles."""
+    if nbytes and (_stream() if device.index == torch.cuda.current_device() else torch.cuda.current_stream(device).cuda_stream) == _PER_THREAD:
+        raise ValueError("the per-thread default stream is another one in each thread: give a workspace, or use a stream of torch's")
+
+
 def _needs(fn: str, *sizes) -> tuple[int, int]:
     n, c = C.c_int64(), C.c_int64()
     _lib.check(fn, getattr(_lib.lib(), fn)(*sizes, C.byref(n), C.byref(c)))
@@ -170,6 +179,7 @@ def attention_prompt(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     out = _out(out, q)
     if workspace is None:
         workspace = prompt_workspace(q.shape[0], page_table.shape[0], q.shape[1], k_pages.shape[1], k_pages.shape[3], q.device)
+        _own_memory(workspace.memory.numel(), q.device)
     _call("nh_attn_prompt", q.device, C.byref(cache), C.byref(batch), q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[0], q.shape[1], stride, scale, *workspace.args(k_pages))
     return out
 
@@ -197,6 +207,7 @@ def attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     if workspace is None:
         _, kv_heads, page_size, head_dim = k_pages.shape
         workspace = decode_workspace(q.shape[0], q.shape[1], kv_heads, head_dim, count, page_size, q.device)
+        _own_memory(workspace.memory.numel(), q.device)
     _call("nh_attn_decode", q.device, C.byref(cache), C.byref(batch), prefix_pages.data_ptr() if count else None, count, q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], q.shape[1], stride, scale,
           *workspace.args(k_pages))
     return out
@@ -205,6 +216,7 @@ def attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
 def _pages_workspace(pages: int, sequences: int, width: int, device) -> torch.Tensor:
     n = _lib.lib().nh_attn_pages_workspace_bytes(pages, sequences, width)
     _lib.check("nh_attn_pages_workspace_bytes", n if n < 0 else 0)
+    _own_memory(n, device)
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 

@@ -270,13 +270,21 @@ at::Tensor ints_like(const at::Tensor& t, at::IntArrayRef sizes) {
 	return at::empty(sizes, t.options());
 }
 
-// Counters of zeros for a call on stream s of t's device.  Every call leaves them zero, so the calls of a stream, which run one after the other,
-// share theirs; a stream that is being captured gets new ones, whose clearing is captured with the call.
+// Whether memory that a call takes for itself and gives back to torch's allocator may go to the next call on a stream of the same handle: not under the handle that names
+// every thread's own default stream, where that call may be another thread's and waits for nothing.  (The Python way refuses it.)
+bool own_memory(void* s) {
+	return s != static_cast<void*>(hipStreamPerThread);
+}
+
+// Counters of zeros for a call on the current stream s of t's device.  Every call leaves them zero, so the calls of a stream, which run one after the other,
+// share theirs.  New ones for a stream that is being captured, whose clearing is captured with the call, and for one that is neither the default stream nor of
+// torch's pool (torch numbers such a stream by its handle): its owner may destroy it, and the handle come back.
 at::Tensor counters_for(const at::Tensor& t, void* s, int64_t bytes) {
 	static auto* kept = new std::map<std::pair<int, void*>, at::Tensor>; // (never destroyed: the interpreter's end is too late to free device memory)
 	hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-	const bool plain = hipStreamIsCapturing(static_cast<hipStream_t>(s), &capturing) == hipSuccess && capturing == hipStreamCaptureStatusNone;
-	const auto zeros = [&](int64_t n) { return at::zeros({ n }, t.options().dtype(at::kInt)); };
+	const bool foreign = s && c10::hip::getCurrentHIPStream().id() == reinterpret_cast<intptr_t>(s);
+	const bool plain   = !foreign && hipStreamIsCapturing(static_cast<hipStream_t>(s), &capturing) == hipSuccess && capturing == hipStreamCaptureStatusNone;
+	const auto zeros   = [&](int64_t n) { return at::zeros({ n }, t.options().dtype(at::kInt)); };
 	if (!plain) {
 		return zeros(bytes / 4);
 	}
@@ -328,9 +336,12 @@ PyObject* attention_prompt(args& in) {
 	if (nh_attn_prompt_needs(rows, p.batch.sequences, heads, p.cache.kv_heads, p.cache.head_dim, &need, &counter_need) != 0) {
 		return nullptr;
 	}
+	void *s = stream(), *ws = nullptr, *cs = nullptr;
+	if (need > 0 && !own_memory(s)) {
+		return nullptr;
+	}
 	const at::Tensor out = like(*q);
 	at::Tensor workspace, counters;
-	void *s = stream(), *ws = nullptr, *cs = nullptr;
 	if (need > 0) {
 		workspace = bytes_like(*q, need), counters = counters_for(*q, s, counter_need);
 		ws = workspace.mutable_data_ptr(), cs = counters.mutable_data_ptr();
@@ -359,7 +370,10 @@ PyObject* attention_decode(args& in) {
 	if (nh_attn_decode_needs(p.batch.sequences, heads, p.cache.kv_heads, p.cache.head_dim, count, p.cache.page_size, &need, &counter_need) != 0) {
 		return nullptr;
 	}
-	void* s				 = stream();
+	void* s = stream();
+	if (need > 0 && !own_memory(s)) {
+		return nullptr;
+	}
 	const at::Tensor out = like(*q), workspace = bytes_like(*q, need), counters = counters_for(*q, s, counter_need);
 	const void* qp	  = q->const_data_ptr();
 	const int32_t* pp = count > 0 ? static_cast<const int32_t*>(prefix->const_data_ptr()) : nullptr;
@@ -380,14 +394,15 @@ PyObject* cache_step(args& in) {
 		return nullptr;
 	}
 	const int64_t n = parents->size(0), need = nh_attn_pages_workspace_bytes(p.cache.pages, n, p.batch.table_width);
-	if (need < 0) {
+	void* s = stream();
+	if (need < 0 || (need > 0 && !own_memory(s))) {
 		return nullptr;
 	}
 	const at::Tensor new_table = ints_like(*table, { n, p.batch.table_width }), now = ints_like(*table, { n }), info = ints_like(*table, { 3 });
 	const at::Tensor workspace = need > 0 ? bytes_like(*table, need) : at::Tensor();
 	const auto *pp = static_cast<const int32_t*>(parents->const_data_ptr()), *gp = static_cast<const int32_t*>(grow->const_data_ptr());
 	auto *tp = static_cast<int32_t*>(new_table.mutable_data_ptr()), *np = static_cast<int32_t*>(now.mutable_data_ptr()), *ip = static_cast<int32_t*>(info.mutable_data_ptr());
-	void *ws = need > 0 ? workspace.mutable_data_ptr() : nullptr, *s = stream();
+	void* ws = need > 0 ? workspace.mutable_data_ptr() : nullptr;
 	PyObject* first = finish(new_table, [&] { return nh_attn_cache_step(&p.cache, &p.batch, pp, gp, n, tp, np, ip, ws, need, s); });
 	return first && THPVariable_Check(first) ? Py_BuildValue("NNN", first, THPVariable_Wrap(now), THPVariable_Wrap(info)) : first;
 }
@@ -404,13 +419,14 @@ PyObject* cache_compact(args& in) {
 		return nullptr;
 	}
 	const int64_t need = nh_attn_pages_workspace_bytes(p.cache.pages, p.batch.sequences, p.batch.table_width);
-	if (need < 0) {
+	void* s = stream();
+	if (need < 0 || (need > 0 && !own_memory(s))) {
 		return nullptr;
 	}
 	const at::Tensor new_table = like(*table), info = ints_like(*table, { 3 });
 	const at::Tensor workspace = need > 0 ? bytes_like(*table, need) : at::Tensor();
 	auto *tp = static_cast<int32_t*>(new_table.mutable_data_ptr()), *ip = static_cast<int32_t*>(info.mutable_data_ptr());
-	void *ws = need > 0 ? workspace.mutable_data_ptr() : nullptr, *s = stream();
+	void* ws = need > 0 ? workspace.mutable_data_ptr() : nullptr;
 	PyObject* first = finish(new_table, [&] { return nh_attn_cache_compact(&p.cache, &p.batch, tp, ip, ws, need, s); });
 	return first && THPVariable_Check(first) ? Py_BuildValue("NN", first, THPVariable_Wrap(info)) : first;
 }

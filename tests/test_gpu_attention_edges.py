@@ -66,3 +66,56 @@ def test_odd_values_far_below_the_largest_score(A, kernel, dtype, cache, dim, pa
         for prefix in (None, torch.tensor(b.common, dtype=torch.int32).cuda()):
             out = A.attention_decode(q[:1].cuda(), k, v, table, lengths, prefix_pages=prefix).cpu()
             _check_with_odd_values(out[0], q[0], keys, values, there, dim**-0.5, dtype, ("decode", top, prefix is not None))
+
+
+PER_THREAD = 2  # the handle that names the calling thread's own default stream, whichever thread that is
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_the_stream_that_is_another_one_in_each_thread(A, monkeypatch, native):  # noqa: F811
+    # Memory that a call takes for itself goes to the next call on a stream of the same handle, here another thread's, which does not wait for this one.
+    if not native:
+        monkeypatch.setattr(A, "_calls", None)
+    b = Batch(43, [700, 33], 32, 2, 64, F16)
+    q = b.rows(2, 8, F32)
+    k, v, table, dl = b.device()
+    x, starts = q.cuda(), torch.tensor([0, 1, 2], dtype=torch.int32).cuda()
+    large = tuple(t[0] for t in A.empty_cache(1, 50000, 1, 16, 64))
+    ints = torch.zeros(2, dtype=torch.int32).cuda()
+    spaces = A.decode_workspace(2, 8, 2, 64), A.prompt_workspace(2, 2, 8, 2, 64)
+    want = A.attention_decode(x, k, v, table, dl), A.attention_prompt(x, k, v, table, dl, starts)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.ExternalStream(PER_THREAD)):
+        for call in (lambda: A.attention_decode(x, k, v, table, dl), lambda: A.attention_prompt(x, k, v, table, dl, starts), lambda: A.cache_step(large[0][None], large[1][None], table, dl, ints, ints),
+                     lambda: A.cache_compact(large[0][None], large[1][None], table, dl)):
+            with pytest.raises(ValueError):
+                call()
+        got = A.attention_decode(x, k, v, table, dl, workspace=spaces[0]), A.attention_prompt(x, k, v, table, dl, starts, workspace=spaces[1])
+        A.cache_step(k[None], v[None], table, dl, ints, ints)  # (a small cache's step needs no memory)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_streams_of_other_owners_leave_nothing_behind(A):  # noqa: F811
+    # the handle of a stream that somebody else made and destroyed may be given out again: nothing is kept under it
+    import ctypes
+
+    path = next(line.split()[-1] for line in open("/proc/self/maps") if "libamdhip64" in line)
+    hip = ctypes.CDLL(path)
+    b = Batch(47, [3000, 50, 900], 64, 2, 128, F16)
+    k, v, table, dl = b.device()
+    q = b.rows(3, 8, F32).cuda()
+    want = A.attention_decode(q, k, v, table, dl)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(6):
+        handle = ctypes.c_void_p()
+        assert hip.hipStreamCreate(ctypes.byref(handle)) == 0
+        with torch.cuda.stream(torch.cuda.ExternalStream(handle.value)):
+            for _ in range(3):
+                got = A.attention_decode(q, k, v, table, dl)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        del got
+        assert torch.cuda.memory_allocated() == before
+        assert hip.hipStreamDestroy(handle) == 0
