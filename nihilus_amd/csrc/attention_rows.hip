@@ -212,7 +212,7 @@ template<int CACHE, int TYPE, int D>
 __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_t* lengths, const int32_t* page_table, const void* q_rows, const uint16_t* k_pages, const int32_t* starts,
 	uint32_t shape, int first_width, int prefix_or_rows, uint32_t heads, rows_args) {
 	// What the first loads take comes first, in fourteen dwords: those arrive in registers, the rest is read from memory, as far away as the data.
-	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | one row per sequence << 31
+	// heads: kv_heads | group << 16;  shape: sequences | log2 of the page size << 21 | log2 of the units << 25 | whether starts are checked << 30 | one row per sequence << 31
 	const int first_kv_heads = heads & 0xFFFF, first_group = heads >> 16, sequences = shape & 0x1FFFFF, first_page_shift = (shape >> 21) & 15;
 	const bool one_each = (shape >> 31) != 0;
 	const int all_rows	= one_each ? sequences : prefix_or_rows, prefix_count = one_each ? prefix_or_rows : 0; // (only a decode step has a prefix)
@@ -288,6 +288,16 @@ __global__ __launch_bounds__(THREADS, 2) void attention_rows_kernel(const int32_
 	};
 	const int little	  = longer_than(1024) ? 32 : longer_than(384) ? 20 : longer_than(64) ? 8 : WAVES;
 	const int first_share = max((total + (1 << log2_units) - 1) >> log2_units, little);
+	if (shape >> 30 & 1) { // starts that descend could have the same rows in so many sequences that their work has no 32-bit number: nothing is done then
+		bool descend = false;
+		for (int seq = first_lane; seq < sequences; seq += 64) {
+			descend |= starts[seq + 1] < starts[seq];
+		}
+		if (__builtin_amdgcn_ballot_w64(descend)) {
+			wait_stores_acknowledged();
+			return;
+		}
+	}
 	int at			= blockIdx.y * first_share;
 	const int end	= min(at + first_share, total);
 	if (at >= end) {
@@ -813,6 +823,10 @@ bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t 
 	const int64_t row_groups = one_each ? sequences * ((group + COLUMNS - 1) / COLUMNS) : rows * group / COLUMNS + sequences;
 	return row_groups * (table_keys / STEP + 1 + FIXED) < (int64_t{ 1 } << 30);
 }
+// the same whatever the starts are: each sequence may have all rows (double: up to 2^20 sequences, 2^26 row groups and 2^25 steps)
+static bool any_starts_fit(int64_t rows, int64_t sequences, int64_t group, int64_t table_keys) {
+	return static_cast<double>(sequences) * static_cast<double>(rows * group / COLUMNS + 1) * static_cast<double>(table_keys / STEP + 1 + FIXED) < 1073741824.0;
+}
 
 template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attention_args& a, hipStream_t s) {
 	const int64_t group = a.q_heads / a.cache.kv_heads, sequences = a.batch.sequences;
@@ -833,13 +847,14 @@ template<int CACHE, int TYPE, int D> static hipError_t launch_rows(const attenti
 	const int64_t steps		 = (static_cast<int64_t>(a.batch.width) << a.cache.page_shift) / STEP + 1 + FIXED;
 	attention_args late = a;
 	late.prefix_count	= one_each && !a.prefix_apart ? a.prefix_count : 0;
+	const bool check_starts	= !one_each && !any_starts_fit(a.rows, sequences, group, static_cast<int64_t>(a.batch.width) << a.cache.page_shift);
 	int log2_units			 = 0;
 	while ((2 << log2_units) <= cut.units && (WAVES << log2_units) < row_groups * steps) {
 		++log2_units;
 	}
 	attention_rows_kernel<CACHE, TYPE, D><<<dim3(static_cast<unsigned>(a.cache.kv_heads), 1u << log2_units), dim3(THREADS), 0, s>>>(a.batch.lengths,
 		a.batch.width > 0 ? a.batch.table : a.batch.lengths, a.q, a.cache.k, a.batch.starts,
-		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | static_cast<uint32_t>(log2_units) << 25 | (one_each ? 1u << 31 : 0u), a.batch.width,
+		static_cast<uint32_t>(a.batch.sequences) | static_cast<uint32_t>(a.cache.page_shift) << 21 | static_cast<uint32_t>(log2_units) << 25 | (check_starts ? 1u << 30 : 0u) | (one_each ? 1u << 31 : 0u), a.batch.width,
 		one_each ? (a.prefix_apart ? a.prefix_count : 0) : a.rows, static_cast<uint32_t>(a.cache.kv_heads) | static_cast<uint32_t>(group) << 16, rows_args{ late, w });
 	return hipGetLastError();
 }

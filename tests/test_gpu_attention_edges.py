@@ -119,3 +119,20 @@ def test_streams_of_other_owners_leave_nothing_behind(A):  # noqa: F811
         del got
         assert torch.cuda.memory_allocated() == before
         assert hip.hipStreamDestroy(handle) == 0
+
+
+@pytest.mark.parametrize("heads", [4, 64])
+def test_starts_that_descend(A, kernel, heads):  # noqa: F811
+    # the same rows in half of 2048 sequences of 64000 keys: more work, in steps, than 32 bits hold, also of the sequences that a wave adds up at once
+    rows, n, pages = 1 << 18, 2048, 250
+    rows = rows * 4 // heads
+    k, v = (t[0].zero_() for t in A.empty_cache(1, pages, heads // 4, 256, 64))
+    memory = torch.full((rows + 256, heads, 64), 7.0, dtype=F16, device="cuda")
+    q = torch.zeros(rows, heads, 64, dtype=F16, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32).repeat(n, 1).cuda()
+    lengths = torch.full((n,), 64000, dtype=torch.int32).cuda()
+    starts = torch.tensor([0, rows] * (n // 2) + [0], dtype=torch.int32).cuda()
+    A.attention_prompt(q, k, v, table, lengths, starts, out=memory[128:-128])
+    assert bool((memory[:128] == 7).all()) and bool((memory[-128:] == 7).all())
+    if kernel == 1:
+        assert bool((memory == 7).all())
