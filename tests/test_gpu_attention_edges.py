@@ -136,3 +136,68 @@ def test_starts_that_descend(A, kernel, heads):  # noqa: F811
     assert bool((memory[:128] == 7).all()) and bool((memory[-128:] == 7).all())
     if kernel == 1:
         assert bool((memory == 7).all())
+
+
+def _spoilt(b, seq, missing, odd):
+    """Pages that the cache does not have and values that are not finite, past the keys whose pages a wave holds at once."""
+    for j, d, x in odd:
+        b.v[b.table[seq][j // b.page], :, d, j % b.page] = x
+    for j in missing:
+        b.table[seq][j // b.page] = (-1, len(b.k), 2**31 - 1)[j % 3]
+
+
+def _keys(b, seq, n, prefix=()):
+    """As Batch.keys, for many keys at a time."""
+    row = torch.tensor(list(prefix) + b.table[seq][len(prefix) :])
+    j = torch.arange(n)
+    id = row[j // b.page]
+    there = (id >= 0) & (id < len(b.k))
+    id = torch.where(there, id, 0)
+    k, v = b.k[id, :, j % b.page].double(), b.v[id, :, :, j % b.page].double()  # [n, kv heads, dim]
+    return torch.where(there[:, None, None], k, 0.0).transpose(0, 1), torch.where(there[:, None, None], v, 0.0).transpose(0, 1), there
+
+
+def _check_rows_of_long_prompts(b, out, q, new, heads, dtype):
+    starts, out = _starts(new), out.cpu()
+    for seq, n in enumerate(new):
+        keys, values, there = _keys(b, seq, b.lengths[seq])
+        for i in sorted({0, 1, 127, 128, n // 3, n // 2, n - 129, n - 2, n - 1} & set(range(n))):
+            seen = b.lengths[seq] - n + i + 1
+            _check_with_odd_values(out[starts[seq] + i], q[starts[seq] + i], keys[:, :seen], values[:, :seen], there[:seen], b.dim**-0.5, dtype, (seq, i))
+
+
+# what the sizes choose (plan_tiles in attention_prompt.hip): tiles * kv heads above 320 one group of waves per workgroup, above 160 two, below that pieces of the keys too; parts
+# and pieces of more than sixteen tiles of 64 keys, so that the pages of the next 1024 keys are taken up on the way
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (128, 16)])
+@pytest.mark.parametrize("new,cached,heads,kv_heads,many", [([2600, 300, 1], [700, 1500, 2500], 16, 16, (321, 1 << 20)), ([700], [4500], 32, 8, (161, 320)), ([300], [10000], 32, 8, (1, 160))],
+                         ids=["one_group_of_waves", "two", "pieces"])
+def test_tiles_past_a_thousand_keys(A, dtype, cache, dim, page, new, cached, heads, kv_heads, many):  # noqa: F811
+    tiles = (sum(new) * (heads // kv_heads) // 128 + len(new)) * kv_heads
+    assert many[0] <= tiles <= many[1] and A._lib.lib().nh_attn_debug_prompt_kernel(sum(new), len(new), heads, kv_heads, -1) == 2
+    b = Batch(61, [a + c for a, c in zip(new, cached)], page, kv_heads, dim, cache)
+    last = b.lengths[0] - 1
+    _spoilt(b, 0, [1024, 1153, 2050, last - 200], [(1000, 0, INF), (1100, 1, NAN), (2047, 2, -INF), (2200, 3, INF), (2900, 4, NAN), (last - 1, 5, INF), (last, 6, NAN)])
+    q = b.rows(sum(new), heads, dtype)
+    k, v, table, lengths = b.device()
+    out = A.attention_prompt(q.cuda(), k, v, table, lengths, torch.tensor(_starts(new), dtype=torch.int32).cuda())
+    _check_rows_of_long_prompts(b, out, q, new, heads, dtype)
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_pieces_of_a_prefix_past_a_thousand_keys(A, dtype, cache, dim, page):  # noqa: F811
+    n, prefix = 9, 16384  # nine tiles of rows and eight kv heads: three pieces of 5504 keys, two parts each, apart from the sequences' own keys
+    own = [0, 40, 1, 7, 64, 130, 17, -prefix + 2500, 3]  # the last one ends inside the prefix
+    b = Batch(67, [prefix + x for x in own], page, 8, dim, cache, shared=prefix // page)
+    for j, d, x in [(900, 0, INF), (1500, 1, NAN), (2100, 2, -INF), (3000, 3, INF), (6000, 4, NAN), (12000, 5, -INF), (16383, 6, INF)]:
+        b.v[b.common[j // page], :, d, j % page] = x
+    common = list(b.common)
+    common[1200 // page], common[7000 // page] = -1, len(b.k) + 3
+    q = b.rows(n, 1024, dtype)
+    k, v, table, lengths = b.device()
+    out = A.attention_decode(q.cuda(), k, v, table, lengths, prefix_pages=torch.tensor(common, dtype=torch.int32).cuda()).cpu()
+    for seq in (0, 5, 7):
+        keys, values, there = _keys(b, seq, prefix + own[seq], common)
+        for h in range(0, 1024, 301):  # (of four kv heads)
+            _check_with_odd_values(out[seq, h : h + 1], q[seq, h : h + 1], keys[h // 128 : h // 128 + 1], values[h // 128 : h // 128 + 1], there, dim**-0.5, dtype, (seq, h))
