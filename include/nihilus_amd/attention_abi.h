@@ -79,7 +79,8 @@ int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* ho
  * reads kv head h / (q_heads / kv_heads).  q_heads is a multiple of kv_heads.  starts must not be NULL.  out has no gaps and no byte in
  * common with q (NH_ERR_ARGUMENT).
  * type NH_F32: q and the softmax weights go through the 16-bit matrix instructions as sums of two (fp16 cache) or three (bf16) terms,
- * 22 or 24 bits; type = the cache's: q as it is, the weights rounded once.  Everything else (products' sums, maxima, sums) is fp32.
+ * 22 or 24 bits; type = the cache's: q as it is, the weights as two terms where rows are few and rounded once where they are many (a second term
+ * would be half as much matrix work again; kernel 2 of nh_attn_debug_prompt_kernel, and a prefix that a decode step goes over apart).  Everything else (products' sums, maxima, sums) is fp32.
  * Memory: nh_attn_prompt_needs says how many bytes (0: many rows need none, and the pointers may be NULL), 256-byte aligned. */
 int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes);
 int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, void* out, int type, int64_t rows, int64_t q_heads, int64_t q_stride, float scale,

@@ -3,6 +3,8 @@ another device, batches of nobody, peaked scores across the pieces of a row's ke
 import pytest
 import torch
 
+import attention_reference as R
+
 from test_gpu_attention import A, BF16, F16, F32, INF, KINDS, NAN, Batch, _check, _check_prompt, _check_with_odd_values, _starts, kernel  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -201,3 +203,27 @@ def test_pieces_of_a_prefix_past_a_thousand_keys(A, dtype, cache, dim, page):  #
         keys, values, there = _keys(b, seq, prefix + own[seq], common)
         for h in range(0, 1024, 301):  # (of four kv heads)
             _check_with_odd_values(out[seq, h : h + 1], q[seq, h : h + 1], keys[h // 128 : h // 128 + 1], values[h // 128 : h // 128 + 1], there, dim**-0.5, dtype, (seq, h))
+
+
+@pytest.mark.parametrize("cache", [F16, BF16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_few_rows_of_16_bits_lose_nothing_but_their_own_rounding(A, cache, dim, page):  # noqa: F811
+    # Weights in two terms of 8 (11) bits and rounding to nearest: off by 2^-18 (2^-22) at most, beside the errors of attention_reference.py for fp32 rows
+    lengths = [700, 90, 33, 260]
+    b = Batch(71, lengths, page, 2, dim, cache)
+    q = b.rows(8, 8, cache)
+    k, v, table, dl = b.device()
+    one, several = A.attention_decode(q[:4].cuda(), k, v, table, dl).cpu(), A.attention_prompt(q.cuda(), k, v, table, dl, torch.tensor([0, 2, 4, 6, 8], dtype=torch.int32).cuda()).cpu()
+
+    def check(got, row, seq, seen):
+        keys, values, there = b.keys(seq, seen)
+        ref, mean, d, n = R.attend(row, keys, values, there, dim**-0.5)
+        inner = mean * (2 * (torch.expm1(d)[:, None] + 4 * R.U + 2.0**-18) + (2 * n + 12) * R.U)
+        most = inner + R.half_step(cache) * (ref.abs() + inner) + R.tiny(cache)
+        off = (got.double() - ref).abs()
+        assert bool((off <= most).all()), (seq, seen, float((off / most).max()))
+
+    for s, n in enumerate(lengths):
+        check(one[s], q[s], s, n)
+        check(several[2 * s], q[2 * s], s, n - 1)
+        check(several[2 * s + 1], q[2 * s + 1], s, n)
