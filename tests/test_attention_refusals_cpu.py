@@ -145,3 +145,16 @@ def test_more_table_entries_than_a_step_can_count():
     assert _compact(batch=batch, table=1 << 43) == -5
     if not torch.cuda.is_available():
         assert _fits(_step(batch=_batch(page_table=1 << 40, lengths=1 << 39, sequences=sequences, table_width=width), children=sequences - 1, parents=1 << 41, grow=1 << 42, table=1 << 43, lengths=1 << 44, ws=1 << 45))
+
+
+def test_the_customisation_points_as_calls_of_this_abi_compile():
+    import os
+    import subprocess
+
+    from nihilus_amd.build import hipcc
+    from test_attention_cpu import ROOT
+
+    cxx = os.path.join(os.path.dirname(hipcc()), "amdclang++")
+    src = os.path.join(ROOT, "tests", "cpp", "attention_customisation_points.cpp")
+    res = subprocess.run([cxx, "-std=c++23", "-Wall", "-Wextra", "-Werror", "-fsyntax-only", "-I", os.path.join(ROOT, "include"), src], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
