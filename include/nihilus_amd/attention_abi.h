@@ -77,11 +77,12 @@ int nh_attn_append_rope(const nh_attn_cache* host_cache, const nh_attn_batch* ho
 
 /* out[r] = sum_j softmax_j(scale q[r] . k_j) v_j over the keys j <= position of row r, for every row of every sequence; query head h
  * reads kv head h / (q_heads / kv_heads).  q_heads is a multiple of kv_heads.  starts must not be NULL.  out has no gaps and no byte in
- * common with q (NH_ERR_ARGUMENT).
+ * common with q (NH_ERR_ARGUMENT), nor with the cache or the tables (not checked).  Scores, scale q.k, are fp32: those above 2^23 have no bits behind the
+ * point, and results that hang on them may be anything, also infinite or NaN.
  * type NH_F32: q and the softmax weights go through the 16-bit matrix instructions as sums of two (fp16 cache) or three (bf16) terms,
  * 22 or 24 bits; type = the cache's: q as it is, the weights as two terms where rows are few and rounded once where they are many (a second term
  * would be half as much matrix work again; kernel 2 of nh_attn_debug_prompt_kernel, and a prefix that a decode step goes over apart).  Everything else (products' sums, maxima, sums) is fp32.
- * Memory: nh_attn_prompt_needs says how many bytes (0: many rows need none, and the pointers may be NULL), 256-byte aligned. */
+ * Memory: nh_attn_prompt_needs says how many bytes (0: many rows need none, and the pointers may be NULL; so fewer rows may need more), 256-byte aligned. */
 int nh_attn_prompt_needs(int64_t rows, int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t* host_workspace_bytes, int64_t* host_counter_bytes);
 int nh_attn_prompt(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const void* q, void* out, int type, int64_t rows, int64_t q_heads, int64_t q_stride, float scale,
 	void* workspace, int64_t workspace_bytes, void* counters, int64_t counter_bytes, void* stream);
@@ -94,7 +95,7 @@ int nh_attn_debug_prompt_kernel(int64_t rows, int64_t sequences, int64_t q_heads
 
 /* The same for one row per sequence over all of its keys (starts must be NULL, rows = sequences).  The keys j < prefix_count *
  * page_size of EVERY sequence (as far as its length goes) are those of the pages prefix_pages[0 .. prefix_count): they are read once for the
- * whole batch (where that is faster), and the first prefix_count entries of a page_table row are not looked at.  prefix_count = 0: none shared. */
+ * whole batch (where that is faster), and the first prefix_count entries of a page_table row are not looked at by this call.  prefix_count = 0: none shared. */
 int nh_attn_decode_needs(int64_t sequences, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_count, int64_t page_size, int64_t* host_workspace_bytes,
 	int64_t* host_counter_bytes);
 int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* prefix_pages, int64_t prefix_count, const void* q, void* out, int type, int64_t q_heads,
@@ -106,6 +107,7 @@ int nh_attn_decode(const nh_attn_cache* host_cache, const nh_attn_batch* host_ba
  *   - Pages that stay full are shared.  The page that a child will go on writing into must be its own: if several children hold it,
  *     the lowest of them keeps it (unless some child holds it as a full page) and the others get copies.
  *   - Pages that a child needs beyond its parent's are given to it; tokens in them are not written.
+ *   - Who holds a page is read from the tables alone: the pages of a shared prefix have to be named in a row that goes on, or they are free.
  *   Free pages are given in ascending order, to the children in theirs, to each its copy first; copies move keys and values of all layers.
  * new_table int32 [children][table_width] (entries past a child's last page are -1), new_lengths int32 [children]; these, info and the workspace have no byte in
  * common with each other, the inputs or the cache (NH_ERR_ARGUMENT).
@@ -117,7 +119,7 @@ int64_t nh_attn_pages_workspace_bytes(int64_t pages, int64_t sequences, int64_t 
 int nh_attn_cache_step(const nh_attn_cache* host_cache, const nh_attn_batch* host_batch, const int32_t* parents, const int32_t* grow, int64_t children, int32_t* new_table, int32_t* new_lengths,
 	int32_t* info, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* Moves the pages that hold the sequences' tokens to the front: with n pages in use, the k-th lowest used page >= n goes to the k-th lowest free
+/* Moves the pages that hold the sequences' tokens to the front (as the tables name them, those of a shared prefix too): with n pages in use, the k-th lowest used page >= n goes to the k-th lowest free
  * page < n, in all layers.  new_table int32 [sequences][table_width] names the pages where they are then (entries past a sequence's
  * last page, and those outside the cache, are -1); info int32 [3]: n, pages moved, entries that were outside the cache.  Pages that
  * were free keep what they held unless something moved there.  Workspace, and what may not lie over what, as above. */

@@ -188,8 +188,8 @@ def attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
                      scale: float | None = None, out: torch.Tensor | None = None, workspace: Workspace | None = None) -> torch.Tensor:
     """Attention of one row per sequence, q [sequences, q_heads, head_dim], over all of its keys.
 
-    prefix_pages, int32: pages whose keys every sequence begins with; they are read once for the whole batch, and that many entries at the front of
-    each page_table row are not looked at.  A sequence of no tokens gives zeros.  workspace: see decode_workspace; without one the call has its own."""
+    prefix_pages, int32: pages whose keys every sequence begins with; they are read once for the whole batch where that is faster, and that many entries at the front of
+    each page_table row are not looked at here (cache_step and cache_compact do: to them a page that no row names is free).  A sequence of no tokens gives zeros.  workspace: see decode_workspace; without one the call has its own."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if out is None and workspace is None and _calls is not None:
         r = _native(_calls.attention_decode(q, k_pages, v_pages, page_table, lengths, prefix_pages, scale), "nh_attn_decode")

@@ -82,8 +82,8 @@ std::atomic<int> forced_prompt_kernel{ 0 };
 
 // Whether a decode step's shared prefix is gone over once for all sequences, by the tile kernel, or by each with its own keys.  The first takes a launch more
 // and the join of its results, some 7 us and more with more sequences; the second reads the prefix from the caches once for each sequence.
-// us, apart | with their own (fp16, own keys 200; 32 / 8 heads of 128): prefix 1024: 8 sequences 16.0 | 11.8, 64 28.1 | 23.9;  4096: 8 19.6 | 15.8, 16 24.2 | 25.1,
-// 64 34.6 | 58.8;  8192: 4 23.0 | 16.6, 8 24.5 | 23.7, 16 27.1 | 39.2;  16 / 2 heads, 8192: 32 34.0 | 25.8, 64 30.5 | 39.2
+// us, apart | with their own (fp16, own keys 200; 32 / 8 heads of 128): prefix 1024: 8 sequences 16.3 | 12.3, 64 28.6 | 25.0;  4096: 8 19.9 | 16.9, 16 24.3 | 27.1,
+// 64 35.1 | 61.2;  8192: 4 23.6 | 17.2, 8 24.4 | 25.3, 16 27.0 | 42.2;  16 / 2 heads, 8192: 32 34.2 | 27.3, 64 30.5 | 42.0
 static bool prefix_apart(int64_t sequences, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys) {
 	if (const int forced = forced_prompt_kernel.load(std::memory_order_relaxed)) {
 		return forced == 2;
@@ -101,10 +101,10 @@ bool nh::prompt_by_rows(int64_t rows, int64_t sequences, int64_t q_heads, int64_
 	// The rows kernel reads a sequence's keys again for every 16 rows, but spreads any shape over the chip; the tile kernel reads them for every 128, and a
 	// workgroup's way to its first result is longer.  So: the first while its row groups are all on the chip at once, or where no tile has more than one.
 	// us, rows | tiles (fp16, 32 / 8 heads of 128 where nothing else is said):
-	//   256 row groups:  a prompt of 128 rows 7.2 | 12.6, behind 1024 keys 19 | 23, behind 8192 keys 63 | 40
-	//   512:             a prompt of 256 rows 8.8 | 14.6, behind 1024 keys 22 | 24, behind 8192 keys 109 | 54; 8 of 32 rows 7.0 | 11.6
-	//   1024:            a prompt of 512 rows 19.6 | 18.5, behind 1024 keys 41 | 28, behind 8192 keys 205 | 89; 16 / 2 heads of 64, 64 of 16 rows 9.3 | 8.5
-	//   2048:            8 prompts of 128 rows 22 | 12.5, 64 of 16 rows 19 | 12; but 32 / 32 heads, 64 of 16 rows, each tile with one row group: 21 | 33
+	//   256 row groups:  a prompt of 128 rows 7.0 | 12.8, behind 1024 keys 18 | 23, behind 8192 keys 68 | 40
+	//   512:             a prompt of 256 rows 8.7 | 14.3, behind 1024 keys 23 | 24, behind 8192 keys 120 | 55; 8 of 32 rows 6.8 | 11.6
+	//   1024:            a prompt of 512 rows 20.0 | 18.5, behind 1024 keys 44 | 28, behind 8192 keys 231 | 91; 16 / 2 heads of 64, 64 of 16 rows 8.7 | 8.4
+	//   2048:            8 prompts of 128 rows 21 | 15, 64 of 16 rows 19 | 11.5; but 32 / 32 heads, 64 of 16 rows, each tile with one row group: 21 | 34
 	// (How many keys there are is not known on the host: a table has room for more.)
 	const int64_t each = (rows + sequences - 1) / sequences * (q_heads / kv_heads); // the lengths are not known here: as if all were alike
 	const int64_t row_groups = sequences * kv_heads * ((each + 15) / 16), tiles = sequences * kv_heads * ((each + 127) / 128);

@@ -57,7 +57,7 @@ template<int CACHE, int N> __device__ __forceinline__ void split8(const float (&
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
-	return __builtin_amdgcn_exp2f(x); // v_exp_f32: 1 ulp; arguments here are <= 0, results below 2^-126 are flushed, far under a sum that holds a 1
+	return __builtin_amdgcn_exp2f(x); // v_exp_f32: 1 ulp; arguments here are below 16 (see weight_bias), results below 2^-126 are flushed, far under a sum that holds a 1
 }
 // What the sums of a part of the keys are multiplied with when parts are joined: 2^x, x how far (in powers of two) the part's maximum lies below the joint one.
 // Never zero: an infinite value has been added to its part by then and has to stay one (infinity times zero is NaN), and 2^-126 of a part shows nowhere
@@ -107,9 +107,13 @@ __device__ __forceinline__ int sequence_of_row(const int32_t* starts, int sequen
 	return lo > 0 && lo <= sequences ? lo - 1 : -1;
 }
 
-// Softmax weights are formed as 2^(t - m + bias), t = scale log2(e) q.k, m the row's running maximum of t: sums and products carry the
-// same factor, which the last division takes out.  fp16 weights then lie in (0, 2^8] and keep all their bits down to 2^-22 of the largest.
+// Softmax weights are formed as 2^(t - m + bias), t = scale log2(e) q.k, m what the row's weights are kept below: sums and products carry the same factor, which
+// the last division takes out.  In the rows kernel m is the running maximum of t: fp16 weights lie in (0, 2^8] and keep all their bits down to 2^-22 of the
+// largest.  In the tile kernel the maximum may have risen above m by up to `weight_rise` powers of two without being followed: fp16 weights lie in (0, 2^15].  (m is
+// an fp32 number: t - m is off by up to 2^-24 |m|, so what is said here holds for scores of up to 2^23.)
 template<int CACHE> constexpr float weight_bias = CACHE == NH_F16 ? 8.0f : 0.0f;
+constexpr float weight_rise = 7.0f;
+static_assert(weight_bias<NH_F16> + weight_rise < 16.0f, "a weight above 65504 is infinite in fp16");
 constexpr float LOG2_E = 1.44269504088896340736f;
 
 // Eight consecutive values of a q row as fp32 (all zero where there is no row).
@@ -231,7 +235,7 @@ prefix_cut plan_prefix(int64_t sequences, int64_t group, int64_t kv_heads, int64
 bool prefix_fits(const prefix_cut& cut, int64_t kv_heads); // one launch
 // partial results [piece][sequence][q_head]: o unnormalised, ml the running maximum (log2) and the sum of the weights
 hipError_t launch_attention_prefix(const attention_args& a, int cache_type, int type, const prefix_cut& cut, float* o, float2* ml, hipStream_t s);
-// The rows kernel (attention_rows.hip): 16 rows of a sequence at a time, keys and values straight from memory and cut into pieces.
+// The rows kernel (attention_rows.hip): 16 rows of a sequence at a time, each wave's keys and values through LDS of its own, long sequences in pieces.
 attention_needs attention_rows_needs(int64_t sequences, bool one_each, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t prefix_keys);
 // whether all work, in steps of 32 keys, surely has a 32-bit number (table_keys: what a sequence's table has room for)
 bool attention_rows_fit(int64_t rows, int64_t sequences, bool one_each, int64_t group, int64_t table_keys);

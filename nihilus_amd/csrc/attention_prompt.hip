@@ -15,9 +15,9 @@
 // Result rows 8 (i / 4) + 4 (l / 32) + i % 4 of a lane have to be keys 16 (i / 8) + 8 (l / 32) + i % 8, so operand row m takes key m with bits
 // 2 and 3 swapped.
 //
-// Bound by the matrix unit, and with that by power: a prompt of 8192 rows (64 query heads over 8 kv heads of 128, fp16) takes 1.10 ms, 1.0 PFLOP/s of visible pairs, with
-// the matrix unit busy 57 % of the time at a clock that falls to 1.77 GHz; the library's matrix product of 8192 x 8192 x 8192 reaches 1.15.  Seven ragged prompts of up
-// to 2048 rows behind up to 1500 cached keys, bf16: 114 us, 785 TFLOP/s; their diagonals and the last workgroups' ends are the rest.  The next tile's scores are
+// Bound by the matrix unit, and with that by power: a prompt of 8192 rows (64 query heads over 8 kv heads of 128, fp16) takes 1.13 to 1.16 ms, 0.95 to 0.97 PFLOP/s of visible pairs,
+// with the matrix unit busy 54 % of the time at a clock that falls to 1.77 GHz; the library's matrix product of 8192 x 8192 x 8192 reaches 1.15.  Seven ragged prompts of up
+// to 2048 rows behind up to 1500 cached keys, bf16: 117 us, 760 TFLOP/s; their diagonals and the last workgroups' ends are the rest.  The next tile's scores are
 // worked out beside this one's weights, so that both units have work (8192 rows: 1.31 ms without that and without the two buffers).
 //
 // Where the tiles are few, the keys are split: two groups of waves in a workgroup, each half of the keys (tile buffers of their own, joined in LDS), and then pieces
@@ -50,7 +50,7 @@ __device__ __forceinline__ int v_swizzle(int row) {
 
 // The weights of a row are formed below a maximum that is followed only when the scores rise above it by more than this (as a power of two): fp16
 // weights stay below 2^(8 + 7), and after a row's first tiles its results are hardly ever brought below a new one.
-constexpr float RISE = 7.0f;
+constexpr float RISE = weight_rise;
 
 // Results between workgroups: device scope, past the caches that another XCD does not see.
 __device__ __forceinline__ void put(float* p, float x) {
@@ -428,6 +428,8 @@ __global__ __launch_bounds__(64 * WAVES * PARTS, (terms<CACHE, TYPE>) == 3 && PA
 			if constexpr (AHEAD) {
 				scores(kt + 1, next); // (behind the last tile: of whatever is there, for nothing)
 			}
+			// (q of the cache's type: weights rounded once.  Results are off by as much again as their own rounding, bf16 2.3e-3 of their size instead of 1.7e-3, fp16 2.7e-4
+			// instead of 2.0e-4; two terms would double the second product: 8192 rows 1130 -> 1623 us, seven ragged prompts 117 -> 155.)
 			vec t[4][N];
 #pragma unroll
 			for (int g = 0; g < 4; ++g) {

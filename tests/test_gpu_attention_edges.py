@@ -227,3 +227,22 @@ def test_few_rows_of_16_bits_lose_nothing_but_their_own_rounding(A, cache, dim, 
         check(one[s], q[s], s, n)
         check(several[2 * s], q[2 * s], s, n - 1)
         check(several[2 * s + 1], q[2 * s + 1], s, n)
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+def test_scores_that_just_have_bits_behind_the_point(A, kernel, dtype, cache):  # noqa: F811
+    # One key far above the others, at 7e6 of a score: the row's weights are formed below a number of that size, in fp16 too. Its value comes out, off by the weight's
+    # rounding (half a step of 16 bits, 2^-20 in terms) and the result's own.
+    length, top, dim = 300, 170, 64
+    b = Batch(73, [length], 16, 1, dim, cache)
+    ahead = torch.sign(torch.randn(dim, generator=b.g))
+    b.k[b.table[0][top // 16], :, top % 16] = (4 * ahead).to(cache)
+    q = (4 * ahead + 0.25 * b.rows(4, 4, F32)).to(dtype)
+    k, v, table, dl = b.device()
+    scale = 7e6 / float((4 * ahead).double() @ (4 * ahead).double())
+    want = b.v[b.table[0][top // 16], :, :, top % 16].double().expand(4, dim)
+    most = want.abs() * (R.half_step(dtype) + 2.0**-20 + (R.half_step(cache) if dtype == cache else 0.0)) * 1.01
+    outs = A.attention_prompt(q.cuda(), k, v, table, dl, torch.tensor([0, 4], dtype=torch.int32).cuda(), scale=scale), A.attention_decode(q[:1].cuda(), k, v, table, dl, scale=scale)
+    for out in outs:
+        for row in out.cpu().double():
+            assert bool(((row - want).abs() <= most).all()), float(((row - want).abs() / most).max())
