@@ -24,8 +24,8 @@
  *   one).  Rows starts[b] .. starts[b + 1] - 1 of q (k, v, out) are the last tokens of sequence b, whose length counts them: row r stands
  *   at position lengths[b] - (starts[b + 1] - r).  Key j of a sequence is in page page_table[b][j / page_size] at j % page_size.
  *   Sequences of no rows and of no keys are allowed.  Rows in front of starts[0] and from starts[sequences] on belong to nobody: nothing is read or
- *   written for them.  starts must not descend (if they do, rows
- *   between the first and the last of them get any result or none, and nothing else is touched).
+ *   written for them.  starts must not descend: if they do, a row gets any result or none and may be written into any place of
+ *   the sequences' pages, but nothing else is touched.
  *   The tables are device memory and are not looked at before the launch, so what they hold is checked where it is used: a key whose
  *   page is not one of the cache's (an entry outside [0, pages), a position past the table) does not exist -- it is not written, and
  *   attention leaves it out; a row that has no key at all gives zeros.  What lies in the cache behind a sequence's last key is never

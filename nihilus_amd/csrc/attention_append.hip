@@ -10,7 +10,7 @@
 // Memory-bound.  A thread owns the same two pairs of every head that it touches, so their sines are worked out once per thread and row,
 // without a table and without a barrier.  Many rows: one workgroup per row; few rows: the heads of a row over several workgroups, for latency.
 // v is transposed inside its page, 64 rows at a time through LDS, so that consecutive lanes write consecutive tokens.
-// Measured: prompts of up to 3001 rows of 64 query heads over 8 kv heads of 128, fp32 to fp16, 552 MB, take 112 us, 4.9 TB/s, the rate of a large copy; one row 4.9 us with its call, the kernel 3.1, an empty launch 2.3.
+// Measured: prompts of up to 3001 rows of 64 query heads over 8 kv heads of 128, fp32 to fp16, 552 MB, take 112 us, 4.9 TB/s, the rate of a large copy; one row 4.9 us with its call, the kernel 3.1 to 3.3, an empty launch 2.3.
 #include "attention_device.h"
 
 namespace nh {
