@@ -202,7 +202,7 @@ def run(state):
     losses, lse = i8.token_losses(w, xq, s["targets"], n, k)
     if s["op"] == "loss":
         return {"losses": losses, "lse": lse}
-    return {"losses": losses, "lse": lse, "dx": i8.token_losses_grad(w, xq, s["targets"], lse, n, k, grad=s["grad"], dtype=s["x"].dtype)}
+    return {"losses": losses, "lse": lse, "dx": i8.token_losses_grad(w, xq, s["targets"], losses, lse, n, k, grad=s["grad"], dtype=s["x"].dtype)}
 
 
 # ---- what a pass cannot do without ----------------------------------------------------------------------------------------------
