@@ -1,4 +1,4 @@
-"""ctypes binding of libnihilus_q8_hip.so, the C ABI declared in include/nihilus_amd/q8_0_abi.h and attention_abi.h.
+"""ctypes binding of libnihilus_q8_hip.so, the C ABI declared in include/nihilus_amd/q8_0_abi.h, attention_abi.h and i8_abi.h.
 
 There is no fallback: if the library is missing, loading raises, and every wrapper turns a non-zero
 status into ``Q8Error``.
@@ -90,6 +90,23 @@ ATTENTION_SIGNATURES = {
     "nh_attn_cache_compact": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 
+# the same of i8_abi.h
+I8_SIGNATURES = {
+    "nh_i8_tiled_bytes": (_i64, [_i64, _i64]),
+    "nh_i8_quantize": (_int, [_vp, _int, _i64, _vp, _i64, _i64, _vp]),
+    "nh_i8_rms_norm_quantize": (_int, [_vp, _int, _i64, _vp, C.c_float, _vp, _i64, _i64, _vp]),
+    "nh_i8_silu_mul_quantize": (_int, [_vp, _vp, _int, _i64, _i64, _vp, _i64, _i64, _vp]),
+    "nh_i8_tile": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
+    "nh_i8_untile": (_int, [_vp, _vp, _vp, _i64, _i64, _vp]),
+    "nh_i8_gemm": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
+    "nh_i8_mul_mat_workspace_bytes": (_i64, [_i64, _i64]),
+    "nh_i8_mul_mat": (_int, [_vp, _vp, _int, _i64, _vp, C.c_float, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "nh_i8_token_losses_workspace_bytes": (_i64, [_i64, _i64]),
+    "nh_i8_token_losses": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "nh_i8_token_losses_grad_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
+    "nh_i8_token_losses_grad": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp]),
+}
+
 
 class AttnCache(C.Structure):
     """nh_attn_cache"""
@@ -130,7 +147,7 @@ def lib() -> C.CDLL:
                 "there is no CPU fallback for this path"
             )
         handle = C.CDLL(LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **ATTENTION_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **ATTENTION_SIGNATURES, **I8_SIGNATURES}.items():
             fn = getattr(handle, name)  # AttributeError if the library does not export a declared symbol
             fn.restype, fn.argtypes = res, args
         _lib = handle

@@ -15,7 +15,8 @@ LIB_NAME = "libnihilus_q8_hip.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
 SOURCES = ["q8_0_abi.hip", "q8_0_quantize.hip", "q8_0_layout.hip", "q8_0_get_rows.hip", "q8_0_gemv.hip", "q8_0_gemv_rows.hip", "q8_0_gemv_rows_mfma.hip", "q8_0_gemv_group.hip", "q8_0_mul_mat_f32act.hip", "q8_0_ffn.hip", "q8_0_decode_layer.hip", "q8_0_gemm.hip", "q8_0_gemm_skinny.hip", "q8_0_gemm_rows.hip", "q8_0_profile.hip", "gguf_q8_0.cpp",
-           "attention_abi.hip", "attention_append.hip", "attention_prompt.hip", "attention_rows.hip", "attention_pages.hip"]
+           "attention_abi.hip", "attention_append.hip", "attention_prompt.hip", "attention_rows.hip", "attention_pages.hip",
+           "i8_abi.hip", "i8_quantize.hip", "i8_gemm.hip", "i8_loss.hip"]
 
 # -packed-fp32-ops off: v_pk_{add,mul,fma}_f32 are kept out of the generated code on purpose.
 # No -ffast-math: the quantizer needs IEEE divide, unfused multiply and round-half-even.
