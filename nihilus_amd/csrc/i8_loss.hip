@@ -32,7 +32,7 @@ struct i8_stretches {
 	const int32_t* targets;
 	int M, N;
 
-	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x) const {
+	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f*) const {
 		const int lane = threadIdx.x & 63;
 		if (n0 >= N) {
 			return;
@@ -110,25 +110,6 @@ __global__ __launch_bounds__(1024) void i8_join_stretches(const float2* parts, c
 	}
 }
 
-template<class EPI> void forward_product(const i8_matrix& w, const i8_matrix& x, int first_n, int n, const EPI& epi, hipStream_t stream) {
-	const int strips = (n + 15) / 16;
-	auto rows = [&](auto kernel, int fn, int fm) {
-		const int n_tiles = (strips + fn - 1) / fn, m_tiles = (x.strips + fm - 1) / fm;
-		kernel<<<i8_grid(n_tiles, m_tiles), 512, 0, stream>>>(w, x, first_n, n_tiles, m_tiles, epi);
-	};
-	if (x.rows <= 16) {
-		rows(i8_rows_product<2, 1, 4, 2, EPI>, 2, 1);
-	} else if (x.rows <= 64) {
-		rows(i8_rows_product<4, 4, 2, 2, EPI>, 4, 4);
-	} else {
-		const int n_tiles = (n + 255) / 256, m_tiles = (x.rows + 255) / 256;
-		i8_tile_product<2, 4, 8, 4><<<i8_grid(n_tiles, m_tiles), 512, 0, stream>>>(w, x, first_n, n_tiles, m_tiles, epi);
-	}
-}
-int stretch_of(int64_t m) { // logits in one, by the kernel above
-	return m <= 64 ? 32 : 128;
-}
-
 constexpr int64_t up(int64_t n, int64_t to) {
 	return (n + to - 1) / to * to;
 }
@@ -182,7 +163,7 @@ template<int TERMS> struct i8_slopes {
 	const float *losses, *lse, *maxima;
 	int M, N, first_n, blocks; // of 32 n in the piece
 
-	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x) const {
+	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f*) const {
 		static_assert(FN % 2 == 0);
 		const int lane = threadIdx.x & 63, block = (n0 - first_n) / 32;
 		const int f	   = scales_exponent(maxima);
@@ -388,7 +369,7 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 	for (int64_t first = 0; first < w.rows; first += plan.piece) {
 		const int64_t n = std::min<int64_t>(plan.piece, w.rows - first), blocks = (n + 31) / 32;
 		const i8_slopes<TERMS> epi{ slopes, g.targets, g.losses, g.lse, maxima, x.rows, w.rows, static_cast<int>(first), static_cast<int>(blocks) };
-		forward_product(w, x, static_cast<int>(first), static_cast<int>(n), epi, stream);
+		i8_launch_product<true>(i8_form_for(i8_strips(n), x.strips, w.steps), w, x, static_cast<int>(first), static_cast<int>(n), epi, stream);
 		i8_slope_product a{};
 		a.p = slopes, a.out = sums;
 		a.M = x.rows, a.columns = w.steps * I8_STEP, a.strips = x.strips, a.blocks = static_cast<int>(blocks), a.first_block = static_cast<int>(first / 32);
@@ -405,16 +386,18 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 
 } // namespace
 
+// (K is not known here: room for the shortest stretches)
 int64_t i8_losses_workspace(int64_t m, int64_t n) {
-	return up(m * 4, 256) + up((n + stretch_of(m) - 1) / stretch_of(m) * m * 8, 256);
+	return up(m * 4, 256) + up((n + 31) / 32 * m * 8, 256);
 }
 
 hipError_t launch_i8_losses(const i8_matrix& w, const i8_matrix& x, const i8_losses& l, hipStream_t stream) {
-	char* ws	   = static_cast<char*>(l.workspace);
-	float* hit	   = reinterpret_cast<float*>(ws);
-	float2* parts  = reinterpret_cast<float2*>(ws + up(static_cast<int64_t>(x.rows) * 4, 256));
-	const int each = stretch_of(x.rows);
-	forward_product(w, x, 0, w.rows, i8_stretches{ parts, hit, l.targets, x.rows, w.rows }, stream);
+	char* ws		   = static_cast<char*>(l.workspace);
+	float* hit		   = reinterpret_cast<float*>(ws);
+	float2* parts	   = reinterpret_cast<float2*>(ws + up(static_cast<int64_t>(x.rows) * 4, 256));
+	const i8_form form = i8_form_for(w.strips, x.strips, w.steps);
+	const int each	   = i8_stretch(form);
+	i8_launch_product<true>(form, w, x, 0, w.rows, i8_stretches{ parts, hit, l.targets, x.rows, w.rows }, stream);
 	i8_join_stretches<<<(x.rows + 15) / 16, 1024, 0, stream>>>(parts, hit, l.targets, l.losses, l.lse, x.rows, w.rows, (w.rows + each - 1) / each);
 	return hipGetLastError();
 }

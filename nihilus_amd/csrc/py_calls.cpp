@@ -1,6 +1,6 @@
 // The calls of a model step on several rows (mul_mat, gemm, gemm_residual, rms_norm_quantize, gate_up_silu) and those between its
-// projections (append_rope, attention_prompt, attention_decode, cache_step, cache_compact) as one native function each, for
-// nihilus_amd/q8_0.py and attention.py: the checks, the output's allocation, the current stream and the call through the C ABI.
+// projections (append_rope, attention_prompt, attention_decode, cache_step, cache_compact), and those on int8 matrices with a scale per row, as one native function each, for
+// nihilus_amd/q8_0.py, attention.py and i8.py: the checks, the output's allocation, the current stream and the call through the C ABI.
 //
 // What bounds a small projection is the host.  A launch costs it 2.4 us; the same call from Python through ctypes took 7.9 us ([1024 x 4096]
 // against one row): 1.3 us for the ctypes call itself, 1.5 us for each tensor that Python allocates, 2.4 us for checks, sizes and the
@@ -16,7 +16,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include "nihilus_amd/attention_abi.h"
+#include "nihilus_amd/i8_abi.h"
 
 #include <map>
 #include <utility>
@@ -431,12 +431,170 @@ PyObject* cache_compact(args& in) {
 	return first && THPVariable_Check(first) ? Py_BuildValue("NN", first, THPVariable_Wrap(info)) : first;
 }
 
+// ---- i8.py: layouts and meanings as in i8_abi.h ----
+
+// Rows of activations [rows, k] or [k] on the current GPU, the values of a row side by side.
+struct i8_activations {
+	const at::Tensor* t;
+	int64_t rows = 0, k = 0, stride = 0;
+	int type = -1;
+	bool good = false;
+
+	explicit i8_activations(args& in) : t(rows_tensor(in)) {
+		if (!t || t->dim() < 1 || t->dim() > 2 || (type = type_of(*t)) < 0 || t->device().index() != c10::hip::current_device()) {
+			return;
+		}
+		const bool one = t->dim() == 1;
+		rows = one ? 1 : t->size(0), k = t->size(one ? 0 : 1), stride = rows > 1 ? t->stride(0) : k;
+		good = (k <= 1 || t->stride(one ? 0 : 1) == 1) && stride >= k;
+	}
+	const void* data() const {
+		return t->const_data_ptr();
+	}
+};
+at::ScalarType scalar_of(int64_t type) {
+	return type == NH_F32 ? at::kFloat : type == NH_F16 ? at::kHalf : at::kBFloat16;
+}
+// fp32 or int32 of this many values, on x's GPU
+bool i8_vector(const at::Tensor* t, const at::Tensor& x, int64_t n) {
+	return t->dim() == 1 && t->size(0) == n && t->device() == x.device();
+}
+// w [n][k] and xq [m][k], tiled, on the current GPU (larger buffers than the matrices are taken, as by the Python way)
+bool i8_operands(const at::Tensor& w, const at::Tensor& xq, int64_t m, int64_t n, int64_t k) {
+	const int64_t w_bytes = nh_i8_tiled_bytes(n, k), x_bytes = nh_i8_tiled_bytes(m, k);
+	return w_bytes >= 0 && x_bytes >= 0 && w.numel() >= w_bytes && xq.numel() >= x_bytes && xq.device() == w.device() && w.device().index() == c10::hip::current_device();
+}
+
+// i8_quantize(x)
+PyObject* i8_quantize(args& in) {
+	const i8_activations x(in);
+	const int64_t size = x.good ? nh_i8_tiled_bytes(x.rows, x.k) : -1;
+	if (size < 0) {
+		return nullptr;
+	}
+	const at::Tensor out = at::empty({ size }, x.t->options().dtype(at::kByte));
+	void *op = out.mutable_data_ptr(), *s = stream();
+	return finish(out, [&, xp = x.data()] { return nh_i8_quantize(xp, x.type, x.stride, op, x.rows, x.k, s); });
+}
+
+// i8_rms_norm_quantize(x, norm_weight, eps)
+PyObject* i8_rms_norm_quantize(args& in) {
+	const i8_activations x(in);
+	const at::Tensor* norm = in.tensor(at::kFloat);
+	const float eps		   = in.number();
+	const int64_t size	   = in.good && x.good && i8_vector(norm, *x.t, x.k) ? nh_i8_tiled_bytes(x.rows, x.k) : -1;
+	if (size < 0) {
+		return nullptr;
+	}
+	const at::Tensor out = at::empty({ size }, x.t->options().dtype(at::kByte));
+	void *op = out.mutable_data_ptr(), *s = stream();
+	return finish(out, [&, xp = x.data(), np = floats(*norm)] { return nh_i8_rms_norm_quantize(xp, x.type, x.stride, np, eps, op, x.rows, x.k, s); });
+}
+
+// i8_silu_mul_quantize(gate, up)
+PyObject* i8_silu_mul_quantize(args& in) {
+	const i8_activations gate(in), up(in);
+	const bool same	   = gate.good && up.good && gate.type == up.type && gate.t->sizes() == up.t->sizes();
+	const int64_t size = same ? nh_i8_tiled_bytes(gate.rows, gate.k) : -1;
+	if (size < 0) {
+		return nullptr;
+	}
+	const at::Tensor out = at::empty({ size }, gate.t->options().dtype(at::kByte));
+	void *op = out.mutable_data_ptr(), *s = stream();
+	return finish(out, [&, gp = gate.data(), up_ = up.data()] { return nh_i8_silu_mul_quantize(gp, up_, gate.type, gate.stride, up.stride, op, gate.rows, gate.k, s); });
+}
+
+// i8_gemm(w, xq, m, n, k, type, residual or None)
+PyObject* i8_gemm(args& in) {
+	const at::Tensor *w = in.tensor(at::kByte), *xq = in.tensor(at::kByte);
+	const int64_t m = in.integer(), n = in.integer(), k = in.integer(), type = in.integer();
+	const at::Tensor* residual = in.good ? in.tensor_or_none(scalar_of(type)) : nullptr;
+	if (!in.good || !i8_operands(*w, *xq, m, n, k) || (residual && (residual->dim() != 2 || residual->size(0) != m || residual->size(1) != n || residual->device() != w->device()))) {
+		return nullptr;
+	}
+	const at::Tensor y = at::empty({ m, n }, w->options().dtype(scalar_of(type)));
+	const void *wp = w->const_data_ptr(), *xp = xq->const_data_ptr(), *rp = residual ? residual->const_data_ptr() : nullptr;
+	void *yp = y.mutable_data_ptr(), *s = stream();
+	return finish(y, [&] { return nh_i8_gemm(wp, xp, rp, yp, static_cast<int>(type), m, n, k, s); });
+}
+
+// i8_mul_mat(w, x, n, k, residual or None, norm_weight or None, eps)
+PyObject* i8_mul_mat(args& in) {
+	const at::Tensor* w = in.tensor(at::kByte);
+	const i8_activations x(in);
+	const int64_t n = in.integer(), k = in.integer();
+	if (!in.good || !x.good || x.k != k || w->device() != x.t->device()) {
+		return nullptr;
+	}
+	const at::Tensor *residual = in.tensor_or_none(x.t->scalar_type()), *norm = in.tensor_or_none(at::kFloat);
+	const float eps			   = in.number();
+	const int64_t bytes = nh_i8_tiled_bytes(n, k), need = nh_i8_mul_mat_workspace_bytes(x.rows, k);
+	if (!in.good || bytes < 0 || w->numel() < bytes || need < 0 || (norm && !i8_vector(norm, *x.t, k)) ||
+		(residual && (residual->dim() != 2 || residual->size(0) != x.rows || residual->size(1) != n || residual->device() != w->device()))) {
+		return nullptr;
+	}
+	void* s = stream();
+	if (need > 0 && !own_memory(s)) {
+		return nullptr;
+	}
+	const at::Tensor y = at::empty({ x.rows, n }, x.t->options()), workspace = need > 0 ? bytes_like(*w, need) : at::Tensor();
+	const void *wp = w->const_data_ptr(), *xp = x.data(), *rp = residual ? residual->const_data_ptr() : nullptr;
+	const float* np = norm ? floats(*norm) : nullptr;
+	void *yp = y.mutable_data_ptr(), *ws = need > 0 ? workspace.mutable_data_ptr() : nullptr;
+	return finish(y, [&] { return nh_i8_mul_mat(wp, xp, x.type, x.stride, np, eps, rp, yp, x.rows, n, k, ws, need, s); });
+}
+
+// i8_token_losses(w, xq, targets, n, k): (losses, lse)
+PyObject* i8_token_losses(args& in) {
+	const at::Tensor *w = in.tensor(at::kByte), *xq = in.tensor(at::kByte), *targets = in.tensor(at::kInt);
+	const int64_t n = in.integer(), k = in.integer();
+	if (!in.good || targets->dim() != 1 || targets->device() != w->device()) {
+		return nullptr;
+	}
+	const int64_t m = targets->size(0), need = nh_i8_token_losses_workspace_bytes(m, n);
+	void* s = stream();
+	if (need < 0 || !i8_operands(*w, *xq, m, n, k) || (need > 0 && !own_memory(s))) {
+		return nullptr;
+	}
+	const at::Tensor losses = at::empty({ m }, w->options().dtype(at::kFloat)), lse = at::empty({ m }, w->options().dtype(at::kFloat)), workspace = bytes_like(*w, need);
+	const void *wp = w->const_data_ptr(), *xp = xq->const_data_ptr();
+	const int32_t* tp = static_cast<const int32_t*>(targets->const_data_ptr());
+	float *lp = static_cast<float*>(losses.mutable_data_ptr()), *ep = static_cast<float*>(lse.mutable_data_ptr());
+	void* ws		= workspace.mutable_data_ptr();
+	PyObject* first = finish(losses, [&] { return nh_i8_token_losses(wp, xp, tp, lp, ep, m, n, k, ws, need, s); });
+	return first && THPVariable_Check(first) ? Py_BuildValue("NN", first, THPVariable_Wrap(lse)) : first;
+}
+
+// i8_token_losses_grad(w, xq, targets, losses, lse, n, k, grad or None, type)
+PyObject* i8_token_losses_grad(args& in) {
+	const at::Tensor *w = in.tensor(at::kByte), *xq = in.tensor(at::kByte), *targets = in.tensor(at::kInt), *losses = in.tensor(at::kFloat), *lse = in.tensor(at::kFloat);
+	const int64_t n = in.integer(), k = in.integer();
+	const at::Tensor* grad = in.tensor_or_none(at::kFloat);
+	const int64_t type	   = in.integer();
+	if (!in.good || targets->dim() != 1 || targets->device() != w->device()) {
+		return nullptr;
+	}
+	const int64_t m = targets->size(0), need = nh_i8_token_losses_grad_workspace_bytes(m, n, k, static_cast<int>(type));
+	void* s = stream();
+	if (need < 0 || !i8_operands(*w, *xq, m, n, k) || !i8_vector(losses, *w, m) || !i8_vector(lse, *w, m) || (grad && !i8_vector(grad, *w, m)) || (need > 0 && !own_memory(s))) {
+		return nullptr;
+	}
+	const at::Tensor dx = at::empty({ m, k }, w->options().dtype(scalar_of(type))), workspace = bytes_like(*w, need);
+	const void *wp = w->const_data_ptr(), *xp = xq->const_data_ptr();
+	const int32_t* tp = static_cast<const int32_t*>(targets->const_data_ptr());
+	const float *lp = floats(*losses), *ep = floats(*lse), *gp = grad ? floats(*grad) : nullptr;
+	void *dp = dx.mutable_data_ptr(), *ws = workspace.mutable_data_ptr();
+	return finish(dx, [&] { return nh_i8_token_losses_grad(wp, xp, tp, lp, ep, gp, dp, static_cast<int>(type), m, n, k, ws, need, s); });
+}
+
 template<PyObject* (*F)(args&), int WANT> constexpr PyMethodDef method(const char* name) {
 	return { name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<F, WANT>)), METH_FASTCALL, nullptr };
 }
 PyMethodDef methods[] = { method<mul_mat, 5>("mul_mat"), method<gemm, 6>("gemm"), method<rms_norm_quantize, 3>("rms_norm_quantize"), method<gate_up_silu, 6>("gate_up_silu"),
 	method<append_rope, 10>("append_rope"), method<attention_prompt, 7>("attention_prompt"), method<attention_decode, 7>("attention_decode"), method<cache_step, 6>("cache_step"),
-	method<cache_compact, 4>("cache_compact"),
+	method<cache_compact, 4>("cache_compact"), method<i8_quantize, 1>("i8_quantize"), method<i8_rms_norm_quantize, 3>("i8_rms_norm_quantize"),
+	method<i8_silu_mul_quantize, 2>("i8_silu_mul_quantize"), method<i8_gemm, 7>("i8_gemm"), method<i8_mul_mat, 7>("i8_mul_mat"), method<i8_token_losses, 5>("i8_token_losses"),
+	method<i8_token_losses_grad, 9>("i8_token_losses_grad"),
 	{ nullptr, nullptr, 0, nullptr } };
 PyModuleDef module = { PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr };
 

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from .attention import _TYPES, _call, _own_memory
-from .q8_0 import _holds
+from .q8_0 import _calls, _holds, _native
 
 
 def tiled_bytes(rows: int, k: int) -> int:
@@ -72,6 +72,10 @@ def _workspace(workspace: torch.Tensor | None, n: int, device: torch.device) -> 
 
 def quantize(x: torch.Tensor) -> torch.Tensor:
     """x [rows, k] (or [k]) of fp32, fp16 or bf16, rows apart by any stride -> a tiled matrix with a scale of max |x| / 127 for each row."""
+    if _calls is not None:
+        r = _native(_calls.i8_quantize(x), "nh_i8_quantize")
+        if r is not None:
+            return r
     x, stride = _x(x, "x")
     out = _bytes(tiled_bytes(*x.shape), x.device)
     _call("nh_i8_quantize", x.device, x.data_ptr(), _TYPES[x.dtype], stride, out.data_ptr(), *x.shape)
@@ -80,6 +84,10 @@ def quantize(x: torch.Tensor) -> torch.Tensor:
 
 def rms_norm_quantize(x: torch.Tensor, norm_weight: torch.Tensor, eps: float) -> torch.Tensor:
     """quantize((x * 1/rms(x)) * norm_weight), one kernel; norm_weight fp32 [k]."""
+    if _calls is not None:
+        r = _native(_calls.i8_rms_norm_quantize(x, norm_weight, eps), "nh_i8_rms_norm_quantize")
+        if r is not None:
+            return r
     x, stride = _x(x, "x")
     _plain(norm_weight, torch.float32, x.device, x.shape[1:], "norm_weight")
     out = _bytes(tiled_bytes(*x.shape), x.device)
@@ -89,6 +97,10 @@ def rms_norm_quantize(x: torch.Tensor, norm_weight: torch.Tensor, eps: float) ->
 
 def silu_mul_quantize(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """quantize(silu(gate) * up), one kernel."""
+    if _calls is not None:
+        r = _native(_calls.i8_silu_mul_quantize(gate, up), "nh_i8_silu_mul_quantize")
+        if r is not None:
+            return r
     (gate, gate_stride), (up, up_stride) = _x(gate, "gate"), _x(up, "up")
     if gate.dtype != up.dtype or gate.device != up.device:
         raise TypeError("gate and up must be of the same type, on the same GPU")
@@ -131,6 +143,10 @@ def _gemm(w, xq, m, n, k, kind, residual, out):
 
 def gemm(w: torch.Tensor, xq: torch.Tensor, m: int, n: int, k: int, dtype: torch.dtype = torch.float32, residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Tiled activations [m, k] x tiled weight [n, k] (+ residual [m, n]) -> [m, n] of `dtype` (out may be the residual tensor itself: in-place accumulate)."""
+    if out is None and _calls is not None:
+        r = _native(_calls.i8_gemm(w, xq, m, n, k, _TYPES.get(dtype), residual), "nh_i8_gemm")
+        if r is not None:
+            return r
     if not w.is_cuda or dtype not in _TYPES:
         raise TypeError("w must be a uint8 tensor on the GPU, dtype float32, float16 or bfloat16")
     _tiled(w, w.device, n, k, "w")
@@ -145,6 +161,10 @@ def mul_mat(w: torch.Tensor, x: torch.Tensor, n: int, k: int, residual: torch.Te
     """Activations [m, k] (or [k]) x tiled weight [n, k] -> [m, n] of x's type: quantize (behind the RMS norm, with norm_weight), product, + residual [m, n] if given.
 
     workspace: nh_i8_mul_mat_workspace_bytes(m, k) bytes; without one the call has its own."""
+    if out is None and workspace is None and _calls is not None:
+        r = _native(_calls.i8_mul_mat(w, x, n, k, residual, norm_weight, eps), "nh_i8_mul_mat")
+        if r is not None:
+            return r
     x, stride = _x(x, "x")
     m = x.shape[0]
     if x.shape[1] != k:
@@ -164,6 +184,10 @@ def token_losses(w: torch.Tensor, xq: torch.Tensor, targets: torch.Tensor, n: in
     scored: their loss is 0.  lse is the log of the sum of the exponentials; the log-probability of a row's target is -loss.
 
     workspace: nh_i8_token_losses_workspace_bytes(m, n) bytes; without one the call has its own."""
+    if workspace is None and _calls is not None:
+        r = _native(_calls.i8_token_losses(w, xq, targets, n, k), "nh_i8_token_losses")
+        if r is not None:
+            return r
     if not w.is_cuda:
         raise TypeError("w must be a uint8 tensor on the GPU")
     m = targets.numel()
@@ -181,6 +205,10 @@ def token_losses_grad(w: torch.Tensor, xq: torch.Tensor, targets: torch.Tensor, 
     """The gradient of (grad * losses).sum() with respect to the rows that xq stands for, [m, k] of `dtype`; losses and lse as token_losses gave them, grad fp32 [m] (ones if not given).
 
     A quantizer in front passes it on as it is (straight through).  workspace: nh_i8_token_losses_grad_workspace_bytes(m, n, k, type) bytes; without one the call has its own."""
+    if workspace is None and _calls is not None:
+        r = _native(_calls.i8_token_losses_grad(w, xq, targets, losses, lse, n, k, grad, _TYPES.get(dtype)), "nh_i8_token_losses_grad")
+        if r is not None:
+            return r
     if not w.is_cuda or dtype not in _TYPES:
         raise TypeError("w must be a uint8 tensor on the GPU, dtype float32, float16 or bfloat16")
     m = targets.numel()
