@@ -13,6 +13,7 @@
 #include "i8_product.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace nh {
 
@@ -79,31 +80,43 @@ struct i8_stretches {
 	}
 };
 
-// 16 rows to a workgroup, 64 threads to a row
-__global__ __launch_bounds__(1024) void i8_join_stretches(const float2* parts, const float* hit, const int32_t* targets, float* losses, float* lse, int M, int N, int count) {
-	__shared__ float2 all[64][16];
-	const int col = threadIdx.x & 15, lane = threadIdx.x >> 4, m = blockIdx.x * 16 + col;
-	float top = -__builtin_inff(), sum = 0.0f;
+// ROWS rows to a workgroup, neighbouring threads have neighbouring rows
+template<int ROWS> __global__ __launch_bounds__(1024) void i8_join_stretches(const float2* parts, const float* hit, const int32_t* targets, float* losses, float* lse, int M, int N, int count) {
+	constexpr int LANES = 1024 / ROWS, AT_ONCE = 4;
+	__shared__ float2 all[LANES][ROWS];
+	const int col = threadIdx.x % ROWS, lane = threadIdx.x / ROWS, m = blockIdx.x * ROWS + col;
+	const float none = -__builtin_inff();
+	float top = none, sum = 0.0f;
+	// (a stretch whose logits are all NaN has -infinity and NaN: equal maxima are not subtracted)
+	auto add = [&](float2 p) {
+		const float now = fmaxf(top, p.x);
+		sum				= (top == now ? sum : sum * exp2_native((top - now) * LOG2_E)) + (p.x == now ? p.y : p.y * exp2_native((p.x - now) * LOG2_E));
+		top				= now;
+	};
 	if (m < M) {
-		for (int i = lane; i < count; i += 64) {
-			const float2 p	= parts[static_cast<int64_t>(i) * M + m];
-			const float now = fmaxf(top, p.x);
-			// (a stretch whose logits are all NaN has -infinity and NaN)
-			sum = (top == now ? sum : sum * exp2_native((top - now) * LOG2_E)) + (p.x == now ? p.y : p.y * exp2_native((p.x - now) * LOG2_E));
-			top = now;
+		for (int i = lane; i < count; i += LANES * AT_ONCE) {
+			float2 p[AT_ONCE];
+#pragma unroll
+			for (int j = 0; j < AT_ONCE; ++j) {
+				p[j] = i + LANES * j < count ? parts[static_cast<int64_t>(i + LANES * j) * M + m] : make_float2(none, 0.0f);
+			}
+#pragma unroll
+			for (int j = 0; j < AT_ONCE; ++j) {
+				add(p[j]);
+			}
 		}
 	}
-	all[lane][col] = make_float2(top, sum);
-	__syncthreads();
-	if (threadIdx.x < 16 && m < M) {
-		for (int i = 0; i < 64; ++i) {
-			top = fmaxf(top, all[i][col].x);
+	for (int d = LANES / 2; d > 0; d >>= 1) {
+		if (lane < 2 * d) {
+			all[lane][col] = make_float2(top, sum);
 		}
-		sum = 0.0f;
-		for (int i = 0; i < 64; ++i) {
-			const float2 p = all[i][col];
-			sum += p.x == top ? p.y : p.y * exp2_native((p.x - top) * LOG2_E);
+		__syncthreads();
+		if (lane < d) {
+			add(all[lane + d][col]);
 		}
+		__syncthreads();
+	}
+	if (lane == 0 && m < M) {
 		const float l = top + logf(sum);
 		lse[m]		  = l;
 		losses[m]	  = targets[m] >= 0 && targets[m] < N ? l - hit[m] : 0.0f;
@@ -208,17 +221,19 @@ template<int TERMS> struct i8_slopes {
 	}
 };
 
-// Eight rows n (of 32, two fragments of 16 x 64 beside each other in LDS) of column k as fp16, for the lane's place in the A operand of v_mfma_f32_16x16x32_f16: columns 16 c + lane % 16 of the
+// Eight rows n (of 32, two fragments of 16 x 64 beside each other in LDS) of a column k, for the lane's place in the A operand of v_mfma_f32_16x16x32_f16: columns 16 c + lane % 16 of the
 // fragments, rows 4 (lane / 16) + i of the first and of the second.  In a group of sixteen lanes lane 2 j + h names row j, columns 8 h .. 8 h + 7 of sixteen, and lane L gets column L of all eight rows.
 typedef int v2i __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ v8h i8_columns(const v4u* first, const v4u* second, int c, int lane) {
+__device__ __forceinline__ v2i i8_columns(const v4u* first, const v4u* second, int c, int lane) {
 	const int j = (lane & 15) >> 1, row = 4 * (lane >> 4) + (j & 3);
 	const char* at = reinterpret_cast<const char*>(j < 4 ? first : second) + (c * 16 + row) * 16 + 8 * (lane & 1);
-	const v2i raw  = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(const_cast<char*>(at)));
+	return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(const_cast<char*>(at)));
+}
+// ... as fp16: 128 + q as the low byte of 0x6400 + ... is the fp16 number 1024 + 128 + q
+__device__ __forceinline__ v8h i8_halves(v2i raw) {
 	v8h out;
 #pragma unroll
 	for (int d = 0; d < 2; ++d) {
-		// 128 + q as the low byte of 0x6400 + ... is the fp16 number 1024 + 128 + q
 		const uint32_t u = static_cast<uint32_t>(raw[d]) ^ 0x80808080u;
 		const v2h low = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)), high = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
 		const v2h a = low - static_cast<_Float16>(1152.0f), b = high - static_cast<_Float16>(1152.0f);
@@ -235,83 +250,156 @@ struct i8_slope_product {
 	bool add;
 };
 
-// A workgroup has 16 WK FK columns x 16 WM FM rows of sums over its split's blocks of 32 n, in a ring as the product kernel for many rows.
-template<int WK, int WM, int FK, int FM, int TERMS, int RING> __global__ __launch_bounds__(64 * WK * WM, 2) void i8_slope_kernel(i8_matrix w, i8_slope_product a, int k_tiles, int m_tiles) {
-	constexpr int WAVES = WK * WM, STEPS = WK * FK / 4, NF = 2 * STEPS, FRAGMENTS = NF + WM * FM * TERMS, LOADS = (FRAGMENTS + WAVES - 1) / WAVES;
-	static_assert(WK * FK % 4 == 0);
+// A workgroup has 512 columns x 16 FM rows of sums over its split's blocks of 32 n, a wave 64 of the columns, so that each piece of w is made fp16 by one wave only.  Blocks come through a
+// ring in LDS as in i8_tile_product, and w's pieces of the next block are read and converted among the products of this one.
+template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_kernel(i8_matrix w, i8_slope_product a, int k_tiles, int m_tiles) {
+	constexpr int WAVES = 8, FK = 4, STEPS = WAVES, NF = 2 * STEPS, FRAGMENTS = NF + FM * TERMS, LOADS = FRAGMENTS / WAVES, MORE = FRAGMENTS % WAVES, RING = 4;
+	// P of the next block in registers too, where there is room for it
+	constexpr bool AHEAD = FM * TERMS <= 8;
 	__shared__ v4u ring[RING][FRAGMENTS][64];
 	const int split = blockIdx.y;
 	const i8_place p = i8_place_of(k_tiles, m_tiles);
 	if (!p.there) {
 		return;
 	}
-	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wk = wave % WK, wm = wave / WK;
-	const int step0 = p.n * STEPS, strip0 = p.m * WM * FM;
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int step0 = p.n * STEPS, strip0 = p.m * FM;
 	const int begin = split * a.per, blocks = min(a.per, a.blocks - begin);
-	auto load = [&](int s) {
-		const int block = begin + s;
+	// this wave's fragments of a block: [two strips of w][step], then [strip of P][term]; the first MORE waves have one more
+	const bool more = wave < MORE;
+	const v4u* from[LOADS + 1];
+	int64_t onward[LOADS + 1]; // from a block to the next
+	int last[LOADS + 1]; // of a strip of w that there is
 #pragma unroll
-		for (int j = 0; j < LOADS; ++j) { // (past the last fragment: that one again, to the same place)
-			const int f = min(wave * LOADS + j, FRAGMENTS - 1);
-			const v4u* from;
-			if (f < NF) { // fragments [step][2]
-				from = w.q + (static_cast<int64_t>(min(2 * (a.first_block + block) + (f & 1), w.strips - 1)) * w.steps + min(step0 + (f >> 1), w.steps - 1)) * 64;
-			} else {
-				const int t = (f - NF) % TERMS, strip = min(strip0 + (f - NF) / TERMS, a.strips - 1);
-				from		= reinterpret_cast<const v4u*>(a.p) + ((static_cast<int64_t>(t) * a.strips + strip) * a.blocks + block) * 64;
+	for (int j = 0; j < LOADS + 1; ++j) {
+		const int f = j < LOADS ? wave + WAVES * j : WAVES * LOADS + min(wave, MORE - 1);
+		if (f < NF) {
+			// (the last block's second strip may not be there: one before it instead, which meets zeros)
+			const int strip = min(2 * (a.first_block + begin) + f / STEPS, w.strips - 1);
+			from[j]			= w.q + (static_cast<int64_t>(strip) * w.steps + min(step0 + f % STEPS, w.steps - 1)) * 64;
+			onward[j]		= static_cast<int64_t>(2) * w.steps * 64;
+			last[j]			= (w.strips - 1 - strip) >> 1;
+		} else {
+			const int t = (f - NF) % TERMS, strip = min(strip0 + (f - NF) / TERMS, a.strips - 1);
+			from[j]		= reinterpret_cast<const v4u*>(a.p) + ((static_cast<int64_t>(t) * a.strips + strip) * a.blocks + begin) * 64;
+			onward[j]	= 64;
+			last[j]		= a.blocks;
+		}
+	}
+	auto load = [&](int s) {
+#pragma unroll
+		for (int j = 0; j < LOADS + 1; ++j) {
+			if (j < LOADS || more) {
+				load_global_to_lds_b128(from[j] + min(s, last[j]) * onward[j], 16 * lane, &ring[s % RING][j < LOADS ? wave + WAVES * j : WAVES * LOADS + wave][0]);
 			}
-			load_global_to_lds_b128(from, 16 * lane, &ring[s % RING][f][0]);
 		}
 	};
-	auto arrive = [&](int s, int asked) { // step s is in LDS, steps below `asked` may be on their way
-		const int ahead = min(blocks, asked) - 1 - s;
-		if (ahead >= 2) {
-			i8_arrive<2 * LOADS>();
-		} else if (ahead == 1) {
-			i8_arrive<LOADS>();
+	auto arrive_by = [&](auto loads, int behind) { // a block is in LDS, those up to `behind` blocks after it may be on their way
+		constexpr int L = decltype(loads)::value;
+		if (behind >= 3) {
+			i8_arrive<3 * L>();
+		} else if (behind == 2) {
+			i8_arrive<2 * L>();
+		} else if (behind == 1) {
+			i8_arrive<L>();
 		} else {
 			i8_arrive<0>();
 		}
 	};
-	v4f sums[FK][FM] = {};
-	for (int s = 0; s < min(blocks, RING - 1); ++s) {
-		load(s);
-	}
-	for (int s = 0; s < blocks; ++s) {
-		arrive(s, s + RING - 1); // (and everybody has read the step before)
-		if (s + RING - 1 < blocks) {
-			load(s + RING - 1);
+	auto arrive = [&](int behind) {
+		if (MORE && more) {
+			arrive_by(std::integral_constant<int, LOADS + 1>{}, behind);
+		} else {
+			arrive_by(std::integral_constant<int, LOADS>{}, behind);
 		}
-		const auto& at = ring[s % RING];
-		v8h k[FK];
+	};
+	auto read_k = [&](int s, v2i(&raw)[FK]) {
 #pragma unroll
-		for (int f = 0; f < FK; ++f) {
-			const int c = wk * FK + f;
-			k[f]		= i8_columns(at[2 * (c >> 2)], at[2 * (c >> 2) + 1], c & 3, lane);
+		for (int c = 0; c < FK; ++c) {
+			raw[c] = i8_columns(ring[s % RING][wave], ring[s % RING][STEPS + wave], c, lane);
 		}
+	};
+	auto read_p = [&](int s, v8h(&d)[FM][TERMS]) {
+#pragma unroll
+		for (int i = 0; i < FM; ++i) {
+#pragma unroll
+			for (int t = 0; t < TERMS; ++t) {
+				d[i][t] = __builtin_bit_cast(v8h, ring[s % RING][NF + i * TERMS + t][lane]);
+			}
+		}
+	};
+	v4f sums[FK][FM] = {};
+	auto multiply	 = [&](const v8h(&k)[FK], const v8h(&d)[FM][TERMS]) {
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
 #pragma unroll
 			for (int t = TERMS - 1; t >= 0; --t) { // the small term first
-				const v8h d = __builtin_bit_cast(v8h, at[NF + (wm * FM + i) * TERMS + t][lane]);
 #pragma unroll
 				for (int f = 0; f < FK; ++f) {
-					sums[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[f], d, sums[f][i], 0, 0, 0);
+					sums[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[f], d[i][t], sums[f][i], 0, 0, 0);
+				}
+			}
+		}
+	};
+	v2i raw[FK];
+	v8h k[2][FK], d[2][FM][TERMS];
+	if (blocks > 0) {
+		// with AHEAD nobody reads block s any more once block s + 1 is there, and block s + RING takes its place; else that of block s - 1 is free
+		constexpr int ASKED = AHEAD ? RING : RING - 1;
+		for (int s = 0; s < min(blocks, ASKED); ++s) {
+			load(s);
+		}
+		arrive(min(blocks, ASKED) - 1);
+		read_k(0, raw);
+		if constexpr (AHEAD) {
+			read_p(0, d[0]);
+		}
+#pragma unroll
+		for (int f = 0; f < FK; ++f) {
+			k[0][f] = i8_halves(raw[f]);
+		}
+#pragma unroll 1
+		for (int s = 0; s < blocks; s += 2) {
+#pragma unroll
+			for (int h = 0; h < 2; ++h) {
+				if (s + h >= blocks) {
+					break;
+				}
+				const bool next = s + h + 1 < blocks;
+				if (next) {
+					arrive(min(blocks, s + h + ASKED) - 1 - (s + h + 1));
+					if (s + h + ASKED < blocks) {
+						load(s + h + ASKED);
+					}
+					read_k(s + h + 1, raw);
+					if constexpr (AHEAD) {
+						read_p(s + h + 1, d[1 - h]);
+					}
+				}
+				if constexpr (!AHEAD) {
+					read_p(s + h, d[h]);
+				}
+				multiply(k[h], d[h]);
+				if (next) {
+#pragma unroll
+					for (int f = 0; f < FK; ++f) {
+						k[1 - h][f] = i8_halves(raw[f]);
+					}
 				}
 			}
 		}
 	}
 #pragma unroll
 	for (int i = 0; i < FM; ++i) {
-		const int m = 16 * (strip0 + wm * FM + i) + (lane & 15);
+		const int m = 16 * (strip0 + i) + (lane & 15);
 		if (m >= a.M) {
 			continue;
 		}
 #pragma unroll
 		for (int f = 0; f < FK; ++f) {
-			const int k = 64 * step0 + 16 * (wk * FK + f) + 4 * (lane >> 4);
-			if (k < a.columns) {
-				v4f* to = reinterpret_cast<v4f*>(a.out + (static_cast<int64_t>(split) * a.M + m) * a.columns + k);
+			const int at = 64 * (step0 + wave) + 16 * f + 4 * (lane >> 4);
+			if (at < a.columns) {
+				v4f* to = reinterpret_cast<v4f*>(a.out + (static_cast<int64_t>(split) * a.M + m) * a.columns + at);
 				*to		= a.add ? *to + sums[f][i] : sums[f][i];
 			}
 		}
@@ -322,7 +410,7 @@ template<int WK, int WM, int FK, int FM, int TERMS, int RING> __global__ __launc
 template<int TYPE> __global__ __launch_bounds__(256) void i8_slope_results(const float* sums, const float* maxima, const int32_t* targets, const float* losses, const float* grad,
 	typename i8_type<TYPE>::store* dx, int M, int N, int K, int columns, int splits) {
 	const int f = scales_exponent(maxima);
-	const int m = blockIdx.y * gridDim.z + blockIdx.z, k = 4 * (blockIdx.x * 256 + threadIdx.x);
+	const int m = blockIdx.x * gridDim.y + blockIdx.y, k = 4 * (blockIdx.z * 256 + threadIdx.x);
 	if (m >= M || k >= K) {
 		return;
 	}
@@ -346,8 +434,7 @@ struct gradient_plan {
 	int64_t piece, blocks; // n, blocks of 32 n
 	int64_t k_tiles, m_tiles, splits;
 	int64_t slopes, sums; // bytes
-	bool many;
-	int terms;
+	int strips, terms; // strips of rows in a tile
 };
 gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k, int type) {
 	gradient_plan g{};
@@ -356,9 +443,9 @@ gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k, int type) {
 	const int64_t row	 = strips * 16 * 2 * g.terms;
 	g.piece				 = std::min(up(n, 32), std::max<int64_t>((int64_t{ 1 } << 27) / row / 256 * 256, 1024));
 	g.blocks			 = g.piece / 32;
-	g.many				 = m > 64;
-	g.k_tiles			 = (steps + 3) / 4;
-	g.m_tiles			 = g.many ? (m + 255) / 256 : (m + 63) / 64;
+	g.strips			 = m > 64 ? 8 : m > 16 ? 4 : 1;
+	g.k_tiles			 = (steps + 7) / 8;
+	g.m_tiles			 = (strips + g.strips - 1) / g.strips;
 	g.splits			 = std::max<int64_t>(1, std::min(g.blocks / 8, 256 / (g.k_tiles * g.m_tiles)));
 	g.slopes			 = up(row * g.piece, 256);
 	g.sums				 = up(g.splits * m * steps * I8_STEP * 4, 256);
@@ -376,10 +463,15 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 		a.per = static_cast<int>((blocks + plan.splits - 1) / plan.splits);
 		a.add = first > 0;
 		const dim3 grid(i8_grid(plan.k_tiles, plan.m_tiles), static_cast<unsigned>(plan.splits));
-		if (plan.many) {
-			i8_slope_kernel<4, 2, 4, 8, TERMS, TERMS == 1 ? 4 : 3><<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(plan.m_tiles));
+		auto multiply = [&](auto kernel) {
+			kernel<<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(plan.m_tiles));
+		};
+		if (plan.strips == 8) {
+			multiply(i8_slope_kernel<8, TERMS>);
+		} else if (plan.strips == 4) {
+			multiply(i8_slope_kernel<4, TERMS>);
 		} else {
-			i8_slope_kernel<4, 2, 4, 2, TERMS, 4><<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(plan.m_tiles));
+			multiply(i8_slope_kernel<1, TERMS>);
 		}
 	}
 }
@@ -398,7 +490,11 @@ hipError_t launch_i8_losses(const i8_matrix& w, const i8_matrix& x, const i8_los
 	const i8_form form = i8_form_for(w.strips, x.strips, w.steps);
 	const int each	   = i8_stretch(form);
 	i8_launch_product<true>(form, w, x, 0, w.rows, i8_stretches{ parts, hit, l.targets, x.rows, w.rows }, stream);
-	i8_join_stretches<<<(x.rows + 15) / 16, 1024, 0, stream>>>(parts, hit, l.targets, l.losses, l.lse, x.rows, w.rows, (w.rows + each - 1) / each);
+	if (x.rows <= 256) { // a workgroup to a row
+		i8_join_stretches<1><<<x.rows, 1024, 0, stream>>>(parts, hit, l.targets, l.losses, l.lse, x.rows, w.rows, (w.rows + each - 1) / each);
+	} else {
+		i8_join_stretches<8><<<(x.rows + 7) / 8, 1024, 0, stream>>>(parts, hit, l.targets, l.losses, l.lse, x.rows, w.rows, (w.rows + each - 1) / each);
+	}
 	return hipGetLastError();
 }
 
@@ -420,8 +516,8 @@ hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_g
 		gradient_sums<1>(w, x, g, plan, slopes, sums, maxima, stream);
 	}
 	const int columns = w.steps * I8_STEP;
-	const unsigned high = static_cast<unsigned>((x.rows + 63) / 64);
-	const dim3 grid(static_cast<unsigned>((g.k + 1023) / 1024), high, 64);
+	const unsigned beside = static_cast<unsigned>(std::min(x.rows, 64));
+	const dim3 grid((x.rows + beside - 1) / beside, beside, static_cast<unsigned>((g.k + 1023) / 1024));
 	auto results = [&](auto kernel, auto* dx) {
 		kernel<<<grid, 256, 0, stream>>>(sums, maxima, g.targets, g.losses, g.grad, dx, x.rows, w.rows, g.k, columns, static_cast<int>(plan.splits));
 	};

@@ -6,32 +6,27 @@
 // q = 0; a row with an infinity or NaN has s = NaN and q = 0, so that whatever is formed from it is NaN, and nothing else is.
 // v of a norm: fl32(fl32(x r) w), r = fl32(1 / sqrt(mean x^2 + eps)) with the mean in 64 bits, where the order of the sum does not show.
 //
-// Bound by memory.  A workgroup has four rows, 64 or 256 threads to a row, a thread sixteen values at a time (one 16-byte piece of a fragment), up to 64 of them kept in registers
-// between the passes that a row's maximum and a norm need; longer rows are read again, from the caches.  The four workgroups of a strip go to one XCD, whose L2 joins their
-// pieces to whole lines.
+// Bound by memory where rows are many, by the chain of a row's passes where they are few: a workgroup has one row or four, a thread sixteen values at a time (one 16-byte piece of a
+// fragment), up to 64 of them kept in registers between the passes that a row's maximum and a norm need; longer rows are read again, from the caches.  The workgroups of a strip go to one XCD,
+// whose L2 joins their pieces to whole lines.
 #include "i8_device.h"
 
 namespace nh {
 
 namespace {
 
-constexpr int ROWS = 4; // of a workgroup
 constexpr int HELD = 4; // pieces of sixteen values that a thread keeps
 
-template<int TYPE> __device__ __forceinline__ void load16(const void* base, int64_t at, int left, bool wide, float (&v)[16]) {
-	using T					  = i8_type<TYPE>;
-	const auto* p			  = static_cast<const typename T::store*>(base) + at;
-	constexpr int PER		  = 16 / sizeof(typename T::store);
-	if (wide && left >= 16) {
+// sixteen values; those from `left` on are zero (rows begin anywhere: the hardware takes any address)
+template<int TYPE> __device__ __forceinline__ void load16(const void* base, int64_t at, int left, float (&v)[16]) {
+	using T		  = i8_type<TYPE>;
+	const auto* p = static_cast<const typename T::store*>(base) + at;
+	if (left >= 16) {
+		typename T::store part[16];
+		__builtin_memcpy(part, p, sizeof(part));
 #pragma unroll
-		for (int i = 0; i < 16 / PER; ++i) {
-			typename T::store part[PER];
-			const v4u raw = *reinterpret_cast<const v4u*>(p + PER * i);
-			__builtin_memcpy(part, &raw, 16);
-#pragma unroll
-			for (int j = 0; j < PER; ++j) {
-				v[PER * i + j] = T::widen(part[j]);
-			}
+		for (int j = 0; j < 16; ++j) {
+			v[j] = T::widen(part[j]);
 		}
 		return;
 	}
@@ -41,43 +36,79 @@ template<int TYPE> __device__ __forceinline__ void load16(const void* base, int6
 	}
 }
 
-// The nearest whole number to v / s.  c is one of the two next to the quotient; v - c s is exact wherever it is close to half of s (a difference of multiples of the last place
-// of the smaller of v and s, below s), so comparing it with s / 2 decides between the two.
-__device__ __forceinline__ int nearest(float v, float s, float inverse) {
-	float c		  = rintf(v * inverse);
-	const float e = fmaf(-c, s, v), half = 0.5f * s;
-	if (fabsf(e) >= half && (fabsf(e) > half || (static_cast<int>(c) & 1))) {
-		c += copysignf(1.0f, e);
+// The whole numbers nearest to v / s as bytes, `inverse` being 1 / s to a unit in the last place.  c, the product with that rounded, is one of the two next to the quotient, and v - c s is
+// exact wherever it is close to half of s (a difference of multiples of the last place of the smaller of v and s, below s): comparing it with s / 2 decides between the two.  Where no
+// value of the wave's is that close, which is nearly always, c is right as it is.
+// (`doubt`: they may be past 127, which rows below the normal numbers reach, whose scale has few bits)
+__device__ __forceinline__ v4u nearest16(const float (&v)[16], float s, float inverse, bool doubt) {
+	constexpr float magic = 12582912.0f; // 1.5 * 2^23: the sum's low byte is the whole number
+	float c[16], far = 0.0f;
+#pragma unroll
+	for (int j = 0; j < 16; ++j) {
+		c[j] = fmaf(v[j], inverse, magic);
+		far	 = fmaxf(far, fabsf(fmaf(magic - c[j], s, v[j])));
 	}
-	return static_cast<int>(fminf(fmaxf(c, -127.0f), 127.0f));
+	if (doubt || far >= 0.5f * s) {
+#pragma unroll
+		for (int j = 0; j < 16; ++j) {
+			float n		  = c[j] - magic;
+			const float e = fmaf(-n, s, v[j]), half = 0.5f * s;
+			if (fabsf(e) >= half && (fabsf(e) > half || (static_cast<int>(n) & 1))) {
+				n += copysignf(1.0f, e);
+			}
+			c[j] = fminf(fmaxf(n, -127.0f), 127.0f) + magic;
+		}
+	}
+	v4u out;
+#pragma unroll
+	for (int d = 0; d < 4; ++d) { // (selector: 0..3 bytes of the second operand, 4..7 of the first)
+		const uint32_t low	= __builtin_amdgcn_perm(__float_as_uint(c[4 * d + 1]), __float_as_uint(c[4 * d]), 0x0c0c0400u);
+		const uint32_t high = __builtin_amdgcn_perm(__float_as_uint(c[4 * d + 3]), __float_as_uint(c[4 * d + 2]), 0x04000c0cu);
+		out[d]				= low | high;
+	}
+	return out;
 }
 
-template<int TYPE, int FRONT, int THREADS> __global__ __launch_bounds__(ROWS* THREADS) void i8_quantize_kernel(i8_rows in, v4u* q, float* scale, int steps, bool wide, bool wide_up) {
+// silu(g) u within 3 units in the last place: -g log2(e) in two parts, the exponential's one unit, a sum, a quotient by one correction step (so within half a unit and little more), a product.
+// Below g = -87 the exponential is held at 2^126: what is left is below 2^-119 of up.
+__device__ __forceinline__ float silu_times(float g, float u) {
+	constexpr float log2e = 1.44269502162933349609375f, log2e_rest = 1.925963033500011e-8f, ln2 = 0.693147182464599609375f;
+	const float t	 = -g * log2e;
+	const float rest = fmaf(-g, log2e, -t) - g * log2e_rest;
+	float e			 = __builtin_amdgcn_exp2f(fminf(t, 126.0f));
+	e				 = fmaf(e, rest * ln2, e);
+	const float d = 1.0f + (t > 126.0f ? 0x1p126f : e), r = __builtin_amdgcn_rcpf(d);
+	const float q = g * r;
+	return fmaf(fmaf(-q, d, g), r, q) * u;
+}
+
+template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds__(ROWS* THREADS) void i8_quantize_kernel(i8_rows in, v4u* q, float* scale, int steps) {
+	constexpr int PARTS = I8_ROWS / ROWS; // workgroups of a strip
 	constexpr int WAVES = THREADS / 64; // of a row
 	__shared__ double sums[ROWS][WAVES];
 	__shared__ uint32_t tops[ROWS][WAVES];
 	const int i	  = blockIdx.x >> 3;
-	const int row = ((i >> 2) * 8 + (blockIdx.x & 7)) * I8_ROWS + ROWS * (i & 3) + threadIdx.x / THREADS;
+	const int row = (i / PARTS * 8 + (blockIdx.x & 7)) * I8_ROWS + ROWS * (i % PARTS) + threadIdx.x / THREADS;
 	const int mine = threadIdx.x / THREADS, t = threadIdx.x % THREADS, wave = t >> 6;
 	const bool there = row < in.rows;
 	const int pieces = there ? 4 * steps : 0;
 	const int64_t at = static_cast<int64_t>(row) * in.stride, up_at = static_cast<int64_t>(row) * in.up_stride;
 	float r = 1.0f;
 	auto get = [&](int c, float(&v)[16]) { // without the norm
-		load16<TYPE>(in.x, at + 16 * c, in.k - 16 * c, wide, v);
+		load16<TYPE>(in.x, at + 16 * c, in.k - 16 * c, v);
 		if constexpr (FRONT == I8_SILU) {
 			float u[16];
-			load16<TYPE>(in.up, up_at + 16 * c, in.k - 16 * c, wide_up, u);
+			load16<TYPE>(in.up, up_at + 16 * c, in.k - 16 * c, u);
 #pragma unroll
 			for (int j = 0; j < 16; ++j) {
-				v[j] = silu_mul(v[j], u[j]);
+				v[j] = silu_times(v[j], u[j]);
 			}
 		}
 	};
 	auto normed = [&](int c, float(&v)[16]) {
 		if constexpr (FRONT == I8_NORM) {
 			float w[16];
-			load16<NH_F32>(in.norm, 16 * c, in.k - 16 * c, true, w);
+			load16<NH_F32>(in.norm, 16 * c, in.k - 16 * c, w);
 #pragma unroll
 			for (int j = 0; j < 16; ++j) {
 				v[j] = __fmul_rn(__fmul_rn(v[j], r), w[j]);
@@ -171,18 +202,15 @@ template<int TYPE, int FRONT, int THREADS> __global__ __launch_bounds__(ROWS* TH
 	const float step	= s * lift;
 	const bool nothing	= !finite || s == 0.0f;
 	const float inverse = nothing ? 0.0f : __builtin_amdgcn_rcpf(step);
-	auto put			= [&](int c, const float(&v)[16]) {
-		   v4u out;
+	auto put			= [&](int c, float(&v)[16]) {
+		   if (lift != 1.0f) {
 #pragma unroll
-		   for (int d = 0; d < 4; ++d) {
-			   uint32_t word = 0;
-#pragma unroll
-			   for (int j = 0; j < 4; ++j) {
-				   word |= (static_cast<uint32_t>(nearest(v[4 * d + j] * lift, step, inverse)) & 0xFFu) << (8 * j);
+			   for (int j = 0; j < 16; ++j) {
+				   v[j] *= lift;
 			   }
-			   out[d] = nothing ? 0u : word;
 		   }
-		   q[(static_cast<int64_t>(row >> 4) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = out;
+		   const v4u out = nearest16(v, step, inverse, lift != 1.0f);
+		   q[(static_cast<int64_t>(row >> 4) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = nothing ? v4u{} : out;
 	};
 #pragma unroll
 	for (int h = 0; h < HELD; ++h) {
@@ -243,13 +271,21 @@ __global__ __launch_bounds__(256) void i8_untile_kernel(const v4u* in, const flo
 }
 
 template<int TYPE, int FRONT> hipError_t quantize(const i8_rows& in, v4u* q, float* scale, int steps, hipStream_t stream) {
-	constexpr int64_t size = sizeof(typename i8_type<TYPE>::store);
-	auto apart			   = [&](const void* p, int64_t stride) {
-		return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride * size % 16 == 0;
+	const int64_t groups = (i8_strips(in.rows) + 7) / 8;
+	auto launch			 = [&](auto kernel, int rows, int threads) {
+		kernel<<<static_cast<unsigned>(groups * 8 * (I8_ROWS / rows)), rows * threads, 0, stream>>>(in, q, scale, steps);
 	};
-	const bool wide	 = apart(in.x, in.stride), wide_up = FRONT == I8_SILU && apart(in.up, in.up_stride);
-	const int blocks = static_cast<int>((i8_strips(in.rows) + 7) / 8) * 32;
-	i8_quantize_kernel<TYPE, FRONT, 256><<<blocks, ROWS * 256, 0, stream>>>(in, q, scale, steps, wide, wide_up);
+	if (in.rows <= 1024) {
+		if (steps <= 64) {
+			launch(i8_quantize_kernel<TYPE, FRONT, 1, 256>, 1, 256);
+		} else {
+			launch(i8_quantize_kernel<TYPE, FRONT, 1, 1024>, 1, 1024);
+		}
+	} else if (steps <= 64) {
+		launch(i8_quantize_kernel<TYPE, FRONT, 4, 64>, 4, 64);
+	} else {
+		launch(i8_quantize_kernel<TYPE, FRONT, 4, 256>, 4, 256);
+	}
 	return hipGetLastError();
 }
 template<int TYPE> hipError_t quantize(const i8_rows& in, int front, v4u* q, float* scale, int steps, hipStream_t stream) {

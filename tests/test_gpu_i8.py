@@ -113,6 +113,16 @@ def test_rows_of_nothing_of_borders_and_of_what_is_not_finite(i8):
     assert torch.equal(y[~bad], R.product(wq, ws, q[~bad], s[~bad], torch.float32))
 
 
+def test_rows_below_the_normal_numbers(i8):
+    # a scale of few bits: 190 units / 127 is one unit, and values past 127 of it are held there; a scale of none for rows below 64
+    units = torch.tensor([190, -190, 128, 127, 126, 64, 63, 1, -1, 0], dtype=torch.float64, device="cuda")
+    x = torch.stack([(units * u * 2.0**-149).float() for u in (1, 2, 3, 1000, 2**20, 2**24)] + [(units.clamp(-63, 63) * 2.0**-149).float()])
+    q, s = i8.untile(i8.quantize(x), *x.shape)
+    want_q, want_s = R.quantize(x.double())
+    assert torch.equal(s, want_s) and torch.equal(q, want_q)
+    assert q[0, 0] == 127 and q[0, 1] == -127 and s[0] > 0 and s[-1] == 0
+
+
 def test_quotients_next_to_halves(i8):
     # numbers around (n + 1/2) scales, one unit in the last place apart: the true quotient decides, not a rounded one
     g = _gen(11)
