@@ -34,41 +34,63 @@ struct i8_stretches {
 	int M, N;
 
 	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f*) const {
-		const int lane = threadIdx.x & 63;
+		const int lane = threadIdx.x & 63, group = lane >> 4;
 		if (n0 >= N) {
 			return;
+		}
+		const bool all = n0 + 16 * FN <= N;
+		v4f sw[FN];
+#pragma unroll
+		for (int f = 0; f < FN; ++f) {
+			sw[f] = i8_scales4(w, n0 + 16 * f + 4 * group);
 		}
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
 			const int m		 = m0 + 16 * i + (lane & 15);
 			const bool there = m < M;
 			const float sx	 = there ? x.scale[m] : 0.0f;
-			const int target = there ? targets[m] : -1;
-			float top		 = -__builtin_inff();
+			const int target = there ? targets[m] - n0 : -1; // in this stretch?
+			v4f l[FN];
+			float top = -__builtin_inff();
 #pragma unroll
 			for (int f = 0; f < FN; ++f) {
-				const int n	 = n0 + 16 * f + 4 * (lane >> 4);
-				const v4f sw = i8_scales4(w, n);
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
-					const float l = static_cast<float>(sums[f][i][e]) * sx * sw[e];
-					top			  = n + e < N ? fmaxf(top, l) : top;
-					if (n + e == target && n + e < N) {
-						hit[m] = l;
+					l[f][e] = static_cast<float>(sums[f][i][e]) * sx * sw[f][e];
+				}
+			}
+			if (!all) { // nothing past the vocabulary
+#pragma unroll
+				for (int f = 0; f < FN; ++f) {
+#pragma unroll
+					for (int e = 0; e < 4; ++e) {
+						l[f][e] = n0 + 16 * f + 4 * group + e < N ? l[f][e] : -__builtin_inff();
 					}
 				}
+			}
+			if (target >= 0 && target < 16 * FN && n0 + target < N) {
+#pragma unroll
+				for (int f = 0; f < FN; ++f) {
+#pragma unroll
+					for (int e = 0; e < 4; ++e) {
+						if (16 * f + 4 * group + e == target) {
+							hit[m] = l[f][e];
+						}
+					}
+				}
+			}
+#pragma unroll
+			for (int f = 0; f < FN; ++f) {
+				top = fmaxf(fmaxf(top, fmaxf(l[f][0], l[f][1])), fmaxf(l[f][2], l[f][3]));
 			}
 			top = fmaxf(top, __shfl_xor(top, 16));
 			top = fmaxf(top, __shfl_xor(top, 32));
 			float sum = 0.0f;
 #pragma unroll
 			for (int f = 0; f < FN; ++f) {
-				const int n	 = n0 + 16 * f + 4 * (lane >> 4);
-				const v4f sw = i8_scales4(w, n);
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
-					const float l = static_cast<float>(sums[f][i][e]) * sx * sw[e];
-					sum += n + e < N ? exp2_native((l - top) * LOG2_E) : 0.0f;
+					sum += exp2_native((l[f][e] - top) * LOG2_E);
 				}
 			}
 			sum += __shfl_xor(sum, 16);
@@ -178,8 +200,14 @@ template<int TERMS> struct i8_slopes {
 
 	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f*) const {
 		static_assert(FN % 2 == 0);
-		const int lane = threadIdx.x & 63, block = (n0 - first_n) / 32;
+		const int lane = threadIdx.x & 63, group = lane >> 4, block = (n0 - first_n) / 32;
 		const int f	   = scales_exponent(maxima);
+		const bool all = n0 + 16 * FN <= N;
+		v4f sw[FN];
+#pragma unroll
+		for (int c = 0; c < FN; ++c) {
+			sw[c] = i8_scales4(w, n0 + 16 * c + 4 * group);
+		}
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
 			const int strip = m0 / 16 + i, m = 16 * strip + (lane & 15);
@@ -188,28 +216,41 @@ template<int TERMS> struct i8_slopes {
 			}
 			const int target  = m < M ? targets[m] : -1;
 			const bool scored = target >= 0 && target < N;
+			// (a row that is not scored: finite numbers times nothing)
 			const float sx = scored ? x.scale[m] : 0.0f, below = scored ? lse[m] : 0.0f;
 			const float lift = scored ? ldexpf(1.0f, slopes_exponent(losses[m])) : 0.0f;
+			const bool here	 = scored && target >= n0 && target < n0 + 16 * FN;
 #pragma unroll
 			for (int b = 0; b < FN / 2; ++b) {
 				if (block + b >= blocks) {
 					continue;
 				}
-				v8h out[TERMS];
+				float v[8];
 #pragma unroll
 				for (int h = 0; h < 2; ++h) {
-					const int n	 = n0 + 32 * b + 16 * h + 4 * (lane >> 4);
-					const v4f sw = i8_scales4(w, n);
 #pragma unroll
 					for (int e = 0; e < 4; ++e) {
-						const float l = static_cast<float>(sums[2 * b + h][i][e]) * sx * sw[e];
-						const float d = exp2_native((l - below) * LOG2_E) - (n + e == target ? 1.0f : 0.0f);
-						float v		  = scored && n + e < N ? d * lift * ldexpf(sw[e], f) : 0.0f;
+						const float l = static_cast<float>(sums[2 * b + h][i][e]) * sx * sw[2 * b + h][e];
+						v[4 * h + e]  = exp2_native((l - below) * LOG2_E);
+					}
+				}
+				if (here) {
 #pragma unroll
-						for (int t = 0; t < TERMS; ++t) {
-							out[t][4 * h + e] = static_cast<_Float16>(v);
-							v -= static_cast<float>(out[t][4 * h + e]);
-						}
+					for (int j = 0; j < 8; ++j) {
+						v[j] -= n0 + 32 * b + 16 * (j >> 2) + 4 * group + (j & 3) == target ? 1.0f : 0.0f;
+					}
+				}
+				v8h out[TERMS];
+#pragma unroll
+				for (int j = 0; j < 8; ++j) {
+					v[j] *= ldexpf(sw[2 * b + (j >> 2)][j & 3], f) * lift;
+					if (!all) {
+						v[j] = n0 + 32 * b + 16 * (j >> 2) + 4 * group + (j & 3) < N ? v[j] : 0.0f;
+					}
+#pragma unroll
+					for (int t = 0; t < TERMS; ++t) {
+						out[t][j] = static_cast<_Float16>(v[j]);
+						v[j] -= static_cast<float>(out[t][j]);
 					}
 				}
 #pragma unroll
@@ -226,7 +267,8 @@ template<int TERMS> struct i8_slopes {
 typedef int v2i __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ v2i i8_columns(const v4u* first, const v4u* second, int c, int lane) {
 	const int j = (lane & 15) >> 1, row = 4 * (lane >> 4) + (j & 3);
-	const char* at = reinterpret_cast<const char*>(j < 4 ? first : second) + (c * 16 + row) * 16 + 8 * (lane & 1);
+	// (the second strip's rows lie eight further, so that the 32 lanes that are served together meet no bank twice)
+	const char* at = reinterpret_cast<const char*>(j < 4 ? first : second) + (c * 16 + (j < 4 ? row : row ^ 8)) * 16 + 8 * (lane & 1);
 	return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(const_cast<char*>(at)));
 }
 // ... as fp16: 128 + q as the low byte of 0x6400 + ... is the fp16 number 1024 + 128 + q
@@ -252,53 +294,47 @@ struct i8_slope_product {
 
 // A workgroup has 512 columns x 16 FM rows of sums over its split's blocks of 32 n, a wave 64 of the columns, so that each piece of w is made fp16 by one wave only.  Blocks come through a
 // ring in LDS as in i8_tile_product, and w's pieces of the next block are read and converted among the products of this one.
-template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_kernel(i8_matrix w, i8_slope_product a, int k_tiles, int m_tiles) {
+template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_kernel(i8_matrix w, i8_slope_product a, int k_tiles, int m_tiles, int splits) {
 	constexpr int WAVES = 8, FK = 4, STEPS = WAVES, NF = 2 * STEPS, FRAGMENTS = NF + FM * TERMS, LOADS = FRAGMENTS / WAVES, MORE = FRAGMENTS % WAVES, RING = 4;
-	// P of the next block in registers too, where there is room for it
-	constexpr bool AHEAD = FM * TERMS <= 8;
+	constexpr int FIRST = (FM * TERMS + 1) / 2 < 4 ? FM : 4 / TERMS; // strips of P that are in registers before a block begins; the others are read in it
 	__shared__ v4u ring[RING][FRAGMENTS][64];
-	const int split = blockIdx.y;
-	const i8_place p = i8_place_of(k_tiles, m_tiles);
-	if (!p.there) {
+	// each XCD has a run of tiles, the tiles of a split (which have w's rows, or P's, in common) one behind the other
+	const int tiles = k_tiles * m_tiles, run = (tiles * splits + 7) >> 3, place = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+	if (place >= tiles * splits) {
 		return;
 	}
+	const int split = place / tiles, tile = place % tiles;
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-	const int step0 = p.n * STEPS, strip0 = p.m * FM;
+	const int step0 = tile % k_tiles * STEPS, strip0 = tile / k_tiles * FM;
 	const int begin = split * a.per, blocks = min(a.per, a.blocks - begin);
 	// this wave's fragments of a block: [two strips of w][step], then [strip of P][term]; the first MORE waves have one more
 	const bool more = wave < MORE;
-	const v4u* from[LOADS + 1];
-	int64_t onward[LOADS + 1]; // from a block to the next
-	int last[LOADS + 1]; // of a strip of w that there is
+	const v4u* from[LOADS + 1]; // where the next block that is asked for lies
 #pragma unroll
 	for (int j = 0; j < LOADS + 1; ++j) {
 		const int f = j < LOADS ? wave + WAVES * j : WAVES * LOADS + min(wave, MORE - 1);
 		if (f < NF) {
-			// (the last block's second strip may not be there: one before it instead, which meets zeros)
-			const int strip = min(2 * (a.first_block + begin) + f / STEPS, w.strips - 1);
-			from[j]			= w.q + (static_cast<int64_t>(strip) * w.steps + min(step0 + f % STEPS, w.steps - 1)) * 64;
-			onward[j]		= static_cast<int64_t>(2) * w.steps * 64;
-			last[j]			= (w.strips - 1 - strip) >> 1;
+			from[j] = w.q + (static_cast<int64_t>(2 * (a.first_block + begin) + f / STEPS) * w.steps + min(step0 + f % STEPS, w.steps - 1)) * 64;
 		} else {
 			const int t = (f - NF) % TERMS, strip = min(strip0 + (f - NF) / TERMS, a.strips - 1);
 			from[j]		= reinterpret_cast<const v4u*>(a.p) + ((static_cast<int64_t>(t) * a.strips + strip) * a.blocks + begin) * 64;
-			onward[j]	= 64;
-			last[j]		= a.blocks;
 		}
 	}
+	static_assert(LOADS >= 2 && STEPS == WAVES); // so that j is which strip of w, or P
+	const int whole = (w.strips >> 1) - a.first_block - begin; // blocks whose second strip there is; the last one's place meets zeros in P
 	auto load = [&](int s) {
 #pragma unroll
 		for (int j = 0; j < LOADS + 1; ++j) {
 			if (j < LOADS || more) {
-				load_global_to_lds_b128(from[j] + min(s, last[j]) * onward[j], 16 * lane, &ring[s % RING][j < LOADS ? wave + WAVES * j : WAVES * LOADS + wave][0]);
+				const v4u* at = j == 1 && s >= whole ? from[0] : from[j];
+				load_global_to_lds_b128(at, 16 * (j == 1 ? lane ^ 8 : lane), &ring[s % RING][j < LOADS ? wave + WAVES * j : WAVES * LOADS + wave][0]);
+				from[j] += j < 2 ? static_cast<int64_t>(2) * w.steps * 64 : 64;
 			}
 		}
 	};
 	auto arrive_by = [&](auto loads, int behind) { // a block is in LDS, those up to `behind` blocks after it may be on their way
 		constexpr int L = decltype(loads)::value;
-		if (behind >= 3) {
-			i8_arrive<3 * L>();
-		} else if (behind == 2) {
+		if (behind >= 2) {
 			i8_arrive<2 * L>();
 		} else if (behind == 1) {
 			i8_arrive<L>();
@@ -319,74 +355,78 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 			raw[c] = i8_columns(ring[s % RING][wave], ring[s % RING][STEPS + wave], c, lane);
 		}
 	};
-	auto read_p = [&](int s, v8h(&d)[FM][TERMS]) {
+	auto read_p = [&](int s, int i, v8h(&d)[TERMS]) {
 #pragma unroll
-		for (int i = 0; i < FM; ++i) {
-#pragma unroll
-			for (int t = 0; t < TERMS; ++t) {
-				d[i][t] = __builtin_bit_cast(v8h, ring[s % RING][NF + i * TERMS + t][lane]);
-			}
+		for (int t = 0; t < TERMS; ++t) {
+			d[t] = __builtin_bit_cast(v8h, ring[s % RING][NF + i * TERMS + t][lane]);
 		}
 	};
 	v4f sums[FK][FM] = {};
-	auto multiply	 = [&](const v8h(&k)[FK], const v8h(&d)[FM][TERMS]) {
+	auto multiply	 = [&](const v8h(&k)[FK], int i, const v8h(&d)[TERMS]) {
 #pragma unroll
-		for (int i = 0; i < FM; ++i) {
+		for (int t = TERMS - 1; t >= 0; --t) { // the small term first
 #pragma unroll
-			for (int t = TERMS - 1; t >= 0; --t) { // the small term first
-#pragma unroll
-				for (int f = 0; f < FK; ++f) {
-					sums[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[f], d[i][t], sums[f][i], 0, 0, 0);
-				}
+			for (int f = 0; f < FK; ++f) {
+				sums[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[f], d[t], sums[f][i], 0, 0, 0);
 			}
 		}
 	};
 	v2i raw[FK];
-	v8h k[2][FK], d[2][FM][TERMS];
+	v8h k[2][FK], d[2][FIRST][TERMS];
+	auto block = [&](int s, int h) { // block s, from registers of parity h; the next one is in LDS
+		v8h late[FM - FIRST + 1][TERMS];
+#pragma unroll
+		for (int i = FIRST; i < FM; ++i) {
+			read_p(s, i, late[i - FIRST]);
+		}
+		read_k(s + 1, raw);
+#pragma unroll
+		for (int i = 0; i < FIRST; ++i) {
+			multiply(k[h], i, d[h][i]);
+		}
+#pragma unroll
+		for (int i = 0; i < FIRST; ++i) {
+			read_p(s + 1, i, d[1 - h][i]);
+		}
+#pragma unroll
+		for (int f = 0; f < FK; ++f) {
+			k[1 - h][f] = i8_halves(raw[f]);
+		}
+#pragma unroll
+		for (int i = FIRST; i < FM; ++i) {
+			multiply(k[h], i, late[i - FIRST]);
+		}
+	};
 	if (blocks > 0) {
-		// with AHEAD nobody reads block s any more once block s + 1 is there, and block s + RING takes its place; else that of block s - 1 is free
-		constexpr int ASKED = AHEAD ? RING : RING - 1;
+		constexpr int ASKED = RING - 1; // once block s + 1 is there nobody reads block s - 1 any more: block s + ASKED takes its place
 		for (int s = 0; s < min(blocks, ASKED); ++s) {
 			load(s);
 		}
 		arrive(min(blocks, ASKED) - 1);
 		read_k(0, raw);
-		if constexpr (AHEAD) {
-			read_p(0, d[0]);
+#pragma unroll
+		for (int i = 0; i < FIRST; ++i) {
+			read_p(0, i, d[0][i]);
 		}
 #pragma unroll
 		for (int f = 0; f < FK; ++f) {
 			k[0][f] = i8_halves(raw[f]);
 		}
-#pragma unroll 1
-		for (int s = 0; s < blocks; s += 2) {
-#pragma unroll
-			for (int h = 0; h < 2; ++h) {
-				if (s + h >= blocks) {
-					break;
-				}
-				const bool next = s + h + 1 < blocks;
-				if (next) {
-					arrive(min(blocks, s + h + ASKED) - 1 - (s + h + 1));
-					if (s + h + ASKED < blocks) {
-						load(s + h + ASKED);
-					}
-					read_k(s + h + 1, raw);
-					if constexpr (AHEAD) {
-						read_p(s + h + 1, d[1 - h]);
-					}
-				}
-				if constexpr (!AHEAD) {
-					read_p(s + h, d[h]);
-				}
-				multiply(k[h], d[h]);
-				if (next) {
-#pragma unroll
-					for (int f = 0; f < FK; ++f) {
-						k[1 - h][f] = i8_halves(raw[f]);
-					}
-				}
+		auto next = [&](int s) { // block s + 1 is there, and everybody is through with block s - 1
+			arrive(min(blocks, s + ASKED) - 2 - s);
+			if (s + ASKED < blocks) {
+				load(s + ASKED);
 			}
+		};
+		// (behind the last block something is read that lies in LDS, and not used)
+		for (int s = 0; s < blocks; ++s) {
+			next(s);
+			block(s, 0);
+			if (++s >= blocks) {
+				break;
+			}
+			next(s);
+			block(s, 1);
 		}
 	}
 #pragma unroll
@@ -462,9 +502,9 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 		a.M = x.rows, a.columns = w.steps * I8_STEP, a.strips = x.strips, a.blocks = static_cast<int>(blocks), a.first_block = static_cast<int>(first / 32);
 		a.per = static_cast<int>((blocks + plan.splits - 1) / plan.splits);
 		a.add = first > 0;
-		const dim3 grid(i8_grid(plan.k_tiles, plan.m_tiles), static_cast<unsigned>(plan.splits));
+		const unsigned grid = i8_grid(plan.k_tiles * plan.splits, plan.m_tiles);
 		auto multiply = [&](auto kernel) {
-			kernel<<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(plan.m_tiles));
+			kernel<<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(plan.m_tiles), static_cast<int>(plan.splits));
 		};
 		if (plan.strips == 8) {
 			multiply(i8_slope_kernel<8, TERMS>);
