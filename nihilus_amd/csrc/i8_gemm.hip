@@ -3,6 +3,7 @@
 // The sums are whole numbers and exact (K is limited so that they stay below 2^31); each is brought to fp32, scaled by the row's and then by the channel's scale, the residual added,
 // and rounded once to y's type.  The kernels are in i8_product.h.
 #include "i8_product.h"
+#include "i8_values.h"
 
 namespace nh {
 
@@ -14,6 +15,16 @@ template<int TYPE> struct i8_store {
 	value* y;
 	const value* residual;
 	int M, N;
+
+	// the only row's sums of a strip of n, in all of a fragment's columns
+	__device__ __forceinline__ void token(v4i sums, int n0, float sx, const i8_matrix& w) const {
+		const int lane = threadIdx.x & 63, n = n0 + 4 * (lane >> 4) + (lane & 3);
+		if ((lane & 15) < 4 && n < N) { // a lane takes one of its four
+			const int sum = (lane & 2) ? (lane & 1) ? sums[3] : sums[2] : (lane & 1) ? sums[1] : sums[0];
+			const float v = static_cast<float>(sum) * sx * w.scale[n];
+			y[n]		  = T::narrow(residual ? v + T::widen(residual[n]) : v);
+		}
+	}
 
 	// A lane has four neighbouring n of sixteen different rows m: sixteen rows at a time go through LDS, so that a wave's stores run along the rows.  Pieces of four values lie at
 	// places permuted by the row, which spreads them over the banks either way.
@@ -80,6 +91,151 @@ template<int TYPE> struct i8_store {
 	}
 };
 
+// One row, quantized inside (behind the norm if there is one): every workgroup brings the whole row to 8 bits in LDS by itself, which takes less than a launch of its own and the wait for it, while the
+// first of its weights are on their way.  Then as i8_rows_product for one strip of x, all of whose rows are this one.  PIECES: of eight values per thread, so K up to 4096 PIECES.
+constexpr int TOKEN_STEPS = 256; // K up to 16384
+template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(512) void i8_token_product(i8_matrix w, const void* x, const float* norm, float eps, int K, int n_tiles, i8_store<TYPE> epi) {
+	constexpr int WAVES = 8, AHEAD = 8 / FN;
+	__shared__ v4u row[PIECES * 256]; // [step][16 values]
+	__shared__ v4i parts[WAVES][FN][64];
+	__shared__ double squares[WAVES];
+	__shared__ uint32_t tops[WAVES];
+	const i8_place p = i8_place_of(n_tiles, 1);
+	if (!p.there) {
+		return;
+	}
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int pieces = 8 * w.steps;
+	float v[PIECES][8];
+#pragma unroll
+	for (int j = 0; j < PIECES; ++j) {
+		const int c = threadIdx.x + 512 * j;
+		if (c < pieces) {
+			i8_load<TYPE>(x, 8 * c, K - 8 * c, v[j]);
+		}
+	}
+	const int n_strip = p.n * FN;
+	const v4u* a[FN];
+#pragma unroll
+	for (int f = 0; f < FN; ++f) {
+		a[f] = w.q + static_cast<int64_t>(min(n_strip + f, w.strips - 1)) * w.steps * 64 + lane;
+	}
+	const int per = (w.steps + WAVES - 1) / WAVES, begin = wave * per, end = min(w.steps, begin + per), last = max(min(end, w.steps) - 1, 0);
+	v4u ahead[AHEAD][FN];
+	auto load = [&](int s) { // (past the wave's last step: that one again, or any where it has none)
+#pragma unroll
+		for (int u = 0; u < AHEAD; ++u) {
+#pragma unroll
+			for (int f = 0; f < FN; ++f) {
+				ahead[u][f] = a[f][min(s + u, last) * 64];
+			}
+		}
+	};
+	load(begin);
+	if constexpr (NORM) {
+		double sum = 0.0;
+#pragma unroll
+		for (int j = 0; j < PIECES; ++j) {
+			if (threadIdx.x + 512 * j < static_cast<unsigned>(pieces)) {
+#pragma unroll
+				for (int e = 0; e < 8; ++e) {
+					sum = fma(static_cast<double>(v[j][e]), static_cast<double>(v[j][e]), sum);
+				}
+			}
+		}
+#pragma unroll
+		for (int d = 32; d > 0; d >>= 1) {
+			sum += __shfl_xor(sum, d);
+		}
+		if (lane == 0) {
+			squares[wave] = sum;
+		}
+		__syncthreads();
+		sum = squares[0];
+#pragma unroll
+		for (int i = 1; i < WAVES; ++i) {
+			sum += squares[i];
+		}
+		const float r = i8_rms(sum, K, eps);
+#pragma unroll
+		for (int j = 0; j < PIECES; ++j) {
+			const int c = threadIdx.x + 512 * j;
+			if (c < pieces) {
+				float g[8];
+				i8_load<NH_F32>(norm, 8 * c, K - 8 * c, g);
+#pragma unroll
+				for (int e = 0; e < 8; ++e) {
+					v[j][e] = __fmul_rn(__fmul_rn(v[j][e], r), g[e]);
+				}
+			}
+		}
+	}
+	uint32_t top = 0;
+#pragma unroll
+	for (int j = 0; j < PIECES; ++j) {
+		if (threadIdx.x + 512 * j < static_cast<unsigned>(pieces)) {
+#pragma unroll
+			for (int e = 0; e < 8; ++e) {
+				top = max(top, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
+			}
+		}
+	}
+#pragma unroll
+	for (int d = 32; d > 0; d >>= 1) {
+		top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+	}
+	if (lane == 0) {
+		tops[wave] = top;
+	}
+	__syncthreads();
+#pragma unroll
+	for (int i = 0; i < WAVES; ++i) {
+		top = max(top, tops[i]);
+	}
+	const i8_step step(top);
+#pragma unroll
+	for (int j = 0; j < PIECES; ++j) {
+		const int c = threadIdx.x + 512 * j;
+		if (c < pieces) {
+			uint32_t out[2];
+			step.round(v[j], out);
+			reinterpret_cast<v2u*>(row)[c] = v2u{ out[0], out[1] };
+		}
+	}
+	__syncthreads();
+	v4i sums[FN][1] = {};
+	const v4u* b = row + (lane >> 4);
+#pragma unroll 1
+	for (int s = begin; s < end;) {
+#pragma unroll
+		for (int u = 0; u < AHEAD; ++u) {
+			if (s + u < end) {
+#pragma unroll
+				for (int f = 0; f < FN; ++f) {
+					sums[f][0] = i8_mfma(ahead[u][f], b[4 * (s + u)], sums[f][0]);
+				}
+			}
+		}
+		s += AHEAD;
+		if (s < end) {
+			load(s);
+		}
+	}
+#pragma unroll
+	for (int f = 0; f < FN; ++f) {
+		parts[wave][f][lane] = sums[f][0];
+	}
+	__syncthreads();
+	if (wave < FN) {
+		v4i all = parts[0][wave][lane];
+#pragma unroll
+		for (int i = 1; i < WAVES; ++i) {
+			all += parts[i][wave][lane];
+		}
+		epi.token(all, (n_strip + wave) * I8_ROWS, step.scale, w);
+	}
+}
+
 template<int TYPE> hipError_t gemm(const i8_matrix& w, const i8_matrix& x, const void* residual, void* y, hipStream_t stream) {
 	typedef typename i8_type<TYPE>::store value;
 	const i8_store<TYPE> epi{ static_cast<value*>(y), static_cast<const value*>(residual), x.rows, w.rows };
@@ -87,7 +243,30 @@ template<int TYPE> hipError_t gemm(const i8_matrix& w, const i8_matrix& x, const
 	return hipGetLastError();
 }
 
+template<int TYPE> hipError_t token(const i8_matrix& w, const i8_rows& in, const void* residual, void* y, hipStream_t stream) {
+	typedef typename i8_type<TYPE>::store value;
+	const i8_store<TYPE> epi{ static_cast<value*>(y), static_cast<const value*>(residual), 1, w.rows };
+	auto launch = [&](auto kernel, int n_strips) {
+		const int n_tiles = (w.strips + n_strips - 1) / n_strips;
+		kernel<<<i8_grid(n_tiles, 1), 512, 0, stream>>>(w, in.x, in.norm, in.eps, in.k, n_tiles, epi);
+	};
+	const bool one = w.steps <= 64, few = w.strips <= 512;
+	if (in.norm) {
+		one ? few ? launch(i8_token_product<TYPE, true, 1, 1>, 1) : launch(i8_token_product<TYPE, true, 1, 2>, 2) : few ? launch(i8_token_product<TYPE, true, 4, 1>, 1) : launch(i8_token_product<TYPE, true, 4, 2>, 2);
+	} else {
+		one ? few ? launch(i8_token_product<TYPE, false, 1, 1>, 1) : launch(i8_token_product<TYPE, false, 1, 2>, 2) : few ? launch(i8_token_product<TYPE, false, 4, 1>, 1) : launch(i8_token_product<TYPE, false, 4, 2>, 2);
+	}
+	return hipGetLastError();
+}
+
 } // namespace
+
+bool i8_token_fits(int64_t m, int64_t k) {
+	return m == 1 && i8_steps(k) <= TOKEN_STEPS;
+}
+hipError_t launch_i8_token(const i8_matrix& w, const i8_rows& in, int type, const void* residual, void* y, hipStream_t stream) {
+	return type == NH_F32 ? token<NH_F32>(w, in, residual, y, stream) : type == NH_F16 ? token<NH_F16>(w, in, residual, y, stream) : token<NH_BF16>(w, in, residual, y, stream);
+}
 
 hipError_t launch_i8_gemm(const i8_matrix& w, const i8_matrix& x, const void* residual, void* y, int type, hipStream_t stream) {
 	return type == NH_F32 ? gemm<NH_F32>(w, x, residual, y, stream) : type == NH_F16 ? gemm<NH_F16>(w, x, residual, y, stream) : gemm<NH_BF16>(w, x, residual, y, stream);

@@ -9,65 +9,13 @@
 // Bound by memory where rows are many, by the chain of a row's passes where they are few: a workgroup has one row or four, a thread sixteen values at a time (one 16-byte piece of a
 // fragment), up to 64 of them kept in registers between the passes that a row's maximum and a norm need; longer rows are read again, from the caches.  The workgroups of a strip go to one XCD,
 // whose L2 joins their pieces to whole lines.
-#include "i8_device.h"
+#include "i8_values.h"
 
 namespace nh {
 
 namespace {
 
 constexpr int HELD = 4; // pieces of sixteen values that a thread keeps
-
-// sixteen values; those from `left` on are zero (rows begin anywhere: the hardware takes any address)
-template<int TYPE> __device__ __forceinline__ void load16(const void* base, int64_t at, int left, float (&v)[16]) {
-	using T		  = i8_type<TYPE>;
-	const auto* p = static_cast<const typename T::store*>(base) + at;
-	if (left >= 16) {
-		typename T::store part[16];
-		__builtin_memcpy(part, p, sizeof(part));
-#pragma unroll
-		for (int j = 0; j < 16; ++j) {
-			v[j] = T::widen(part[j]);
-		}
-		return;
-	}
-#pragma unroll
-	for (int j = 0; j < 16; ++j) {
-		v[j] = j < left ? T::widen(p[j]) : 0.0f;
-	}
-}
-
-// The whole numbers nearest to v / s as bytes, `inverse` being 1 / s to a unit in the last place.  c, the product with that rounded, is one of the two next to the quotient, and v - c s is
-// exact wherever it is close to half of s (a difference of multiples of the last place of the smaller of v and s, below s): comparing it with s / 2 decides between the two.  Where no
-// value of the wave's is that close, which is nearly always, c is right as it is.
-// (`doubt`: they may be past 127, which rows below the normal numbers reach, whose scale has few bits)
-__device__ __forceinline__ v4u nearest16(const float (&v)[16], float s, float inverse, bool doubt) {
-	constexpr float magic = 12582912.0f; // 1.5 * 2^23: the sum's low byte is the whole number
-	float c[16], far = 0.0f;
-#pragma unroll
-	for (int j = 0; j < 16; ++j) {
-		c[j] = fmaf(v[j], inverse, magic);
-		far	 = fmaxf(far, fabsf(fmaf(magic - c[j], s, v[j])));
-	}
-	if (doubt || far >= 0.5f * s) {
-#pragma unroll
-		for (int j = 0; j < 16; ++j) {
-			float n		  = c[j] - magic;
-			const float e = fmaf(-n, s, v[j]), half = 0.5f * s;
-			if (fabsf(e) >= half && (fabsf(e) > half || (static_cast<int>(n) & 1))) {
-				n += copysignf(1.0f, e);
-			}
-			c[j] = fminf(fmaxf(n, -127.0f), 127.0f) + magic;
-		}
-	}
-	v4u out;
-#pragma unroll
-	for (int d = 0; d < 4; ++d) { // (selector: 0..3 bytes of the second operand, 4..7 of the first)
-		const uint32_t low	= __builtin_amdgcn_perm(__float_as_uint(c[4 * d + 1]), __float_as_uint(c[4 * d]), 0x0c0c0400u);
-		const uint32_t high = __builtin_amdgcn_perm(__float_as_uint(c[4 * d + 3]), __float_as_uint(c[4 * d + 2]), 0x04000c0cu);
-		out[d]				= low | high;
-	}
-	return out;
-}
 
 // silu(g) u within 3 units in the last place: -g log2(e) in two parts, the exponential's one unit, a sum, a quotient by one correction step (so within half a unit and little more), a product.
 // Below g = -87 the exponential is held at 2^126: what is left is below 2^-119 of up.
@@ -95,10 +43,10 @@ template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds_
 	const int64_t at = static_cast<int64_t>(row) * in.stride, up_at = static_cast<int64_t>(row) * in.up_stride;
 	float r = 1.0f;
 	auto get = [&](int c, float(&v)[16]) { // without the norm
-		load16<TYPE>(in.x, at + 16 * c, in.k - 16 * c, v);
+		i8_load<TYPE>(in.x, at + 16 * c, in.k - 16 * c, v);
 		if constexpr (FRONT == I8_SILU) {
 			float u[16];
-			load16<TYPE>(in.up, up_at + 16 * c, in.k - 16 * c, u);
+			i8_load<TYPE>(in.up, up_at + 16 * c, in.k - 16 * c, u);
 #pragma unroll
 			for (int j = 0; j < 16; ++j) {
 				v[j] = silu_times(v[j], u[j]);
@@ -108,7 +56,7 @@ template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds_
 	auto normed = [&](int c, float(&v)[16]) {
 		if constexpr (FRONT == I8_NORM) {
 			float w[16];
-			load16<NH_F32>(in.norm, 16 * c, in.k - 16 * c, w);
+			i8_load<NH_F32>(in.norm, 16 * c, in.k - 16 * c, w);
 #pragma unroll
 			for (int j = 0; j < 16; ++j) {
 				v[j] = __fmul_rn(__fmul_rn(v[j], r), w[j]);
@@ -156,7 +104,7 @@ template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds_
 				sum += sums[mine][w];
 			}
 		}
-		r = static_cast<float>(1.0 / sqrt(sum / in.k + static_cast<double>(in.eps)));
+		r = i8_rms(sum, in.k, in.eps);
 	}
 	uint32_t top = 0; // of the values' bits without their signs: infinities and NaN are above all others
 	auto raise	 = [&](const float(&v)[16]) {
@@ -192,25 +140,14 @@ template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds_
 			top = max(top, tops[mine][w]);
 		}
 	}
-	const bool finite = top < 0x7F800000u;
-	const float s	  = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __builtin_nanf("");
+	const i8_step step(top);
 	if (there && t == 0) {
-		scale[row] = s;
+		scale[row] = step.scale;
 	}
-	// far down both are brought up, which is exact, so that the reciprocal and the products stay normal numbers
-	const float lift	= s < 0x1p-100f ? 0x1p100f : 1.0f;
-	const float step	= s * lift;
-	const bool nothing	= !finite || s == 0.0f;
-	const float inverse = nothing ? 0.0f : __builtin_amdgcn_rcpf(step);
-	auto put			= [&](int c, float(&v)[16]) {
-		   if (lift != 1.0f) {
-#pragma unroll
-			   for (int j = 0; j < 16; ++j) {
-				   v[j] *= lift;
-			   }
-		   }
-		   const v4u out = nearest16(v, step, inverse, lift != 1.0f);
-		   q[(static_cast<int64_t>(row >> 4) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = nothing ? v4u{} : out;
+	auto put = [&](int c, float(&v)[16]) {
+		uint32_t out[4];
+		step.round(v, out);
+		q[(static_cast<int64_t>(row >> 4) * steps + (c >> 2)) * 64 + (c & 3) * 16 + (row & 15)] = v4u{ out[0], out[1], out[2], out[3] };
 	};
 #pragma unroll
 	for (int h = 0; h < HELD; ++h) {

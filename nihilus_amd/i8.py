@@ -61,7 +61,9 @@ def _need(fn: str, *sizes) -> int:
     return n
 
 
-def _workspace(workspace: torch.Tensor | None, n: int, device: torch.device) -> tuple[torch.Tensor, int, int]:
+def _workspace(workspace: torch.Tensor | None, n: int, device: torch.device) -> tuple[torch.Tensor | None, int | None, int]:
+    if n == 0 and workspace is None:
+        return None, None, 0
     if workspace is None:
         _own_memory(n, device)
         workspace = _bytes(n, device)

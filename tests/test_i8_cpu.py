@@ -28,7 +28,8 @@ def test_every_declared_function_is_exported_and_bound(lib):
 def test_bytes_of_a_tiled_matrix(lib, rows, k):
     strips = (rows + 15) // 16
     assert lib.nh_i8_tiled_bytes(rows, k) == strips * ((k + 63) // 64 * 1024 + 64)
-    assert lib.nh_i8_mul_mat_workspace_bytes(rows, k) == lib.nh_i8_tiled_bytes(rows, k)
+    # (one row of up to 16384 values is quantized inside the product)
+    assert lib.nh_i8_mul_mat_workspace_bytes(rows, k) == (0 if rows == 1 and k <= 16384 else lib.nh_i8_tiled_bytes(rows, k))
 
 
 def test_sizes_that_are_refused(lib):
