@@ -74,6 +74,7 @@ int quantize(const void* x, const void* up, const float* norm, float eps, int fr
 	nh::i8_rows in{};
 	in.x = x, in.up = up, in.norm = norm, in.eps = eps;
 	in.stride = rows > 1 ? stride : 0, in.up_stride = rows > 1 ? up_stride : 0;
+	in.part = 1.0 / static_cast<double>(k);
 	in.rows = static_cast<int>(rows), in.k = static_cast<int>(k);
 	return from_hip(nh::launch_i8_quantize(in, front, type, tiled, as_stream(stream)));
 }
@@ -147,6 +148,7 @@ int nh_i8_mul_mat(const void* w_tiled, const void* x, int type, int64_t x_stride
 		NH_TRY(require_device());
 		nh::i8_rows in{};
 		in.x = x, in.norm = norm_weight, in.eps = eps;
+		in.part = 1.0 / static_cast<double>(K);
 		in.rows = 1, in.k = static_cast<int>(K);
 		return from_hip(nh::launch_i8_token(nh::i8_view(w_tiled, N, K), in, type, residual, y, as_stream(stream)));
 	}

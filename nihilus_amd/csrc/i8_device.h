@@ -76,6 +76,7 @@ struct i8_rows {
 	const void* up; // I8_SILU: x is the gate
 	const float* norm; // I8_NORM
 	int64_t stride, up_stride; // elements from one row to the next
+	double part; // 1 / k
 	float eps;
 	int rows, k;
 };

@@ -94,7 +94,7 @@ template<int TYPE> struct i8_store {
 // One row, quantized inside (behind the norm if there is one): every workgroup brings the whole row to 8 bits in LDS by itself, which takes less than a launch of its own and the wait for it, while the
 // first of its weights are on their way.  Then as i8_rows_product for one strip of x, all of whose rows are this one.  PIECES: of eight values per thread, so K up to 4096 PIECES.
 constexpr int TOKEN_STEPS = 256; // K up to 16384
-template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(512) void i8_token_product(i8_matrix w, const void* x, const float* norm, float eps, int K, int n_tiles, i8_store<TYPE> epi) {
+template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(512) void i8_token_product(i8_matrix w, const void* x, const float* norm, double part, float eps, int K, int n_tiles, i8_store<TYPE> epi) {
 	constexpr int WAVES = 8, AHEAD = 8 / FN;
 	__shared__ v4u row[PIECES * 256]; // [step][16 values]
 	__shared__ v4i parts[WAVES][FN][64];
@@ -156,7 +156,7 @@ template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(5
 		for (int i = 1; i < WAVES; ++i) {
 			sum += squares[i];
 		}
-		const float r = i8_rms(sum, K, eps);
+		const float r = i8_rms(sum, part, eps);
 #pragma unroll
 		for (int j = 0; j < PIECES; ++j) {
 			const int c = threadIdx.x + 512 * j;
@@ -248,7 +248,7 @@ template<int TYPE> hipError_t token(const i8_matrix& w, const i8_rows& in, const
 	const i8_store<TYPE> epi{ static_cast<value*>(y), static_cast<const value*>(residual), 1, w.rows };
 	auto launch = [&](auto kernel, int n_strips) {
 		const int n_tiles = (w.strips + n_strips - 1) / n_strips;
-		kernel<<<i8_grid(n_tiles, 1), 512, 0, stream>>>(w, in.x, in.norm, in.eps, in.k, n_tiles, epi);
+		kernel<<<i8_grid(n_tiles, 1), 512, 0, stream>>>(w, in.x, in.norm, in.part, in.eps, in.k, n_tiles, epi);
 	};
 	const bool one = w.steps <= 64, few = w.strips <= 512;
 	if (in.norm) {

@@ -155,6 +155,7 @@ constexpr int MAXIMA = 64;
 __global__ __launch_bounds__(256) void i8_largest_scales(const float* scale, int n, float* out) {
 	__shared__ float tops[4];
 	float top = 0.0f;
+#pragma unroll 8
 	for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += MAXIMA * 256) {
 		top = fmaxf(top, fabsf(scale[i]));
 	}
@@ -456,6 +457,7 @@ template<int TYPE> __global__ __launch_bounds__(256) void i8_slope_results(const
 	}
 	const bool scored = targets[m] >= 0 && targets[m] < N;
 	v4f all{};
+#pragma unroll 8
 	for (int s = 0; s < splits; ++s) {
 		all += *reinterpret_cast<const v4f*>(sums + (static_cast<int64_t>(s) * M + m) * columns + k);
 	}

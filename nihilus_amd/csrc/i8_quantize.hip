@@ -6,16 +6,14 @@
 // q = 0; a row with an infinity or NaN has s = NaN and q = 0, so that whatever is formed from it is NaN, and nothing else is.
 // v of a norm: fl32(fl32(x r) w), r = fl32(1 / sqrt(mean x^2 + eps)) with the mean in 64 bits, where the order of the sum does not show.
 //
-// Bound by memory where rows are many, by the chain of a row's passes where they are few: a workgroup has one row or four, a thread sixteen values at a time (one 16-byte piece of a
-// fragment), up to 64 of them kept in registers between the passes that a row's maximum and a norm need; longer rows are read again, from the caches.  The workgroups of a strip go to one XCD,
+// Bound by memory where rows are many, by the chain of a row's passes where they are few: a workgroup has a row, a thread HELD pieces of sixteen values (16 bytes of a fragment each), which it
+// keeps in registers between the passes that a row's maximum and a norm need; rows longer than that are read again, from the caches.  The sixteen workgroups of a strip go to one XCD,
 // whose L2 joins their pieces to whole lines.
 #include "i8_values.h"
 
 namespace nh {
 
 namespace {
-
-constexpr int HELD = 4; // pieces of sixteen values that a thread keeps
 
 // silu(g) u within 3 units in the last place: -g log2(e) in two parts, the exponential's one unit, a sum, a quotient by one correction step (so within half a unit and little more), a product.
 // Below g = -87 the exponential is held at 2^126: what is left is below 2^-119 of up.
@@ -30,16 +28,17 @@ __device__ __forceinline__ float silu_times(float g, float u) {
 	return fmaf(fmaf(-q, d, g), r, q) * u;
 }
 
-template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds__(ROWS* THREADS) void i8_quantize_kernel(i8_rows in, v4u* q, float* scale, int steps) {
-	constexpr int PARTS = I8_ROWS / ROWS; // workgroups of a strip
+template<int TYPE, int FRONT, int THREADS, int HELD> __global__ __launch_bounds__(THREADS) void i8_quantize_kernel(i8_rows in, v4u* q, float* scale, int steps) {
 	constexpr int WAVES = THREADS / 64; // of a row
-	__shared__ double sums[ROWS][WAVES];
-	__shared__ uint32_t tops[ROWS][WAVES];
+	__shared__ double sums[WAVES];
+	__shared__ uint32_t tops[WAVES];
 	const int i	  = blockIdx.x >> 3;
-	const int row = (i / PARTS * 8 + (blockIdx.x & 7)) * I8_ROWS + ROWS * (i % PARTS) + threadIdx.x / THREADS;
-	const int mine = threadIdx.x / THREADS, t = threadIdx.x % THREADS, wave = t >> 6;
-	const bool there = row < in.rows;
-	const int pieces = there ? 4 * steps : 0;
+	const int row = ((i >> 4) * 8 + (blockIdx.x & 7)) * I8_ROWS + (i & 15);
+	const int t	  = threadIdx.x, wave = t >> 6;
+	if (row >= in.rows) {
+		return;
+	}
+	const int pieces = 4 * steps;
 	const int64_t at = static_cast<int64_t>(row) * in.stride, up_at = static_cast<int64_t>(row) * in.up_stride;
 	float r = 1.0f;
 	auto get = [&](int c, float(&v)[16]) { // without the norm
@@ -95,16 +94,16 @@ template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds_
 		}
 		if constexpr (WAVES > 1) {
 			if ((t & 63) == 0) {
-				sums[mine][wave] = sum;
+				sums[wave] = sum;
 			}
 			__syncthreads();
-			sum = sums[mine][0];
+			sum = sums[0];
 #pragma unroll
 			for (int w = 1; w < WAVES; ++w) {
-				sum += sums[mine][w];
+				sum += sums[w];
 			}
 		}
-		r = i8_rms(sum, in.k, in.eps);
+		r = i8_rms(sum, in.part, in.eps);
 	}
 	uint32_t top = 0; // of the values' bits without their signs: infinities and NaN are above all others
 	auto raise	 = [&](const float(&v)[16]) {
@@ -132,16 +131,16 @@ template<int TYPE, int FRONT, int ROWS, int THREADS> __global__ __launch_bounds_
 	}
 	if constexpr (WAVES > 1) {
 		if ((t & 63) == 0) {
-			tops[mine][wave] = top;
+			tops[wave] = top;
 		}
 		__syncthreads();
 #pragma unroll
 		for (int w = 0; w < WAVES; ++w) {
-			top = max(top, tops[mine][w]);
+			top = max(top, tops[w]);
 		}
 	}
 	const i8_step step(top);
-	if (there && t == 0) {
+	if (t == 0) {
 		scale[row] = step.scale;
 	}
 	auto put = [&](int c, float(&v)[16]) {
@@ -208,20 +207,20 @@ __global__ __launch_bounds__(256) void i8_untile_kernel(const v4u* in, const flo
 }
 
 template<int TYPE, int FRONT> hipError_t quantize(const i8_rows& in, v4u* q, float* scale, int steps, hipStream_t stream) {
-	const int64_t groups = (i8_strips(in.rows) + 7) / 8;
-	auto launch			 = [&](auto kernel, int rows, int threads) {
-		kernel<<<static_cast<unsigned>(groups * 8 * (I8_ROWS / rows)), rows * threads, 0, stream>>>(in, q, scale, steps);
+	const unsigned blocks = static_cast<unsigned>((i8_strips(in.rows) + 7) / 8 * 8 * I8_ROWS);
+	auto launch			  = [&](auto kernel, int threads) {
+		kernel<<<blocks, threads, 0, stream>>>(in, q, scale, steps);
 	};
-	if (in.rows <= 1024) {
-		if (steps <= 64) {
-			launch(i8_quantize_kernel<TYPE, FRONT, 1, 256>, 1, 256);
-		} else {
-			launch(i8_quantize_kernel<TYPE, FRONT, 1, 1024>, 1, 1024);
-		}
-	} else if (steps <= 64) {
-		launch(i8_quantize_kernel<TYPE, FRONT, 4, 64>, 4, 64);
+	// Few rows: all of a row at once; many: fewer threads to a row, so that more rows are under way.  us: 13 x 8192 bf16 3.8 by 1024 threads, 5.0 by 256; 8192 x 8192 bf16 behind a norm 71 by four
+	// rows of 256 threads to a workgroup, 58 by one; silu of 512 x 14336 bf16 18.1 and 13.7 (by 1024).
+	if (steps <= 64) {
+		launch(i8_quantize_kernel<TYPE, FRONT, 256, 1>, 256);
+	} else if (in.rows <= 1024) {
+		launch(i8_quantize_kernel<TYPE, FRONT, 1024, 1>, 1024);
+	} else if (steps <= 128) {
+		launch(i8_quantize_kernel<TYPE, FRONT, 256, 2>, 256);
 	} else {
-		launch(i8_quantize_kernel<TYPE, FRONT, 4, 256>, 4, 256);
+		launch(i8_quantize_kernel<TYPE, FRONT, 256, 4>, 256);
 	}
 	return hipGetLastError();
 }

@@ -85,9 +85,9 @@ struct i8_step {
 		}
 	}
 };
-// 1 / rms of a row as the norm wants it
-__device__ __forceinline__ float i8_rms(double sum, int k, float eps) {
-	return static_cast<float>(1.0 / sqrt(sum / k + static_cast<double>(eps)));
+// 1 / rms of a row as the norm wants it, from the sum of its squares and 1 / k
+__device__ __forceinline__ float i8_rms(double sum, double part, float eps) {
+	return static_cast<float>(rsqrt(fma(sum, part, static_cast<double>(eps))));
 }
 
 } // namespace nh
