@@ -26,14 +26,36 @@ template<int TYPE> struct i8_store {
 		}
 	}
 
-	// A lane has four neighbouring n of sixteen different rows m: sixteen rows at a time go through LDS, so that a wave's stores run along the rows.  Pieces of four values lie at
-	// places permuted by the row, which spreads them over the banks either way.
-	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f* scratch) const {
-		constexpr int PIECES = 4 * FN; // of a row
+	// A lane has four neighbouring n of sixteen different rows m: sixteen rows at a time go through LDS, so that a wave's loads and stores run along the rows, four values to a lane if N is a multiple of
+	// four (ALONG = 4), else one.  Pieces of four values lie at places permuted by the row, which spreads them over the banks either way.  The residual of the next sixteen rows is on its
+	// way while these are stored (y may be the residual: a row's is loaded before any of that row is stored).
+	template<int FN, int FM, int ALONG> __device__ __forceinline__ void along_rows(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f* scratch) const {
+		constexpr int PIECES = 4 * FN, LANES = 16 * FN / ALONG < 64 ? 16 * FN / ALONG : 64, ROWS = 64 / LANES, TIMES = 16 / ROWS, ACROSS = 16 * FN / (LANES * ALONG);
 		const int lane = threadIdx.x & 63, row = lane & 15;
-		const bool fours = (N & 3) == 0; // then four neighbours lie together in y
+		const int c0 = ALONG * (lane % LANES), r0 = lane / LANES; // this lane's first column and row when it moves values
+		struct values {
+			value v[ALONG];
+		};
+		constexpr int SETS = FN < 8 ? 2 : 1; // (in the largest tiles the sums leave no room for two)
+		values add[SETS][TIMES][ACROSS] = {};
+		auto fetch = [&](int i, values(&to)[TIMES][ACROSS]) { // (past the end: the last ones, for nothing)
+#pragma unroll
+			for (int t = 0; t < TIMES; ++t) {
+#pragma unroll
+				for (int c = 0; c < ACROSS; ++c) {
+					const int64_t m = min(m0 + 16 * i + r0 + ROWS * t, M - 1), n = min(n0 + c0 + LANES * ALONG * c, N - ALONG);
+					__builtin_memcpy(&to[t][c], __builtin_assume_aligned(residual + m * N + n, sizeof(values)), sizeof(values));
+				}
+			}
+		};
+		if (residual && SETS == 2) {
+			fetch(0, add[0]);
+		}
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
+			if (residual && SETS == 1) {
+				fetch(i, add[0]);
+			}
 			const int m	   = m0 + 16 * i;
 			const float sx = m + row < M ? x.scale[m + row] : 0.0f;
 #pragma unroll
@@ -47,46 +69,35 @@ template<int TYPE> struct i8_store {
 				}
 				scratch[row * PIECES + (piece ^ (row % PIECES))] = v;
 			}
+			if (residual && SETS == 2 && i + 1 < FM) {
+				fetch(i + 1, add[(i + 1) % SETS]);
+			}
 			__builtin_amdgcn_wave_barrier(); // (one wave's own LDS accesses are in order)
-			if (fours) {
-				constexpr int AT_ONCE = 64 / PIECES; // rows
 #pragma unroll
-				for (int r0 = 0; r0 < 16; r0 += AT_ONCE) {
-					const int r = r0 + lane / PIECES, piece = lane % PIECES, n = n0 + 4 * piece;
-					v4f v = scratch[r * PIECES + (piece ^ (r % PIECES))];
-					if (m + r < M && n < N) {
-						const int64_t at = static_cast<int64_t>(m + r) * N + n;
-						value out[4];
-						if (residual) {
-							__builtin_memcpy(out, __builtin_assume_aligned(residual + at, 4 * sizeof(value)), sizeof(out));
+			for (int t = 0; t < TIMES; ++t) {
 #pragma unroll
-							for (int e = 0; e < 4; ++e) {
-								v[e] += T::widen(out[e]);
-							}
-						}
+				for (int c = 0; c < ACROSS; ++c) {
+					const int r = r0 + ROWS * t, at = c0 + LANES * ALONG * c;
+					const v4f four = scratch[r * PIECES + ((at >> 2) ^ (r % PIECES))];
+					values out;
 #pragma unroll
-						for (int e = 0; e < 4; ++e) {
-							out[e] = T::narrow(v[e]);
-						}
-						__builtin_memcpy(__builtin_assume_aligned(y + at, 4 * sizeof(value)), out, sizeof(out));
+					for (int e = 0; e < ALONG; ++e) {
+						const float v = ALONG == 4 ? four[e] : (at & 2) ? (at & 1) ? four[3] : four[2] : (at & 1) ? four[1] : four[0];
+						out.v[e]	  = T::narrow(residual ? v + T::widen(add[i % SETS][t][c].v[e]) : v);
 					}
-				}
-			} else {
-				constexpr int LANES = 16 * FN < 64 ? 16 * FN : 64, AT_ONCE = 64 / LANES;
-#pragma unroll
-				for (int r0 = 0; r0 < 16; r0 += AT_ONCE) {
-					const int r = r0 + lane / LANES;
-#pragma unroll
-					for (int c = lane % LANES; c < 16 * FN; c += LANES) {
-						float v = scratch[r * PIECES + ((c >> 2) ^ (r % PIECES))][c & 3];
-						if (m + r < M && n0 + c < N) {
-							const int64_t at = static_cast<int64_t>(m + r) * N + n0 + c;
-							y[at]			 = T::narrow(residual ? v + T::widen(residual[at]) : v);
-						}
+					if (m + r < M && n0 + at < N) {
+						__builtin_memcpy(__builtin_assume_aligned(y + static_cast<int64_t>(m + r) * N + n0 + at, sizeof(values)), &out, sizeof(values));
 					}
 				}
 			}
 			__builtin_amdgcn_wave_barrier();
+		}
+	}
+	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f* scratch) const {
+		if ((N & 3) == 0) {
+			along_rows<FN, FM, 4>(sums, n0, m0, w, x, scratch);
+		} else {
+			along_rows<FN, FM, 1>(sums, n0, m0, w, x, scratch);
 		}
 	}
 };
