@@ -45,7 +45,7 @@ int nh_i8_untile(const void* tiled, int8_t* q, float* scales, int64_t rows, int6
 /* y [M][N] of `type` = x . w^T + residual (NULL: none; [M][N] of the same type, may be y itself): the whole-number sum over K brought to fp32, times x's scale, times w's, plus the residual, rounded
  * once.  y has no byte in common with w or x, nor with the residual unless it is the same buffer (not checked). */
 int nh_i8_gemm(const void* w_tiled, const void* x_tiled, const void* residual, void* y, int type, int64_t M, int64_t N, int64_t K, void* stream);
-/* quantize (norm_weight not NULL: rms_norm_quantize) and gemm; x and y of the same type.  workspace: nh_i8_mul_mat_workspace_bytes(M, K) bytes; one row of up
+/* quantize (norm_weight not NULL: rms_norm_quantize) and gemm; x and y of the same type.  workspace: nh_i8_mul_mat_workspace_bytes(M, K) bytes; one row of up to
  * 16384 values is quantized inside the product's launch and needs none (0, and the pointer may be NULL). */
 int64_t nh_i8_mul_mat_workspace_bytes(int64_t M, int64_t K);
 int nh_i8_mul_mat(const void* w_tiled, const void* x, int type, int64_t x_stride, const float* norm_weight, float eps, const void* residual, void* y, int64_t M, int64_t N, int64_t K,

@@ -130,7 +130,7 @@ int nh_i8_gemm(const void* w_tiled, const void* x_tiled, const void* residual, v
 
 int64_t nh_i8_mul_mat_workspace_bytes(int64_t M, int64_t K) {
 	const int64_t bytes = nh_i8_tiled_bytes(M, K);
-	return bytes > 0 && nh::i8_token_fits(M, K) ? 0 : bytes;
+	return bytes > 0 && M == 1 && nh::i8_token_fits(1, 1, K, false) ? 0 : bytes; // (N and the norm are not known here)
 }
 int nh_i8_mul_mat(const void* w_tiled, const void* x, int type, int64_t x_stride, const float* norm_weight, float eps, const void* residual, void* y, int64_t M, int64_t N, int64_t K,
 	void* workspace, int64_t workspace_bytes, void* stream) {
@@ -144,12 +144,12 @@ int nh_i8_mul_mat(const void* w_tiled, const void* x, int type, int64_t x_stride
 	NH_REQUIRE(w_tiled && y, NH_ERR_NULL_POINTER);
 	NH_REQUIRE(aligned16(w_tiled) && aligned16(y) && aligned16(residual) && aligned16(norm_weight), NH_ERR_ALIGNMENT);
 	NH_TRY(check_workspace(workspace, workspace_bytes, nh_i8_mul_mat_workspace_bytes(M, K)));
-	if (nh::i8_token_fits(M, K)) {
+	if (nh::i8_token_fits(M, N, K, norm_weight != nullptr)) {
 		NH_TRY(require_device());
 		nh::i8_rows in{};
-		in.x = x, in.norm = norm_weight, in.eps = eps;
+		in.x = x, in.norm = norm_weight, in.eps = eps, in.stride = x_stride;
 		in.part = 1.0 / static_cast<double>(K);
-		in.rows = 1, in.k = static_cast<int>(K);
+		in.rows = static_cast<int>(M), in.k = static_cast<int>(K);
 		return from_hip(nh::launch_i8_token(nh::i8_view(w_tiled, N, K), in, type, residual, y, as_stream(stream)));
 	}
 	NH_TRY(quantize(x, nullptr, norm_weight, eps, norm_weight ? nh::I8_NORM : nh::I8_PLAIN, type, x_stride, 0, workspace, M, K, stream));

@@ -88,8 +88,8 @@ hipError_t launch_i8_untile(const void* tiled, int8_t* q, float* scales, int64_t
 // y [M][N] of `type` = x . w^T (+ residual), x [M][K], w [N][K]
 hipError_t launch_i8_gemm(const i8_matrix& w, const i8_matrix& x, const void* residual, void* y, int type, hipStream_t stream);
 
-// The same for one row that is quantized in the call: whether there is such a form, and it.
-bool i8_token_fits(int64_t m, int64_t k);
+// The same for a row, or a few, quantized in the launch: whether it is for these sizes, and it.
+bool i8_token_fits(int64_t m, int64_t n, int64_t k, bool norm);
 hipError_t launch_i8_token(const i8_matrix& w, const i8_rows& in, int type, const void* residual, void* y, hipStream_t stream);
 
 struct i8_losses {

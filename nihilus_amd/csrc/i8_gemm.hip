@@ -102,27 +102,31 @@ template<int TYPE> struct i8_store {
 	}
 };
 
-// One row, quantized inside (behind the norm if there is one): every workgroup brings the whole row to 8 bits in LDS by itself, which takes less than a launch of its own and the wait for it, while the
-// first of its weights are on their way.  Then as i8_rows_product for one strip of x, all of whose rows are this one.  PIECES: of eight values per thread, so K up to 4096 PIECES.
-constexpr int TOKEN_STEPS = 256; // K up to 16384
-template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(512) void i8_token_product(i8_matrix w, const void* x, const float* norm, double part, float eps, int K, int n_tiles, i8_store<TYPE> epi) {
+// Up to ROWS rows, quantized inside (behind the norm if there is one): every workgroup brings the rows to 8 bits in LDS by itself, which takes less than a launch of its own and the wait for it, while
+// the first of its weights are on their way.  Then as i8_rows_product for one strip of x, whose other rows repeat the last one.  PIECES: of eight values per thread, so K up to 4096 PIECES.
+template<int TYPE, bool NORM, int ROWS, int PIECES, int FN> __global__ __launch_bounds__(512) void i8_token_product(i8_matrix w, const void* x, const float* norm, double part, float eps, int K, int64_t stride, int n_tiles,
+	i8_store<TYPE> epi) {
 	constexpr int WAVES = 8, AHEAD = 8 / FN;
-	__shared__ v4u row[PIECES * 256]; // [step][16 values]
+	__shared__ v4u row[PIECES * 256 * ROWS]; // [step][16 values][row]
 	__shared__ v4i parts[WAVES][FN][64];
-	__shared__ double squares[WAVES];
-	__shared__ uint32_t tops[WAVES];
+	__shared__ double squares[ROWS][WAVES];
+	__shared__ uint32_t tops[ROWS][WAVES];
+	__shared__ float scales[I8_ROWS];
 	const i8_place p = i8_place_of(n_tiles, 1);
 	if (!p.there) {
 		return;
 	}
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 	const int pieces = 8 * w.steps;
-	float v[PIECES][8];
+	float v[ROWS][PIECES][8];
 #pragma unroll
-	for (int j = 0; j < PIECES; ++j) {
-		const int c = threadIdx.x + 512 * j;
-		if (c < pieces) {
-			i8_load<TYPE>(x, 8 * c, K - 8 * c, v[j]);
+	for (int i = 0; i < ROWS; ++i) {
+#pragma unroll
+		for (int j = 0; j < PIECES; ++j) {
+			const int c = threadIdx.x + 512 * j;
+			if (c < pieces) {
+				i8_load<TYPE>(x, min(i, epi.M - 1) * stride + 8 * c, K - 8 * c, v[i][j]);
+			}
 		}
 	}
 	const int n_strip = p.n * FN;
@@ -144,30 +148,37 @@ template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(5
 	};
 	load(begin);
 	if constexpr (NORM) {
-		double sum = 0.0;
+		double sum[ROWS] = {};
 #pragma unroll
-		for (int j = 0; j < PIECES; ++j) {
-			if (threadIdx.x + 512 * j < static_cast<unsigned>(pieces)) {
+		for (int i = 0; i < ROWS; ++i) {
 #pragma unroll
-				for (int e = 0; e < 8; ++e) {
-					sum = fma(static_cast<double>(v[j][e]), static_cast<double>(v[j][e]), sum);
+			for (int j = 0; j < PIECES; ++j) {
+				if (threadIdx.x + 512 * j < static_cast<unsigned>(pieces)) {
+#pragma unroll
+					for (int e = 0; e < 8; ++e) {
+						sum[i] = fma(static_cast<double>(v[i][j][e]), static_cast<double>(v[i][j][e]), sum[i]);
+					}
 				}
 			}
-		}
 #pragma unroll
-		for (int d = 32; d > 0; d >>= 1) {
-			sum += __shfl_xor(sum, d);
-		}
-		if (lane == 0) {
-			squares[wave] = sum;
+			for (int d = 32; d > 0; d >>= 1) {
+				sum[i] += __shfl_xor(sum[i], d);
+			}
+			if (lane == 0) {
+				squares[i][wave] = sum[i];
+			}
 		}
 		__syncthreads();
-		sum = squares[0];
+		float r[ROWS];
 #pragma unroll
-		for (int i = 1; i < WAVES; ++i) {
-			sum += squares[i];
+		for (int i = 0; i < ROWS; ++i) {
+			sum[i] = squares[i][0];
+#pragma unroll
+			for (int u = 1; u < WAVES; ++u) {
+				sum[i] += squares[i][u];
+			}
+			r[i] = i8_rms(sum[i], part, eps);
 		}
-		const float r = i8_rms(sum, part, eps);
 #pragma unroll
 		for (int j = 0; j < PIECES; ++j) {
 			const int c = threadIdx.x + 512 * j;
@@ -175,47 +186,62 @@ template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(5
 				float g[8];
 				i8_load<NH_F32>(norm, 8 * c, K - 8 * c, g);
 #pragma unroll
-				for (int e = 0; e < 8; ++e) {
-					v[j][e] = __fmul_rn(__fmul_rn(v[j][e], r), g[e]);
+				for (int i = 0; i < ROWS; ++i) {
+#pragma unroll
+					for (int e = 0; e < 8; ++e) {
+						v[i][j][e] = __fmul_rn(__fmul_rn(v[i][j][e], r[i]), g[e]);
+					}
 				}
 			}
 		}
 	}
-	uint32_t top = 0;
 #pragma unroll
-	for (int j = 0; j < PIECES; ++j) {
-		if (threadIdx.x + 512 * j < static_cast<unsigned>(pieces)) {
+	for (int i = 0; i < ROWS; ++i) {
+		uint32_t top = 0;
 #pragma unroll
-			for (int e = 0; e < 8; ++e) {
-				top = max(top, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
+		for (int j = 0; j < PIECES; ++j) {
+			if (threadIdx.x + 512 * j < static_cast<unsigned>(pieces)) {
+#pragma unroll
+				for (int e = 0; e < 8; ++e) {
+					top = max(top, __float_as_uint(v[i][j][e]) & 0x7FFFFFFFu);
+				}
 			}
 		}
-	}
 #pragma unroll
-	for (int d = 32; d > 0; d >>= 1) {
-		top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
-	}
-	if (lane == 0) {
-		tops[wave] = top;
+		for (int d = 32; d > 0; d >>= 1) {
+			top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
+		}
+		if (lane == 0) {
+			tops[i][wave] = top;
+		}
 	}
 	__syncthreads();
+	float scale = 0.0f; // of the only row
 #pragma unroll
-	for (int i = 0; i < WAVES; ++i) {
-		top = max(top, tops[i]);
-	}
-	const i8_step step(top);
+	for (int i = 0; i < ROWS; ++i) {
+		uint32_t top = tops[i][0];
 #pragma unroll
-	for (int j = 0; j < PIECES; ++j) {
-		const int c = threadIdx.x + 512 * j;
-		if (c < pieces) {
-			uint32_t out[2];
-			step.round(v[j], out);
-			reinterpret_cast<v2u*>(row)[c] = v2u{ out[0], out[1] };
+		for (int u = 1; u < WAVES; ++u) {
+			top = max(top, tops[i][u]);
+		}
+		const i8_step step(top);
+		scale = step.scale;
+		if (ROWS > 1 && threadIdx.x == 0) {
+			scales[i] = scale;
+		}
+#pragma unroll
+		for (int j = 0; j < PIECES; ++j) {
+			const int c = threadIdx.x + 512 * j;
+			if (c < pieces) {
+				uint32_t out[2];
+				step.round(v[i][j], out);
+				reinterpret_cast<v2u*>(row)[((c >> 1) * ROWS + i) * 2 + (c & 1)] = v2u{ out[0], out[1] };
+			}
 		}
 	}
 	__syncthreads();
 	v4i sums[FN][1] = {};
-	const v4u* b = row + (lane >> 4);
+	const v4u* b = row + (lane >> 4) * ROWS + min(lane & 15, ROWS - 1);
 #pragma unroll 1
 	for (int s = begin; s < end;) {
 #pragma unroll
@@ -223,7 +249,7 @@ template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(5
 			if (s + u < end) {
 #pragma unroll
 				for (int f = 0; f < FN; ++f) {
-					sums[f][0] = i8_mfma(ahead[u][f], b[4 * (s + u)], sums[f][0]);
+					sums[f][0] = i8_mfma(ahead[u][f], b[4 * ROWS * (s + u)], sums[f][0]);
 				}
 			}
 		}
@@ -243,7 +269,13 @@ template<int TYPE, bool NORM, int PIECES, int FN> __global__ __launch_bounds__(5
 		for (int i = 1; i < WAVES; ++i) {
 			all += parts[i][wave][lane];
 		}
-		epi.token(all, (n_strip + wave) * I8_ROWS, step.scale, w);
+		if constexpr (ROWS == 1) {
+			epi.token(all, (n_strip + wave) * I8_ROWS, scale, w);
+		} else {
+			const v4i only[1][1] = { { all } };
+			const i8_matrix there{ nullptr, scales, epi.M, 1, w.steps };
+			epi.template operator()<1, 1>(only, (n_strip + wave) * I8_ROWS, 0, w, there, reinterpret_cast<v4f*>(&parts[0][wave][0]));
+		}
 	}
 }
 
@@ -254,26 +286,37 @@ template<int TYPE> hipError_t gemm(const i8_matrix& w, const i8_matrix& x, const
 	return hipGetLastError();
 }
 
-template<int TYPE> hipError_t token(const i8_matrix& w, const i8_rows& in, const void* residual, void* y, hipStream_t stream) {
+template<int TYPE, bool NORM> hipError_t token(const i8_matrix& w, const i8_rows& in, const void* residual, void* y, hipStream_t stream) {
 	typedef typename i8_type<TYPE>::store value;
-	const i8_store<TYPE> epi{ static_cast<value*>(y), static_cast<const value*>(residual), 1, w.rows };
+	const i8_store<TYPE> epi{ static_cast<value*>(y), static_cast<const value*>(residual), in.rows, w.rows };
 	auto launch = [&](auto kernel, int n_strips) {
 		const int n_tiles = (w.strips + n_strips - 1) / n_strips;
-		kernel<<<i8_grid(n_tiles, 1), 512, 0, stream>>>(w, in.x, in.norm, in.part, in.eps, in.k, n_tiles, epi);
+		kernel<<<i8_grid(n_tiles, 1), 512, 0, stream>>>(w, in.x, in.norm, in.part, in.eps, in.k, in.stride, n_tiles, epi);
 	};
-	const bool one = w.steps <= 64, few = w.strips <= 512;
-	if (in.norm) {
-		one ? few ? launch(i8_token_product<TYPE, true, 1, 1>, 1) : launch(i8_token_product<TYPE, true, 1, 2>, 2) : few ? launch(i8_token_product<TYPE, true, 4, 1>, 1) : launch(i8_token_product<TYPE, true, 4, 2>, 2);
+	const bool few = w.strips <= 512; // so that there are workgroups for all CUs
+	if (in.rows > 2) {
+		if constexpr (!NORM) {
+			few ? launch(i8_token_product<TYPE, false, 4, 1, 1>, 1) : launch(i8_token_product<TYPE, false, 4, 1, 2>, 2);
+		}
+	} else if (in.rows == 2) {
+		few ? launch(i8_token_product<TYPE, NORM, 2, 2, 1>, 1) : launch(i8_token_product<TYPE, NORM, 2, 2, 2>, 2);
+	} else if (w.steps <= 64) {
+		few ? launch(i8_token_product<TYPE, NORM, 1, 1, 1>, 1) : launch(i8_token_product<TYPE, NORM, 1, 1, 2>, 2);
 	} else {
-		one ? few ? launch(i8_token_product<TYPE, false, 1, 1>, 1) : launch(i8_token_product<TYPE, false, 1, 2>, 2) : few ? launch(i8_token_product<TYPE, false, 4, 1>, 1) : launch(i8_token_product<TYPE, false, 4, 2>, 2);
+		few ? launch(i8_token_product<TYPE, NORM, 1, 4, 1>, 1) : launch(i8_token_product<TYPE, NORM, 1, 4, 2>, 2);
 	}
 	return hipGetLastError();
+}
+template<int TYPE> hipError_t token(const i8_matrix& w, const i8_rows& in, const void* residual, void* y, hipStream_t stream) {
+	return in.norm ? token<TYPE, true>(w, in, residual, y, stream) : token<TYPE, false>(w, in, residual, y, stream);
 }
 
 } // namespace
 
-bool i8_token_fits(int64_t m, int64_t k) {
-	return m == 1 && i8_steps(k) <= TOKEN_STEPS;
+// Measured, us as here / as two launches, fp32: one row of 4096 against 1024 rows of w 3.5 / 6.4, 4096 5.0 / 8.2, 14336 10.8 / 13.9, 128256 83 / 83; two rows 4096 6.7 / 8.3, 32768 25.8 / 29.4, 65536 47.7 / 48.7, behind
+// a norm 50.5 / 50; four rows 4096 7.6 / 8.4, 14336 11.6 / 14.0, 32768 28.8 / 29.6, 65536 52 / 49, behind a norm 4096 9.6 / 9.3.
+bool i8_token_fits(int64_t m, int64_t n, int64_t k, bool norm) {
+	return (m == 1 && k <= 16384) || (n <= 32768 && ((m == 2 && k <= 8192) || (m > 2 && m <= 4 && k <= 4096 && !norm)));
 }
 hipError_t launch_i8_token(const i8_matrix& w, const i8_rows& in, int type, const void* residual, void* y, hipStream_t stream) {
 	return type == NH_F32 ? token<NH_F32>(w, in, residual, y, stream) : type == NH_F16 ? token<NH_F16>(w, in, residual, y, stream) : token<NH_BF16>(w, in, residual, y, stream);

@@ -174,12 +174,11 @@ __global__ __launch_bounds__(256) void i8_tile_kernel(const int8_t* q, const flo
 	const int lane	  = i & 63;
 	const int64_t row = (i >> 6) / steps * I8_ROWS + (lane & 15), at = (i >> 6) % steps * I8_STEP + 16 * (lane >> 4);
 	uint32_t word[4]  = {};
-	if (row < rows) {
-#pragma unroll
-		for (int j = 0; j < 16; ++j) {
-			if (at + j < k) {
-				word[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(q[row * k + at + j])) << (8 * (j % 4));
-			}
+	if (row < rows && at + 16 <= k) {
+		__builtin_memcpy(word, q + row * k + at, 16);
+	} else if (row < rows) {
+		for (int j = 0; at + j < k; ++j) {
+			word[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(q[row * k + at + j])) << (8 * (j % 4));
 		}
 	}
 	out[i] = v4u{ word[0], word[1], word[2], word[3] };
@@ -197,10 +196,14 @@ __global__ __launch_bounds__(256) void i8_untile_kernel(const v4u* in, const flo
 	const int64_t row = (i >> 6) / steps * I8_ROWS + (lane & 15), at = (i >> 6) % steps * I8_STEP + 16 * (lane >> 4);
 	if (row < rows) {
 		const v4u v = in[i];
+		if (at + 16 <= k) {
+			__builtin_memcpy(q + row * k + at, &v, 16);
+		} else {
 #pragma unroll
-		for (int j = 0; j < 16; ++j) {
-			if (at + j < k) {
-				q[row * k + at + j] = static_cast<int8_t>(v[j / 4] >> (8 * (j % 4)));
+			for (int j = 0; j < 16; ++j) {
+				if (at + j < k) {
+					q[row * k + at + j] = static_cast<int8_t>(v[j / 4] >> (8 * (j % 4)));
+				}
 			}
 		}
 	}

@@ -184,7 +184,7 @@ def test_sums_up_to_the_last_bit(i8, m):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (1, 14336, 4096), (1, 77, 100), (1, 1, 1), (1, 33, 63), (1, 1000, 4097), (1, 500, 16384), (1, 515, 14336), (1, 9000, 8191), (1, 100, 16385), (1, 20, 5000), (2, 1000, 4096), (4, 515, 1507), (5, 64, 64), (13, 8192, 8192), (117, 1000, 512), (600, 13000, 96)])
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (1, 14336, 4096), (1, 77, 100), (1, 1, 1), (1, 33, 63), (1, 1000, 4097), (1, 500, 16384), (1, 515, 14336), (1, 9000, 8191), (1, 100, 16385), (1, 20, 5000), (2, 1000, 4096), (2, 33, 8191), (2, 9001, 8192), (2, 300, 8193), (3, 1001, 4095), (4, 515, 1507), (4, 9004, 4096), (4, 40, 4097), (5, 64, 64), (13, 8192, 8192), (117, 1000, 512), (600, 13000, 96)])
 def test_mul_mat_is_quantize_and_gemm(i8, m, n, k, kind):
     g = _gen(m + n + k)
     wq, ws = _matrix(g, n, k)

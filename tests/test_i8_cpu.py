@@ -24,7 +24,7 @@ def test_every_declared_function_is_exported_and_bound(lib):
     assert names == sorted(_lib.I8_SIGNATURES) and all(hasattr(lib, n) for n in names)
 
 
-@pytest.mark.parametrize("rows,k", [(0, 1), (1, 1), (16, 64), (17, 65), (128256, 4096), (4096, 14336)])
+@pytest.mark.parametrize("rows,k", [(0, 1), (1, 1), (1, 16385), (2, 8192), (2, 8193), (3, 4096), (4, 4097), (5, 64), (16, 64), (17, 65), (128256, 4096), (4096, 14336)])
 def test_bytes_of_a_tiled_matrix(lib, rows, k):
     strips = (rows + 15) // 16
     assert lib.nh_i8_tiled_bytes(rows, k) == strips * ((k + 63) // 64 * 1024 + 64)
@@ -59,7 +59,7 @@ def _calls(lib):
         "tile": (lib.nh_i8_tile, [P, P, P, 2, 64, None], [0, 1, 2]),
         "untile": (lib.nh_i8_untile, [P, P, P, 2, 64, None], [0, 1, 2]),
         "gemm": (lib.nh_i8_gemm, [P, P, None, P, 0, 2, 32, 64, None], [0, 1, 3]),
-        "mul_mat": (lib.nh_i8_mul_mat, [P, P, 0, 64, None, 0.0, None, P, 2, 32, 64, P, 1 << 20, None], [0, 1, 7, 11]),
+        "mul_mat": (lib.nh_i8_mul_mat, [P, P, 0, 64, None, 0.0, None, P, 5, 32, 64, P, 1 << 20, None], [0, 1, 7, 11]),
         "losses": (lib.nh_i8_token_losses, [P, P, P, P, P, 2, 32, 64, P, 1 << 20, None], [0, 1, 2, 3, 4, 8]),
         "grad": (lib.nh_i8_token_losses_grad, [P, P, P, P, P, None, P, 0, 2, 32, 64, P, 1 << 30, None], [0, 1, 2, 3, 4, 6, 11]),
     }
@@ -120,7 +120,7 @@ def test_types_and_eps(lib):
 
 
 def test_a_workspace_that_is_too_small(lib):
-    assert _call(lib, "mul_mat", a12=lib.nh_i8_mul_mat_workspace_bytes(2, 64) - 1) == -6
+    assert _call(lib, "mul_mat", a12=lib.nh_i8_mul_mat_workspace_bytes(5, 64) - 1) == -6
     assert _call(lib, "losses", a9=lib.nh_i8_token_losses_workspace_bytes(2, 32) - 1) == -6
     assert _call(lib, "grad", a12=lib.nh_i8_token_losses_grad_workspace_bytes(2, 32, 64, 0) - 1) == -6
 
