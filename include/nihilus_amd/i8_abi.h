@@ -18,6 +18,7 @@
  * Quantizing a row of fp32 values v:  scale = fp32(max |v| / 127),  q = the whole number nearest to v / scale (the true quotient), ties to even, within +-127.  A row of
  * zeros has scale 0 and q = 0.  A row that has an infinity or NaN has scale NaN and q = 0: what is formed from it is NaN.
  *
+ * What a call writes (results, workspace) has no byte in common with what it reads or with anything else that it writes, but for a result that is the residual itself (NH_ERR_ARGUMENT).
  * Limits (NH_ERR_TOO_LARGE): rows up to 2^22, K up to 131008 (a sum of K products stays below 2^31), a matrix up to 32 GiB, ceil(M / 256) ceil(N / 256) up to 2^22.  Pointers are 16-byte aligned, or where noted only as their type.
  */
 #ifndef NIHILUS_AMD_I8_ABI_H
@@ -43,7 +44,7 @@ int nh_i8_tile(const int8_t* q, const float* scales, void* tiled, int64_t rows, 
 int nh_i8_untile(const void* tiled, int8_t* q, float* scales, int64_t rows, int64_t k, void* stream);
 
 /* y [M][N] of `type` = x . w^T + residual (NULL: none; [M][N] of the same type, may be y itself): the whole-number sum over K brought to fp32, times x's scale, times w's, plus the residual, rounded
- * once.  y has no byte in common with w or x, nor with the residual unless it is the same buffer (not checked). */
+ * once. */
 int nh_i8_gemm(const void* w_tiled, const void* x_tiled, const void* residual, void* y, int type, int64_t M, int64_t N, int64_t K, void* stream);
 /* quantize (norm_weight not NULL: rms_norm_quantize) and gemm; x and y of the same type.  workspace: nh_i8_mul_mat_workspace_bytes(M, K) bytes; one row of up to
  * 16384 values is quantized inside the product's launch and needs none (0, and the pointer may be NULL). */
@@ -54,12 +55,12 @@ int nh_i8_mul_mat(const void* w_tiled, const void* x, int type, int64_t x_stride
 /* Softmax cross entropy of rows x [M][K] on an output projection w [N][K]:  l[m][n] = the product above in fp32,
  *   lse[m] = log sum_n exp l[m][n],   losses[m] = lse[m] - l[m][targets[m]],  0 where targets[m] (int32) is outside [0, N): such a row is not scored.
  * The logits are formed a tile at a time and not kept. */
-int64_t nh_i8_token_losses_workspace_bytes(int64_t M, int64_t N);
+int64_t nh_i8_token_losses_workspace_bytes(int64_t M, int64_t N, int64_t K); /* up to about 64 MiB, whatever M is, unless N is far past a million */
 int nh_i8_token_losses(const void* w_tiled, const void* x_tiled, const int32_t* targets, float* losses, float* lse, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* The gradient of sum_m grad[m] losses[m] (grad fp32 [M]; NULL: ones) with respect to what the rows of x stand for:
  *   dx[m][k] = grad[m] sum_n (exp(l[m][n] - lse[m]) - [n = targets[m]]) w[n][k],  zero for rows that are not scored;  dx [M][K] of `type`, rounded once.
- * losses and lse as nh_i8_token_losses gave them.  The slopes are formed again from x and w, so many of the vocabulary at a time that they stay below 128 MiB (or a piece of 1024), and enter the
+ * losses and lse as nh_i8_token_losses gave them.  The slopes are formed again from x and w, for 8192 rows at a time and so much of the vocabulary that they stay below 128 MiB, and enter the
  * second product as fp16 numbers below a power of two of the row's own: one (11 bits) where dx is of 16 bits, a sum of two (22 bits) where it is of 32. */
 int64_t nh_i8_token_losses_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int type);
 int nh_i8_token_losses_grad(const void* w_tiled, const void* x_tiled, const int32_t* targets, const float* losses, const float* lse, const float* grad, void* dx, int type, int64_t M, int64_t N,

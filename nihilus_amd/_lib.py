@@ -101,7 +101,7 @@ I8_SIGNATURES = {
     "nh_i8_gemm": (_int, [_vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp]),
     "nh_i8_mul_mat_workspace_bytes": (_i64, [_i64, _i64]),
     "nh_i8_mul_mat": (_int, [_vp, _vp, _int, _i64, _vp, C.c_float, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
-    "nh_i8_token_losses_workspace_bytes": (_i64, [_i64, _i64]),
+    "nh_i8_token_losses_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "nh_i8_token_losses": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp]),
     "nh_i8_token_losses_grad_workspace_bytes": (_i64, [_i64, _i64, _i64, _int]),
     "nh_i8_token_losses_grad": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _vp, _i64, _vp]),

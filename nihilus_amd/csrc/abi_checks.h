@@ -12,6 +12,11 @@ namespace nh {
 inline bool aligned16(const void* p) {
 	return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
+// whether two pieces of memory (of at least a byte each) have one in common
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+	const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+	return a && b && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
 inline hipStream_t as_stream(void* s) {
 	return static_cast<hipStream_t>(s);
 }

@@ -15,6 +15,7 @@ namespace {
 using nh::aligned16;
 using nh::as_stream;
 using nh::from_hip;
+using nh::overlap;
 using nh::require_device;
 
 // row, token and tile numbers are 32-bit inside the kernels, with room for sums of two
@@ -59,10 +60,6 @@ inline int check_rows(const nh_attn_cache* c, int type, int64_t rows, int64_t he
 	NH_REQUIRE(stride >= heads * c->head_dim && stride <= (int64_t{ 1 } << 40), NH_ERR_SHAPE);
 	NH_REQUIRE(stride * value_bytes(type) % 16 == 0, NH_ERR_ALIGNMENT);
 	return NH_OK;
-}
-inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-	const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-	return a && b && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
 }
 // bytes that rows of a stride reach over
 inline int64_t span(int64_t rows, int64_t heads, int64_t head_dim, int64_t stride, int type) {

@@ -95,9 +95,10 @@ hipError_t launch_i8_token(const i8_matrix& w, const i8_rows& in, int type, cons
 struct i8_losses {
 	const int32_t* targets;
 	float *losses, *lse;
+	int k;
 	void* workspace;
 };
-int64_t i8_losses_workspace(int64_t m, int64_t n);
+int64_t i8_losses_workspace(int64_t m, int64_t n, int64_t k);
 hipError_t launch_i8_losses(const i8_matrix& w, const i8_matrix& x, const i8_losses& l, hipStream_t stream);
 
 struct i8_gradient {

@@ -324,10 +324,11 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 	static_assert(LOADS >= 2 && STEPS == WAVES); // so that j is which strip of w, or P
 	const int whole = (w.strips >> 1) - a.first_block - begin; // blocks whose second strip there is; the last one's place meets zeros in P
 	auto load = [&](int s) {
+		const v4u* instead = from[0];
 #pragma unroll
 		for (int j = 0; j < LOADS + 1; ++j) {
 			if (j < LOADS || more) {
-				const v4u* at = j == 1 && s >= whole ? from[0] : from[j];
+				const v4u* at = j == 1 && s >= whole ? instead : from[j];
 				load_global_to_lds_b128(at, 16 * (j == 1 ? lane ^ 8 : lane), &ring[s % RING][j < LOADS ? wave + WAVES * j : WAVES * LOADS + wave][0]);
 				from[j] += j < 2 ? static_cast<int64_t>(2) * w.steps * 64 : 64;
 			}
@@ -471,7 +472,13 @@ template<int TYPE> __global__ __launch_bounds__(256) void i8_slope_results(const
 	}
 }
 
-// How the backward pass is cut: pieces of the vocabulary by memory, splits of a piece so that the second product has some 256 workgroups.
+// some of x's rows, from a multiple of sixteen on
+i8_matrix rows_of(const i8_matrix& x, int64_t first, int64_t rows) {
+	return { x.q + first / I8_ROWS * x.steps * 64, x.scale + first, static_cast<int>(rows), static_cast<int>(i8_strips(rows)), x.steps };
+}
+
+// How the backward pass is cut: 8192 rows at a time, whose sums are kept; pieces of the vocabulary, whose slopes are; splits of a piece, so that the second product has some 256 workgroups.
+constexpr int64_t GRADIENT_ROWS = 8192;
 struct gradient_plan {
 	int64_t piece, blocks; // n, blocks of 32 n
 	int64_t k_tiles, m_tiles, splits;
@@ -504,9 +511,10 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 		a.M = x.rows, a.columns = w.steps * I8_STEP, a.strips = x.strips, a.blocks = static_cast<int>(blocks), a.first_block = static_cast<int>(first / 32);
 		a.per = static_cast<int>((blocks + plan.splits - 1) / plan.splits);
 		a.add = first > 0;
-		const unsigned grid = i8_grid(plan.k_tiles * plan.splits, plan.m_tiles);
+		const int64_t m_tiles = (x.strips + plan.strips - 1) / plan.strips;
+		const unsigned grid	  = i8_grid(plan.k_tiles * plan.splits, m_tiles);
 		auto multiply = [&](auto kernel) {
-			kernel<<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(plan.m_tiles), static_cast<int>(plan.splits));
+			kernel<<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(m_tiles), static_cast<int>(plan.splits));
 		};
 		if (plan.strips == 8) {
 			multiply(i8_slope_kernel<8, TERMS>);
@@ -518,57 +526,89 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 	}
 }
 
+// Rows of the forward pass that go together: as many as leave 64 MiB of stretches, 256 at least.
+struct losses_plan {
+	i8_form form;
+	int64_t stretches, rows;
+};
+losses_plan plan_losses(int64_t m, int64_t n, int64_t k) {
+	losses_plan p{};
+	const int64_t shortest = (n + 31) / 32, some = std::max<int64_t>((int64_t{ 1 } << 26) / (8 * shortest) / 256 * 256, 256);
+	p.rows				   = std::min(m, std::max<int64_t>(some, 8192));
+	p.form				   = i8_form_for(i8_strips(n), i8_strips(p.rows), i8_steps(k));
+	p.stretches			   = (n + i8_stretch(p.form) - 1) / i8_stretch(p.form);
+	if (p.stretches * p.rows * 8 > (int64_t{ 1 } << 26) && some < p.rows) { // (a large vocabulary)
+		p.rows		= some;
+		p.form		= i8_form_for(i8_strips(n), i8_strips(p.rows), i8_steps(k));
+		p.stretches = (n + i8_stretch(p.form) - 1) / i8_stretch(p.form);
+	}
+	return p;
+}
+
 } // namespace
 
-// (K is not known here: room for the shortest stretches)
-int64_t i8_losses_workspace(int64_t m, int64_t n) {
-	return up(m * 4, 256) + up((n + 31) / 32 * m * 8, 256);
+int64_t i8_losses_workspace(int64_t m, int64_t n, int64_t k) {
+	const losses_plan p = plan_losses(m, n, k);
+	return up(p.rows * 4, 256) + up(p.stretches * p.rows * 8, 256);
 }
 
 hipError_t launch_i8_losses(const i8_matrix& w, const i8_matrix& x, const i8_losses& l, hipStream_t stream) {
-	char* ws		   = static_cast<char*>(l.workspace);
-	float* hit		   = reinterpret_cast<float*>(ws);
-	float2* parts	   = reinterpret_cast<float2*>(ws + up(static_cast<int64_t>(x.rows) * 4, 256));
-	const i8_form form = i8_form_for(w.strips, x.strips, w.steps);
-	const int each	   = i8_stretch(form);
-	i8_launch_product<true>(form, w, x, 0, w.rows, i8_stretches{ parts, hit, l.targets, x.rows, w.rows }, stream);
-	if (x.rows <= 256) { // a workgroup to a row
-		i8_join_stretches<1><<<x.rows, 1024, 0, stream>>>(parts, hit, l.targets, l.losses, l.lse, x.rows, w.rows, (w.rows + each - 1) / each);
-	} else {
-		i8_join_stretches<8><<<(x.rows + 7) / 8, 1024, 0, stream>>>(parts, hit, l.targets, l.losses, l.lse, x.rows, w.rows, (w.rows + each - 1) / each);
+	const losses_plan plan = plan_losses(x.rows, w.rows, l.k);
+	char* ws			   = static_cast<char*>(l.workspace);
+	float* hit			   = reinterpret_cast<float*>(ws);
+	float2* parts		   = reinterpret_cast<float2*>(ws + up(plan.rows * 4, 256));
+	const int stretches	   = static_cast<int>(plan.stretches);
+	for (int64_t first = 0; first < x.rows; first += plan.rows) { // (the last of them may be fewer, and are cut as the others)
+		const i8_matrix some	= rows_of(x, first, std::min<int64_t>(plan.rows, x.rows - first));
+		const int32_t* targets	= l.targets + first;
+		float *losses = l.losses + first, *lse = l.lse + first;
+		i8_launch_product<true>(plan.form, w, some, 0, w.rows, i8_stretches{ parts, hit, targets, some.rows, w.rows }, stream);
+		if (some.rows <= 256) { // a workgroup to a row
+			i8_join_stretches<1><<<some.rows, 1024, 0, stream>>>(parts, hit, targets, losses, lse, some.rows, w.rows, stretches);
+		} else {
+			i8_join_stretches<8><<<(some.rows + 7) / 8, 1024, 0, stream>>>(parts, hit, targets, losses, lse, some.rows, w.rows, stretches);
+		}
 	}
 	return hipGetLastError();
 }
 
 int64_t i8_gradient_workspace(int64_t m, int64_t n, int64_t k, int type) {
-	const gradient_plan g = plan_gradient(m, n, k, type);
+	const gradient_plan g = plan_gradient(std::min(m, GRADIENT_ROWS), n, k, type);
 	return MAXIMA * 4 + g.slopes + g.sums;
 }
 
-hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_gradient& g, hipStream_t stream) {
-	const gradient_plan plan = plan_gradient(x.rows, w.rows, g.k, g.type);
-	char* ws				 = static_cast<char*>(g.workspace);
-	float* maxima			 = reinterpret_cast<float*>(ws);
-	v8h* slopes				 = reinterpret_cast<v8h*>(ws + MAXIMA * 4);
-	float* sums				 = reinterpret_cast<float*>(ws + MAXIMA * 4 + plan.slopes);
+hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_gradient& all, hipStream_t stream) {
+	char* ws	  = static_cast<char*>(all.workspace);
+	float* maxima = reinterpret_cast<float*>(ws);
+	v8h* slopes	  = reinterpret_cast<v8h*>(ws + MAXIMA * 4);
 	i8_largest_scales<<<MAXIMA, 256, 0, stream>>>(w.scale, w.rows, maxima);
-	if (plan.terms == 2) {
-		gradient_sums<2>(w, x, g, plan, slopes, sums, maxima, stream);
-	} else {
-		gradient_sums<1>(w, x, g, plan, slopes, sums, maxima, stream);
-	}
-	const int columns = w.steps * I8_STEP;
-	const unsigned beside = static_cast<unsigned>(std::min(x.rows, 64));
-	const dim3 grid((x.rows + beside - 1) / beside, beside, static_cast<unsigned>((g.k + 1023) / 1024));
-	auto results = [&](auto kernel, auto* dx) {
-		kernel<<<grid, 256, 0, stream>>>(sums, maxima, g.targets, g.losses, g.grad, dx, x.rows, w.rows, g.k, columns, static_cast<int>(plan.splits));
-	};
-	if (g.type == NH_F32) {
-		results(i8_slope_results<NH_F32>, static_cast<float*>(g.dx));
-	} else if (g.type == NH_F16) {
-		results(i8_slope_results<NH_F16>, static_cast<uint16_t*>(g.dx));
-	} else {
-		results(i8_slope_results<NH_BF16>, static_cast<uint16_t*>(g.dx));
+	const gradient_plan most = plan_gradient(std::min<int64_t>(x.rows, GRADIENT_ROWS), w.rows, all.k, all.type);
+	float* sums				 = reinterpret_cast<float*>(ws + MAXIMA * 4 + most.slopes);
+	for (int64_t first = 0; first < x.rows; first += GRADIENT_ROWS) {
+		const i8_matrix some = rows_of(x, first, std::min<int64_t>(GRADIENT_ROWS, x.rows - first));
+		i8_gradient g		 = all;
+		g.targets += first, g.losses += first, g.lse += first;
+		g.grad = all.grad ? all.grad + first : nullptr;
+		g.dx   = static_cast<char*>(all.dx) + first * all.k * (all.type == NH_F32 ? 4 : 2);
+		// (fewer rows behind others are cut as those are, which is what there is room for)
+		if (most.terms == 2) {
+			gradient_sums<2>(w, some, g, most, slopes, sums, maxima, stream);
+		} else {
+			gradient_sums<1>(w, some, g, most, slopes, sums, maxima, stream);
+		}
+		const int columns	  = w.steps * I8_STEP;
+		const unsigned beside = static_cast<unsigned>(std::min(some.rows, 64));
+		const dim3 grid((some.rows + beside - 1) / beside, beside, static_cast<unsigned>((g.k + 1023) / 1024));
+		auto results = [&](auto kernel, auto* dx) {
+			kernel<<<grid, 256, 0, stream>>>(sums, maxima, g.targets, g.losses, g.grad, dx, some.rows, w.rows, g.k, columns, static_cast<int>(most.splits));
+		};
+		if (g.type == NH_F32) {
+			results(i8_slope_results<NH_F32>, static_cast<float*>(g.dx));
+		} else if (g.type == NH_F16) {
+			results(i8_slope_results<NH_F16>, static_cast<uint16_t*>(g.dx));
+		} else {
+			results(i8_slope_results<NH_BF16>, static_cast<uint16_t*>(g.dx));
+		}
 	}
 	return hipGetLastError();
 }

@@ -551,7 +551,7 @@ PyObject* i8_token_losses(args& in) {
 	if (!in.good || targets->dim() != 1 || targets->device() != w->device()) {
 		return nullptr;
 	}
-	const int64_t m = targets->size(0), need = nh_i8_token_losses_workspace_bytes(m, n);
+	const int64_t m = targets->size(0), need = nh_i8_token_losses_workspace_bytes(m, n, k);
 	void* s = stream();
 	if (need < 0 || !i8_operands(*w, *xq, m, n, k) || (need > 0 && !own_memory(s))) {
 		return nullptr;

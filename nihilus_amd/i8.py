@@ -185,7 +185,7 @@ def token_losses(w: torch.Tensor, xq: torch.Tensor, targets: torch.Tensor, n: in
     """Softmax cross entropy of tiled rows [m, k] on a tiled projection [n, k]: (losses, lse), fp32 [m]; targets int32 [m], rows with a target outside [0, n) are not
     scored: their loss is 0.  lse is the log of the sum of the exponentials; the log-probability of a row's target is -loss.
 
-    workspace: nh_i8_token_losses_workspace_bytes(m, n) bytes; without one the call has its own."""
+    workspace: nh_i8_token_losses_workspace_bytes(m, n, k) bytes; without one the call has its own."""
     if workspace is None and _calls is not None:
         r = _native(_calls.i8_token_losses(w, xq, targets, n, k), "nh_i8_token_losses")
         if r is not None:
@@ -197,7 +197,7 @@ def token_losses(w: torch.Tensor, xq: torch.Tensor, targets: torch.Tensor, n: in
     _tiled(w, w.device, n, k, "w")
     _tiled(xq, w.device, m, k, "xq")
     losses, lse = (torch.empty(m, dtype=torch.float32, device=w.device) for _ in range(2))
-    workspace, ws, ws_bytes = _workspace(workspace, _need("nh_i8_token_losses_workspace_bytes", m, n), w.device)
+    workspace, ws, ws_bytes = _workspace(workspace, _need("nh_i8_token_losses_workspace_bytes", m, n, k), w.device)
     _call("nh_i8_token_losses", w.device, w.data_ptr(), xq.data_ptr(), targets.data_ptr(), losses.data_ptr(), lse.data_ptr(), m, n, k, ws, ws_bytes)
     return losses, lse
 

@@ -318,6 +318,21 @@ def test_pieces_of_the_vocabulary_and_splits(i8):
     assert ((dx[some].double() - R.gradient(l, targets[some], wq, ws)).abs() <= R.gradient_bound(l, targets[some], wq, ws, torch.float32)).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(8200, 600, 64), (16500, 40, 130), (9001, 130000, 64)])
+def test_rows_so_many_that_they_go_in_parts(i8, m, n, k):
+    wq, ws, xq, xs, targets = _loss_case(i8, m, n, k)
+    w, x = i8.tile(wq, ws), i8.tile(xq, xs)
+    losses, lse = i8.token_losses(w, x, targets, n, k)
+    grad = torch.rand(m, device="cuda", generator=_gen(3))
+    dx = i8.token_losses_grad(w, x, targets, losses, lse, n, k, grad=grad, dtype=torch.bfloat16)
+    some = torch.cat([torch.arange(0, m, 211, device="cuda"), torch.arange(8180, 8200, device="cuda"), torch.arange(m - 10, m, device="cuda")])
+    l = R.logits(wq, ws, xq[some], xs[some])
+    want, want_lse = R.losses(l, targets[some])
+    assert ((lse[some].double() - want_lse).abs() <= R.lse_bound(l)).all()
+    assert ((losses[some].double() - want).abs() <= R.lse_bound(l) + R.logit_bound(l) + 4 * R.U * want.abs()).all()
+    assert ((dx[some].double() - R.gradient(l, targets[some], wq, ws, grad[some])).abs() <= R.gradient_bound(l, targets[some], wq, ws, torch.bfloat16, grad[some])).all()
+
+
 # ---- as they are used
 
 

@@ -7,6 +7,7 @@ import torch
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 P = 0x10000  # a pointer that nothing follows
+Q = [P << (4 * i) for i in range(8)]  # ... and others far from it
 
 
 @pytest.fixture(scope="module")
@@ -35,33 +36,34 @@ def test_bytes_of_a_tiled_matrix(lib, rows, k):
 def test_sizes_that_are_refused(lib):
     assert lib.nh_i8_tiled_bytes(-1, 64) == -3 and lib.nh_i8_tiled_bytes(1, 0) == -3 and lib.nh_i8_tiled_bytes(1, -5) == -3
     assert lib.nh_i8_tiled_bytes((1 << 22) + 1, 64) == -5 and lib.nh_i8_tiled_bytes(1, 131009) == -5 and lib.nh_i8_tiled_bytes(1 << 22, 131008) == -5
-    assert lib.nh_i8_token_losses_workspace_bytes(1 << 22, 1 << 22) == -5 and lib.nh_i8_token_losses_workspace_bytes(-1, 4) == -3
+    assert lib.nh_i8_token_losses_workspace_bytes(1 << 22, 1 << 22, 64) == -5 and lib.nh_i8_token_losses_workspace_bytes(-1, 4, 64) == -3
     assert lib.nh_i8_token_losses_grad_workspace_bytes(4, 4, 64, 3) == -6 and lib.nh_i8_token_losses_grad_workspace_bytes(4, 4, 0, 0) == -3
     assert lib.nh_i8_token_losses_grad_workspace_bytes(0, 4, 64, 0) == 0
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 128256, 4096), (2048, 128256, 4096), (65, 1000, 64), (1 << 20, 1000, 64), (1, 1 << 22, 64)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 128256, 4096), (2048, 128256, 4096), (65, 1000, 64), (100000, 128256, 4096), (1 << 20, 1000, 64), (1, 1 << 22, 64)])
 def test_a_workspace_holds_no_logits(lib, m, n, k):
-    # slopes of some of the vocabulary at a time (128 MiB, or 1024 tokens of all rows), and sums of which there are at most 256 tiles
+    # stretches of 64 MiB; slopes of 128 MiB, or of 1024 tokens for 8192 rows, and sums of at most 256 tiles of 512 x 128, or one set for 8192 rows
     for kind, terms in ((0, 2), (1, 1), (2, 1)):
         need = lib.nh_i8_token_losses_grad_workspace_bytes(m, n, k, kind)
-        rows = (m + 15) // 16 * 16
-        assert 0 < need <= max(2 * (1 << 27), rows * 2048 * terms) + max(256 * 256 * 256 * 4, (m + 256) * (k + 64) * 4) + 4096
-    assert lib.nh_i8_token_losses_workspace_bytes(m, n) <= m * 4 + 256 + (n // 32 + 1) * m * 8 + 256
+        rows = min((m + 15) // 16 * 16, 8192)
+        assert 0 < need <= max(1 << 27, rows * 2048 * terms) + max(256 * 512 * 128 * 4, rows * (k + 64) * 4) + 4096
+    assert lib.nh_i8_token_losses_workspace_bytes(m, n, k) <= (1 << 26) + 4 * min(m, 1 << 21) + 4096
 
 
 def _calls(lib):
     """name -> (function, good arguments, which are pointers)"""
+    a, b, c, d, e, f, g, _ = Q
     return {
-        "quantize": (lib.nh_i8_quantize, [P, 0, 64, P, 2, 64, None], [0, 3]),
-        "norm": (lib.nh_i8_rms_norm_quantize, [P, 0, 64, P, 1e-5, P, 2, 64, None], [0, 3, 5]),
-        "silu": (lib.nh_i8_silu_mul_quantize, [P, P, 0, 64, 64, P, 2, 64, None], [0, 1, 5]),
-        "tile": (lib.nh_i8_tile, [P, P, P, 2, 64, None], [0, 1, 2]),
-        "untile": (lib.nh_i8_untile, [P, P, P, 2, 64, None], [0, 1, 2]),
-        "gemm": (lib.nh_i8_gemm, [P, P, None, P, 0, 2, 32, 64, None], [0, 1, 3]),
-        "mul_mat": (lib.nh_i8_mul_mat, [P, P, 0, 64, None, 0.0, None, P, 5, 32, 64, P, 1 << 20, None], [0, 1, 7, 11]),
-        "losses": (lib.nh_i8_token_losses, [P, P, P, P, P, 2, 32, 64, P, 1 << 20, None], [0, 1, 2, 3, 4, 8]),
-        "grad": (lib.nh_i8_token_losses_grad, [P, P, P, P, P, None, P, 0, 2, 32, 64, P, 1 << 30, None], [0, 1, 2, 3, 4, 6, 11]),
+        "quantize": (lib.nh_i8_quantize, [a, 0, 64, b, 2, 64, None], [0, 3]),
+        "norm": (lib.nh_i8_rms_norm_quantize, [a, 0, 64, c, 1e-5, b, 2, 64, None], [0, 3, 5]),
+        "silu": (lib.nh_i8_silu_mul_quantize, [a, c, 0, 64, 64, b, 2, 64, None], [0, 1, 5]),
+        "tile": (lib.nh_i8_tile, [a, c, b, 2, 64, None], [0, 1, 2]),
+        "untile": (lib.nh_i8_untile, [b, a, c, 2, 64, None], [0, 1, 2]),
+        "gemm": (lib.nh_i8_gemm, [a, c, None, b, 0, 2, 32, 64, None], [0, 1, 3]),
+        "mul_mat": (lib.nh_i8_mul_mat, [a, c, 0, 64, None, 0.0, None, b, 5, 32, 64, d, 1 << 20, None], [0, 1, 7, 11]),
+        "losses": (lib.nh_i8_token_losses, [a, b, c, d, e, 2, 32, 64, f, 1 << 20, None], [0, 1, 2, 3, 4, 8]),
+        "grad": (lib.nh_i8_token_losses_grad, [a, b, c, d, e, None, f, 0, 2, 32, 64, g, 1 << 30, None], [0, 1, 2, 3, 4, 6, 11]),
     }
 
 
@@ -85,7 +87,7 @@ def test_a_pointer_that_is_not_there(lib, name):
 @pytest.mark.parametrize("name,at", [("quantize", 0), ("quantize", 3), ("norm", 3), ("norm", 5), ("silu", 1), ("silu", 5), ("tile", 1), ("tile", 2), ("untile", 0), ("gemm", 0), ("gemm", 1), ("gemm", 2), ("gemm", 3),
                                      ("mul_mat", 0), ("mul_mat", 1), ("mul_mat", 4), ("mul_mat", 6), ("mul_mat", 7), ("mul_mat", 11), ("losses", 1), ("losses", 2), ("losses", 3), ("losses", 8), ("grad", 5), ("grad", 6), ("grad", 11)])
 def test_a_pointer_that_is_not_aligned(lib, name, at):
-    assert _call(lib, name, **{f"a{at}": P + 2}) == -2
+    assert _call(lib, name, **{f"a{at}": Q[7] + 2}) == -2
 
 
 # (rows, k) of the quantizers, (M, N, K) of the products
@@ -121,8 +123,26 @@ def test_types_and_eps(lib):
 
 def test_a_workspace_that_is_too_small(lib):
     assert _call(lib, "mul_mat", a12=lib.nh_i8_mul_mat_workspace_bytes(5, 64) - 1) == -6
-    assert _call(lib, "losses", a9=lib.nh_i8_token_losses_workspace_bytes(2, 32) - 1) == -6
+    assert _call(lib, "losses", a9=lib.nh_i8_token_losses_workspace_bytes(2, 32, 64) - 1) == -6
     assert _call(lib, "grad", a12=lib.nh_i8_token_losses_grad_workspace_bytes(2, 32, 64, 0) - 1) == -6
+
+
+# name -> which arguments are written, which are read
+USES = {"quantize": ([3], [0]), "norm": ([5], [0, 3]), "silu": ([5], [0, 1]), "tile": ([2], [0, 1]), "untile": ([1, 2], [0]), "gemm": ([3], [0, 1]), "mul_mat": ([7, 11], [0, 1]), "losses": ([3, 4, 8], [0, 1, 2]),
+        "grad": ([6, 11], [0, 1, 2, 3, 4])}
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_results_over_what_is_read_or_over_each_other(lib, name):
+    args, (written, read) = _calls(lib)[name][1], USES[name]
+    for i, w in enumerate(written):
+        for other in read + written[:i]:
+            assert _call(lib, name, **{f"a{w}": args[other]}) == -6, (w, other)
+    if name in ("gemm", "mul_mat"):  # the residual: the result itself, or apart from it
+        at, y = (2, 3) if name == "gemm" else (6, 7)
+        assert _call(lib, name, **{f"a{at}": args[y] + 16}) == -6 and _call(lib, name, **{f"a{at}": args[y] - 16}) == -6
+    if name == "mul_mat":
+        assert _call(lib, name, a6=args[11]) == -6 and _call(lib, name, a4=args[7]) == -6
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="would run")
