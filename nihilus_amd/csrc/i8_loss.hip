@@ -273,16 +273,15 @@ __device__ __forceinline__ v2i i8_columns(const v4u* first, const v4u* second, i
 	return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(const_cast<char*>(at)));
 }
 // ... as fp16: 128 + q as the low byte of 0x6400 + ... is the fp16 number 1024 + 128 + q
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ v4h i8_halves(int raw) {
+	const uint32_t u = static_cast<uint32_t>(raw) ^ 0x80808080u;
+	const v2h low = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)), high = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
+	const v2h a = low - static_cast<_Float16>(1152.0f), b = high - static_cast<_Float16>(1152.0f);
+	return v4h{ a[0], a[1], b[0], b[1] };
+}
 __device__ __forceinline__ v8h i8_halves(v2i raw) {
-	v8h out;
-#pragma unroll
-	for (int d = 0; d < 2; ++d) {
-		const uint32_t u = static_cast<uint32_t>(raw[d]) ^ 0x80808080u;
-		const v2h low = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)), high = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u));
-		const v2h a = low - static_cast<_Float16>(1152.0f), b = high - static_cast<_Float16>(1152.0f);
-		out[4 * d] = a[0], out[4 * d + 1] = a[1], out[4 * d + 2] = b[0], out[4 * d + 3] = b[1];
-	}
-	return out;
+	return __builtin_shufflevector(i8_halves(raw[0]), i8_halves(raw[1]), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 struct i8_slope_product {
@@ -448,20 +447,157 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 	}
 }
 
-// the splits' sums, brought back from the powers of two, times the row's grad
-template<int TYPE> __global__ __launch_bounds__(256) void i8_slope_results(const float* sums, const float* maxima, const int32_t* targets, const float* losses, const float* grad,
-	typename i8_type<TYPE>::store* dx, int M, int N, int K, int columns, int splits) {
+// Few rows (up to 16) of up to 512 STEPS values: logits, slopes and their product with w in one pass over w, by 16 tokens (a strip) at a time.  A wave has 64 STEPS of the columns to itself: its part of a strip
+// comes by direct transfers into LDS that is its own, two strips ahead, and is used there twice, for the wave's part of the logits and, after all waves' parts have been added up, for its
+// columns of the sums, which stay in registers over all of the workgroup's strips.  One barrier a strip.  Bound by memory: w is read once (5 rows of 128256 x 4096, fp32: 95
+// us, 175 as two products).
+template<int TERMS, int STEPS> __global__ __launch_bounds__(512, 2) void i8_few_slopes(i8_matrix w, i8_matrix x, const int32_t* targets, const float* losses, const float* lse, const float* maxima, float* out) {
+	constexpr int WAVES = 8, SCALES = 4;
+	__shared__ v4u strip[WAVES][2][STEPS][64];
+	__shared__ v4i parts[2][WAVES][64];
+	__shared__ v4f scales[SCALES][64]; // of a strip: the first four
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 4, m = lane & 15;
+	const int step0 = wave * STEPS, mine = max(0, min(STEPS, w.steps - step0)); // this wave's steps of K
+	const int M = x.rows, N = w.rows;
 	const int f = scales_exponent(maxima);
-	const int m = blockIdx.x * gridDim.y + blockIdx.y, k = 4 * (blockIdx.z * 256 + threadIdx.x);
-	if (m >= M || k >= K) {
+	// rows of the odd sixteens of columns lie eight further, so that the lanes of a transposing read that are served together meet no bank twice
+	const int turned = lane ^ ((lane & 16) >> 1);
+	v4u xs[STEPS];
+#pragma unroll
+	for (int s = 0; s < STEPS; ++s) {
+		xs[s] = s < mine ? x.q[(step0 + s) * 64 + lane] : v4u{};
+	}
+	const int target  = m < M ? targets[m] : -1;
+	const bool scored = target >= 0 && target < N;
+	const float sx = scored ? x.scale[m] : 0.0f, below = scored ? lse[m] : 0.0f;
+	const float lift = scored ? ldexpf(1.0f, slopes_exponent(losses[m])) : 0.0f;
+	const int stride = gridDim.x, count = (w.strips - static_cast<int>(blockIdx.x) + stride - 1) / stride; // strips of this workgroup
+	asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (from here on only transfers are counted)
+	auto load = [&](int b) {
+		const int at = static_cast<int>(blockIdx.x) + b * stride;
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			load_global_to_lds_b128(w.q + (static_cast<int64_t>(at) * w.steps + min(step0 + s, w.steps - 1)) * 64, 16 * turned, &strip[wave][b & 1][s][0]);
+		}
+		if (wave == 0) {
+			load_global_to_lds_b128(w.scale + 16 * at, 16 * min(lane, 3), &scales[b % SCALES][0]);
+		}
+	};
+	constexpr int ALL = 15 | (7 << 4) | (3 << 14); // s_waitcnt: lgkmcnt(0) alone
+	auto landed = [&](bool another) { // the strip is there; the next one may be on its way
+		asm volatile("" ::: "memory");
+		if (!another) {
+			__builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (15 << 8));
+		} else if (wave == 0) {
+			__builtin_amdgcn_s_waitcnt(((STEPS + 1) & 15) | (7 << 4) | (15 << 8));
+		} else {
+			__builtin_amdgcn_s_waitcnt((STEPS & 15) | (7 << 4) | (15 << 8));
+		}
+		asm volatile("" ::: "memory");
+	};
+	v4f sums[STEPS][4] = {};
+	load(0);
+	if (count > 1) {
+		load(1);
+	}
+	for (int b = 0; b < count; ++b) {
+		const auto& here = strip[wave][b & 1];
+		landed(b + 1 < count);
+		v4i part[2] = {};
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) { // (x is zero past K)
+			part[s & 1] = i8_mfma(here[s][turned], xs[s], part[s & 1]);
+		}
+		parts[b & 1][wave][lane] = part[0] + part[1];
+		asm volatile("" ::: "memory");
+		__builtin_amdgcn_s_waitcnt(ALL);
+		__builtin_amdgcn_s_barrier();
+		asm volatile("" ::: "memory");
+		v4i all = parts[b & 1][0][lane];
+#pragma unroll
+		for (int u = 1; u < WAVES; ++u) {
+			all += parts[b & 1][u][lane];
+		}
+		const v4f sw = scales[b % SCALES][group];
+		const int n	 = 16 * (static_cast<int>(blockIdx.x) + b * stride) + 4 * group;
+		v4h p[TERMS];
+#pragma unroll
+		for (int e = 0; e < 4; ++e) {
+			const float l = static_cast<float>(all[e]) * sx * sw[e];
+			float v		  = exp2_native((l - below) * LOG2_E) - (scored && n + e == target ? 1.0f : 0.0f);
+			v			  = n + e < N ? v * (ldexpf(sw[e], f) * lift) : 0.0f;
+#pragma unroll
+			for (int t = 0; t < TERMS; ++t) {
+				p[t][e] = static_cast<_Float16>(v);
+				v -= static_cast<float>(p[t][e]);
+			}
+		}
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			v2i raw[2];
+#pragma unroll
+			for (int h = 0; h < 2; ++h) { // columns 32 h .. + 15 and + 16 .. + 31 of the step, rows 4 group + i of each
+				const int j = (lane & 15) >> 1, c = 2 * h + (j >> 2), row = (4 * group + (j & 3)) ^ (8 * (j >> 2));
+				const char* at = reinterpret_cast<const char*>(&here[s][0]) + (c * 16 + row) * 16 + 8 * (lane & 1);
+				raw[h]		   = __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i*)(const_cast<char*>(at)));
+			}
+#pragma unroll
+			for (int c = 0; c < 4; ++c) {
+				const v4h k = i8_halves(raw[c >> 1][c & 1]);
+#pragma unroll
+				for (int t = TERMS - 1; t >= 0; --t) {
+					sums[s][c] = __builtin_amdgcn_mfma_f32_16x16x16f16(k, p[t], sums[s][c], 0, 0, 0);
+				}
+			}
+		}
+		if (b + 2 < count) { // what this strip lay in is this wave's own, and has been read
+			asm volatile("" ::: "memory");
+			__builtin_amdgcn_s_waitcnt(ALL);
+			load(b + 2);
+		}
+	}
+	if (m < M) {
+#pragma unroll
+		for (int s = 0; s < STEPS; ++s) {
+			if (s < mine) {
+#pragma unroll
+				for (int c = 0; c < 4; ++c) {
+					*reinterpret_cast<v4f*>(out + (static_cast<int64_t>(blockIdx.x) * M + m) * (w.steps * I8_STEP) + 64 * (step0 + s) + 16 * c + 4 * group) = sums[s][c];
+				}
+			}
+		}
+	}
+}
+
+// the splits' sums, brought back from the powers of two, times the row's grad; LANES threads to four columns
+template<int TYPE, int LANES> __global__ __launch_bounds__(256) void i8_slope_results(const float* sums, const float* maxima, const int32_t* targets, const float* losses, const float* grad,
+	typename i8_type<TYPE>::store* dx, int M, int N, int K, int columns, int splits) {
+	__shared__ v4f others[LANES][256 / LANES];
+	const int f = scales_exponent(maxima);
+	const int col = threadIdx.x % (256 / LANES), part = threadIdx.x / (256 / LANES);
+	const int m = blockIdx.x * gridDim.y + blockIdx.y, k = 4 * (blockIdx.z * (256 / LANES) + col);
+	const bool there = m < M && k < K;
+	v4f all{};
+	if (there) {
+#pragma unroll 8
+		for (int s = part; s < splits; s += LANES) {
+			all += *reinterpret_cast<const v4f*>(sums + (static_cast<int64_t>(s) * M + m) * columns + k);
+		}
+	}
+	if constexpr (LANES > 1) {
+		others[part][col] = all;
+		__syncthreads();
+		if (part == 0) {
+#pragma unroll
+			for (int i = 1; i < LANES; ++i) {
+				all += others[i][col];
+			}
+		}
+	}
+	if (!there || part > 0) {
 		return;
 	}
 	const bool scored = targets[m] >= 0 && targets[m] < N;
-	v4f all{};
-#pragma unroll 8
-	for (int s = 0; s < splits; ++s) {
-		all += *reinterpret_cast<const v4f*>(sums + (static_cast<int64_t>(s) * M + m) * columns + k);
-	}
 	const int back	= scored ? -f - slopes_exponent(losses[m]) : 0;
 	const float g	= grad ? grad[m] : 1.0f;
 #pragma unroll
@@ -484,11 +620,18 @@ struct gradient_plan {
 	int64_t k_tiles, m_tiles, splits;
 	int64_t slopes, sums; // bytes
 	int strips, terms; // strips of rows in a tile
+	bool few; // one pass
 };
 gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k, int type) {
 	gradient_plan g{};
 	const int64_t strips = i8_strips(m), steps = i8_steps(k);
 	g.terms				 = type == NH_F32 ? 2 : 1;
+	g.few				 = strips == 1 && steps <= 64;
+	if (g.few) { // a workgroup to a CU, or to a strip
+		g.splits = std::min<int64_t>(256, i8_strips(n));
+		g.sums	 = up(g.splits * m * steps * I8_STEP * 4, 256);
+		return g;
+	}
 	const int64_t row	 = strips * 16 * 2 * g.terms;
 	g.piece				 = std::min(up(n, 32), std::max<int64_t>((int64_t{ 1 } << 27) / row / 256 * 256, 1024));
 	g.blocks			 = g.piece / 32;
@@ -502,6 +645,13 @@ gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k, int type) {
 }
 
 template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, const i8_gradient& g, const gradient_plan& plan, v8h* slopes, float* sums, const float* maxima, hipStream_t stream) {
+	if (plan.few) {
+		auto launch = [&](auto kernel) {
+			kernel<<<static_cast<unsigned>(plan.splits), 512, 0, stream>>>(w, x, g.targets, g.losses, g.lse, maxima, sums);
+		};
+		w.steps <= 16 ? launch(i8_few_slopes<TERMS, 2>) : w.steps <= 32 ? launch(i8_few_slopes<TERMS, 4>) : launch(i8_few_slopes<TERMS, 8>);
+		return;
+	}
 	for (int64_t first = 0; first < w.rows; first += plan.piece) {
 		const int64_t n = std::min<int64_t>(plan.piece, w.rows - first), blocks = (n + 31) / 32;
 		const i8_slopes<TERMS> epi{ slopes, g.targets, g.losses, g.lse, maxima, x.rows, w.rows, static_cast<int>(first), static_cast<int>(blocks) };
@@ -598,16 +748,18 @@ hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_g
 		}
 		const int columns	  = w.steps * I8_STEP;
 		const unsigned beside = static_cast<unsigned>(std::min(some.rows, 64));
-		const dim3 grid((some.rows + beside - 1) / beside, beside, static_cast<unsigned>((g.k + 1023) / 1024));
-		auto results = [&](auto kernel, auto* dx) {
-			kernel<<<grid, 256, 0, stream>>>(sums, maxima, g.targets, g.losses, g.grad, dx, some.rows, w.rows, g.k, columns, static_cast<int>(most.splits));
+		const bool many		  = most.splits >= 32; // then sixteen threads to four columns
+		const int at_once	  = many ? 64 : 1024;
+		const dim3 grid((some.rows + beside - 1) / beside, beside, static_cast<unsigned>((g.k + at_once - 1) / at_once));
+		auto results = [&](auto one, auto sixteen, auto* dx) {
+			(many ? sixteen : one)<<<grid, 256, 0, stream>>>(sums, maxima, g.targets, g.losses, g.grad, dx, some.rows, w.rows, g.k, columns, static_cast<int>(most.splits));
 		};
 		if (g.type == NH_F32) {
-			results(i8_slope_results<NH_F32>, static_cast<float*>(g.dx));
+			results(i8_slope_results<NH_F32, 1>, i8_slope_results<NH_F32, 16>, static_cast<float*>(g.dx));
 		} else if (g.type == NH_F16) {
-			results(i8_slope_results<NH_F16>, static_cast<uint16_t*>(g.dx));
+			results(i8_slope_results<NH_F16, 1>, i8_slope_results<NH_F16, 16>, static_cast<uint16_t*>(g.dx));
 		} else {
-			results(i8_slope_results<NH_BF16>, static_cast<uint16_t*>(g.dx));
+			results(i8_slope_results<NH_BF16, 1>, i8_slope_results<NH_BF16, 16>, static_cast<uint16_t*>(g.dx));
 		}
 	}
 	return hipGetLastError();

@@ -214,7 +214,7 @@ def _loss_case(i8, m, n, k, seed=0, spread=1.0):
     return wq, ws, xq, xs, targets
 
 
-LOSSES = [(1, 1, 64), (1, 2, 1), (1, 1000, 64), (2, 33, 65), (3, 4097, 256), (16, 128, 100), (17, 5000, 130), (64, 250, 64), (65, 1003, 200), (130, 257, 64), (300, 2000, 128), (700, 9001, 64), (1, 128256, 512)]
+LOSSES = [(1, 1, 64), (1, 2, 1), (1, 1000, 64), (2, 33, 65), (3, 4097, 256), (16, 128, 100), (17, 5000, 130), (64, 250, 64), (65, 1003, 200), (130, 257, 64), (300, 2000, 128), (700, 9001, 64), (1, 128256, 512), (16, 6001, 1030), (9, 4099, 2050), (5, 4100, 4096), (4, 515, 3000)]
 
 
 @pytest.mark.parametrize("m,n,k", LOSSES)
