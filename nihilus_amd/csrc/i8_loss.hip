@@ -19,6 +19,8 @@ namespace nh {
 
 namespace {
 
+// ns that 256 x 256 exponentials take behind a product, with no other workgroup on the CU whose products would hide them
+constexpr int64_t EPILOGUE = 6000;
 constexpr float LOG2_E = 1.44269504088896340736f;
 
 // 2^x, within 2 ulp for the arguments here (x <= 0 up to rounding)
@@ -655,7 +657,7 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 	for (int64_t first = 0; first < w.rows; first += plan.piece) {
 		const int64_t n = std::min<int64_t>(plan.piece, w.rows - first), blocks = (n + 31) / 32;
 		const i8_slopes<TERMS> epi{ slopes, g.targets, g.losses, g.lse, maxima, x.rows, w.rows, static_cast<int>(first), static_cast<int>(blocks) };
-		i8_launch_product<true>(i8_form_for(i8_strips(n), x.strips, w.steps), w, x, static_cast<int>(first), static_cast<int>(n), epi, stream);
+		i8_launch_product<true>(i8_form_for(i8_strips(n), x.strips, w.steps, EPILOGUE), w, x, static_cast<int>(first), static_cast<int>(n), epi, stream);
 		i8_slope_product a{};
 		a.p = slopes, a.out = sums;
 		a.M = x.rows, a.columns = w.steps * I8_STEP, a.strips = x.strips, a.blocks = static_cast<int>(blocks), a.first_block = static_cast<int>(first / 32);
@@ -685,11 +687,11 @@ losses_plan plan_losses(int64_t m, int64_t n, int64_t k) {
 	losses_plan p{};
 	const int64_t shortest = (n + 31) / 32, some = std::max<int64_t>((int64_t{ 1 } << 26) / (8 * shortest) / 256 * 256, 256);
 	p.rows				   = std::min(m, std::max<int64_t>(some, 8192));
-	p.form				   = i8_form_for(i8_strips(n), i8_strips(p.rows), i8_steps(k));
+	p.form				   = i8_form_for(i8_strips(n), i8_strips(p.rows), i8_steps(k), EPILOGUE);
 	p.stretches			   = (n + i8_stretch(p.form) - 1) / i8_stretch(p.form);
 	if (p.stretches * p.rows * 8 > (int64_t{ 1 } << 26) && some < p.rows) { // (a large vocabulary)
 		p.rows		= some;
-		p.form		= i8_form_for(i8_strips(n), i8_strips(p.rows), i8_steps(k));
+		p.form		= i8_form_for(i8_strips(n), i8_strips(p.rows), i8_steps(k), EPILOGUE);
 		p.stretches = (n + i8_stretch(p.form) - 1) / i8_stretch(p.form);
 	}
 	return p;

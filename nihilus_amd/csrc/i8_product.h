@@ -257,7 +257,7 @@ enum i8_form { I8_ROWS_16, I8_ROWS_32, I8_TILE_64, I8_TILE_128_64, I8_TILE_128, 
 // workgroups as run at once, one to a CU, or two (then, if there are no more than 256, it is the `alone` ns).  Measured, us at [n x k], m rows (form chosen / next best / 256 x 256 tiles):
 // [4096 x 4096], 64: 6.4 / 8.9 / 46; 256: 10.2 / 12 / 47; 512: 14.9 / 16 / 47; 1024: 22.5 / 23.5 / 48; 2048: 36 / 36 / 50.  [14336 x 4096], 117: 14.6 / 15.7 / 47; 512: 33 / 34 / 49; 2048: 107 (256) / 126.
 // [4096 x 14336], 512: 35 / 43 / 138.  [5003 x 1507], 1001: 18 / 18 / 32.  [8192 x 8192], 8192: 392 (256) / 499.
-inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps) {
+inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t epilogue) {
 	if (m == 1) {
 		return I8_ROWS_16;
 	}
@@ -265,8 +265,8 @@ inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps) {
 		i8_form form;
 		int64_t n, m, at_once, step, alone, round;
 	};
-	constexpr shape shapes[] = { { I8_ROWS_32, 2, 2, 256, 53, 53, 1500 }, { I8_TILE_64, 4, 4, 512, 174, 100, 2500 }, { I8_TILE_128_64, 8, 4, 256, 145, 145, 2500 }, { I8_TILE_128, 8, 8, 512, 506, 290, 2500 },
-		{ I8_TILE_256, 16, 16, 256, 770, 770, 2500 } };
+	const shape shapes[] = { { I8_ROWS_32, 2, 2, 256, 53, 53, 1500 }, { I8_TILE_64, 4, 4, 512, 174, 100, 2500 }, { I8_TILE_128_64, 8, 4, 256, 145, 145, 2500 }, { I8_TILE_128, 8, 8, 512, 506, 290, 2500 },
+		{ I8_TILE_256, 16, 16, 256, 770, 770, 2500 + epilogue } };
 	i8_form best = I8_TILE_256;
 	int64_t least = INT64_MAX;
 	for (const shape& s : shapes) {

@@ -432,6 +432,43 @@ def test_weights_from_q8_0(i8, q8):
     assert torch.equal(q, want_q) and torch.equal(s, want_s)
 
 
+def test_the_native_calls_and_the_python_way(i8, monkeypatch):
+    assert i8._calls is not None
+    g = _gen(8)
+    m, n, k = 6, 90, 200
+    w, norm, r = i8.tile(*_matrix(g, n, k)), 1.0 + 0.1 * _normal(g, k), _normal(g, m, n, dtype=torch.float16)
+    wide = _normal(g, m, k + 7, dtype=torch.float16)
+    x = wide[:, 3 : k + 3]
+    targets, grad = torch.randint(0, n, (m,), device="cuda", dtype=torch.int32, generator=g), _normal(g, m)
+
+    def both(call):
+        out = []
+        for native in (i8._calls, None):
+            monkeypatch.setattr(i8, "_calls", native)
+            try:
+                out.append(call())
+            except Exception as e:  # noqa: BLE001
+                out.append((type(e), str(e)))
+        monkeypatch.undo()
+        return out
+
+    xq = i8.quantize(x)
+    losses, lse = i8.token_losses(w, xq, targets, n, k)
+    for call in (lambda: i8.untile(i8.quantize(x), m, k), lambda: i8.untile(i8.quantize(x[0]), 1, k), lambda: i8.untile(i8.rms_norm_quantize(x, norm, 1e-5), m, k), lambda: i8.untile(i8.silu_mul_quantize(x, x), m, k),
+                 lambda: (i8.gemm(w, xq, m, n, k, dtype=torch.bfloat16), i8.gemm(w, xq, m, n, k, dtype=torch.float16, residual=r)), lambda: (i8.mul_mat(w, x, n, k, residual=r), i8.mul_mat(w, x[:1], n, k, norm_weight=norm, eps=1e-5)),
+                 lambda: i8.token_losses(w, xq, targets, n, k), lambda: (i8.token_losses_grad(w, xq, targets, losses, lse, n, k, grad=grad), i8.token_losses_grad(w, xq, targets, losses, lse, n, k, dtype=torch.float16))):
+        native, python = both(call)
+        assert all(torch.equal(a, b) for a, b in zip(native, python))
+    for call in (lambda: i8.quantize(x.t()), lambda: i8.quantize(x.double()), lambda: i8.quantize(x.expand(3, m, k)), lambda: i8.quantize(x[:1].expand(3, k)), lambda: i8.rms_norm_quantize(x, norm[1:], 1e-5),
+                 lambda: i8.rms_norm_quantize(x, norm, -1.0), lambda: i8.silu_mul_quantize(x, x[1:]), lambda: i8.silu_mul_quantize(x, x.float()), lambda: i8.gemm(w[:-1], xq, m, n, k), lambda: i8.gemm(w, xq, m + 16, n, k),
+                 lambda: i8.gemm(w, xq, m, n, k, dtype=torch.float64), lambda: i8.gemm(w, xq, m, n, k, residual=r), lambda: i8.gemm(w, xq, m, n, 0), lambda: i8.mul_mat(w, x, n, k - 1), lambda: i8.mul_mat(w, x, n + 16, k),
+                 lambda: i8.mul_mat(w, x, n, k, residual=r[1:]), lambda: i8.token_losses(w, xq, targets.long(), n, k), lambda: i8.token_losses(w, xq, targets[None], n, k), lambda: i8.token_losses(w, xq[64:], targets, n, k),
+                 lambda: i8.token_losses_grad(w, xq, targets, losses[1:], lse, n, k), lambda: i8.token_losses_grad(w, xq, targets, losses, lse, n, k, grad=grad.double()),
+                 lambda: i8.token_losses_grad(w, xq, targets, losses, lse, n, k, dtype=torch.int32)):
+        native, python = both(call)
+        assert isinstance(native, tuple) and issubclass(native[0], Exception) and native == python, native
+
+
 def test_empty_calls(i8):
     w = i8.tile(*_matrix(_gen(1), 32, 64))
     x = torch.empty(0, 64, device="cuda")
