@@ -214,16 +214,16 @@ template<int TYPE, int FRONT> hipError_t quantize(const i8_rows& in, v4u* q, flo
 	auto launch			  = [&](auto kernel, int threads) {
 		kernel<<<blocks, threads, 0, stream>>>(in, q, scale, steps);
 	};
-	// Few rows: all of a row at once; many: fewer threads to a row, so that more rows are under way.  us: 13 x 8192 bf16 3.8 by 1024 threads, 5.0 by 256; 8192 x 8192 bf16 behind a norm 71 by four
-	// rows of 256 threads to a workgroup, 58 by one; silu of 512 x 14336 bf16 18.1 and 13.7 (by 1024).
+	// Few rows: more threads to a row; many: fewer, so that more rows are under way.  us: 13 x 8192 bf16 3.8 by 512 threads, 5.0 by 256; 8192 x 8192 bf16 behind a norm 58 by 256, 71 by four rows of 256 threads to
+	// a workgroup; silu of 512 x 14336 bf16 12.1 by 512 threads, 13.7 by 1024; of 8192 x 14336 128 by 256 threads, 169 by 1024.
 	if (steps <= 64) {
 		launch(i8_quantize_kernel<TYPE, FRONT, 256, 1>, 256);
-	} else if (in.rows <= 1024) {
-		launch(i8_quantize_kernel<TYPE, FRONT, 1024, 1>, 1024);
 	} else if (steps <= 128) {
-		launch(i8_quantize_kernel<TYPE, FRONT, 256, 2>, 256);
+		in.rows <= 1024 ? launch(i8_quantize_kernel<TYPE, FRONT, 512, 1>, 512) : launch(i8_quantize_kernel<TYPE, FRONT, 256, 2>, 256);
+	} else if (steps <= 256) {
+		in.rows <= 1024 ? launch(i8_quantize_kernel<TYPE, FRONT, 512, 2>, 512) : launch(i8_quantize_kernel<TYPE, FRONT, 256, 4>, 256);
 	} else {
-		launch(i8_quantize_kernel<TYPE, FRONT, 256, 4>, 256);
+		launch(i8_quantize_kernel<TYPE, FRONT, 512, 4>, 512);
 	}
 	return hipGetLastError();
 }

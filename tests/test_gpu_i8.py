@@ -33,7 +33,7 @@ def _matrix(g, rows, k):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("rows,k", [(1, 1), (1, 64), (2, 63), (3, 65), (15, 16), (16, 1000), (17, 4096), (33, 130), (130, 257), (5, 16385), (1, 20000)])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 64), (2, 63), (3, 65), (15, 16), (16, 1000), (17, 4096), (33, 130), (130, 257), (5, 16385), (1, 20000), (1100, 8200), (1030, 5000), (3, 40000)])
 def test_quantize(i8, rows, k, kind):
     x = _normal(_gen(rows * k), rows, k, dtype=kind)
     x[:, ::7] *= 5.0
@@ -43,7 +43,7 @@ def test_quantize(i8, rows, k, kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("rows,k,eps", [(1, 64, 1e-5), (2, 63, 0.0), (17, 4096, 1e-5), (33, 130, 1e-6), (4, 16401, 1e-5)])
+@pytest.mark.parametrize("rows,k,eps", [(1, 64, 1e-5), (2, 63, 0.0), (17, 4096, 1e-5), (33, 130, 1e-6), (4, 16401, 1e-5), (1040, 9000, 1e-5), (2, 33000, 1e-6)])
 def test_rms_norm_quantize(i8, rows, k, eps, kind):
     g = _gen(rows + k)
     x, w = _normal(g, rows, k, dtype=kind, std=3.0), 1.0 + 0.3 * _normal(g, k)
