@@ -250,13 +250,13 @@ __device__ __forceinline__ v4f i8_scales4(const i8_matrix& w, int n) {
 	return n < w.strips * I8_ROWS ? *reinterpret_cast<const v4f*>(w.scale + n) : v4f{};
 }
 
-// The kernels' forms, by the tile of a workgroup (n x m).  I8_ROWS_16, _32: the kernel for few rows; _64, _128_64: tiles with K in two halves.
-enum i8_form { I8_ROWS_16, I8_ROWS_32, I8_TILE_64, I8_TILE_128_64, I8_TILE_128, I8_TILE_256 };
+// The kernels' forms, by the tile of a workgroup (n x m).  I8_ROWS_16, _32: the kernel for few rows; _64, _128_64, _128_HALVES: tiles with K in two halves.
+enum i8_form { I8_ROWS_16, I8_ROWS_32, I8_TILE_64, I8_TILE_128_64, I8_TILE_128_HALVES, I8_TILE_128, I8_TILE_256 };
 
 // The form for [n] x [m] strips of 16 and so many steps: the one with the least time by what a round of workgroups takes, `step` ns for each step and `round` ns besides; a round is as many
-// workgroups as run at once, one to a CU, or two (then, if there are no more than 256, it is the `alone` ns).  Measured, us at [n x k], m rows (form chosen / next best / 256 x 256 tiles):
-// [4096 x 4096], 64: 6.4 / 8.9 / 46; 256: 10.2 / 12 / 47; 512: 14.9 / 16 / 47; 1024: 22.5 / 23.5 / 48; 2048: 36 / 36 / 50.  [14336 x 4096], 117: 14.6 / 15.7 / 47; 512: 33 / 34 / 49; 2048: 107 (256) / 126.
-// [4096 x 14336], 512: 35 / 43 / 138.  [5003 x 1507], 1001: 18 / 18 / 32.  [8192 x 8192], 8192: 392 (256) / 499.
+// workgroups as run at once, one to a CU, or two (then, if there are no more than 256, a step takes `alone` ns).  `epilogue`: what the largest tile's takes that nothing hides.  Measured, us at
+// [n x k], m rows, the form chosen / the next best / 256 x 256 tiles:  [4096 x 4096], 64: 6.4 / 8.9 / 46; 256: 10.2 / 12 / 47; 512: 14 / 16 / 47; 1024: 19.8 / 22.4 / 48; 2048: 33 / 36 / 48.
+// [14336 x 4096], 117: 14 / 15 / 46; 512: 32 / 40 / 48; 2048: 102 (256 x 256) / 114.  [4096 x 14336], 512: 33 / 42 / 138.  [5003 x 1507], 1001: 18 / 18 / 32.  [8192 x 8192], 8192: 390 (256 x 256) / 485.
 inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t epilogue) {
 	if (m == 1) {
 		return I8_ROWS_16;
@@ -265,8 +265,8 @@ inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t epilogue
 		i8_form form;
 		int64_t n, m, at_once, step, alone, round;
 	};
-	const shape shapes[] = { { I8_ROWS_32, 2, 2, 256, 53, 53, 1500 }, { I8_TILE_64, 4, 4, 512, 174, 100, 2500 }, { I8_TILE_128_64, 8, 4, 256, 145, 145, 2500 }, { I8_TILE_128, 8, 8, 512, 506, 290, 2500 },
-		{ I8_TILE_256, 16, 16, 256, 770, 770, 2500 + epilogue } };
+	const shape shapes[] = { { I8_ROWS_32, 2, 2, 256, 53, 53, 1500 }, { I8_TILE_64, 4, 4, 512, 174, 100, 2500 }, { I8_TILE_128_64, 8, 4, 256, 145, 145, 2500 }, { I8_TILE_128_HALVES, 8, 8, 256, 255, 255, 2500 },
+		{ I8_TILE_128, 8, 8, 512, 506, 290, 2500 },		{ I8_TILE_256, 16, 16, 256, 770, 770, 2500 + epilogue } };
 	i8_form best = I8_TILE_256;
 	int64_t least = INT64_MAX;
 	for (const shape& s : shapes) {
@@ -283,7 +283,7 @@ inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t epilogue
 }
 // n that an epilogue gets at a time (16 FN), in forms whose epilogues get pairs of fragments at least
 inline int i8_stretch(i8_form form) {
-	return form == I8_TILE_256 ? 128 : form == I8_TILE_128 ? 64 : 32;
+	return form == I8_TILE_256 ? 128 : form == I8_TILE_128 || form == I8_TILE_128_HALVES ? 64 : 32;
 }
 
 // The product of w's rows from first_n on, n of them, and x.  PAIRS: the epilogue wants fragments two by two along n.
@@ -311,6 +311,9 @@ template<bool PAIRS, class EPI> void i8_launch_product(i8_form form, const i8_ma
 			break;
 		case I8_TILE_128_64:
 			launch(i8_tile_product<4, 1, 2, 4, 2, EPI>, 8, 4, 512);
+			break;
+		case I8_TILE_128_HALVES:
+			launch(i8_tile_product<2, 4, 4, 2, 2, EPI>, 8, 8, 1024);
 			break;
 		case I8_TILE_128:
 			launch(i8_tile_product<2, 4, 4, 2, 1, EPI>, 8, 8, 512);
