@@ -260,6 +260,19 @@ def test_gradient(i8, m, n, k, kind):
         assert (dx[1] == 0).all() and (dx[2] == 0).all()
 
 
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,k", [(700, 130), (1056, 580)])
+@pytest.mark.parametrize("m", [17, 32, 33, 49, 66, 81, 97, 113, 129, 145, 177, 209, 241, 257, 310])
+def test_gradient_of_rows_in_tiles_of_every_height(i8, m, n, k, kind):
+    wq, ws, xq, xs, targets = _loss_case(i8, m, n, k)
+    w, x = i8.tile(wq, ws), i8.tile(xq, xs)
+    losses, lse = i8.token_losses(w, x, targets, n, k)
+    l = R.logits(wq, ws, xq, xs)
+    grad = _normal(_gen(m), m)
+    dx = i8.token_losses_grad(w, x, targets, losses, lse, n, k, grad=grad, dtype=kind)
+    assert ((dx.double() - R.gradient(l, targets, wq, ws, grad)).abs() <= R.gradient_bound(l, targets, wq, ws, kind, grad)).all()
+
+
 @pytest.mark.parametrize("m", [3, 80])
 def test_gradient_of_rows_that_are_sure_and_of_rows_that_are_not_finite(i8, m):
     n, k = 1100, 256
