@@ -104,10 +104,11 @@ struct i8_stretches {
 	}
 };
 
-// ROWS rows to a workgroup, neighbouring threads have neighbouring rows
-template<int ROWS> __global__ __launch_bounds__(1024) void i8_join_stretches(const float2* parts, const float* hit, const int32_t* targets, float* losses, float* lse, int M, int N, int count) {
-	constexpr int LANES = 1024 / ROWS, AT_ONCE = 4;
-	__shared__ float2 all[LANES][ROWS];
+// ROWS rows to a workgroup, neighbouring threads have neighbouring rows; joined among a wave's lanes first, then the waves', with one barrier (105 rows of [1088 x 1088] 6.9 us, 7.5 with a barrier a
+// halving; few stretches: 128 threads to a row)
+template<int ROWS, int THREADS> __global__ __launch_bounds__(THREADS) void i8_join_stretches(const float2* parts, const float* hit, const int32_t* targets, float* losses, float* lse, int M, int N, int count) {
+	constexpr int LANES = THREADS / ROWS, AT_ONCE = 4, WAVES = THREADS / 64;
+	__shared__ float2 all[WAVES][ROWS];
 	const int col = threadIdx.x % ROWS, lane = threadIdx.x / ROWS, m = blockIdx.x * ROWS + col;
 	const float none = -__builtin_inff();
 	float top = none, sum = 0.0f;
@@ -116,6 +117,12 @@ template<int ROWS> __global__ __launch_bounds__(1024) void i8_join_stretches(con
 		const float now = fmaxf(top, p.x);
 		sum				= (top == now ? sum : sum * exp2_native((top - now) * LOG2_E)) + (p.x == now ? p.y : p.y * exp2_native((p.x - now) * LOG2_E));
 		top				= now;
+	};
+	auto across = [&](int first) { // lanes of a wave that have the same row
+#pragma unroll
+		for (int d = first; d >= ROWS; d >>= 1) {
+			add(make_float2(__shfl_xor(top, d), __shfl_xor(sum, d)));
+		}
 	};
 	if (m < M) {
 		for (int i = lane; i < count; i += LANES * AT_ONCE) {
@@ -130,16 +137,21 @@ template<int ROWS> __global__ __launch_bounds__(1024) void i8_join_stretches(con
 			}
 		}
 	}
-	for (int d = LANES / 2; d > 0; d >>= 1) {
-		if (lane < 2 * d) {
-			all[lane][col] = make_float2(top, sum);
-		}
-		__syncthreads();
-		if (lane < d) {
-			add(all[lane + d][col]);
-		}
-		__syncthreads();
+	across(32);
+	if ((threadIdx.x & 63) < ROWS) {
+		all[threadIdx.x / 64][col] = make_float2(top, sum);
 	}
+	__syncthreads();
+	if (threadIdx.x >= 64) {
+		return;
+	}
+	top = none, sum = 0.0f;
+#pragma unroll
+	for (int u = 0; u < (WAVES * ROWS + 63) / 64; ++u) { // the waves' sums
+		const int from = lane + u * (64 / ROWS);
+		add(from < WAVES ? all[from][col] : make_float2(none, 0.0f));
+	}
+	across(32);
 	if (lane == 0 && m < M) {
 		const float l = top + logf(sum);
 		lse[m]		  = l;
@@ -720,10 +732,15 @@ hipError_t launch_i8_losses(const i8_matrix& w, const i8_matrix& x, const i8_los
 		const int32_t* targets	= l.targets + first;
 		float *losses = l.losses + first, *lse = l.lse + first;
 		i8_launch_product<true>(plan.form, w, some, 0, w.rows, i8_stretches{ parts, hit, targets, some.rows, w.rows }, stream);
-		if (some.rows <= 256) { // a workgroup to a row
-			i8_join_stretches<1><<<some.rows, 1024, 0, stream>>>(parts, hit, targets, losses, lse, some.rows, w.rows, stretches);
+		auto join = [&](auto kernel, int rows, int threads) {
+			kernel<<<(some.rows + rows - 1) / rows, threads, 0, stream>>>(parts, hit, targets, losses, lse, some.rows, w.rows, stretches);
+		};
+		if (some.rows > 256) {
+			join(i8_join_stretches<8, 1024>, 8, 1024);
+		} else if (stretches > 512) { // a workgroup to a row
+			join(i8_join_stretches<1, 1024>, 1, 1024);
 		} else {
-			i8_join_stretches<8><<<(some.rows + 7) / 8, 1024, 0, stream>>>(parts, hit, targets, losses, lse, some.rows, w.rows, stretches);
+			join(i8_join_stretches<1, 128>, 1, 128);
 		}
 	}
 	return hipGetLastError();
