@@ -26,28 +26,47 @@ template<int TYPE> struct i8_store {
 		}
 	}
 
-	// A lane has four neighbouring n of sixteen different rows m: sixteen rows at a time go through LDS, so that a wave's loads and stores run along the rows, four values to a lane if N is a multiple of
-	// four (ALONG = 4), else one.  Pieces of four values lie at places permuted by the row, which spreads them over the banks either way.  The residual of the next sixteen rows is on its
-	// way while these are stored (y may be the residual: a row's is loaded before any of that row is stored).
-	template<int FN, int FM, int ALONG> __device__ __forceinline__ void along_rows(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f* scratch) const {
-		constexpr int PIECES = 4 * FN, LANES = 16 * FN / ALONG < 64 ? 16 * FN / ALONG : 64, ROWS = 64 / LANES, TIMES = 16 / ROWS, ACROSS = 16 * FN / (LANES * ALONG);
+	// A lane has four neighbouring n of sixteen different rows m: sixteen rows at a time go through LDS, so that a wave's loads and stores run along the rows, four values to a lane.  Pieces of four
+	// values lie at places permuted by the row, which spreads them over the banks either way.  The residual of the next sixteen rows is on its way while these are stored (y may be the residual: a
+	// row's is loaded before any of that row is stored).  FOURS: N is a multiple of four.  If not, a row's fours lie at any multiple of a value's size, which the card's loads and stores take, and its
+	// last values go one by one.
+	template<int FN, int FM, bool FOURS> __device__ __forceinline__ void along_rows(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f* scratch) const {
+		constexpr int PIECES = 4 * FN, LANES = PIECES < 64 ? PIECES : 64, ROWS = 64 / LANES, TIMES = 16 / ROWS;
 		const int lane = threadIdx.x & 63, row = lane & 15;
-		const int c0 = ALONG * (lane % LANES), r0 = lane / LANES; // this lane's first column and row when it moves values
+		const int c0 = lane % LANES, r0 = lane / LANES, n = n0 + 4 * c0; // this lane's piece and first row when it moves values
 		struct values {
-			value v[ALONG];
+			value v[4];
 		};
+		constexpr int ALIGNMENT = FOURS ? sizeof(values) : sizeof(value);
+		const bool four			= FOURS || n + 4 <= N;
 		constexpr int SETS = FN < 8 ? 2 : 1; // (in the largest tiles the sums leave no room for two)
-		values add[SETS][TIMES][ACROSS] = {};
-		auto fetch = [&](int i, values(&to)[TIMES][ACROSS]) { // (past the end: the last ones, for nothing)
+		values add[SETS][TIMES] = {};
+		auto fetch = [&](int i, values(&to)[TIMES]) { // (past the end: the last ones, for nothing)
 #pragma unroll
 			for (int t = 0; t < TIMES; ++t) {
+				const value* from = residual + static_cast<int64_t>(min(m0 + 16 * i + r0 + ROWS * t, M - 1)) * N;
+				if (four) {
+					__builtin_memcpy(&to[t], __builtin_assume_aligned(from + (FOURS ? min(n, N - 4) : n), ALIGNMENT), sizeof(values));
+				} else {
 #pragma unroll
-				for (int c = 0; c < ACROSS; ++c) {
-					const int64_t m = min(m0 + 16 * i + r0 + ROWS * t, M - 1), n = min(n0 + c0 + LANES * ALONG * c, N - ALONG);
-					__builtin_memcpy(&to[t][c], __builtin_assume_aligned(residual + m * N + n, sizeof(values)), sizeof(values));
+					for (int e = 0; e < 4; ++e) {
+						to[t].v[e] = from[min(n + e, N - 1)];
+					}
 				}
 			}
 		};
+		// all scales before the first store: a wait for a load is also one for the stores before it
+		v4f sw[FN];
+		float sx[FM];
+#pragma unroll
+		for (int f = 0; f < FN; ++f) {
+			sw[f] = i8_scales4(w, n0 + 4 * (4 * f + (lane >> 4)));
+		}
+#pragma unroll
+		for (int i = 0; i < FM; ++i) {
+			const int m = m0 + 16 * i + row;
+			sx[i]		= m < M ? x.scale[m] : 0.0f;
+		}
 		if (residual && SETS == 2) {
 			fetch(0, add[0]);
 		}
@@ -56,16 +75,14 @@ template<int TYPE> struct i8_store {
 			if (residual && SETS == 1) {
 				fetch(i, add[0]);
 			}
-			const int m	   = m0 + 16 * i;
-			const float sx = m + row < M ? x.scale[m + row] : 0.0f;
+			const int m = m0 + 16 * i;
 #pragma unroll
 			for (int f = 0; f < FN; ++f) {
 				const int piece = 4 * f + (lane >> 4);
-				const v4f sw	= i8_scales4(w, n0 + 4 * piece);
 				v4f v;
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
-					v[e] = static_cast<float>(sums[f][i][e]) * sx * sw[e];
+					v[e] = static_cast<float>(sums[f][i][e]) * sx[i] * sw[f][e];
 				}
 				scratch[row * PIECES + (piece ^ (row % PIECES))] = v;
 			}
@@ -75,18 +92,22 @@ template<int TYPE> struct i8_store {
 			__builtin_amdgcn_wave_barrier(); // (one wave's own LDS accesses are in order)
 #pragma unroll
 			for (int t = 0; t < TIMES; ++t) {
+				const int r = r0 + ROWS * t;
+				const v4f v = scratch[r * PIECES + (c0 ^ (r % PIECES))];
+				values out;
 #pragma unroll
-				for (int c = 0; c < ACROSS; ++c) {
-					const int r = r0 + ROWS * t, at = c0 + LANES * ALONG * c;
-					const v4f four = scratch[r * PIECES + ((at >> 2) ^ (r % PIECES))];
-					values out;
+				for (int e = 0; e < 4; ++e) {
+					out.v[e] = T::narrow(residual ? v[e] + T::widen(add[i % SETS][t].v[e]) : v[e]);
+				}
+				value* to = y + static_cast<int64_t>(m + r) * N + n;
+				if (m + r < M && four && n < N) {
+					__builtin_memcpy(__builtin_assume_aligned(to, ALIGNMENT), &out, sizeof(values));
+				} else if (!FOURS && m + r < M) {
 #pragma unroll
-					for (int e = 0; e < ALONG; ++e) {
-						const float v = ALONG == 4 ? four[e] : (at & 2) ? (at & 1) ? four[3] : four[2] : (at & 1) ? four[1] : four[0];
-						out.v[e]	  = T::narrow(residual ? v + T::widen(add[i % SETS][t][c].v[e]) : v);
-					}
-					if (m + r < M && n0 + at < N) {
-						__builtin_memcpy(__builtin_assume_aligned(y + static_cast<int64_t>(m + r) * N + n0 + at, sizeof(values)), &out, sizeof(values));
+					for (int e = 0; e < 4; ++e) {
+						if (n + e < N) {
+							to[e] = out.v[e];
+						}
 					}
 				}
 			}
@@ -95,9 +116,9 @@ template<int TYPE> struct i8_store {
 	}
 	template<int FN, int FM> __device__ __forceinline__ void operator()(const v4i (&sums)[FN][FM], int n0, int m0, const i8_matrix& w, const i8_matrix& x, v4f* scratch) const {
 		if ((N & 3) == 0) {
-			along_rows<FN, FM, 4>(sums, n0, m0, w, x, scratch);
+			along_rows<FN, FM, true>(sums, n0, m0, w, x, scratch);
 		} else {
-			along_rows<FN, FM, 1>(sums, n0, m0, w, x, scratch);
+			along_rows<FN, FM, false>(sums, n0, m0, w, x, scratch);
 		}
 	}
 };

@@ -46,12 +46,21 @@ struct i8_stretches {
 		for (int f = 0; f < FN; ++f) {
 			sw[f] = i8_scales4(w, n0 + 16 * f + 4 * group);
 		}
+		// all rows' before the first store: a wait for a load is also one for the stores before it
+		float scales[FM];
+		int places[FM];
+#pragma unroll
+		for (int i = 0; i < FM; ++i) {
+			const int m	 = m0 + 16 * i + (lane & 15);
+			scales[i]	 = m < M ? x.scale[m] : 0.0f;
+			places[i]	 = m < M ? targets[m] - n0 : -1;
+		}
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
 			const int m		 = m0 + 16 * i + (lane & 15);
 			const bool there = m < M;
-			const float sx	 = there ? x.scale[m] : 0.0f;
-			const int target = there ? targets[m] - n0 : -1; // in this stretch?
+			const float sx	 = scales[i];
+			const int target = places[i]; // in this stretch?
 			v4f l[FN];
 			float top = -__builtin_inff();
 #pragma unroll
@@ -223,18 +232,26 @@ template<int TERMS> struct i8_slopes {
 		for (int c = 0; c < FN; ++c) {
 			sw[c] = i8_scales4(w, n0 + 16 * c + 4 * group);
 		}
+		// all rows' before the first store: a wait for a load is also one for the stores before it.  (A row that is not scored: finite numbers times nothing.)
+		int places[FM];
+		float scales[FM], belows[FM], lifts[FM];
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
-			const int strip = m0 / 16 + i, m = 16 * strip + (lane & 15);
+			const int m		  = m0 + 16 * i + (lane & 15);
+			places[i]		  = m < M ? targets[m] : -1;
+			const bool scored = places[i] >= 0 && places[i] < N;
+			scales[i] = scored ? x.scale[m] : 0.0f, belows[i] = scored ? lse[m] : 0.0f;
+			lifts[i] = scored ? ldexpf(1.0f, slopes_exponent(losses[m])) : 0.0f;
+		}
+#pragma unroll
+		for (int i = 0; i < FM; ++i) {
+			const int strip = m0 / 16 + i;
 			if (strip >= x.strips) {
 				continue;
 			}
-			const int target  = m < M ? targets[m] : -1;
-			const bool scored = target >= 0 && target < N;
-			// (a row that is not scored: finite numbers times nothing)
-			const float sx = scored ? x.scale[m] : 0.0f, below = scored ? lse[m] : 0.0f;
-			const float lift = scored ? ldexpf(1.0f, slopes_exponent(losses[m])) : 0.0f;
-			const bool here	 = scored && target >= n0 && target < n0 + 16 * FN;
+			const int target = places[i];
+			const float sx = scales[i], below = belows[i], lift = lifts[i];
+			const bool here = target >= 0 && target < N && target >= n0 && target < n0 + 16 * FN;
 #pragma unroll
 			for (int b = 0; b < FN / 2; ++b) {
 				if (block + b >= blocks) {
