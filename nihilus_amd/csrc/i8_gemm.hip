@@ -300,10 +300,13 @@ template<int TYPE, bool NORM, int ROWS, int PIECES, int FN> __global__ __launch_
 	}
 }
 
+// ns that a byte of 16 x 16 results takes (i8_form_for)
+constexpr int64_t STORE = 38;
+
 template<int TYPE> hipError_t gemm(const i8_matrix& w, const i8_matrix& x, const void* residual, void* y, hipStream_t stream) {
 	typedef typename i8_type<TYPE>::store value;
 	const i8_store<TYPE> epi{ static_cast<value*>(y), static_cast<const value*>(residual), x.rows, w.rows };
-	i8_launch_product<false>(i8_form_for(w.strips, x.strips, w.steps, 0), w, x, 0, w.rows, epi, stream);
+	i8_launch_product<false>(i8_form_for(w.strips, x.strips, w.steps, STORE * int64_t{ sizeof(value) }), w, x, 0, w.rows, epi, stream);
 	return hipGetLastError();
 }
 

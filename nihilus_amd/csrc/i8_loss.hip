@@ -19,8 +19,8 @@ namespace nh {
 
 namespace {
 
-// ns that 256 x 256 exponentials take behind a product, with no other workgroup on the CU whose products would hide them
-constexpr int64_t EPILOGUE = 6000;
+// ns that 16 x 16 exponentials take behind a product
+constexpr int64_t EPILOGUE = 72;
 constexpr float LOG2_E = 1.44269504088896340736f;
 
 // 2^x, within 2 ulp for the arguments here (x <= 0 up to rounding)

@@ -253,27 +253,28 @@ __device__ __forceinline__ v4f i8_scales4(const i8_matrix& w, int n) {
 // The kernels' forms, by the tile of a workgroup (n x m).  I8_ROWS_16, _32: the kernel for few rows; _64, _128_64, _128_HALVES: tiles with K in two halves.
 enum i8_form { I8_ROWS_16, I8_ROWS_32, I8_TILE_64, I8_TILE_128_64, I8_TILE_128_HALVES, I8_TILE_128, I8_TILE_256 };
 
-// The form for [n] x [m] strips of 16 and so many steps: the one with the least time by what a round of workgroups takes, `step` ns for each step and `round` ns besides; a round is as many
-// workgroups as run at once, one to a CU, or two (then, if there are no more than 256, a step takes `alone` ns).  `epilogue`: what the largest tile's takes that nothing hides.  Measured, us at
-// [n x k], m rows, the form chosen / the next best / 256 x 256 tiles:  [4096 x 4096], 64: 6.4 / 8.9 / 46; 256: 10.2 / 12 / 47; 512: 14 / 16 / 47; 1024: 19.8 / 22.4 / 48; 2048: 33 / 36 / 48.
-// [14336 x 4096], 117: 14 / 15 / 46; 512: 32 / 40 / 48; 2048: 102 (256 x 256) / 114.  [4096 x 14336], 512: 33 / 42 / 138.  [5003 x 1507], 1001: 18 / 18 / 32.  [8192 x 8192], 8192: 390 (256 x 256) / 485.
-inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t epilogue) {
+// The form for [n] x [m] strips of 16 and so many steps: the one with the least time by what a round of workgroups takes, `step` ns for each step, `round` ns besides, and `behind` ns for each 16 x 16
+// results of a CU; a round is as many workgroups as run at once, one to a CU, or two (then, if there are no more than 256, a step takes `alone` ns).  The numbers are a fit to all forms' times at 72
+// shapes of 17 to 8192 rows, 64 to 32768 n and 64 to 16384 k, results in two bytes and in four, and at 42 shapes of losses: on average the form taken is within 0.3 % of the best, at worst 10 %.
+// Measured, us at [n x k], m rows, the form taken / the next best / 256 x 256 tiles:  [4096 x 4096], 64: 6.4 / 8.9 / 46; 256: 10.2 / 12 / 45; 512: 14 / 16 / 45; 1024: 20.4 / 21.7 / 45.
+// [14336 x 4096], 117: 14 / 15 / 46; 512: 36 / 44 / 48; 2048: 104 (256 x 256) / 117.  [9216 x 128], 1927: 15.8 / 20.9 (256 x 256).  [5003 x 1507], 1001: 18 / 21 / 29.  [8192 x 8192], 8192: 382 (256 x 256) / 495.
+inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t behind) {
 	if (m == 1) {
 		return I8_ROWS_16;
 	}
 	struct shape {
 		i8_form form;
-		int64_t n, m, at_once, step, alone, round;
+		int64_t n, m, per_cu, step, alone, round; // per_cu: workgroups
 	};
-	const shape shapes[] = { { I8_ROWS_32, 2, 2, 256, 53, 53, 1500 }, { I8_TILE_64, 4, 4, 512, 174, 100, 2500 }, { I8_TILE_128_64, 8, 4, 256, 145, 145, 2500 }, { I8_TILE_128_HALVES, 8, 8, 256, 255, 255, 2500 },
-		{ I8_TILE_128, 8, 8, 512, 506, 290, 2500 },		{ I8_TILE_256, 16, 16, 256, 770, 770, 2500 + epilogue } };
+	const shape shapes[] = { { I8_ROWS_32, 2, 2, 1, 53, 53, 1500 }, { I8_TILE_64, 4, 4, 2, 174, 114, 3200 }, { I8_TILE_128_64, 8, 4, 1, 145, 145, 3600 }, { I8_TILE_128_HALVES, 8, 8, 1, 265, 265, 2500 },
+		{ I8_TILE_128, 8, 8, 2, 490, 290, 1000 },		{ I8_TILE_256, 16, 16, 1, 704, 704, 2600 } };
 	i8_form best = I8_TILE_256;
 	int64_t least = INT64_MAX;
 	for (const shape& s : shapes) {
-		const int64_t tiles = (n + s.n - 1) / s.n * ((m + s.m - 1) / s.m), left = tiles % s.at_once;
-		int64_t time		= tiles / s.at_once * (steps * s.step + s.round);
+		const int64_t tiles = (n + s.n - 1) / s.n * ((m + s.m - 1) / s.m), left = tiles % (256 * s.per_cu), results = behind * s.n * s.m;
+		int64_t time		= tiles / (256 * s.per_cu) * (steps * s.step + s.round + results * s.per_cu);
 		if (left) {
-			time += steps * (left <= 256 ? s.alone : s.step) + s.round;
+			time += s.round + (left <= 256 ? steps * s.alone + results : steps * s.step + results * s.per_cu);
 		}
 		if (time < least) {
 			least = time, best = s.form;
