@@ -397,12 +397,18 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 	};
 	v4f sums[FK][FM] = {};
 	auto multiply	 = [&](const v8h(&k)[FK], int i, const v8h(&d)[TERMS]) {
+		if constexpr (TERMS == 2) { // before the other wave's conversions: fp32 gradients 3.5 % faster (with one term 1 % slower)
+			__builtin_amdgcn_s_setprio(1);
+		}
 #pragma unroll
 		for (int t = TERMS - 1; t >= 0; --t) { // the small term first
 #pragma unroll
 			for (int f = 0; f < FK; ++f) {
 				sums[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[f], d[t], sums[f][i], 0, 0, 0);
 			}
+		}
+		if constexpr (TERMS == 2) {
+			__builtin_amdgcn_s_setprio(0);
 		}
 	};
 	v2i raw[FK];
@@ -425,6 +431,7 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 #pragma unroll
 		for (int f = 0; f < FK; ++f) {
 			k[1 - h][f] = i8_halves(raw[f]);
+			asm volatile("" : "+v"(k[1 - h][f])); // here: the compiler would move it behind the test for the last block, in front of the products that take it
 		}
 #pragma unroll
 		for (int i = FIRST; i < FM; ++i) {
