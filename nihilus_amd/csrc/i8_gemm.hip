@@ -301,7 +301,7 @@ template<int TYPE, bool NORM, int ROWS, int PIECES, int FN> __global__ __launch_
 }
 
 // ns that a byte of 16 x 16 results takes (i8_form_for)
-constexpr int64_t STORE = 38;
+constexpr int64_t STORE = 39;
 
 template<int TYPE> hipError_t gemm(const i8_matrix& w, const i8_matrix& x, const void* residual, void* y, hipStream_t stream) {
 	typedef typename i8_type<TYPE>::store value;

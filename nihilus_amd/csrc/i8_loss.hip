@@ -20,7 +20,7 @@ namespace nh {
 namespace {
 
 // ns that 16 x 16 exponentials take behind a product
-constexpr int64_t EPILOGUE = 72;
+constexpr int64_t EPILOGUE = 66;
 constexpr float LOG2_E = 1.44269504088896340736f;
 
 // 2^x, within 2 ulp for the arguments here (x <= 0 up to rounding)

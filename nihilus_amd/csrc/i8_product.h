@@ -6,6 +6,8 @@
 
 #include "i8_device.h"
 
+#include <type_traits>
+
 namespace nh {
 
 __device__ __forceinline__ v4i i8_mfma(v4u a, v4u b, v4i c) {
@@ -45,8 +47,8 @@ template<int N> __device__ __forceinline__ void i8_arrive() {
 // buffers, three steps ahead, and from there into one of two sets of registers, one step ahead: a wave waits once a step, for transfers that were asked for three steps ago.
 // KS = 2: two such groups of waves with a ring each have the two halves of K, and join their sums in LDS.
 template<int WN, int WM, int FN, int FM, int KS, class EPI> __global__ __launch_bounds__(64 * WN * WM * KS, 2) void i8_tile_product(i8_matrix w, i8_matrix x, int first_n, int n_tiles, int m_tiles, EPI epi) {
-	constexpr int WAVES = WN * WM, NF = WN * FN, FRAGMENTS = NF + WM * FM, LOADS = FRAGMENTS / WAVES, RING = 4;
-	static_assert(FRAGMENTS % WAVES == 0 && (KS == 1 || FM % 2 == 0));
+	constexpr int WAVES = WN * WM, NF = WN * FN, FRAGMENTS = NF + WM * FM, LOADS = FRAGMENTS / WAVES, MORE = FRAGMENTS % WAVES, RING = 4;
+	static_assert(KS == 1 || FM % 2 == 0);
 	__shared__ v4u rings[KS][RING][FRAGMENTS][64];
 	static_assert(WAVES * KS * FN <= KS * RING * FRAGMENTS && (KS == 1 || WAVES * FN * FM <= KS * RING * FRAGMENTS));
 	const i8_place p = i8_place_of(n_tiles, m_tiles);
@@ -57,18 +59,32 @@ template<int WN, int WM, int FN, int FM, int KS, class EPI> __global__ __launch_
 	const int n_strip = first_n / I8_ROWS + p.n * NF, m_strip = p.m * WM * FM;
 	const int steps = (w.steps + KS - 1) / KS, first_step = part * steps, mine = min(steps, w.steps - first_step); // (the second half may be a step shorter)
 	auto& ring = rings[part];
-	const v4u* from[LOADS];
+	// this wave's fragments of a step; the first MORE waves have one more
+	const bool more = MORE && wave < MORE;
+	const auto fragment = [&](int j) { return j < LOADS ? wave * LOADS + j : WAVES * LOADS + min(wave, MORE - 1); };
+	const v4u* from[LOADS + (MORE > 0)];
 #pragma unroll
-	for (int j = 0; j < LOADS; ++j) { // (strips past a matrix's last one: that one again, for sums that nobody takes)
-		const int f			= wave * LOADS + j;
+	for (int j = 0; j < LOADS + (MORE > 0); ++j) { // (strips past a matrix's last one: that one again, for sums that nobody takes)
+		const int f			= fragment(j);
 		const int64_t strip = f < NF ? min(n_strip + f, w.strips - 1) : min(m_strip + f - NF, x.strips - 1);
 		from[j]				= (f < NF ? w.q : x.q) + (strip * w.steps + min(first_step, w.steps - 1)) * 64;
 	}
 	auto load = [&](int s) {
 		const int at = KS == 1 ? s : min(s, max(mine - 1, 0));
 #pragma unroll
-		for (int j = 0; j < LOADS; ++j) {
-			load_global_to_lds_b128(from[j] + at * 64, 16 * lane, &ring[s % RING][wave * LOADS + j][0]);
+		for (int j = 0; j < LOADS + (MORE > 0); ++j) {
+			if (j < LOADS || more) {
+				load_global_to_lds_b128(from[j] + at * 64, 16 * lane, &ring[s % RING][fragment(j)][0]);
+			}
+		}
+	};
+	// all but the last so many steps' transfers done
+	auto arrive_but = [&](auto steps_behind) {
+		constexpr int S = decltype(steps_behind)::value;
+		if (more) {
+			i8_arrive<S * (LOADS + 1)>();
+		} else {
+			i8_arrive<S * LOADS>();
 		}
 	};
 	auto read = [&](int s, v4u(&a)[FN], v4u(&b)[FM]) {
@@ -97,11 +113,11 @@ template<int WN, int WM, int FN, int FM, int KS, class EPI> __global__ __launch_
 	}
 	auto arrive = [&](int behind) { // a step is in LDS, those up to `behind` steps after it may be on their way
 		if (behind >= 3) {
-			i8_arrive<3 * LOADS>();
+			arrive_but(std::integral_constant<int, 3>{});
 		} else if (behind == 2) {
-			i8_arrive<2 * LOADS>();
+			arrive_but(std::integral_constant<int, 2>{});
 		} else if (behind == 1) {
-			i8_arrive<LOADS>();
+			arrive_but(std::integral_constant<int, 1>{});
 		} else {
 			i8_arrive<0>();
 		}
@@ -113,7 +129,7 @@ template<int WN, int WM, int FN, int FM, int KS, class EPI> __global__ __launch_
 	for (; s + 1 + RING < steps; s += 2) {
 #pragma unroll
 		for (int h = 0; h < 2; ++h) {
-			i8_arrive<(RING - 2) * LOADS>(); // step s + h + 1 is there, and everybody has read step s + h
+			arrive_but(std::integral_constant<int, RING - 2>{}); // step s + h + 1 is there, and everybody has read step s + h
 			load(s + h + RING);
 			read(s + h + 1, a[1 - h], b[1 - h]);
 			multiply(a[h], b[h]);
@@ -250,12 +266,13 @@ __device__ __forceinline__ v4f i8_scales4(const i8_matrix& w, int n) {
 	return n < w.strips * I8_ROWS ? *reinterpret_cast<const v4f*>(w.scale + n) : v4f{};
 }
 
-// The kernels' forms, by the tile of a workgroup (n x m).  I8_ROWS_16, _32: the kernel for few rows; _64, _128_64, _128_HALVES: tiles with K in two halves.
-enum i8_form { I8_ROWS_16, I8_ROWS_32, I8_TILE_64, I8_TILE_128_64, I8_TILE_128_HALVES, I8_TILE_128, I8_TILE_256 };
+// The kernels' forms, by the tile of a workgroup (n x m).  I8_ROWS_16, _32: the kernel for few rows; _64, _128_64, _128_HALVES: tiles with K in two halves; _128_96, _128_160, _128_192: so that rows
+// are not padded far (300 of [128256 x 4096]: 210 us as 3 x 128, 169 as 2 x 160) and that tiles fill rounds (640 of [8192 x 8192]: 61 / 44).
+enum i8_form { I8_ROWS_16, I8_ROWS_32, I8_TILE_64, I8_TILE_128_64, I8_TILE_128_HALVES, I8_TILE_128_96, I8_TILE_128, I8_TILE_128_160, I8_TILE_128_192, I8_TILE_256 };
 
 // The form for [n] x [m] strips of 16 and so many steps: the one with the least time by what a round of workgroups takes, `step` ns for each step, `round` ns besides, and `behind` ns for each 16 x 16
-// results of a CU; a round is as many workgroups as run at once, one to a CU, or two (then, if there are no more than 256, a step takes `alone` ns).  The numbers are a fit to all forms' times at 72
-// shapes of 17 to 8192 rows, 64 to 32768 n and 64 to 16384 k, results in two bytes and in four, and at 42 shapes of losses: on average the form taken is within 0.3 % of the best, at worst 10 %.
+// results of a CU; a round is as many workgroups as run at once, one to a CU, or two (then, if there are no more than 256, a step takes `alone` ns).  The numbers are a fit to all forms' times at 136
+// shapes of 17 to 8192 rows, 64 to 32768 n and 64 to 16384 k, results in two bytes and in four, and at 50 shapes of losses: on average the form taken is within 0.5 % of the best, at worst 8 %.
 // Measured, us at [n x k], m rows, the form taken / the next best / 256 x 256 tiles:  [4096 x 4096], 64: 6.4 / 8.9 / 46; 256: 10.2 / 12 / 45; 512: 14 / 16 / 45; 1024: 20.4 / 21.7 / 45.
 // [14336 x 4096], 117: 14 / 15 / 46; 512: 36 / 44 / 48; 2048: 104 (256 x 256) / 117.  [9216 x 128], 1927: 15.8 / 20.9 (256 x 256).  [5003 x 1507], 1001: 18 / 21 / 29.  [8192 x 8192], 8192: 382 (256 x 256) / 495.
 inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t behind) {
@@ -266,8 +283,9 @@ inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t behind) 
 		i8_form form;
 		int64_t n, m, per_cu, step, alone, round; // per_cu: workgroups
 	};
-	const shape shapes[] = { { I8_ROWS_32, 2, 2, 1, 53, 53, 1500 }, { I8_TILE_64, 4, 4, 2, 174, 114, 3200 }, { I8_TILE_128_64, 8, 4, 1, 145, 145, 3600 }, { I8_TILE_128_HALVES, 8, 8, 1, 265, 265, 2500 },
-		{ I8_TILE_128, 8, 8, 2, 490, 290, 1000 },		{ I8_TILE_256, 16, 16, 1, 704, 704, 2600 } };
+	const shape shapes[] = { { I8_ROWS_32, 2, 2, 1, 53, 53, 1100 }, { I8_TILE_64, 4, 4, 2, 174, 114, 3000 }, { I8_TILE_128_64, 8, 4, 1, 142, 142, 3350 }, { I8_TILE_128_HALVES, 8, 8, 1, 250, 250, 2520 },
+		{ I8_TILE_128_96, 8, 6, 2, 450, 240, 1600 },	{ I8_TILE_128, 8, 8, 2, 500, 290, 830 },		{ I8_TILE_128_160, 8, 10, 2, 560, 270, 800 },	{ I8_TILE_128_192, 8, 12, 2, 660, 490, 630 },
+		{ I8_TILE_256, 16, 16, 1, 650, 650, 2600 } };
 	i8_form best = I8_TILE_256;
 	int64_t least = INT64_MAX;
 	for (const shape& s : shapes) {
@@ -315,6 +333,15 @@ template<bool PAIRS, class EPI> void i8_launch_product(i8_form form, const i8_ma
 			break;
 		case I8_TILE_128_HALVES:
 			launch(i8_tile_product<2, 4, 4, 2, 2, EPI>, 8, 8, 1024);
+			break;
+		case I8_TILE_128_96:
+			launch(i8_tile_product<4, 2, 2, 3, 1, EPI>, 8, 6, 512);
+			break;
+		case I8_TILE_128_160:
+			launch(i8_tile_product<4, 2, 2, 5, 1, EPI>, 8, 10, 512);
+			break;
+		case I8_TILE_128_192:
+			launch(i8_tile_product<4, 2, 2, 6, 1, EPI>, 8, 12, 512);
 			break;
 		case I8_TILE_128:
 			launch(i8_tile_product<2, 4, 4, 2, 1, EPI>, 8, 8, 512);

@@ -171,6 +171,13 @@ def test_gemm_bit_for_bit(i8, m, n, k, kind):
     assert i8.gemm(w, x, m, n, k, dtype=kind, residual=r, out=r) is r and torch.equal(r, want)
 
 
+# (rows that are a little less than 96, 160 and 192, n for several hundred tiles, K of one step to ten)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("m,n,k", [(90, 20003, 64), (81, 16400, 577), (150, 16400, 130), (157, 20003, 577), (145, 33002, 400), (180, 16400, 60), (190, 20003, 130), (177, 16402, 577), (310, 20001, 200)])
+def test_gemm_in_tiles_of_other_heights(i8, m, n, k, kind):
+    test_gemm_bit_for_bit(i8, m, n, k, kind)
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_sums_up_to_the_last_bit(i8, m):
     # the longest K with the largest values: whole numbers just below 2^31
@@ -258,6 +265,13 @@ def test_gradient(i8, m, n, k, kind):
         assert (off <= R.gradient_bound(l, targets, wq, ws, kind, g)).all()
     if m > 2:
         assert (dx[1] == 0).all() and (dx[2] == 0).all()
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(90, 16400, 130), (150, 20003, 64), (157, 16400, 330), (180, 16403, 200), (310, 20001, 130)])
+def test_losses_and_gradient_in_tiles_of_other_heights(i8, m, n, k, kind):
+    test_losses(i8, m, n, k)
+    test_gradient(i8, m, n, k, kind)
 
 
 @pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
