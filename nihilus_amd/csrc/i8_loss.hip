@@ -175,11 +175,12 @@ constexpr int64_t up(int64_t n, int64_t to) {
 // ---- backward ----
 
 constexpr int MAXIMA = 64;
-__global__ __launch_bounds__(256) void i8_largest_scales(const float* scale, int n, float* out) {
-	__shared__ float tops[4];
+__global__ __launch_bounds__(1024) void i8_largest_scales(const float* scale, int n, float* out) {
+	constexpr int THREADS = 1024;
+	__shared__ float tops[THREADS / 64];
 	float top = 0.0f;
-#pragma unroll 8
-	for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += MAXIMA * 256) {
+#pragma unroll 4
+	for (int i = blockIdx.x * THREADS + threadIdx.x; i < n; i += MAXIMA * THREADS) {
 		top = fmaxf(top, fabsf(scale[i]));
 	}
 #pragma unroll
@@ -191,7 +192,11 @@ __global__ __launch_bounds__(256) void i8_largest_scales(const float* scale, int
 	}
 	__syncthreads();
 	if (threadIdx.x == 0) {
-		out[blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+#pragma unroll
+		for (int i = 0; i < THREADS / 64; ++i) {
+			top = fmaxf(top, tops[i]);
+		}
+		out[blockIdx.x] = top;
 	}
 }
 // f, such that the largest scale times 2^f is in [1/2, 1) (any f if it is 0 or not finite)
@@ -779,7 +784,7 @@ hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_g
 	char* ws	  = static_cast<char*>(all.workspace);
 	float* maxima = reinterpret_cast<float*>(ws);
 	v8h* slopes	  = reinterpret_cast<v8h*>(ws + MAXIMA * 4);
-	i8_largest_scales<<<MAXIMA, 256, 0, stream>>>(w.scale, w.rows, maxima);
+	i8_largest_scales<<<MAXIMA, 1024, 0, stream>>>(w.scale, w.rows, maxima);
 	const gradient_plan most = plan_gradient(std::min<int64_t>(x.rows, GRADIENT_ROWS), w.rows, all.k, all.type);
 	float* sums				 = reinterpret_cast<float*>(ws + MAXIMA * 4 + most.slopes);
 	for (int64_t first = 0; first < x.rows; first += GRADIENT_ROWS) {
