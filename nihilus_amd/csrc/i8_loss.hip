@@ -330,8 +330,9 @@ struct i8_slope_product {
 
 // A workgroup has 512 columns x 16 FM rows of sums over its split's blocks of 32 n, a wave 64 of the columns, so that each piece of w is made fp16 by one wave only.  Blocks come through a
 // ring in LDS as in i8_tile_product, and w's pieces of the next block are read and converted among the products of this one.
-// FM is such that the rows' tiles are of one height, eight strips at most: 144 rows of [32000 x 4096] are 2 x 80, and take 117 us in fp32 and 95 in bf16 (the gradient as a whole), 146 and 108 as
-// 2 x 128; 300 of [128256 x 4096] 786 and 561 as 3 x 112, 838 and 584 as 3 x 128; 30 of it 198 and 190 as 32, 234 and 198 as 64.
+// FM is such that the rows' tiles are of one height, eight strips at most: 144 rows of [32000 x 4096] are 2 x 80, and take 111 us in fp32 and 89 in bf16 (the gradient as a whole), 140 and 102 as
+// 2 x 128; 300 of [128256 x 4096] 754 and 516 as 3 x 112, 795 and 532 as 3 x 128; 30 of it 198 and 186 as 32, 220 and 190 as 64.  Bound by the card's power: a loop of the same products alone, with
+// nothing read, converted or transferred, takes 78 % (one term) and 86 % (two) of this one's time, which is the rate of the library's fp16 product.
 template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_kernel(i8_matrix w, i8_slope_product a, int k_tiles, int m_tiles, int splits) {
 	constexpr int WAVES = 8, FK = 4, STEPS = WAVES, NF = 2 * STEPS, FRAGMENTS = NF + FM * TERMS, LOADS = FRAGMENTS / WAVES, MORE = FRAGMENTS % WAVES, RING = 4;
 	constexpr int FIRST = (FM * TERMS + 1) / 2 < 4 ? FM : 4 / TERMS; // strips of P that are in registers before a block begins; the others are read in it
