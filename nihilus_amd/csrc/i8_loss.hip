@@ -7,7 +7,8 @@
 //
 // Backward: dx[m][k] = grad[m] sum_n d[m][n] sw[n] w[n][k],  d = exp(l - lse) - [n = t].  Pieces of the vocabulary at a time, the product kernels form l again and leave
 // P = d sw 2^e in fp16, in operand order; a second product sums P w over n.  d is at most 1 - exp(-loss) of its row, so e is chosen by the row (and by the largest of all sw): P is below 2^14, and what
-// is 2^-28 of the row's largest is still a normal number.  fp16 has 11 bits; where dx is fp32, P is a sum of two such numbers (22 bits) and the second product twice as much.
+// is 2^-28 of the row's largest is still a normal number.  fp16 has 11 bits, three more than bf16; where dx is fp32 or fp16, P is a
+// sum of two such numbers (22 bits) and the second product twice as much (one would put as much on an fp16 dx as its own rounding does).
 // w enters the second product as fp16, exactly.  It lies in fragments of 16 rows n x 64 values k, and the sum is over n: ds_read_b64_tr_b8 takes eight rows of sixteen columns out of LDS so that
 // a lane has eight n of one k.
 #include "i8_product.h"
@@ -671,7 +672,7 @@ struct gradient_plan {
 gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k, int type) {
 	gradient_plan g{};
 	const int64_t strips = i8_strips(m), steps = i8_steps(k);
-	g.terms				 = type == NH_F32 ? 2 : 1;
+	g.terms				 = type == NH_BF16 ? 1 : 2;
 	g.few				 = strips == 1 && steps <= 64;
 	if (g.few) { // a workgroup to a CU, or to a strip
 		g.splits = std::min<int64_t>(256, i8_strips(n));

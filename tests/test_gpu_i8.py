@@ -287,6 +287,18 @@ def test_gradient_of_rows_in_tiles_of_every_height(i8, m, n, k, kind):
     assert ((dx.double() - R.gradient(l, targets, wq, ws, grad)).abs() <= R.gradient_bound(l, targets, wq, ws, kind, grad)).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 600, 512), (12, 6001, 576), (5, 3000, 4160), (40, 1500, 300), (160, 3008, 1280), (310, 2001, 130)])
+def test_gradient_in_fp16_is_off_by_its_rounding_alone(i8, m, n, k):
+    # what fp32 is off by, and half a step of the result (2^-11 of a normal number, 2^-25 of the smallest)
+    wq, ws, xq, xs, targets = _loss_case(i8, m, n, k)
+    w, x = i8.tile(wq, ws), i8.tile(xq, xs)
+    losses, lse = i8.token_losses(w, x, targets, n, k)
+    l = R.logits(wq, ws, xq, xs)
+    dx = i8.token_losses_grad(w, x, targets, losses, lse, n, k, dtype=torch.float16)
+    want = R.gradient(l, targets, wq, ws)
+    assert ((dx.double() - want).abs() <= R.gradient_bound(l, targets, wq, ws, torch.float32) + want.abs() * 2.0**-11 + 2.0**-25).all()
+
+
 @pytest.mark.parametrize("m", [3, 80])
 def test_gradient_of_rows_that_are_sure_and_of_rows_that_are_not_finite(i8, m):
     n, k = 1100, 256
