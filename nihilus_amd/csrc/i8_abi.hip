@@ -222,7 +222,7 @@ int nh_i8_token_losses(const void* w_tiled, const void* x_tiled, const int32_t* 
 int64_t nh_i8_token_losses_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int type) {
 	NH_TRY(check_type(type));
 	const int bad = check_product(M, N, K);
-	return bad ? bad : M == 0 || N == 0 ? 0 : nh::i8_gradient_workspace(M, N, K, type);
+	return bad ? bad : M == 0 || N == 0 ? 0 : nh::i8_gradient_workspace(M, N, K);
 }
 int nh_i8_token_losses_grad(const void* w_tiled, const void* x_tiled, const int32_t* targets, const float* losses, const float* lse, const float* grad, void* dx, int type, int64_t M, int64_t N,
 	int64_t K, void* workspace, int64_t workspace_bytes, void* stream) {

@@ -108,7 +108,7 @@ struct i8_gradient {
 	int k, type;
 	void* workspace;
 };
-int64_t i8_gradient_workspace(int64_t m, int64_t n, int64_t k, int type);
+int64_t i8_gradient_workspace(int64_t m, int64_t n, int64_t k);
 hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_gradient& g, hipStream_t stream);
 
 } // namespace nh

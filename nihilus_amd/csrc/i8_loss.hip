@@ -7,8 +7,8 @@
 //
 // Backward: dx[m][k] = grad[m] sum_n d[m][n] sw[n] w[n][k],  d = exp(l - lse) - [n = t].  Pieces of the vocabulary at a time, the product kernels form l again and leave
 // P = d sw 2^e in fp16, in operand order; a second product sums P w over n.  d is at most 1 - exp(-loss) of its row, so e is chosen by the row (and by the largest of all sw): P is below 2^14, and what
-// is 2^-28 of the row's largest is still a normal number.  fp16 has 11 bits, three more than bf16; where dx is fp32 or fp16, P is a
-// sum of two such numbers (22 bits) and the second product twice as much (one would put as much on an fp16 dx as its own rounding does).
+// is 2^-28 of the row's largest is still a normal number.  P is a sum of two such numbers (22 bits), whatever dx is rounded to: with one (11 bits) 2048 rows of [128256 x 4096] took 2.7 ms instead of 3.9,
+// and one bf16 dx in sixteen was another number.
 // w enters the second product as fp16, exactly.  It lies in fragments of 16 rows n x 64 values k, and the sum is over n: ds_read_b64_tr_b8 takes eight rows of sixteen columns out of LDS so that
 // a lane has eight n of one k.
 #include "i8_product.h"
@@ -221,8 +221,10 @@ __device__ __forceinline__ int slopes_exponent(float loss) {
 	return 13 - e;
 }
 
+constexpr int TERMS = 2; // of fp16 that a slope is a sum of
+
 // P of a piece of the vocabulary: [term][strip of 16 rows][32 n][lane], lane's eight numbers n = 16 h + 4 (lane / 16) + i at 4 h + i, row lane % 16
-template<int TERMS> struct i8_slopes {
+struct i8_slopes {
 	v8h* p;
 	const int32_t* targets;
 	const float *losses, *lse, *maxima;
@@ -331,10 +333,10 @@ struct i8_slope_product {
 
 // A workgroup has 512 columns x 16 FM rows of sums over its split's blocks of 32 n, a wave 64 of the columns, so that each piece of w is made fp16 by one wave only.  Blocks come through a
 // ring in LDS as in i8_tile_product, and w's pieces of the next block are read and converted among the products of this one.
-// FM is such that the rows' tiles are of one height, eight strips at most: 144 rows of [32000 x 4096] are 2 x 80, and take 111 us in fp32 and 89 in bf16 (the gradient as a whole), 140 and 102 as
-// 2 x 128; 300 of [128256 x 4096] 754 and 516 as 3 x 112, 795 and 532 as 3 x 128; 30 of it 198 and 186 as 32, 220 and 190 as 64.  Bound by the card's power: a loop of the same products alone, with
-// nothing read, converted or transferred, takes 78 % (one term) and 86 % (two) of this one's time, which is the rate of the library's fp16 product.
-template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_kernel(i8_matrix w, i8_slope_product a, int k_tiles, int m_tiles, int splits) {
+// FM is such that the rows' tiles are of one height, eight strips at most: 144 rows of [32000 x 4096] are 2 x 80, and take 111 us (the gradient as a whole), 140 as 2 x 128; 300 of [128256 x 4096] 754 as
+// 3 x 112, 795 as 3 x 128; 30 of it 198 as 32, 220 as 64.  Bound by the card's power: a loop of the same products alone, with nothing read, converted or transferred, takes 86 % of this one's time, which
+// is the rate of the library's fp16 product.
+template<int FM> __global__ __launch_bounds__(512, 2) void i8_slope_kernel(i8_matrix w, i8_slope_product a, int k_tiles, int m_tiles, int splits) {
 	constexpr int WAVES = 8, FK = 4, STEPS = WAVES, NF = 2 * STEPS, FRAGMENTS = NF + FM * TERMS, LOADS = FRAGMENTS / WAVES, MORE = FRAGMENTS % WAVES, RING = 4;
 	constexpr int FIRST = (FM * TERMS + 1) / 2 < 4 ? FM : 4 / TERMS; // strips of P that are in registers before a block begins; the others are read in it
 	__shared__ v4u ring[RING][FRAGMENTS][64];
@@ -404,9 +406,7 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 	};
 	v4f sums[FK][FM] = {};
 	auto multiply	 = [&](const v8h(&k)[FK], int i, const v8h(&d)[TERMS]) {
-		if constexpr (TERMS == 2) { // before the other wave's conversions: fp32 gradients 3.5 % faster (with one term 1 % slower)
-			__builtin_amdgcn_s_setprio(1);
-		}
+		__builtin_amdgcn_s_setprio(1); // before the other wave's conversions: 3.5 % faster
 #pragma unroll
 		for (int t = TERMS - 1; t >= 0; --t) { // the small term first
 #pragma unroll
@@ -414,9 +414,7 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 				sums[f][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[f], d[t], sums[f][i], 0, 0, 0);
 			}
 		}
-		if constexpr (TERMS == 2) {
-			__builtin_amdgcn_s_setprio(0);
-		}
+		__builtin_amdgcn_s_setprio(0);
 	};
 	v2i raw[FK];
 	v8h k[2][FK], d[2][FIRST][TERMS];
@@ -498,7 +496,7 @@ template<int FM, int TERMS> __global__ __launch_bounds__(512, 2) void i8_slope_k
 // comes by direct transfers into LDS that is its own, two strips ahead, and is used there twice, for the wave's part of the logits and, after all waves' parts have been added up, for its
 // columns of the sums, which stay in registers over all of the workgroup's strips.  One barrier a strip.  Bound by memory: w is read once (5 rows of 128256 x 4096, fp32: 95
 // us, 175 as two products).
-template<int TERMS, int STEPS> __global__ __launch_bounds__(512, 2) void i8_few_slopes(i8_matrix w, i8_matrix x, const int32_t* targets, const float* losses, const float* lse, const float* maxima, float* out) {
+template<int STEPS> __global__ __launch_bounds__(512, 2) void i8_few_slopes(i8_matrix w, i8_matrix x, const int32_t* targets, const float* losses, const float* lse, const float* maxima, float* out) {
 	constexpr int WAVES = 8, SCALES = 4;
 	__shared__ v4u strip[WAVES][2][STEPS][64];
 	__shared__ v4i parts[2][WAVES][64];
@@ -666,20 +664,19 @@ struct gradient_plan {
 	int64_t piece, blocks; // n, blocks of 32 n
 	int64_t k_tiles, m_tiles, splits;
 	int64_t slopes, sums; // bytes
-	int strips, terms; // strips of rows in a tile
+	int strips; // of rows in a tile
 	bool few; // one pass
 };
-gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k, int type) {
+gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k) {
 	gradient_plan g{};
 	const int64_t strips = i8_strips(m), steps = i8_steps(k);
-	g.terms				 = type == NH_BF16 ? 1 : 2;
 	g.few				 = strips == 1 && steps <= 64;
 	if (g.few) { // a workgroup to a CU, or to a strip
 		g.splits = std::min<int64_t>(256, i8_strips(n));
 		g.sums	 = up(g.splits * m * steps * I8_STEP * 4, 256);
 		return g;
 	}
-	const int64_t row	 = strips * 16 * 2 * g.terms;
+	const int64_t row	 = strips * 16 * 2 * TERMS;
 	g.piece				 = std::min(up(n, 32), std::max<int64_t>((int64_t{ 1 } << 27) / row / 256 * 256, 1024));
 	g.blocks			 = g.piece / 32;
 	g.k_tiles			 = (steps + 7) / 8;
@@ -691,17 +688,17 @@ gradient_plan plan_gradient(int64_t m, int64_t n, int64_t k, int type) {
 	return g;
 }
 
-template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, const i8_gradient& g, const gradient_plan& plan, v8h* slopes, float* sums, const float* maxima, hipStream_t stream) {
+void gradient_sums(const i8_matrix& w, const i8_matrix& x, const i8_gradient& g, const gradient_plan& plan, v8h* slopes, float* sums, const float* maxima, hipStream_t stream) {
 	if (plan.few) {
 		auto launch = [&](auto kernel) {
 			kernel<<<static_cast<unsigned>(plan.splits), 512, 0, stream>>>(w, x, g.targets, g.losses, g.lse, maxima, sums);
 		};
-		w.steps <= 16 ? launch(i8_few_slopes<TERMS, 2>) : w.steps <= 32 ? launch(i8_few_slopes<TERMS, 4>) : launch(i8_few_slopes<TERMS, 8>);
+		w.steps <= 16 ? launch(i8_few_slopes<2>) : w.steps <= 32 ? launch(i8_few_slopes<4>) : launch(i8_few_slopes<8>);
 		return;
 	}
 	for (int64_t first = 0; first < w.rows; first += plan.piece) {
 		const int64_t n = std::min<int64_t>(plan.piece, w.rows - first), blocks = (n + 31) / 32;
-		const i8_slopes<TERMS> epi{ slopes, g.targets, g.losses, g.lse, maxima, x.rows, w.rows, static_cast<int>(first), static_cast<int>(blocks) };
+		const i8_slopes epi{ slopes, g.targets, g.losses, g.lse, maxima, x.rows, w.rows, static_cast<int>(first), static_cast<int>(blocks) };
 		i8_launch_product<true>(i8_form_for(i8_strips(n), x.strips, w.steps, EPILOGUE), w, x, static_cast<int>(first), static_cast<int>(n), epi, stream);
 		i8_slope_product a{};
 		a.p = slopes, a.out = sums;
@@ -714,14 +711,14 @@ template<int TERMS> void gradient_sums(const i8_matrix& w, const i8_matrix& x, c
 			kernel<<<grid, 512, 0, stream>>>(w, a, static_cast<int>(plan.k_tiles), static_cast<int>(m_tiles), static_cast<int>(plan.splits));
 		};
 		switch (plan.strips) {
-		case 8: multiply(i8_slope_kernel<8, TERMS>); break;
-		case 7: multiply(i8_slope_kernel<7, TERMS>); break;
-		case 6: multiply(i8_slope_kernel<6, TERMS>); break;
-		case 5: multiply(i8_slope_kernel<5, TERMS>); break;
-		case 4: multiply(i8_slope_kernel<4, TERMS>); break;
-		case 3: multiply(i8_slope_kernel<3, TERMS>); break;
-		case 2: multiply(i8_slope_kernel<2, TERMS>); break;
-		default: multiply(i8_slope_kernel<1, TERMS>); break;
+		case 8: multiply(i8_slope_kernel<8>); break;
+		case 7: multiply(i8_slope_kernel<7>); break;
+		case 6: multiply(i8_slope_kernel<6>); break;
+		case 5: multiply(i8_slope_kernel<5>); break;
+		case 4: multiply(i8_slope_kernel<4>); break;
+		case 3: multiply(i8_slope_kernel<3>); break;
+		case 2: multiply(i8_slope_kernel<2>); break;
+		default: multiply(i8_slope_kernel<1>); break;
 		}
 	}
 }
@@ -777,8 +774,8 @@ hipError_t launch_i8_losses(const i8_matrix& w, const i8_matrix& x, const i8_los
 	return hipGetLastError();
 }
 
-int64_t i8_gradient_workspace(int64_t m, int64_t n, int64_t k, int type) {
-	const gradient_plan g = plan_gradient(std::min(m, GRADIENT_ROWS), n, k, type);
+int64_t i8_gradient_workspace(int64_t m, int64_t n, int64_t k) {
+	const gradient_plan g = plan_gradient(std::min(m, GRADIENT_ROWS), n, k);
 	return MAXIMA * 4 + g.slopes + g.sums;
 }
 
@@ -787,7 +784,7 @@ hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_g
 	float* maxima = reinterpret_cast<float*>(ws);
 	v8h* slopes	  = reinterpret_cast<v8h*>(ws + MAXIMA * 4);
 	i8_largest_scales<<<MAXIMA, 1024, 0, stream>>>(w.scale, w.rows, maxima);
-	const gradient_plan most = plan_gradient(std::min<int64_t>(x.rows, GRADIENT_ROWS), w.rows, all.k, all.type);
+	const gradient_plan most = plan_gradient(std::min<int64_t>(x.rows, GRADIENT_ROWS), w.rows, all.k);
 	float* sums				 = reinterpret_cast<float*>(ws + MAXIMA * 4 + most.slopes);
 	for (int64_t first = 0; first < x.rows; first += GRADIENT_ROWS) {
 		const i8_matrix some = rows_of(x, first, std::min<int64_t>(GRADIENT_ROWS, x.rows - first));
@@ -796,11 +793,7 @@ hipError_t launch_i8_gradient(const i8_matrix& w, const i8_matrix& x, const i8_g
 		g.grad = all.grad ? all.grad + first : nullptr;
 		g.dx   = static_cast<char*>(all.dx) + first * all.k * (all.type == NH_F32 ? 4 : 2);
 		// (fewer rows behind others are cut as those are, which is what there is room for)
-		if (most.terms == 2) {
-			gradient_sums<2>(w, some, g, most, slopes, sums, maxima, stream);
-		} else {
-			gradient_sums<1>(w, some, g, most, slopes, sums, maxima, stream);
-		}
+		gradient_sums(w, some, g, most, slopes, sums, maxima, stream);
 		const int columns	  = w.steps * I8_STEP;
 		const unsigned beside = static_cast<unsigned>(std::min(some.rows, 64));
 		const bool many		  = most.splits >= 32; // then sixteen threads to four columns
