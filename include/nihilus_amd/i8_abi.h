@@ -54,7 +54,7 @@ int nh_i8_mul_mat(const void* w_tiled, const void* x, int type, int64_t x_stride
 
 /* Softmax cross entropy of rows x [M][K] on an output projection w [N][K]:  l[m][n] = the product above in fp32,
  *   lse[m] = log sum_n exp l[m][n],   losses[m] = lse[m] - l[m][targets[m]],  0 where targets[m] (int32) is outside [0, N): such a row is not scored.
- * The logits are formed a tile at a time and not kept. */
+ * A loss is formed from the largest logit, not from the rounded lse, so that a small one keeps its digits however large the logits are.  These are formed a tile at a time and not kept. */
 int64_t nh_i8_token_losses_workspace_bytes(int64_t M, int64_t N, int64_t K); /* up to about 64 MiB, whatever M is, unless N is far past a million */
 int nh_i8_token_losses(const void* w_tiled, const void* x_tiled, const int32_t* targets, float* losses, float* lse, int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -163,9 +163,9 @@ template<int ROWS, int THREADS> __global__ __launch_bounds__(THREADS) void i8_jo
 	}
 	across(32);
 	if (lane == 0 && m < M) {
-		const float l = top + logf(sum);
-		lse[m]		  = l;
-		losses[m]	  = targets[m] >= 0 && targets[m] < N ? l - hit[m] : 0.0f;
+		const float rest = logf(sum);
+		lse[m]			 = top + rest;
+		losses[m]		 = targets[m] >= 0 && targets[m] < N ? (top - hit[m]) + rest : 0.0f; // (not by lse: a small loss would be left in steps of its last place)
 	}
 }
 

@@ -46,3 +46,72 @@ def test_a_gradient_in_16_bits_is_the_one_of_32_rounded(i8, m, n, k, kind):
     # The last product (a row's grad) may be rounded to fp16 at once, which leaves another number only where fp32 rounds it to the middle of two: both are as far from it then, exactly.
     far = [(t.double() - wide.double()).abs() for t in (narrow, wide.to(kind))]
     assert wide.abs().max() > 0 and torch.equal(*far) and (kind != torch.bfloat16 or torch.equal(narrow, wide.to(kind)))
+
+
+# ---- rows that are sure of their target, at logits of any size
+
+
+def _exact_logits(wanted, fine):
+    """wanted [m, n] fp64, multiples of 2^-fine[i] in row i and below 2^18 of them: int8 operands and scales (powers of two, of three sizes) whose products are exactly those, row i in 64 values of its own.
+
+    A row's 62 values of 127 and one of 1 are met by 62 values whose sum is a token's number / 127, and the rest."""
+    m, n = wanted.shape
+    steps = (wanted * torch.tensor([2.0**f for f in fine], dtype=torch.float64)[:, None]).round().long()
+    ws = torch.tensor([2.0 ** -(j % 3) for j in range(n)])
+    whole = steps * (1.0 / ws).long()[None]  # of 2^-fine ws
+    assert whole.abs().max() <= 62 * 127 * 127
+    most = (whole.abs() + 63) // 127
+    places = torch.arange(62)
+    wq, xq = torch.zeros(n, 64 * m, dtype=torch.int8), torch.zeros(m, 64 * m, dtype=torch.int8)
+    for i in range(m):
+        part = ((most[i][:, None] - 127 * places).clamp(0, 127) * whole[i].sign()[:, None]).to(torch.int8)
+        wq[:, 64 * i : 64 * i + 62] = part
+        wq[:, 64 * i + 62] = (whole[i] - 127 * part.long().sum(1)).to(torch.int8)
+        xq[i, 64 * i : 64 * i + 62], xq[i, 64 * i + 62] = 127, 1
+    xs = torch.tensor([2.0**-f for f in fine])
+    wq, ws, xq, xs = (t.cuda() for t in (wq, ws, xq, xs))
+    l = R.logits(wq, ws, xq, xs)
+    assert torch.equal(l.cpu(), steps.double() / torch.tensor([2.0**f for f in fine], dtype=torch.float64)[:, None])
+    return wq, ws, xq, xs, l
+
+
+# largest logit, how fine the logits are
+SIZES = [(25.0, 11), (300.0, 9), (4000.0, 5), (20000.0, 2), (-20000.0, 2), (30000.0, 2), (120000.0, 0)]
+
+
+def _sure_case(m, n, seed=0):
+    """Rows of every size of logits, with a few tokens from 1/4 to 14 below the target's (which is theirs in one row of five), all others 40 to 90 below."""
+    g = torch.Generator().manual_seed(seed + m)
+    wanted, fine, targets = torch.empty(m, n, dtype=torch.float64), [], torch.empty(m, dtype=torch.int32)
+    for i in range(m):
+        top, f = SIZES[i % len(SIZES)]
+        fine.append(f)
+        gaps = 40.0 + 50.0 * torch.rand(n, generator=g, dtype=torch.float64)
+        order = torch.randperm(n, generator=g)
+        near = 1 + i % 3
+        gaps[order[0]] = 0.0
+        gaps[order[1 : 1 + near]] = [0.25, 1.0, 3.0, 6.0, 8.0, 9.0, 11.0, 14.0][i // 2 % 8] + torch.randint(0, 2, (near,), generator=g).double()
+        wanted[i] = ((top - gaps) * 2**f).round() / 2**f
+        targets[i] = order[1] if i % 5 == 3 else order[0]
+    return (*_exact_logits(wanted, fine), targets.cuda())
+
+
+def _sum_bound(l):
+    """How far the log of a row's sum of exponentials, over the largest, may be off.  The differences are exact here.  An addition rounds by U of the sum: 32 of a lane and two among lanes in a stretch, one to a thread
+    (stretches are fewer than threads), six among lanes, and one of the two waves or three of more.  An exponential below the largest is off by twice its exponent's and the two ulp (4 U): 6 U where it is most, and so
+    again wherever it is joined to a larger one, seven times at most."""
+    s = torch.exp(l - l.amax(dim=1, keepdim=True)).sum(dim=1)
+    return R.U * (44 + 48 * (1 - 1 / s))
+
+
+SURE = [(5, 331), (16, 600), (40, 331), (300, 250)]
+
+
+@pytest.mark.parametrize("m,n", SURE)
+def test_losses_of_rows_that_are_sure(i8, m, n):
+    wq, ws, xq, xs, l, targets = _sure_case(m, n)
+    losses, lse = i8.token_losses(i8.tile(wq, ws), i8.tile(xq, xs), targets, n, 64 * m)
+    want, want_lse = R.losses(l, targets)
+    # the target's distance from the largest is exact; a logarithm of two ulp, and a sum
+    assert ((losses.double() - want).abs() <= _sum_bound(l) + 6 * R.U * want).all()
+    assert ((lse.double() - want_lse).abs() <= _sum_bound(l) + 6 * R.U * want + R.U * want_lse.abs()).all()
