@@ -213,9 +213,13 @@ __device__ __forceinline__ int scales_exponent(const float* maxima) {
 	}
 	return -e;
 }
-// e, such that 2^e (1 - exp(-loss)) is in [2^12, 2^13); where that is below 2^-16, lse itself does not tell such d from nothing
-__device__ __forceinline__ int slopes_exponent(float loss) {
-	const float most = fminf(fmaxf(1.0f - exp2_native(-loss * LOG2_E), 0x1p-16f), 1.0f);
+// d of a row's target, from the loss: exp(l - lse) less one would keep of a sure row's what the rounding of lse leaves (at lse 25 and 1 - p = 1e-4, 8e-3 of it)
+__device__ __forceinline__ float target_slope(float loss) {
+	return expm1f(-loss);
+}
+// e, such that 2^e (1 - exp(-loss)) is in [2^12, 2^13); where that is below 2^-16 (the sum's rounding is up to 2^-18 of it), as for that
+__device__ __forceinline__ int slopes_exponent(float of_target) {
+	const float most = fminf(fmaxf(-of_target, 0x1p-16f), 1.0f);
 	int e;
 	(void)frexpf(most, &e);
 	return 13 - e;
@@ -242,14 +246,15 @@ struct i8_slopes {
 		}
 		// all rows' before the first store: a wait for a load is also one for the stores before it.  (A row that is not scored: finite numbers times nothing.)
 		int places[FM];
-		float scales[FM], belows[FM], lifts[FM];
+		float scales[FM], belows[FM], lifts[FM], owns[FM];
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
 			const int m		  = m0 + 16 * i + (lane & 15);
 			places[i]		  = m < M ? targets[m] : -1;
 			const bool scored = places[i] >= 0 && places[i] < N;
 			scales[i] = scored ? x.scale[m] : 0.0f, belows[i] = scored ? lse[m] : 0.0f;
-			lifts[i] = scored ? ldexpf(1.0f, slopes_exponent(losses[m])) : 0.0f;
+			owns[i]	 = scored ? target_slope(losses[m]) : 0.0f;
+			lifts[i] = scored ? ldexpf(1.0f, slopes_exponent(owns[i])) : 0.0f;
 		}
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
@@ -277,7 +282,7 @@ struct i8_slopes {
 				if (here) {
 #pragma unroll
 					for (int j = 0; j < 8; ++j) {
-						v[j] -= n0 + 32 * b + 16 * (j >> 2) + 4 * group + (j & 3) == target ? 1.0f : 0.0f;
+						v[j] = n0 + 32 * b + 16 * (j >> 2) + 4 * group + (j & 3) == target ? owns[i] : v[j];
 					}
 				}
 				v8h out[TERMS];
@@ -515,7 +520,8 @@ template<int STEPS> __global__ __launch_bounds__(512, 2) void i8_few_slopes(i8_m
 	const int target  = m < M ? targets[m] : -1;
 	const bool scored = target >= 0 && target < N;
 	const float sx = scored ? x.scale[m] : 0.0f, below = scored ? lse[m] : 0.0f;
-	const float lift = scored ? ldexpf(1.0f, slopes_exponent(losses[m])) : 0.0f;
+	const float own	 = scored ? target_slope(losses[m]) : 0.0f;
+	const float lift = scored ? ldexpf(1.0f, slopes_exponent(own)) : 0.0f;
 	const int stride = gridDim.x, count = (w.strips - static_cast<int>(blockIdx.x) + stride - 1) / stride; // strips of this workgroup
 	asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (from here on only transfers are counted)
 	auto load = [&](int b) {
@@ -569,7 +575,7 @@ template<int STEPS> __global__ __launch_bounds__(512, 2) void i8_few_slopes(i8_m
 #pragma unroll
 		for (int e = 0; e < 4; ++e) {
 			const float l = static_cast<float>(all[e]) * sx * sw[e];
-			float v		  = exp2_native((l - below) * LOG2_E) - (scored && n + e == target ? 1.0f : 0.0f);
+			float v		  = scored && n + e == target ? own : exp2_native((l - below) * LOG2_E);
 			v			  = n + e < N ? v * (ldexpf(sw[e], f) * lift) : 0.0f;
 #pragma unroll
 			for (int t = 0; t < TERMS; ++t) {
@@ -643,7 +649,7 @@ template<int TYPE, int LANES> __global__ __launch_bounds__(256) void i8_slope_re
 		return;
 	}
 	const bool scored = targets[m] >= 0 && targets[m] < N;
-	const int back	= scored ? -f - slopes_exponent(losses[m]) : 0;
+	const int back	= scored ? -f - slopes_exponent(target_slope(losses[m])) : 0;
 	const float g	= grad ? grad[m] : 1.0f;
 #pragma unroll
 	for (int e = 0; e < 4; ++e) {
