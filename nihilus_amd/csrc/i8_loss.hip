@@ -6,7 +6,7 @@
 // it comes by; a second kernel joins the stretches.
 //
 // Backward: dx[m][k] = grad[m] sum_n d[m][n] sw[n] w[n][k],  d = exp(l - lse) - [n = t].  Pieces of the vocabulary at a time, the product kernels form l again and leave
-// P = d sw 2^e in fp16, in operand order; a second product sums P w over n.  d is at most 1 - exp(-loss) of its row, so e is chosen by the row (and by the largest of all sw): P is below 2^14, and what
+// P = d sw 2^e in fp16, in operand order; a second product sums P w over n.  d is at most 1 - exp(-loss) of its row, so e is chosen by the row (and by the largest of all sw): P is below 2^15, and what
 // is 2^-28 of the row's largest is still a normal number.  P is a sum of two such numbers (22 bits), whatever dx is rounded to: with one (11 bits) 2048 rows of [128256 x 4096] took 2.7 ms instead of 3.9,
 // and one bf16 dx in sixteen was another number.
 // w enters the second product as fp16, exactly.  It lies in fragments of 16 rows n x 64 values k, and the sum is over n: ds_read_b64_tr_b8 takes eight rows of sixteen columns out of LDS so that
@@ -217,7 +217,9 @@ __device__ __forceinline__ int scales_exponent(const float* maxima) {
 __device__ __forceinline__ float target_slope(float loss) {
 	return expm1f(-loss);
 }
-// e, such that 2^e (1 - exp(-loss)) is in [2^12, 2^13); where that is below 2^-16 (the sum's rounding is up to 2^-18 of it), as for that
+// e, such that 2^e (1 - exp(-loss)) is in [2^12, 2^13); where that is below 2^-16 (the sum's rounding is up to 2^-18 of it), as for that.
+// However lse is rounded, the other slopes as they are computed are at most a little over twice that.  lse is the largest logit plus log(sum), log(sum) >= 0, and so not below the largest once it is
+// rounded either: a slope is at most exp(l - largest).  If the target has the largest, that is at most sum - 1 = exp(loss) - 1, or 1; if not, it is at most 1, and 1 - exp(-loss) is 1/2 or more.
 __device__ __forceinline__ int slopes_exponent(float of_target) {
 	const float most = fminf(fmaxf(-of_target, 0x1p-16f), 1.0f);
 	int e;

@@ -117,6 +117,20 @@ def test_losses_of_rows_that_are_sure(i8, m, n):
     assert ((lse.double() - want_lse).abs() <= _sum_bound(l) + 6 * R.U * want + R.U * want_lse.abs()).all()
 
 
+def _sure_bound(l, targets, wq, ws, kind, grad):
+    n = l.shape[1]
+    losses, lse = R.losses(l, targets)
+    want, d = R.gradient(l, targets, wq, ws, grad), R.slopes(l, targets)
+    own = torch.zeros_like(d, dtype=torch.bool).scatter_(1, targets.long()[:, None], True)
+    # The target's slope, exp(-loss) - 1: as exact as the loss, and two ulp.  The others, exp(l - lse): lse's rounding and its sum's, a difference and a product by log2 e (3 U of the exponent), two ulp.
+    off_own = (torch.exp(-losses) * (_sum_bound(l) + 6 * R.U * losses))[:, None] + 4 * R.U * d.abs()
+    off = torch.where(own, off_own, d.abs() * (R.U * lse.abs() + _sum_bound(l) + 6 * R.U * losses)[:, None] + d.abs() * R.U * (3 * (lse[:, None] - l) + 4))
+    # two products, two fp16 numbers (2^-22 of a slope, or half of the smallest number, 2^-25, where the largest is 2^12 or more), sums over n in fp32
+    off = off + d.abs() * (2 * R.U + 2.0**-22 + (n + 64) * R.U)
+    least = 2.0**-25 * 2.0**-12 * (-torch.expm1(-losses)).clamp(min=2.0**-16)[:, None] * 2 * ws.max().double() * wq.double().abs().sum(0)[None]
+    return (off @ (wq.double().abs() * ws.double()[:, None]) + least) * grad.double()[:, None] + want.abs() * (R.HALF[kind] + 2 * R.U) + (2.0**-25 if kind == torch.float16 else 0.0)
+
+
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("m,n", SURE)
 def test_gradient_of_rows_that_are_sure(i8, m, n, kind):
@@ -125,17 +139,29 @@ def test_gradient_of_rows_that_are_sure(i8, m, n, kind):
     losses, lse = i8.token_losses(w, x, targets, n, 64 * m)
     grad = torch.rand(m, device="cuda", generator=_gen(m))
     dx = i8.token_losses_grad(w, x, targets, losses, lse, n, 64 * m, grad=grad, dtype=kind).double()
-    want_losses, want_lse = R.losses(l, targets)
-    want, d = R.gradient(l, targets, wq, ws, grad), R.slopes(l, targets)
-    own = torch.zeros_like(d, dtype=torch.bool).scatter_(1, targets.long()[:, None], True)
-    # The target's slope, exp(-loss) - 1: as exact as the loss, and two ulp.  The others, exp(l - lse): lse's rounding and its sum's, a difference and a product by log2 e (3 U of the exponent), two ulp.
-    off_own = (torch.exp(-want_losses) * (_sum_bound(l) + 6 * R.U * want_losses))[:, None] + 4 * R.U * d.abs()
-    off = torch.where(own, off_own, d.abs() * (R.U * want_lse.abs() + _sum_bound(l) + 6 * R.U * want_losses)[:, None] + d.abs() * R.U * (3 * (want_lse[:, None] - l) + 4))
-    # two products, two fp16 numbers (2^-22 of a slope, or half of the smallest number, 2^-25, where the largest is 2^12 or more), sums over n in fp32
-    off = off + d.abs() * (2 * R.U + 2.0**-22 + (n + 64) * R.U)
-    least = 2.0**-25 * 2.0**-12 * (-torch.expm1(-want_losses)).clamp(min=2.0**-16)[:, None] * 2 * ws.max().double() * wq.double().abs().sum(0)[None]
-    bound = (off @ (wq.double().abs() * ws.double()[:, None]) + least) * grad.double()[:, None] + want.abs() * (R.HALF[kind] + 2 * R.U) + (2.0**-25 if kind == torch.float16 else 0.0)
+    want, bound = R.gradient(l, targets, wq, ws, grad), _sure_bound(l, targets, wq, ws, kind, grad)
     assert torch.isfinite(dx).all() and ((dx - want).abs() <= bound).all()
     # ... which says something of every row whose loss is above 1e-4, whatever its logits
-    told = want_losses > 1e-4
+    told = R.losses(l, targets)[0] > 1e-4
     assert told.sum() >= m // 2 and ((bound.amax(1) < 0.2 * want.abs().amax(1)) | ~told).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("m", [8, 24])
+def test_gradient_of_two_tokens_far_up(i8, m, kind):
+    # A loss in steps of lse's last place was nothing here, and the other token's slope, which lse does not hide, past fp16 in units of the smallest.
+    n = 40
+    sizes = [(9000.0, 8.0, 4), (20000.0, 7.75, 2), (20000.0, 6.25, 2), (50000.0, 9.0, 1), (100000.0, 7.0, 0), (-100000.0, 8.0, 0), (2.0**22, 32.0, -5), (2.0**29, 2.0**12, -12)]
+    wanted, fine = torch.empty(m, n, dtype=torch.float64), [sizes[i % 8][2] for i in range(m)]
+    targets = torch.tensor([(7 * i + 3) % n for i in range(m)], dtype=torch.int32)
+    for i in range(m):
+        top, gap, f = sizes[i % 8]
+        wanted[i] = top - max(64.0, 2.0**-f)
+        wanted[i, targets[i]], wanted[i, (7 * i + 3 + i) % n if i % n else 0] = top, top - gap
+    wq, ws, xq, xs, l = _exact_logits(wanted, fine)
+    targets = targets.cuda()
+    w, x, grad = i8.tile(wq, ws), i8.tile(xq, xs), torch.ones(m, device="cuda")
+    losses, lse = i8.token_losses(w, x, targets, n, 64 * m)
+    dx = i8.token_losses_grad(w, x, targets, losses, lse, n, 64 * m, dtype=kind).double()
+    assert torch.isfinite(dx).all()
+    assert ((dx - R.gradient(l, targets, wq, ws, grad)).abs() <= _sure_bound(l, targets, wq, ws, kind, grad)).all()
