@@ -97,12 +97,14 @@ struct i8_stretches {
 			}
 			top = fmaxf(top, __shfl_xor(top, 16));
 			top = fmaxf(top, __shfl_xor(top, 32));
-			float sum = 0.0f;
+			// (an infinite largest one is not subtracted: a stretch of -infinities adds nothing, +infinity is the row's lse, and only NaN gives NaN)
+			const float from = fabsf(top) < __builtin_inff() ? top : 0.0f;
+			float sum		 = 0.0f;
 #pragma unroll
 			for (int f = 0; f < FN; ++f) {
 #pragma unroll
 				for (int e = 0; e < 4; ++e) {
-					sum += exp2_native((l[f][e] - top) * LOG2_E);
+					sum += exp2_native((l[f][e] - from) * LOG2_E);
 				}
 			}
 			sum += __shfl_xor(sum, 16);

@@ -165,3 +165,36 @@ def test_gradient_of_two_tokens_far_up(i8, m, kind):
     dx = i8.token_losses_grad(w, x, targets, losses, lse, n, 64 * m, dtype=kind).double()
     assert torch.isfinite(dx).all()
     assert ((dx - R.gradient(l, targets, wq, ws, grad)).abs() <= _sure_bound(l, targets, wq, ws, kind, grad)).all()
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_losses_of_logits_past_fp32(i8, m):
+    # a row's scale is so large that some logits, or all of a stretch, are infinite: the sums' scale takes the first 128 tokens there, the others' takes them back
+    n, k = 700, 64
+    g = _gen(m)
+    wq, ws = _matrix(g, n, k)
+    xq = torch.randint(1, 128, (m, k), device="cuda", dtype=torch.int8, generator=g)
+    xs = torch.full((m,), 2.0**100, device="cuda")
+    ws[:128] = 2.0**30
+    ws[128:] *= 2.0**-100
+    wq[:128] = -wq[:128].abs() - 1  # -infinity
+    wq[:128].clamp_(min=-127)
+    targets = torch.randint(128, n, (m,), device="cuda", dtype=torch.int32, generator=g)
+    w, x = i8.tile(wq, ws), i8.tile(xq, xs)
+    losses, lse = i8.token_losses(w, x, targets, n, k)
+    want, want_lse = R.losses(R.logits(wq[128:], ws[128:], xq, xs), targets - 128)
+    l = R.logits(wq[128:], ws[128:], xq, xs)
+    assert ((lse.double() - want_lse).abs() <= R.lse_bound(l)).all()
+    assert ((losses.double() - want).abs() <= R.lse_bound(l) + R.logit_bound(l) + 4 * R.U * want.abs()).all()
+    targets[0] = 5  # a target at -infinity
+    losses, lse = i8.token_losses(w, x, targets, n, k)
+    assert losses[0] == float("inf") and torch.isfinite(losses[1:]).all() and torch.isfinite(lse).all()
+    wq[9] = 127  # and one of all tokens at +infinity
+    losses, lse = i8.token_losses(i8.tile(wq, ws), x, targets, n, k)
+    assert (lse == float("inf")).all() and (losses == float("inf")).all()
+    targets[0] = 9  # infinity less infinity
+    losses, _ = i8.token_losses(i8.tile(wq, ws), x, targets, n, k)
+    assert torch.isnan(losses[0]) and (losses[1:] == float("inf")).all()
+    ws[9] = float("nan")
+    losses, lse = i8.token_losses(i8.tile(wq, ws), x, targets, n, k)
+    assert torch.isnan(lse).all() and torch.isnan(losses).all()
