@@ -37,7 +37,7 @@ int64_t nh_i8_tiled_bytes(int64_t rows, int64_t k);
 int nh_i8_quantize(const void* x, int type, int64_t x_stride, void* x_tiled, int64_t rows, int64_t k, void* stream);
 /* The same of fp32((x * r) * norm_weight), r = fp32(1 / sqrt(mean of the row's x^2 + eps)), the mean in 64 bits; norm_weight fp32 [k]. */
 int nh_i8_rms_norm_quantize(const void* x, int type, int64_t x_stride, const float* norm_weight, float eps, void* x_tiled, int64_t rows, int64_t k, void* stream);
-/* The same of silu(gate) * up, silu(g) = g / (1 + exp(-g)), in fp32 (within 3 units in the last place). */
+/* The same of silu(gate) * up, silu(g) = g / (1 + exp(-g)), in fp32 (within 3 units of 2^-23 of itself, or of 2^-149; 0 for finite gates below -132). */
 int nh_i8_silu_mul_quantize(const void* gate, const void* up, int type, int64_t gate_stride, int64_t up_stride, void* x_tiled, int64_t rows, int64_t k, void* stream);
 /* A plain int8 matrix [rows][k] with scales fp32 [rows] into the tiled layout, and back. */
 int nh_i8_tile(const int8_t* q, const float* scales, void* tiled, int64_t rows, int64_t k, void* stream);

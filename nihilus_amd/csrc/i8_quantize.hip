@@ -15,17 +15,43 @@ namespace nh {
 
 namespace {
 
-// silu(g) u within 3 units in the last place: -g log2(e) in two parts, the exponential's one unit, a sum, a quotient by one correction step (so within half a unit and little more), a product.
-// Below g = -87 the exponential is held at 2^126: what is left is below 2^-119 of up.
-__device__ __forceinline__ float silu_times(float g, float u) {
+// silu(g) u within 3 units of 2^-23 of itself, or of 2^-149.  -g log2(e) in two parts (the second brought in behind the exponential), the exponential's one unit, a sum, a quotient by one correction step (so
+// within half a unit and little more), a product.  NEAR: |g| is up to 80 or NaN, where exp(-g), the sum and the quotient are normal numbers.  Above that 1 + exp(-g) is 1; below -80 it is exp(-g), and the
+// result g exp(g) u, formed 2^64 times as large: exp(g) is then a normal number down to g = -131, past which 0 is taken.
+template<bool NEAR> __device__ __forceinline__ float silu_times(float g, float u) {
 	constexpr float log2e = 1.44269502162933349609375f, log2e_rest = 1.925963033500011e-8f, ln2 = 0.693147182464599609375f;
-	const float t	 = -g * log2e;
-	const float rest = fmaf(-g, log2e, -t) - g * log2e_rest;
-	float e			 = __builtin_amdgcn_exp2f(fminf(t, 126.0f));
-	e				 = fmaf(e, rest * ln2, e);
-	const float d = 1.0f + (t > 126.0f ? 0x1p126f : e), r = __builtin_amdgcn_rcpf(d);
-	const float q = g * r;
+	const bool far_down = !NEAR && g < -80.0f;
+	const float held	= NEAR ? g : fminf(fmaxf(g, -256.0f), 80.0f), at = far_down ? held : -held;
+	const float t		= at * log2e;
+	const float rest	= fmaf(at, log2e, -t) + at * log2e_rest;
+	float e				= __builtin_amdgcn_exp2f(far_down ? t + 64.0f : t); // (that sum is exact)
+	e					= fmaf(e, rest * ln2, e);
+	if (far_down) {
+		return g * e * u * 0x1p-64f;
+	}
+	if (!NEAR && g > 80.0f) {
+		return g * u;
+	}
+	const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), q = g * r;
 	return fmaf(fmaf(-q, d, g), r, q) * u;
+}
+template<int N> __device__ __forceinline__ void silu_times(float (&g)[N], const float (&u)[N]) {
+	float far = 0.0f;
+#pragma unroll
+	for (int j = 0; j < N; ++j) {
+		far = fmaxf(far, fabsf(g[j]));
+	}
+	if (far <= 80.0f) {
+#pragma unroll
+		for (int j = 0; j < N; ++j) {
+			g[j] = silu_times<true>(g[j], u[j]);
+		}
+	} else {
+#pragma unroll
+		for (int j = 0; j < N; ++j) {
+			g[j] = silu_times<false>(g[j], u[j]);
+		}
+	}
 }
 
 template<int TYPE, int FRONT, int THREADS, int HELD> __global__ __launch_bounds__(THREADS) void i8_quantize_kernel(i8_rows in, v4u* q, float* scale, int steps) {
@@ -46,10 +72,7 @@ template<int TYPE, int FRONT, int THREADS, int HELD> __global__ __launch_bounds_
 		if constexpr (FRONT == I8_SILU) {
 			float u[16];
 			i8_load<TYPE>(in.up, up_at + 16 * c, in.k - 16 * c, u);
-#pragma unroll
-			for (int j = 0; j < 16; ++j) {
-				v[j] = silu_times(v[j], u[j]);
-			}
+			silu_times(v, u);
 		}
 	};
 	auto normed = [&](int c, float(&v)[16]) {

@@ -29,6 +29,52 @@ def _matrix(g, rows, k):
     return q, torch.empty(rows, device="cuda").uniform_(0.5, 1.5, generator=g) / (127.0 * max(k, 1) ** 0.5)
 
 
+# ---- gates of any size
+
+
+def _silu_rows(gate, up):
+    """silu(gate) up in 64 bits (exp(-gate) of gates far down is past them: gate exp(gate) there)"""
+    g = gate.double()
+    return torch.where(g < -600, g * torch.exp(g.clamp(max=-600)), g / (1.0 + torch.exp(-g.clamp(min=-600)))) * up.double()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("k", [70, 9000, 40000])
+def test_silu_of_gates_of_any_size(i8, k, kind):
+    most = torch.finfo(kind).max
+    tops = [60.0, 79.0, 81.0, 88.0, 104.0, 1000.0, 65504.0, 1e30, 2.3e38, 2.4e38, 3.3e38]
+    tops = torch.tensor([t for t in tops if t <= most] + [most], device="cuda")
+    g = _gen(k)
+    # rows of gates that are all far up, all far down (what is left of them, or nothing), of either sign, and a single one among ordinary ones
+    size = tops[:, None] * torch.empty(len(tops), k, device="cuda").uniform_(0.95, 1.0, generator=g)
+    size[:, 0] = tops
+    ordinary = _normal(g, len(tops), k, std=3.0)
+    single, down = ordinary.clone(), ordinary.clone()
+    single[:, 3], down[:, k - 2] = tops, -tops
+    signs = torch.randint(0, 2, (len(tops), k), device="cuda", generator=g) * 2 - 1
+    gate = torch.cat([size, -size, size * signs, single, down]).to(kind)
+    up = _normal(g, *gate.shape, dtype=kind).clamp(-1, 1)
+    q, s = i8.untile(i8.silu_mul_quantize(gate, up), *gate.shape)
+    v = _silu_rows(gate, up)
+    # v within 3 units of 2^-23 of itself, or of the smallest number; the scale is rounded once more, and the whole number is one of the two next to the quotient
+    top = v.abs().amax(dim=1)
+    assert torch.isfinite(s).all() and ((s.double() - top / 127).abs() <= 8 * R.U * top / 127 + 4 * 2.0**-149).all()
+    few = 2.0**-149 * 4 / s.double().clamp(min=2.0**-149)[:, None]  # (units of the smallest number in a scale: more than a few bits only far below the normal numbers)
+    off = (q.double() * s.double()[:, None] - v).abs()
+    assert (off <= s.double()[:, None] * (0.5 + 127 * (16 * R.U + few)) + 4 * 2.0**-149).all()
+    far = (gate[:, 1:] < -140).all(dim=1)
+    assert far.sum() >= 2 and (s[far] == 0).all() and (q[far] == 0).all()
+
+
+def test_silu_of_gates_that_are_not_finite(i8):
+    gate, up = torch.zeros(5, 100, device="cuda"), torch.ones(5, 100, device="cuda")
+    gate[0, 7], gate[1, 8], gate[2, 9] = float("nan"), float("inf"), -float("inf")  # (an infinity over an infinity)
+    gate[3, 0] = 3e38
+    gate[4] = 1.0
+    q, s = i8.untile(i8.silu_mul_quantize(gate, up), 5, 100)
+    assert torch.isnan(s[:3]).all() and (q[:3] == 0).all() and torch.isfinite(s[3:]).all() and q[3, 0] == 127
+
+
 # ---- gradients of every type
 
 
