@@ -244,3 +244,47 @@ def test_losses_of_logits_past_fp32(i8, m):
     ws[9] = float("nan")
     losses, lse = i8.token_losses(i8.tile(wq, ws), x, targets, n, k)
     assert torch.isnan(lse).all() and torch.isnan(losses).all()
+
+
+# ---- memory
+
+
+# (one pass over the vocabulary; tiles of an odd last strip, several heights and splits; two pieces of the vocabulary; rows past 8192, cut as the first ones)
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(5, 50, 70), (16, 2001, 1000), (33, 2001, 130), (310, 2001, 130), (129, 16404, 200), (40, 33, 5000), (8192, 4200, 64), (8217, 700, 64)])
+def test_workspaces_of_the_losses_are_enough(i8, m, n, k, kind):
+    g = _gen(m + n)
+    w, x = i8.tile(*_matrix(g, n, k)), i8.quantize(_normal(g, m, k))
+    targets = torch.randint(0, n, (m,), device="cuda", dtype=torch.int32, generator=g)
+    losses, lse = i8.token_losses(w, x, targets, n, k)
+    dx = i8.token_losses_grad(w, x, targets, losses, lse, n, k, dtype=kind)
+    for need, call, want in ((i8._need("nh_i8_token_losses_workspace_bytes", m, n, k), lambda ws: i8.token_losses(w, x, targets, n, k, workspace=ws), (losses, lse)),
+                             (i8._need("nh_i8_token_losses_grad_workspace_bytes", m, n, k, i8._TYPES[kind]), lambda ws: (i8.token_losses_grad(w, x, targets, losses, lse, n, k, dtype=kind, workspace=ws),), (dx,))):
+        for fill in (77, 255):  # (what is there before means nothing: 255 is NaN in every type)
+            memory = torch.full((need + 4096,), fill, device="cuda", dtype=torch.uint8)
+            assert all(torch.equal(a, b) for a, b in zip(call(memory[:need]), want)) and (memory[need:] == fill).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 77, 100), (1, 4096, 4096), (2, 333, 1000), (4, 515, 1507), (5, 515, 1507), (117, 1003, 512)])
+def test_mul_mat_onto_its_residual(i8, m, n, k, kind):
+    g = _gen(m + n + k)
+    w, x, norm, r = i8.tile(*_matrix(g, n, k)), _normal(g, m, k, dtype=kind), 1.0 + 0.2 * _normal(g, k), _normal(g, m, n, dtype=kind)
+    for weight, eps in ((None, 0.0), (norm, 1e-5)):
+        want, onto = i8.mul_mat(w, x, n, k, residual=r, norm_weight=weight, eps=eps), r.clone()
+        assert i8.mul_mat(w, x, n, k, residual=onto, norm_weight=weight, eps=eps, out=onto) is onto and torch.equal(onto, want)
+
+
+@pytest.mark.parametrize("m", [5, 40])
+def test_targets_at_the_ends_of_their_type(i8, m):
+    n, k = 300, 64
+    g = _gen(m)
+    w, x = i8.tile(*_matrix(g, n, k)), i8.quantize(_normal(g, m, k))
+    targets = torch.randint(0, n, (m,), device="cuda", dtype=torch.int32, generator=g)
+    losses, lse = i8.token_losses(w, x, targets, n, k)
+    dx = i8.token_losses_grad(w, x, targets, losses, lse, n, k)
+    targets[0], targets[1], targets[2], targets[3] = -(2**31), 2**31 - 1, -1, n
+    some, some_lse = i8.token_losses(w, x, targets, n, k)
+    assert (some[:4] == 0).all() and torch.equal(some[4:], losses[4:]) and torch.equal(some_lse, lse)
+    some = i8.token_losses_grad(w, x, targets, some, some_lse, n, k)
+    assert (some[:4] == 0).all() and torch.equal(some[4:], dx[4:])
