@@ -54,7 +54,7 @@ inline int check_eps(float eps) {
 }
 inline int check_workspace(const void* workspace, int64_t bytes, int64_t need) {
 	NH_REQUIRE(workspace || need == 0, NH_ERR_NULL_POINTER);
-	NH_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, NH_ERR_ALIGNMENT);
+	NH_REQUIRE(aligned16(workspace), NH_ERR_ALIGNMENT);
 	NH_REQUIRE(bytes >= need, NH_ERR_ARGUMENT);
 	return NH_OK;
 }

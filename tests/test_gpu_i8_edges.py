@@ -288,3 +288,19 @@ def test_targets_at_the_ends_of_their_type(i8, m):
     assert (some[:4] == 0).all() and torch.equal(some[4:], losses[4:]) and torch.equal(some_lse, lse)
     some = i8.token_losses_grad(w, x, targets, some, some_lse, n, k)
     assert (some[:4] == 0).all() and torch.equal(some[4:], dx[4:])
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 700, 300), (40, 700, 300), (300, 2001, 130)])
+def test_workspaces_anywhere_at_16_bytes(i8, m, n, k):
+    g = _gen(m + n)
+    w, x = i8.tile(*_matrix(g, n, k)), _normal(g, m, k)
+    xq = i8.quantize(x)
+    targets = torch.randint(0, n, (m,), device="cuda", dtype=torch.int32, generator=g)
+    losses, lse = i8.token_losses(w, xq, targets, n, k)
+    needs = (i8._need("nh_i8_mul_mat_workspace_bytes", m, k), i8._need("nh_i8_token_losses_workspace_bytes", m, n, k), i8._need("nh_i8_token_losses_grad_workspace_bytes", m, n, k, 0))
+    for need, call in zip(needs, (lambda ws: (i8.mul_mat(w, x, n, k, workspace=ws),), lambda ws: i8.token_losses(w, xq, targets, n, k, workspace=ws),
+                                  lambda ws: (i8.token_losses_grad(w, xq, targets, losses, lse, n, k, workspace=ws),))):
+        memory = torch.full((need + 1024,), 77, device="cuda", dtype=torch.uint8)
+        for by in (16, 240):
+            assert all(torch.equal(a, b) for a, b in zip(call(memory[by : by + need]), call(None))) and (memory[by + need :] == 77).all()
+            memory.fill_(77)
