@@ -14,10 +14,10 @@ using nh::from_hip;
 using nh::overlap;
 using nh::require_device;
 
-constexpr int64_t MAX_ROWS		= int64_t{ 1 } << 22; // a quantize launch has four to a workgroup of 1024
+constexpr int64_t MAX_ROWS		= int64_t{ 1 } << 22; // a quantize launch has a workgroup of up to 512 threads to each
 constexpr int64_t MAX_K			= 131008; // 128 * 128 * K stays below 2^31, K a multiple of 64
 constexpr int64_t MAX_FRAGMENTS = int64_t{ 1 } << 25; // of a matrix: a tile launch has a thread to each 16 bytes
-constexpr int64_t MAX_TILES		= int64_t{ 1 } << 22; // of 256 x 256 sums: workgroups of 512 threads
+constexpr int64_t MAX_TILES		= int64_t{ 1 } << 22; // of 256 x 256 sums: workgroups of 512 threads (i8_form_for takes these tiles where smaller ones would be too many)
 
 inline int64_t element(int type) {
 	return type == NH_F32 ? 4 : 2;

@@ -294,7 +294,7 @@ inline i8_form i8_form_for(int64_t n, int64_t m, int64_t steps, int64_t behind) 
 		if (left) {
 			time += s.round + (left <= 256 ? steps * s.alone + results : steps * s.step + results * s.per_cu);
 		}
-		if (time < least) {
+		if (time < least && (s.form == I8_TILE_256 || tiles < (int64_t{ 1 } << 21))) { // (a grid has fewer than 2^32 threads, which the largest tiles keep to at every size)
 			least = time, best = s.form;
 		}
 	}
