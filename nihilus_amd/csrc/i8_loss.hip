@@ -54,14 +54,14 @@ struct i8_stretches {
 		for (int i = 0; i < FM; ++i) {
 			const int m	 = m0 + 16 * i + (lane & 15);
 			scales[i]	 = m < M ? x.scale[m] : 0.0f;
-			places[i]	 = m < M ? targets[m] - n0 : -1;
+			places[i]	 = m < M ? targets[m] : -1;
 		}
 #pragma unroll
 		for (int i = 0; i < FM; ++i) {
 			const int m		 = m0 + 16 * i + (lane & 15);
 			const bool there = m < M;
 			const float sx	 = scales[i];
-			const int target = places[i]; // in this stretch?
+			const int target = places[i];
 			v4f l[FN];
 			float top = -__builtin_inff();
 #pragma unroll
@@ -80,12 +80,12 @@ struct i8_stretches {
 					}
 				}
 			}
-			if (target >= 0 && target < 16 * FN && n0 + target < N) {
+			if (target >= n0 && target < n0 + 16 * FN && target < N) { // in this stretch
 #pragma unroll
 				for (int f = 0; f < FN; ++f) {
 #pragma unroll
 					for (int e = 0; e < 4; ++e) {
-						if (16 * f + 4 * group + e == target) {
+						if (n0 + 16 * f + 4 * group + e == target) {
 							hit[m] = l[f][e];
 						}
 					}

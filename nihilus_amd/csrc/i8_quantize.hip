@@ -115,16 +115,14 @@ template<int TYPE, int FRONT, int THREADS, int HELD> __global__ __launch_bounds_
 		for (int d = 32; d > 0; d >>= 1) {
 			sum += __shfl_xor(sum, d);
 		}
-		if constexpr (WAVES > 1) {
-			if ((t & 63) == 0) {
-				sums[wave] = sum;
-			}
-			__syncthreads();
-			sum = sums[0];
+		if ((t & 63) == 0) {
+			sums[wave] = sum;
+		}
+		__syncthreads();
+		sum = sums[0];
 #pragma unroll
-			for (int w = 1; w < WAVES; ++w) {
-				sum += sums[w];
-			}
+		for (int w = 1; w < WAVES; ++w) {
+			sum += sums[w];
 		}
 		r = i8_rms(sum, in.part, in.eps);
 	}
@@ -152,15 +150,13 @@ template<int TYPE, int FRONT, int THREADS, int HELD> __global__ __launch_bounds_
 	for (int d = 32; d > 0; d >>= 1) {
 		top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d)));
 	}
-	if constexpr (WAVES > 1) {
-		if ((t & 63) == 0) {
-			tops[wave] = top;
-		}
-		__syncthreads();
+	if ((t & 63) == 0) {
+		tops[wave] = top;
+	}
+	__syncthreads();
 #pragma unroll
-		for (int w = 0; w < WAVES; ++w) {
-			top = max(top, tops[w]);
-		}
+	for (int w = 0; w < WAVES; ++w) {
+		top = max(top, tops[w]);
 	}
 	const i8_step step(top);
 	if (t == 0) {
