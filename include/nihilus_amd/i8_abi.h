@@ -60,8 +60,9 @@ int nh_i8_token_losses(const void* w_tiled, const void* x_tiled, const int32_t* 
 
 /* The gradient of sum_m grad[m] losses[m] (grad fp32 [M]; NULL: ones) with respect to what the rows of x stand for:
  *   dx[m][k] = grad[m] sum_n (exp(l[m][n] - lse[m]) - [n = targets[m]]) w[n][k],  zero for rows that are not scored;  dx [M][K] of `type`, rounded once.
- * losses and lse as nh_i8_token_losses gave them: the target's own slope is formed as exp(-losses[m]) - 1, the others are as exact as lse is (2^-24 |lse| relative to themselves).  The slopes are formed again from x and w, for 8192 rows at a time and so much of the vocabulary that they stay below 128 MiB, and enter the
- * second product as sums of two fp16 numbers (22 bits) below a power of two of the row's own. */
+ * losses and lse as nh_i8_token_losses gave them: the target's own slope is formed as exp(-losses[m]) - 1, the others are as exact as lse is (2^-24 |lse| relative to themselves).
+ * The slopes are formed again from x and w, for 8192 rows at a time and so much of the vocabulary that they stay below 128 MiB, and enter the second product, times w's scales, as sums of two fp16
+ * numbers (22 bits) below a power of two of the row's own: what is 2^-37 of the row's largest slope and of w's largest scale is lost. */
 int64_t nh_i8_token_losses_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int type);
 int nh_i8_token_losses_grad(const void* w_tiled, const void* x_tiled, const int32_t* targets, const float* losses, const float* lse, const float* grad, void* dx, int type, int64_t M, int64_t N,
 	int64_t K, void* workspace, int64_t workspace_bytes, void* stream);

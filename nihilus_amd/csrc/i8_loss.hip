@@ -7,7 +7,7 @@
 //
 // Backward: dx[m][k] = grad[m] sum_n d[m][n] sw[n] w[n][k],  d = exp(l - lse) - [n = t].  Pieces of the vocabulary at a time, the product kernels form l again and leave
 // P = d sw 2^e in fp16, in operand order; a second product sums P w over n.  d is at most 1 - exp(-loss) of its row, so e is chosen by the row (and by the largest of all sw): P is below 2^15, and what
-// is 2^-28 of the row's largest is still a normal number.  P is a sum of two such numbers (22 bits), whatever dx is rounded to: with one (11 bits) 2048 rows of [128256 x 4096] took 2.7 ms instead of 3.9,
+// is 2^-28 of the row's largest is still a normal number.  P is a sum of two such numbers (22 bits), whatever dx is rounded to: with one (11 bits) 2048 rows of [128256 x 4096] took 2.6 ms instead of 3.7,
 // and one bf16 dx in sixteen was another number.
 // w enters the second product as fp16, exactly.  It lies in fragments of 16 rows n x 64 values k, and the sum is over n: ds_read_b64_tr_b8 takes eight rows of sixteen columns out of LDS so that
 // a lane has eight n of one k.
